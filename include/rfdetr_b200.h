@@ -22,8 +22,8 @@
 extern "C" {
 #endif
 
-/* Element types. */
-enum rfdetr_dtype { RFDETR_F32 = 0, RFDETR_BF16 = 1 };
+/* Element types (int32 for rotary positions only). */
+enum rfdetr_dtype { RFDETR_F32 = 0, RFDETR_BF16 = 1, RFDETR_I32 = 2 };
 
 /* Status codes. */
 enum rfdetr_status {
@@ -62,7 +62,7 @@ int rfdetr_abi_version(void);
 int rfdetr_set_tuning(const char *name, const char *value);
 
 /* Reads and clears the device fault word.  Kernels that wait on hardware barriers (the TMA
- * tile loads of the sampler backward) bound every wait; a wait that gives up sets this word and
+ * tile loads of the sampler backward, the packed attention) bound every wait; a wait that gives up sets this word and
  * the kernel finishes with undefined outputs instead of hanging.  Synchronises `stream`.
  * Returns RFDETR_OK when no wait gave up since the last call, RFDETR_ERR_LIMIT when one did,
  * RFDETR_ERR_CUDA when the copy fails.  No reference counterpart: the reference's sampler runs
@@ -351,6 +351,69 @@ int rfdetr_ipc_open_handle(const void *handle, void **base_out);
 int rfdetr_ipc_close_handle(void *base);
 int rfdetr_allreduce_sum_f32(void *stream, float *const *buffers, unsigned *const *flags, int rank, int world,
                              int64_t n, uint32_t epoch, int ctas, int32_t *status_out);
+
+/* ---------------------------------------------------------------------------------------
+ * Softmax attention over packed sequences, and its gradients.
+ *
+ * The self-attention of the decoder's query groups and of the backbone's windows or images of
+ * unequal size (src/rfdetr_jax/models/layers.py:54-98 computes one padded batch), without padding;
+ * with `causal` and grouped heads also that of a text prompt.
+ *   query   [tokens, n_heads, head_dim]         bf16, token and head strides in elements (multiples
+ *   key     [key_tokens, n_kv_heads, head_dim]  of 8), channels contiguous, 16-byte aligned
+ *   value   [key_tokens, n_kv_heads, head_dim]
+ *   offsets, key_offsets  device int32 [n_sequences + 1], ascending: sequence s is rows
+ *           offsets[s] .. offsets[s + 1] - 1 of query and key_offsets[s] .. of key and value;
+ *           key_offsets may be NULL (the same as offsets).  Values are clamped to the tensors.
+ *   output  [tokens, n_heads, head_dim] bf16 contiguous;  lse [n_heads, tokens] f32 or NULL
+ * Query i of sequence s sees its keys j, with `causal` those with j <= i + Lk - Lq.  Head h reads
+ * key head h / (n_heads / n_kv_heads).  A query that sees no key, and every row outside all
+ * sequences, gets output 0 and lse -inf; such rows of query, key and value have gradient 0.
+ * Scores, softmax statistics and sums are float32; the softmax weights (and, backward, dS) are
+ * rounded to bf16 for the tensor cores.  A non-finite value reaches the outputs of its own sequence
+ * only.  Bitwise reproducible.
+ * Limits: head_dim a multiple of 8 up to 128, n_heads a multiple of n_kv_heads, scale > 0.
+ * rfdetr_packed_attention needs a 16-byte aligned workspace of the size its query returns (0 unless
+ * the keys are split over blocks); the backward call one of tokens * n_heads floats.  grad_lse may be NULL.
+ * ------------------------------------------------------------------------------------- */
+size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, int64_t tokens, int64_t key_tokens,
+                                               int64_t n_heads, int64_t n_kv_heads, int64_t head_dim);
+int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride,
+                            const void *key, int64_t key_token_stride, int64_t key_head_stride,
+                            const void *value, int64_t value_token_stride, int64_t value_head_stride,
+                            const int32_t *offsets, const int32_t *key_offsets, void *output, float *lse,
+                            void *workspace, size_t workspace_bytes, int64_t n_sequences, int64_t tokens,
+                            int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int causal,
+                            float scale);
+size_t rfdetr_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t n_heads);
+int rfdetr_packed_attention_backward(void *stream, const void *query, int64_t query_token_stride,
+                                     int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                     int64_t key_head_stride, const void *value, int64_t value_token_stride,
+                                     int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
+                                     const void *output, const float *lse, const void *grad_output,
+                                     int64_t grad_token_stride, int64_t grad_head_stride, const float *grad_lse,
+                                     void *grad_query, void *grad_key, void *grad_value, void *workspace,
+                                     size_t workspace_bytes, int64_t n_sequences, int64_t tokens, int64_t key_tokens,
+                                     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int causal, float scale);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary positions with several axes (time, height, width) on queries and keys, one launch.
+ *
+ * Frequency i of sum(sections) belongs to axis a(i), the sections being consecutive, and turns a
+ * pair of channels of every head of token t by theta = positions[t, a(i)] * inv_freq[i]:
+ * (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin), the pair being channels (i, i + sum(sections)), or
+ * (2i, 2i + 1) with `interleaved`.  Channels from 2 * sum(sections) on are copied.  `inverse` turns by
+ * -theta, which is the gradient.  Angles are reduced in float64.
+ *   query [tokens, n_heads, head_dim], key [tokens, n_kv_heads, head_dim] (n_kv_heads may be 0): f32 or
+ *   bf16, strides in elements, channels contiguous; outputs contiguous, not overlapping the inputs;
+ *   positions [tokens, n_axes] f32 or int32 contiguous; inv_freq device f32; sections host int64.
+ * Limits: head_dim <= 1024, n_axes <= 8; interleaved pairs must be aligned to a pair.
+ * No reference counterpart: the reference's backbone adds learned positions.
+ * ------------------------------------------------------------------------------------- */
+int rfdetr_axial_rotary(void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride,
+                        const void *key, int64_t key_token_stride, int64_t key_head_stride, int dtype,
+                        const void *positions, int position_dtype, const float *inv_freq, const int64_t *sections,
+                        int64_t n_axes, void *query_out, void *key_out, int64_t tokens, int64_t n_heads,
+                        int64_t n_kv_heads, int64_t head_dim, int interleaved, int inverse);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,167 @@
+"""Softmax attention over packed sequences on B200, forward and backward on the tensor cores.
+
+The decoder's grouped self-attention (every detection group of queries attends within itself) and
+the backbone's windows, or images of unequal size, are sequences of different lengths in one
+packed tensor; the reference computes them as padded batches
+(``src/rfdetr_jax/models/layers.py:54-98``).  :func:`packed_attention` takes the rows of all
+sequences and their offsets, with grouped heads and an optional causal mask.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+
+def _packed(name: str, t: torch.Tensor, heads: int | None, dim: int | None) -> torch.Tensor:
+    """Checks ``[tokens, heads, dim]`` bf16 and returns it with strides the kernels take (a view of
+    a fused projection passes as it is; anything else is made contiguous)."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
+    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {list(t.shape)}")
+    token, head, channel = t.stride()
+    if channel != 1 or token <= 0 or head <= 0 or token % 8 or head % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _offsets(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 1 or t.numel() < 1 or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 [sequences + 1]")
+    return t.to(torch.int32).contiguous()
+
+
+def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
+    """Reads the offsets on the host (synchronises)."""
+    values = t.tolist()
+    if values[0] < 0 or values[-1] > total or any(b < a for a, b in zip(values, values[1:])):
+        raise ValueError(f"{name} must ascend within [0, {total}]")
+
+
+def attention_forward(query, key, value, offsets, key_offsets, causal, scale, want_lse):
+    """One forward call; inputs already checked.  Returns ``(output, lse or None)``."""
+    tokens, heads, dim = query.shape
+    key_tokens, kv_heads, _ = key.shape
+    sequences = offsets.numel() - 1
+    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
+    lse = torch.empty((heads, tokens), dtype=torch.float32, device=query.device) if want_lse else None
+    lib = N.lib()
+    ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+    status = lib.rfdetr_packed_attention(
+        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
+        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), offsets.data_ptr(), N.ptr(key_offsets),
+        out.data_ptr(), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads, kv_heads, dim,
+        int(causal), scale)
+    N.check(status, "rfdetr_packed_attention")
+    return out, lse
+
+
+def attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, lse, grad_output, grad_lse):
+    """One backward call; returns ``(grad_query, grad_key, grad_value)``, contiguous."""
+    tokens, heads, dim = query.shape
+    key_tokens, kv_heads, _ = key.shape
+    grad_output = _packed("grad_output", grad_output.to(query.dtype), heads, dim)
+    if grad_lse is not None:
+        grad_lse = grad_lse.to(torch.float32).contiguous()
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    grads = new(query), new(key), new(value)
+    lib = N.lib()
+    ws_bytes = lib.rfdetr_packed_attention_backward_workspace_bytes(tokens, heads)
+    workspace = torch.empty(max(1, ws_bytes), dtype=torch.uint8, device=query.device)
+    status = lib.rfdetr_packed_attention_backward(
+        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
+        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), offsets.data_ptr(), N.ptr(key_offsets),
+        out.data_ptr(), lse.data_ptr(), grad_output.data_ptr(), grad_output.stride(0), grad_output.stride(1),
+        N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
+        offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale)
+    N.check(status, "rfdetr_packed_attention_backward")
+    return grads
+
+
+class PackedAttentionFunction(torch.autograd.Function):
+    """Forward keeps the output and the log-sum-exp; backward forms the weights again from them."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, offsets, key_offsets, causal, scale):
+        out, lse = attention_forward(query, key, value, offsets, key_offsets, causal, scale, True)
+        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, lse)
+        ctx.how = (causal, scale)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output, grad_lse):
+        query, key, value, offsets, key_offsets, out, lse = ctx.saved_tensors
+        if grad_output is None and grad_lse is None:
+            return (None,) * 7
+        if grad_output is None:
+            grad_output = torch.zeros_like(out)
+        grads = attention_backward(query, key, value, offsets, key_offsets, *ctx.how, out, lse, grad_output, grad_lse)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
+
+
+def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: torch.Tensor,
+                     key_offsets: torch.Tensor | None = None, *, causal: bool = False, scale: float | None = None,
+                     return_lse: bool = False, check: bool = False):
+    """``softmax(scale * q k^T) v`` within each sequence of packed tensors.
+
+    Args:
+        query: ``[tokens, heads, head_dim]`` bfloat16, ``head_dim`` a multiple of 8 up to 128.  Views
+            of a fused projection are read in place (channels contiguous, strides multiples of 8).
+        key, value: ``[key_tokens, kv_heads, head_dim]``; head ``h`` reads key head
+            ``h // (heads // kv_heads)``.
+        offsets: int32 ``[sequences + 1]`` on the device: sequence ``s`` is rows ``offsets[s]`` to
+            ``offsets[s + 1] - 1`` of ``query``.
+        key_offsets: the same for ``key`` and ``value``; None where they are the queries' own tokens.
+        causal: query ``i`` of ``Lq`` sees keys ``j <= i + Lk - Lq`` (the last query sees all).
+        scale: of the scores, positive; ``head_dim ** -0.5`` by default.
+        return_lse: also return the scores' log-sum-exp ``[heads, tokens]`` float32.
+        check: read the offsets on the host (synchronises) and raise ``ValueError`` unless they
+            ascend within the tensors; otherwise the kernels clamp them.
+
+    Returns:
+        ``[tokens, heads, head_dim]`` bfloat16, differentiable with respect to query, key and value
+        (and through the log-sum-exp).  A query without any key, and rows outside all sequences,
+        give 0 (log-sum-exp ``-inf``) and gradient 0.
+    """
+    N.require_cuda(query, key, value, offsets, key_offsets)
+    query = _packed("query", query, None, None)
+    tokens, heads, dim = query.shape
+    key = _packed("key", key, None, dim)
+    value = _packed("value", value, key.shape[1], dim)
+    if value.shape[0] != key.shape[0]:
+        raise ValueError("key and value must have the same tokens")
+    if key.shape[1] < 1 or heads < 1 or heads % key.shape[1]:
+        raise ValueError(f"{heads} query heads are not a multiple of {key.shape[1]} key heads")
+    if dim % 8 or not 8 <= dim <= 128:
+        raise ValueError(f"head_dim must be a multiple of 8 up to 128, got {dim}")
+    if max(tokens, key.shape[0]) > 1 << 30 or heads > 65536:
+        raise ValueError("at most 2^30 tokens and 65536 heads")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 3.4028234663852886e38 or not math.isfinite(scale):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    offsets = _offsets("offsets", offsets)
+    if key_offsets is not None:
+        key_offsets = _offsets("key_offsets", key_offsets)
+        if key_offsets.numel() != offsets.numel():
+            raise ValueError("offsets and key_offsets must have the same length")
+    elif key.shape[0] != tokens:
+        raise ValueError("key_offsets is needed where keys and queries are not the same tokens")
+    if check:
+        _check_offsets("offsets", offsets, tokens)
+        if key_offsets is not None:
+            _check_offsets("key_offsets", key_offsets, key.shape[0])
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)
+    else:
+        out, lse = attention_forward(query, key, value, offsets, key_offsets, bool(causal), scale, return_lse)
+    return (out, lse) if return_lse else out

@@ -1,0 +1,1284 @@
+// Softmax attention over packed sequences, forward and backward, on the tensor cores (tcgen05).
+//
+// For sequence s with Lq queries and Lk keys, query i of head h and key j of head h / G:
+//   S_ij = scale q_i.k_j,  lse_i = log sum_j exp S_ij,  P_ij = exp(S_ij - lse_i),  o_i = sum_j P_ij v_j
+// over the keys that i may see: all, or with `causal` those with j <= i + Lk - Lq.  A query that
+// sees none has o_i = 0 and lse_i = -inf.  With the cotangent g of o (and c of lse):
+//   dP_ij = g_i.v_j,  delta_i = o_i.g_i - c_i,  dS_ij = P_ij (dP_ij - delta_i),
+//   dV_j = sum_i P_ij g_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j
+// (dK, dV summed over the G query heads of a key head).
+//
+// Sequences are ranges of rows of q and of k/v, given by offsets on the device.  A block finds its
+// rows from its index alone: sequence x owns the tile slots from start(x) / R + x on (R rows to a
+// slot), which never overlap and always suffice, so no plan has to be made and no length has to be
+// known on the host.  The rows before the first and after the last sequence count as sequences
+// without keys: their outputs and gradients are zero.  Offsets are clamped to the tensors.
+//
+// Queries of the heads that share a key head are rows of one tile (token-major, heads inner), so
+// K and V are read once for all of them and a few tokens still fill a tile.
+#include <cfloat>
+#include <cstring>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace rfdetr {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+    const int32_t *q_off, *k_off;  // [n_seq + 1]
+    int n_seq, Tq, Tk;
+    int Hq, Hkv, D;
+    int pack;    // query heads in one tile (of those that share a key head)
+    int subs;    // tiles' head groups per key head: (Hq / Hkv) / pack
+    int causal;
+    float scale, scale_log2;
+};
+
+// Bytes of a tile row panel and panels per row, for channels padded to DP.
+template <int DP> struct Tile {
+    static constexpr int kRowBytes = DP == 32 ? 64 : 128;
+    static constexpr int kPanels = DP * 2 / kRowBytes;
+    static constexpr int kCols = kRowBytes / 2;  // channels in a panel
+};
+
+__device__ __forceinline__ int off_at(const int32_t *off, int n_seq, int T, int x) {
+    if (x <= 0) return 0;
+    if (x > n_seq + 1) return T;
+    return min(max(off[x - 1], 0), T);
+}
+
+// The rows of one tile slot: sequence (-1: none to serve keys), first row in it, its rows.
+struct Slot {
+    int seq;    // index into the offsets, or -1 for rows outside every sequence
+    int first;  // first row of the slot within the sequence
+    int base;   // the sequence's first row in the packed tensor
+    int len;    // the sequence's rows
+};
+
+// Whole warp.  Extended sequence x: rows off_at(x) .. off_at(x + 1), x = 0 and n_seq + 1 being the
+// rows before and after all sequences.  A search over 32 probes a step.
+__device__ __forceinline__ Slot find_slot(const int32_t *off, int n_seq, int T, int R, int slot) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = n_seq + 2;
+    while (n > 1) {
+        const int step = (n + 31) >> 5;
+        const int i = lane * step;
+        bool before = false;
+        if (i < n) before = off_at(off, n_seq, T, lo + i) / R + lo + i <= slot;
+        const unsigned m = __ballot_sync(0xffffffffu, before);
+        const int p = m ? 31 - __clz(m) : 0;
+        lo += p * step;
+        n = min(step, n - p * step);
+    }
+    Slot r;
+    r.base = off_at(off, n_seq, T, lo);
+    r.len = max(0, off_at(off, n_seq, T, lo + 1) - r.base);
+    r.first = (slot - (r.base / R + lo)) * R;
+    r.seq = (lo >= 1 && lo <= n_seq) ? lo - 1 : -1;
+    return r;
+}
+
+__device__ __forceinline__ void seq_range(const int32_t *off, int n_seq, int T, int seq, int &base, int &len) {
+    base = 0;
+    len = 0;
+    if (seq < 0) return;
+    base = off_at(off, n_seq, T, seq + 1);
+    len = max(0, off_at(off, n_seq, T, seq + 2) - base);
+}
+
+inline long long slots_for(long long T, long long R, long long n_seq) { return T / R + n_seq + 2; }
+
+// Polls of a wait before the block gives up.  Every wait here is for work of the same block.
+constexpr int kAttnWaitLimit = 1 << 21;
+
+__device__ __forceinline__ bool wait_one(uint64_t *bar, unsigned parity, volatile int *abort) {
+    return mbar_wait(bar, parity, abort, kAttnWaitLimit);
+}
+// The same for a whole warp: all of its lanes go on, or none (tensor memory is moved by warps).
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volatile int *abort) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kAttnWaitLimit));
+}
+
+// Zeroes rows [from, to) of a swizzled tile (whole warp; whole rows, so the swizzle does not matter).
+template <int DP>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int rows_in_panel, int from, int to) {
+    constexpr int CH = Tile<DP>::kRowBytes / 16;
+    const int lane = threadIdx.x & 31;
+    const int n = (to - from) * CH;
+    for (int p = 0; p < Tile<DP>::kPanels; ++p) {
+        const uint32_t a = tile + p * rows_in_panel * Tile<DP>::kRowBytes + from * Tile<DP>::kRowBytes;
+        for (int i = lane; i < n; i += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + i * 16), "r"(0) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Forward.
+//
+// A block serves NT tiles of 128 rows (queries x packed heads) of one sequence and key head, and
+// walks its keys in tiles of 128: per tile S = Q K^T (both operands in shared memory) into TMEM, a
+// warpgroup per row tile turns it into P = exp2(scale log2(e) (S - m)) in registers, one row per
+// thread, and writes it back as bf16 over S; O += P V takes P from TMEM.  With two row tiles the
+// tensor core works on one while the other's exponentials run.  The reference m of a row is its
+// running maximum, but moves only when that grew by more than kLazy (in powers of two; P and its
+// sum stay below 2^kLazy times their true scale, far from any limit in float32, and bf16's relative
+// rounding does not depend on the scale), so that O in TMEM is seldom rescaled.
+// P is rounded to bf16 because that is what the tensor core takes; its row sum is kept in float32
+// from the unrounded values.
+// With few row tiles the keys are split over `splits` blocks; each writes its normalised part in
+// float32 and its lse, and attn_join_kernel adds them by weight.
+// ---------------------------------------------------------------------------------------------
+constexpr float kLazy = 8.0f;
+constexpr int kKeys = 128;  // keys in a tile
+
+template <int DP, int NT> struct FwdShape {
+    static constexpr int kTileBytes = 128 * DP * 2;
+    static constexpr int kStages = 4;
+    static constexpr int kThreads = NT * 128 + 64;
+    static constexpr int kTmem = NT * (128 + DP) <= 256 ? 256 : 512;
+    static constexpr size_t kSmem = 1024 + (size_t)(NT + kStages) * kTileBytes;
+};
+
+template <int NT> struct FwdShared {
+    uint64_t q_full[NT], kv_full[4], kv_raw, kv_empty[4], s_full[NT], p_ready[NT], o_done[NT], drain;
+    uint32_t tmem;
+    int abort;
+};
+
+struct FwdRange {
+    int n[2];       // key tiles of each row tile (end, exclusive)
+    int nmax;       // end over the row tiles
+    int j0;         // first key tile
+    int tok[2];     // tokens of each row tile
+};
+
+// Whole warp; returns how many tiles of K and V were asked for.
+template <int DP, int NT>
+__device__ int fwd_load(const AttnArgs &A, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
+                         FwdShared<NT> &sh, uint32_t smem_q, uint32_t smem_kv, const FwdRange &r, int kvh, int qhead,
+                         int qrow, int tok_per_tile, int krow, int klen) {
+    using S = FwdShape<DP, NT>;
+    using TL = Tile<DP>;
+    const int lane = threadIdx.x & 31;
+    volatile int *abort = &sh.abort;
+    if (r.nmax <= r.j0) return 0;
+    if (lane == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (r.n[t] <= r.j0) continue;
+            mbar_arrive_expect_tx(&sh.q_full[t], tok_per_tile * A.pack * TL::kRowBytes * TL::kPanels);
+            for (int p = 0; p < TL::kPanels; ++p)
+                tma_load_3d(smem_q + t * S::kTileBytes + p * 128 * TL::kRowBytes, mq, &sh.q_full[t], p * TL::kCols,
+                            qhead, qrow + t * tok_per_tile);
+        }
+    }
+    const int loads = 2 * (r.nmax - r.j0);
+    int issued = 0;
+    unsigned raw_phase = 0;
+    for (; issued < loads; ++issued) {
+        const int st = issued % S::kStages;
+        if (issued >= S::kStages && !wait_warp(&sh.kv_empty[st], ((issued / S::kStages) - 1) & 1, abort)) break;
+        const int j = r.j0 + (issued >> 1);
+        const bool is_v = issued & 1;
+        // The last tile of V may reach into rows that are not this sequence's: P is 0 there, but
+        // 0 x inf is not, so they are cleared before the tensor core sees the tile.
+        const int foreign = is_v ? j * kKeys + kKeys - klen : 0;
+        const uint32_t dst = smem_kv + st * S::kTileBytes;
+        uint64_t *bar = foreign > 0 ? &sh.kv_raw : &sh.kv_full[st];
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar, S::kTileBytes);
+            for (int p = 0; p < TL::kPanels; ++p)
+                tma_load_3d(dst + p * 128 * TL::kRowBytes, is_v ? mv : mk, bar, p * TL::kCols, kvh, krow + j * kKeys);
+        }
+        if (foreign > 0) {
+            if (!wait_warp(&sh.kv_raw, raw_phase, abort)) {
+                mbar_drain(&sh.kv_raw, raw_phase, kAttnWaitLimit);
+                break;
+            }
+            raw_phase ^= 1;
+            zero_rows<DP>(dst, 128, kKeys - foreign, kKeys);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+        }
+    }
+    return issued;
+}
+
+// After a wait gave up: every copy of this block that may still be landing.
+template <int DP, int NT> __device__ void fwd_drain(FwdShared<NT> &sh, const FwdRange &r, int issued) {
+    using S = FwdShape<DP, NT>;
+    for (int t = 0; t < NT; ++t)
+        if (r.n[t] > r.j0) mbar_drain(&sh.q_full[t], 0, kAttnWaitLimit);
+    for (int i = max(0, issued - S::kStages); i < issued; ++i)
+        mbar_drain(&sh.kv_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
+}
+
+// One thread.
+template <int DP, int NT>
+__device__ bool fwd_mma_loop(FwdShared<NT> &sh, uint32_t smem_q, uint32_t smem_kv, const FwdRange &r, uint32_t tmem) {
+    using S = FwdShape<DP, NT>;
+    using TL = Tile<DP>;
+    constexpr uint32_t kIdS = mma_idesc(128, kKeys, false), kIdO = mma_idesc(128, DP, true);
+    constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
+    volatile int *abort = &sh.abort;
+    auto scores = [&](int t, int st) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t o = (k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes;
+            mma_ss(tmem + t * 128, smem_desc<TL::kRowBytes>(smem_q + t * S::kTileBytes + o, 16, kSbo),
+                   smem_desc<TL::kRowBytes>(smem_kv + st * S::kTileBytes + o, 16, kSbo), kIdS, k > 0);
+        }
+        tc_commit(&sh.s_full[t]);
+    };
+    auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
+        return wait_one(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
+    };
+    const int n = r.nmax - r.j0;
+    int st = kv(0);
+    if (st < 0) return false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if (r.n[t] <= r.j0) continue;
+        if (!wait_one(&sh.q_full[t], 0, abort)) return false;
+        tc_fence_after();
+        scores(t, st);
+    }
+    tc_commit(&sh.kv_empty[st]);
+    for (int i = 0; i < n; ++i) {
+        int sv = -1, sk = -1;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
+            if (left > 0) {
+                if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
+                if (!wait_one(&sh.p_ready[t], i & 1, abort)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                    mma_ts(tmem + NT * 128 + t * DP, tmem + t * 128 + k * 8,
+                           smem_desc<TL::kRowBytes>(smem_kv + sv * S::kTileBytes + k * 16 * TL::kRowBytes, kLbo, kSbo),
+                           kIdO, i > 0 || k > 0);
+                tc_commit(&sh.o_done[t]);
+            }
+            if (left > 1) {
+                if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
+                tc_fence_after();
+                scores(t, sk);
+            }
+        }
+        if (sv >= 0) tc_commit(&sh.kv_empty[sv]);
+        if (sk >= 0) tc_commit(&sh.kv_empty[sk]);
+    }
+    return true;
+}
+
+// The largest of m and 32 values.
+__device__ __forceinline__ float max32(const float *s, float m) {
+    float a = m, b = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+        a = fmaxf(fmaxf(a, s[c]), s[c + 1]);
+        b = fmaxf(fmaxf(b, s[c + 2]), s[c + 3]);
+    }
+    return fmaxf(a, b);
+}
+
+// A warpgroup: the rows of row tile t.
+template <int DP, int NT, bool SPLIT>
+__device__ void fwd_softmax(const AttnArgs &A, FwdShared<NT> &sh, const FwdRange &r, int t, uint32_t tmem, int row,
+                            int tok_first, int qlen, int klen, int qbase, int qhead, bf16 *out, float *lse, float *part,
+                            float *part_lse) {
+    volatile int *abort = &sh.abort;
+    const uint32_t lane_base = (uint32_t)((threadIdx.x >> 5) & 3) << 21;  // lane 32 (w % 4)
+    const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + NT * 128 + t * DP;
+    const int tok = tok_first + row / A.pack;
+    const int head = qhead + row % A.pack;
+    const bool live = row / A.pack < r.tok[t];
+    const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - qlen)) : klen;
+    // Keys that every row of the tile sees (rows past the last token do not count).
+    const int all_see = A.causal ? min(klen, tok_first + 1 + klen - qlen) : klen;
+    const float sc = A.scale_log2;
+    float m = -INFINITY, sum = 0.0f;
+    const int n = r.n[t] - r.j0;
+    for (int i = 0; i < n; ++i) {
+        if (!wait_warp(&sh.s_full[t], i & 1, abort)) return;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
+        tmem_wait_ld();
+        pin<128>(s);
+        const int k0 = (r.j0 + i) * kKeys;
+        if (k0 + kKeys > all_see) {
+            const int seen = limit - k0;
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx = max32(s + c * 32, mx);
+        if (i == 0) {
+            m = mx;
+        } else {
+            const bool grown = mx * sc > m * sc + kLazy;
+            if (__any_sync(0xffffffffu, grown)) {
+                // O must hold the products of every tile before this one.
+                if (!wait_warp(&sh.o_done[t], (i - 1) & 1, abort)) return;
+                tc_fence_after();
+                const float to_m = fmaxf(m, mx);
+                const float f = to_m == -INFINITY ? 1.0f : exp2_fast((m - to_m) * sc);
+                m = to_m;
+                sum *= f;
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    float o[32];
+                    tmem_ld32(to + c * 32, o);
+                    tmem_wait_ld();
+                    pin<32>(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] *= f;
+                    tmem_st32(to + c * 32, reinterpret_cast<uint32_t *>(o));
+                }
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : -m * sc;
+        const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
+        float2 acc = make_float2(0.0f, 0.0f), acc1 = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t p[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                float2 x = fma2(make_float2(s[h * 64 + 2 * c], s[h * 64 + 2 * c + 1]), sc2, ref2);
+                x.x = exp2_fast(x.x);
+                x.y = exp2_fast(x.y);
+                if (c & 1) acc1 = add2(acc1, x);
+                else acc = add2(acc, x);
+                p[c] = pack_bf16(x.x, x.y);
+            }
+            tmem_st32(ts + h * 32, p);
+        }
+        sum += (acc.x + acc.y) + (acc1.x + acc1.y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_ready[t]);
+    }
+    const size_t token = (size_t)qbase + tok;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float l = sum == 0.0f ? -INFINITY : m * A.scale + logf(sum);
+    if (live) {
+        if (SPLIT) part_lse[(size_t)head * A.Tq + token] = l;
+        else if (lse) lse[(size_t)head * A.Tq + token] = l;
+    }
+    if (n > 0) {
+        if (!wait_warp(&sh.o_done[t], (n - 1) & 1, abort)) return;
+        tc_fence_after();
+    }
+    const size_t at = (token * A.Hq + head) * A.D;
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+        float o[32];
+        if (n > 0) {
+            tmem_ld32(to + c * 32, o);
+            tmem_wait_ld();
+            pin<32>(o);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (!live) continue;
+        if (SPLIT) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+                if (c * 32 + e < A.D)
+                    *reinterpret_cast<float4 *>(part + at + c * 32 + e) =
+                        make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+                if (c * 32 + e < A.D) {
+                    uint4 w;
+                    w.x = pack_bf16(o[e] * inv, o[e + 1] * inv);
+                    w.y = pack_bf16(o[e + 2] * inv, o[e + 3] * inv);
+                    w.z = pack_bf16(o[e + 4] * inv, o[e + 5] * inv);
+                    w.w = pack_bf16(o[e + 6] * inv, o[e + 7] * inv);
+                    *reinterpret_cast<uint4 *>(out + at + c * 32 + e) = w;
+                }
+        }
+    }
+}
+
+template <int DP, int NT, bool SPLIT>
+__global__ void __launch_bounds__(FwdShape<DP, NT>::kThreads, 1)
+attn_forward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                    const __grid_constant__ CUtensorMap mv, bf16 *__restrict__ out, float *__restrict__ lse,
+                    float *__restrict__ part, float *__restrict__ part_lse, int slots) {
+    using S = FwdShape<DP, NT>;
+    extern __shared__ unsigned char dyn[];
+    __shared__ FwdShared<NT> sh;
+    const int warp = threadIdx.x >> 5;
+    const int heads = A.Hkv * A.subs;
+    const int hx = blockIdx.x % heads;
+    // Later slots first: under a causal mask they see more keys.
+    const int slot = slots - 1 - (int)(blockIdx.x / heads);
+    const int per = 128 / A.pack;  // tokens in a row tile
+    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per * NT, slot);
+    if (q.first >= q.len) return;
+    int kbase, klen;
+    seq_range(A.k_off, A.n_seq, A.Tk, q.seq, kbase, klen);
+    const int kvh = hx / A.subs;
+    const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+
+    FwdRange r;
+    r.nmax = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        r.tok[t] = min(per, max(0, q.len - q.first - t * per));
+        const int last = q.first + t * per + r.tok[t] - 1;
+        const int sees = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
+        r.n[t] = (sees + kKeys - 1) / kKeys;
+        r.nmax = max(r.nmax, r.n[t]);
+    }
+    r.j0 = 0;
+    if (SPLIT) {
+        const int each = (r.nmax + (int)gridDim.z - 1) / (int)gridDim.z;
+        r.j0 = min(r.nmax, each * (int)blockIdx.z);
+        const int end = min(r.nmax, r.j0 + each);
+        for (int t = 0; t < NT; ++t) r.n[t] = max(r.j0, min(r.n[t], end));
+        r.nmax = end;
+        part += (size_t)blockIdx.z * A.Tq * A.Hq * A.D;
+        part_lse += (size_t)blockIdx.z * A.Tq * A.Hq;
+    }
+
+    if (warp == NT * 4) {
+        if ((threadIdx.x & 31) == 0) {
+            for (int t = 0; t < NT; ++t) {
+                mbar_init(&sh.q_full[t], 1);
+                mbar_init(&sh.s_full[t], 1);
+                mbar_init(&sh.p_ready[t], 4);
+                mbar_init(&sh.o_done[t], 1);
+            }
+            for (int i = 0; i < S::kStages; ++i) {
+                mbar_init(&sh.kv_full[i], 1);
+                mbar_init(&sh.kv_empty[i], 1);
+            }
+            mbar_init(&sh.kv_raw, 1);
+            mbar_init(&sh.drain, 1);
+            sh.abort = 0;
+            mbar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&sh.tmem, S::kTmem);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const uint32_t smem_q = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t smem_kv = smem_q + NT * S::kTileBytes;
+
+    int issued = 0;
+    if (warp == NT * 4) {
+        if ((threadIdx.x & 31) == 0 && r.nmax > r.j0) fwd_mma_loop<DP, NT>(sh, smem_q, smem_kv, r, tmem);
+    } else if (warp == NT * 4 + 1) {
+        issued = fwd_load<DP, NT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
+                                  klen);
+    } else {
+        const int t = warp >> 2;
+        if (r.tok[t] > 0)
+            fwd_softmax<DP, NT, SPLIT>(A, sh, r, t, tmem, threadIdx.x & 127, q.first + t * per, q.len, klen, q.base,
+                                       qhead, out, lse, part, part_lse);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (sh.abort && warp == NT * 4 + 1 && (threadIdx.x & 31) == 0) fwd_drain<DP, NT>(sh, r, issued);
+    if (warp == NT * 4) {
+        if (sh.abort && (threadIdx.x & 31) == 0) {
+            tc_commit(&sh.drain);
+            mbar_drain(&sh.drain, 0, kAttnWaitLimit);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+// o = sum_s w_s part_s with w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s).  Eight channels
+// per thread; a part that saw no keys (lse -inf) has weight 0 and is not read.
+__global__ void __launch_bounds__(256)
+attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, int splits, long long rows, int Hq,
+                 int Tq, int D, bf16 *__restrict__ out, float *__restrict__ lse) {
+    const int per = D / 8;
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= rows * per) return;
+    const long long row = i / per;  // token * Hq + head
+    const int c = (int)(i % per) * 8;
+    const long long token = row / Hq;
+    const int head = (int)(row % Hq);
+    const float *pl = part_lse + (size_t)head * Tq + token;
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, pl[(size_t)s * rows]);
+    float total = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < splits; ++s) {
+        const float l = pl[(size_t)s * rows];
+        if (l == -INFINITY) continue;
+        const float w = expf(l - top);
+        total += w;
+        float x[8];
+        load_vec<float, 8, true>(part + (size_t)s * rows * D + row * D + c, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(w, x[e], o[e]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= inv;
+    store_vec<bf16, 8>(out + row * D + c, o);
+    if (lse && c == 0) lse[(size_t)head * Tq + token] = total == 0.0f ? -INFINITY : top + logf(total);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Backward.
+//
+// Two kernels of one form, so that no sum needs an atomic and results do not depend on the order of
+// blocks: one holds a tile of 128 keys (K, V) and walks the queries, accumulating dK and dV in
+// TMEM; the other holds 128 query rows (Q, g) and walks the keys, accumulating dQ.  Both form S and
+// dP again (three products where one kernel with atomics would share two of them).
+//   X0, X1: the held tiles (K, V or Q, g); Y0, Y1: the walked ones, 64 rows a step (Q, g or K, V)
+//   A = X0 Y0^T, B = X1 Y1^T  (128 x 64 each, TMEM)  ->  P = exp2(scale log2(e) A - log2(e) lse),
+//   dS = P (B - delta)        (bf16, written over A and B)
+//   acc0 += dS Y0             (dK or dQ, times scale at the end), acc1 += P Y1 (dV)
+// Two pairs (A, B) alternate between two warpgroups: while one turns its pair into P and dS, the
+// tensor core forms the other's and adds the one before.  64 rows a step is what TMEM leaves: two
+// pairs of 64 + 64 columns beside two accumulators of up to 128.
+// P and dS are rounded to bf16 for the tensor core; every sum is float32.
+// A row that sees exactly one key has P = 1 whatever its score, so its dS is set to what is left of
+// it, the cotangent of its lse, rather than to the difference of two roundings of the same number.
+// ---------------------------------------------------------------------------------------------
+constexpr int kWalk = 64;  // rows of Y a step
+
+template <int DP> struct BwdShape {
+    static constexpr int kXBytes = 128 * DP * 2;
+    static constexpr int kYBytes = kWalk * DP * 2;
+    static constexpr int kStages = 4;
+    static constexpr int kThreads = 2 * 128 + 64;
+    static constexpr int kTmem = 512;
+    static constexpr size_t kSmem = 1024 + 2 * kXBytes + (size_t)kStages * 2 * kYBytes;
+};
+
+struct BwdShared {
+    uint64_t x_full, y_full[4], y_raw, y_empty[4], s_full[2], ds_ready[2], acc_done, drain;
+    uint32_t tmem;
+    int abort;
+    // Per walked row, for the dK/dV kernel: -log2(e) lse, -delta and the lse's cotangent.
+    alignas(16) float neg_lse2[4][kWalk];
+    alignas(16) float neg_delta[4][kWalk];
+    alignas(16) float one_ds[4][kWalk];
+};
+
+// What a block walks.  DKV: `steps_per_sub` tiles of `tok` tokens from token `first` on, for each of
+// `subs` head groups.  DQ: tiles of 64 keys.
+struct BwdRange {
+    int steps, steps_per_sub;
+    int first;      // DKV: first query token
+    int qbase, qlen, kbase, klen;
+    int tok;        // DKV: tokens a step
+    int k0;         // DKV: first key of the held tile
+    int q0, qtok;   // DQ: first token and tokens of the held tile
+    int kvh, qhead; // key head; DQ: first query head of the tile (DKV: of the key head)
+};
+
+// Whole warp; returns how many steps were asked for.
+template <int DP, bool DKV>
+__device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtensorMap *mx1, const CUtensorMap *my0,
+                        const CUtensorMap *my1, BwdShared &sh, uint32_t smem_x, uint32_t smem_y, const BwdRange &r,
+                        const float *lse, const float *delta, const float *g_lse) {
+    using S = BwdShape<DP>;
+    using TL = Tile<DP>;
+    const int lane = threadIdx.x & 31;
+    volatile int *abort = &sh.abort;
+    if (r.steps == 0) return 0;
+    const int xrows = DKV ? 128 : (128 / A.pack) * A.pack;
+    if (lane == 0) {
+        mbar_arrive_expect_tx(&sh.x_full, 2 * xrows * TL::kRowBytes * TL::kPanels);
+        const int head = DKV ? r.kvh : r.qhead, at = DKV ? r.kbase + r.k0 : r.qbase + r.q0;
+        for (int p = 0; p < TL::kPanels; ++p) {
+            const uint32_t o = p * 128 * TL::kRowBytes;
+            tma_load_3d(smem_x + o, mx0, &sh.x_full, p * TL::kCols, head, at);
+            tma_load_3d(smem_x + S::kXBytes + o, mx1, &sh.x_full, p * TL::kCols, head, at);
+        }
+    }
+    const int yrows = DKV ? r.tok * A.pack : kWalk;
+    unsigned raw_phase = 0;
+    int i = 0;
+    for (; i < r.steps; ++i) {
+        const int st = i % S::kStages;
+        if (i >= S::kStages && !wait_warp(&sh.y_empty[st], ((i / S::kStages) - 1) & 1, abort)) break;
+        const int sub = DKV ? i / r.steps_per_sub : 0;
+        const int at = DKV ? r.first + (i - sub * r.steps_per_sub) * r.tok : i * kWalk;  // within the sequence
+        const int head = DKV ? r.qhead + sub * A.pack : r.kvh;
+        const int base = DKV ? r.qbase : r.kbase;
+        // Rows of the box past the sequence's end belong to another sequence: cleared, since the
+        // accumulating products multiply them by 0.
+        const int good = DKV ? min(r.tok, r.qlen - at) * A.pack : min(kWalk, r.klen - at);
+        uint64_t *bar = good < yrows ? &sh.y_raw : &sh.y_full[st];
+        const uint32_t y0 = smem_y + st * 2 * S::kYBytes, y1 = y0 + S::kYBytes;
+        __syncwarp();
+        if (lane == 0) {
+            mbar_expect_tx(bar, 2 * yrows * TL::kRowBytes * TL::kPanels);
+            for (int p = 0; p < TL::kPanels; ++p) {
+                const uint32_t o = p * kWalk * TL::kRowBytes;
+                tma_load_3d(y0 + o, my0, bar, p * TL::kCols, head, base + at);
+                tma_load_3d(y1 + o, my1, bar, p * TL::kCols, head, base + at);
+            }
+        }
+        if (DKV) {
+#pragma unroll
+            for (int h = 0; h < kWalk / 32; ++h) {
+                const int c = lane + h * 32;
+                float nl = 0.0f, nd = 0.0f, od = 0.0f;
+                if (c < good) {
+                    const size_t x = (size_t)(head + c % A.pack) * A.Tq + base + at + c / A.pack;
+                    nl = -lse[x] * kLog2e;
+                    nd = -delta[x];
+                    if (g_lse) od = g_lse[x];
+                }
+                sh.neg_lse2[st][c] = nl;
+                sh.neg_delta[st][c] = nd;
+                sh.one_ds[st][c] = od;
+            }
+            __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(bar);
+        if (good < yrows) {
+            if (!wait_warp(&sh.y_raw, raw_phase, abort)) {
+                mbar_drain(&sh.y_raw, raw_phase, kAttnWaitLimit);
+                break;
+            }
+            raw_phase ^= 1;
+            zero_rows<DP>(y0, kWalk, good, yrows);
+            zero_rows<DP>(y1, kWalk, good, yrows);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.y_full[st]);
+        }
+    }
+    return i;
+}
+
+// One thread.
+template <int DP, bool DKV>
+__device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, int steps, uint32_t tmem) {
+    using S = BwdShape<DP>;
+    using TL = Tile<DP>;
+    constexpr uint32_t kIdS = mma_idesc(128, kWalk, false), kIdAcc = mma_idesc(128, DP, true);
+    constexpr uint32_t kSbo = 8 * TL::kRowBytes;
+    constexpr uint32_t kXPanel = 128 * TL::kRowBytes, kYPanel = kWalk * TL::kRowBytes;
+    volatile int *abort = &sh.abort;
+    auto scores = [&](int i) {
+        const int st = i % S::kStages;
+        if (!wait_one(&sh.y_full[st], (i / S::kStages) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t y = smem_y + st * 2 * S::kYBytes;
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
+                mma_ss(tmem + (i & 1) * 2 * kWalk + which * kWalk,
+                       smem_desc<TL::kRowBytes>(smem_x + which * S::kXBytes + panel * kXPanel + in, 16, kSbo),
+                       smem_desc<TL::kRowBytes>(y + which * S::kYBytes + panel * kYPanel + in, 16, kSbo), kIdS, k > 0);
+            }
+        tc_commit(&sh.s_full[i & 1]);
+        return true;
+    };
+    if (!wait_one(&sh.x_full, 0, abort)) return false;
+    if (!scores(0)) return false;
+    if (steps > 1 && !scores(1)) return false;
+    for (int i = 0; i < steps; ++i) {
+        const int st = i % S::kStages;
+        const uint32_t y = smem_y + st * 2 * S::kYBytes;
+        if (!wait_one(&sh.ds_ready[i & 1], (i >> 1) & 1, abort)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kWalk / 16; ++k) {
+            const uint32_t row = k * 16 * TL::kRowBytes;
+            if (DKV)
+                mma_ts(tmem + 4 * kWalk + DP, tmem + (i & 1) * 2 * kWalk + k * 8,
+                       smem_desc<TL::kRowBytes>(y + S::kYBytes + row, kYPanel, kSbo), kIdAcc, i > 0 || k > 0);
+            mma_ts(tmem + 4 * kWalk, tmem + (i & 1) * 2 * kWalk + kWalk + k * 8,
+                   smem_desc<TL::kRowBytes>(y + row, kYPanel, kSbo), kIdAcc, i > 0 || k > 0);
+        }
+        tc_commit(&sh.y_empty[st]);
+        if (i + 2 < steps && !scores(i + 2)) return false;
+    }
+    tc_commit(&sh.acc_done);
+    return true;
+}
+
+// Warpgroup w: the steps i with i % 2 == w.
+template <int DP, bool DKV>
+__device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const float *lse,
+                          const float *delta, const float *g_lse) {
+    using S = BwdShape<DP>;
+    volatile int *abort = &sh.abort;
+    const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
+    const uint32_t ts = tmem + ((uint32_t)((threadIdx.x >> 5) & 3) << 21) + w * 2 * kWalk;
+    const float2 sc2 = make_float2(A.scale_log2, A.scale_log2);
+    const int shift = r.klen - r.qlen;  // under a causal mask token t sees keys <= t + shift
+    // DKV: this row's key.  DQ: this row's query.
+    const int key = r.k0 + row;
+    const int tok = r.q0 + row / A.pack;
+    int limit = 0;
+    float row_nl = 0.0f, row_nd = 0.0f, row_od = 0.0f;
+    if (!DKV && row / A.pack < r.qtok) {
+        limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
+        const size_t x = (size_t)(r.qhead + row % A.pack) * A.Tq + r.qbase + tok;
+        row_nl = -lse[x] * kLog2e;
+        row_nd = -delta[x];
+        if (g_lse) row_od = g_lse[x];
+    }
+    // DQ: keys that every row of the tile sees, and whether some row sees a single one.
+    const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
+    for (int i = w; i < r.steps; i += 2) {
+        const int st = i % S::kStages;
+        if (!wait_warp(&sh.s_full[w], (i >> 1) & 1, abort)) return;
+        tc_fence_after();
+        // Columns [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or the
+        // whole row is (DQ) a query with a single key.
+        int lo = 0, hi = kWalk, one_lo = 0, one_hi = 0;
+        bool mask;
+        if (DKV) {
+            const int at = r.first + (i % r.steps_per_sub) * r.tok;
+            const int good = min(r.tok, r.qlen - at) * A.pack;
+            mask = good < kWalk || r.k0 + 128 > r.klen || (A.causal && at + shift < r.k0 + 127);
+            if (mask) {
+                hi = key < r.klen ? good : 0;
+                if (A.causal) {
+                    lo = max(0, (key - shift - at) * A.pack);
+                    one_lo = (-shift - at) * A.pack;  // the token that sees key 0 only
+                    one_hi = one_lo + A.pack;
+                }
+                if (r.klen == 1) {
+                    one_lo = 0;
+                    one_hi = kWalk;
+                }
+            }
+        } else {
+            mask = (i + 1) * kWalk > all_see;
+            if (mask) {
+                hi = limit - i * kWalk;
+                one_hi = limit == 1 ? kWalk : 0;
+            }
+        }
+        float s[kWalk], d[kWalk];
+#pragma unroll
+        for (int c = 0; c < kWalk; c += 32) {
+            tmem_ld32(ts + c, s + c);
+            tmem_ld32(ts + kWalk + c, d + c);
+        }
+        tmem_wait_ld();
+        pin<kWalk>(s);
+        pin<kWalk>(d);
+#pragma unroll
+        for (int c = 0; c < kWalk; c += 4) {
+            float4 nl, nd;
+            if (DKV) {
+                nl = *reinterpret_cast<const float4 *>(&sh.neg_lse2[st][c]);
+                nd = *reinterpret_cast<const float4 *>(&sh.neg_delta[st][c]);
+            } else {
+                nl = make_float4(row_nl, row_nl, row_nl, row_nl);
+                nd = make_float4(row_nd, row_nd, row_nd, row_nd);
+            }
+            const float2 a = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(nl.x, nl.y));
+            const float2 b = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(nl.z, nl.w));
+            const float2 p = make_float2(exp2_fast(a.x), exp2_fast(a.y)), q = make_float2(exp2_fast(b.x), exp2_fast(b.y));
+            const float2 e = mul2(p, add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
+            const float2 f = mul2(q, add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
+            s[c] = p.x, s[c + 1] = p.y, s[c + 2] = q.x, s[c + 3] = q.y;
+            d[c] = e.x, d[c + 1] = e.y, d[c + 2] = f.x, d[c + 3] = f.y;
+        }
+        if (mask) {
+#pragma unroll
+            for (int c = 0; c < kWalk; ++c) {
+                const bool seen = c >= lo && c < hi;
+                s[c] = seen ? s[c] : 0.0f;
+                const bool one = c >= one_lo && c < one_hi;
+                d[c] = seen ? one ? (DKV ? sh.one_ds[st][c] : row_od) : d[c] : 0.0f;
+            }
+        }
+        uint32_t pk[32];
+        if (DKV) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pk[c] = pack_bf16(s[2 * c], s[2 * c + 1]);
+            tmem_st32(ts, pk);
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) pk[c] = pack_bf16(d[2 * c], d[2 * c + 1]);
+        tmem_st32(ts + kWalk, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.ds_ready[w]);
+    }
+    if (r.steps > 0) wait_warp(&sh.acc_done, 0, abort);
+    tc_fence_after();
+}
+
+// Writes columns [from, to) of a row of an accumulator (whole warp; `live` rows only).
+template <int DP>
+__device__ __forceinline__ void store_acc(uint32_t addr, bool any, int from, int to, float scale, bf16 *dst, int D,
+                                          bool live) {
+    for (int c = from; c < to; c += 32) {
+        float o[32];
+        if (any) {
+            tmem_ld32(addr + c, o);
+            tmem_wait_ld();
+            pin<32>(o);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+            if (c + e < D) {
+                uint4 v;
+                v.x = pack_bf16(o[e] * scale, o[e + 1] * scale);
+                v.y = pack_bf16(o[e + 2] * scale, o[e + 3] * scale);
+                v.z = pack_bf16(o[e + 4] * scale, o[e + 5] * scale);
+                v.w = pack_bf16(o[e + 6] * scale, o[e + 7] * scale);
+                *reinterpret_cast<uint4 *>(dst + c + e) = v;
+            }
+    }
+}
+
+// DKV: g0 = dK, g1 = dV.  Otherwise g0 = dQ.
+template <int DP, bool DKV>
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, const __grid_constant__ CUtensorMap mx1,
+                     const __grid_constant__ CUtensorMap my0, const __grid_constant__ CUtensorMap my1,
+                     const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ g_lse,
+                     bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots) {
+    using S = BwdShape<DP>;
+    extern __shared__ unsigned char dyn[];
+    __shared__ __align__(16) BwdShared sh;
+    const int warp = threadIdx.x >> 5;
+    const int heads = DKV ? A.Hkv : A.Hkv * A.subs;
+    const int hx = blockIdx.x % heads;
+    // The tiles with most work under a causal mask first: the first keys, the last queries.
+    const int slot = DKV ? blockIdx.x / heads : slots - 1 - (int)(blockIdx.x / heads);
+    const int per = DKV ? 128 : 128 / A.pack;
+    const Slot x = DKV ? find_slot(A.k_off, A.n_seq, A.Tk, per, slot) : find_slot(A.q_off, A.n_seq, A.Tq, per, slot);
+    if (x.first >= x.len) return;
+    const int G = A.Hq / A.Hkv;
+    BwdRange r;
+    r.kvh = DKV ? hx : hx / A.subs;
+    r.qhead = r.kvh * G + (DKV ? 0 : (hx % A.subs) * A.pack);
+    r.tok = kWalk / A.pack;
+    r.first = r.k0 = r.q0 = r.qtok = 0;
+    r.steps_per_sub = 1;
+    if (DKV) {
+        r.kbase = x.base, r.klen = x.len, r.k0 = x.first;
+        seq_range(A.q_off, A.n_seq, A.Tq, x.seq, r.qbase, r.qlen);
+        r.first = A.causal ? min(r.qlen, max(0, r.k0 + r.qlen - r.klen)) : 0;
+        r.steps_per_sub = (r.qlen - r.first + r.tok - 1) / r.tok;
+        r.steps = r.steps_per_sub * A.subs;
+    } else {
+        r.qbase = x.base, r.qlen = x.len, r.q0 = x.first;
+        seq_range(A.k_off, A.n_seq, A.Tk, x.seq, r.kbase, r.klen);
+        r.qtok = min(per, r.qlen - r.q0);
+        const int sees = A.causal ? min(r.klen, max(0, r.q0 + r.qtok + r.klen - r.qlen)) : r.klen;
+        r.steps = (sees + kWalk - 1) / kWalk;
+    }
+    const uint32_t smem_x = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t smem_y = smem_x + 2 * S::kXBytes;
+
+    if (warp == 8) {
+        if ((threadIdx.x & 31) == 0) {
+            mbar_init(&sh.x_full, 1);
+            for (int i = 0; i < S::kStages; ++i) {
+                mbar_init(&sh.y_full[i], 1);
+                mbar_init(&sh.y_empty[i], 1);
+            }
+            mbar_init(&sh.y_raw, 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&sh.s_full[b], 1);
+                mbar_init(&sh.ds_ready[b], 4);
+            }
+            mbar_init(&sh.acc_done, 1);
+            mbar_init(&sh.drain, 1);
+            sh.abort = 0;
+            mbar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&sh.tmem, S::kTmem);
+    }
+    // Rows of a step that no box ever fills (heads that do not divide 64) must hold numbers.
+    if (DKV && r.tok * A.pack < kWalk) {
+        for (int i = threadIdx.x; i < S::kStages * 2 * S::kYBytes / 16; i += S::kThreads)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_y + i * 16), "r"(0) : "memory");
+        fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    int issued = 0;
+    if (warp == 8) {
+        if ((threadIdx.x & 31) == 0 && r.steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, r.steps, tmem);
+    } else if (warp == 9) {
+        issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
+    } else {
+        bwd_grads<DP, DKV>(A, sh, r, tmem, lse, delta, g_lse);
+        __syncwarp();
+        const int w = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + 4 * kWalk;
+        const bool any = r.steps > 0;
+        if (DKV) {
+            const bool live = r.k0 + row < r.klen;
+            const size_t at = ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D;
+            if (w == 0) store_acc<DP>(acc, any, 0, DP, A.scale, g0 + at, A.D, live);
+            else store_acc<DP>(acc + DP, any, 0, DP, 1.0f, g1 + at, A.D, live);
+        } else {
+            const bool live = row / A.pack < r.qtok;
+            const size_t at =
+                ((size_t)(r.qbase + r.q0 + row / A.pack) * A.Hq + r.qhead + row % A.pack) * A.D;
+            const int half = DP >= 64 ? DP / 2 : DP;  // columns of the first warpgroup
+            store_acc<DP>(acc, any, w * half, w == 0 ? half : DP, A.scale, g0 + at, A.D, live);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0 && r.steps > 0) {
+        mbar_drain(&sh.x_full, 0, kAttnWaitLimit);
+        for (int i = max(0, issued - S::kStages); i < issued; ++i)
+            mbar_drain(&sh.y_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
+    }
+    if (warp == 8) {
+        if (sh.abort && (threadIdx.x & 31) == 0) {
+            tc_commit(&sh.drain);
+            mbar_drain(&sh.drain, 0, kAttnWaitLimit);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+// delta[h][t] = o.g - c per row, LANES lanes of eight channels to a row.
+template <int LANES>
+__global__ void __launch_bounds__(256)
+attn_delta_kernel(const bf16 *__restrict__ out, const bf16 *__restrict__ g, long long g_token, long long g_head,
+                  const float *__restrict__ g_lse, int Tq, int Hq, int D, float *__restrict__ delta) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = i / LANES;  // token * Hq + head
+    const int c = (int)(i % LANES) * 8;
+    const bool live = row < (long long)Tq * Hq && c < D;
+    const long long token = row / Hq;
+    const int head = (int)(row % Hq);
+    float sum = 0.0f;
+    if (live) {
+        float a[8], b[8];
+        load_vec<bf16, 8, true>(out + row * D + c, a);
+        load_vec<bf16, 8, true>(g + token * g_token + head * g_head + c, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (live && c == 0) {
+        const size_t x = (size_t)head * Tq + token;
+        delta[x] = sum - (g_lse ? g_lse[x] : 0.0f);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------------------------
+
+// The largest divisor of the group that is at most `most`.
+int pack_of(long long group, int most) {
+    for (int p = (int)(group < most ? group : most); p > 1; --p)
+        if (group % p == 0) return p;
+    return 1;
+}
+
+int padded_dim(long long D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+struct Strided {
+    const void *p;
+    int64_t token, head;  // strides in elements
+};
+
+// Boxes of `heads` x `tokens` rows, one column panel wide.
+bool make_map(CUtensorMap *map, const Strided &t, long long T, long long H, long long D, int heads, int tokens,
+              const void *spare) {
+    const int cols = D <= 32 ? 32 : 64;
+    uint64_t dims[3] = {(uint64_t)D, (uint64_t)H, (uint64_t)(T > 0 ? T : 1)};
+    uint64_t strides[2] = {(uint64_t)t.head * 2, (uint64_t)t.token * 2};
+    const void *base = t.p;
+    if (T == 0) {  // never loaded from; any valid description does
+        strides[0] = strides[1] = 16;
+        dims[0] = 8;
+        dims[1] = 1;
+        base = spare;
+    }
+    const uint32_t box[3] = {(uint32_t)cols, (uint32_t)heads, (uint32_t)tokens};
+    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box,
+                             cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename K> int allow_smem(K kernel, size_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess
+               ? RFDETR_OK
+               : RFDETR_ERR_CUDA;
+}
+
+constexpr long long kMaxRows = 1ll << 30;  // rows and offsets are int32 in the kernels
+
+int check_sizes(int64_t n_seq, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D) {
+    if (n_seq < 0 || n_seq > kMaxRows || Tq < 0 || Tq > kMaxRows || Tk < 0 || Tk > kMaxRows) return RFDETR_ERR_SHAPE;
+    if (Hkv < 1 || Hq < Hkv || Hq > 65536 || Hq % Hkv) return RFDETR_ERR_SHAPE;
+    if (D < 8 || D > 128 || D % 8) return RFDETR_ERR_SHAPE;
+    return RFDETR_OK;
+}
+
+int check_tensor(const Strided &t, int64_t T, int64_t H) {
+    if (T == 0) return RFDETR_OK;
+    if (!t.p || !aligned(t.p, 16)) return RFDETR_ERR_ALIGN;
+    // Strides of a size-1 axis do not matter to the caller, but the tensor map wants them valid.
+    if (t.token <= 0 || t.head <= 0 || t.token % 8 || t.head % 8) return RFDETR_ERR_ALIGN;
+    if (t.token >= (1ll << 38) || t.head >= (1ll << 38)) return RFDETR_ERR_SHAPE;
+    (void)H;
+    return RFDETR_OK;
+}
+
+// Row tiles per block: one where the sequences are short enough (by their mean) that a second
+// tile would mostly be empty.
+int row_tiles(int64_t n_seq, int64_t Tq, int per) { (void)n_seq, (void)Tq, (void)per; return 2; }
+
+// Blocks over which each row tile's keys are split.
+int key_splits(int64_t n_seq, int64_t Tq, int64_t Tk, long long tiles_per_row, int per, int nt) {
+    (void)n_seq, (void)Tq, (void)Tk, (void)tiles_per_row, (void)per, (void)nt;
+    return 1;
+}
+
+template <int DP, int NT>
+int launch_forward(const AttnArgs &A, const Strided &q, const Strided &k, const Strided &v, bf16 *out, float *lse,
+                   float *part, float *part_lse, int splits, cudaStream_t stream) {
+    using S = FwdShape<DP, NT>;
+    const int per = 128 / A.pack;
+    CUtensorMap mq, mk, mv;
+    if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
+        !make_map(&mv, v, A.Tk, A.Hkv, A.D, 1, 128, q.p))
+        return RFDETR_ERR_CUDA;
+    const long long slots = slots_for(A.Tq, per * NT, A.n_seq);
+    const long long blocks = slots * A.Hkv * A.subs;
+    if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+    const dim3 grid((unsigned)blocks, 1, (unsigned)splits);
+    if (splits > 1) {
+        if (int st = allow_smem(attn_forward_kernel<DP, NT, true>, S::kSmem)) return st;
+        attn_forward_kernel<DP, NT, true>
+            <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
+        if (int st = launch_status()) return st;
+        const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
+        if ((n + 255) / 256 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+        attn_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(part, part_lse, splits, rows, A.Hq, A.Tq, A.D,
+                                                                         out, lse);
+    } else {
+        if (int st = allow_smem(attn_forward_kernel<DP, NT, false>, S::kSmem)) return st;
+        attn_forward_kernel<DP, NT, false>
+            <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
+    }
+    return launch_status();
+}
+
+template <int DP>
+int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
+                    const float *lse, const float *delta, const float *g_lse, bf16 *dq, bf16 *dk, bf16 *dv,
+                    cudaStream_t stream) {
+    using S = BwdShape<DP>;
+    CUtensorMap kx, vx, qy, gy, qx, gx, ky, vy;
+    const int ytok = kWalk / A.pack, xtok = 128 / A.pack;
+    if (!make_map(&kx, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) || !make_map(&vx, v, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
+        !make_map(&ky, k, A.Tk, A.Hkv, A.D, 1, kWalk, q.p) || !make_map(&vy, v, A.Tk, A.Hkv, A.D, 1, kWalk, q.p) ||
+        !make_map(&qy, q, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) || !make_map(&gy, g, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) ||
+        !make_map(&qx, q, A.Tq, A.Hq, A.D, A.pack, xtok, k.p) || !make_map(&gx, g, A.Tq, A.Hq, A.D, A.pack, xtok, k.p))
+        return RFDETR_ERR_CUDA;
+    if (A.Tk > 0) {
+        const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
+        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+        if (int st = allow_smem(attn_backward_kernel<DP, true>, S::kSmem)) return st;
+        attn_backward_kernel<DP, true>
+            <<<(unsigned)blocks, S::kThreads, S::kSmem, stream>>>(A, kx, vx, qy, gy, lse, delta, g_lse, dk, dv,
+                                                                  (int)slots);
+        if (int st = launch_status()) return st;
+    }
+    if (A.Tq > 0) {
+        const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
+        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+        if (int st = allow_smem(attn_backward_kernel<DP, false>, S::kSmem)) return st;
+        attn_backward_kernel<DP, false><<<(unsigned)blocks, S::kThreads, S::kSmem, stream>>>(
+            A, qx, gx, ky, vy, lse, delta, g_lse, dq, nullptr, (int)slots);
+    }
+    return launch_status();
+}
+
+AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, int64_t Tq, int64_t Tk, int64_t Hq,
+                   int64_t Hkv, int64_t D, int causal, float scale, int most_packed) {
+    AttnArgs A;
+    A.q_off = q_off;
+    A.k_off = k_off ? k_off : q_off;
+    A.n_seq = (int)n_seq;
+    A.Tq = (int)Tq;
+    A.Tk = (int)Tk;
+    A.Hq = (int)Hq;
+    A.Hkv = (int)Hkv;
+    A.D = (int)D;
+    A.pack = pack_of(Hq / Hkv, most_packed);
+    A.subs = (int)(Hq / Hkv) / A.pack;
+    A.causal = causal != 0;
+    A.scale = scale;
+    A.scale_log2 = scale * kLog2e;
+    return A;
+}
+
+struct ForwardPlan {
+    int nt, splits;
+};
+ForwardPlan plan_forward(const AttnArgs &A) {
+    const int per = 128 / A.pack;
+    ForwardPlan p;
+    p.nt = row_tiles(A.n_seq, A.Tq, per);
+    p.splits = key_splits(A.n_seq, A.Tq, A.Tk, (long long)A.Hkv * A.subs, per, p.nt);
+    return p;
+}
+
+size_t split_bytes(const AttnArgs &A, int splits) {
+    return splits <= 1 ? 0 : (size_t)splits * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
+}
+
+}  // namespace
+
+// Reads and clears this file's device fault word; bits are those of mbar_wait / mbar_drain.
+int take_attention_fault(cudaStream_t stream, unsigned *word) {
+    void *p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_device_fault) != cudaSuccess) return RFDETR_ERR_CUDA;
+    if (cudaMemcpyAsync(word, p, sizeof(unsigned), cudaMemcpyDeviceToHost, stream) != cudaSuccess)
+        return RFDETR_ERR_CUDA;
+    if (cudaMemsetAsync(p, 0, sizeof(unsigned), stream) != cudaSuccess) return RFDETR_ERR_CUDA;
+    return cudaStreamSynchronize(stream) == cudaSuccess ? RFDETR_OK : RFDETR_ERR_CUDA;
+}
+
+}  // namespace rfdetr
+
+extern "C" size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, int64_t tokens, int64_t key_tokens,
+                                                          int64_t n_heads, int64_t n_kv_heads, int64_t head_dim) {
+    using namespace rfdetr;
+    if (check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim) != RFDETR_OK) return 0;
+    const AttnArgs A = make_args(nullptr, nullptr, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, 0,
+                                 1.0f, 128);
+    return split_bytes(A, plan_forward(A).splits);
+}
+
+extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride,
+                                       int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                       int64_t key_head_stride, const void *value, int64_t value_token_stride,
+                                       int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
+                                       void *output, float *lse, void *workspace, size_t workspace_bytes,
+                                       int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
+                                       int64_t n_kv_heads, int64_t head_dim, int causal, float scale) {
+    using namespace rfdetr;
+    if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
+    if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
+    if (tokens == 0) return RFDETR_OK;
+    const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
+        v{value, value_token_stride, value_head_stride};
+    if (int st = check_tensor(q, tokens, n_heads)) return st;
+    if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
+    if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
+    if (!output || !aligned(output, 16) || !aligned(lse, 4) || !offsets || !aligned(offsets, 4) ||
+        !aligned(key_offsets, 4))
+        return RFDETR_ERR_ALIGN;
+    const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
+                                 causal, scale, 128);
+    const ForwardPlan p = plan_forward(A);
+    const size_t need = split_bytes(A, p.splits);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return RFDETR_ERR_WORKSPACE;
+    float *part = static_cast<float *>(workspace);
+    float *part_lse = need ? part + (size_t)p.splits * A.Tq * A.Hq * A.D : nullptr;
+    bf16 *out = static_cast<bf16 *>(output);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (padded_dim(head_dim)) {
+        case 32: return launch_forward<32, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
+        case 64: return launch_forward<64, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
+        default: return launch_forward<128, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
+    }
+}
+
+extern "C" size_t rfdetr_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t n_heads) {
+    if (tokens < 0 || tokens > rfdetr::kMaxRows || n_heads < 0 || n_heads > 65536) return 0;
+    return (size_t)tokens * n_heads * sizeof(float);
+}
+
+extern "C" int rfdetr_packed_attention_backward(
+    void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride, const void *key,
+    int64_t key_token_stride, int64_t key_head_stride, const void *value, int64_t value_token_stride,
+    int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets, const void *output,
+    const float *lse, const void *grad_output, int64_t grad_token_stride, int64_t grad_head_stride,
+    const float *grad_lse, void *grad_query, void *grad_key, void *grad_value, void *workspace, size_t workspace_bytes,
+    int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+    int causal, float scale) {
+    using namespace rfdetr;
+    if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
+    if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
+    if (tokens == 0 && key_tokens == 0) return RFDETR_OK;
+    const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
+        v{value, value_token_stride, value_head_stride}, g{grad_output, grad_token_stride, grad_head_stride};
+    if (int st = check_tensor(q, tokens, n_heads)) return st;
+    if (int st = check_tensor(g, tokens, n_heads)) return st;
+    if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
+    if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
+    if (!offsets || !aligned(offsets, 4) || !aligned(key_offsets, 4)) return RFDETR_ERR_ALIGN;
+    if (tokens > 0 && (!output || !aligned(output, 16) || !grad_query || !aligned(grad_query, 16) || !lse ||
+                       !aligned(lse, 4) || !aligned(grad_lse, 4)))
+        return RFDETR_ERR_ALIGN;
+    if (key_tokens > 0 && (!grad_key || !grad_value || !aligned(grad_key, 16) || !aligned(grad_value, 16)))
+        return RFDETR_ERR_ALIGN;
+    const size_t need = rfdetr_packed_attention_backward_workspace_bytes(tokens, n_heads);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 4))) return RFDETR_ERR_WORKSPACE;
+    const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
+                                 causal, scale, kWalk);
+    float *delta = static_cast<float *>(workspace);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tokens > 0) {
+        const int dp = padded_dim(head_dim);
+        const long long rows = (long long)tokens * n_heads, blocks = (rows * (dp / 8) + 255) / 256;
+        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+        const bf16 *o = static_cast<const bf16 *>(output), *go = static_cast<const bf16 *>(grad_output);
+        auto launch = [&](auto kernel) {
+            kernel<<<(unsigned)blocks, 256, 0, s>>>(o, go, grad_token_stride, grad_head_stride, grad_lse, (int)tokens,
+                                                    (int)n_heads, (int)head_dim, delta);
+        };
+        if (dp == 32) launch(attn_delta_kernel<4>);
+        else if (dp == 64) launch(attn_delta_kernel<8>);
+        else launch(attn_delta_kernel<16>);
+        if (int st = launch_status()) return st;
+    }
+    bf16 *dq = static_cast<bf16 *>(grad_query), *dk = static_cast<bf16 *>(grad_key),
+         *dv = static_cast<bf16 *>(grad_value);
+    switch (padded_dim(head_dim)) {
+        case 32: return launch_backward<32>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
+        case 64: return launch_backward<64>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
+        default: return launch_backward<128>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
+    }
+}

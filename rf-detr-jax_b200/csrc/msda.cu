@@ -3420,13 +3420,19 @@ extern "C" int rfdetr_selftest_bounded_wait(void *stream, int polls, int32_t *re
     return launch_status();
 }
 
+namespace rfdetr {
+int take_attention_fault(cudaStream_t stream, unsigned *word);  // attention.cu
+}
+
 extern "C" int rfdetr_take_device_fault(void *stream) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    unsigned int attention = 0;
+    if (int st = rfdetr::take_attention_fault(s, &attention)) return st;
     unsigned int v = 0;
     if (cudaMemcpyFromSymbolAsync(&v, rfdetr::g_device_fault, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
         cudaStreamSynchronize(s) != cudaSuccess)
         return RFDETR_ERR_CUDA;
-    if (v == 0) return RFDETR_OK;
+    if (v == 0) return attention ? RFDETR_ERR_LIMIT : RFDETR_OK;
     const unsigned int zero = 0;
     if (cudaMemcpyToSymbolAsync(rfdetr::g_device_fault, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
         cudaStreamSynchronize(s) != cudaSuccess)

@@ -1,0 +1,187 @@
+// Rotary positions with several axes, for queries and keys in one launch.
+//
+// Frequency i of R/2 belongs to an axis a(i) (consecutive sections, one per axis) and turns the
+// pair (x1, x2) of every head of token t by theta = positions[t, a(i)] * inv_freq[i]:
+//   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
+// with (x1, x2) the channels (i, i + R/2), or (2i, 2i + 1) when interleaved; channels from R on are
+// copied.  The gradient is the same turn by -theta.
+//
+// The bound is memory: each value is read and written once, and the turns are a few operations on
+// it.  So that the sines stay out of the way, a block takes a few tokens, forms their cosines and
+// sines once in shared memory for all heads of q and k, and then streams the heads through in
+// 16-byte pieces.  The angle is formed in float64 and reduced to a fraction of a turn before it is
+// narrowed: at position 16384 a float32 product is already wrong by 1e-3 radians.
+#include "common.cuh"
+
+namespace rfdetr {
+namespace {
+
+constexpr int kMaxAxes = 8;
+constexpr int kRotaryThreads = 256;
+constexpr double kInvTwoPi = 0.15915494309189533576888;
+
+struct RotaryArgs {
+    const void *in[2];       // q, k
+    void *out[2];            // contiguous [T, H, D]
+    long long token[2], head[2];  // input strides, elements
+    int heads[2];
+    const void *positions;   // [T, n_axes]
+    const float *inv_freq;   // [half]
+    int ends[kMaxAxes];      // end of each axis's section of frequencies
+    int n_axes;
+    long long T;
+    int D, half;
+    int per_block;           // tokens
+    float sign;              // -1: the inverse turn
+};
+
+// Pieces of VEC channels.  A head's pieces: the turned ones first (one piece of x1 and one of x2,
+// or one piece of VEC / 2 pairs), then the copied ones.
+template <typename T, typename P, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotaryThreads) axial_rotary_kernel(const RotaryArgs A) {
+    extern __shared__ float2 turn[];  // [token][half]
+    const long long t0 = (long long)blockIdx.x * A.per_block;
+    const int tokens = (int)min((long long)A.per_block, A.T - t0);
+    const P *pos = static_cast<const P *>(A.positions) + t0 * A.n_axes;
+    for (int x = threadIdx.x; x < tokens * A.half; x += kRotaryThreads) {
+        const int t = x / A.half, i = x - t * A.half;
+        int axis = 0;
+        while (i >= A.ends[axis]) ++axis;
+        const double turns = (double)pos[t * A.n_axes + axis] * (double)__ldg(A.inv_freq + i) * kInvTwoPi;
+        float s, c;
+        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+        turn[x] = make_float2(c, s * A.sign);
+    }
+    __syncthreads();
+
+    const int R = 2 * A.half;
+    const int turned = INTERLEAVED ? R / VEC : A.half / VEC;
+    const int per_head = turned + (A.D - R) / VEC;
+    const int per_token = per_head * (A.heads[0] + A.heads[1]);
+    for (int x = threadIdx.x; x < tokens * per_token; x += kRotaryThreads) {
+        const int t = x / per_token, y = x - t * per_token;
+        int h = y / per_head;
+        const int piece = y - h * per_head;
+        const int which = h >= A.heads[0];
+        h -= which ? A.heads[0] : 0;
+        const T *in = static_cast<const T *>(A.in[which]) + (t0 + t) * A.token[which] + h * A.head[which];
+        T *out = static_cast<T *>(A.out[which]) + ((t0 + t) * A.heads[which] + h) * A.D;
+        const float2 *cs = turn + t * A.half;
+        if (piece >= turned) {
+            const int c = R + (piece - turned) * VEC;
+            float v[VEC];
+            load_vec<T, VEC, true>(in + c, v);
+            store_vec<T, VEC>(out + c, v);
+        } else if constexpr (INTERLEAVED) {
+            const int c = piece * VEC;
+            float v[VEC], w[VEC];
+            load_vec<T, VEC, true>(in + c, v);
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+                const float2 r = cs[(c + e) >> 1];
+                w[e] = v[e] * r.x - v[e + 1] * r.y;
+                w[e + 1] = v[e + 1] * r.x + v[e] * r.y;
+            }
+            store_vec<T, VEC>(out + c, w);
+        } else {
+            const int c = piece * VEC;
+            float a[VEC], b[VEC], u[VEC], w[VEC];
+            load_vec<T, VEC, true>(in + c, a);
+            load_vec<T, VEC, true>(in + c + A.half, b);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 r = cs[c + e];
+                u[e] = a[e] * r.x - b[e] * r.y;
+                w[e] = b[e] * r.x + a[e] * r.y;
+            }
+            store_vec<T, VEC>(out + c, u);
+            store_vec<T, VEC>(out + c + A.half, w);
+        }
+    }
+}
+
+template <typename T, typename P, int VEC>
+int launch_rotary(const RotaryArgs &A, bool interleaved, cudaStream_t stream) {
+    const long long blocks = (A.T + A.per_block - 1) / A.per_block;
+    if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+    const size_t smem = (size_t)A.per_block * A.half * sizeof(float2);
+    if (interleaved) {
+        if constexpr (VEC >= 2)
+            axial_rotary_kernel<T, P, VEC, true><<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(A);
+        else
+            return RFDETR_ERR_SHAPE;
+    } else {
+        axial_rotary_kernel<T, P, VEC, false><<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(A);
+    }
+    return launch_status();
+}
+
+template <typename T, typename P>
+int dispatch_rotary(const RotaryArgs &A, bool interleaved, int vec, cudaStream_t stream) {
+    if (vec * sizeof(T) >= 16) return launch_rotary<T, P, 16 / sizeof(T)>(A, interleaved, stream);
+    if (vec >= 2) return launch_rotary<T, P, 2>(A, interleaved, stream);
+    return launch_rotary<T, P, 1>(A, interleaved, stream);
+}
+
+}  // namespace
+}  // namespace rfdetr
+
+extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t query_token_stride,
+                                   int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                   int64_t key_head_stride, int dtype, const void *positions, int position_dtype,
+                                   const float *inv_freq, const int64_t *sections, int64_t n_axes, void *query_out,
+                                   void *key_out, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                   int64_t head_dim, int interleaved, int inverse) {
+    using namespace rfdetr;
+    if (dtype_size(dtype) == 0 || (position_dtype != RFDETR_F32 && position_dtype != RFDETR_I32))
+        return RFDETR_ERR_DTYPE;
+    if (tokens < 0 || tokens > (1ll << 40) || n_heads < 0 || n_heads > 65536 || n_kv_heads < 0 || n_kv_heads > 65536 ||
+        head_dim < 2 || head_dim > 1024 || n_axes < 1 || n_axes > kMaxAxes || !sections)
+        return RFDETR_ERR_SHAPE;
+    if (query_token_stride < 0 || query_head_stride < 0 || key_token_stride < 0 || key_head_stride < 0)
+        return RFDETR_ERR_SHAPE;
+    RotaryArgs A{};
+    long long half = 0;
+    for (int a = 0; a < n_axes; ++a) {
+        if (sections[a] < 0 || sections[a] > head_dim) return RFDETR_ERR_SHAPE;
+        half += sections[a];
+        A.ends[a] = (int)half;
+    }
+    if (half < 1 || 2 * half > head_dim) return RFDETR_ERR_SHAPE;
+    if (n_kv_heads == 0) key = query, key_out = query_out;  // not read or written
+    if (tokens == 0 || n_heads + n_kv_heads == 0) return RFDETR_OK;
+    const int size = dtype_size(dtype);
+    if ((n_heads && (!query || !query_out || !aligned(query, size) || !aligned(query_out, size))) ||
+        (n_kv_heads && (!key || !key_out || !aligned(key, size) || !aligned(key_out, size))) || !positions ||
+        !aligned(positions, 4) || !inv_freq || !aligned(inv_freq, 4))
+        return RFDETR_ERR_ALIGN;
+    A.in[0] = query, A.in[1] = key, A.out[0] = query_out, A.out[1] = key_out;
+    A.token[0] = query_token_stride, A.token[1] = key_token_stride;
+    A.head[0] = query_head_stride, A.head[1] = key_head_stride;
+    A.heads[0] = (int)n_heads, A.heads[1] = (int)n_kv_heads;
+    A.positions = positions, A.inv_freq = inv_freq, A.n_axes = (int)n_axes;
+    A.T = tokens, A.D = (int)head_dim, A.half = (int)half, A.sign = inverse ? -1.0f : 1.0f;
+    // The widest piece, up to 16 bytes, that every address and boundary allows.
+    int vec = 16 / size;
+    auto fits = [&](int v) {
+        const long long b = (long long)v * size;
+        bool ok = head_dim % v == 0 && (interleaved ? 2 * half : half) % v == 0;
+        for (int w = 0; w < 2; ++w)
+            if (A.heads[w])
+                ok = ok && aligned(A.in[w], b) && aligned(A.out[w], b) && A.token[w] % v == 0 && A.head[w] % v == 0;
+        return ok;
+    };
+    if (!fits(vec)) vec = fits(2) ? 2 : 1;
+    if (interleaved && vec < 2) return RFDETR_ERR_ALIGN;
+    // Tokens to a block: enough blocks to fill the device several times, and few enough sines at
+    // once to leave shared memory to the other blocks of an SM.
+    long long per = tokens / ((long long)num_sms() * 8);
+    const long long most = 16384 / (half * (long long)sizeof(float2));
+    per = per < 1 ? 1 : per > 16 ? 16 : per;
+    A.per_block = (int)(per > most ? (most < 1 ? 1 : most) : per);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool il = interleaved != 0, real = position_dtype == RFDETR_F32;
+    if (dtype == RFDETR_BF16)
+        return real ? dispatch_rotary<bf16, float>(A, il, vec, s) : dispatch_rotary<bf16, int32_t>(A, il, vec, s);
+    return real ? dispatch_rotary<float, float>(A, il, vec, s) : dispatch_rotary<float, int32_t>(A, il, vec, s);
+}

@@ -23,8 +23,8 @@
 namespace rfdetr {
 
 // Set (bit 0) when a bounded device wait gave up.  The library compiles each .cu file as its
-// own device module, so this word is per translation unit; the waits live in msda.cu, whose
-// copy rfdetr_take_device_fault() reads.
+// own device module, so this word is per translation unit; the waits live in msda.cu and
+// attention.cu, whose copies rfdetr_take_device_fault() reads.
 static __device__ unsigned int g_device_fault = 0;
 
 constexpr int kWaitLimit = 1 << 22;

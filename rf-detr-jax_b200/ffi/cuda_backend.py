@@ -37,7 +37,7 @@ _lib = ctypes.cdll.LoadLibrary(os.environ.get("RFDETR_FFI_LIB", os.path.join(_HE
 
 HANDLERS = ("RfdetrMsdaFwd", "RfdetrMsdaBwd", "RfdetrMsdaBwdNoAlloc", "RfdetrMsdaPrologue", "RfdetrMsdaPrologueBwd",
             "RfdetrTopkSelect", "RfdetrSelectRows", "RfdetrMatchCost", "RfdetrLsapBatched", "RfdetrMatchStacked",
-            "RfdetrSetLosses")
+            "RfdetrSetLosses", "RfdetrPackedAttention", "RfdetrPackedAttentionBwd", "RfdetrAxialRotary")
 for _name in HANDLERS:
     jax.ffi.register_ffi_target(_name, jax.ffi.pycapsule(getattr(_lib, _name)), platform="CUDA")
 
@@ -241,3 +241,61 @@ def _set_losses_bwd(focal_alpha, ia_bce, residuals, g):
 
 
 set_losses.defvjp(_set_losses_fwd, _set_losses_bwd)
+
+
+# ---- packed attention and rotary positions -----------------------------------------------------
+@functools.partial(jax.custom_vjp, nondiff_argnums=(5, 6))
+def packed_attention(query, key, value, offsets, key_offsets, causal=False, scale=None):
+    """Attention within the sequences of packed rows (the padded batches of ``layers.py:54-98``
+    without their padding): ``(output [T, H, D], lse [H, T])``."""
+    return _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+
+
+def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale):
+    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype),
+            jax.ShapeDtypeStruct((query.shape[1], query.shape[0]), jnp.float32))
+    return jax.ffi.ffi_call("RfdetrPackedAttention", outs)(
+        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32),
+        causal=np.int32(1 if causal else 0), scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
+
+
+def _packed_attention_fwd(query, key, value, offsets, key_offsets, causal, scale):
+    out, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    return (out, lse), (query, key, value, offsets, key_offsets, out, lse)
+
+
+def _packed_attention_bwd(causal, scale, residuals, g):
+    query, key, value, offsets, key_offsets, out, lse = residuals
+    shapes = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key, value))
+    grads = jax.ffi.ffi_call("RfdetrPackedAttentionBwd", shapes)(
+        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, lse, g[0].astype(out.dtype),
+        g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
+        scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
+    return *grads, None, None
+
+
+packed_attention.defvjp(_packed_attention_fwd, _packed_attention_bwd)
+
+
+@functools.partial(jax.custom_vjp, nondiff_argnums=(4, 5))
+def axial_rotary(query, key, positions, inv_freq, sections, interleaved=False):
+    """Queries and keys turned by their tokens' positions on several axes."""
+    return _axial_rotary_call(query, key, positions, inv_freq, sections, interleaved, False)
+
+
+def _axial_rotary_call(query, key, positions, inv_freq, sections, interleaved, inverse):
+    outs = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key))
+    return jax.ffi.ffi_call("RfdetrAxialRotary", outs)(
+        query, key, positions, inv_freq.astype(jnp.float32), sections=np.asarray(sections, np.int64),
+        interleaved=np.int32(1 if interleaved else 0), inverse=np.int32(1 if inverse else 0))
+
+
+def _axial_rotary_fwd(query, key, positions, inv_freq, sections, interleaved):
+    return (_axial_rotary_call(query, key, positions, inv_freq, sections, interleaved, False), (positions, inv_freq))
+
+
+def _axial_rotary_bwd(sections, interleaved, residuals, g):
+    return *_axial_rotary_call(*g, *residuals, sections, interleaved, True), None, None
+
+
+axial_rotary.defvjp(_axial_rotary_fwd, _axial_rotary_bwd)

@@ -375,3 +375,116 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrSetLosses, SetLosses,
                                   .Ret<ffi::Buffer<ffi::F32>>()
                                   .Ret<ffi::Buffer<ffi::F32>>()
                                   .Ret<ffi::Buffer<ffi::F32>>());
+
+// Packed attention: (query [T, H, D], key, value [Tk, Hkv, D] bf16, offsets, key_offsets int32 [S + 1])
+// -> (output, lse [H, T]).
+static ffi::Error PackedAttention(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query,
+                                  ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
+                                  ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets, int32_t causal,
+                                  float scale, ffi::Result<ffi::Buffer<ffi::BF16>> output,
+                                  ffi::Result<ffi::Buffer<ffi::F32>> lse) {
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
+    const int64_t S = dim(offsets, 0) - 1;
+    const size_t bytes = rfdetr_packed_attention_workspace_bytes(S, T, Tk, H, Hkv, D);
+    void *ws = nullptr;
+    if (bytes) {
+        auto block = scratch.Allocate(bytes, 256);
+        if (!block.has_value())
+            return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrPackedAttention: workspace");
+        ws = *block;
+    }
+    return status_error(
+        rfdetr_packed_attention(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
+                                value.untyped_data(), Hkv * D, D, offsets.typed_data(), key_offsets.typed_data(),
+                                output->untyped_data(), lse->typed_data(), ws, bytes, S, T, Tk, H, Hkv, D, causal,
+                                scale),
+        "RfdetrPackedAttention");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrPackedAttention, PackedAttention,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Attr<int32_t>("causal")
+                                  .Attr<float>("scale")
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// Its gradients: (query, key, value, offsets, key_offsets, output, lse, grad_output, grad_lse) ->
+// (grad_query, grad_key, grad_value).
+static ffi::Error PackedAttentionBwd(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query,
+                                     ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
+                                     ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets,
+                                     ffi::Buffer<ffi::BF16> output, ffi::Buffer<ffi::F32> lse,
+                                     ffi::Buffer<ffi::BF16> grad_output, ffi::Buffer<ffi::F32> grad_lse,
+                                     int32_t causal, float scale, ffi::Result<ffi::Buffer<ffi::BF16>> grad_query,
+                                     ffi::Result<ffi::Buffer<ffi::BF16>> grad_key,
+                                     ffi::Result<ffi::Buffer<ffi::BF16>> grad_value) {
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
+    const size_t bytes = rfdetr_packed_attention_backward_workspace_bytes(T, H);
+    void *ws = nullptr;
+    if (bytes) {
+        auto block = scratch.Allocate(bytes, 256);
+        if (!block.has_value())
+            return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrPackedAttentionBwd: workspace");
+        ws = *block;
+    }
+    return status_error(
+        rfdetr_packed_attention_backward(
+            stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D, value.untyped_data(), Hkv * D, D,
+            offsets.typed_data(), key_offsets.typed_data(), output.untyped_data(), lse.typed_data(),
+            grad_output.untyped_data(), H * D, D, grad_lse.typed_data(), grad_query->untyped_data(),
+            grad_key->untyped_data(), grad_value->untyped_data(), ws, bytes, dim(offsets, 0) - 1, T, Tk, H, Hkv, D,
+            causal, scale),
+        "RfdetrPackedAttentionBwd");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrPackedAttentionBwd, PackedAttentionBwd,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int32_t>("causal")
+                                  .Attr<float>("scale")
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
+
+// Rotary positions: (query [T, H, D], key [T, Hkv, D], positions [T, A] f32 or int32, inv_freq) ->
+// (query, key) turned; `inverse` for the gradient.
+static ffi::Error AxialRotary(cudaStream_t stream, ffi::AnyBuffer query, ffi::AnyBuffer key, ffi::AnyBuffer positions,
+                              ffi::Buffer<ffi::F32> inv_freq, ffi::Span<const int64_t> sections, int32_t interleaved,
+                              int32_t inverse, ffi::Result<ffi::AnyBuffer> query_out,
+                              ffi::Result<ffi::AnyBuffer> key_out) {
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Hkv = dim(key, 1);
+    const int pd = positions.element_type() == ffi::DataType::S32 ? RFDETR_I32 : dtype_code(positions.element_type());
+    return status_error(
+        rfdetr_axial_rotary(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
+                            dtype_code(query.element_type()), positions.untyped_data(), pd, inv_freq.typed_data(),
+                            sections.begin(), static_cast<int64_t>(sections.size()), query_out->untyped_data(),
+                            key_out->untyped_data(), T, H, Hkv, D, interleaved, inverse),
+        "RfdetrAxialRotary");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrAxialRotary, AxialRotary,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<ffi::Span<const int64_t>>("sections")
+                                  .Attr<int32_t>("interleaved")
+                                  .Attr<int32_t>("inverse")
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>());

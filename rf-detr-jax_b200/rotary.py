@@ -1,0 +1,106 @@
+"""Rotary positions with several axes on B200: queries and keys turned in one launch.
+
+For attention over image or video tokens whose place is told by angles (time, height, width), next
+to :func:`.attention.packed_attention`.  The gradient is the inverse turn, by the same kernel.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+
+def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
+    return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
+
+
+def rotary_launch(query, key, positions, inv_freq, sections, interleaved, inverse):
+    """One launch over checked inputs; ``key`` may be None."""
+    tokens, heads, dim = query.shape
+    pairs = query.data_ptr() % (2 * query.element_size()) == 0 and query.stride(0) % 2 == 0 and query.stride(1) % 2 == 0
+    if interleaved and not pairs:
+        query = query.clone(memory_format=torch.contiguous_format)
+    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
+    key_out, kv_heads, key_strides = None, 0, (0, 0)
+    if key is not None:
+        if interleaved and (key.data_ptr() % (2 * key.element_size()) or key.stride(0) % 2 or key.stride(1) % 2):
+            key = key.clone(memory_format=torch.contiguous_format)
+        kv_heads, key_strides = key.shape[1], (key.stride(0), key.stride(1))
+        key_out = torch.empty((tokens, kv_heads, dim), dtype=key.dtype, device=key.device)
+    status = N.lib().rfdetr_axial_rotary(
+        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), N.ptr(key), *key_strides,
+        N.dtype_code(query.dtype), positions.data_ptr(), N.F32 if positions.dtype == torch.float32 else N.I32,
+        inv_freq.data_ptr(), N.int64_array(sections), len(sections), out.data_ptr(), N.ptr(key_out), tokens, heads,
+        kv_heads, dim, int(interleaved), int(inverse))
+    N.check(status, "rfdetr_axial_rotary")
+    return out, key_out
+
+
+class AxialRotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, positions, inv_freq, sections, interleaved):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = (sections, interleaved)
+        return rotary_launch(query, key, positions, inv_freq, sections, interleaved, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_query, grad_key):
+        positions, inv_freq = ctx.saved_tensors
+        grads = rotary_launch(_rows("grad_query", grad_query), None if grad_key is None else _rows("grad_key", grad_key),
+                              positions, inv_freq, *ctx.how, True)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
+
+
+def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 sections, *, interleaved: bool = False):
+    """Turns the channels of queries and keys by their tokens' positions.
+
+    Args:
+        query, key: ``[tokens, heads, head_dim]`` and ``[tokens, kv_heads, head_dim]`` float32 or
+            bfloat16 (views of a fused projection are read in place); ``key`` may be None.
+        positions: ``[tokens, axes]`` float32 or int32 (int64 is narrowed).
+        inv_freq: ``[sum(sections)]`` float32, radians per unit of position.
+        sections: frequencies per axis, in order; ``2 * sum(sections) <= head_dim`` and the channels
+            beyond are copied.
+        interleaved: pairs of channels ``(2i, 2i + 1)`` instead of ``(i, i + sum(sections))``.
+
+    Returns:
+        ``(query, key)`` turned, contiguous, in their own type; differentiable with respect to
+        both (not to the positions or frequencies).
+    """
+    N.require_cuda(query, key, positions, inv_freq)
+    query = _rows("query", query)
+    tokens, _, dim = query.shape
+    if query.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"query must be float32 or bfloat16, got {query.dtype}")
+    if key is not None:
+        key = _rows("key", key)
+        if key.shape[0] != tokens or key.shape[2] != dim or key.dtype != query.dtype:
+            raise ValueError("key must have the query's tokens, head_dim and type")
+    sections = tuple(int(n) for n in sections)
+    half = sum(sections)
+    if not 1 <= len(sections) <= 8 or min(sections) < 0 or half < 1 or 2 * half > dim:
+        raise ValueError(f"sections {sections} do not fit head_dim {dim}")
+    if positions.shape != (tokens, len(sections)):
+        raise ValueError(f"positions must be [{tokens}, {len(sections)}], got {list(positions.shape)}")
+    if positions.dtype == torch.int64:
+        positions = positions.to(torch.int32)
+    if positions.dtype not in (torch.float32, torch.int32):
+        raise ValueError(f"positions must be float32 or int32, got {positions.dtype}")
+    if inv_freq.shape != (half,) or inv_freq.dtype != torch.float32:
+        raise ValueError(f"inv_freq must be float32 [{half}]")
+    if positions.requires_grad or inv_freq.requires_grad:
+        raise ValueError("positions and inv_freq have no gradient")
+    if dim > 1024:
+        raise ValueError(f"head_dim must be at most 1024, got {dim}")
+    if interleaved and dim % 2:
+        raise ValueError("interleaved pairs need an even head_dim")
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        return AxialRotaryFunction.apply(query, key, positions, inv_freq, sections, bool(interleaved))
+    return rotary_launch(query, key, positions, inv_freq, sections, bool(interleaved), False)
