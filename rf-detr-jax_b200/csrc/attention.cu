@@ -102,180 +102,39 @@ __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kAttnWaitLimit));
 }
 
-// Zeroes rows [from, to) of a swizzled tile (whole warp; whole rows, so the swizzle does not matter).
+// Zeroes rows [from, to) of a swizzled tile by the first `threads` threads of a block or a warp's
+// lanes (32); whole rows, so the swizzle does not matter.
 template <int DP>
-__device__ __forceinline__ void zero_rows(uint32_t tile, int rows_in_panel, int from, int to) {
+__device__ __forceinline__ void zero_rows(uint32_t tile, int rows_in_panel, int from, int to, int threads) {
     constexpr int CH = Tile<DP>::kRowBytes / 16;
-    const int lane = threadIdx.x & 31;
     const int n = (to - from) * CH;
     for (int p = 0; p < Tile<DP>::kPanels; ++p) {
         const uint32_t a = tile + p * rows_in_panel * Tile<DP>::kRowBytes + from * Tile<DP>::kRowBytes;
-        for (int i = lane; i < n; i += 32)
+        for (int i = threadIdx.x & (threads - 1); i < n; i += threads)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + i * 16), "r"(0) : "memory");
     }
+}
+
+// Bytes that a box of `rows` tile rows brings (boxes past a tensor's end are filled up with zeros).
+template <int DP> __device__ __forceinline__ unsigned box_bytes(int rows) {
+    return rows * Tile<DP>::kRowBytes * Tile<DP>::kPanels;
 }
 
 // ---------------------------------------------------------------------------------------------
 // Forward.
 //
-// A block serves NT tiles of 128 rows (queries x packed heads) of one sequence and key head, and
-// walks its keys in tiles of 128: per tile S = Q K^T (both operands in shared memory) into TMEM, a
-// warpgroup per row tile turns it into P = exp2(scale log2(e) (S - m)) in registers, one row per
-// thread, and writes it back as bf16 over S; O += P V takes P from TMEM.  With two row tiles the
-// tensor core works on one while the other's exponentials run.  The reference m of a row is its
-// running maximum, but moves only when that grew by more than kLazy (in powers of two; P and its
-// sum stay below 2^kLazy times their true scale, far from any limit in float32, and bf16's relative
-// rounding does not depend on the scale), so that O in TMEM is seldom rescaled.
-// P is rounded to bf16 because that is what the tensor core takes; its row sum is kept in float32
-// from the unrounded values.
-// With few row tiles the keys are split over `splits` blocks; each writes its normalised part in
-// float32 and its lse, and attn_join_kernel adds them by weight.
+// A row tile is 128 rows (queries x packed heads) of one sequence and key head; keys come in tiles.
+// Per key tile S = Q K^T (both operands in shared memory) into TMEM; a warpgroup turns it into
+// P = exp2(scale log2(e) (S - m)) in registers, one row per thread, and writes it back as bf16 over
+// S; O += P V takes P from TMEM.  The reference m of a row is its running maximum, but moves only
+// when that grew by more than kLazy (in powers of two; P and its sum stay below 2^kLazy times their
+// true scale, far from any limit in float32, and bf16's relative rounding does not depend on the
+// scale), so that O in TMEM is seldom rescaled.  P is rounded to bf16 because that is what the
+// tensor core takes; its row sum is kept in float32 from the unrounded values.  The last tile of
+// the keys works on as many columns as are seen, in steps of 16, and warps whose rows are all past
+// the sequence do none of it.
 // ---------------------------------------------------------------------------------------------
 constexpr float kLazy = 8.0f;
-constexpr int kKeys = 128;  // keys in a tile
-
-template <int DP, int NT> struct FwdShape {
-    static constexpr int kTileBytes = 128 * DP * 2;
-    static constexpr int kStages = 4;
-    static constexpr int kThreads = NT * 128 + 64;
-    static constexpr int kTmem = NT * (128 + DP) <= 256 ? 256 : 512;
-    static constexpr size_t kSmem = 1024 + (size_t)(NT + kStages) * kTileBytes;
-};
-
-template <int NT> struct FwdShared {
-    uint64_t q_full[NT], kv_full[4], kv_raw, kv_empty[4], s_full[NT], p_ready[NT], o_done[NT], drain;
-    uint32_t tmem;
-    int abort;
-};
-
-struct FwdRange {
-    int n[2];       // key tiles of each row tile (end, exclusive)
-    int nmax;       // end over the row tiles
-    int j0;         // first key tile
-    int tok[2];     // tokens of each row tile
-};
-
-// Whole warp; returns how many tiles of K and V were asked for.
-template <int DP, int NT>
-__device__ int fwd_load(const AttnArgs &A, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
-                         FwdShared<NT> &sh, uint32_t smem_q, uint32_t smem_kv, const FwdRange &r, int kvh, int qhead,
-                         int qrow, int tok_per_tile, int krow, int klen) {
-    using S = FwdShape<DP, NT>;
-    using TL = Tile<DP>;
-    const int lane = threadIdx.x & 31;
-    volatile int *abort = &sh.abort;
-    if (r.nmax <= r.j0) return 0;
-    if (lane == 0) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (r.n[t] <= r.j0) continue;
-            mbar_arrive_expect_tx(&sh.q_full[t], tok_per_tile * A.pack * TL::kRowBytes * TL::kPanels);
-            for (int p = 0; p < TL::kPanels; ++p)
-                tma_load_3d(smem_q + t * S::kTileBytes + p * 128 * TL::kRowBytes, mq, &sh.q_full[t], p * TL::kCols,
-                            qhead, qrow + t * tok_per_tile);
-        }
-    }
-    const int loads = 2 * (r.nmax - r.j0);
-    int issued = 0;
-    unsigned raw_phase = 0;
-    for (; issued < loads; ++issued) {
-        const int st = issued % S::kStages;
-        if (issued >= S::kStages && !wait_warp(&sh.kv_empty[st], ((issued / S::kStages) - 1) & 1, abort)) break;
-        const int j = r.j0 + (issued >> 1);
-        const bool is_v = issued & 1;
-        // The last tile of V may reach into rows that are not this sequence's: P is 0 there, but
-        // 0 x inf is not, so they are cleared before the tensor core sees the tile.
-        const int foreign = is_v ? j * kKeys + kKeys - klen : 0;
-        const uint32_t dst = smem_kv + st * S::kTileBytes;
-        uint64_t *bar = foreign > 0 ? &sh.kv_raw : &sh.kv_full[st];
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive_expect_tx(bar, S::kTileBytes);
-            for (int p = 0; p < TL::kPanels; ++p)
-                tma_load_3d(dst + p * 128 * TL::kRowBytes, is_v ? mv : mk, bar, p * TL::kCols, kvh, krow + j * kKeys);
-        }
-        if (foreign > 0) {
-            if (!wait_warp(&sh.kv_raw, raw_phase, abort)) {
-                mbar_drain(&sh.kv_raw, raw_phase, kAttnWaitLimit);
-                break;
-            }
-            raw_phase ^= 1;
-            zero_rows<DP>(dst, 128, kKeys - foreign, kKeys);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.kv_full[st]);
-        }
-    }
-    return issued;
-}
-
-// After a wait gave up: every copy of this block that may still be landing.
-template <int DP, int NT> __device__ void fwd_drain(FwdShared<NT> &sh, const FwdRange &r, int issued) {
-    using S = FwdShape<DP, NT>;
-    for (int t = 0; t < NT; ++t)
-        if (r.n[t] > r.j0) mbar_drain(&sh.q_full[t], 0, kAttnWaitLimit);
-    for (int i = max(0, issued - S::kStages); i < issued; ++i)
-        mbar_drain(&sh.kv_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
-}
-
-// One thread.
-template <int DP, int NT>
-__device__ bool fwd_mma_loop(FwdShared<NT> &sh, uint32_t smem_q, uint32_t smem_kv, const FwdRange &r, uint32_t tmem) {
-    using S = FwdShape<DP, NT>;
-    using TL = Tile<DP>;
-    constexpr uint32_t kIdS = mma_idesc(128, kKeys, false), kIdO = mma_idesc(128, DP, true);
-    constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
-    volatile int *abort = &sh.abort;
-    auto scores = [&](int t, int st) {
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t o = (k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes;
-            mma_ss(tmem + t * 128, smem_desc<TL::kRowBytes>(smem_q + t * S::kTileBytes + o, 16, kSbo),
-                   smem_desc<TL::kRowBytes>(smem_kv + st * S::kTileBytes + o, 16, kSbo), kIdS, k > 0);
-        }
-        tc_commit(&sh.s_full[t]);
-    };
-    auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
-        return wait_one(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
-    };
-    const int n = r.nmax - r.j0;
-    int st = kv(0);
-    if (st < 0) return false;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (r.n[t] <= r.j0) continue;
-        if (!wait_one(&sh.q_full[t], 0, abort)) return false;
-        tc_fence_after();
-        scores(t, st);
-    }
-    tc_commit(&sh.kv_empty[st]);
-    for (int i = 0; i < n; ++i) {
-        int sv = -1, sk = -1;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
-            if (left > 0) {
-                if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
-                if (!wait_one(&sh.p_ready[t], i & 1, abort)) return false;
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(tmem + NT * 128 + t * DP, tmem + t * 128 + k * 8,
-                           smem_desc<TL::kRowBytes>(smem_kv + sv * S::kTileBytes + k * 16 * TL::kRowBytes, kLbo, kSbo),
-                           kIdO, i > 0 || k > 0);
-                tc_commit(&sh.o_done[t]);
-            }
-            if (left > 1) {
-                if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
-                tc_fence_after();
-                scores(t, sk);
-            }
-        }
-        if (sv >= 0) tc_commit(&sh.kv_empty[sv]);
-        if (sk >= 0) tc_commit(&sh.kv_empty[sk]);
-    }
-    return true;
-}
 
 // The largest of m and 32 values.
 __device__ __forceinline__ float max32(const float *s, float m) {
@@ -288,103 +147,88 @@ __device__ __forceinline__ float max32(const float *s, float m) {
     return fmaxf(a, b);
 }
 
-// A warpgroup: the rows of row tile t.
-template <int DP, int NT, bool SPLIT>
-__device__ void fwd_softmax(const AttnArgs &A, FwdShared<NT> &sh, const FwdRange &r, int t, uint32_t tmem, int row,
-                            int tok_first, int qlen, int klen, int qbase, int qhead, bf16 *out, float *lse, float *part,
-                            float *part_lse) {
-    volatile int *abort = &sh.abort;
-    const uint32_t lane_base = (uint32_t)((threadIdx.x >> 5) & 3) << 21;  // lane 32 (w % 4)
-    const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + NT * 128 + t * DP;
-    const int tok = tok_first + row / A.pack;
-    const int head = qhead + row % A.pack;
-    const bool live = row / A.pack < r.tok[t];
-    const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - qlen)) : klen;
-    // Keys that every row of the tile sees (rows past the last token do not count).
-    const int all_see = A.causal ? min(klen, tok_first + 1 + klen - qlen) : klen;
-    const float sc = A.scale_log2;
-    float m = -INFINITY, sum = 0.0f;
-    const int n = r.n[t] - r.j0;
-    for (int i = 0; i < n; ++i) {
-        if (!wait_warp(&sh.s_full[t], i & 1, abort)) return;
-        tc_fence_after();
-        float s[128];
+// A row's softmax so far: P and sum are relative to exp2(m scale log2(e)).
+struct RowState {
+    float m, sum;
+};
+
+// Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P in place; `to` is O, which
+// must hold the products of all tiles before.  `cols` columns are in use, of which this row sees
+// `seen` where `mask` is set.
+template <int DP, int KEYS>
+__device__ __forceinline__ void softmax_tile(RowState &r, uint32_t ts, uint32_t to, int cols, bool mask, int seen,
+                                             bool first, float sc) {
+    constexpr int NC = KEYS / 32;
+    float s[KEYS];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
-        tmem_wait_ld();
-        pin<128>(s);
-        const int k0 = (r.j0 + i) * kKeys;
-        if (k0 + kKeys > all_see) {
-            const int seen = limit - k0;
+    for (int c = 0; c < NC; ++c)
+        if (c * 32 < cols) tmem_ld32(ts + c * 32, s + c * 32);
+    tmem_wait_ld();
+    pin<KEYS>(s);
+    if (mask) {
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx = max32(s + c * 32, mx);
-        if (i == 0) {
-            m = mx;
-        } else {
-            const bool grown = mx * sc > m * sc + kLazy;
-            if (__any_sync(0xffffffffu, grown)) {
-                // O must hold the products of every tile before this one.
-                if (!wait_warp(&sh.o_done[t], (i - 1) & 1, abort)) return;
-                tc_fence_after();
-                const float to_m = fmaxf(m, mx);
-                const float f = to_m == -INFINITY ? 1.0f : exp2_fast((m - to_m) * sc);
-                m = to_m;
-                sum *= f;
-#pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    float o[32];
-                    tmem_ld32(to + c * 32, o);
-                    tmem_wait_ld();
-                    pin<32>(o);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= f;
-                    tmem_st32(to + c * 32, reinterpret_cast<uint32_t *>(o));
-                }
-            }
-        }
-        const float ref = m == -INFINITY ? 0.0f : -m * sc;
-        const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
-        float2 acc = make_float2(0.0f, 0.0f), acc1 = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                float2 x = fma2(make_float2(s[h * 64 + 2 * c], s[h * 64 + 2 * c + 1]), sc2, ref2);
-                x.x = exp2_fast(x.x);
-                x.y = exp2_fast(x.y);
-                if (c & 1) acc1 = add2(acc1, x);
-                else acc = add2(acc, x);
-                p[c] = pack_bf16(x.x, x.y);
-            }
-            tmem_st32(ts + h * 32, p);
-        }
-        sum += (acc.x + acc.y) + (acc1.x + acc1.y);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_ready[t]);
+        for (int c = 0; c < KEYS; ++c) s[c] = c < seen ? s[c] : -INFINITY;
     }
-    const size_t token = (size_t)qbase + tok;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float l = sum == 0.0f ? -INFINITY : m * A.scale + logf(sum);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+        if (c * 32 < cols) mx = max32(s + c * 32, mx);
+    if (first) {
+        r.m = mx;
+    } else if (__any_sync(0xffffffffu, mx * sc > r.m * sc + kLazy)) {
+        const float to_m = fmaxf(r.m, mx);
+        const float f = to_m == -INFINITY ? 1.0f : exp2_fast((r.m - to_m) * sc);
+        r.m = to_m;
+        r.sum *= f;
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+            float o[32];
+            tmem_ld32(to + c * 32, o);
+            tmem_wait_ld();
+            pin<32>(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tmem_st32(to + c * 32, reinterpret_cast<uint32_t *>(o));
+        }
+    }
+    const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
+    const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
+    float2 acc = make_float2(0.0f, 0.0f), acc1 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int h = 0; h < NC; ++h) {
+        if (h * 32 >= cols) break;
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            float2 x = fma2(make_float2(s[h * 32 + 2 * c], s[h * 32 + 2 * c + 1]), sc2, ref2);
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
+            if (c & 1) acc1 = add2(acc1, x);
+            else acc = add2(acc, x);
+            p[c] = pack_bf16(x.x, x.y);
+        }
+        tmem_st16(ts + h * 16, p);
+    }
+    r.sum += (acc.x + acc.y) + (acc1.x + acc1.y);
+    tmem_wait_st();
+}
+
+// Whole warp: a row's result from O (or zeros) and its log-sum-exp.
+template <int DP, bool SPLIT>
+__device__ __forceinline__ void write_row(const AttnArgs &A, const RowState &r, uint32_t to, bool any, bool live,
+                                          size_t token, int head, bf16 *out, float *lse, float *part,
+                                          float *part_lse) {
+    const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
     if (live) {
+        const float l = r.sum == 0.0f ? -INFINITY : r.m * A.scale + logf(r.sum);
         if (SPLIT) part_lse[(size_t)head * A.Tq + token] = l;
         else if (lse) lse[(size_t)head * A.Tq + token] = l;
-    }
-    if (n > 0) {
-        if (!wait_warp(&sh.o_done[t], (n - 1) & 1, abort)) return;
-        tc_fence_after();
     }
     const size_t at = (token * A.Hq + head) * A.D;
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c) {
         float o[32];
-        if (n > 0) {
+        if (any) {
             tmem_ld32(to + c * 32, o);
             tmem_wait_ld();
             pin<32>(o);
@@ -414,35 +258,197 @@ __device__ void fwd_softmax(const AttnArgs &A, FwdShared<NT> &sh, const FwdRange
     }
 }
 
-template <int DP, int NT, bool SPLIT>
-__global__ void __launch_bounds__(FwdShape<DP, NT>::kThreads, 1)
-attn_forward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                    const __grid_constant__ CUtensorMap mv, bf16 *__restrict__ out, float *__restrict__ lse,
-                    float *__restrict__ part, float *__restrict__ part_lse, int slots) {
-    using S = FwdShape<DP, NT>;
+// Columns of a key tile that a row tile works on.
+__device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return min(keys, (sees - k0 + 15) & ~15); }
+
+// ---- long sequences: two row tiles to a block, roles by warp -------------------------------------
+// One warp loads, one thread issues the matrix products, a warpgroup serves each row tile: while the
+// tensor core works on one tile, the other's exponentials run, and K and V are read from L2 once
+// for 256 rows.  128 keys a tile.  The warpgroups take their registers from the other two warps
+// (setmaxnreg): a row of S is 128 values.
+// With few row tiles the keys are split over blocks (SPLIT): each writes its normalised part in
+// float32 and its lse, and attn_join_kernel adds them by weight.
+template <int DP> struct LongShape {
+    static constexpr int kKeys = 128;
+    static constexpr int kTileBytes = 128 * DP * 2;
+    static constexpr int kStages = 4;
+    static constexpr int kThreads = 384;
+    static constexpr int kTmem = 512;
+    static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
+};
+// Registers at launch: 65536 / 384 -> 168; 2 x 208 + 88 = 3 x 168.
+constexpr int kLaunchRegs = 168, kMoreRegs = 208, kLessRegs = 88;
+static_assert(2 * kMoreRegs + kLessRegs <= 3 * kLaunchRegs, "a warpgroup would wait for registers for good");
+
+struct LongShared {
+    uint64_t q_full[2], kv_full[4], kv_raw, kv_empty[4], s_full[2], p_ready[2], o_done[2], drain;
+    uint32_t tmem;
+    int abort;
+};
+
+struct LongRange {
+    int sees[2];    // keys that each row tile works on, from key j0 * 128 on
+    int n[2];       // key tiles of each row tile (end, exclusive)
+    int nmax;       // end over the row tiles
+    int j0;         // first key tile
+    int tok[2];     // tokens of each row tile
+};
+
+// Whole warp; returns how many tiles of K and V were asked for.
+template <int DP>
+__device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
+                         LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, int kvh, int qhead,
+                         int qrow, int tok_per_tile, int krow, int klen) {
+    using S = LongShape<DP>;
+    using TL = Tile<DP>;
+    const int lane = threadIdx.x & 31;
+    volatile int *abort = &sh.abort;
+    if (r.nmax <= r.j0) return 0;
+    const int loads = 2 * (r.nmax - r.j0);
+    int issued = 0;
+    unsigned raw_phase = 0;
+    for (; issued < loads; ++issued) {
+        const int st = issued % S::kStages;
+        if (issued >= S::kStages && !wait_warp(&sh.kv_empty[st], ((issued / S::kStages) - 1) & 1, abort)) break;
+        const int j = r.j0 + (issued >> 1);
+        const bool is_v = issued & 1;
+        // The last tile of V may reach into rows that are not this sequence's: P is 0 there, but
+        // 0 x inf is not, so they are cleared before the tensor core sees the tile.
+        const int foreign = is_v ? (j + 1) * S::kKeys - klen : 0;
+        const uint32_t dst = smem_kv + st * S::kTileBytes;
+        uint64_t *bar = foreign > 0 ? &sh.kv_raw : &sh.kv_full[st];
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar, S::kTileBytes);
+            for (int p = 0; p < TL::kPanels; ++p)
+                tma_load_3d(dst + p * 128 * TL::kRowBytes, is_v ? mv : mk, bar, p * TL::kCols, kvh,
+                            krow + j * S::kKeys);
+            if (issued == 0) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (r.n[t] <= r.j0) continue;
+                    mbar_arrive_expect_tx(&sh.q_full[t], box_bytes<DP>(tok_per_tile * A.pack));
+                    for (int p = 0; p < TL::kPanels; ++p)
+                        tma_load_3d(smem_q + t * S::kTileBytes + p * 128 * TL::kRowBytes, mq, &sh.q_full[t],
+                                    p * TL::kCols, qhead, qrow + t * tok_per_tile);
+                }
+            }
+        }
+        if (foreign > 0) {
+            if (!wait_warp(&sh.kv_raw, raw_phase, abort)) {
+                mbar_drain(&sh.kv_raw, raw_phase, kAttnWaitLimit);
+                break;
+            }
+            raw_phase ^= 1;
+            zero_rows<DP>(dst, 128, S::kKeys - foreign, S::kKeys, 32);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+        }
+    }
+    return issued;
+}
+
+// After a wait gave up: every copy of this block that may still be landing.
+template <int DP> __device__ void long_drain(LongShared &sh, const LongRange &r, int issued) {
+    using S = LongShape<DP>;
+    for (int t = 0; t < 2; ++t)
+        if (r.n[t] > r.j0) mbar_drain(&sh.q_full[t], 0, kAttnWaitLimit);
+    for (int i = max(0, issued - S::kStages); i < issued; ++i)
+        mbar_drain(&sh.kv_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
+}
+
+// One thread.
+template <int DP>
+__device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, uint32_t tmem) {
+    using S = LongShape<DP>;
+    using TL = Tile<DP>;
+    constexpr uint32_t kIdO = mma_idesc(128, DP, true);
+    constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
+    volatile int *abort = &sh.abort;
+    auto scores = [&](int t, int st, int j) {
+        const uint32_t id = mma_idesc(128, tile_cols(r.sees[t], j * S::kKeys, S::kKeys), false);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t o = (k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes;
+            mma_ss(tmem + t * 128, smem_desc<TL::kRowBytes>(smem_q + t * S::kTileBytes + o, 16, kSbo),
+                   smem_desc<TL::kRowBytes>(smem_kv + st * S::kTileBytes + o, 16, kSbo), id, k > 0);
+        }
+        tc_commit(&sh.s_full[t]);
+    };
+    auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
+        return wait_one(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
+    };
+    const int n = r.nmax - r.j0;
+    int st = kv(0);
+    if (st < 0) return false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (r.n[t] <= r.j0) continue;
+        if (!wait_one(&sh.q_full[t], 0, abort)) return false;
+        tc_fence_after();
+        scores(t, st, r.j0);
+    }
+    tc_commit(&sh.kv_empty[st]);
+    for (int i = 0; i < n; ++i) {
+        int sv = -1, sk = -1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
+            if (left > 0) {
+                if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
+                if (!wait_one(&sh.p_ready[t], i & 1, abort)) return false;
+                tc_fence_after();
+                const int steps = tile_cols(r.sees[t], (r.j0 + i) * S::kKeys, S::kKeys) / 16;
+                for (int k = 0; k < steps; ++k)
+                    mma_ts(tmem + 256 + t * DP, tmem + t * 128 + k * 8,
+                           smem_desc<TL::kRowBytes>(smem_kv + sv * S::kTileBytes + k * 16 * TL::kRowBytes, kLbo, kSbo),
+                           kIdO, i > 0 || k > 0);
+                if (left == 1) tc_commit(&sh.o_done[t]);
+            }
+            if (left > 1) {
+                if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
+                tc_fence_after();
+                // In issue order after the product above, so its commit tells of that product too.
+                scores(t, sk, r.j0 + i + 1);
+            }
+        }
+        if (sv >= 0) tc_commit(&sh.kv_empty[sv]);
+        if (sk >= 0) tc_commit(&sh.kv_empty[sk]);
+    }
+    return true;
+}
+
+template <int DP, bool SPLIT>
+__global__ void __launch_bounds__(LongShape<DP>::kThreads, 1)
+attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
+                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                         bf16 *__restrict__ out, float *__restrict__ lse, float *__restrict__ part,
+                         float *__restrict__ part_lse, int slots) {
+    using S = LongShape<DP>;
     extern __shared__ unsigned char dyn[];
-    __shared__ FwdShared<NT> sh;
+    __shared__ LongShared sh;
     const int warp = threadIdx.x >> 5;
     const int heads = A.Hkv * A.subs;
     const int hx = blockIdx.x % heads;
     // Later slots first: under a causal mask they see more keys.
     const int slot = slots - 1 - (int)(blockIdx.x / heads);
     const int per = 128 / A.pack;  // tokens in a row tile
-    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per * NT, slot);
+    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per * 2, slot);
     if (q.first >= q.len) return;
     int kbase, klen;
     seq_range(A.k_off, A.n_seq, A.Tk, q.seq, kbase, klen);
     const int kvh = hx / A.subs;
     const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
 
-    FwdRange r;
+    LongRange r;
     r.nmax = 0;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < 2; ++t) {
         r.tok[t] = min(per, max(0, q.len - q.first - t * per));
         const int last = q.first + t * per + r.tok[t] - 1;
-        const int sees = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
-        r.n[t] = (sees + kKeys - 1) / kKeys;
+        r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
+        r.n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
         r.nmax = max(r.nmax, r.n[t]);
     }
     r.j0 = 0;
@@ -450,15 +456,15 @@ attn_forward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq, co
         const int each = (r.nmax + (int)gridDim.z - 1) / (int)gridDim.z;
         r.j0 = min(r.nmax, each * (int)blockIdx.z);
         const int end = min(r.nmax, r.j0 + each);
-        for (int t = 0; t < NT; ++t) r.n[t] = max(r.j0, min(r.n[t], end));
+        for (int t = 0; t < 2; ++t) r.n[t] = max(r.j0, min(r.n[t], end));
         r.nmax = end;
         part += (size_t)blockIdx.z * A.Tq * A.Hq * A.D;
         part_lse += (size_t)blockIdx.z * A.Tq * A.Hq;
     }
 
-    if (warp == NT * 4) {
+    if (warp == 8) {
         if ((threadIdx.x & 31) == 0) {
-            for (int t = 0; t < NT; ++t) {
+            for (int t = 0; t < 2; ++t) {
                 mbar_init(&sh.q_full[t], 1);
                 mbar_init(&sh.s_full[t], 1);
                 mbar_init(&sh.p_ready[t], 4);
@@ -481,26 +487,242 @@ attn_forward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq, co
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     const uint32_t smem_q = (smem_u32(dyn) + 1023u) & ~1023u;
-    const uint32_t smem_kv = smem_q + NT * S::kTileBytes;
+    const uint32_t smem_kv = smem_q + 2 * S::kTileBytes;
 
     int issued = 0;
-    if (warp == NT * 4) {
-        if ((threadIdx.x & 31) == 0 && r.nmax > r.j0) fwd_mma_loop<DP, NT>(sh, smem_q, smem_kv, r, tmem);
-    } else if (warp == NT * 4 + 1) {
-        issued = fwd_load<DP, NT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
-                                  klen);
+    if (warp >= 8) {
+        regs_less<kLessRegs>();
+        if (warp == 8) {
+            if ((threadIdx.x & 31) == 0 && r.nmax > r.j0) long_mma_loop<DP>(sh, smem_q, smem_kv, r, tmem);
+        } else if (warp == 9) {
+            issued = long_load<DP>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
+                                   klen);
+        }
     } else {
+        regs_more<kMoreRegs>();
         const int t = warp >> 2;
-        if (r.tok[t] > 0)
-            fwd_softmax<DP, NT, SPLIT>(A, sh, r, t, tmem, threadIdx.x & 127, q.first + t * per, q.len, klen, q.base,
-                                       qhead, out, lse, part, part_lse);
+        if (r.tok[t] > 0) {
+            volatile int *abort = &sh.abort;
+            const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lane 32 (w % 4)
+            const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + 256 + t * DP;
+            const int row = threadIdx.x & 127;
+            const int tok_first = q.first + t * per, tok = tok_first + row / A.pack;
+            const bool live = row / A.pack < r.tok[t];
+            const bool warp_live = (row & ~31) < r.tok[t] * A.pack;
+            const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
+            // Keys that every row of the tile sees (rows past the last token do not count).
+            const int all_see = A.causal ? min(klen, tok_first + 1 + klen - q.len) : klen;
+            RowState rs{-INFINITY, 0.0f};
+            const int n = r.n[t] - r.j0;
+            bool ok = true;
+            for (int i = 0; i < n && ok; ++i) {
+                ok = wait_warp(&sh.s_full[t], i & 1, abort);
+                if (!ok) break;
+                tc_fence_after();
+                const int k0 = (r.j0 + i) * S::kKeys;
+                if (warp_live)
+                    softmax_tile<DP, S::kKeys>(rs, ts, to, tile_cols(r.sees[t], k0, S::kKeys), k0 + S::kKeys > all_see,
+                                               limit - k0, i == 0, A.scale_log2);
+                tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_ready[t]);
+            }
+            if (ok && n > 0) ok = wait_warp(&sh.o_done[t], 0, abort);
+            tc_fence_after();
+            if (ok)
+                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row % A.pack, out, lse, part,
+                                     part_lse);
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sh.abort && warp == NT * 4 + 1 && (threadIdx.x & 31) == 0) fwd_drain<DP, NT>(sh, r, issued);
-    if (warp == NT * 4) {
+    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0) long_drain<DP>(sh, r, issued);
+    if (warp == 8) {
         if (sh.abort && (threadIdx.x & 31) == 0) {
+            tc_commit(&sh.drain);
+            mbar_drain(&sh.drain, 0, kAttnWaitLimit);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+// ---- short sequences: one row tile to a block, several blocks to an SM ---------------------------
+// With a few key tiles to a block, most of its time would be its start and its end; four blocks to
+// an SM (two with 128 channels) cover each other's instead of roles within one.  128 threads: each
+// owns a row, thread 0 also issues the copies and the products.  64 keys a tile, so that S and O of
+// four blocks fit TMEM and a row of S is 64 registers.
+template <int DP> struct ShortShape {
+    static constexpr int kKeys = 64;
+    static constexpr int kQBytes = 128 * DP * 2;
+    static constexpr int kTileBytes = kKeys * DP * 2;
+    static constexpr int kTmem = DP <= 64 ? 128 : 256;  // S 64, O DP
+    static constexpr int kBlocks = DP <= 64 ? 4 : 2;
+    static constexpr size_t kSmem = 1024 + kQBytes + 4 * (size_t)kTileBytes;
+};
+
+struct ShortShared {
+    uint64_t k_full[2], v_full[2], s_full, o_done, drain;
+    uint32_t tmem;
+    int abort;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(128, ShortShape<DP>::kBlocks)
+attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
+                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                          bf16 *__restrict__ out, float *__restrict__ lse, int slots) {
+    using S = ShortShape<DP>;
+    using TL = Tile<DP>;
+    constexpr int KEYS = S::kKeys;
+    constexpr uint32_t kIdO = mma_idesc(128, DP, true);
+    constexpr uint32_t kSbo = 8 * TL::kRowBytes, kQPanel = 128 * TL::kRowBytes, kPanel = KEYS * TL::kRowBytes;
+    extern __shared__ unsigned char dyn[];
+    __shared__ ShortShared sh;
+    const int warp = threadIdx.x >> 5;
+    const int heads = A.Hkv * A.subs;
+    const int hx = blockIdx.x % heads;
+    const int slot = slots - 1 - (int)(blockIdx.x / heads);
+    const int per = 128 / A.pack;
+    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per, slot);
+    if (q.first >= q.len) return;
+    int kbase, klen;
+    seq_range(A.k_off, A.n_seq, A.Tk, q.seq, kbase, klen);
+    const int kvh = hx / A.subs;
+    const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+    const int ntok = min(per, q.len - q.first);
+    const int sees = A.causal ? min(klen, max(0, q.first + ntok + klen - q.len)) : klen;
+    const int n = (sees + KEYS - 1) / KEYS;
+    const bool boss = threadIdx.x == 0;
+
+    if (warp == 0) {
+        if (boss) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh.k_full[i], 1);
+                mbar_init(&sh.v_full[i], 1);
+            }
+            mbar_init(&sh.s_full, 1);
+            mbar_init(&sh.o_done, 1);
+            mbar_init(&sh.drain, 1);
+            sh.abort = 0;
+            mbar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&sh.tmem, S::kTmem);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const uint32_t smem_q = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t smem_k = smem_q + S::kQBytes, smem_v = smem_k + 2 * S::kTileBytes;
+    volatile int *abort = &sh.abort;
+
+    auto load = [&](const CUtensorMap *map, uint64_t *bar, uint32_t dst, int j) {
+        for (int p = 0; p < TL::kPanels; ++p)
+            tma_load_3d(dst + p * kPanel, map, bar, p * TL::kCols, kvh, kbase + j * KEYS);
+    };
+    auto load_k = [&](int j, unsigned more) {
+        mbar_arrive_expect_tx(&sh.k_full[j & 1], S::kTileBytes + more);
+        load(&mk, &sh.k_full[j & 1], smem_k + (j & 1) * S::kTileBytes, j);
+    };
+    auto load_v = [&](int j) {
+        mbar_arrive_expect_tx(&sh.v_full[j & 1], S::kTileBytes);
+        load(&mv, &sh.v_full[j & 1], smem_v + (j & 1) * S::kTileBytes, j);
+    };
+    auto scores = [&](int j) {
+        if (!wait_one(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t id = mma_idesc(128, tile_cols(sees, j * KEYS, KEYS), false);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
+            mma_ss(tmem, smem_desc<TL::kRowBytes>(smem_q + panel * kQPanel + in, 16, kSbo),
+                   smem_desc<TL::kRowBytes>(smem_k + (j & 1) * S::kTileBytes + panel * kPanel + in, 16, kSbo), id,
+                   k > 0);
+        }
+        tc_commit(&sh.s_full);
+        return true;
+    };
+    int k_issued = 0, v_issued = 0;  // thread 0
+    bool ok = true;
+    if (boss && n > 0) {
+        load_k(0, box_bytes<DP>(per * A.pack));
+        for (int p = 0; p < TL::kPanels; ++p)
+            tma_load_3d(smem_q + p * kQPanel, &mq, &sh.k_full[0], p * TL::kCols, qhead, q.base + q.first);
+        load_v(0);
+        k_issued = v_issued = 1;
+        if (n > 1) {
+            load_k(1, 0);
+            k_issued = 2;
+        }
+        ok = scores(0);
+    }
+
+    const uint32_t ts = tmem + ((uint32_t)warp << 21), to = ts + KEYS;
+    const int row = threadIdx.x;
+    const int tok = q.first + row / A.pack;
+    const bool live = row / A.pack < ntok;
+    const bool warp_live = (row & ~31) < ntok * A.pack;
+    const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
+    const int all_see = A.causal ? min(klen, q.first + 1 + klen - q.len) : klen;
+    RowState rs{-INFINITY, 0.0f};
+    bool gave_up = false;
+    for (int i = 0; i < n; ++i) {
+        ok = wait_warp(&sh.s_full, i & 1, abort) && ok;
+        tc_fence_after();
+        // S of tile i is done, and with it (in issue order) P V of tile i - 1: K's buffer of tile i and
+        // V's of tile i - 1 are free.
+        if (boss && ok) {
+            if (i + 2 < n) load_k(i + 2, 0), ++k_issued;
+            if (i + 1 < n) load_v(i + 1), ++v_issued;
+        }
+        __syncwarp();
+        const int k0 = i * KEYS;
+        if (warp_live)
+            softmax_tile<DP, KEYS>(rs, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS > all_see, limit - k0, i == 0,
+                                   A.scale_log2);
+        // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
+        if (k0 + KEYS > klen) {
+            ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort) && ok;
+            zero_rows<DP>(smem_v + (i & 1) * S::kTileBytes, KEYS, klen - k0, KEYS, 128);
+            fence_async_smem();
+        }
+        tc_fence_before();
+        gave_up = __syncthreads_or(!ok);
+        if (gave_up) break;
+        if (boss) {
+            tc_fence_after();
+            ok = wait_one(&sh.v_full[i & 1], (i >> 1) & 1, abort);
+            const int steps = tile_cols(sees, k0, KEYS) / 16;
+            for (int k = 0; k < steps && ok; ++k)
+                mma_ts(tmem + KEYS, tmem + k * 8,
+                       smem_desc<TL::kRowBytes>(smem_v + (i & 1) * S::kTileBytes + k * 16 * TL::kRowBytes, kPanel,
+                                                kSbo),
+                       kIdO, i > 0 || k > 0);
+            if (i + 1 < n) ok = ok && scores(i + 1);
+            else tc_commit(&sh.o_done);
+        }
+        __syncwarp();
+    }
+    if (!gave_up) {
+        if (n > 0) ok = wait_warp(&sh.o_done, 0, abort);
+        tc_fence_after();
+        if (ok)
+            write_row<DP, false>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row % A.pack, out, lse, nullptr,
+                                 nullptr);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (boss && sh.abort) {
+            for (int i = max(0, k_issued - 2); i < k_issued; ++i)
+                mbar_drain(&sh.k_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
+            for (int i = max(0, v_issued - 2); i < v_issued; ++i)
+                mbar_drain(&sh.v_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
             tc_commit(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
         }
@@ -606,7 +828,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
     if (r.steps == 0) return 0;
     const int xrows = DKV ? 128 : (128 / A.pack) * A.pack;
     if (lane == 0) {
-        mbar_arrive_expect_tx(&sh.x_full, 2 * xrows * TL::kRowBytes * TL::kPanels);
+        mbar_arrive_expect_tx(&sh.x_full, 2 * box_bytes<DP>(xrows));
         const int head = DKV ? r.kvh : r.qhead, at = DKV ? r.kbase + r.k0 : r.qbase + r.q0;
         for (int p = 0; p < TL::kPanels; ++p) {
             const uint32_t o = p * 128 * TL::kRowBytes;
@@ -631,7 +853,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
         const uint32_t y0 = smem_y + st * 2 * S::kYBytes, y1 = y0 + S::kYBytes;
         __syncwarp();
         if (lane == 0) {
-            mbar_expect_tx(bar, 2 * yrows * TL::kRowBytes * TL::kPanels);
+            mbar_expect_tx(bar, 2 * box_bytes<DP>(yrows));
             for (int p = 0; p < TL::kPanels; ++p) {
                 const uint32_t o = p * kWalk * TL::kRowBytes;
                 tma_load_3d(y0 + o, my0, bar, p * TL::kCols, head, base + at);
@@ -662,8 +884,8 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 break;
             }
             raw_phase ^= 1;
-            zero_rows<DP>(y0, kWalk, good, yrows);
-            zero_rows<DP>(y1, kWalk, good, yrows);
+            zero_rows<DP>(y0, kWalk, good, yrows, 32);
+            zero_rows<DP>(y1, kWalk, good, yrows, 32);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.y_full[st]);
@@ -1062,41 +1284,72 @@ int check_tensor(const Strided &t, int64_t T, int64_t H) {
     return RFDETR_OK;
 }
 
-// Row tiles per block: one where the sequences are short enough (by their mean) that a second
-// tile would mostly be empty.
-int row_tiles(int64_t n_seq, int64_t Tq, int per) { (void)n_seq, (void)Tq, (void)per; return 2; }
+// Which forward kernel, and over how many blocks each row tile's keys are split.
+struct ForwardPlan {
+    bool is_short;
+    int splits;
+};
 
-// Blocks over which each row tile's keys are split.
-int key_splits(int64_t n_seq, int64_t Tq, int64_t Tk, long long tiles_per_row, int per, int nt) {
-    (void)n_seq, (void)Tq, (void)Tk, (void)tiles_per_row, (void)per, (void)nt;
-    return 1;
+ForwardPlan plan_forward(const AttnArgs &A) {
+    ForwardPlan p{false, 1};
+    const int per = 128 / A.pack;
+    const long long heads = (long long)A.Hkv * A.subs;
+    const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
+    const long long rows = A.Tq / n_seq, keys = A.Tk / n_seq;  // of the mean sequence
+    // Blocks of two row tiles, if every sequence were the mean one.
+    const long long blocks = heads * n_seq * ((rows + 2 * per - 1) / (2 * per));
+    const long long tiles = (keys + 127) / 128;
+    const KnobValue forced = knob(kKnobAttnFwd);
+    if (forced.count > 0 && forced.v[0] > 0) {
+        p.is_short = forced.v[0] == 2;
+        p.splits = p.is_short || forced.v[1] < 1 ? 1 : forced.v[1] > 64 ? 64 : forced.v[1];
+        return p;
+    }
+    if (blocks * 2 <= num_sms() && tiles >= 8) {
+        long long s = num_sms() / (blocks > 0 ? blocks : 1);
+        if (s > tiles / 4) s = tiles / 4;
+        p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+        return p;
+    }
+    p.is_short = rows <= 4 * per && keys <= 512;
+    return p;
 }
 
-template <int DP, int NT>
-int launch_forward(const AttnArgs &A, const Strided &q, const Strided &k, const Strided &v, bf16 *out, float *lse,
-                   float *part, float *part_lse, int splits, cudaStream_t stream) {
-    using S = FwdShape<DP, NT>;
-    const int per = 128 / A.pack;
+size_t split_bytes(const AttnArgs &A, int splits) {
+    return splits <= 1 ? 0 : (size_t)splits * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
+}
+
+template <int DP>
+int launch_forward(const AttnArgs &A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
+                   bf16 *out, float *lse, float *part, float *part_lse, cudaStream_t stream) {
+    const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP>::kKeys;
     CUtensorMap mq, mk, mv;
-    if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
-        !make_map(&mv, v, A.Tk, A.Hkv, A.D, 1, 128, q.p))
+    if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, keys, q.p) ||
+        !make_map(&mv, v, A.Tk, A.Hkv, A.D, 1, keys, q.p))
         return RFDETR_ERR_CUDA;
-    const long long slots = slots_for(A.Tq, per * NT, A.n_seq);
+    const long long slots = slots_for(A.Tq, plan.is_short ? per : per * 2, A.n_seq);
     const long long blocks = slots * A.Hkv * A.subs;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    const dim3 grid((unsigned)blocks, 1, (unsigned)splits);
-    if (splits > 1) {
-        if (int st = allow_smem(attn_forward_kernel<DP, NT, true>, S::kSmem)) return st;
-        attn_forward_kernel<DP, NT, true>
+    const dim3 grid((unsigned)blocks, 1, (unsigned)plan.splits);
+    if (plan.is_short) {
+        using S = ShortShape<DP>;
+        if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
+        attn_forward_short_kernel<DP><<<grid, 128, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, (int)slots);
+        return launch_status();
+    }
+    using S = LongShape<DP>;
+    if (plan.splits > 1) {
+        if (int st = allow_smem(attn_forward_long_kernel<DP, true>, S::kSmem)) return st;
+        attn_forward_long_kernel<DP, true>
             <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
         if (int st = launch_status()) return st;
         const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
         if ((n + 255) / 256 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-        attn_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(part, part_lse, splits, rows, A.Hq, A.Tq, A.D,
-                                                                         out, lse);
+        attn_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(part, part_lse, plan.splits, rows, A.Hq, A.Tq,
+                                                                         A.D, out, lse);
     } else {
-        if (int st = allow_smem(attn_forward_kernel<DP, NT, false>, S::kSmem)) return st;
-        attn_forward_kernel<DP, NT, false>
+        if (int st = allow_smem(attn_forward_long_kernel<DP, false>, S::kSmem)) return st;
+        attn_forward_long_kernel<DP, false>
             <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
     }
     return launch_status();
@@ -1152,21 +1405,6 @@ AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, in
     return A;
 }
 
-struct ForwardPlan {
-    int nt, splits;
-};
-ForwardPlan plan_forward(const AttnArgs &A) {
-    const int per = 128 / A.pack;
-    ForwardPlan p;
-    p.nt = row_tiles(A.n_seq, A.Tq, per);
-    p.splits = key_splits(A.n_seq, A.Tq, A.Tk, (long long)A.Hkv * A.subs, per, p.nt);
-    return p;
-}
-
-size_t split_bytes(const AttnArgs &A, int splits) {
-    return splits <= 1 ? 0 : (size_t)splits * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
-}
-
 }  // namespace
 
 // Reads and clears this file's device fault word; bits are those of mbar_wait / mbar_drain.
@@ -1219,9 +1457,9 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     bf16 *out = static_cast<bf16 *>(output);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (padded_dim(head_dim)) {
-        case 32: return launch_forward<32, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
-        case 64: return launch_forward<64, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
-        default: return launch_forward<128, 2>(A, q, k, v, out, lse, part, part_lse, p.splits, s);
+        case 32: return launch_forward<32>(A, p, q, k, v, out, lse, part, part_lse, s);
+        case 64: return launch_forward<64>(A, p, q, k, v, out, lse, part, part_lse, s);
+        default: return launch_forward<128>(A, p, q, k, v, out, lse, part, part_lse, s);
     }
 }
 

@@ -115,6 +115,7 @@ enum Knob {
     kKnobLsapStepCap,   // "RFDETR_LSAP_STEP_CAP": scan steps an augmenting path may take (default: the column count)
     kKnobTopkSort,      // "RFDETR_TOPK_SORT": any value selects the one-CTA sort kernels
     kKnobTopkUnstaged,  // "RFDETR_TOPK_UNSTAGED": any value keeps the radix select's keys out of shared memory
+    kKnobAttnFwd,       // "RFDETR_ATTN_FWD": packed attention forward (1 long or 2 short kernel, key splits of the long one)
     kKnobCount
 };
 struct KnobValue {

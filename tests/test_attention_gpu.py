@@ -310,3 +310,23 @@ def test_refusals(pkg):
             (t(4, 2, 64), t(4, 2, 64).cpu(), t(4, 2, 64), off, None, {})]:
         with pytest.raises(ValueError):
             call(q, k, v, o, ko, **kw)
+
+
+@pytest.mark.parametrize("knob", ["1,1", "1,3", "1,64", "2"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_every_forward_kernel(pkg, tuning, knob, dim):
+    """Both kernels, and the first with its keys split over blocks (more blocks than key tiles
+    among them), whatever the sizes would choose."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    _check(pkg, (1, 300, 0, 517, 64), heads=6, kv=2, dim=dim, causal=True, seed=dim)
+    _check(pkg, (3, 130, 40, 7), (900, 0, 17, 129), heads=4, kv=1, dim=dim, seed=dim)
+    _check(pkg, (130, 5), (30, 1000), heads=2, kv=2, dim=dim, causal=True, seed=dim)
+
+
+def test_one_token_over_long_keys(pkg):
+    """The form for single tokens: the keys are split over blocks."""
+    N = pkg._native
+    assert N.lib().rfdetr_packed_attention_workspace_bytes(3, 3, 9000, 8, 2, 128) > 0
+    _check(pkg, (1, 1, 1), (5000, 1, 3999), heads=8, kv=2, dim=128, causal=True, grad=False)
+    _check(pkg, (1,), (7000,), heads=4, kv=4, dim=64)
+    _check(pkg, (2, 0, 1), (3000, 3000, 3000), heads=7, kv=1, dim=80, causal=True)
