@@ -32,10 +32,15 @@ struct AttnArgs {
     int n_seq, Tq, Tk;
     int Hq, Hkv, D;
     int pack;    // query heads in one tile (of those that share a key head)
+    int pack_inv;  // 65536 / pack rounded up: row / pack for rows up to 255
     int subs;    // tiles' head groups per key head: (Hq / Hkv) / pack
     int causal;
     float scale, scale_log2;
 };
+
+// A tile row's token within the tile and its head among the packed ones.
+__device__ __forceinline__ int row_token(const AttnArgs &A, int row) { return (row * A.pack_inv) >> 16; }
+__device__ __forceinline__ int row_head(const AttnArgs &A, int row) { return row - row_token(A, row) * A.pack; }
 
 // Bytes of a tile row panel and panels per row, for channels padded to DP.
 template <int DP> struct Tile {
@@ -50,43 +55,44 @@ __device__ __forceinline__ int off_at(const int32_t *off, int n_seq, int T, int 
     return min(max(off[x - 1], 0), T);
 }
 
-// The rows of one tile slot: sequence (-1: none to serve keys), first row in it, its rows.
+// The rows of one tile slot, and the keys of its sequence (of the other tensor).
 struct Slot {
-    int seq;    // index into the offsets, or -1 for rows outside every sequence
     int first;  // first row of the slot within the sequence
-    int base;   // the sequence's first row in the packed tensor
-    int len;    // the sequence's rows
+    int base, len;  // the sequence's first row in the packed tensor, and its rows
+    int other_base, other_len;  // the same of the tensor on the other side (none outside all sequences)
 };
 
 // Whole warp.  Extended sequence x: rows off_at(x) .. off_at(x + 1), x = 0 and n_seq + 1 being the
-// rows before and after all sequences.  A search over 32 probes a step.
-__device__ __forceinline__ Slot find_slot(const int32_t *off, int n_seq, int T, int R, int slot) {
+// rows before and after all sequences.  A search over 31 probes a step; the last step's probes
+// already hold the answer, so up to 30 sequences take one round trip to memory, up to 960 two.
+__device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *other, int n_seq, int T, int T_other,
+                                          int R, int slot) {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = n_seq + 2;
-    while (n > 1) {
-        const int step = (n + 31) >> 5;
-        const int i = lane * step;
-        bool before = false;
-        if (i < n) before = off_at(off, n_seq, T, lo + i) / R + lo + i <= slot;
+    while (true) {
+        const int step = (n + 30) / 31;
+        const int x = lo + lane * step;
+        const int e = off_at(off, n_seq, T, x);
+        int f = 0;
+        if (step == 1 && x > 0) f = off == other ? min(e, T_other) : off_at(other, n_seq, T_other, x);
+        const bool before = lane * step < n && e / R + x <= slot;
         const unsigned m = __ballot_sync(0xffffffffu, before);
-        const int p = m ? 31 - __clz(m) : 0;
+        const int p = m ? 31 - __clz(m) : 0;  // at most 30
+        if (step == 1) {
+            Slot r;
+            lo += p;
+            r.base = __shfl_sync(0xffffffffu, e, p);
+            r.len = max(0, __shfl_sync(0xffffffffu, e, p + 1) - r.base);
+            r.first = (slot - (r.base / R + lo)) * R;
+            const int a = __shfl_sync(0xffffffffu, f, p), b = __shfl_sync(0xffffffffu, f, p + 1);
+            const bool real = lo >= 1 && lo <= n_seq;
+            r.other_base = real ? a : 0;
+            r.other_len = real ? max(0, b - a) : 0;
+            return r;
+        }
         lo += p * step;
         n = min(step, n - p * step);
     }
-    Slot r;
-    r.base = off_at(off, n_seq, T, lo);
-    r.len = max(0, off_at(off, n_seq, T, lo + 1) - r.base);
-    r.first = (slot - (r.base / R + lo)) * R;
-    r.seq = (lo >= 1 && lo <= n_seq) ? lo - 1 : -1;
-    return r;
-}
-
-__device__ __forceinline__ void seq_range(const int32_t *off, int n_seq, int T, int seq, int &base, int &len) {
-    base = 0;
-    len = 0;
-    if (seq < 0) return;
-    base = off_at(off, n_seq, T, seq + 1);
-    len = max(0, off_at(off, n_seq, T, seq + 2) - base);
 }
 
 inline long long slots_for(long long T, long long R, long long n_seq) { return T / R + n_seq + 2; }
@@ -94,13 +100,14 @@ inline long long slots_for(long long T, long long R, long long n_seq) { return T
 // Polls of a wait before the block gives up.  Every wait here is for work of the same block.
 constexpr int kAttnWaitLimit = 1 << 21;
 
-__device__ __forceinline__ bool wait_one(uint64_t *bar, unsigned parity, volatile int *abort) {
-    return mbar_wait(bar, parity, abort, kAttnWaitLimit);
-}
-// The same for a whole warp: all of its lanes go on, or none (tensor memory is moved by warps).
+// A whole warp's wait: all of its lanes go on, or none (tensor memory is moved by warps).
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volatile int *abort) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kAttnWaitLimit));
 }
+
+// The warp's index as a value that the compiler knows to be the same in all lanes.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
 // Zeroes rows [from, to) of a swizzled tile by the first `threads` threads of a block or a warp's
 // lanes (32); whole rows, so the swizzle does not matter.
@@ -301,7 +308,6 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
                          int qrow, int tok_per_tile, int krow, int klen) {
     using S = LongShape<DP>;
     using TL = Tile<DP>;
-    const int lane = threadIdx.x & 31;
     volatile int *abort = &sh.abort;
     if (r.nmax <= r.j0) return 0;
     const int loads = 2 * (r.nmax - r.j0);
@@ -317,21 +323,20 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
         const int foreign = is_v ? (j + 1) * S::kKeys - klen : 0;
         const uint32_t dst = smem_kv + st * S::kTileBytes;
         uint64_t *bar = foreign > 0 ? &sh.kv_raw : &sh.kv_full[st];
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive_expect_tx(bar, S::kTileBytes);
-            for (int p = 0; p < TL::kPanels; ++p)
-                tma_load_3d(dst + p * 128 * TL::kRowBytes, is_v ? mv : mk, bar, p * TL::kCols, kvh,
-                            krow + j * S::kKeys);
-            if (issued == 0) {
+        mbar_arrive_expect_one(bar, S::kTileBytes);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (r.n[t] <= r.j0) continue;
-                    mbar_arrive_expect_tx(&sh.q_full[t], box_bytes<DP>(tok_per_tile * A.pack));
-                    for (int p = 0; p < TL::kPanels; ++p)
-                        tma_load_3d(smem_q + t * S::kTileBytes + p * 128 * TL::kRowBytes, mq, &sh.q_full[t],
+        for (int p = 0; p < TL::kPanels; ++p)
+            tma_load_3d_one(dst + p * 128 * TL::kRowBytes, is_v ? mv : mk, bar, p * TL::kCols, kvh,
+                            krow + j * S::kKeys);
+        if (issued == 0) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (r.n[t] <= r.j0) continue;
+                mbar_arrive_expect_one(&sh.q_full[t], box_bytes<DP>(tok_per_tile * A.pack));
+#pragma unroll
+                for (int p = 0; p < TL::kPanels; ++p)
+                    tma_load_3d_one(smem_q + t * S::kTileBytes + p * 128 * TL::kRowBytes, mq, &sh.q_full[t],
                                     p * TL::kCols, qhead, qrow + t * tok_per_tile);
-                }
             }
         }
         if (foreign > 0) {
@@ -343,7 +348,7 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
             zero_rows<DP>(dst, 128, S::kKeys - foreign, S::kKeys, 32);
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+            mbar_arrive_one(&sh.kv_full[st]);
         }
     }
     return issued;
@@ -358,7 +363,7 @@ template <int DP> __device__ void long_drain(LongShared &sh, const LongRange &r,
         mbar_drain(&sh.kv_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
 }
 
-// One thread.
+// Whole warp.
 template <int DP>
 __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, uint32_t tmem) {
     using S = LongShape<DP>;
@@ -366,18 +371,21 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
     constexpr uint32_t kIdO = mma_idesc(128, DP, true);
     constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
     volatile int *abort = &sh.abort;
+    const uint64_t q_desc = smem_desc<TL::kRowBytes>(smem_q, 16, kSbo);
+    const uint64_t k_desc = smem_desc<TL::kRowBytes>(smem_kv, 16, kSbo);
+    const uint64_t v_desc = smem_desc<TL::kRowBytes>(smem_kv, kLbo, kSbo);
     auto scores = [&](int t, int st, int j) {
         const uint32_t id = mma_idesc(128, tile_cols(r.sees[t], j * S::kKeys, S::kKeys), false);
+        const uint64_t a = q_desc + t * (S::kTileBytes / 16), b = k_desc + st * (S::kTileBytes / 16);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t o = (k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes;
-            mma_ss(tmem + t * 128, smem_desc<TL::kRowBytes>(smem_q + t * S::kTileBytes + o, 16, kSbo),
-                   smem_desc<TL::kRowBytes>(smem_kv + st * S::kTileBytes + o, 16, kSbo), id, k > 0);
+            const uint32_t o = ((k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes) / 16;
+            mma_ss_one(tmem + t * 128, a + o, b + o, id, k > 0);
         }
-        tc_commit(&sh.s_full[t]);
+        tc_commit_one(&sh.s_full[t]);
     };
     auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
-        return wait_one(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
+        return wait_warp(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
     };
     const int n = r.nmax - r.j0;
     int st = kv(0);
@@ -385,11 +393,11 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         if (r.n[t] <= r.j0) continue;
-        if (!wait_one(&sh.q_full[t], 0, abort)) return false;
+        if (!wait_warp(&sh.q_full[t], 0, abort)) return false;
         tc_fence_after();
         scores(t, st, r.j0);
     }
-    tc_commit(&sh.kv_empty[st]);
+    tc_commit_one(&sh.kv_empty[st]);
     for (int i = 0; i < n; ++i) {
         int sv = -1, sk = -1;
 #pragma unroll
@@ -397,14 +405,16 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
             const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
             if (left > 0) {
                 if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
-                if (!wait_one(&sh.p_ready[t], i & 1, abort)) return false;
+                if (!wait_warp(&sh.p_ready[t], i & 1, abort)) return false;
                 tc_fence_after();
                 const int steps = tile_cols(r.sees[t], (r.j0 + i) * S::kKeys, S::kKeys) / 16;
-                for (int k = 0; k < steps; ++k)
-                    mma_ts(tmem + 256 + t * DP, tmem + t * 128 + k * 8,
-                           smem_desc<TL::kRowBytes>(smem_kv + sv * S::kTileBytes + k * 16 * TL::kRowBytes, kLbo, kSbo),
-                           kIdO, i > 0 || k > 0);
-                if (left == 1) tc_commit(&sh.o_done[t]);
+                const uint64_t b = v_desc + sv * (S::kTileBytes / 16);
+#pragma unroll
+                for (int k = 0; k < S::kKeys / 16; ++k)
+                    if (k < steps)
+                        mma_ts_one(tmem + 256 + t * DP, tmem + t * 128 + k * 8, b + k * TL::kRowBytes, kIdO,
+                                   i > 0 || k > 0);
+                if (left == 1) tc_commit_one(&sh.o_done[t]);
             }
             if (left > 1) {
                 if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
@@ -413,8 +423,8 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
                 scores(t, sk, r.j0 + i + 1);
             }
         }
-        if (sv >= 0) tc_commit(&sh.kv_empty[sv]);
-        if (sk >= 0) tc_commit(&sh.kv_empty[sk]);
+        if (sv >= 0) tc_commit_one(&sh.kv_empty[sv]);
+        if (sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
     }
     return true;
 }
@@ -428,16 +438,15 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     using S = LongShape<DP>;
     extern __shared__ unsigned char dyn[];
     __shared__ LongShared sh;
-    const int warp = threadIdx.x >> 5;
+    const int warp = warp_index();
     const int heads = A.Hkv * A.subs;
     const int hx = blockIdx.x % heads;
     // Later slots first: under a causal mask they see more keys.
     const int slot = slots - 1 - (int)(blockIdx.x / heads);
     const int per = 128 / A.pack;  // tokens in a row tile
-    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per * 2, slot);
+    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per * 2, slot);
     if (q.first >= q.len) return;
-    int kbase, klen;
-    seq_range(A.k_off, A.n_seq, A.Tk, q.seq, kbase, klen);
+    const int kbase = q.other_base, klen = q.other_len;
     const int kvh = hx / A.subs;
     const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
 
@@ -485,7 +494,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
     const uint32_t smem_q = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t smem_kv = smem_q + 2 * S::kTileBytes;
 
@@ -493,7 +502,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     if (warp >= 8) {
         regs_less<kLessRegs>();
         if (warp == 8) {
-            if ((threadIdx.x & 31) == 0 && r.nmax > r.j0) long_mma_loop<DP>(sh, smem_q, smem_kv, r, tmem);
+            if (r.nmax > r.j0) long_mma_loop<DP>(sh, smem_q, smem_kv, r, tmem);
         } else if (warp == 9) {
             issued = long_load<DP>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
                                    klen);
@@ -506,8 +515,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lane 32 (w % 4)
             const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + 256 + t * DP;
             const int row = threadIdx.x & 127;
-            const int tok_first = q.first + t * per, tok = tok_first + row / A.pack;
-            const bool live = row / A.pack < r.tok[t];
+            const int tok_first = q.first + t * per, tok = tok_first + row_token(A, row);
+            const bool live = row_token(A, row) < r.tok[t];
             const bool warp_live = (row & ~31) < r.tok[t] * A.pack;
             const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
             // Keys that every row of the tile sees (rows past the last token do not count).
@@ -525,12 +534,12 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                                                limit - k0, i == 0, A.scale_log2);
                 tc_fence_before();
                 __syncwarp();
-                if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_ready[t]);
+                mbar_arrive_one(&sh.p_ready[t]);
             }
             if (ok && n > 0) ok = wait_warp(&sh.o_done[t], 0, abort);
             tc_fence_after();
             if (ok)
-                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row % A.pack, out, lse, part,
+                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse, part,
                                      part_lse);
         }
     }
@@ -539,8 +548,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     __syncthreads();
     if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0) long_drain<DP>(sh, r, issued);
     if (warp == 8) {
-        if (sh.abort && (threadIdx.x & 31) == 0) {
-            tc_commit(&sh.drain);
+        if (sh.abort) {
+            tc_commit_one(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
         }
         __syncwarp();
@@ -552,7 +561,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
 // ---- short sequences: one row tile to a block, several blocks to an SM ---------------------------
 // With a few key tiles to a block, most of its time would be its start and its end; four blocks to
 // an SM (two with 128 channels) cover each other's instead of roles within one.  128 threads: each
-// owns a row, thread 0 also issues the copies and the products.  64 keys a tile, so that S and O of
+// owns a row, warp 0 also issues the copies and the products.  64 keys a tile, so that S and O of
 // four blocks fit TMEM and a row of S is 64 registers.
 template <int DP> struct ShortShape {
     static constexpr int kKeys = 64;
@@ -581,24 +590,23 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     constexpr uint32_t kSbo = 8 * TL::kRowBytes, kQPanel = 128 * TL::kRowBytes, kPanel = KEYS * TL::kRowBytes;
     extern __shared__ unsigned char dyn[];
     __shared__ ShortShared sh;
-    const int warp = threadIdx.x >> 5;
+    const int warp = warp_index();
     const int heads = A.Hkv * A.subs;
     const int hx = blockIdx.x % heads;
     const int slot = slots - 1 - (int)(blockIdx.x / heads);
     const int per = 128 / A.pack;
-    const Slot q = find_slot(A.q_off, A.n_seq, A.Tq, per, slot);
+    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per, slot);
     if (q.first >= q.len) return;
-    int kbase, klen;
-    seq_range(A.k_off, A.n_seq, A.Tk, q.seq, kbase, klen);
+    const int kbase = q.other_base, klen = q.other_len;
     const int kvh = hx / A.subs;
     const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
     const int ntok = min(per, q.len - q.first);
     const int sees = A.causal ? min(klen, max(0, q.first + ntok + klen - q.len)) : klen;
     const int n = (sees + KEYS - 1) / KEYS;
-    const bool boss = threadIdx.x == 0;
+    const bool boss = warp == 0;  // this warp also asks for copies and products
 
-    if (warp == 0) {
-        if (boss) {
+    if (boss) {
+        if (threadIdx.x == 0) {
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh.k_full[i], 1);
                 mbar_init(&sh.v_full[i], 1);
@@ -615,43 +623,47 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
     const uint32_t smem_q = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t smem_k = smem_q + S::kQBytes, smem_v = smem_k + 2 * S::kTileBytes;
     volatile int *abort = &sh.abort;
 
     auto load = [&](const CUtensorMap *map, uint64_t *bar, uint32_t dst, int j) {
+#pragma unroll
         for (int p = 0; p < TL::kPanels; ++p)
-            tma_load_3d(dst + p * kPanel, map, bar, p * TL::kCols, kvh, kbase + j * KEYS);
+            tma_load_3d_one(dst + p * kPanel, map, bar, p * TL::kCols, kvh, kbase + j * KEYS);
     };
     auto load_k = [&](int j, unsigned more) {
-        mbar_arrive_expect_tx(&sh.k_full[j & 1], S::kTileBytes + more);
+        mbar_arrive_expect_one(&sh.k_full[j & 1], S::kTileBytes + more);
         load(&mk, &sh.k_full[j & 1], smem_k + (j & 1) * S::kTileBytes, j);
     };
     auto load_v = [&](int j) {
-        mbar_arrive_expect_tx(&sh.v_full[j & 1], S::kTileBytes);
+        mbar_arrive_expect_one(&sh.v_full[j & 1], S::kTileBytes);
         load(&mv, &sh.v_full[j & 1], smem_v + (j & 1) * S::kTileBytes, j);
     };
+    const uint64_t q_desc = smem_desc<TL::kRowBytes>(smem_q, 16, kSbo);
+    const uint64_t k_desc = smem_desc<TL::kRowBytes>(smem_k, 16, kSbo);
+    const uint64_t v_desc = smem_desc<TL::kRowBytes>(smem_v, kPanel, kSbo);
     auto scores = [&](int j) {
-        if (!wait_one(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return false;
+        if (!wait_warp(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t id = mma_idesc(128, tile_cols(sees, j * KEYS, KEYS), false);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
             const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
-            mma_ss(tmem, smem_desc<TL::kRowBytes>(smem_q + panel * kQPanel + in, 16, kSbo),
-                   smem_desc<TL::kRowBytes>(smem_k + (j & 1) * S::kTileBytes + panel * kPanel + in, 16, kSbo), id,
-                   k > 0);
+            mma_ss_one(tmem, q_desc + (panel * kQPanel + in) / 16,
+                       k_desc + ((j & 1) * S::kTileBytes + panel * kPanel + in) / 16, id, k > 0);
         }
-        tc_commit(&sh.s_full);
+        tc_commit_one(&sh.s_full);
         return true;
     };
-    int k_issued = 0, v_issued = 0;  // thread 0
+    int k_issued = 0, v_issued = 0;  // warp 0
     bool ok = true;
     if (boss && n > 0) {
         load_k(0, box_bytes<DP>(per * A.pack));
+#pragma unroll
         for (int p = 0; p < TL::kPanels; ++p)
-            tma_load_3d(smem_q + p * kQPanel, &mq, &sh.k_full[0], p * TL::kCols, qhead, q.base + q.first);
+            tma_load_3d_one(smem_q + p * kQPanel, &mq, &sh.k_full[0], p * TL::kCols, qhead, q.base + q.first);
         load_v(0);
         k_issued = v_issued = 1;
         if (n > 1) {
@@ -663,8 +675,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
 
     const uint32_t ts = tmem + ((uint32_t)warp << 21), to = ts + KEYS;
     const int row = threadIdx.x;
-    const int tok = q.first + row / A.pack;
-    const bool live = row / A.pack < ntok;
+    const int tok = q.first + row_token(A, row);
+    const bool live = row_token(A, row) < ntok;
     const bool warp_live = (row & ~31) < ntok * A.pack;
     const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
     const int all_see = A.causal ? min(klen, q.first + 1 + klen - q.len) : klen;
@@ -679,7 +691,6 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             if (i + 2 < n) load_k(i + 2, 0), ++k_issued;
             if (i + 1 < n) load_v(i + 1), ++v_issued;
         }
-        __syncwarp();
         const int k0 = i * KEYS;
         if (warp_live)
             softmax_tile<DP, KEYS>(rs, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS > all_see, limit - k0, i == 0,
@@ -695,35 +706,36 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         if (gave_up) break;
         if (boss) {
             tc_fence_after();
-            ok = wait_one(&sh.v_full[i & 1], (i >> 1) & 1, abort);
-            const int steps = tile_cols(sees, k0, KEYS) / 16;
-            for (int k = 0; k < steps && ok; ++k)
-                mma_ts(tmem + KEYS, tmem + k * 8,
-                       smem_desc<TL::kRowBytes>(smem_v + (i & 1) * S::kTileBytes + k * 16 * TL::kRowBytes, kPanel,
-                                                kSbo),
-                       kIdO, i > 0 || k > 0);
-            if (i + 1 < n) ok = ok && scores(i + 1);
-            else tc_commit(&sh.o_done);
+            ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort);
+            if (ok) {
+                const int steps = tile_cols(sees, k0, KEYS) / 16;
+                const uint64_t b = v_desc + (i & 1) * (S::kTileBytes / 16);
+#pragma unroll
+                for (int k = 0; k < KEYS / 16; ++k)
+                    if (k < steps)
+                        mma_ts_one(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                if (i + 1 < n) ok = scores(i + 1);
+                else tc_commit_one(&sh.o_done);
+            }
         }
-        __syncwarp();
     }
     if (!gave_up) {
         if (n > 0) ok = wait_warp(&sh.o_done, 0, abort);
         tc_fence_after();
         if (ok)
-            write_row<DP, false>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row % A.pack, out, lse, nullptr,
+            write_row<DP, false>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse, nullptr,
                                  nullptr);
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
-        if (boss && sh.abort) {
+    if (boss) {
+        if (sh.abort) {
             for (int i = max(0, k_issued - 2); i < k_issued; ++i)
                 mbar_drain(&sh.k_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
             for (int i = max(0, v_issued - 2); i < v_issued; ++i)
                 mbar_drain(&sh.v_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
-            tc_commit(&sh.drain);
+            tc_commit_one(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
         }
         __syncwarp();
@@ -827,13 +839,14 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
     volatile int *abort = &sh.abort;
     if (r.steps == 0) return 0;
     const int xrows = DKV ? 128 : (128 / A.pack) * A.pack;
-    if (lane == 0) {
-        mbar_arrive_expect_tx(&sh.x_full, 2 * box_bytes<DP>(xrows));
+    {
+        mbar_arrive_expect_one(&sh.x_full, 2 * box_bytes<DP>(xrows));
         const int head = DKV ? r.kvh : r.qhead, at = DKV ? r.kbase + r.k0 : r.qbase + r.q0;
+#pragma unroll
         for (int p = 0; p < TL::kPanels; ++p) {
             const uint32_t o = p * 128 * TL::kRowBytes;
-            tma_load_3d(smem_x + o, mx0, &sh.x_full, p * TL::kCols, head, at);
-            tma_load_3d(smem_x + S::kXBytes + o, mx1, &sh.x_full, p * TL::kCols, head, at);
+            tma_load_3d_one(smem_x + o, mx0, &sh.x_full, p * TL::kCols, head, at);
+            tma_load_3d_one(smem_x + S::kXBytes + o, mx1, &sh.x_full, p * TL::kCols, head, at);
         }
     }
     const int yrows = DKV ? r.tok * A.pack : kWalk;
@@ -851,14 +864,12 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
         const int good = DKV ? min(r.tok, r.qlen - at) * A.pack : min(kWalk, r.klen - at);
         uint64_t *bar = good < yrows ? &sh.y_raw : &sh.y_full[st];
         const uint32_t y0 = smem_y + st * 2 * S::kYBytes, y1 = y0 + S::kYBytes;
-        __syncwarp();
-        if (lane == 0) {
-            mbar_expect_tx(bar, 2 * box_bytes<DP>(yrows));
-            for (int p = 0; p < TL::kPanels; ++p) {
-                const uint32_t o = p * kWalk * TL::kRowBytes;
-                tma_load_3d(y0 + o, my0, bar, p * TL::kCols, head, base + at);
-                tma_load_3d(y1 + o, my1, bar, p * TL::kCols, head, base + at);
-            }
+        mbar_expect_one(bar, 2 * box_bytes<DP>(yrows));
+#pragma unroll
+        for (int p = 0; p < TL::kPanels; ++p) {
+            const uint32_t o = p * kWalk * TL::kRowBytes;
+            tma_load_3d_one(y0 + o, my0, bar, p * TL::kCols, head, base + at);
+            tma_load_3d_one(y1 + o, my1, bar, p * TL::kCols, head, base + at);
         }
         if (DKV) {
 #pragma unroll
@@ -866,7 +877,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 const int c = lane + h * 32;
                 float nl = 0.0f, nd = 0.0f, od = 0.0f;
                 if (c < good) {
-                    const size_t x = (size_t)(head + c % A.pack) * A.Tq + base + at + c / A.pack;
+                    const size_t x = (size_t)(head + row_head(A, c)) * A.Tq + base + at + row_token(A, c);
                     nl = -lse[x] * kLog2e;
                     nd = -delta[x];
                     if (g_lse) od = g_lse[x];
@@ -877,7 +888,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
             }
             __syncwarp();
         }
-        if (lane == 0) mbar_arrive(bar);
+        mbar_arrive_one(bar);
         if (good < yrows) {
             if (!wait_warp(&sh.y_raw, raw_phase, abort)) {
                 mbar_drain(&sh.y_raw, raw_phase, kAttnWaitLimit);
@@ -888,13 +899,13 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
             zero_rows<DP>(y1, kWalk, good, yrows, 32);
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.y_full[st]);
+            mbar_arrive_one(&sh.y_full[st]);
         }
     }
     return i;
 }
 
-// One thread.
+// Whole warp.
 template <int DP, bool DKV>
 __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, int steps, uint32_t tmem) {
     using S = BwdShape<DP>;
@@ -903,44 +914,46 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
     constexpr uint32_t kSbo = 8 * TL::kRowBytes;
     constexpr uint32_t kXPanel = 128 * TL::kRowBytes, kYPanel = kWalk * TL::kRowBytes;
     volatile int *abort = &sh.abort;
+    const uint64_t x_desc = smem_desc<TL::kRowBytes>(smem_x, 16, kSbo);
+    const uint64_t y_desc = smem_desc<TL::kRowBytes>(smem_y, 16, kSbo);
+    const uint64_t yt_desc = smem_desc<TL::kRowBytes>(smem_y, kYPanel, kSbo);
     auto scores = [&](int i) {
         const int st = i % S::kStages;
-        if (!wait_one(&sh.y_full[st], (i / S::kStages) & 1, abort)) return false;
+        if (!wait_warp(&sh.y_full[st], (i / S::kStages) & 1, abort)) return false;
         tc_fence_after();
-        const uint32_t y = smem_y + st * 2 * S::kYBytes;
+        const uint64_t y = y_desc + st * (2 * S::kYBytes / 16);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
                 const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
-                mma_ss(tmem + (i & 1) * 2 * kWalk + which * kWalk,
-                       smem_desc<TL::kRowBytes>(smem_x + which * S::kXBytes + panel * kXPanel + in, 16, kSbo),
-                       smem_desc<TL::kRowBytes>(y + which * S::kYBytes + panel * kYPanel + in, 16, kSbo), kIdS, k > 0);
+                mma_ss_one(tmem + (i & 1) * 2 * kWalk + which * kWalk,
+                           x_desc + (which * S::kXBytes + panel * kXPanel + in) / 16,
+                           y + (which * S::kYBytes + panel * kYPanel + in) / 16, kIdS, k > 0);
             }
-        tc_commit(&sh.s_full[i & 1]);
+        tc_commit_one(&sh.s_full[i & 1]);
         return true;
     };
-    if (!wait_one(&sh.x_full, 0, abort)) return false;
+    if (!wait_warp(&sh.x_full, 0, abort)) return false;
     if (!scores(0)) return false;
     if (steps > 1 && !scores(1)) return false;
     for (int i = 0; i < steps; ++i) {
         const int st = i % S::kStages;
-        const uint32_t y = smem_y + st * 2 * S::kYBytes;
-        if (!wait_one(&sh.ds_ready[i & 1], (i >> 1) & 1, abort)) return false;
+        const uint64_t y = yt_desc + st * (2 * S::kYBytes / 16);
+        if (!wait_warp(&sh.ds_ready[i & 1], (i >> 1) & 1, abort)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kWalk / 16; ++k) {
-            const uint32_t row = k * 16 * TL::kRowBytes;
             if (DKV)
-                mma_ts(tmem + 4 * kWalk + DP, tmem + (i & 1) * 2 * kWalk + k * 8,
-                       smem_desc<TL::kRowBytes>(y + S::kYBytes + row, kYPanel, kSbo), kIdAcc, i > 0 || k > 0);
-            mma_ts(tmem + 4 * kWalk, tmem + (i & 1) * 2 * kWalk + kWalk + k * 8,
-                   smem_desc<TL::kRowBytes>(y + row, kYPanel, kSbo), kIdAcc, i > 0 || k > 0);
+                mma_ts_one(tmem + 4 * kWalk + DP, tmem + (i & 1) * 2 * kWalk + k * 8,
+                           y + S::kYBytes / 16 + k * TL::kRowBytes, kIdAcc, i > 0 || k > 0);
+            mma_ts_one(tmem + 4 * kWalk, tmem + (i & 1) * 2 * kWalk + kWalk + k * 8, y + k * TL::kRowBytes, kIdAcc,
+                       i > 0 || k > 0);
         }
-        tc_commit(&sh.y_empty[st]);
+        tc_commit_one(&sh.y_empty[st]);
         if (i + 2 < steps && !scores(i + 2)) return false;
     }
-    tc_commit(&sh.acc_done);
+    tc_commit_one(&sh.acc_done);
     return true;
 }
 
@@ -956,12 +969,12 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     const int shift = r.klen - r.qlen;  // under a causal mask token t sees keys <= t + shift
     // DKV: this row's key.  DQ: this row's query.
     const int key = r.k0 + row;
-    const int tok = r.q0 + row / A.pack;
+    const int tok = r.q0 + row_token(A, row);
     int limit = 0;
     float row_nl = 0.0f, row_nd = 0.0f, row_od = 0.0f;
-    if (!DKV && row / A.pack < r.qtok) {
+    if (!DKV && row_token(A, row) < r.qtok) {
         limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
-        const size_t x = (size_t)(r.qhead + row % A.pack) * A.Tq + r.qbase + tok;
+        const size_t x = (size_t)(r.qhead + row_head(A, row)) * A.Tq + r.qbase + tok;
         row_nl = -lse[x] * kLog2e;
         row_nd = -delta[x];
         if (g_lse) row_od = g_lse[x];
@@ -1047,7 +1060,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.ds_ready[w]);
+        mbar_arrive_one(&sh.ds_ready[w]);
     }
     if (r.steps > 0) wait_warp(&sh.acc_done, 0, abort);
     tc_fence_after();
@@ -1091,13 +1104,14 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     using S = BwdShape<DP>;
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(16) BwdShared sh;
-    const int warp = threadIdx.x >> 5;
+    const int warp = warp_index();
     const int heads = DKV ? A.Hkv : A.Hkv * A.subs;
     const int hx = blockIdx.x % heads;
     // The tiles with most work under a causal mask first: the first keys, the last queries.
     const int slot = DKV ? blockIdx.x / heads : slots - 1 - (int)(blockIdx.x / heads);
     const int per = DKV ? 128 : 128 / A.pack;
-    const Slot x = DKV ? find_slot(A.k_off, A.n_seq, A.Tk, per, slot) : find_slot(A.q_off, A.n_seq, A.Tq, per, slot);
+    const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, per, slot)
+                       : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per, slot);
     if (x.first >= x.len) return;
     const int G = A.Hq / A.Hkv;
     BwdRange r;
@@ -1108,13 +1122,13 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     r.steps_per_sub = 1;
     if (DKV) {
         r.kbase = x.base, r.klen = x.len, r.k0 = x.first;
-        seq_range(A.q_off, A.n_seq, A.Tq, x.seq, r.qbase, r.qlen);
+        r.qbase = x.other_base, r.qlen = x.other_len;
         r.first = A.causal ? min(r.qlen, max(0, r.k0 + r.qlen - r.klen)) : 0;
         r.steps_per_sub = (r.qlen - r.first + r.tok - 1) / r.tok;
         r.steps = r.steps_per_sub * A.subs;
     } else {
         r.qbase = x.base, r.qlen = x.len, r.q0 = x.first;
-        seq_range(A.k_off, A.n_seq, A.Tk, x.seq, r.kbase, r.klen);
+        r.kbase = x.other_base, r.klen = x.other_len;
         r.qtok = min(per, r.qlen - r.q0);
         const int sees = A.causal ? min(r.klen, max(0, r.q0 + r.qtok + r.klen - r.qlen)) : r.klen;
         r.steps = (sees + kWalk - 1) / kWalk;
@@ -1151,11 +1165,11 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
 
     int issued = 0;
     if (warp == 8) {
-        if ((threadIdx.x & 31) == 0 && r.steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, r.steps, tmem);
+        if (r.steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, r.steps, tmem);
     } else if (warp == 9) {
         issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
     } else {
@@ -1170,9 +1184,9 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
             if (w == 0) store_acc<DP>(acc, any, 0, DP, A.scale, g0 + at, A.D, live);
             else store_acc<DP>(acc + DP, any, 0, DP, 1.0f, g1 + at, A.D, live);
         } else {
-            const bool live = row / A.pack < r.qtok;
+            const bool live = row_token(A, row) < r.qtok;
             const size_t at =
-                ((size_t)(r.qbase + r.q0 + row / A.pack) * A.Hq + r.qhead + row % A.pack) * A.D;
+                ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
             const int half = DP >= 64 ? DP / 2 : DP;  // columns of the first warpgroup
             store_acc<DP>(acc, any, w * half, w == 0 ? half : DP, A.scale, g0 + at, A.D, live);
         }
@@ -1186,8 +1200,8 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
             mbar_drain(&sh.y_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
     }
     if (warp == 8) {
-        if (sh.abort && (threadIdx.x & 31) == 0) {
-            tc_commit(&sh.drain);
+        if (sh.abort) {
+            tc_commit_one(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
         }
         __syncwarp();
@@ -1398,6 +1412,7 @@ AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, in
     A.Hkv = (int)Hkv;
     A.D = (int)D;
     A.pack = pack_of(Hq / Hkv, most_packed);
+    A.pack_inv = (65536 + A.pack - 1) / A.pack;
     A.subs = (int)(Hq / Hkv) / A.pack;
     A.causal = causal != 0;
     A.scale = scale;

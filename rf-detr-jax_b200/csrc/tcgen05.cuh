@@ -7,6 +7,11 @@
 //     tcgen05.commit, which arrives on an mbarrier when every earlier instruction of that thread
 //     is done.  Instructions of one thread execute in issue order, so a later one may overwrite
 //     TMEM that an earlier one reads;
+//   * the functions whose names end in _one are called by a whole converged warp with the same
+//     arguments in every lane, and one elected lane (always the same) carries them out.  The warp
+//     stays converged, so addresses and descriptors stay in uniform registers: eight matrix
+//     instructions issue in 188 cycles, where the same ones inside a branch of one thread, which
+//     moves every operand there first, took 650;
 //   * TMEM is 128 lanes x 512 columns of 32 bits.  An accumulator with M = 128 rows has one row
 //     per lane; warp w of a block reaches lanes 32 (w % 4) .. + 31, so a thread of a warpgroup
 //     owns one row;
@@ -47,18 +52,34 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // Makes this thread's shared-memory writes visible to the tensor core and TMA (async proxy).
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void mbar_arrive_one(uint64_t *bar) {
+    asm volatile(
+        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+        "@q mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(smem_u32(bar))
+        : "memory");
 }
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, unsigned bytes) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
+// Adds to the bytes that the current phase waits for, without arriving.
+__device__ __forceinline__ void mbar_expect_one(uint64_t *bar, unsigned bytes) {
+    asm volatile(
+        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+        "@q mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n}\n" ::"r"(smem_u32(bar)),
+        "r"(bytes)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_one(uint64_t *bar, unsigned bytes) {
+    asm volatile(
+        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(smem_u32(bar)),
+        "r"(bytes)
+        : "memory");
 }
 
-// Arrives on `bar` once every matrix instruction issued so far by this thread has completed.
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+// Arrives on `bar` once every matrix instruction issued so far by the elected lane has completed.
+__device__ __forceinline__ void tc_commit_one(uint64_t *bar) {
+    asm volatile(
+        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+        : "memory");
 }
 
 // ---- descriptors ----
@@ -67,7 +88,8 @@ template <int ROWBYTES> struct SmemSwizzle;
 template <> struct SmemSwizzle<128> { static constexpr uint64_t kMode = 2; };
 template <> struct SmemSwizzle<64> { static constexpr uint64_t kMode = 4; };
 
-// Operand descriptor of a swizzled tile at shared address `addr`.  `sbo`: bytes from one group of
+// Operand descriptor of a swizzled tile at shared address `addr`; that of a part of it `bytes` further on is
+// the descriptor + bytes / 16.  `sbo`: bytes from one group of
 // eight rows to the next.  `lbo`: for a tile whose rows run along the contraction (the operand is
 // "MN-major"), bytes from one column panel to the next; ignored when a row holds the contraction
 // ("K-major").
@@ -84,23 +106,25 @@ __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool b_mn_major) 
 }
 
 // D[tmem] (+)= A[smem] B[smem]; one step of 16 along the contraction.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q;\n"
+        "elect.sync _|q, 0xffffffff;\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
         "}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]; A holds two bf16 per column, 8 columns per step.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts_one(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q;\n"
+        "elect.sync _|q, 0xffffffff;\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
         "}\n" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
@@ -184,11 +208,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // 3-D tiled load of one box into shared memory, completing on `bar`.
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1,
-                                            int c2) {
+__device__ __forceinline__ void tma_load_3d_one(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1,
+                                                int c2) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(dst),
+        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];\n}\n" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
         : "memory");
 }
