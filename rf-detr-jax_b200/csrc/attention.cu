@@ -17,7 +17,7 @@
 // Queries of the heads that share a key head are rows of one tile (token-major, heads inner), so
 // K and V are read once for all of them and a few tokens still fill a tile.
 #include <cfloat>
-#include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -108,6 +108,11 @@ __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volati
 
 // The warp's index as a value that the compiler knows to be the same in all lanes.
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+
+// Blocks of three warpgroups, two of which compute: registers at launch 65536 / 384 -> 168, then
+// 2 x 208 + 88 = 3 x 168.
+constexpr int kLaunchRegs = 168, kMoreRegs = 208, kLessRegs = 88;
+static_assert(2 * kMoreRegs + kLessRegs <= 3 * kLaunchRegs, "a warpgroup would wait for registers for good");
 
 // Zeroes rows [from, to) of a swizzled tile by the first `threads` threads of a block or a warp's
 // lanes (32); whole rows, so the swizzle does not matter.
@@ -283,10 +288,6 @@ template <int DP> struct LongShape {
     static constexpr int kTmem = 512;
     static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
 };
-// Registers at launch: 65536 / 384 -> 168; 2 x 208 + 88 = 3 x 168.
-constexpr int kLaunchRegs = 168, kMoreRegs = 208, kLessRegs = 88;
-static_assert(2 * kMoreRegs + kLessRegs <= 3 * kLaunchRegs, "a warpgroup would wait for registers for good");
-
 struct LongShared {
     uint64_t q_full[2], kv_full[4], kv_raw, kv_empty[4], s_full[2], p_ready[2], o_done[2], drain;
     uint32_t tmem;
@@ -788,6 +789,9 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
 //   A = X0 Y0^T, B = X1 Y1^T  (128 x 64 each, TMEM)  ->  P = exp2(scale log2(e) A - log2(e) lse),
 //   dS = P (B - delta)        (bf16, written over A and B)
 //   acc0 += dS Y0             (dK or dQ, times scale at the end), acc1 += P Y1 (dV)
+// With few held tiles (or, under a causal mask, one that walks far longer than the mean) a cluster of
+// blocks shares a tile's steps; their accumulators are added through distributed shared memory, in
+// rank order, each block writing its share of the columns.
 // Two pairs (A, B) alternate between two warpgroups: while one turns its pair into P and dS, the
 // tensor core forms the other's and adds the one before.  64 rows a step is what TMEM leaves: two
 // pairs of 64 + 64 columns beside two accumulators of up to 128.
@@ -801,7 +805,7 @@ template <int DP> struct BwdShape {
     static constexpr int kXBytes = 128 * DP * 2;
     static constexpr int kYBytes = kWalk * DP * 2;
     static constexpr int kStages = 4;
-    static constexpr int kThreads = 2 * 128 + 64;
+    static constexpr int kThreads = 384;
     static constexpr int kTmem = 512;
     static constexpr size_t kSmem = 1024 + 2 * kXBytes + (size_t)kStages * 2 * kYBytes;
 };
@@ -820,6 +824,7 @@ struct BwdShared {
 // `subs` head groups.  DQ: tiles of 64 keys.
 struct BwdRange {
     int steps, steps_per_sub;
+    int start;      // this block's first step (its cluster's blocks share a tile's steps); steps ends them
     int first;      // DKV: first query token
     int qbase, qlen, kbase, klen;
     int tok;        // DKV: tokens a step
@@ -837,7 +842,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
     using TL = Tile<DP>;
     const int lane = threadIdx.x & 31;
     volatile int *abort = &sh.abort;
-    if (r.steps == 0) return 0;
+    if (r.steps <= r.start) return 0;
     const int xrows = DKV ? 128 : (128 / A.pack) * A.pack;
     {
         mbar_arrive_expect_one(&sh.x_full, 2 * box_bytes<DP>(xrows));
@@ -852,11 +857,12 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
     const int yrows = DKV ? r.tok * A.pack : kWalk;
     unsigned raw_phase = 0;
     int i = 0;
-    for (; i < r.steps; ++i) {
+    for (; i < r.steps - r.start; ++i) {
         const int st = i % S::kStages;
         if (i >= S::kStages && !wait_warp(&sh.y_empty[st], ((i / S::kStages) - 1) & 1, abort)) break;
-        const int sub = DKV ? i / r.steps_per_sub : 0;
-        const int at = DKV ? r.first + (i - sub * r.steps_per_sub) * r.tok : i * kWalk;  // within the sequence
+        const int step = r.start + i;
+        const int sub = DKV ? step / r.steps_per_sub : 0;
+        const int at = DKV ? r.first + (step - sub * r.steps_per_sub) * r.tok : step * kWalk;  // within the sequence
         const int head = DKV ? r.qhead + sub * A.pack : r.kvh;
         const int base = DKV ? r.qbase : r.kbase;
         // Rows of the box past the sequence's end belong to another sequence: cleared, since the
@@ -981,7 +987,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     }
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
-    for (int i = w; i < r.steps; i += 2) {
+    for (int i = w; i < r.steps - r.start; i += 2) {
         const int st = i % S::kStages;
         if (!wait_warp(&sh.s_full[w], (i >> 1) & 1, abort)) return;
         tc_fence_after();
@@ -990,7 +996,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         int lo = 0, hi = kWalk, one_lo = 0, one_hi = 0;
         bool mask;
         if (DKV) {
-            const int at = r.first + (i % r.steps_per_sub) * r.tok;
+            const int at = r.first + ((r.start + i) % r.steps_per_sub) * r.tok;
             const int good = min(r.tok, r.qlen - at) * A.pack;
             mask = good < kWalk || r.k0 + 128 > r.klen || (A.causal && at + shift < r.k0 + 127);
             if (mask) {
@@ -1006,9 +1012,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 }
             }
         } else {
-            mask = (i + 1) * kWalk > all_see;
+            mask = (r.start + i + 1) * kWalk > all_see;
             if (mask) {
-                hi = limit - i * kWalk;
+                hi = limit - (r.start + i) * kWalk;
                 one_hi = limit == 1 ? kWalk : 0;
             }
         }
@@ -1021,6 +1027,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         tmem_wait_ld();
         pin<kWalk>(s);
         pin<kWalk>(d);
+        uint32_t ps[32], pd[32];
+        // Straight code in either case: the exponentials' latencies overlap.
+        auto weights = [&](auto masked) {
 #pragma unroll
         for (int c = 0; c < kWalk; c += 4) {
             float4 nl, nd;
@@ -1033,36 +1042,36 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             }
             const float2 a = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(nl.x, nl.y));
             const float2 b = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(nl.z, nl.w));
-            const float2 p = make_float2(exp2_fast(a.x), exp2_fast(a.y)), q = make_float2(exp2_fast(b.x), exp2_fast(b.y));
-            const float2 e = mul2(p, add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
-            const float2 f = mul2(q, add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
-            s[c] = p.x, s[c + 1] = p.y, s[c + 2] = q.x, s[c + 3] = q.y;
-            d[c] = e.x, d[c + 1] = e.y, d[c + 2] = f.x, d[c + 3] = f.y;
-        }
-        if (mask) {
+            float p[4] = {exp2_fast(a.x), exp2_fast(a.y), exp2_fast(b.x), exp2_fast(b.y)};
+            const float2 e = mul2(make_float2(p[0], p[1]), add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
+            const float2 f =
+                mul2(make_float2(p[2], p[3]), add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
+            float ds[4] = {e.x, e.y, f.x, f.y};
+            if (masked) {
 #pragma unroll
-            for (int c = 0; c < kWalk; ++c) {
-                const bool seen = c >= lo && c < hi;
-                s[c] = seen ? s[c] : 0.0f;
-                const bool one = c >= one_lo && c < one_hi;
-                d[c] = seen ? one ? (DKV ? sh.one_ds[st][c] : row_od) : d[c] : 0.0f;
+                for (int k = 0; k < 4; ++k) {
+                    const bool seen = c + k >= lo && c + k < hi;
+                    const bool one = c + k >= one_lo && c + k < one_hi;
+                    p[k] = seen ? p[k] : 0.0f;
+                    ds[k] = seen ? one ? (DKV ? sh.one_ds[st][c + k] : row_od) : ds[k] : 0.0f;
+                }
             }
+            ps[c / 2] = pack_bf16(p[0], p[1]);
+            ps[c / 2 + 1] = pack_bf16(p[2], p[3]);
+            pd[c / 2] = pack_bf16(ds[0], ds[1]);
+            pd[c / 2 + 1] = pack_bf16(ds[2], ds[3]);
         }
-        uint32_t pk[32];
-        if (DKV) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) pk[c] = pack_bf16(s[2 * c], s[2 * c + 1]);
-            tmem_st32(ts, pk);
-        }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) pk[c] = pack_bf16(d[2 * c], d[2 * c + 1]);
-        tmem_st32(ts + kWalk, pk);
+        };
+        if (mask) weights(std::true_type{});
+        else weights(std::false_type{});
+        if (DKV) tmem_st32(ts, ps);
+        tmem_st32(ts + kWalk, pd);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         mbar_arrive_one(&sh.ds_ready[w]);
     }
-    if (r.steps > 0) wait_warp(&sh.acc_done, 0, abort);
+    if (r.steps > r.start) wait_warp(&sh.acc_done, 0, abort);
     tc_fence_after();
 }
 
@@ -1095,20 +1104,69 @@ __device__ __forceinline__ void store_acc(uint32_t addr, bool any, int from, int
 }
 
 // DKV: g0 = dK, g1 = dV.  Otherwise g0 = dQ.
+// Whole block: this block's accumulator columns into its shared memory (column-major: a warp's rows
+// are consecutive), then the cluster's sums of this block's share of the columns to memory.
+template <int DP, bool DKV>
+__device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t smem, int ranks, int rank, size_t row_at,
+                          bool live, bf16 *g0, bf16 *g1) {
+    constexpr int kAll = DKV ? 2 * DP : DP;
+    const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
+    if (w < 2) {
+        // Warpgroup 0 the first half of the columns, 1 the second.
+        for (int c = w * (kAll / 2); c < (w + 1) * (kAll / 2); c += 16) {
+            float o[16];
+            if (any) {
+                tmem_ld16(acc + c, o);
+                tmem_wait_ld();
+                pin<16>(o);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + ((c + e) * 128 + row) * 4), "f"(any ? o[e] : 0.0f)
+                             : "memory");
+        }
+    }
+    cluster_sync();
+    const int cols = kAll / ranks;
+    if (w < 2) {
+        for (int c = rank * cols + w * 8; c < (rank + 1) * cols; c += 16) {
+            float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            for (int k = 0; k < ranks; ++k) {
+                const uint32_t from = cluster_addr(smem + (c * 128 + row) * 4, k);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += cluster_ld(from + e * 512);
+            }
+            const bool second = DKV && c >= DP;
+            const int col = second ? c - DP : c;
+            if (live && col < A.D) {
+                const float f = second ? 1.0f : A.scale;
+                uint4 v;
+                v.x = pack_bf16(o[0] * f, o[1] * f);
+                v.y = pack_bf16(o[2] * f, o[3] * f);
+                v.z = pack_bf16(o[4] * f, o[5] * f);
+                v.w = pack_bf16(o[6] * f, o[7] * f);
+                *reinterpret_cast<uint4 *>((second ? g1 : g0) + row_at + col) = v;
+            }
+        }
+    }
+    cluster_sync();  // no block leaves while another reads its shared memory
+}
+
 template <int DP, bool DKV>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
 attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, const __grid_constant__ CUtensorMap mx1,
                      const __grid_constant__ CUtensorMap my0, const __grid_constant__ CUtensorMap my1,
                      const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ g_lse,
-                     bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots) {
+                     bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots, int ranks) {
     using S = BwdShape<DP>;
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(16) BwdShared sh;
     const int warp = warp_index();
     const int heads = DKV ? A.Hkv : A.Hkv * A.subs;
-    const int hx = blockIdx.x % heads;
+    const int rank = blockIdx.x % ranks, tile = blockIdx.x / ranks;
+    const int hx = tile % heads;
     // The tiles with most work under a causal mask first: the first keys, the last queries.
-    const int slot = DKV ? blockIdx.x / heads : slots - 1 - (int)(blockIdx.x / heads);
+    const int slot = DKV ? tile / heads : slots - 1 - tile / heads;
     const int per = DKV ? 128 : 128 / A.pack;
     const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, per, slot)
                        : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per, slot);
@@ -1133,6 +1191,10 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         const int sees = A.causal ? min(r.klen, max(0, r.q0 + r.qtok + r.klen - r.qlen)) : r.klen;
         r.steps = (sees + kWalk - 1) / kWalk;
     }
+    const int each = (r.steps + ranks - 1) / ranks;
+    r.start = min(r.steps, each * rank);
+    r.steps = min(r.steps, r.start + each);
+    const int steps = r.steps - r.start;
     const uint32_t smem_x = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t smem_y = smem_x + 2 * S::kXBytes;
 
@@ -1168,33 +1230,39 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
 
     int issued = 0;
-    if (warp == 8) {
-        if (r.steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, r.steps, tmem);
-    } else if (warp == 9) {
-        issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
+    const int row = threadIdx.x & 127;
+    const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + 4 * kWalk;
+    const bool live = DKV ? r.k0 + row < r.klen : row_token(A, row) < r.qtok;
+    const size_t row_at = DKV ? ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D
+                              : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
+    if (warp >= 8) {
+        regs_less<kLessRegs>();
+        if (warp == 8 && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem);
+        if (warp == 9) issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
     } else {
+        regs_more<kMoreRegs>();
         bwd_grads<DP, DKV>(A, sh, r, tmem, lse, delta, g_lse);
         __syncwarp();
-        const int w = warp >> 2, row = threadIdx.x & 127;
-        const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + 4 * kWalk;
-        const bool any = r.steps > 0;
-        if (DKV) {
-            const bool live = r.k0 + row < r.klen;
-            const size_t at = ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D;
-            if (w == 0) store_acc<DP>(acc, any, 0, DP, A.scale, g0 + at, A.D, live);
-            else store_acc<DP>(acc + DP, any, 0, DP, 1.0f, g1 + at, A.D, live);
-        } else {
-            const bool live = row_token(A, row) < r.qtok;
-            const size_t at =
-                ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
-            const int half = DP >= 64 ? DP / 2 : DP;  // columns of the first warpgroup
-            store_acc<DP>(acc, any, w * half, w == 0 ? half : DP, A.scale, g0 + at, A.D, live);
+        if (ranks == 1) {
+            const int w = warp >> 2;
+            if (DKV) {
+                if (w == 0) store_acc<DP>(acc, steps > 0, 0, DP, A.scale, g0 + row_at, A.D, live);
+                else store_acc<DP>(acc + DP, steps > 0, 0, DP, 1.0f, g1 + row_at, A.D, live);
+            } else {
+                const int half = DP >= 64 ? DP / 2 : DP;  // columns of the first warpgroup
+                store_acc<DP>(acc, steps > 0, w * half, w == 0 ? half : DP, A.scale, g0 + row_at, A.D, live);
+            }
         }
+    }
+    if (ranks > 1) {
+        // Every product of this block is done, so its shared memory is free.
+        __syncthreads();
+        share_acc<DP, DKV>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0 && r.steps > 0) {
+    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0 && steps > 0) {
         mbar_drain(&sh.x_full, 0, kAttnWaitLimit);
         for (int i = max(0, issued - S::kStages); i < issued; ++i)
             mbar_drain(&sh.y_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
@@ -1369,11 +1437,58 @@ int launch_forward(const AttnArgs &A, const ForwardPlan &plan, const Strided &q,
     return launch_status();
 }
 
+// Blocks that share a held tile's steps, in the kernel that holds keys and in the one that holds
+// queries.
+struct BackwardPlan {
+    int kv_ranks, q_ranks;
+};
+
+BackwardPlan plan_backward(const AttnArgs &A) {
+    const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
+    const long long rows = (A.Tq + n_seq - 1) / n_seq, keys = (A.Tk + n_seq - 1) / n_seq;  // of the mean sequence
+    const int per = 128 / A.pack;
+    auto ranks = [&](long long blocks, long long steps) {
+        int r = 1;
+        while (r < 4 && blocks * r < 2ll * num_sms() && steps >= 16 * r) r *= 2;
+        return r;
+    };
+    BackwardPlan p;
+    p.kv_ranks = ranks(n_seq * A.Hkv * ((keys + 127) / 128), rows * A.pack * A.subs / kWalk);
+    p.q_ranks = ranks(n_seq * A.Hkv * A.subs * ((rows + per - 1) / per), keys / kWalk);
+    const KnobValue forced = knob(kKnobAttnBwd);
+    auto valid = [](int r) { return r == 1 || r == 2 || r == 4; };
+    if (forced.count > 0 && valid(forced.v[0])) p.kv_ranks = forced.v[0];
+    if (forced.count > 1 && valid(forced.v[1])) p.q_ranks = forced.v[1];
+    return p;
+}
+
+template <int DP, bool DKV, typename... Args>
+int launch_backward_kernel(long long tiles, int ranks, cudaStream_t stream, Args... args) {
+    using S = BwdShape<DP>;
+    if (tiles * ranks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+    if (int st = allow_smem(attn_backward_kernel<DP, DKV>, S::kSmem)) return st;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(tiles * ranks));
+    config.blockDim = dim3(S::kThreads);
+    config.dynamicSmemBytes = S::kSmem;
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
+    config.attrs = &attr;
+    config.numAttrs = ranks > 1 ? 1 : 0;
+    if (cudaLaunchKernelEx(&config, attn_backward_kernel<DP, DKV>, args..., ranks) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return RFDETR_ERR_CUDA;
+    }
+    return RFDETR_OK;
+}
+
 template <int DP>
-int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
+int launch_backward(const AttnArgs &A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
                     const float *lse, const float *delta, const float *g_lse, bf16 *dq, bf16 *dk, bf16 *dv,
                     cudaStream_t stream) {
-    using S = BwdShape<DP>;
+    const BackwardPlan plan = plan_backward(A);
     CUtensorMap kx, vx, qy, gy, qx, gx, ky, vy;
     const int ytok = kWalk / A.pack, xtok = 128 / A.pack;
     if (!make_map(&kx, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) || !make_map(&vx, v, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
@@ -1383,21 +1498,17 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
         return RFDETR_ERR_CUDA;
     if (A.Tk > 0) {
         const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
-        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-        if (int st = allow_smem(attn_backward_kernel<DP, true>, S::kSmem)) return st;
-        attn_backward_kernel<DP, true>
-            <<<(unsigned)blocks, S::kThreads, S::kSmem, stream>>>(A, kx, vx, qy, gy, lse, delta, g_lse, dk, dv,
-                                                                  (int)slots);
-        if (int st = launch_status()) return st;
+        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, stream, A, kx, vx, qy, gy, lse, delta,
+                                                      g_lse, dk, dv, (int)slots))
+            return st;
     }
     if (A.Tq > 0) {
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
-        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-        if (int st = allow_smem(attn_backward_kernel<DP, false>, S::kSmem)) return st;
-        attn_backward_kernel<DP, false><<<(unsigned)blocks, S::kThreads, S::kSmem, stream>>>(
-            A, qx, gx, ky, vy, lse, delta, g_lse, dq, nullptr, (int)slots);
+        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, stream, A, qx, gx, ky, vy, lse, delta,
+                                                       g_lse, dq, nullptr, (int)slots))
+            return st;
     }
-    return launch_status();
+    return RFDETR_OK;
 }
 
 AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, int64_t Tq, int64_t Tk, int64_t Hq,

@@ -116,6 +116,7 @@ enum Knob {
     kKnobTopkSort,      // "RFDETR_TOPK_SORT": any value selects the one-CTA sort kernels
     kKnobTopkUnstaged,  // "RFDETR_TOPK_UNSTAGED": any value keeps the radix select's keys out of shared memory
     kKnobAttnFwd,       // "RFDETR_ATTN_FWD": packed attention forward (1 long or 2 short kernel, key splits of the long one)
+    kKnobAttnBwd,       // "RFDETR_ATTN_BWD": packed attention backward (blocks sharing a tile of keys, of queries: 1, 2, 4)
     kKnobCount
 };
 struct KnobValue {

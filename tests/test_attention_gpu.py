@@ -323,6 +323,16 @@ def test_every_forward_kernel(pkg, tuning, knob, dim):
     _check(pkg, (130, 5), (30, 1000), heads=2, kv=2, dim=dim, causal=True, seed=dim)
 
 
+@pytest.mark.parametrize("knob", ["1,1", "2,4", "4,2"])
+@pytest.mark.parametrize("dim", [32, 64, 80, 128])
+def test_every_backward_split(pkg, tuning, knob, dim):
+    """Tiles shared by a cluster of blocks, some of them left without a step."""
+    tuning("RFDETR_ATTN_BWD", knob)
+    _check(pkg, (1, 300, 0, 517, 64), heads=6, kv=2, dim=dim, causal=True, seed=dim)
+    _check(pkg, (3, 130, 40, 7), (900, 0, 17, 129), heads=4, kv=1, dim=dim, seed=dim)
+    _check(pkg, (130, 5), (30, 1000), heads=2, kv=2, dim=dim, causal=True, seed=dim, with_lse_grad=True)
+
+
 def test_one_token_over_long_keys(pkg):
     """The form for single tokens: the keys are split over blocks."""
     N = pkg._native
