@@ -148,15 +148,17 @@ template <int DP> __device__ __forceinline__ unsigned box_bytes(int rows) {
 // ---------------------------------------------------------------------------------------------
 constexpr float kLazy = 8.0f;
 
-// The largest of m and 32 values.
-__device__ __forceinline__ float max32(const float *s, float m) {
-    float a = m, b = -INFINITY;
+// The largest of N values.
+template <int N> __device__ __forceinline__ float max_of(const float *s) {
+    float a[4];
 #pragma unroll
-    for (int c = 0; c < 32; c += 4) {
-        a = fmaxf(fmaxf(a, s[c]), s[c + 1]);
-        b = fmaxf(fmaxf(b, s[c + 2]), s[c + 3]);
+    for (int c = 0; c < 4; ++c) a[c] = fmaxf(s[c], s[c + 4]);
+#pragma unroll
+    for (int c = 8; c < N; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = fmaxf(fmaxf(a[e], s[c + e]), s[c + e + 4]);
     }
-    return fmaxf(a, b);
+    return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
 // A row's softmax so far: P and sum are relative to exp2(m scale log2(e)).
@@ -164,27 +166,46 @@ struct RowState {
     float m, sum;
 };
 
-// Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P in place; `to` is O, which
-// must hold the products of all tiles before.  `cols` columns are in use, of which this row sees
-// `seen` where `mask` is set.
-template <int DP, int KEYS>
-__device__ __forceinline__ void softmax_tile(RowState &r, uint32_t ts, uint32_t to, int cols, bool mask, int seen,
-                                             bool first, float sc) {
-    constexpr int NC = KEYS / 32;
+// 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY three pairs of
+// eight take the FMA pipe: 128 values per row then cost about 5 cycles each instead of 9.
+template <int N, bool POLY>
+__device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
+    const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
+#pragma unroll
+    for (int c = 0; c < N / 2; ++c) {
+        float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), sc2, ref2);
+        if (POLY && (c % 8 == 4)) {
+            x = exp2_poly(x);
+        } else {
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
+        }
+        acc[c & 1] = add2(acc[c & 1], x);
+        p[c] = pack_bf16(x.x, x.y);
+    }
+}
+
+// Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
+// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
+// loaded() is called once S is in registers, settle() before P is written or O touched (it returns
+// false to give up), written(half) after each half of P.
+template <int DP, int KEYS, typename Loaded, typename Settle, typename Written>
+__device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
+                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
+                                             Written written) {
     float s[KEYS];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-        if (c * 32 < cols) tmem_ld32(ts + c * 32, s + c * 32);
+    for (int c = 0; c < KEYS; c += 32)
+        if (c < cols) tmem_ld32(ts + c, s + c);
     tmem_wait_ld();
     pin<KEYS>(s);
-    if (mask) {
+    loaded();
+    if (!all) {
 #pragma unroll
         for (int c = 0; c < KEYS; ++c) s[c] = c < seen ? s[c] : -INFINITY;
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-        if (c * 32 < cols) mx = max32(s + c * 32, mx);
+    const float mx = max_of<KEYS>(s);
+    if (!settle()) return false;
     if (first) {
         r.m = mx;
     } else if (__any_sync(0xffffffffu, mx * sc > r.m * sc + kLazy)) {
@@ -193,36 +214,45 @@ __device__ __forceinline__ void softmax_tile(RowState &r, uint32_t ts, uint32_t 
         r.m = to_m;
         r.sum *= f;
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-            float o[32];
-            tmem_ld32(to + c * 32, o);
+        for (int c = 0; c < DP; c += 16) {
+            float o[16];
+            tmem_ld16(to + c, o);
             tmem_wait_ld();
-            pin<32>(o);
+            pin<16>(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_st32(to + c * 32, reinterpret_cast<uint32_t *>(o));
+            for (int e = 0; e < 16; ++e) o[e] *= f;
+            tmem_st16(to + c, reinterpret_cast<uint32_t *>(o));
         }
     }
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
-    const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
-    float2 acc = make_float2(0.0f, 0.0f), acc1 = make_float2(0.0f, 0.0f);
+    float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    if (all) {
 #pragma unroll
-    for (int h = 0; h < NC; ++h) {
-        if (h * 32 >= cols) break;
-        uint32_t p[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            float2 x = fma2(make_float2(s[h * 32 + 2 * c], s[h * 32 + 2 * c + 1]), sc2, ref2);
-            x.x = exp2_fast(x.x);
-            x.y = exp2_fast(x.y);
-            if (c & 1) acc1 = add2(acc1, x);
-            else acc = add2(acc, x);
-            p[c] = pack_bf16(x.x, x.y);
+        for (int h = 0; h < 2; ++h) {
+            uint32_t p[KEYS / 4];
+            exp_pack<KEYS / 2, true>(s + h * (KEYS / 2), sc, ref, p, acc);
+            if (KEYS == 128) tmem_st32(tp + h * 32, p);
+            else tmem_st16(tp + h * 16, p);
+            tmem_wait_st();
+            written(h);
         }
-        tmem_st16(ts + h * 16, p);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < KEYS / 2; c += 32) {
+                uint32_t p[16];
+                if (h * (KEYS / 2) + c < cols) {
+                    exp_pack<32, false>(s + h * (KEYS / 2) + c, sc, ref, p, acc);
+                    tmem_st16(tp + h * (KEYS / 4) + c / 2, p);
+                }
+            }
+            tmem_wait_st();
+            written(h);
+        }
     }
-    r.sum += (acc.x + acc.y) + (acc1.x + acc1.y);
-    tmem_wait_st();
+    r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+    return true;
 }
 
 // Whole warp: a row's result from O (or zeros) and its log-sum-exp.
@@ -287,9 +317,14 @@ template <int DP> struct LongShape {
     static constexpr int kThreads = 384;
     static constexpr int kTmem = 512;
     static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
+    // TMEM: S of both tiles (2 x 128), O of both (2 x DP), and P (2 x 64) where there is room for it;
+    // with 128 channels there is none and P lies over S.  P of its own lets the next S be formed while
+    // this one's exponentials run.
+    static constexpr bool kOwnP = DP <= 64;
+    static constexpr int kO = 256, kP = kOwnP ? 256 + 2 * DP : 0, kPStep = kOwnP ? 64 : 128;
 };
 struct LongShared {
-    uint64_t q_full[2], kv_full[4], kv_raw, kv_empty[4], s_full[2], p_ready[2], o_done[2], drain;
+    uint64_t q_full[2], kv_full[4], kv_raw, kv_empty[4], s_full[2], s_free[2], p_half[2][2], o_done[2], drain;
     uint32_t tmem;
     int abort;
 };
@@ -399,33 +434,55 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
         scores(t, st, r.j0);
     }
     tc_commit_one(&sh.kv_empty[st]);
+    // O_t += P V of tile i, each half as soon as it is written.
+    auto product = [&](int t, int i, int sv) {
+        const int steps = tile_cols(r.sees[t], (r.j0 + i) * S::kKeys, S::kKeys) / 16;
+        const uint64_t b = v_desc + sv * (S::kTileBytes / 16);
+        const uint32_t o = tmem + S::kO + t * DP, p = tmem + S::kP + t * S::kPStep;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!wait_warp(&sh.p_half[t][h], i & 1, abort)) return false;
+            tc_fence_after();
+            if (steps == 8) {
+#pragma unroll
+                for (int k = h * 4; k < h * 4 + 4; ++k)
+                    mma_ts_one(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+            } else {
+                for (int k = h * 4; k < min(steps, h * 4 + 4); ++k)
+                    mma_ts_one(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+            }
+        }
+        tc_commit_one(&sh.o_done[t]);
+        return true;
+    };
     for (int i = 0; i < n; ++i) {
         int sv = -1, sk = -1;
+        if (S::kOwnP) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (r.n[t] - r.j0 - i <= 1) continue;
+                if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
+                if (!wait_warp(&sh.s_free[t], i & 1, abort)) return false;
+                tc_fence_after();
+                scores(t, sk, r.j0 + i + 1);
+            }
+            if (sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
             if (left > 0) {
                 if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
-                if (!wait_warp(&sh.p_ready[t], i & 1, abort)) return false;
-                tc_fence_after();
-                const int steps = tile_cols(r.sees[t], (r.j0 + i) * S::kKeys, S::kKeys) / 16;
-                const uint64_t b = v_desc + sv * (S::kTileBytes / 16);
-#pragma unroll
-                for (int k = 0; k < S::kKeys / 16; ++k)
-                    if (k < steps)
-                        mma_ts_one(tmem + 256 + t * DP, tmem + t * 128 + k * 8, b + k * TL::kRowBytes, kIdO,
-                                   i > 0 || k > 0);
-                if (left == 1) tc_commit_one(&sh.o_done[t]);
+                if (!product(t, i, sv)) return false;
             }
-            if (left > 1) {
+            if (!S::kOwnP && left > 1) {
                 if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
                 tc_fence_after();
-                // In issue order after the product above, so its commit tells of that product too.
                 scores(t, sk, r.j0 + i + 1);
             }
         }
         if (sv >= 0) tc_commit_one(&sh.kv_empty[sv]);
-        if (sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
+        if (!S::kOwnP && sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
     }
     return true;
 }
@@ -477,7 +534,9 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             for (int t = 0; t < 2; ++t) {
                 mbar_init(&sh.q_full[t], 1);
                 mbar_init(&sh.s_full[t], 1);
-                mbar_init(&sh.p_ready[t], 4);
+                mbar_init(&sh.s_free[t], 4);
+                mbar_init(&sh.p_half[t][0], 4);
+                mbar_init(&sh.p_half[t][1], 4);
                 mbar_init(&sh.o_done[t], 1);
             }
             for (int i = 0; i < S::kStages; ++i) {
@@ -514,7 +573,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
         if (r.tok[t] > 0) {
             volatile int *abort = &sh.abort;
             const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lane 32 (w % 4)
-            const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + 256 + t * DP;
+            const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + S::kO + t * DP;
+            const uint32_t tp = tmem + lane_base + S::kP + t * S::kPStep;
             const int row = threadIdx.x & 127;
             const int tok_first = q.first + t * per, tok = tok_first + row_token(A, row);
             const bool live = row_token(A, row) < r.tok[t];
@@ -530,14 +590,35 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 if (!ok) break;
                 tc_fence_after();
                 const int k0 = (r.j0 + i) * S::kKeys;
-                if (warp_live)
-                    softmax_tile<DP, S::kKeys>(rs, ts, to, tile_cols(r.sees[t], k0, S::kKeys), k0 + S::kKeys > all_see,
-                                               limit - k0, i == 0, A.scale_log2);
-                tc_fence_before();
-                __syncwarp();
-                mbar_arrive_one(&sh.p_ready[t]);
+                auto loaded = [&] {
+                    if (!S::kOwnP) return;
+                    tc_fence_before();
+                    mbar_arrive_one(&sh.s_free[t]);
+                };
+                // P V of the tile before: done with S of this one where P lies over S (issue order).
+                auto settle = [&] {
+                    if (!S::kOwnP || i == 0) return true;
+                    if (!wait_warp(&sh.o_done[t], (i - 1) & 1, abort)) return false;
+                    tc_fence_after();
+                    return true;
+                };
+                auto written = [&](int h) {
+                    tc_fence_before();
+                    __syncwarp();
+                    mbar_arrive_one(&sh.p_half[t][h]);
+                };
+                if (warp_live) {
+                    ok = softmax_tile<DP, S::kKeys>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
+                                                    k0 + S::kKeys <= all_see, limit - k0, i == 0, A.scale_log2, loaded,
+                                                    settle, written);
+                } else {
+                    loaded();
+                    ok = settle();
+                    written(0);
+                    written(1);
+                }
             }
-            if (ok && n > 0) ok = wait_warp(&sh.o_done[t], 0, abort);
+            if (ok && n > 0) ok = wait_warp(&sh.o_done[t], (n - 1) & 1, abort);
             tc_fence_after();
             if (ok)
                 write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse, part,
@@ -694,8 +775,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         }
         const int k0 = i * KEYS;
         if (warp_live)
-            softmax_tile<DP, KEYS>(rs, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS > all_see, limit - k0, i == 0,
-                                   A.scale_log2);
+            softmax_tile<DP, KEYS>(rs, ts, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
+                                   A.scale_log2, [] {}, [] { return true; }, [](int) {});
         // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
         if (k0 + KEYS > klen) {
             ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort) && ok;
@@ -711,10 +792,14 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             if (ok) {
                 const int steps = tile_cols(sees, k0, KEYS) / 16;
                 const uint64_t b = v_desc + (i & 1) * (S::kTileBytes / 16);
+                if (steps == KEYS / 16) {
 #pragma unroll
-                for (int k = 0; k < KEYS / 16; ++k)
-                    if (k < steps)
+                    for (int k = 0; k < KEYS / 16; ++k)
                         mma_ts_one(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                } else {
+                    for (int k = 0; k < steps; ++k)
+                        mma_ts_one(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                }
                 if (i + 1 < n) ok = scores(i + 1);
                 else tc_commit_one(&sh.o_done);
             }

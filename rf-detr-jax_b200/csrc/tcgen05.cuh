@@ -225,6 +225,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^x of a pair on the FMA pipe, for sharing exponentials between it and the special-function unit
+// (which takes 8 cycles of an SM quarter for a warp's exponentials, the other pipes idle).  x is
+// split into its nearest integer n and a rest f in [-1/2, 1/2]; 2^f is a polynomial of degree 5 fitted
+// by Lawson's reweighted least squares to the least relative error (2.4e-7 in float32 with the
+// rounding of its steps, as ex2.approx), and n is added to its exponent field.  Below 2^-126 the
+// result stays 2^-126; a NaN does not come out finite and small.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    const float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    const float2 t = add2(x, make_float2(kMagic, kMagic));
+    const float2 n = add2(t, make_float2(-kMagic, -kMagic));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 p = make_float2(0.0013276472454890609f, 0.0013276472454890609f);
+    p = fma2(p, f, make_float2(0.009675541892647743f, 0.009675541892647743f));
+    p = fma2(p, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+    p = fma2(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+    p = fma2(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+    p = fma2(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+    return p;
+}
 // Two bf16 (round to nearest even) in one register, `lo` in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
