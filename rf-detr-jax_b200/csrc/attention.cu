@@ -114,6 +114,15 @@ __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (i
 constexpr int kLaunchRegs = 168, kMoreRegs = 208, kLessRegs = 88;
 static_assert(2 * kMoreRegs + kLessRegs <= 3 * kLaunchRegs, "a warpgroup would wait for registers for good");
 
+// D = A B^T over DP channels, A and B K-major tiles whose column panels are `a_panel` and `b_panel` bytes.
+template <int DP, int A_PANEL, int B_PANEL>
+__device__ __forceinline__ void mma_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    constexpr int N = Tile<DP>::kCols / 16;  // steps in a panel
+#pragma unroll
+    for (int p = 0; p < Tile<DP>::kPanels; ++p)
+        mma_ss_one<N, 2, 2>(d, a + p * (A_PANEL / 16), b + p * (B_PANEL / 16), idesc, p > 0);
+}
+
 // Zeroes rows [from, to) of a swizzled tile by the first `threads` threads of a block or a warp's
 // lanes (32); whole rows, so the swizzle does not matter.
 template <int DP>
@@ -413,11 +422,7 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
     auto scores = [&](int t, int st, int j) {
         const uint32_t id = mma_idesc(128, tile_cols(r.sees[t], j * S::kKeys, S::kKeys), false);
         const uint64_t a = q_desc + t * (S::kTileBytes / 16), b = k_desc + st * (S::kTileBytes / 16);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t o = ((k * 32 / TL::kRowBytes) * kLbo + (k * 32) % TL::kRowBytes) / 16;
-            mma_ss_one(tmem + t * 128, a + o, b + o, id, k > 0);
-        }
+        mma_channels<DP, kLbo, kLbo>(tmem + t * 128, a, b, id);
         tc_commit_one(&sh.s_full[t]);
     };
     auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
@@ -444,12 +449,11 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
             if (!wait_warp(&sh.p_half[t][h], i & 1, abort)) return false;
             tc_fence_after();
             if (steps == 8) {
-#pragma unroll
-                for (int k = h * 4; k < h * 4 + 4; ++k)
-                    mma_ts_one(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                mma_ts_one<4, TL::kRowBytes>(o, p + h * 32, b + h * 4 * TL::kRowBytes, kIdO, i > 0 || h > 0);
             } else {
+#pragma unroll 1
                 for (int k = h * 4; k < min(steps, h * 4 + 4); ++k)
-                    mma_ts_one(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                    mma_ts_one<1, 0>(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
             }
         }
         tc_commit_one(&sh.o_done[t]);
@@ -730,12 +734,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         if (!wait_warp(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t id = mma_idesc(128, tile_cols(sees, j * KEYS, KEYS), false);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
-            mma_ss_one(tmem, q_desc + (panel * kQPanel + in) / 16,
-                       k_desc + ((j & 1) * S::kTileBytes + panel * kPanel + in) / 16, id, k > 0);
-        }
+        mma_channels<DP, kQPanel, kPanel>(tmem, q_desc, k_desc + (j & 1) * (S::kTileBytes / 16), id);
         tc_commit_one(&sh.s_full);
         return true;
     };
@@ -792,13 +791,13 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             if (ok) {
                 const int steps = tile_cols(sees, k0, KEYS) / 16;
                 const uint64_t b = v_desc + (i & 1) * (S::kTileBytes / 16);
-                if (steps == KEYS / 16) {
-#pragma unroll
-                    for (int k = 0; k < KEYS / 16; ++k)
-                        mma_ts_one(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                static_assert(KEYS == 64, "four steps");
+                if (steps == 4) {
+                    mma_ts_one<4, TL::kRowBytes>(tmem + KEYS, tmem, b, kIdO, i > 0);
                 } else {
+#pragma unroll 1
                     for (int k = 0; k < steps; ++k)
-                        mma_ts_one(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                        mma_ts_one<1, 0>(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
                 }
                 if (i + 1 < n) ok = scores(i + 1);
                 else tc_commit_one(&sh.o_done);
@@ -1015,13 +1014,8 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         const uint64_t y = y_desc + st * (2 * S::kYBytes / 16);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t panel = k * 32 / TL::kRowBytes, in = (k * 32) % TL::kRowBytes;
-                mma_ss_one(tmem + (i & 1) * 2 * kWalk + which * kWalk,
-                           x_desc + (which * S::kXBytes + panel * kXPanel + in) / 16,
-                           y + (which * S::kYBytes + panel * kYPanel + in) / 16, kIdS, k > 0);
-            }
+            mma_channels<DP, kXPanel, kYPanel>(tmem + (i & 1) * 2 * kWalk + which * kWalk,
+                                               x_desc + which * (S::kXBytes / 16), y + which * (S::kYBytes / 16), kIdS);
         tc_commit_one(&sh.s_full[i & 1]);
         return true;
     };
@@ -1033,14 +1027,11 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         const uint64_t y = yt_desc + st * (2 * S::kYBytes / 16);
         if (!wait_warp(&sh.ds_ready[i & 1], (i >> 1) & 1, abort)) return false;
         tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < kWalk / 16; ++k) {
-            if (DKV)
-                mma_ts_one(tmem + 4 * kWalk + DP, tmem + (i & 1) * 2 * kWalk + k * 8,
-                           y + S::kYBytes / 16 + k * TL::kRowBytes, kIdAcc, i > 0 || k > 0);
-            mma_ts_one(tmem + 4 * kWalk, tmem + (i & 1) * 2 * kWalk + kWalk + k * 8, y + k * TL::kRowBytes, kIdAcc,
-                       i > 0 || k > 0);
-        }
+        static_assert(kWalk == 64, "four steps");
+        const uint32_t p = tmem + (i & 1) * 2 * kWalk;
+        if (DKV)
+            mma_ts_one<4, TL::kRowBytes>(tmem + 4 * kWalk + DP, p, y + S::kYBytes / 16, kIdAcc, i > 0);
+        mma_ts_one<4, TL::kRowBytes>(tmem + 4 * kWalk, p + kWalk, y, kIdAcc, i > 0);
         tc_commit_one(&sh.y_empty[st]);
         if (i + 2 < steps && !scores(i + 2)) return false;
     }

@@ -105,29 +105,54 @@ __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool b_mn_major) 
            ((uint32_t)(m >> 4) << 24);
 }
 
-// D[tmem] (+)= A[smem] B[smem]; one step of 16 along the contraction.
+// N steps of 16 along the contraction, D[tmem] (+)= A B, the first adding to D where `accumulate` is set:
+// A from shared memory (ss, descriptors AS and BS apart from step to step) or from TMEM (ts, two bf16 to a
+// column, 8 columns a step), B from shared memory.  One block of code, so that a step is little more than the
+// instruction itself: this warp shares its SM quarter, and the instruction cache of that, with warps whose
+// unrolled code is larger than it.
+template <int N, int AS, int BS>
 __device__ __forceinline__ void mma_ss_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p, q;\n"
-        "elect.sync _|q, 0xffffffff;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
+    static_assert(N == 2 || N == 4, "steps");
+    if constexpr (N == 2) {
+        asm volatile(
+            "{\n.reg .pred p, q, t;\n.reg .b64 a, b;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+            "setp.eq.b32 t, 0, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\nadd.s64 a, %1, %5;\nadd.s64 b, %2, %6;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(AS), "n"(BS)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred p, q, t;\n.reg .b64 a, b;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+            "setp.eq.b32 t, 0, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\nadd.s64 a, %1, %5;\nadd.s64 b, %2, %6;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\nadd.s64 a, a, %5;\nadd.s64 b, b, %6;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\nadd.s64 a, a, %5;\nadd.s64 b, b, %6;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(AS), "n"(BS)
+            : "memory");
+    }
 }
-// D[tmem] (+)= A[tmem] B[smem]; A holds two bf16 per column, 8 columns per step.
+template <int N, int BS>
 __device__ __forceinline__ void mma_ts_one(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p, q;\n"
-        "elect.sync _|q, 0xffffffff;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
+    static_assert(N == 1 || N == 4, "steps");
+    if constexpr (N == 1) {
+        asm volatile(
+            "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred p, q, t;\n.reg .b64 b;\n.reg .b32 a;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+            "setp.eq.b32 t, 0, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\nadd.s32 a, %1, 8;\nadd.s64 b, %2, %5;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\nadd.s32 a, a, 8;\nadd.s64 b, b, %5;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\nadd.s32 a, a, 8;\nadd.s64 b, b, %5;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(BS)
+            : "memory");
+    }
 }
 
 // ---- TMEM <-> registers: 32 consecutive columns of this thread's lane (whole warp) ----
