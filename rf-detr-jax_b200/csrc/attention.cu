@@ -100,10 +100,19 @@ inline long long slots_for(long long T, long long R, long long n_seq) { return T
 // Polls of a wait before the block gives up.  Every wait here is for work of the same block.
 constexpr int kAttnWaitLimit = 1 << 21;
 
-// A whole warp's wait: all of its lanes go on, or none (tensor memory is moved by warps).
+// A whole warp's wait: all of its lanes go on, or none (tensor memory is moved by warps).  Written to
+// be small: the kernels' loops have to stay in the instruction cache.
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volatile int *abort) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kAttnWaitLimit));
+    int left = kAttnWaitLimit;
+#pragma unroll 1
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        if (__any_sync(0xffffffffu, *abort || --left == 0)) {
+            *abort = 1;
+            atomicOr(&g_device_fault, 1u);
+            return false;
+        }
+    }
+    return true;
 }
 
 // The warp's index as a value that the compiler knows to be the same in all lanes.
@@ -129,8 +138,10 @@ template <int DP>
 __device__ __forceinline__ void zero_rows(uint32_t tile, int rows_in_panel, int from, int to, int threads) {
     constexpr int CH = Tile<DP>::kRowBytes / 16;
     const int n = (to - from) * CH;
+#pragma unroll 1
     for (int p = 0; p < Tile<DP>::kPanels; ++p) {
         const uint32_t a = tile + p * rows_in_panel * Tile<DP>::kRowBytes + from * Tile<DP>::kRowBytes;
+#pragma unroll 1
         for (int i = threadIdx.x & (threads - 1); i < n; i += threads)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a + i * 16), "r"(0) : "memory");
     }
@@ -194,27 +205,10 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
     }
 }
 
-// Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
-// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
-// loaded() is called once S is in registers, settle() before P is written or O touched (it returns
-// false to give up), written(half) after each half of P.
-template <int DP, int KEYS, typename Loaded, typename Settle, typename Written>
-__device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
-                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
-                                             Written written) {
-    float s[KEYS];
-#pragma unroll
-    for (int c = 0; c < KEYS; c += 32)
-        if (c < cols) tmem_ld32(ts + c, s + c);
-    tmem_wait_ld();
-    pin<KEYS>(s);
-    loaded();
-    if (!all) {
-#pragma unroll
-        for (int c = 0; c < KEYS; ++c) s[c] = c < seen ? s[c] : -INFINITY;
-    }
-    const float mx = max_of<KEYS>(s);
-    if (!settle()) return false;
+// Whole warp: moves the reference to the new maximum where some row's grew far enough, and O and the
+// sum with it.
+template <int DP> __device__ __forceinline__ void move_reference(RowState &r, uint32_t to, float mx, bool first,
+                                                                 float sc) {
     if (first) {
         r.m = mx;
     } else if (__any_sync(0xffffffffu, mx * sc > r.m * sc + kLazy)) {
@@ -233,9 +227,30 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
             tmem_st16(to + c, reinterpret_cast<uint32_t *>(o));
         }
     }
-    const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
+}
+
+// Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
+// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
+// loaded() is called once S has been read, settle() before P is written or O touched (it returns
+// false to give up), written(half) after each half of P.
+// Tiles that are seen whole, the many, are read once into registers and run straight through; the
+// others go over S twice in a small loop.
+template <int DP, int KEYS, typename Loaded, typename Settle, typename Written>
+__device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
+                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
+                                             Written written) {
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     if (all) {
+        float s[KEYS];
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 32) tmem_ld32(ts + c, s + c);
+        tmem_wait_ld();
+        pin<KEYS>(s);
+        loaded();
+        const float mx = max_of<KEYS>(s);
+        if (!settle()) return false;
+        move_reference<DP>(r, to, mx, first, sc);
+        const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t p[KEYS / 4];
@@ -246,19 +261,35 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
             written(h);
         }
     } else {
+        float mx = -INFINITY;
+        float s[32];
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+            tmem_ld32(ts + c, s);
+            tmem_wait_ld();
+            pin<32>(s);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int c = 0; c < KEYS / 2; c += 32) {
-                uint32_t p[16];
-                if (h * (KEYS / 2) + c < cols) {
-                    exp_pack<32, false>(s + h * (KEYS / 2) + c, sc, ref, p, acc);
-                    tmem_st16(tp + h * (KEYS / 4) + c / 2, p);
-                }
-            }
-            tmem_wait_st();
-            written(h);
+            for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
+        if (!settle()) return false;
+        move_reference<DP>(r, to, mx, first, sc);
+        const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
+        // P of 32 keys takes 16 columns: over S it stays behind what has been read.
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+            tmem_ld32(ts + c, s);
+            tmem_wait_ld();
+            pin<32>(s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = c + e < seen ? s[e] : -INFINITY;
+            uint32_t p[16];
+            exp_pack<32, false>(s, sc, ref, p, acc);
+            tmem_st16(tp + c / 2, p);
+        }
+        tmem_wait_st();
+        loaded();
+        written(0);
+        written(1);
     }
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
     return true;
@@ -276,7 +307,7 @@ __device__ __forceinline__ void write_row(const AttnArgs &A, const RowState &r, 
         else if (lse) lse[(size_t)head * A.Tq + token] = l;
     }
     const size_t at = (token * A.Hq + head) * A.D;
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < DP / 32; ++c) {
         float o[32];
         if (any) {
@@ -358,6 +389,7 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
     const int loads = 2 * (r.nmax - r.j0);
     int issued = 0;
     unsigned raw_phase = 0;
+#pragma unroll 1
     for (; issued < loads; ++issued) {
         const int st = issued % S::kStages;
         if (issued >= S::kStages && !wait_warp(&sh.kv_empty[st], ((issued / S::kStages) - 1) & 1, abort)) break;
@@ -459,6 +491,7 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
         tc_commit_one(&sh.o_done[t]);
         return true;
     };
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
         int sv = -1, sk = -1;
         if (S::kOwnP) {
@@ -589,6 +622,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             RowState rs{-INFINITY, 0.0f};
             const int n = r.n[t] - r.j0;
             bool ok = true;
+#pragma unroll 1
             for (int i = 0; i < n && ok; ++i) {
                 ok = wait_warp(&sh.s_full[t], i & 1, abort);
                 if (!ok) break;
@@ -763,6 +797,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     const int all_see = A.causal ? min(klen, q.first + 1 + klen - q.len) : klen;
     RowState rs{-INFINITY, 0.0f};
     bool gave_up = false;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
         ok = wait_warp(&sh.s_full, i & 1, abort) && ok;
         tc_fence_after();
@@ -843,6 +878,7 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
     const int head = (int)(row % Hq);
     const float *pl = part_lse + (size_t)head * Tq + token;
     float top = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) top = fmaxf(top, pl[(size_t)s * rows]);
     float total = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int s = 0; s < splits; ++s) {
@@ -941,6 +977,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
     const int yrows = DKV ? r.tok * A.pack : kWalk;
     unsigned raw_phase = 0;
     int i = 0;
+#pragma unroll 1
     for (; i < r.steps - r.start; ++i) {
         const int st = i % S::kStages;
         if (i >= S::kStages && !wait_warp(&sh.y_empty[st], ((i / S::kStages) - 1) & 1, abort)) break;
@@ -1022,6 +1059,7 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
     if (!wait_warp(&sh.x_full, 0, abort)) return false;
     if (!scores(0)) return false;
     if (steps > 1 && !scores(1)) return false;
+#pragma unroll 1
     for (int i = 0; i < steps; ++i) {
         const int st = i % S::kStages;
         const uint64_t y = yt_desc + st * (2 * S::kYBytes / 16);
@@ -1063,6 +1101,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     }
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
+#pragma unroll 1
     for (int i = w; i < r.steps - r.start; i += 2) {
         const int st = i % S::kStages;
         if (!wait_warp(&sh.s_full[w], (i >> 1) & 1, abort)) return;
@@ -1155,6 +1194,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
 template <int DP>
 __device__ __forceinline__ void store_acc(uint32_t addr, bool any, int from, int to, float scale, bf16 *dst, int D,
                                           bool live) {
+#pragma unroll 1
     for (int c = from; c < to; c += 32) {
         float o[32];
         if (any) {
@@ -1189,6 +1229,7 @@ __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t sm
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
     if (w < 2) {
         // Warpgroup 0 the first half of the columns, 1 the second.
+#pragma unroll 1
         for (int c = w * (kAll / 2); c < (w + 1) * (kAll / 2); c += 16) {
             float o[16];
             if (any) {
@@ -1205,8 +1246,10 @@ __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t sm
     cluster_sync();
     const int cols = kAll / ranks;
     if (w < 2) {
+#pragma unroll 1
         for (int c = rank * cols + w * 8; c < (rank + 1) * cols; c += 16) {
             float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
             for (int k = 0; k < ranks; ++k) {
                 const uint32_t from = cluster_addr(smem + (c * 128 + row) * 4, k);
 #pragma unroll
