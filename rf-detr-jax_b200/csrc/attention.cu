@@ -118,10 +118,12 @@ __device__ __forceinline__ bool wait_warp(uint64_t *bar, unsigned parity, volati
 // The warp's index as a value that the compiler knows to be the same in all lanes.
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
-// Blocks of three warpgroups, two of which compute: registers at launch 65536 / 384 -> 168, then
-// 2 x 208 + 88 = 3 x 168.
-constexpr int kLaunchRegs = 168, kMoreRegs = 208, kLessRegs = 88;
-static_assert(2 * kMoreRegs + kLessRegs <= 3 * kLaunchRegs, "a warpgroup would wait for registers for good");
+// Registers of a block's warpgroups: `GROUPS` that compute and one that loads and issues.  A launch gives
+// each thread LAUNCH; the last warpgroup's give theirs up to LESS and the others take MORE.
+template <int GROUPS, int LAUNCH, int MORE, int LESS> struct Registers {
+    static constexpr int kMore = MORE, kLess = LESS;
+    static_assert(GROUPS * MORE + LESS <= (GROUPS + 1) * LAUNCH, "a warpgroup would wait for registers for good");
+};
 
 // D = A B^T over DP channels, A and B K-major tiles whose column panels are `a_panel` and `b_panel` bytes.
 template <int DP, int A_PANEL, int B_PANEL>
@@ -355,6 +357,7 @@ template <int DP> struct LongShape {
     static constexpr int kTileBytes = 128 * DP * 2;
     static constexpr int kStages = 4;
     static constexpr int kThreads = 384;
+    using Regs = Registers<2, 168, 208, 88>;  // 65536 / 384 -> 168
     static constexpr int kTmem = 512;
     static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
     // TMEM: S of both tiles (2 x 128), O of both (2 x DP), and P (2 x 64) where there is room for it;
@@ -597,7 +600,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
 
     int issued = 0;
     if (warp >= 8) {
-        regs_less<kLessRegs>();
+        regs_less<S::Regs::kLess>();
         if (warp == 8) {
             if (r.nmax > r.j0) long_mma_loop<DP>(sh, smem_q, smem_kv, r, tmem);
         } else if (warp == 9) {
@@ -605,7 +608,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                                    klen);
         }
     } else {
-        regs_more<kMoreRegs>();
+        regs_more<S::Regs::kMore>();
         const int t = warp >> 2;
         if (r.tok[t] > 0) {
             volatile int *abort = &sh.abort;
@@ -912,9 +915,11 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
 // With few held tiles (or, under a causal mask, one that walks far longer than the mean) a cluster of
 // blocks shares a tile's steps; their accumulators are added through distributed shared memory, in
 // rank order, each block writing its share of the columns.
-// Two pairs (A, B) alternate between two warpgroups: while one turns its pair into P and dS, the
-// tensor core forms the other's and adds the one before.  64 rows a step is what TMEM leaves: two
-// pairs of 64 + 64 columns beside two accumulators of up to 128.
+// Two warpgroups turn a pair (A, B) into P and dS, each 32 of its 64 columns.  64 rows a step is what TMEM
+// leaves.  Up to 64 channels, one pair and two accumulators take half of it, and two blocks of an SM cover each
+// other, their starts and ends too; with 128, two pairs alternate in one block: while one is in work, the
+// tensor core forms the other and adds the one before.  (Two pairs in one block with 64 channels: 440 against
+// 403 us for 4 x 2048 tokens of 12 heads, 392 against 277 for 104 x 300 of 8 heads of 32, forward included.)
 // P and dS are rounded to bf16 for the tensor core; every sum is float32.
 // A row that sees exactly one key has P = 1 whatever its score, so its dS is set to what is left of
 // it, the cotangent of its lse, rather than to the difference of two roundings of the same number.
@@ -922,11 +927,18 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
 constexpr int kWalk = 64;  // rows of Y a step
 
 template <int DP> struct BwdShape {
+    static constexpr int kPairs = DP <= 64 ? 1 : 2;
     static constexpr int kXBytes = 128 * DP * 2;
     static constexpr int kYBytes = kWalk * DP * 2;
     static constexpr int kStages = 4;
-    static constexpr int kThreads = 384;
-    static constexpr int kTmem = 512;
+    static constexpr int kCompute = kPairs * 8;  // warps
+    static constexpr int kThreads = kPairs * 256 + 128;
+    static constexpr int kBlocks = kPairs == 2 ? 1 : 2;
+    // 65536 / 640 -> 96; 65536 / 768 -> 80.
+    using Regs = std::conditional_t<kPairs == 2, Registers<4, 96, 104, 64>, Registers<2, 80, 96, 48>>;
+    static constexpr int kTmem = kPairs == 2 ? 512 : 256;
+    static constexpr int kAcc = kPairs * 2 * kWalk;  // first accumulator column
+    static_assert(kAcc + 2 * DP <= kTmem, "TMEM");
     static constexpr size_t kSmem = 1024 + 2 * kXBytes + (size_t)kStages * 2 * kYBytes;
 };
 
@@ -1051,40 +1063,45 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         const uint64_t y = y_desc + st * (2 * S::kYBytes / 16);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-            mma_channels<DP, kXPanel, kYPanel>(tmem + (i & 1) * 2 * kWalk + which * kWalk,
+            mma_channels<DP, kXPanel, kYPanel>(tmem + (i % S::kPairs) * 2 * kWalk + which * kWalk,
                                                x_desc + which * (S::kXBytes / 16), y + which * (S::kYBytes / 16), kIdS);
-        tc_commit_one(&sh.s_full[i & 1]);
+        tc_commit_one(&sh.s_full[i % S::kPairs]);
         return true;
     };
     if (!wait_warp(&sh.x_full, 0, abort)) return false;
     if (!scores(0)) return false;
-    if (steps > 1 && !scores(1)) return false;
+    if (S::kPairs == 2 && steps > 1 && !scores(1)) return false;
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
         const int st = i % S::kStages;
         const uint64_t y = yt_desc + st * (2 * S::kYBytes / 16);
-        if (!wait_warp(&sh.ds_ready[i & 1], (i >> 1) & 1, abort)) return false;
+        if (!wait_warp(&sh.ds_ready[i % S::kPairs], (i / S::kPairs) & 1, abort)) return false;
         tc_fence_after();
         static_assert(kWalk == 64, "four steps");
-        const uint32_t p = tmem + (i & 1) * 2 * kWalk;
-        if (DKV)
-            mma_ts_one<4, TL::kRowBytes>(tmem + 4 * kWalk + DP, p, y + S::kYBytes / 16, kIdAcc, i > 0);
-        mma_ts_one<4, TL::kRowBytes>(tmem + 4 * kWalk, p + kWalk, y, kIdAcc, i > 0);
+        const uint32_t p = tmem + (i % S::kPairs) * 2 * kWalk;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint64_t yh = y + h * 2 * TL::kRowBytes;
+            if (DKV)
+                mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc + DP, p + h * 32, yh + S::kYBytes / 16, kIdAcc,
+                                             i > 0 || h > 0);
+            mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc, p + kWalk + h * 32, yh, kIdAcc, i > 0 || h > 0);
+        }
         tc_commit_one(&sh.y_empty[st]);
-        if (i + 2 < steps && !scores(i + 2)) return false;
+        if (i + S::kPairs < steps && !scores(i + S::kPairs)) return false;
     }
     tc_commit_one(&sh.acc_done);
     return true;
 }
 
-// Warpgroup w: the steps i with i % 2 == w.
+// Warpgroups 2 w and 2 w + 1: the steps i with i % kPairs == w, the first 32 columns and the others.
 template <int DP, bool DKV>
 __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const float *lse,
                           const float *delta, const float *g_lse) {
     using S = BwdShape<DP>;
     volatile int *abort = &sh.abort;
-    const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
-    const uint32_t ts = tmem + ((uint32_t)((threadIdx.x >> 5) & 3) << 21) + w * 2 * kWalk;
+    const int w = threadIdx.x >> 8, c0 = ((threadIdx.x >> 7) & 1) * 32, row = threadIdx.x & 127;
+    const uint32_t ts = tmem + ((uint32_t)((threadIdx.x >> 5) & 3) << 21) + w * 2 * kWalk + c0;
     const float2 sc2 = make_float2(A.scale_log2, A.scale_log2);
     const int shift = r.klen - r.qlen;  // under a causal mask token t sees keys <= t + shift
     // DKV: this row's key.  DQ: this row's query.
@@ -1102,11 +1119,11 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
 #pragma unroll 1
-    for (int i = w; i < r.steps - r.start; i += 2) {
+    for (int i = w; i < r.steps - r.start; i += S::kPairs) {
         const int st = i % S::kStages;
-        if (!wait_warp(&sh.s_full[w], (i >> 1) & 1, abort)) return;
+        if (!wait_warp(&sh.s_full[w], (i / S::kPairs) & 1, abort)) return;
         tc_fence_after();
-        // Columns [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or the
+        // Of this thread's columns c0 ..: [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or the
         // whole row is (DQ) a query with a single key.
         int lo = 0, hi = kWalk, one_lo = 0, one_hi = 0;
         bool mask;
@@ -1133,24 +1150,22 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 one_hi = limit == 1 ? kWalk : 0;
             }
         }
-        float s[kWalk], d[kWalk];
-#pragma unroll
-        for (int c = 0; c < kWalk; c += 32) {
-            tmem_ld32(ts + c, s + c);
-            tmem_ld32(ts + kWalk + c, d + c);
-        }
+        lo -= c0, hi -= c0, one_lo -= c0, one_hi -= c0;
+        float s[32], d[32];
+        tmem_ld32(ts, s);
+        tmem_ld32(ts + kWalk, d);
         tmem_wait_ld();
-        pin<kWalk>(s);
-        pin<kWalk>(d);
-        uint32_t ps[32], pd[32];
+        pin<32>(s);
+        pin<32>(d);
+        uint32_t ps[16], pd[16];
         // Straight code in either case: the exponentials' latencies overlap.
         auto weights = [&](auto masked) {
 #pragma unroll
-        for (int c = 0; c < kWalk; c += 4) {
+        for (int c = 0; c < 32; c += 4) {
             float4 nl, nd;
             if (DKV) {
-                nl = *reinterpret_cast<const float4 *>(&sh.neg_lse2[st][c]);
-                nd = *reinterpret_cast<const float4 *>(&sh.neg_delta[st][c]);
+                nl = *reinterpret_cast<const float4 *>(&sh.neg_lse2[st][c0 + c]);
+                nd = *reinterpret_cast<const float4 *>(&sh.neg_delta[st][c0 + c]);
             } else {
                 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
                 nd = make_float4(row_nd, row_nd, row_nd, row_nd);
@@ -1168,7 +1183,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                     const bool seen = c + k >= lo && c + k < hi;
                     const bool one = c + k >= one_lo && c + k < one_hi;
                     p[k] = seen ? p[k] : 0.0f;
-                    ds[k] = seen ? one ? (DKV ? sh.one_ds[st][c + k] : row_od) : ds[k] : 0.0f;
+                    ds[k] = seen ? one ? (DKV ? sh.one_ds[st][c0 + c + k] : row_od) : ds[k] : 0.0f;
                 }
             }
             ps[c / 2] = pack_bf16(p[0], p[1]);
@@ -1179,8 +1194,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         };
         if (mask) weights(std::true_type{});
         else weights(std::false_type{});
-        if (DKV) tmem_st32(ts, ps);
-        tmem_st32(ts + kWalk, pd);
+        // Over this half of A and B: the other half may not have been read yet.
+        if (DKV) tmem_st16(ts, ps);
+        tmem_st16(ts + kWalk, pd);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -1190,47 +1206,41 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     tc_fence_after();
 }
 
-// Writes columns [from, to) of a row of an accumulator (whole warp; `live` rows only).
-template <int DP>
-__device__ __forceinline__ void store_acc(uint32_t addr, bool any, int from, int to, float scale, bf16 *dst, int D,
-                                          bool live) {
+// Writes a row's part of the accumulators: the GROUPS warpgroups take 16 columns in turn.
+template <int DP, bool DKV, int GROUPS>
+__device__ __forceinline__ void store_acc(const AttnArgs &A, uint32_t acc, bool any, size_t row_at, bool live, bf16 *g0,
+                                          bf16 *g1) {
+    constexpr int kAll = DKV ? 2 * DP : DP;
 #pragma unroll 1
-    for (int c = from; c < to; c += 32) {
-        float o[32];
+    for (int c = (threadIdx.x >> 7) * 16; c < kAll; c += GROUPS * 16) {
+        float o[16];
         if (any) {
-            tmem_ld32(addr + c, o);
+            tmem_ld16(acc + c, o);
             tmem_wait_ld();
-            pin<32>(o);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            pin<16>(o);
         }
         if (!live) continue;
+        const bool second = DKV && c >= DP;
+        const int col = second ? c - DP : c;
+        const float f = second ? 1.0f : A.scale;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-            if (c + e < D) {
-                uint4 v;
-                v.x = pack_bf16(o[e] * scale, o[e + 1] * scale);
-                v.y = pack_bf16(o[e + 2] * scale, o[e + 3] * scale);
-                v.z = pack_bf16(o[e + 4] * scale, o[e + 5] * scale);
-                v.w = pack_bf16(o[e + 6] * scale, o[e + 7] * scale);
-                *reinterpret_cast<uint4 *>(dst + c + e) = v;
-            }
+        for (int e = 0; e < 16; ++e) o[e] = any ? o[e] * f : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 8)
+            if (col + e < A.D) store_vec<bf16, 8>((second ? g1 : g0) + row_at + col + e, o + e);
     }
 }
 
-// DKV: g0 = dK, g1 = dV.  Otherwise g0 = dQ.
 // Whole block: this block's accumulator columns into its shared memory (column-major: a warp's rows
 // are consecutive), then the cluster's sums of this block's share of the columns to memory.
-template <int DP, bool DKV>
+template <int DP, bool DKV, int GROUPS>
 __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t smem, int ranks, int rank, size_t row_at,
                           bool live, bf16 *g0, bf16 *g1) {
     constexpr int kAll = DKV ? 2 * DP : DP;
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
-    if (w < 2) {
-        // Warpgroup 0 the first half of the columns, 1 the second.
+    if (w < GROUPS) {
 #pragma unroll 1
-        for (int c = w * (kAll / 2); c < (w + 1) * (kAll / 2); c += 16) {
+        for (int c = w * 16; c < kAll; c += GROUPS * 16) {
             float o[16];
             if (any) {
                 tmem_ld16(acc + c, o);
@@ -1245,9 +1255,9 @@ __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t sm
     }
     cluster_sync();
     const int cols = kAll / ranks;
-    if (w < 2) {
+    if (w < GROUPS) {
 #pragma unroll 1
-        for (int c = rank * cols + w * 8; c < (rank + 1) * cols; c += 16) {
+        for (int c = rank * cols + w * 8; c < (rank + 1) * cols; c += GROUPS * 8) {
             float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
             for (int k = 0; k < ranks; ++k) {
@@ -1258,13 +1268,9 @@ __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t sm
             const bool second = DKV && c >= DP;
             const int col = second ? c - DP : c;
             if (live && col < A.D) {
-                const float f = second ? 1.0f : A.scale;
-                uint4 v;
-                v.x = pack_bf16(o[0] * f, o[1] * f);
-                v.y = pack_bf16(o[2] * f, o[3] * f);
-                v.z = pack_bf16(o[4] * f, o[5] * f);
-                v.w = pack_bf16(o[6] * f, o[7] * f);
-                *reinterpret_cast<uint4 *>((second ? g1 : g0) + row_at + col) = v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] *= second ? 1.0f : A.scale;
+                store_vec<bf16, 8>((second ? g1 : g0) + row_at + col, o);
             }
         }
     }
@@ -1272,7 +1278,7 @@ __device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t sm
 }
 
 template <int DP, bool DKV>
-__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, const __grid_constant__ CUtensorMap mx1,
                      const __grid_constant__ CUtensorMap my0, const __grid_constant__ CUtensorMap my1,
                      const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ g_lse,
@@ -1317,7 +1323,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const uint32_t smem_x = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t smem_y = smem_x + 2 * S::kXBytes;
 
-    if (warp == 8) {
+    if (warp == S::kCompute) {
         if ((threadIdx.x & 31) == 0) {
             mbar_init(&sh.x_full, 1);
             for (int i = 0; i < S::kStages; ++i) {
@@ -1327,7 +1333,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
             mbar_init(&sh.y_raw, 1);
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&sh.s_full[b], 1);
-                mbar_init(&sh.ds_ready[b], 4);
+                mbar_init(&sh.ds_ready[b], 8);
             }
             mbar_init(&sh.acc_done, 1);
             mbar_init(&sh.drain, 1);
@@ -1350,43 +1356,35 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
 
     int issued = 0;
     const int row = threadIdx.x & 127;
-    const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + 4 * kWalk;
+    const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + S::kAcc;
     const bool live = DKV ? r.k0 + row < r.klen : row_token(A, row) < r.qtok;
     const size_t row_at = DKV ? ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D
                               : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
-    if (warp >= 8) {
-        regs_less<kLessRegs>();
-        if (warp == 8 && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem);
-        if (warp == 9) issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
+    if (warp >= S::kCompute) {
+        regs_less<S::Regs::kLess>();
+        if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem);
+        if (warp == S::kCompute + 1)
+            issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
     } else {
-        regs_more<kMoreRegs>();
+        regs_more<S::Regs::kMore>();
         bwd_grads<DP, DKV>(A, sh, r, tmem, lse, delta, g_lse);
         __syncwarp();
-        if (ranks == 1) {
-            const int w = warp >> 2;
-            if (DKV) {
-                if (w == 0) store_acc<DP>(acc, steps > 0, 0, DP, A.scale, g0 + row_at, A.D, live);
-                else store_acc<DP>(acc + DP, steps > 0, 0, DP, 1.0f, g1 + row_at, A.D, live);
-            } else {
-                const int half = DP >= 64 ? DP / 2 : DP;  // columns of the first warpgroup
-                store_acc<DP>(acc, steps > 0, w * half, w == 0 ? half : DP, A.scale, g0 + row_at, A.D, live);
-            }
-        }
+        if (ranks == 1) store_acc<DP, DKV, 2 * S::kPairs>(A, acc, steps > 0, row_at, live, g0, g1);
     }
     if (ranks > 1) {
         // Every product of this block is done, so its shared memory is free.
         __syncthreads();
-        share_acc<DP, DKV>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
+        share_acc<DP, DKV, 2 * S::kPairs>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0 && steps > 0) {
+    if (sh.abort && warp == S::kCompute + 1 && (threadIdx.x & 31) == 0 && steps > 0) {
         mbar_drain(&sh.x_full, 0, kAttnWaitLimit);
         for (int i = max(0, issued - S::kStages); i < issued; ++i)
             mbar_drain(&sh.y_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
     }
-    if (warp == 8) {
+    if (warp == S::kCompute) {
         if (sh.abort) {
             tc_commit_one(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
@@ -1506,12 +1504,17 @@ ForwardPlan plan_forward(const AttnArgs &A) {
         p.splits = p.is_short || forced.v[1] < 1 ? 1 : forced.v[1] > 64 ? 64 : forced.v[1];
         return p;
     }
-    if (blocks * 2 <= num_sms() && tiles >= 8) {
-        long long s = num_sms() / (blocks > 0 ? blocks : 1);
-        if (s > tiles / 4) s = tiles / 4;
-        p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    // Few blocks with many keys: split until there are two to an SM (the lengths differ), with four key
+    // tiles at least to a part.  8 x 300 queries over 0 to 4000 keys, 8 heads of 80: 42.8 us in two parts, 58.4
+    // in one; one token each over 1 to 16384 keys, 4 key heads of 128: 57.5 us in 4 to 8 parts, 188 in one.
+    long long s = 2ll * num_sms() / (blocks > 0 ? blocks : 1);
+    if (s > tiles / 4) s = tiles / 4;
+    if (s >= 2) {
+        p.splits = (int)(s > 64 ? 64 : s);
         return p;
     }
+    // 104 x 300 tokens, 8 heads of 32: 62 us in the short kernel, 103 in the long one; 32 x 145, 6 of 64: 12.7
+    // and 16.2; 16 of 1 to 1601, 6 of 64: 52.6 and 52.8; 8 x 300 over 0 to 4000 keys, 8 of 80: 100 and 58.
     p.is_short = rows <= 4 * per && keys <= 512;
     return p;
 }

@@ -135,12 +135,20 @@ __device__ __forceinline__ void mma_ss_one(uint32_t d, uint64_t a, uint64_t b, u
 }
 template <int N, int BS>
 __device__ __forceinline__ void mma_ts_one(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    static_assert(N == 1 || N == 4, "steps");
+    static_assert(N == 1 || N == 2 || N == 4, "steps");
     if constexpr (N == 1) {
         asm volatile(
             "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
             "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
+    } else if constexpr (N == 2) {
+        asm volatile(
+            "{\n.reg .pred p, q, t;\n.reg .b64 b;\n.reg .b32 a;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+            "setp.eq.b32 t, 0, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\nadd.s32 a, %1, 8;\nadd.s64 b, %2, %5;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(BS)
             : "memory");
     } else {
         asm volatile(
