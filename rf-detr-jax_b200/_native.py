@@ -151,8 +151,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    """The current torch stream of ``t``'s device, as a raw ``cudaStream_t``."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current torch stream of ``t``'s device, as a raw ``cudaStream_t`` (without the stream object that
+    ``torch.cuda.current_stream`` makes, 2.3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

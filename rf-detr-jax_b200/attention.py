@@ -9,33 +9,29 @@ sequences and their offsets, with grouped heads and an optional causal mask.
 
 from __future__ import annotations
 
-import math
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
 
-def _packed(name: str, t: torch.Tensor, heads: int | None, dim: int | None) -> torch.Tensor:
+def _packed(name: str, t: torch.Tensor) -> torch.Tensor:
     """Checks ``[tokens, heads, dim]`` bf16 and returns it with strides the kernels take (a view of
     a fused projection passes as it is; anything else is made contiguous)."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
     if t.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
-    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {list(t.shape)}")
     token, head, channel = t.stride()
-    if channel != 1 or token <= 0 or head <= 0 or token % 8 or head % 8 or t.data_ptr() % 16:
+    if channel != 1 or token <= 0 or head <= 0 or (token | head) & 7 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _offsets(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.dim() != 1 or t.numel() < 1 or t.dtype not in (torch.int32, torch.int64):
+    if t.dim() != 1 or t.shape[0] < 1 or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 [sequences + 1]")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
@@ -50,14 +46,14 @@ def attention_forward(query, key, value, offsets, key_offsets, causal, scale, wa
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
     sequences = offsets.numel() - 1
-    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
-    lse = torch.empty((heads, tokens), dtype=torch.float32, device=query.device) if want_lse else None
+    out = query.new_empty((tokens, heads, dim))
+    lse = query.new_empty((heads, tokens), dtype=torch.float32) if want_lse else None
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+    workspace = query.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     status = lib.rfdetr_packed_attention(
-        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
-        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), offsets.data_ptr(), N.ptr(key_offsets),
+        N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+        value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
         out.data_ptr(), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads, kv_heads, dim,
         int(causal), scale)
     N.check(status, "rfdetr_packed_attention")
@@ -68,18 +64,17 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
     """One backward call; returns ``(grad_query, grad_key, grad_value)``, contiguous."""
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
-    grad_output = _packed("grad_output", grad_output.to(query.dtype), heads, dim)
+    grad_output = _packed("grad_output", grad_output.to(query.dtype))
     if grad_lse is not None:
         grad_lse = grad_lse.to(torch.float32).contiguous()
-    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    grads = new(query), new(key), new(value)
+    grads = tuple(t.new_empty(t.shape) for t in (query, key, value))
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_backward_workspace_bytes(tokens, heads)
-    workspace = torch.empty(max(1, ws_bytes), dtype=torch.uint8, device=query.device)
+    workspace = query.new_empty(max(1, ws_bytes), dtype=torch.uint8)
     status = lib.rfdetr_packed_attention_backward(
-        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
-        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), offsets.data_ptr(), N.ptr(key_offsets),
-        out.data_ptr(), lse.data_ptr(), grad_output.data_ptr(), grad_output.stride(0), grad_output.stride(1),
+        N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+        value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
+        out.data_ptr(), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
         N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
         offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale)
     N.check(status, "rfdetr_packed_attention_backward")
@@ -134,32 +129,32 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         give 0 (log-sum-exp ``-inf``) and gradient 0.
     """
     N.require_cuda(query, key, value, offsets, key_offsets)
-    query = _packed("query", query, None, None)
+    query, key, value = _packed("query", query), _packed("key", key), _packed("value", value)
     tokens, heads, dim = query.shape
-    key = _packed("key", key, None, dim)
-    value = _packed("value", value, key.shape[1], dim)
-    if value.shape[0] != key.shape[0]:
-        raise ValueError("key and value must have the same tokens")
-    if key.shape[1] < 1 or heads < 1 or heads % key.shape[1]:
-        raise ValueError(f"{heads} query heads are not a multiple of {key.shape[1]} key heads")
+    key_tokens, kv_heads, key_dim = key.shape
+    if key_dim != dim or value.shape != key.shape:
+        raise ValueError(f"key and value must be [key_tokens, kv_heads, {dim}], got {list(key.shape)} and "
+                         f"{list(value.shape)}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"head_dim must be a multiple of 8 up to 128, got {dim}")
-    if max(tokens, key.shape[0]) > 1 << 30 or heads > 65536:
+    if tokens > 1 << 30 or key_tokens > 1 << 30 or heads > 65536:
         raise ValueError("at most 2^30 tokens and 65536 heads")
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale <= 3.4028234663852886e38 or not math.isfinite(scale):
+    if not 0.0 < scale <= 3.4028234663852886e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     offsets = _offsets("offsets", offsets)
     if key_offsets is not None:
         key_offsets = _offsets("key_offsets", key_offsets)
         if key_offsets.numel() != offsets.numel():
             raise ValueError("offsets and key_offsets must have the same length")
-    elif key.shape[0] != tokens:
+    elif key_tokens != tokens:
         raise ValueError("key_offsets is needed where keys and queries are not the same tokens")
     if check:
         _check_offsets("offsets", offsets, tokens)
         if key_offsets is not None:
-            _check_offsets("key_offsets", key_offsets, key.shape[0])
+            _check_offsets("key_offsets", key_offsets, key_tokens)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)
     else:

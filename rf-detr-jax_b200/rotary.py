@@ -15,24 +15,29 @@ from . import _native as N
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
-    return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _pairs(t: torch.Tensor) -> torch.Tensor:
+    """Interleaved pairs are read as one: aligned to a pair, or copied."""
+    token, head, _ = t.stride()
+    if (token | head) & 1 or t.data_ptr() % (2 * t.element_size()):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def rotary_launch(query, key, positions, inv_freq, sections, interleaved, inverse):
     """One launch over checked inputs; ``key`` may be None."""
     tokens, heads, dim = query.shape
-    pairs = query.data_ptr() % (2 * query.element_size()) == 0 and query.stride(0) % 2 == 0 and query.stride(1) % 2 == 0
-    if interleaved and not pairs:
-        query = query.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
+    if interleaved:
+        query, key = _pairs(query), None if key is None else _pairs(key)
+    out = query.new_empty((tokens, heads, dim))
     key_out, kv_heads, key_strides = None, 0, (0, 0)
     if key is not None:
-        if interleaved and (key.data_ptr() % (2 * key.element_size()) or key.stride(0) % 2 or key.stride(1) % 2):
-            key = key.clone(memory_format=torch.contiguous_format)
-        kv_heads, key_strides = key.shape[1], (key.stride(0), key.stride(1))
-        key_out = torch.empty((tokens, kv_heads, dim), dtype=key.dtype, device=key.device)
+        kv_heads, key_strides = key.shape[1], key.stride()[:2]
+        key_out = key.new_empty((tokens, kv_heads, dim))
     status = N.lib().rfdetr_axial_rotary(
-        N.stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), N.ptr(key), *key_strides,
+        N.stream_of(query), query.data_ptr(), *query.stride()[:2], N.ptr(key), *key_strides,
         N.dtype_code(query.dtype), positions.data_ptr(), N.F32 if positions.dtype == torch.float32 else N.I32,
         inv_freq.data_ptr(), N.int64_array(sections), len(sections), out.data_ptr(), N.ptr(key_out), tokens, heads,
         kv_heads, dim, int(interleaved), int(inverse))
