@@ -83,7 +83,8 @@ __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *oth
             lo += p;
             r.base = __shfl_sync(0xffffffffu, e, p);
             r.len = max(0, __shfl_sync(0xffffffffu, e, p + 1) - r.base);
-            r.first = (slot - (r.base / R + lo)) * R;
+            const int ahead = slot - (r.base / R + lo);
+            r.first = ahead > r.len / R ? r.len : ahead * R;  // slots past a sequence's rows are empty
             const int a = __shfl_sync(0xffffffffu, f, p), b = __shfl_sync(0xffffffffu, f, p + 1);
             const bool real = lo >= 1 && lo <= n_seq;
             r.other_base = real ? a : 0;
@@ -132,6 +133,13 @@ __device__ __forceinline__ void mma_channels(uint32_t d, uint64_t a, uint64_t b,
 #pragma unroll
     for (int p = 0; p < Tile<DP>::kPanels; ++p)
         mma_ss_one<N, 2, 2>(d, a + p * (A_PANEL / 16), b + p * (B_PANEL / 16), idesc, p > 0);
+}
+
+// Bits lo .. hi - 1 of a word.
+__device__ __forceinline__ uint32_t bits(int lo, int hi) {
+    lo = max(lo, 0);
+    hi = min(hi, 32);
+    return hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
 }
 
 // Zeroes rows [from, to) of a swizzled tile by the first `threads` threads of a block or a warp's
@@ -237,10 +245,11 @@ template <int DP> __device__ __forceinline__ void move_reference(RowState &r, ui
 // false to give up), written(half) after each half of P.
 // Tiles that are seen whole, the many, are read once into registers and run straight through; the
 // others go over S twice in a small loop.
-template <int DP, int KEYS, typename Loaded, typename Settle, typename Written>
+template <int DP, typename Loaded, typename Settle, typename Written>
 __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
                                              int seen, bool first, float sc, Loaded loaded, Settle settle,
                                              Written written) {
+    constexpr int KEYS = 128;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     if (all) {
         float s[KEYS];
@@ -257,8 +266,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
         for (int h = 0; h < 2; ++h) {
             uint32_t p[KEYS / 4];
             exp_pack<KEYS / 2, true>(s + h * (KEYS / 2), sc, ref, p, acc);
-            if (KEYS == 128) tmem_st32(tp + h * 32, p);
-            else tmem_st16(tp + h * 16, p);
+            tmem_st32(tp + h * 32, p);
             tmem_wait_st();
             written(h);
         }
@@ -295,6 +303,43 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
     }
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
     return true;
+}
+
+// The same for one warpgroup's tile of 64 keys, P over S.  Masked tiles run straight through too: in short
+// sequences they are many.
+template <int DP>
+__device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_t to, int cols, bool all, int seen,
+                                               bool first, float sc) {
+    float s[64];
+    tmem_ld32(ts, s);
+    if (cols > 32) tmem_ld32(ts + 32, s + 32);
+    tmem_wait_ld();
+    pin<64>(s);
+    if (!all) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t m = bits(0, seen - h * 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
+        }
+    }
+    move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
+    float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    uint32_t p[32];
+    if (all) {
+        exp_pack<64, true>(s, sc, ref, p, acc);
+        tmem_st32(ts, p);
+    } else {
+        exp_pack<32, false>(s, sc, ref, p, acc);
+        tmem_st16(ts, p);
+        if (cols > 32) {
+            exp_pack<32, false>(s + 32, sc, ref, p + 16, acc);
+            tmem_st16(ts + 16, p + 16);
+        }
+    }
+    tmem_wait_st();
+    r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
 }
 
 // Whole warp: a row's result from O (or zeros) and its log-sum-exp.
@@ -649,7 +694,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                     mbar_arrive_one(&sh.p_half[t][h]);
                 };
                 if (warp_live) {
-                    ok = softmax_tile<DP, S::kKeys>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
+                    ok = softmax_tile<DP>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
                                                     k0 + S::kKeys <= all_see, limit - k0, i == 0, A.scale_log2, loaded,
                                                     settle, written);
                 } else {
@@ -812,8 +857,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         }
         const int k0 = i * KEYS;
         if (warp_live)
-            softmax_tile<DP, KEYS>(rs, ts, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
-                                   A.scale_log2, [] {}, [] { return true; }, [](int) {});
+            softmax_tile64<DP>(rs, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
+                               A.scale_log2);
         // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
         if (k0 + KEYS > klen) {
             ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort) && ok;
@@ -1118,10 +1163,16 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     }
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
+    // A warp without a live row leaves its rows of P and dS as they are: they reach no other row.
+    const bool warp_live = DKV ? r.k0 + (row & ~31) < r.klen : (row & ~31) < r.qtok * A.pack;
 #pragma unroll 1
     for (int i = w; i < r.steps - r.start; i += S::kPairs) {
         const int st = i % S::kStages;
         if (!wait_warp(&sh.s_full[w], (i / S::kPairs) & 1, abort)) return;
+        if (!warp_live) {
+            mbar_arrive_one(&sh.ds_ready[w]);
+            continue;
+        }
         tc_fence_after();
         // Of this thread's columns c0 ..: [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or the
         // whole row is (DQ) a query with a single key.
@@ -1134,8 +1185,8 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             if (mask) {
                 hi = key < r.klen ? good : 0;
                 if (A.causal) {
-                    lo = max(0, (key - shift - at) * A.pack);
-                    one_lo = (-shift - at) * A.pack;  // the token that sees key 0 only
+                    lo = min(max(key - shift - at, 0), kWalk) * A.pack;
+                    one_lo = min(max(-shift - at, -kWalk), kWalk) * A.pack;  // the token that sees key 0 only
                     one_hi = one_lo + A.pack;
                 }
                 if (r.klen == 1) {
@@ -1150,7 +1201,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 one_hi = limit == 1 ? kWalk : 0;
             }
         }
-        lo -= c0, hi -= c0, one_lo -= c0, one_hi -= c0;
+        const uint32_t seen = bits(lo - c0, hi - c0), one = seen & bits(one_lo - c0, one_hi - c0);
         float s[32], d[32];
         tmem_ld32(ts, s);
         tmem_ld32(ts + kWalk, d);
@@ -1180,10 +1231,10 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             if (masked) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const bool seen = c + k >= lo && c + k < hi;
-                    const bool one = c + k >= one_lo && c + k < one_hi;
-                    p[k] = seen ? p[k] : 0.0f;
-                    ds[k] = seen ? one ? (DKV ? sh.one_ds[st][c0 + c + k] : row_od) : ds[k] : 0.0f;
+                    const uint32_t bit = 1u << (c + k);
+                    p[k] = seen & bit ? p[k] : 0.0f;
+                    ds[k] = seen & bit ? ds[k] : 0.0f;
+                    if (masked == 2 && (one & bit)) ds[k] = DKV ? sh.one_ds[st][c0 + c + k] : row_od;
                 }
             }
             ps[c / 2] = pack_bf16(p[0], p[1]);
@@ -1192,8 +1243,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             pd[c / 2 + 1] = pack_bf16(ds[2], ds[3]);
         }
         };
-        if (mask) weights(std::true_type{});
-        else weights(std::false_type{});
+        if (!mask) weights(std::integral_constant<int, 0>{});
+        else if (!__any_sync(0xffffffffu, one)) weights(std::integral_constant<int, 1>{});
+        else weights(std::integral_constant<int, 2>{});
         // Over this half of A and B: the other half may not have been read yet.
         if (DKV) tmem_st16(ts, ps);
         tmem_st16(ts + kWalk, pd);
