@@ -27,6 +27,21 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A divisor known to the host, and division by it for x up to 2^31 (Granlund and Montgomery's: the high half
+// of x times 2^32 (2^shift - d) / d, rounded up, plus x, shifted).
+struct Divisor {
+    unsigned magic, shift;
+    int d;
+};
+inline Divisor divisor(int d) {
+    unsigned l = 0;
+    while ((1ll << l) < d) ++l;
+    return {(unsigned)(((1ull << 32) * ((1ull << l) - (unsigned)d)) / (unsigned)d + 1), l, d};
+}
+__device__ __forceinline__ int quotient(int x, const Divisor &d) {
+    return (int)((__umulhi(d.magic, (unsigned)x) + (unsigned)x) >> d.shift);
+}
+
 struct AttnArgs {
     const int32_t *q_off, *k_off;  // [n_seq + 1]
     int n_seq, Tq, Tk;
@@ -36,6 +51,8 @@ struct AttnArgs {
     int subs;    // tiles' head groups per key head: (Hq / Hkv) / pack
     int causal;
     float scale, scale_log2;
+    Divisor slot_rows;  // rows (of the tensor that the launch tiles) in a slot
+    Divisor heads;      // key heads x head groups: blocks or row tiles to a slot
 };
 
 // A tile row's token within the tile and its head among the packed ones.
@@ -66,7 +83,7 @@ struct Slot {
 // rows before and after all sequences.  A search over 31 probes a step; the last step's probes
 // already hold the answer, so up to 30 sequences take one round trip to memory, up to 960 two.
 __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *other, int n_seq, int T, int T_other,
-                                          int R, int slot) {
+                                          const Divisor &R, int slot) {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = n_seq + 2;
     while (true) {
@@ -75,7 +92,7 @@ __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *oth
         const int e = off_at(off, n_seq, T, x);
         int f = 0;
         if (step == 1 && x > 0) f = off == other ? min(e, T_other) : off_at(other, n_seq, T_other, x);
-        const bool before = lane * step < n && e / R + x <= slot;
+        const bool before = lane * step < n && quotient(e, R) + x <= slot;
         const unsigned m = __ballot_sync(0xffffffffu, before);
         const int p = m ? 31 - __clz(m) : 0;  // at most 30
         if (step == 1) {
@@ -83,8 +100,8 @@ __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *oth
             lo += p;
             r.base = __shfl_sync(0xffffffffu, e, p);
             r.len = max(0, __shfl_sync(0xffffffffu, e, p + 1) - r.base);
-            const int ahead = slot - (r.base / R + lo);
-            r.first = ahead > r.len / R ? r.len : ahead * R;  // slots past a sequence's rows are empty
+            const int ahead = slot - (quotient(r.base, R) + lo);
+            r.first = ahead > quotient(r.len, R) ? r.len : ahead * R.d;  // slots past a sequence's rows are empty
             const int a = __shfl_sync(0xffffffffu, f, p), b = __shfl_sync(0xffffffffu, f, p + 1);
             const bool real = lo >= 1 && lo <= n_seq;
             r.other_base = real ? a : 0;
@@ -582,12 +599,11 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     extern __shared__ unsigned char dyn[];
     __shared__ LongShared sh;
     const int warp = warp_index();
-    const int heads = A.Hkv * A.subs;
-    const int hx = blockIdx.x % heads;
+    const int s = quotient(blockIdx.x, A.heads), hx = blockIdx.x - s * A.heads.d;
     // Later slots first: under a causal mask they see more keys.
-    const int slot = slots - 1 - (int)(blockIdx.x / heads);
+    const int slot = slots - 1 - s;
     const int per = 128 / A.pack;  // tokens in a row tile
-    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per * 2, slot);
+    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
     if (q.first >= q.len) return;
     const int kbase = q.other_base, klen = q.other_len;
     const int kvh = hx / A.subs;
@@ -726,11 +742,13 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     }
 }
 
-// ---- short sequences: one row tile to a block, several blocks to an SM ---------------------------
-// With a few key tiles to a block, most of its time would be its start and its end; four blocks to
-// an SM (two with 128 channels) cover each other's instead of roles within one.  128 threads: each
-// owns a row, warp 0 also issues the copies and the products.  64 keys a tile, so that S and O of
-// four blocks fit TMEM and a row of S is 64 registers.
+// ---- short sequences: one row tile at a time, several blocks to an SM ----------------------------
+// With a few key tiles to a row tile, most of a block's time would be its start and its end; four blocks
+// to an SM (two with 128 channels) cover each other's instead of roles within one, and stay for the whole
+// launch: each takes every gridDim.x-th row tile, and looks up and asks for the next one's Q, K and V while
+// it works (104 x 300 tokens of 8 heads of 32: blocks that come and go cost 13.7 us by themselves, and
+// finding their rows 14 more, of 62).  128 threads: each owns a row, warp 0 also issues the copies and
+// the products.  64 keys a tile, so that S and O of four blocks fit TMEM and a row of S is 64 registers.
 template <int DP> struct ShortShape {
     static constexpr int kKeys = 64;
     static constexpr int kQBytes = 128 * DP * 2;
@@ -746,6 +764,34 @@ struct ShortShared {
     int abort;
 };
 
+// One row tile's work.
+struct ShortItem {
+    int qrow, qhead, tok0;   // first packed row, first head, first token within the sequence
+    int ntok, qlen;
+    int kvh, krow, klen;
+    int sees, n;             // keys that the tile works on, key tiles
+    bool any;                // a row tile at all
+};
+
+__device__ __forceinline__ ShortItem short_item(const AttnArgs &A, int slots, int idx, int per) {
+    ShortItem t;
+    const int s = quotient(idx, A.heads), hx = idx - s * A.heads.d;
+    // Later slots first: under a causal mask they see more keys.
+    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slots - 1 - s);
+    t.any = q.first < q.len;
+    t.kvh = hx / A.subs;
+    t.qhead = t.kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+    t.qrow = q.base + q.first;
+    t.tok0 = q.first;
+    t.ntok = min(per, q.len - q.first);
+    t.qlen = q.len;
+    t.krow = q.other_base;
+    t.klen = q.other_len;
+    t.sees = A.causal ? min(t.klen, max(0, q.first + t.ntok + t.klen - q.len)) : t.klen;
+    t.n = t.any ? (t.sees + ShortShape<32>::kKeys - 1) / ShortShape<32>::kKeys : 0;
+    return t;
+}
+
 template <int DP>
 __global__ void __launch_bounds__(128, ShortShape<DP>::kBlocks)
 attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
@@ -759,19 +805,9 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     extern __shared__ unsigned char dyn[];
     __shared__ ShortShared sh;
     const int warp = warp_index();
-    const int heads = A.Hkv * A.subs;
-    const int hx = blockIdx.x % heads;
-    const int slot = slots - 1 - (int)(blockIdx.x / heads);
-    const int per = 128 / A.pack;
-    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per, slot);
-    if (q.first >= q.len) return;
-    const int kbase = q.other_base, klen = q.other_len;
-    const int kvh = hx / A.subs;
-    const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
-    const int ntok = min(per, q.len - q.first);
-    const int sees = A.causal ? min(klen, max(0, q.first + ntok + klen - q.len)) : klen;
-    const int n = (sees + KEYS - 1) / KEYS;
     const bool boss = warp == 0;  // this warp also asks for copies and products
+    const int per = 128 / A.pack;
+    const int items = slots * A.heads.d;  // at most 2^31 - 1 by the launch
 
     if (boss) {
         if (threadIdx.x == 0) {
@@ -788,6 +824,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         __syncwarp();
         tmem_alloc(&sh.tmem, S::kTmem);
     }
+    int idx = blockIdx.x;
+    ShortItem it = short_item(A, slots, idx, per);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -796,112 +834,140 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     const uint32_t smem_k = smem_q + S::kQBytes, smem_v = smem_k + 2 * S::kTileBytes;
     volatile int *abort = &sh.abort;
 
-    auto load = [&](const CUtensorMap *map, uint64_t *bar, uint32_t dst, int j) {
+    // Tiles of K and V are counted over all of the block's row tiles: the count says stage and phase.
+    auto load_k = [&](const ShortItem &t, int g, int j, unsigned more) {
+        mbar_arrive_expect_one(&sh.k_full[g & 1], S::kTileBytes + more);
 #pragma unroll
         for (int p = 0; p < TL::kPanels; ++p)
-            tma_load_3d_one(dst + p * kPanel, map, bar, p * TL::kCols, kvh, kbase + j * KEYS);
+            tma_load_3d_one(smem_k + (g & 1) * S::kTileBytes + p * kPanel, &mk, &sh.k_full[g & 1], p * TL::kCols, t.kvh,
+                            t.krow + j * KEYS);
     };
-    auto load_k = [&](int j, unsigned more) {
-        mbar_arrive_expect_one(&sh.k_full[j & 1], S::kTileBytes + more);
-        load(&mk, &sh.k_full[j & 1], smem_k + (j & 1) * S::kTileBytes, j);
+    auto load_v = [&](const ShortItem &t, int g, int j) {
+        mbar_arrive_expect_one(&sh.v_full[g & 1], S::kTileBytes);
+#pragma unroll
+        for (int p = 0; p < TL::kPanels; ++p)
+            tma_load_3d_one(smem_v + (g & 1) * S::kTileBytes + p * kPanel, &mv, &sh.v_full[g & 1], p * TL::kCols, t.kvh,
+                            t.krow + j * KEYS);
     };
-    auto load_v = [&](int j) {
-        mbar_arrive_expect_one(&sh.v_full[j & 1], S::kTileBytes);
-        load(&mv, &sh.v_full[j & 1], smem_v + (j & 1) * S::kTileBytes, j);
+    // The first tiles of a row tile whose count starts at g: Q with K's.
+    auto load_first = [&](const ShortItem &t, int g) {
+        load_k(t, g, 0, box_bytes<DP>(per * A.pack));
+#pragma unroll
+        for (int p = 0; p < TL::kPanels; ++p)
+            tma_load_3d_one(smem_q + p * kQPanel, &mq, &sh.k_full[g & 1], p * TL::kCols, t.qhead, t.qrow);
+        load_v(t, g, 0);
+        if (t.n > 1) load_k(t, g + 1, 1, 0);
     };
     const uint64_t q_desc = smem_desc<TL::kRowBytes>(smem_q, 16, kSbo);
     const uint64_t k_desc = smem_desc<TL::kRowBytes>(smem_k, 16, kSbo);
     const uint64_t v_desc = smem_desc<TL::kRowBytes>(smem_v, kPanel, kSbo);
-    auto scores = [&](int j) {
-        if (!wait_warp(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return false;
+    auto scores = [&](int sees, int g, int j) {
+        if (!wait_warp(&sh.k_full[g & 1], (g >> 1) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t id = mma_idesc(128, tile_cols(sees, j * KEYS, KEYS), false);
-        mma_channels<DP, kQPanel, kPanel>(tmem, q_desc, k_desc + (j & 1) * (S::kTileBytes / 16), id);
+        mma_channels<DP, kQPanel, kPanel>(tmem, q_desc, k_desc + (g & 1) * (S::kTileBytes / 16), id);
         tc_commit_one(&sh.s_full);
         return true;
     };
-    int k_issued = 0, v_issued = 0;  // warp 0
-    bool ok = true;
-    if (boss && n > 0) {
-        load_k(0, box_bytes<DP>(per * A.pack));
-#pragma unroll
-        for (int p = 0; p < TL::kPanels; ++p)
-            tma_load_3d_one(smem_q + p * kQPanel, &mq, &sh.k_full[0], p * TL::kCols, qhead, q.base + q.first);
-        load_v(0);
-        k_issued = v_issued = 1;
-        if (n > 1) {
-            load_k(1, 0);
-            k_issued = 2;
-        }
-        ok = scores(0);
-    }
 
     const uint32_t ts = tmem + ((uint32_t)warp << 21), to = ts + KEYS;
-    const int row = threadIdx.x;
-    const int tok = q.first + row_token(A, row);
-    const bool live = row_token(A, row) < ntok;
-    const bool warp_live = (row & ~31) < ntok * A.pack;
-    const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
-    const int all_see = A.causal ? min(klen, q.first + 1 + klen - q.len) : klen;
-    RowState rs{-INFINITY, 0.0f};
-    bool gave_up = false;
+    const int row = threadIdx.x, row_tok = row_token(A, row);
+    int g = 0;                       // tiles of K and V before this row tile
+    int k_asked = 0, v_asked = 0;    // warp 0: counts that copies were asked for
+    unsigned done_phase = 0;
+    bool ok = true, gave_up = false;
+    if (boss && it.n > 0) {
+        load_first(it, 0);
+        k_asked = min(it.n, 2), v_asked = 1;
+    }
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-        ok = wait_warp(&sh.s_full, i & 1, abort) && ok;
-        tc_fence_after();
-        // S of tile i is done, and with it (in issue order) P V of tile i - 1: K's buffer of tile i and
-        // V's of tile i - 1 are free.
-        if (boss && ok) {
-            if (i + 2 < n) load_k(i + 2, 0), ++k_issued;
-            if (i + 1 < n) load_v(i + 1), ++v_issued;
-        }
-        const int k0 = i * KEYS;
-        if (warp_live)
-            softmax_tile64<DP>(rs, ts, to, tile_cols(sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
-                               A.scale_log2);
-        // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
-        if (k0 + KEYS > klen) {
-            ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort) && ok;
-            zero_rows<DP>(smem_v + (i & 1) * S::kTileBytes, KEYS, klen - k0, KEYS, 128);
-            fence_async_smem();
-        }
-        tc_fence_before();
-        gave_up = __syncthreads_or(!ok);
-        if (gave_up) break;
-        if (boss) {
+    while (true) {
+        if (boss && it.n > 0) ok = scores(it.sees, g, 0);
+        // The next row tile, looked up while the tensor core starts on this one.
+        idx = idx < items - (int)gridDim.x ? idx + (int)gridDim.x : items;
+        ShortItem next;
+        next.any = false;
+        next.n = 0;
+        if (idx < items) next = short_item(A, slots, idx, per);
+        const bool live = it.any && row_tok < it.ntok;
+        const bool warp_live = it.any && (row & ~31) < it.ntok * A.pack;
+        const int limit = A.causal ? min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)) : it.klen;
+        const int all_see = A.causal ? min(it.klen, it.tok0 + 1 + it.klen - it.qlen) : it.klen;
+        RowState rs{-INFINITY, 0.0f};
+#pragma unroll 1
+        for (int i = 0; i < it.n; ++i) {
+            const int t = g + i;
+            ok = wait_warp(&sh.s_full, t & 1, abort) && ok;
             tc_fence_after();
-            ok = wait_warp(&sh.v_full[i & 1], (i >> 1) & 1, abort);
-            if (ok) {
-                const int steps = tile_cols(sees, k0, KEYS) / 16;
-                const uint64_t b = v_desc + (i & 1) * (S::kTileBytes / 16);
-                static_assert(KEYS == 64, "four steps");
-                if (steps == 4) {
-                    mma_ts_one<4, TL::kRowBytes>(tmem + KEYS, tmem, b, kIdO, i > 0);
-                } else {
-#pragma unroll 1
-                    for (int k = 0; k < steps; ++k)
-                        mma_ts_one<1, 0>(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+            // S of this tile is done, and with it (in issue order) P V of the one before: K's buffer of this tile
+            // and V's of the one before are free; after the last tile Q's and K's other buffer too.
+            if (boss && ok) {
+                if (i + 2 < it.n) load_k(it, t + 2, i + 2, 0), k_asked = t + 3;
+                if (i + 1 < it.n) {
+                    load_v(it, t + 1, i + 1), v_asked = t + 2;
+                } else if (next.n > 0) {
+                    load_first(next, t + 1);
+                    k_asked = t + 1 + min(next.n, 2), v_asked = t + 2;
                 }
-                if (i + 1 < n) ok = scores(i + 1);
-                else tc_commit_one(&sh.o_done);
+            }
+            const int k0 = i * KEYS;
+            if (warp_live)
+                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
+                                   A.scale_log2);
+            // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
+            if (k0 + KEYS > it.klen) {
+                ok = wait_warp(&sh.v_full[t & 1], (t >> 1) & 1, abort) && ok;
+                zero_rows<DP>(smem_v + (t & 1) * S::kTileBytes, KEYS, it.klen - k0, KEYS, 128);
+                fence_async_smem();
+            }
+            tc_fence_before();
+            gave_up = __syncthreads_or(!ok);
+            if (gave_up) break;
+            if (boss) {
+                tc_fence_after();
+                ok = wait_warp(&sh.v_full[t & 1], (t >> 1) & 1, abort);
+                if (ok) {
+                    const int steps = tile_cols(it.sees, k0, KEYS) / 16;
+                    const uint64_t b = v_desc + (t & 1) * (S::kTileBytes / 16);
+                    static_assert(KEYS == 64, "four steps");
+                    if (steps == 4) {
+                        mma_ts_one<4, TL::kRowBytes>(tmem + KEYS, tmem, b, kIdO, i > 0);
+                    } else {
+#pragma unroll 1
+                        for (int k = 0; k < steps; ++k)
+                            mma_ts_one<1, 0>(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                    }
+                    if (i + 1 < it.n) ok = scores(it.sees, t + 1, i + 1);
+                    else tc_commit_one(&sh.o_done);
+                }
             }
         }
-    }
-    if (!gave_up) {
-        if (n > 0) ok = wait_warp(&sh.o_done, 0, abort);
+        if (gave_up) break;
+        if (it.n > 0) {
+            ok = wait_warp(&sh.o_done, done_phase, abort) && ok;
+            done_phase ^= 1;
+        } else if (boss && next.n > 0) {
+            load_first(next, g);
+            k_asked = g + min(next.n, 2), v_asked = g + 1;
+        }
         tc_fence_after();
-        if (ok)
-            write_row<DP, false>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse, nullptr,
-                                 nullptr);
+        // (O is written over only after the next row tile's first barrier.)
+        if (ok && it.any)
+            write_row<DP, false>(A, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok, it.qhead + row_head(A, row), out,
+                                 lse, nullptr, nullptr);
+        tc_fence_before();
+        g += it.n;
+        if (idx >= items) break;
+        it = next;
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (boss) {
         if (sh.abort) {
-            for (int i = max(0, k_issued - 2); i < k_issued; ++i)
+            for (int i = max(0, k_asked - 2); i < k_asked; ++i)
                 mbar_drain(&sh.k_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
-            for (int i = max(0, v_issued - 2); i < v_issued; ++i)
+            for (int i = max(0, v_asked - 2); i < v_asked; ++i)
                 mbar_drain(&sh.v_full[i & 1], (i >> 1) & 1, kAttnWaitLimit);
             tc_commit_one(&sh.drain);
             mbar_drain(&sh.drain, 0, kAttnWaitLimit);
@@ -1339,14 +1405,14 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(16) BwdShared sh;
     const int warp = warp_index();
-    const int heads = DKV ? A.Hkv : A.Hkv * A.subs;
-    const int rank = blockIdx.x % ranks, tile = blockIdx.x / ranks;
-    const int hx = tile % heads;
+    const int log_ranks = __popc(ranks - 1);  // 1, 2 or 4
+    const int rank = blockIdx.x & (ranks - 1), tile = blockIdx.x >> log_ranks;
+    const int s = quotient(tile, A.heads), hx = tile - s * A.heads.d;
     // The tiles with most work under a causal mask first: the first keys, the last queries.
-    const int slot = DKV ? tile / heads : slots - 1 - tile / heads;
+    const int slot = DKV ? s : slots - 1 - s;
     const int per = DKV ? 128 : 128 / A.pack;
-    const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, per, slot)
-                       : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, per, slot);
+    const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, A.slot_rows, slot)
+                       : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
     if (x.first >= x.len) return;
     const int G = A.Hq / A.Hkv;
     BwdRange r;
@@ -1576,7 +1642,7 @@ size_t split_bytes(const AttnArgs &A, int splits) {
 }
 
 template <int DP>
-int launch_forward(const AttnArgs &A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
+int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
                    bf16 *out, float *lse, float *part, float *part_lse, cudaStream_t stream) {
     const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP>::kKeys;
     CUtensorMap mq, mk, mv;
@@ -1586,11 +1652,15 @@ int launch_forward(const AttnArgs &A, const ForwardPlan &plan, const Strided &q,
     const long long slots = slots_for(A.Tq, plan.is_short ? per : per * 2, A.n_seq);
     const long long blocks = slots * A.Hkv * A.subs;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+    A.slot_rows = divisor(plan.is_short ? per : per * 2);
+    A.heads = divisor(A.Hkv * A.subs);
     const dim3 grid((unsigned)blocks, 1, (unsigned)plan.splits);
     if (plan.is_short) {
         using S = ShortShape<DP>;
         if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
-        attn_forward_short_kernel<DP><<<grid, 128, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, (int)slots);
+        const long long stay = (long long)S::kBlocks * num_sms();
+        attn_forward_short_kernel<DP>
+            <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, (int)slots);
         return launch_status();
     }
     using S = LongShape<DP>;
@@ -1659,7 +1729,7 @@ int launch_backward_kernel(long long tiles, int ranks, cudaStream_t stream, Args
 }
 
 template <int DP>
-int launch_backward(const AttnArgs &A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
+int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
                     const float *lse, const float *delta, const float *g_lse, bf16 *dq, bf16 *dk, bf16 *dv,
                     cudaStream_t stream) {
     const BackwardPlan plan = plan_backward(A);
@@ -1672,12 +1742,16 @@ int launch_backward(const AttnArgs &A, const Strided &q, const Strided &k, const
         return RFDETR_ERR_CUDA;
     if (A.Tk > 0) {
         const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
+        A.slot_rows = divisor(128);
+        A.heads = divisor(A.Hkv);
         if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, stream, A, kx, vx, qy, gy, lse, delta,
                                                       g_lse, dk, dv, (int)slots))
             return st;
     }
     if (A.Tq > 0) {
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
+        A.slot_rows = divisor(xtok);
+        A.heads = divisor(A.Hkv * A.subs);
         if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, stream, A, qx, gx, ky, vy, lse, delta,
                                                        g_lse, dq, nullptr, (int)slots))
             return st;
