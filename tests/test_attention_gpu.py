@@ -333,6 +333,18 @@ def test_every_backward_split(pkg, tuning, knob, dim):
     _check(pkg, (130, 5), (30, 1000), heads=2, kv=2, dim=dim, causal=True, seed=dim, with_lse_grad=True)
 
 
+@pytest.mark.parametrize("dim", [32, 128])
+def test_blocks_that_stay(pkg, tuning, dim):
+    """More row tiles than the short kernel's resident blocks, with empty ones, tiles without keys and
+    ragged ends between them, taken in turn."""
+    tuning("RFDETR_ATTN_FWD", "2")
+    rng = np.random.default_rng(21)
+    lengths = [int(n) for n in rng.integers(0, 200, 150)]
+    keys = [int(n) if rng.random() > 0.2 else 0 for n in rng.integers(0, 300, 150)]
+    _check(pkg, lengths, keys, heads=8, kv=8, dim=dim, causal=True)
+    _check(pkg, keys, heads=12, kv=4, dim=dim)
+
+
 def test_one_token_over_long_keys(pkg):
     """The form for single tokens: the keys are split over blocks."""
     N = pkg._native
