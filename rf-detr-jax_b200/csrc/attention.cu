@@ -414,8 +414,10 @@ __device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return mi
 // for 256 rows.  128 keys a tile.  The warpgroups take their registers from the other two warps
 // (setmaxnreg): a row of S is 128 values.
 // With few row tiles the keys are split over blocks (SPLIT): each writes its normalised part in
-// float32 and its lse, and attn_join_kernel adds them by weight.
-template <int DP> struct LongShape {
+// float32 and its lse, and attn_join_kernel adds them by weight.  Where a sequence's queries fill one row
+// tile at most (single tokens), a second would be empty: the block's two halves then take its key
+// tiles in turn, each with sums of its own that make a part (ALT).
+template <int DP, bool ALT> struct LongShape {
     static constexpr int kKeys = 128;
     static constexpr int kTileBytes = 128 * DP * 2;
     static constexpr int kStages = 4;
@@ -426,7 +428,7 @@ template <int DP> struct LongShape {
     // TMEM: S of both tiles (2 x 128), O of both (2 x DP), and P (2 x 64) where there is room for it;
     // with 128 channels there is none and P lies over S.  P of its own lets the next S be formed while
     // this one's exponentials run.
-    static constexpr bool kOwnP = DP <= 64;
+    static constexpr bool kOwnP = DP <= 64 && !ALT;
     static constexpr int kO = 256, kP = kOwnP ? 256 + 2 * DP : 0, kPStep = kOwnP ? 64 : 128;
 };
 struct LongShared {
@@ -436,23 +438,21 @@ struct LongShared {
 };
 
 struct LongRange {
-    int sees[2];    // keys that each row tile works on, from key j0 * 128 on
-    int n[2];       // key tiles of each row tile (end, exclusive)
-    int nmax;       // end over the row tiles
-    int j0;         // first key tile
+    int sees[2];    // keys that each row tile works on
+    int cnt[2];     // key tiles that each row tile (or, ALT, each half of the block) works on
+    int j0, end;    // key tiles of the block
     int tok[2];     // tokens of each row tile
 };
 
 // Whole warp; returns how many tiles of K and V were asked for.
-template <int DP>
+template <int DP, bool ALT>
 __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtensorMap *mk, const CUtensorMap *mv,
                          LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, int kvh, int qhead,
                          int qrow, int tok_per_tile, int krow, int klen) {
-    using S = LongShape<DP>;
+    using S = LongShape<DP, ALT>;
     using TL = Tile<DP>;
     volatile int *abort = &sh.abort;
-    if (r.nmax <= r.j0) return 0;
-    const int loads = 2 * (r.nmax - r.j0);
+    const int loads = 2 * (r.end - r.j0);
     int issued = 0;
     unsigned raw_phase = 0;
 #pragma unroll 1
@@ -473,8 +473,8 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
                             krow + j * S::kKeys);
         if (issued == 0) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (r.n[t] <= r.j0) continue;
+            for (int t = 0; t < (ALT ? 1 : 2); ++t) {
+                if (r.cnt[t] == 0) continue;
                 mbar_arrive_expect_one(&sh.q_full[t], box_bytes<DP>(tok_per_tile * A.pack));
 #pragma unroll
                 for (int p = 0; p < TL::kPanels; ++p)
@@ -498,18 +498,18 @@ __device__ int long_load(const AttnArgs &A, const CUtensorMap *mq, const CUtenso
 }
 
 // After a wait gave up: every copy of this block that may still be landing.
-template <int DP> __device__ void long_drain(LongShared &sh, const LongRange &r, int issued) {
-    using S = LongShape<DP>;
-    for (int t = 0; t < 2; ++t)
-        if (r.n[t] > r.j0) mbar_drain(&sh.q_full[t], 0, kAttnWaitLimit);
+template <int DP, bool ALT> __device__ void long_drain(LongShared &sh, const LongRange &r, int issued) {
+    using S = LongShape<DP, ALT>;
+    for (int t = 0; t < (ALT ? 1 : 2); ++t)
+        if (r.cnt[t] > 0) mbar_drain(&sh.q_full[t], 0, kAttnWaitLimit);
     for (int i = max(0, issued - S::kStages); i < issued; ++i)
         mbar_drain(&sh.kv_full[i % S::kStages], (i / S::kStages) & 1, kAttnWaitLimit);
 }
 
 // Whole warp.
-template <int DP>
+template <int DP, bool ALT>
 __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, uint32_t tmem) {
-    using S = LongShape<DP>;
+    using S = LongShape<DP, ALT>;
     using TL = Tile<DP>;
     constexpr uint32_t kIdO = mma_idesc(128, DP, true);
     constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
@@ -519,27 +519,30 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
     const uint64_t v_desc = smem_desc<TL::kRowBytes>(smem_kv, kLbo, kSbo);
     auto scores = [&](int t, int st, int j) {
         const uint32_t id = mma_idesc(128, tile_cols(r.sees[t], j * S::kKeys, S::kKeys), false);
-        const uint64_t a = q_desc + t * (S::kTileBytes / 16), b = k_desc + st * (S::kTileBytes / 16);
+        const uint64_t a = q_desc + (ALT ? 0 : t) * (S::kTileBytes / 16), b = k_desc + st * (S::kTileBytes / 16);
         mma_channels<DP, kLbo, kLbo>(tmem + t * 128, a, b, id);
         tc_commit_one(&sh.s_full[t]);
     };
     auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
         return wait_warp(&sh.kv_full[load % S::kStages], (load / S::kStages) & 1, abort) ? load % S::kStages : -1;
     };
-    const int n = r.nmax - r.j0;
-    int st = kv(0);
-    if (st < 0) return false;
+    // The key tile of a row tile's i-th round; its loads are the ring's 2 (j - j0) for K and the next for V.
+    auto tile = [&](int t, int i) { return r.j0 + (ALT ? 2 * i + t : i); };
+    int st = -1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        if (r.n[t] <= r.j0) continue;
-        if (!wait_warp(&sh.q_full[t], 0, abort)) return false;
+        if (r.cnt[t] == 0) continue;
+        if (ALT || st < 0)
+            if ((st = kv(2 * (tile(t, 0) - r.j0))) < 0) return false;
+        if (!wait_warp(&sh.q_full[ALT ? 0 : t], 0, abort)) return false;
         tc_fence_after();
-        scores(t, st, r.j0);
+        scores(t, st, tile(t, 0));
+        if (ALT) tc_commit_one(&sh.kv_empty[st]);
     }
-    tc_commit_one(&sh.kv_empty[st]);
+    if (!ALT) tc_commit_one(&sh.kv_empty[st]);
     // O_t += P V of tile i, each half as soon as it is written.
     auto product = [&](int t, int i, int sv) {
-        const int steps = tile_cols(r.sees[t], (r.j0 + i) * S::kKeys, S::kKeys) / 16;
+        const int steps = tile_cols(r.sees[t], tile(t, i) * S::kKeys, S::kKeys) / 16;
         const uint64_t b = v_desc + sv * (S::kTileBytes / 16);
         const uint32_t o = tmem + S::kO + t * DP, p = tmem + S::kP + t * S::kPStep;
 #pragma unroll
@@ -557,46 +560,51 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
         tc_commit_one(&sh.o_done[t]);
         return true;
     };
+    const int n = max(r.cnt[0], r.cnt[1]);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
         int sv = -1, sk = -1;
         if (S::kOwnP) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (r.n[t] - r.j0 - i <= 1) continue;
+                if (r.cnt[t] - i <= 1) continue;
                 if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
                 if (!wait_warp(&sh.s_free[t], i & 1, abort)) return false;
                 tc_fence_after();
-                scores(t, sk, r.j0 + i + 1);
+                scores(t, sk, tile(t, i + 1));
             }
             if (sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int left = r.n[t] - r.j0 - i;  // key tiles of this row tile from here on
+            const int left = r.cnt[t] - i;  // key tiles of this row tile from here on
             if (left > 0) {
-                if (sv < 0 && (sv = kv(2 * i + 1)) < 0) return false;
+                if (ALT || sv < 0)
+                    if ((sv = kv(2 * (tile(t, i) - r.j0) + 1)) < 0) return false;
                 if (!product(t, i, sv)) return false;
+                if (ALT) tc_commit_one(&sh.kv_empty[sv]);
             }
             if (!S::kOwnP && left > 1) {
-                if (sk < 0 && (sk = kv(2 * i + 2)) < 0) return false;
+                if (ALT || sk < 0)
+                    if ((sk = kv(2 * (tile(t, i + 1) - r.j0))) < 0) return false;
                 tc_fence_after();
-                scores(t, sk, r.j0 + i + 1);
+                scores(t, sk, tile(t, i + 1));
+                if (ALT) tc_commit_one(&sh.kv_empty[sk]);
             }
         }
-        if (sv >= 0) tc_commit_one(&sh.kv_empty[sv]);
-        if (!S::kOwnP && sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
+        if (!ALT && sv >= 0) tc_commit_one(&sh.kv_empty[sv]);
+        if (!ALT && !S::kOwnP && sk >= 0) tc_commit_one(&sh.kv_empty[sk]);
     }
     return true;
 }
 
-template <int DP, bool SPLIT>
-__global__ void __launch_bounds__(LongShape<DP>::kThreads, 1)
+template <int DP, bool SPLIT, bool ALT>
+__global__ void __launch_bounds__(LongShape<DP, ALT>::kThreads, 1)
 attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                          bf16 *__restrict__ out, float *__restrict__ lse, float *__restrict__ part,
                          float *__restrict__ part_lse, int slots) {
-    using S = LongShape<DP>;
+    using S = LongShape<DP, ALT>;
     extern __shared__ unsigned char dyn[];
     __shared__ LongShared sh;
     const int warp = warp_index();
@@ -611,25 +619,25 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
 
     LongRange r;
-    r.nmax = 0;
+    int n[2];  // key tiles of each row tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        r.tok[t] = min(per, max(0, q.len - q.first - t * per));
-        const int last = q.first + t * per + r.tok[t] - 1;
+        const int first = q.first + (ALT ? 0 : t * per);
+        r.tok[t] = min(per, max(0, q.len - first));
+        const int last = first + r.tok[t] - 1;
         r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
-        r.n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
-        r.nmax = max(r.nmax, r.n[t]);
+        n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
     }
     r.j0 = 0;
+    r.end = max(n[0], n[1]);
     if (SPLIT) {
-        const int each = (r.nmax + (int)gridDim.z - 1) / (int)gridDim.z;
-        r.j0 = min(r.nmax, each * (int)blockIdx.z);
-        const int end = min(r.nmax, r.j0 + each);
-        for (int t = 0; t < 2; ++t) r.n[t] = max(r.j0, min(r.n[t], end));
-        r.nmax = end;
-        part += (size_t)blockIdx.z * A.Tq * A.Hq * A.D;
-        part_lse += (size_t)blockIdx.z * A.Tq * A.Hq;
+        const int each = (r.end + (int)gridDim.z - 1) / (int)gridDim.z;
+        r.j0 = min(r.end, each * (int)blockIdx.z);
+        r.end = min(r.end, r.j0 + each);
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        r.cnt[t] = ALT ? (r.end - r.j0 + 1 - t) / 2 : max(0, min(n[t], r.end) - r.j0);
 
     if (warp == 8) {
         if ((threadIdx.x & 31) == 0) {
@@ -664,9 +672,9 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     if (warp >= 8) {
         regs_less<S::Regs::kLess>();
         if (warp == 8) {
-            if (r.nmax > r.j0) long_mma_loop<DP>(sh, smem_q, smem_kv, r, tmem);
+            if (r.end > r.j0) long_mma_loop<DP, ALT>(sh, smem_q, smem_kv, r, tmem);
         } else if (warp == 9) {
-            issued = long_load<DP>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
+            issued = long_load<DP, ALT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
                                    klen);
         }
     } else {
@@ -678,21 +686,21 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + S::kO + t * DP;
             const uint32_t tp = tmem + lane_base + S::kP + t * S::kPStep;
             const int row = threadIdx.x & 127;
-            const int tok_first = q.first + t * per, tok = tok_first + row_token(A, row);
+            const int tok_first = q.first + (ALT ? 0 : t * per), tok = tok_first + row_token(A, row);
             const bool live = row_token(A, row) < r.tok[t];
             const bool warp_live = (row & ~31) < r.tok[t] * A.pack;
             const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
             // Keys that every row of the tile sees (rows past the last token do not count).
             const int all_see = A.causal ? min(klen, tok_first + 1 + klen - q.len) : klen;
             RowState rs{-INFINITY, 0.0f};
-            const int n = r.n[t] - r.j0;
+            const int n = r.cnt[t];
             bool ok = true;
 #pragma unroll 1
             for (int i = 0; i < n && ok; ++i) {
                 ok = wait_warp(&sh.s_full[t], i & 1, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const int k0 = (r.j0 + i) * S::kKeys;
+                const int k0 = (r.j0 + (ALT ? 2 * i + t : i)) * S::kKeys;
                 auto loaded = [&] {
                     if (!S::kOwnP) return;
                     tc_fence_before();
@@ -723,15 +731,16 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             }
             if (ok && n > 0) ok = wait_warp(&sh.o_done[t], (n - 1) & 1, abort);
             tc_fence_after();
+            const size_t which = ALT ? 2 * blockIdx.z + t : blockIdx.z;  // of the parts
             if (ok)
-                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse, part,
-                                     part_lse);
+                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse,
+                                     part + which * A.Tq * A.Hq * A.D, part_lse + which * A.Tq * A.Hq);
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0) long_drain<DP>(sh, r, issued);
+    if (sh.abort && warp == 9 && (threadIdx.x & 31) == 0) long_drain<DP, ALT>(sh, r, issued);
     if (warp == 8) {
         if (sh.abort) {
             tc_commit_one(&sh.drain);
@@ -980,8 +989,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
 }
 
 // o = sum_s w_s part_s with w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s).  Eight channels
-// per thread; a part that saw no keys (lse -inf) has weight 0 and is not read.
-__global__ void __launch_bounds__(256)
+// per thread.  A part that saw no keys has lse -inf, weight 0 and wrote zeros.
+__global__ void __launch_bounds__(128)
 attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, int splits, long long rows, int Hq,
                  int Tq, int D, bf16 *__restrict__ out, float *__restrict__ lse) {
     const int per = D / 8;
@@ -992,17 +1001,18 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
     const long long token = row / Hq;
     const int head = (int)(row % Hq);
     const float *pl = part_lse + (size_t)head * Tq + token;
+    const float *px = part + row * D + c;
     float top = -INFINITY;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, pl[(size_t)s * rows]);
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, __ldg(pl + (size_t)s * rows));
+    const float ref = top == -INFINITY ? 0.0f : top;
     float total = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-        const float l = pl[(size_t)s * rows];
-        if (l == -INFINITY) continue;
-        const float w = expf(l - top);
+        const float w = expf(__ldg(pl + (size_t)s * rows) - ref);
         total += w;
         float x[8];
-        load_vec<float, 8, true>(part + (size_t)s * rows * D + row * D + c, x);
+        load_vec<float, 8, true>(px + (size_t)s * rows * D, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = fmaf(w, x[e], o[e]);
     }
@@ -1605,55 +1615,65 @@ int check_tensor(const Strided &t, int64_t T, int64_t H) {
 // Which forward kernel, and over how many blocks each row tile's keys are split.
 struct ForwardPlan {
     bool is_short;
-    int splits;
+    int splits;     // blocks to a row tile's keys
+    bool alternate; // the two halves of such a block take key tiles in turn
+    int parts() const { return alternate ? 2 * splits : splits; }
 };
 
 ForwardPlan plan_forward(const AttnArgs &A) {
-    ForwardPlan p{false, 1};
+    ForwardPlan p{false, 1, false};
     const int per = 128 / A.pack;
     const long long heads = (long long)A.Hkv * A.subs;
     const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
     const long long rows = A.Tq / n_seq, keys = A.Tk / n_seq;  // of the mean sequence
-    // Blocks of two row tiles, if every sequence were the mean one.
-    const long long blocks = heads * n_seq * ((rows + 2 * per - 1) / (2 * per));
+    // One row tile to a sequence, its keys taken by halves; or blocks of two row tiles, if every sequence were
+    // the mean one.
+    const bool single = rows <= per;
+    const long long blocks = heads * n_seq * (single ? 1 : (rows + 2 * per - 1) / (2 * per));
     const long long tiles = (keys + 127) / 128;
     const KnobValue forced = knob(kKnobAttnFwd);
     if (forced.count > 0 && forced.v[0] > 0) {
         p.is_short = forced.v[0] == 2;
         p.splits = p.is_short || forced.v[1] < 1 ? 1 : forced.v[1] > 64 ? 64 : forced.v[1];
+        p.alternate = forced.v[0] == 3;
         return p;
     }
-    // Few blocks with many keys: split until there are two to an SM (the lengths differ), with four key
-    // tiles at least to a part.  8 x 300 queries over 0 to 4000 keys, 8 heads of 80: 42.8 us in two parts, 58.4
-    // in one; one token each over 1 to 16384 keys, 4 key heads of 128: 57.5 us in 4 to 8 parts, 188 in one.
-    long long s = 2ll * num_sms() / (blocks > 0 ? blocks : 1);
-    if (s > tiles / 4) s = tiles / 4;
-    if (s >= 2) {
-        p.splits = (int)(s > 64 ? 64 : s);
-        return p;
-    }
+    // Few blocks with many keys: split into one block to an SM, or, where the keys are other tokens and their
+    // lengths may differ from block to block, in two even if that leaves some SMs with two; four key tiles at
+    // least to a block (eight in turn).  One token over 30,000 keys, 32 / 8
+    // heads of 128: 334 us whole, 42.3 in 16, 58.3 in 37; 4 x 64 tokens over 8000 keys, 16 / 4: 107.7 whole, 34.8 in 9,
+    // 47.5 in 18; 8 x 300 over 0 to 4000 keys, 8 of 80: 58 whole, 42 in two, but 2048 causal
+    // tokens, 16 / 4 of 128: 35.0 whole, 42.9 in two.  Halves in turn: one token each over
+    // 1 to 16384 keys, 16 / 4 heads of 128: 47.1 us in 4, 54.2 without in 9.
+    long long s = num_sms() / (blocks > 0 ? blocks : 1);
+    if (s < 2 && A.Tq != A.Tk) s = (3ll * num_sms() / 2 + blocks / 2) / (blocks > 0 ? blocks : 1);
+    if (s > tiles / (single ? 8 : 4)) s = tiles / (single ? 8 : 4);
+    p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    p.alternate = single && tiles >= 4;
+    if (p.parts() > 1) return p;
     // 104 x 300 tokens, 8 heads of 32: 62 us in the short kernel, 103 in the long one; 32 x 145, 6 of 64: 12.7
     // and 16.2; 16 of 1 to 1601, 6 of 64: 52.6 and 52.8; 8 x 300 over 0 to 4000 keys, 8 of 80: 100 and 58.
     p.is_short = rows <= 4 * per && keys <= 512;
     return p;
 }
 
-size_t split_bytes(const AttnArgs &A, int splits) {
-    return splits <= 1 ? 0 : (size_t)splits * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
+size_t split_bytes(const AttnArgs &A, int parts) {
+    return parts <= 1 ? 0 : (size_t)parts * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
 }
 
 template <int DP>
 int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
                    bf16 *out, float *lse, float *part, float *part_lse, cudaStream_t stream) {
-    const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP>::kKeys;
+    const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP, false>::kKeys;
     CUtensorMap mq, mk, mv;
     if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, keys, q.p) ||
         !make_map(&mv, v, A.Tk, A.Hkv, A.D, 1, keys, q.p))
         return RFDETR_ERR_CUDA;
-    const long long slots = slots_for(A.Tq, plan.is_short ? per : per * 2, A.n_seq);
+    const int slot_rows = plan.is_short || plan.alternate ? per : per * 2;
+    const long long slots = slots_for(A.Tq, slot_rows, A.n_seq);
     const long long blocks = slots * A.Hkv * A.subs;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    A.slot_rows = divisor(plan.is_short ? per : per * 2);
+    A.slot_rows = divisor(slot_rows);
     A.heads = divisor(A.Hkv * A.subs);
     const dim3 grid((unsigned)blocks, 1, (unsigned)plan.splits);
     if (plan.is_short) {
@@ -1664,21 +1684,20 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
             <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, (int)slots);
         return launch_status();
     }
-    using S = LongShape<DP>;
-    if (plan.splits > 1) {
-        if (int st = allow_smem(attn_forward_long_kernel<DP, true>, S::kSmem)) return st;
-        attn_forward_long_kernel<DP, true>
-            <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
-        if (int st = launch_status()) return st;
-        const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
-        if ((n + 255) / 256 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-        attn_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(part, part_lse, plan.splits, rows, A.Hq, A.Tq,
-                                                                         A.D, out, lse);
-    } else {
-        if (int st = allow_smem(attn_forward_long_kernel<DP, false>, S::kSmem)) return st;
-        attn_forward_long_kernel<DP, false>
-            <<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
-    }
+    using S = LongShape<DP, false>;  // (its block and shared memory are those of the alternating kernel too)
+    auto launch = [&](auto kernel) {
+        if (int st = allow_smem(kernel, S::kSmem)) return st;
+        kernel<<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
+        return launch_status();
+    };
+    if (plan.parts() == 1) return launch(attn_forward_long_kernel<DP, false, false>);
+    if (int st = plan.alternate ? launch(attn_forward_long_kernel<DP, true, true>)
+                                : launch(attn_forward_long_kernel<DP, true, false>))
+        return st;
+    const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
+    if ((n + 127) / 128 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+    attn_join_kernel<<<(unsigned)((n + 127) / 128), 128, 0, stream>>>(part, part_lse, plan.parts(), rows, A.Hq, A.Tq, A.D,
+                                                                     out, lse);
     return launch_status();
 }
 
@@ -1800,7 +1819,7 @@ extern "C" size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, i
     if (check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim) != RFDETR_OK) return 0;
     const AttnArgs A = make_args(nullptr, nullptr, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, 0,
                                  1.0f, 128);
-    return split_bytes(A, plan_forward(A).splits);
+    return split_bytes(A, plan_forward(A).parts());
 }
 
 extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride,
@@ -1825,10 +1844,10 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
                                  causal, scale, 128);
     const ForwardPlan p = plan_forward(A);
-    const size_t need = split_bytes(A, p.splits);
+    const size_t need = split_bytes(A, p.parts());
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return RFDETR_ERR_WORKSPACE;
     float *part = static_cast<float *>(workspace);
-    float *part_lse = need ? part + (size_t)p.splits * A.Tq * A.Hq * A.D : nullptr;
+    float *part_lse = need ? part + (size_t)p.parts() * A.Tq * A.Hq * A.D : nullptr;
     bf16 *out = static_cast<bf16 *>(output);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (padded_dim(head_dim)) {

@@ -312,11 +312,11 @@ def test_refusals(pkg):
             call(q, k, v, o, ko, **kw)
 
 
-@pytest.mark.parametrize("knob", ["1,1", "1,3", "1,64", "2"])
+@pytest.mark.parametrize("knob", ["1,1", "1,3", "1,64", "2", "3,1", "3,3", "3,64"])
 @pytest.mark.parametrize("dim", [32, 64, 128])
 def test_every_forward_kernel(pkg, tuning, knob, dim):
-    """Both kernels, and the first with its keys split over blocks (more blocks than key tiles
-    among them), whatever the sizes would choose."""
+    """The kernels, whole and with their keys split over blocks (more blocks than key tiles among them)
+    or taken in turn by a block's halves, whatever the sizes would choose."""
     tuning("RFDETR_ATTN_FWD", knob)
     _check(pkg, (1, 300, 0, 517, 64), heads=6, kv=2, dim=dim, causal=True, seed=dim)
     _check(pkg, (3, 130, 40, 7), (900, 0, 17, 129), heads=4, kv=1, dim=dim, seed=dim)
