@@ -368,7 +368,9 @@ int rfdetr_allreduce_sum_f32(void *stream, float *const *buffers, unsigned *cons
  *   offsets, key_offsets  device int32 [n_sequences + 1], ascending: sequence s is rows
  *           offsets[s] .. offsets[s + 1] - 1 of query and key_offsets[s] .. of key and value;
  *           key_offsets may be NULL (the same as offsets).  Values are clamped to the tensors.
- *   output  [tokens, n_heads, head_dim] bf16 contiguous;  lse [n_heads, tokens] f32 or NULL
+ *   output  [tokens, n_heads, head_dim] bf16 contiguous;  lse [n_heads, tokens] f32 or NULL;
+ *   output_low  as output, or NULL: what each result lost in its rounding to bf16, itself as bf16.  The backward
+ *           call needs it (its output . grad_output is taken from both).
  * Query i of sequence s sees its keys j, with `causal` those with j <= i + Lk - Lq.  Head h reads
  * key head h / (n_heads / n_kv_heads).  A query that sees no key, and every row outside all
  * sequences, gets output 0 and lse -inf; such rows of query, key and value have gradient 0.
@@ -384,17 +386,17 @@ size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, int64_t toke
 int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride,
                             const void *key, int64_t key_token_stride, int64_t key_head_stride,
                             const void *value, int64_t value_token_stride, int64_t value_head_stride,
-                            const int32_t *offsets, const int32_t *key_offsets, void *output, float *lse,
-                            void *workspace, size_t workspace_bytes, int64_t n_sequences, int64_t tokens,
-                            int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int causal,
-                            float scale);
+                            const int32_t *offsets, const int32_t *key_offsets, void *output, void *output_low,
+                            float *lse, void *workspace, size_t workspace_bytes, int64_t n_sequences,
+                            int64_t tokens, int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads,
+                            int64_t head_dim, int causal, float scale);
 size_t rfdetr_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t n_heads);
 int rfdetr_packed_attention_backward(void *stream, const void *query, int64_t query_token_stride,
                                      int64_t query_head_stride, const void *key, int64_t key_token_stride,
                                      int64_t key_head_stride, const void *value, int64_t value_token_stride,
                                      int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
-                                     const void *output, const float *lse, const void *grad_output,
-                                     int64_t grad_token_stride, int64_t grad_head_stride, const float *grad_lse,
+                                     const void *output, const void *output_low, const float *lse,
+                                     const void *grad_output, int64_t grad_token_stride, int64_t grad_head_stride, const float *grad_lse,
                                      void *grad_query, void *grad_key, void *grad_value, void *workspace,
                                      size_t workspace_bytes, int64_t n_sequences, int64_t tokens, int64_t key_tokens,
                                      int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int causal, float scale);

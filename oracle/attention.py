@@ -23,6 +23,7 @@ def attention(q, k, v, offsets, key_offsets=None, causal=False, scale=None, grad
     * dv:   U sum_i P |g_i| + U |dv|;
     * delta = sum_d g o is off by U sum_d |g| (|o| + sum_j P |v_j|), so dS by U |dS| + P times
       that, and dq and dk by those times scale |k| and scale |q|, plus U of themselves.
+      (With the part that o's rounding lost kept beside it, the |o| term is slack.)
     """
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     T, H, D = q.shape

@@ -41,26 +41,28 @@ def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
         raise ValueError(f"{name} must ascend within [0, {total}]")
 
 
-def attention_forward(query, key, value, offsets, key_offsets, causal, scale, want_lse):
-    """One forward call; inputs already checked.  Returns ``(output, lse or None)``."""
+def attention_forward(query, key, value, offsets, key_offsets, causal, scale, want_lse, want_low):
+    """One forward call; inputs already checked.  Returns ``(output, lse or None, low or None)``, low being
+    what the output lost in its rounding to bf16 (the backward pass reads it)."""
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
     sequences = offsets.numel() - 1
     out = query.new_empty((tokens, heads, dim))
     lse = query.new_empty((heads, tokens), dtype=torch.float32) if want_lse else None
+    low = query.new_empty((tokens, heads, dim)) if want_low else None
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
     workspace = query.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     status = lib.rfdetr_packed_attention(
         N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
-        out.data_ptr(), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads, kv_heads, dim,
+        out.data_ptr(), N.ptr(low), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads, kv_heads, dim,
         int(causal), scale)
     N.check(status, "rfdetr_packed_attention")
-    return out, lse
+    return out, lse, low
 
 
-def attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, lse, grad_output, grad_lse):
+def attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, low, lse, grad_output, grad_lse):
     """One backward call; returns ``(grad_query, grad_key, grad_value)``, contiguous."""
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
@@ -74,7 +76,7 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
     status = lib.rfdetr_packed_attention_backward(
         N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
-        out.data_ptr(), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
+        out.data_ptr(), N.ptr(low), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
         N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
         offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale)
     N.check(status, "rfdetr_packed_attention_backward")
@@ -82,12 +84,13 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
 
 
 class PackedAttentionFunction(torch.autograd.Function):
-    """Forward keeps the output and the log-sum-exp; backward forms the weights again from them."""
+    """Forward keeps the output (and what its rounding lost) and the log-sum-exp; backward forms the weights
+    again from them."""
 
     @staticmethod
     def forward(ctx, query, key, value, offsets, key_offsets, causal, scale):
-        out, lse = attention_forward(query, key, value, offsets, key_offsets, causal, scale, True)
-        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, lse)
+        out, lse, low = attention_forward(query, key, value, offsets, key_offsets, causal, scale, True, True)
+        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, low, lse)
         ctx.how = (causal, scale)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -95,12 +98,13 @@ class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output, grad_lse):
-        query, key, value, offsets, key_offsets, out, lse = ctx.saved_tensors
+        query, key, value, offsets, key_offsets, out, low, lse = ctx.saved_tensors
         if grad_output is None and grad_lse is None:
             return (None,) * 7
         if grad_output is None:
             grad_output = torch.zeros_like(out)
-        grads = attention_backward(query, key, value, offsets, key_offsets, *ctx.how, out, lse, grad_output, grad_lse)
+        grads = attention_backward(query, key, value, offsets, key_offsets, *ctx.how, out, low, lse, grad_output,
+                                   grad_lse)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
 
@@ -158,5 +162,6 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)
     else:
-        out, lse = attention_forward(query, key, value, offsets, key_offsets, bool(causal), scale, return_lse)
+        out, lse, _ = attention_forward(query, key, value, offsets, key_offsets, bool(causal), scale, return_lse,
+                                        False)
     return (out, lse) if return_lse else out

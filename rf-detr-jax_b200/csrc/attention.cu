@@ -214,8 +214,8 @@ struct RowState {
 };
 
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
-// the FMA pipe (prompts of 10,052 tokens, 16 / 4 heads of 128: 156 us without, 152 with one, 151 with two of
-// eight for the 8192-token one).  The short kernel, whose four blocks hide more, gains nothing by it.
+// the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
+// with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
 template <int N, bool POLY>
 __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
     const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
@@ -360,47 +360,56 @@ __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
 }
 
-// Whole warp: a row's result from O (or zeros) and its log-sum-exp.
+// Where results go.  `low` is what a result lost in its rounding to bf16, itself in bf16, for the backward
+// pass: delta = o.g taken from the rounded o alone is off by as much as dS's own rounding in short sequences.
+struct FwdOut {
+    bf16 *out, *low;         // low, lse: or null
+    float *lse;
+    float *part, *part_lse;  // parts of split keys
+};
+
+// Eight values of a result and, where that is wanted, what their rounding lost.
+__device__ __forceinline__ void store_result(const FwdOut &f, size_t at, const float *v) {
+    store_vec<bf16, 8>(f.out + at, v);
+    if (f.low) {
+        float rest[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rest[e] = v[e] - to_f32(from_f32<bf16>(v[e]));
+        store_vec<bf16, 8>(f.low + at, rest);
+    }
+}
+
+// Whole warp: a row's result from O (or zeros) and its log-sum-exp; with SPLIT as part `which`.
 template <int DP, bool SPLIT>
-__device__ __forceinline__ void write_row(const AttnArgs &A, const RowState &r, uint32_t to, bool any, bool live,
-                                          size_t token, int head, bf16 *out, float *lse, float *part,
-                                          float *part_lse) {
+__device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, size_t which, const RowState &r,
+                                          uint32_t to, bool any, bool live, size_t token, int head) {
     const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
     if (live) {
         const float l = r.sum == 0.0f ? -INFINITY : r.m * A.scale + logf(r.sum);
-        if (SPLIT) part_lse[(size_t)head * A.Tq + token] = l;
-        else if (lse) lse[(size_t)head * A.Tq + token] = l;
+        if (SPLIT) f.part_lse[(which * A.Hq + head) * A.Tq + token] = l;
+        else if (f.lse) f.lse[(size_t)head * A.Tq + token] = l;
     }
     const size_t at = (token * A.Hq + head) * A.D;
 #pragma unroll 1
-    for (int c = 0; c < DP / 32; ++c) {
-        float o[32];
+    for (int c = 0; c < DP; c += 16) {
+        float o[16];
         if (any) {
-            tmem_ld32(to + c * 32, o);
+            tmem_ld16(to + c, o);
             tmem_wait_ld();
-            pin<32>(o);
+            pin<16>(o);
         } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            for (int e = 0; e < 16; ++e) o[e] = 0.0f;
         }
         if (!live) continue;
-        if (SPLIT) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-                if (c * 32 + e < A.D)
-                    *reinterpret_cast<float4 *>(part + at + c * 32 + e) =
-                        make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-        } else {
+        for (int e = 0; e < 16; e += 8) {
+            if (c + e >= A.D) continue;
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-                if (c * 32 + e < A.D) {
-                    uint4 w;
-                    w.x = pack_bf16(o[e] * inv, o[e + 1] * inv);
-                    w.y = pack_bf16(o[e + 2] * inv, o[e + 3] * inv);
-                    w.z = pack_bf16(o[e + 4] * inv, o[e + 5] * inv);
-                    w.w = pack_bf16(o[e + 6] * inv, o[e + 7] * inv);
-                    *reinterpret_cast<uint4 *>(out + at + c * 32 + e) = w;
-                }
+            for (int i = 0; i < 8; ++i) x[i] = o[e + i] * inv;
+            if (SPLIT) store_vec<float, 8>(f.part + which * A.Tq * A.Hq * A.D + at + c + e, x);
+            else store_result(f, at + c + e, x);
         }
     }
 }
@@ -409,10 +418,15 @@ __device__ __forceinline__ void write_row(const AttnArgs &A, const RowState &r, 
 __device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return min(keys, (sees - k0 + 15) & ~15); }
 
 // ---- long sequences: two row tiles to a block, roles by warp -------------------------------------
-// One warp loads, one thread issues the matrix products, a warpgroup serves each row tile: while the
+// One warp loads, one issues the matrix products, a warpgroup serves each row tile: while the
 // tensor core works on one tile, the other's exponentials run, and K and V are read from L2 once
 // for 256 rows.  128 keys a tile.  The warpgroups take their registers from the other two warps
 // (setmaxnreg): a row of S is 128 values.
+// What bounds it is the chain of a row tile from S through the maximum, the exponentials and P to P V, of
+// which two tiles in flight hide about half: 10,052 causal tokens of six prompts, 16 / 4 heads of 128, take
+// 129 us, 970 TFLOP/s of the products that the mask leaves (59% of the measured peak), with the tensor pipe
+// 50%, the special-function unit 45% and the issue slots 37% busy.  Four warpgroups, two to a row tile, took
+// 150 us: what each waits for is the other roles, not its own work.
 // With few row tiles the keys are split over blocks (SPLIT): each writes its normalised part in
 // float32 and its lse, and attn_join_kernel adds them by weight.  Where a sequence's queries fill one row
 // tile at most (single tokens), a second would be empty: the block's two halves then take its key
@@ -602,8 +616,7 @@ template <int DP, bool SPLIT, bool ALT>
 __global__ void __launch_bounds__(LongShape<DP, ALT>::kThreads, 1)
 attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                         bf16 *__restrict__ out, float *__restrict__ lse, float *__restrict__ part,
-                         float *__restrict__ part_lse, int slots) {
+                         const FwdOut f, int slots) {
     using S = LongShape<DP, ALT>;
     extern __shared__ unsigned char dyn[];
     __shared__ LongShared sh;
@@ -733,8 +746,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             tc_fence_after();
             const size_t which = ALT ? 2 * blockIdx.z + t : blockIdx.z;  // of the parts
             if (ok)
-                write_row<DP, SPLIT>(A, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row), out, lse,
-                                     part + which * A.Tq * A.Hq * A.D, part_lse + which * A.Tq * A.Hq);
+                write_row<DP, SPLIT>(A, f, which, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row));
         }
     }
     __syncwarp();
@@ -759,6 +771,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
 // it works (104 x 300 tokens of 8 heads of 32: blocks that come and go cost 13.7 us by themselves, and
 // finding their rows 14 more, of 62).  128 threads: each owns a row, warp 0 also issues the copies and
 // the products.  64 keys a tile, so that S and O of four blocks fit TMEM and a row of S is 64 registers.
+// Those 104 x 300 tokens take 57 us (62 with `low`), 32 x 145 of 6 heads of 64 12.0 us: latencies still (a third of the special
+// functions' rate, 42% of the issue slots); 256 threads, half a row each, took 66 and 15.3 us.
 template <int DP> struct ShortShape {
     static constexpr int kKeys = 64;
     static constexpr int kQBytes = 128 * DP * 2;
@@ -806,7 +820,7 @@ template <int DP>
 __global__ void __launch_bounds__(128, ShortShape<DP>::kBlocks)
 attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                           const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                          bf16 *__restrict__ out, float *__restrict__ lse, int slots) {
+                          const FwdOut f, int slots) {
     using S = ShortShape<DP>;
     using TL = Tile<DP>;
     constexpr int KEYS = S::kKeys;
@@ -963,8 +977,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         tc_fence_after();
         // (O is written over only after the next row tile's first barrier.)
         if (ok && it.any)
-            write_row<DP, false>(A, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok, it.qhead + row_head(A, row), out,
-                                 lse, nullptr, nullptr);
+            write_row<DP, false>(A, f, 0, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
+                                 it.qhead + row_head(A, row));
         tc_fence_before();
         g += it.n;
         if (idx >= items) break;
@@ -991,8 +1005,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
 // o = sum_s w_s part_s with w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s).  Eight channels
 // per thread.  A part that saw no keys has lse -inf, weight 0 and wrote zeros.
 __global__ void __launch_bounds__(128)
-attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, int splits, long long rows, int Hq,
-                 int Tq, int D, bf16 *__restrict__ out, float *__restrict__ lse) {
+attn_join_kernel(const FwdOut f, int splits, long long rows, int Hq, int Tq, int D) {
     const int per = D / 8;
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= rows * per) return;
@@ -1000,8 +1013,8 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
     const int c = (int)(i % per) * 8;
     const long long token = row / Hq;
     const int head = (int)(row % Hq);
-    const float *pl = part_lse + (size_t)head * Tq + token;
-    const float *px = part + row * D + c;
+    const float *pl = f.part_lse + (size_t)head * Tq + token;
+    const float *px = f.part + row * D + c;
     float top = -INFINITY;
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) top = fmaxf(top, __ldg(pl + (size_t)s * rows));
@@ -1019,8 +1032,8 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] *= inv;
-    store_vec<bf16, 8>(out + row * D + c, o);
-    if (lse && c == 0) lse[(size_t)head * Tq + token] = total == 0.0f ? -INFINITY : top + logf(total);
+    store_result(f, row * D + c, o);
+    if (f.lse && c == 0) f.lse[(size_t)head * Tq + token] = total == 0.0f ? -INFINITY : top + logf(total);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1042,6 +1055,9 @@ attn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_
 // other, their starts and ends too; with 128, two pairs alternate in one block: while one is in work, the
 // tensor core forms the other and adds the one before.  (Two pairs in one block with 64 channels: 440 against
 // 403 us for 4 x 2048 tokens of 12 heads, 392 against 277 for 104 x 300 of 8 heads of 32, forward included.)
+// What bounds it is the chain of a step, as forward: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, take
+// 310 us for dK and dV (two blocks to a tile; four products a step) and 195 us for dQ (three), 1.0 and 1.2
+// PFLOP/s of what they compute; 104 x 300 tokens, 8 heads of 32, 106 and 79 us.
 // P and dS are rounded to bf16 for the tensor core; every sum is float32.
 // A row that sees exactly one key has P = 1 whatever its score, so its dS is set to what is left of
 // it, the cotangent of its lse, rather than to the difference of two roundings of the same number.
@@ -1524,10 +1540,13 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     }
 }
 
-// delta[h][t] = o.g - c per row, LANES lanes of eight channels to a row.
+// delta[h][t] = o.g - c per row, LANES lanes of eight channels to a row; o is the output with what its rounding
+// lost (with the rounded output alone dQ and dK were off by 1.5 to 1.6 times what plain bf16 calls are, with both
+// by 1.4).  Reads three rows and writes one number: 31,200 tokens of 256 channels 8.2 us (5.8 TB/s).
 template <int LANES>
 __global__ void __launch_bounds__(256)
-attn_delta_kernel(const bf16 *__restrict__ out, const bf16 *__restrict__ g, long long g_token, long long g_head,
+attn_delta_kernel(const bf16 *__restrict__ out, const bf16 *__restrict__ low, const bf16 *__restrict__ g,
+                  long long g_token, long long g_head,
                   const float *__restrict__ g_lse, int Tq, int Hq, int D, float *__restrict__ delta) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long row = i / LANES;  // token * Hq + head
@@ -1540,6 +1559,9 @@ attn_delta_kernel(const bf16 *__restrict__ out, const bf16 *__restrict__ g, long
         float a[8], b[8];
         load_vec<bf16, 8, true>(out + row * D + c, a);
         load_vec<bf16, 8, true>(g + token * g_token + head * g_head + c, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+        load_vec<bf16, 8, true>(low + row * D + c, a);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
     }
@@ -1663,7 +1685,7 @@ size_t split_bytes(const AttnArgs &A, int parts) {
 
 template <int DP>
 int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
-                   bf16 *out, float *lse, float *part, float *part_lse, cudaStream_t stream) {
+                   const FwdOut &f, cudaStream_t stream) {
     const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP, false>::kKeys;
     CUtensorMap mq, mk, mv;
     if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, keys, q.p) ||
@@ -1678,16 +1700,16 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
     const dim3 grid((unsigned)blocks, 1, (unsigned)plan.splits);
     if (plan.is_short) {
         using S = ShortShape<DP>;
-        if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
         const long long stay = (long long)S::kBlocks * num_sms();
+        if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
         attn_forward_short_kernel<DP>
-            <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, (int)slots);
+            <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, f, (int)slots);
         return launch_status();
     }
     using S = LongShape<DP, false>;  // (its block and shared memory are those of the alternating kernel too)
     auto launch = [&](auto kernel) {
         if (int st = allow_smem(kernel, S::kSmem)) return st;
-        kernel<<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, out, lse, part, part_lse, (int)slots);
+        kernel<<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, f, (int)slots);
         return launch_status();
     };
     if (plan.parts() == 1) return launch(attn_forward_long_kernel<DP, false, false>);
@@ -1696,8 +1718,7 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
         return st;
     const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
     if ((n + 127) / 128 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    attn_join_kernel<<<(unsigned)((n + 127) / 128), 128, 0, stream>>>(part, part_lse, plan.parts(), rows, A.Hq, A.Tq, A.D,
-                                                                     out, lse);
+    attn_join_kernel<<<(unsigned)((n + 127) / 128), 128, 0, stream>>>(f, plan.parts(), rows, A.Hq, A.Tq, A.D);
     return launch_status();
 }
 
@@ -1826,7 +1847,8 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
                                        int64_t query_head_stride, const void *key, int64_t key_token_stride,
                                        int64_t key_head_stride, const void *value, int64_t value_token_stride,
                                        int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
-                                       void *output, float *lse, void *workspace, size_t workspace_bytes,
+                                       void *output, void *output_low, float *lse, void *workspace,
+                                       size_t workspace_bytes,
                                        int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
                                        int64_t n_kv_heads, int64_t head_dim, int causal, float scale) {
     using namespace rfdetr;
@@ -1838,7 +1860,7 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     if (int st = check_tensor(q, tokens, n_heads)) return st;
     if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
     if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
-    if (!output || !aligned(output, 16) || !aligned(lse, 4) || !offsets || !aligned(offsets, 4) ||
+    if (!output || !aligned(output, 16) || !aligned(output_low, 16) || !aligned(lse, 4) || !offsets || !aligned(offsets, 4) ||
         !aligned(key_offsets, 4))
         return RFDETR_ERR_ALIGN;
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
@@ -1846,14 +1868,16 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     const ForwardPlan p = plan_forward(A);
     const size_t need = split_bytes(A, p.parts());
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return RFDETR_ERR_WORKSPACE;
-    float *part = static_cast<float *>(workspace);
-    float *part_lse = need ? part + (size_t)p.parts() * A.Tq * A.Hq * A.D : nullptr;
-    bf16 *out = static_cast<bf16 *>(output);
+    FwdOut f{static_cast<bf16 *>(output), static_cast<bf16 *>(output_low), lse, nullptr, nullptr};
+    if (need) {
+        f.part = static_cast<float *>(workspace);
+        f.part_lse = f.part + (size_t)p.parts() * A.Tq * A.Hq * A.D;
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (padded_dim(head_dim)) {
-        case 32: return launch_forward<32>(A, p, q, k, v, out, lse, part, part_lse, s);
-        case 64: return launch_forward<64>(A, p, q, k, v, out, lse, part, part_lse, s);
-        default: return launch_forward<128>(A, p, q, k, v, out, lse, part, part_lse, s);
+        case 32: return launch_forward<32>(A, p, q, k, v, f, s);
+        case 64: return launch_forward<64>(A, p, q, k, v, f, s);
+        default: return launch_forward<128>(A, p, q, k, v, f, s);
     }
 }
 
@@ -1866,7 +1890,8 @@ extern "C" int rfdetr_packed_attention_backward(
     void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride, const void *key,
     int64_t key_token_stride, int64_t key_head_stride, const void *value, int64_t value_token_stride,
     int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets, const void *output,
-    const float *lse, const void *grad_output, int64_t grad_token_stride, int64_t grad_head_stride,
+    const void *output_low, const float *lse, const void *grad_output, int64_t grad_token_stride,
+    int64_t grad_head_stride,
     const float *grad_lse, void *grad_query, void *grad_key, void *grad_value, void *workspace, size_t workspace_bytes,
     int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
     int causal, float scale) {
@@ -1881,7 +1906,7 @@ extern "C" int rfdetr_packed_attention_backward(
     if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
     if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
     if (!offsets || !aligned(offsets, 4) || !aligned(key_offsets, 4)) return RFDETR_ERR_ALIGN;
-    if (tokens > 0 && (!output || !aligned(output, 16) || !grad_query || !aligned(grad_query, 16) || !lse ||
+    if (tokens > 0 && (!output || !aligned(output, 16) || !output_low || !aligned(output_low, 16) || !grad_query || !aligned(grad_query, 16) || !lse ||
                        !aligned(lse, 4) || !aligned(grad_lse, 4)))
         return RFDETR_ERR_ALIGN;
     if (key_tokens > 0 && (!grad_key || !grad_value || !aligned(grad_key, 16) || !aligned(grad_value, 16)))
@@ -1896,9 +1921,10 @@ extern "C" int rfdetr_packed_attention_backward(
         const int dp = padded_dim(head_dim);
         const long long rows = (long long)tokens * n_heads, blocks = (rows * (dp / 8) + 255) / 256;
         if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
+        const bf16 *low = static_cast<const bf16 *>(output_low);
         const bf16 *o = static_cast<const bf16 *>(output), *go = static_cast<const bf16 *>(grad_output);
         auto launch = [&](auto kernel) {
-            kernel<<<(unsigned)blocks, 256, 0, s>>>(o, go, grad_token_stride, grad_head_stride, grad_lse, (int)tokens,
+            kernel<<<(unsigned)blocks, 256, 0, s>>>(o, low, go, grad_token_stride, grad_head_stride, grad_lse, (int)tokens,
                                                     (int)n_heads, (int)head_dim, delta);
         };
         if (dp == 32) launch(attn_delta_kernel<4>);

@@ -47,8 +47,9 @@ __device__ __forceinline__ float second_of(float x1, float x2, float2 r) {
 // Pieces of VEC channels.  A head's pieces: the turned ones first (one piece of x1 and one of x2,
 // or one piece of VEC / 2 pairs), then the copied ones.  A thread asks for its first piece before the
 // sines are formed, so that their time covers the load's.  More pieces in flight per thread cost more in
-// resident threads than they gave: 32,768 tokens of 20 x 128 channels, bf16, 60.1 us (5.59 TB/s) with one, 70.3
-// with two, 87.9 with four; 20,011 of 8 x 80, partly turned, 30.7, 28.7 and 36.2 us there and back.
+// resident threads than they gave: 32,768 tokens of 20 x 128 channels, bf16, 65 us (5.2 TB/s, 81% of the
+// measured copy rate) with one, 70 with two, 88 with four; 20,011 of 8 x 80, partly turned, 30.7, 28.7 and
+// 36.2 us there and back.
 
 template <typename T, typename P, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotaryThreads) axial_rotary_kernel(const RotaryArgs A) {
@@ -202,7 +203,8 @@ extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t quer
     };
     if (!fits(vec)) vec = fits(2) ? 2 : 1;
     if (interleaved && vec < 2) return RFDETR_ERR_ALIGN;
-    // Tokens to a block: two pieces to a thread (4096 pieces a block: 71.5 us for the video tokens above),
+    // Tokens to a block: two pieces to a thread (one: 84 us for the first of the tokens above; eight: 66 us, and
+    // 35.1 for the second),
     // fewer where that would leave SMs without four blocks, and no more than 16 KB of sines.
     const long long turned = interleaved ? 2 * half / vec : half / vec;
     const long long per_token = (turned + (head_dim - 2 * half) / vec) * (n_heads + n_kv_heads);

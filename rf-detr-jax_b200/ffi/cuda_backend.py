@@ -248,11 +248,12 @@ set_losses.defvjp(_set_losses_fwd, _set_losses_bwd)
 def packed_attention(query, key, value, offsets, key_offsets, causal=False, scale=None):
     """Attention within the sequences of packed rows (the padded batches of ``layers.py:54-98``
     without their padding): ``(output [T, H, D], lse [H, T])``."""
-    return _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    out, _, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    return out, lse
 
 
 def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale):
-    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype),
+    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype), jax.ShapeDtypeStruct(query.shape, query.dtype),
             jax.ShapeDtypeStruct((query.shape[1], query.shape[0]), jnp.float32))
     return jax.ffi.ffi_call("RfdetrPackedAttention", outs)(
         query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32),
@@ -260,15 +261,15 @@ def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scal
 
 
 def _packed_attention_fwd(query, key, value, offsets, key_offsets, causal, scale):
-    out, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
-    return (out, lse), (query, key, value, offsets, key_offsets, out, lse)
+    out, low, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    return (out, lse), (query, key, value, offsets, key_offsets, out, low, lse)
 
 
 def _packed_attention_bwd(causal, scale, residuals, g):
-    query, key, value, offsets, key_offsets, out, lse = residuals
+    query, key, value, offsets, key_offsets, out, low, lse = residuals
     shapes = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key, value))
     grads = jax.ffi.ffi_call("RfdetrPackedAttentionBwd", shapes)(
-        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, lse, g[0].astype(out.dtype),
+        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, low, lse, g[0].astype(out.dtype),
         g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
         scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
     return *grads, None, None

@@ -352,3 +352,23 @@ def test_one_token_over_long_keys(pkg):
     _check(pkg, (1, 1, 1), (5000, 1, 3999), heads=8, kv=2, dim=128, causal=True, grad=False)
     _check(pkg, (1,), (7000,), heads=4, kv=4, dim=64)
     _check(pkg, (2, 0, 1), (3000, 3000, 3000), heads=7, kv=1, dim=80, causal=True)
+
+
+def test_rows_beyond_32_bit_offsets(pkg):
+    """Keys, values and cotangents whose rows lie further apart than 2^31 elements (a wide cache)."""
+    rng = np.random.default_rng(31)
+    wide = torch.empty((1400, 1_600_000), device=DEV, dtype=torch.bfloat16)  # 4.5 GB
+    rows = _bf16(rng, 1400, 8, 64)
+    wide[:, :512] = rows.view(1400, 512)
+    k, v, q, g = (wide[:, i * 128:(i + 1) * 128].view(1400, 2, 64) for i in range(4))
+    off = _offsets((100, 1300))
+    a = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    b = [x.detach().contiguous().requires_grad_(True) for x in (q, k, v)]
+    x, y = pkg.packed_attention(*a, off, causal=True), pkg.packed_attention(*b, off, causal=True)
+    assert torch.equal(x, y)
+    for d, e in zip(torch.autograd.grad(x, a, g), torch.autograd.grad(y, b, g.contiguous())):
+        assert torch.equal(d, e)
+    pos, freq = torch.rand((1400, 1), device=DEV), torch.rand(32, device=DEV)
+    for d, e in zip(pkg.axial_rotary(q, k, pos, freq, (32,)),
+                    pkg.axial_rotary(q.contiguous(), k.contiguous(), pos, freq, (32,))):
+        assert torch.equal(d, e)

@@ -9,7 +9,7 @@ import torch
 
 def _attention(N, T=4, Tk=4, H=2, Hkv=2, D=64, n=1, scale=0.1, q=16, strides=(128, 64), out=16, off=16):
     return N.lib().rfdetr_packed_attention(None, q, *strides, 16, Hkv * D, D, 16, Hkv * D, D, off, None, out, None,
-                                           None, 0, n, T, Tk, H, Hkv, D, 0, scale)
+                                           None, None, 0, n, T, Tk, H, Hkv, D, 0, scale)
 
 
 def test_attention_arguments(pkg):
@@ -25,12 +25,13 @@ def test_attention_arguments(pkg):
     assert lib.rfdetr_packed_attention_backward_workspace_bytes(100, 6) == 2400
     assert lib.rfdetr_packed_attention_backward_workspace_bytes(-1, 6) == 0
     assert lib.rfdetr_packed_attention_workspace_bytes(1, 4, 4, 3, 2, 64) == 0
-    back = lambda ws, nbytes, g=16: lib.rfdetr_packed_attention_backward(  # noqa: E731
-        None, 16, 128, 64, 16, 128, 64, 16, 128, 64, 16, None, 16, 16, g, 128, 64, None, 16, 16, 16, ws, nbytes, 1, 4,
-        4, 2, 2, 64, 0, 0.1)
+    back = lambda ws, nbytes, g=16, low=16: lib.rfdetr_packed_attention_backward(  # noqa: E731
+        None, 16, 128, 64, 16, 128, 64, 16, 128, 64, 16, None, 16, low, 16, g, 128, 64, None, 16, 16, 16, ws,
+        nbytes, 1, 4, 4, 2, 2, 64, 0, 0.1)
     assert back(None, 0) == N.ERR_WORKSPACE
     assert back(16, 31) == N.ERR_WORKSPACE
     assert back(16, 32, None) == N.ERR_ALIGN
+    assert back(16, 32, low=None) == N.ERR_ALIGN and back(16, 32, low=8) == N.ERR_ALIGN
 
 
 def test_rotary_arguments(pkg):
