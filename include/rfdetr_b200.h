@@ -54,9 +54,9 @@ int rfdetr_abi_version(void);
  *   "RFDETR_TOPK_SORT", "RFDETR_TOPK_UNSTAGED" (any value: the one-CTA sort kernels; the radix
  *   select without its shared-memory key stage),
  *   "RFDETR_ATTN_FWD" (packed attention forward: 1 the kernel for long sequences, 2 the one for
- *   short, 3 the first with a block's halves taking keys in turn; over how many blocks 1 and 3 split
- *   the keys), "RFDETR_ATTN_BWD" (its backward: how
- *   many blocks, 1, 2 or 4, share a tile of keys and a tile of queries);
+ *   short, 3 the first with one row tile a block, whose halves take its keys in turn; then, with 3, over
+ *   how many blocks to a row tile in the mean the keys are shared out), "RFDETR_ATTN_BWD" (its
+ *   backward: how many blocks, 1, 2 or 4, share a tile of keys and a tile of queries);
  * `value` is up to five comma-separated integers, or NULL / "" for the default.  Environment
  * variables of the same names are read once, before the first knob is read or set; after that
  * only this call changes a knob (launches read them from atomics, never from the environment).

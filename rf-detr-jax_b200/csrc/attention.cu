@@ -143,13 +143,16 @@ template <int GROUPS, int LAUNCH, int MORE, int LESS> struct Registers {
     static_assert(GROUPS * MORE + LESS <= (GROUPS + 1) * LAUNCH, "a warpgroup would wait for registers for good");
 };
 
-// D = A B^T over DP channels, A and B K-major tiles whose column panels are `a_panel` and `b_panel` bytes.
+// D = A B^T over DP channels, `dim` of them in use, A and B K-major tiles whose column panels are `a_panel` and
+// `b_panel` bytes.
 template <int DP, int A_PANEL, int B_PANEL>
-__device__ __forceinline__ void mma_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int dim) {
     constexpr int N = Tile<DP>::kCols / 16;  // steps in a panel
-#pragma unroll
-    for (int p = 0; p < Tile<DP>::kPanels; ++p)
-        mma_ss_one<N, 2, 2>(d, a + p * (A_PANEL / 16), b + p * (B_PANEL / 16), idesc, p > 0);
+    mma_ss_one<N, 2, 2>(d, a, b, idesc, false);
+    if constexpr (Tile<DP>::kPanels == 2) {
+        if (dim <= 96) mma_ss_one<2, 2, 2>(d, a + A_PANEL / 16, b + B_PANEL / 16, idesc, true);
+        else mma_ss_one<N, 2, 2>(d, a + A_PANEL / 16, b + B_PANEL / 16, idesc, true);
+    }
 }
 
 // Bits lo .. hi - 1 of a word.
@@ -365,7 +368,8 @@ __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_
 struct FwdOut {
     bf16 *out, *low;         // low, lse: or null
     float *lse;
-    float *part, *part_lse;  // parts of split keys
+    float *part, *part_lse;  // of shared-out keys, by block: [blocks][part_rows][D] and [blocks][part_rows]
+    int part_rows;
 };
 
 // Eight values of a result and, where that is wanted, what their rounding lost.
@@ -379,19 +383,24 @@ __device__ __forceinline__ void store_result(const FwdOut &f, size_t at, const f
     }
 }
 
-// Whole warp: a row's result from O (or zeros) and its log-sum-exp; with SPLIT as part `which`.
-template <int DP, bool SPLIT>
-__device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, size_t which, const RowState &r,
-                                          uint32_t to, bool any, bool live, size_t token, int head) {
+// Whole warp: a row's result from O (or zeros) and its log-sum-exp.  With PAIR columns `from` .. `end` of a row's sum
+// of two, O times `times` and `other` (the first column's place) times `more`; where `part_row` is not negative,
+// to that row of the parts.
+template <int DP, bool PAIR>
+__device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, long long part_row, const RowState &r,
+                                          uint32_t to, bool any, bool live, size_t token, int head, int from = 0,
+                                          int end = DP, float times = 1.0f, const float *other = nullptr,
+                                          float more = 0.0f) {
     const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
-    if (live) {
+    const bool is_part = PAIR && part_row >= 0;
+    if (live && from == 0) {
         const float l = r.sum == 0.0f ? -INFINITY : r.m * A.scale + logf(r.sum);
-        if (SPLIT) f.part_lse[(which * A.Hq + head) * A.Tq + token] = l;
+        if (is_part) f.part_lse[part_row] = l;
         else if (f.lse) f.lse[(size_t)head * A.Tq + token] = l;
     }
-    const size_t at = (token * A.Hq + head) * A.D;
+    const size_t at = (is_part ? (size_t)part_row : token * A.Hq + head) * A.D;
 #pragma unroll 1
-    for (int c = 0; c < DP; c += 16) {
+    for (int c = PAIR ? from : 0; c < (PAIR ? end : DP); c += 16) {
         float o[16];
         if (any) {
             tmem_ld16(to + c, o);
@@ -406,9 +415,20 @@ __device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, si
         for (int e = 0; e < 16; e += 8) {
             if (c + e >= A.D) continue;
             float x[8];
+            if (PAIR) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = o[e + i] * inv;
-            if (SPLIT) store_vec<float, 8>(f.part + which * A.Tq * A.Hq * A.D + at + c + e, x);
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 y = *reinterpret_cast<const float4 *>(other + (c - from) + e + i);
+                    x[i] = fmaf(y.x, more, o[e + i] * times) * inv;
+                    x[i + 1] = fmaf(y.y, more, o[e + i + 1] * times) * inv;
+                    x[i + 2] = fmaf(y.z, more, o[e + i + 2] * times) * inv;
+                    x[i + 3] = fmaf(y.w, more, o[e + i + 3] * times) * inv;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = o[e + i] * inv;
+            }
+            if (is_part) store_vec<float, 8>(f.part + at + c + e, x);
             else store_result(f, at + c + e, x);
         }
     }
@@ -427,10 +447,10 @@ __device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return mi
 // 129 us, 970 TFLOP/s of the products that the mask leaves (59% of the measured peak), with the tensor pipe
 // 50%, the special-function unit 45% and the issue slots 37% busy.  Four warpgroups, two to a row tile, took
 // 150 us: what each waits for is the other roles, not its own work.
-// With few row tiles the keys are split over blocks (SPLIT): each writes its normalised part in
-// float32 and its lse, and attn_join_kernel adds them by weight.  Where a sequence's queries fill one row
-// tile at most (single tokens), a second would be empty: the block's two halves then take its key
-// tiles in turn, each with sums of its own that make a part (ALT).
+// Where the launch has no more row tiles than SMs, two to a block would leave SMs without one: a block has one, and
+// its two halves take the key tiles in turn, each with sums of its own, which they add at the end through
+// shared memory (ALT).  With few row tiles their keys are also shared out over blocks (SPLIT): each writes its
+// normalised part in float32 and its lse, and attn_join_kernel adds them by weight.
 template <int DP, bool ALT> struct LongShape {
     static constexpr int kKeys = 128;
     static constexpr int kTileBytes = 128 * DP * 2;
@@ -439,6 +459,8 @@ template <int DP, bool ALT> struct LongShape {
     using Regs = Registers<2, 168, 208, 88>;  // 65536 / 384 -> 168
     static constexpr int kTmem = 512;
     static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes;
+    static constexpr int kLeast = 8;  // key tiles to a block where they are shared out
+    static_assert(!ALT || 128 * (DP + 8) * 4 <= kStages * kTileBytes, "the halves' sums");
     // TMEM: S of both tiles (2 x 128), O of both (2 x DP), and P (2 x 64) where there is room for it;
     // with 128 channels there is none and P lies over S.  P of its own lets the next S be formed while
     // this one's exponentials run.
@@ -449,6 +471,7 @@ struct LongShared {
     uint64_t q_full[2], kv_full[4], kv_raw, kv_empty[4], s_full[2], s_free[2], p_half[2][2], o_done[2], drain;
     uint32_t tmem;
     int abort;
+    long long part_row;  // of the block's first row among the parts; negative: its results are whole
 };
 
 struct LongRange {
@@ -457,6 +480,129 @@ struct LongRange {
     int j0, end;    // key tiles of the block
     int tok[2];     // tokens of each row tile
 };
+
+// Shared-out keys.  The host does not know the lengths, so each block looks at all of them: a slot with w key
+// tiles gets ceil(w / c) blocks a head, with the smallest c that the launch's blocks allow.  Eight single tokens
+// over 1 to 16384 keys, 16 / 4 heads of 128, take 40.5 us, of them 3.5 until a block has its share, 26 for
+// its keys (5.9 TB/s all together), 7 for the join; with four blocks to each slot, whatever its length, 48.
+constexpr int kSharedSlots = 384;  // at most, so that a thread sees to each
+
+struct SharedOut {
+    int off[kSharedSlots + 3], other[kSharedSlots + 3];  // rows and keys at which the extended sequences begin
+    int tiles[kSharedSlots];                             // of each slot; 0 only where it has no rows
+};
+
+// As find_slot, from the copy of the offsets, by one thread.
+__device__ __forceinline__ Slot shared_slot(const AttnArgs &A, const SharedOut &so, int slot) {
+    int lo = 0, n = A.n_seq + 2;  // the last x among lo .. lo + n - 1 that begins at or before the slot
+#pragma unroll 1
+    while (n > 1) {
+        const int half = n >> 1;
+        const bool before = quotient(so.off[lo + half], A.slot_rows) + lo + half <= slot;
+        lo += before ? half : 0;
+        n = before ? n - half : half;
+    }
+    Slot r;
+    r.base = so.off[lo];
+    r.len = max(0, so.off[lo + 1] - r.base);
+    const int ahead = slot - (quotient(r.base, A.slot_rows) + lo);
+    r.first = ahead > quotient(r.len, A.slot_rows) ? r.len : ahead * A.slot_rows.d;
+    const bool real = lo >= 1 && lo <= A.n_seq;
+    r.other_base = real ? so.other[lo] : 0;
+    r.other_len = real ? max(0, so.other[lo + 1] - r.other_base) : 0;
+    return r;
+}
+
+// All threads of a block (two barriers).
+__device__ __forceinline__ void count_tiles(const AttnArgs &A, SharedOut &so, int slots) {
+#pragma unroll 1
+    for (int x = threadIdx.x; x < A.n_seq + 3; x += blockDim.x) {
+        so.off[x] = off_at(A.q_off, A.n_seq, A.Tq, x);
+        so.other[x] = off_at(A.k_off, A.n_seq, A.Tk, x);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int x = threadIdx.x; x < slots; x += blockDim.x) {
+        const Slot q = shared_slot(A, so, x);
+        const int end = min(q.len, q.first + A.slot_rows.d);
+        const int sees = A.causal ? min(q.other_len, max(0, end + q.other_len - q.len)) : q.other_len;
+        so.tiles[x] = q.first >= q.len ? 0 : max(1, (sees + 127) / 128);
+    }
+    __syncthreads();
+}
+
+// Whole warp: the smallest c, and `least` at least, with which a launch of `blocks` suffices: sum ceil(w / c) of all
+// slots and heads.  There are at least as many blocks as slots times heads.
+__device__ __forceinline__ unsigned share_size(const AttnArgs &A, const SharedOut &so, int slots, unsigned least,
+                                               unsigned blocks) {
+    const unsigned lane = threadIdx.x & 31, heads = A.heads.d;
+    unsigned total = 0, live = 0, most = 0;  // total: at most 384 slots of 2^23 tiles
+#pragma unroll 1
+    for (int x = lane; x < slots; x += 32) {
+        const unsigned w = so.tiles[x];
+        total += w;
+        live += w > 0;
+        most = max(most, w);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    live = __reduce_add_sync(0xffffffffu, live);
+    most = __reduce_max_sync(0xffffffffu, most);
+    const unsigned long long all = (unsigned long long)total * heads;
+    auto over = [&](unsigned n) {  // all / n, rounded up
+        if (all >> 31) return (unsigned)min((all + n - 1) / n, 0x7fffffffull);
+        return ((unsigned)all + n - 1) / n;
+    };
+    const unsigned spare = blocks - live * heads;
+    unsigned lo = max(least, over(blocks));
+    unsigned hi = max(lo, most);  // a block to each; and as ceil(w / c) < w / c + 1:
+    if (spare > 0) hi = min(hi, max(lo, over(spare)));
+#pragma unroll 1
+    while (lo < hi) {
+        const unsigned c = (lo + hi) / 2;
+        unsigned n = 0;
+#pragma unroll 1
+        for (int x = lane; x < slots; x += 32) n += (so.tiles[x] + c - 1) / c;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n * heads <= blocks) hi = c;
+        else lo = c + 1;
+    }
+    return lo;
+}
+
+struct Share {
+    int slot, head;    // slot -1: nothing left for this block
+    int which, parts;  // of the slot's key tiles
+};
+
+// Whole warp: block b's share, c key tiles at most.
+__device__ __forceinline__ Share find_share(const AttnArgs &A, const SharedOut &so, int slots, unsigned c, int b) {
+    const int lane = threadIdx.x & 31, heads = A.heads.d;
+    int before = 0;
+#pragma unroll 1
+    for (int x0 = 0; x0 < slots; x0 += 32) {
+        const int parts = x0 + lane < slots ? (so.tiles[x0 + lane] + c - 1) / c : 0;
+        int upto = parts * heads;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        upto += before;
+        const unsigned m = __ballot_sync(0xffffffffu, upto > b);
+        if (m) {
+            const int p = __ffs(m) - 1;
+            Share r;
+            r.slot = x0 + p;
+            r.parts = __shfl_sync(0xffffffffu, parts, p);
+            const int rest = b - (__shfl_sync(0xffffffffu, upto, p) - r.parts * heads);
+            r.which = quotient(rest, A.heads);
+            r.head = rest - r.which * heads;
+            return r;
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {-1, 0, 0, 0};
+}
 
 // Whole warp; returns how many tiles of K and V were asked for.
 template <int DP, bool ALT>
@@ -522,10 +668,11 @@ template <int DP, bool ALT> __device__ void long_drain(LongShared &sh, const Lon
 
 // Whole warp.
 template <int DP, bool ALT>
-__device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, uint32_t tmem) {
+__device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv, const LongRange &r, uint32_t tmem,
+                              int dim) {
     using S = LongShape<DP, ALT>;
     using TL = Tile<DP>;
-    constexpr uint32_t kIdO = mma_idesc(128, DP, true);
+    const uint32_t id_o = mma_idesc(128, (dim + 15) & ~15, true);
     constexpr uint32_t kSbo = 8 * TL::kRowBytes, kLbo = 128 * TL::kRowBytes;
     volatile int *abort = &sh.abort;
     const uint64_t q_desc = smem_desc<TL::kRowBytes>(smem_q, 16, kSbo);
@@ -534,7 +681,7 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
     auto scores = [&](int t, int st, int j) {
         const uint32_t id = mma_idesc(128, tile_cols(r.sees[t], j * S::kKeys, S::kKeys), false);
         const uint64_t a = q_desc + (ALT ? 0 : t) * (S::kTileBytes / 16), b = k_desc + st * (S::kTileBytes / 16);
-        mma_channels<DP, kLbo, kLbo>(tmem + t * 128, a, b, id);
+        mma_channels<DP, kLbo, kLbo>(tmem + t * 128, a, b, id, dim);
         tc_commit_one(&sh.s_full[t]);
     };
     auto kv = [&](int load) {  // waits for a load of the ring; returns its stage or -1
@@ -564,11 +711,11 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
             if (!wait_warp(&sh.p_half[t][h], i & 1, abort)) return false;
             tc_fence_after();
             if (steps == 8) {
-                mma_ts_one<4, TL::kRowBytes>(o, p + h * 32, b + h * 4 * TL::kRowBytes, kIdO, i > 0 || h > 0);
+                mma_ts_one<4, TL::kRowBytes>(o, p + h * 32, b + h * 4 * TL::kRowBytes, id_o, i > 0 || h > 0);
             } else {
 #pragma unroll 1
                 for (int k = h * 4; k < min(steps, h * 4 + 4); ++k)
-                    mma_ts_one<1, 0>(o, p + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                    mma_ts_one<1, 0>(o, p + k * 8, b + k * TL::kRowBytes, id_o, i > 0 || k > 0);
             }
         }
         tc_commit_one(&sh.o_done[t]);
@@ -612,47 +759,22 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
     return true;
 }
 
-template <int DP, bool SPLIT, bool ALT>
+// The two halves of an ALT block's warpgroups.
+__device__ __forceinline__ void half_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <int DP, bool ALT, bool SPLIT>
 __global__ void __launch_bounds__(LongShape<DP, ALT>::kThreads, 1)
 attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                          const FwdOut f, int slots) {
+    static_assert(ALT || !SPLIT, "keys are shared out by single row tiles");
     using S = LongShape<DP, ALT>;
     extern __shared__ unsigned char dyn[];
     __shared__ LongShared sh;
     const int warp = warp_index();
-    const int s = quotient(blockIdx.x, A.heads), hx = blockIdx.x - s * A.heads.d;
-    // Later slots first: under a causal mask they see more keys.
-    const int slot = slots - 1 - s;
     const int per = 128 / A.pack;  // tokens in a row tile
-    const Slot q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
-    if (q.first >= q.len) return;
-    const int kbase = q.other_base, klen = q.other_len;
-    const int kvh = hx / A.subs;
-    const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
-
-    LongRange r;
-    int n[2];  // key tiles of each row tile
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int first = q.first + (ALT ? 0 : t * per);
-        r.tok[t] = min(per, max(0, q.len - first));
-        const int last = first + r.tok[t] - 1;
-        r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
-        n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
-    }
-    r.j0 = 0;
-    r.end = max(n[0], n[1]);
-    if (SPLIT) {
-        const int each = (r.end + (int)gridDim.z - 1) / (int)gridDim.z;
-        r.j0 = min(r.end, each * (int)blockIdx.z);
-        r.end = min(r.end, r.j0 + each);
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-        r.cnt[t] = ALT ? (r.end - r.j0 + 1 - t) / 2 : max(0, min(n[t], r.end) - r.j0);
-
-    if (warp == 8) {
+    auto start = [&] {
+        if (warp != 8) return;
         if ((threadIdx.x & 31) == 0) {
             for (int t = 0; t < 2; ++t) {
                 mbar_init(&sh.q_full[t], 1);
@@ -673,7 +795,62 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
         }
         __syncwarp();
         tmem_alloc(&sh.tmem, S::kTmem);
+    };
+    int slot, hx;
+    Slot q;
+    Share share{0, 0, 0, 1};
+    if constexpr (SPLIT) {
+        __shared__ SharedOut so;
+        launch_dependents();
+        start();
+        tc_fence_before();
+        count_tiles(A, so, slots);
+        tc_fence_after();
+        share = find_share(A, so, slots, share_size(A, so, slots, S::kLeast, gridDim.x), blockIdx.x);
+        if (share.slot < 0) {
+            if (warp == 8) tmem_dealloc(sh.tmem, S::kTmem);
+            return;
+        }
+        slot = share.slot;
+        hx = share.head;
+        q = shared_slot(A, so, slot);
+    } else {
+        const int s = quotient(blockIdx.x, A.heads);
+        hx = blockIdx.x - s * A.heads.d;
+        // Later slots first: under a causal mask they see more keys.
+        slot = slots - 1 - s;
+        q = find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
     }
+    if (!SPLIT && q.first >= q.len) return;
+    const int kbase = q.other_base, klen = q.other_len;
+    const int kvh = hx / A.subs;
+    const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+
+    LongRange r;
+    int n[2];  // key tiles of each row tile
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = q.first + (ALT ? 0 : t * per);
+        r.tok[t] = min(per, max(0, q.len - first));
+        const int last = first + r.tok[t] - 1;
+        r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
+        n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
+    }
+    r.j0 = 0;
+    r.end = max(n[0], n[1]);
+    if (SPLIT) {
+        const int each = (r.end + share.parts - 1) / share.parts;
+        r.j0 = min(r.end, each * share.which);
+        r.end = min(r.end, r.j0 + each);
+        if (threadIdx.x == 0) {
+            sh.part_row = share.parts > 1 ? (long long)blockIdx.x * f.part_rows : -1;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        r.cnt[t] = ALT ? (r.end - r.j0 + 1 - t) / 2 : max(0, min(n[t], r.end) - r.j0);
+
+    if (!SPLIT) start();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -685,7 +862,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     if (warp >= 8) {
         regs_less<S::Regs::kLess>();
         if (warp == 8) {
-            if (r.end > r.j0) long_mma_loop<DP, ALT>(sh, smem_q, smem_kv, r, tmem);
+            if (r.end > r.j0) long_mma_loop<DP, ALT>(sh, smem_q, smem_kv, r, tmem, A.D);
         } else if (warp == 9) {
             issued = long_load<DP, ALT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
                                    klen);
@@ -744,9 +921,54 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             }
             if (ok && n > 0) ok = wait_warp(&sh.o_done[t], (n - 1) & 1, abort);
             tc_fence_after();
-            const size_t which = ALT ? 2 * blockIdx.z + t : blockIdx.z;  // of the parts
-            if (ok)
-                write_row<DP, SPLIT>(A, f, which, rs, to, n > 0, live, (size_t)q.base + tok, qhead + row_head(A, row));
+            const size_t token = (size_t)q.base + tok;
+            const int head = qhead + row_head(A, row);
+            const long long part_row = SPLIT && sh.part_row >= 0 ? sh.part_row + row : -1;
+            if (!ALT) {
+                if (ok) write_row<DP, false>(A, f, -1, rs, to, n > 0, live, token, head);
+            } else {
+                // Each half gives the other its sums of half of the channels, through the room of K and V once
+                // both are through with it.
+                constexpr int kSide = DP / 2 + 4;  // four more: its maximum and sum, and other banks for each row
+                float *side = reinterpret_cast<float *>(dyn + (smem_kv - smem_u32(dyn))) + row * kSide;
+                float *give = side + (1 - t) * 128 * kSide, *take = side + t * 128 * kSide;
+                half_barrier();
+                if (ok && warp_live) {
+                    if (live) *reinterpret_cast<float2 *>(give + DP / 2) = make_float2(rs.m, rs.sum);
+#pragma unroll 1
+                    for (int c = 0; c < DP / 2; c += 16) {
+                        float o[16];
+                        if (n > 0) {
+                            tmem_ld16(to + (1 - t) * (DP / 2) + c, o);
+                            tmem_wait_ld();
+                            pin<16>(o);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+                        }
+                        if (!live) continue;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<float4 *>(give + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+                half_barrier();
+                if (__all_sync(0xffffffffu, ok && !*abort) && warp_live) {
+                    float a = 0.0f, b = 0.0f;
+                    if (live) {
+                        const float2 y = *reinterpret_cast<const float2 *>(take + DP / 2);
+                        const float m = fmaxf(rs.m, y.x);
+                        a = rs.m == -INFINITY ? 0.0f : exp2f((rs.m - m) * A.scale_log2);
+                        b = y.x == -INFINITY ? 0.0f : exp2f((y.x - m) * A.scale_log2);
+                        // In the same order in both, for the same bits.
+                        const float s0 = t == 0 ? rs.sum * a : y.y * b, s1 = t == 0 ? y.y * b : rs.sum * a;
+                        rs.m = m;
+                        rs.sum = s0 + s1;
+                    }
+                    write_row<DP, true>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
+                                               (t + 1) * (DP / 2), a, take, b);
+                }
+            }
         }
     }
     __syncwarp();
@@ -824,7 +1046,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     using S = ShortShape<DP>;
     using TL = Tile<DP>;
     constexpr int KEYS = S::kKeys;
-    constexpr uint32_t kIdO = mma_idesc(128, DP, true);
+    const uint32_t id_o = mma_idesc(128, (A.D + 15) & ~15, true);
     constexpr uint32_t kSbo = 8 * TL::kRowBytes, kQPanel = 128 * TL::kRowBytes, kPanel = KEYS * TL::kRowBytes;
     extern __shared__ unsigned char dyn[];
     __shared__ ShortShared sh;
@@ -889,7 +1111,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         if (!wait_warp(&sh.k_full[g & 1], (g >> 1) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t id = mma_idesc(128, tile_cols(sees, j * KEYS, KEYS), false);
-        mma_channels<DP, kQPanel, kPanel>(tmem, q_desc, k_desc + (g & 1) * (S::kTileBytes / 16), id);
+        mma_channels<DP, kQPanel, kPanel>(tmem, q_desc, k_desc + (g & 1) * (S::kTileBytes / 16), id, A.D);
         tc_commit_one(&sh.s_full);
         return true;
     };
@@ -955,11 +1177,11 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
                     const uint64_t b = v_desc + (t & 1) * (S::kTileBytes / 16);
                     static_assert(KEYS == 64, "four steps");
                     if (steps == 4) {
-                        mma_ts_one<4, TL::kRowBytes>(tmem + KEYS, tmem, b, kIdO, i > 0);
+                        mma_ts_one<4, TL::kRowBytes>(tmem + KEYS, tmem, b, id_o, i > 0);
                     } else {
 #pragma unroll 1
                         for (int k = 0; k < steps; ++k)
-                            mma_ts_one<1, 0>(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, kIdO, i > 0 || k > 0);
+                            mma_ts_one<1, 0>(tmem + KEYS, tmem + k * 8, b + k * TL::kRowBytes, id_o, i > 0 || k > 0);
                     }
                     if (i + 1 < it.n) ok = scores(it.sees, t + 1, i + 1);
                     else tc_commit_one(&sh.o_done);
@@ -977,7 +1199,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         tc_fence_after();
         // (O is written over only after the next row tile's first barrier.)
         if (ok && it.any)
-            write_row<DP, false>(A, f, 0, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
+            write_row<DP, false>(A, f, -1, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
                                  it.qhead + row_head(A, row));
         tc_fence_before();
         g += it.n;
@@ -1002,38 +1224,75 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
     }
 }
 
-// o = sum_s w_s part_s with w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s).  Eight channels
-// per thread.  A part that saw no keys has lse -inf, weight 0 and wrote zeros.
+// o = sum_s w_s part_s with w_s = exp(lse_s - lse), lse = log sum_s exp(lse_s), for a slot and head (x) whose keys
+// were shared out; eight channels per thread.  A part that saw no keys has lse -inf, weight 0 and wrote zeros.
+// Blocks look up their parts while the last of them are still in work, and read four parts at a time (weights
+// relative to the largest lse so far).
 __global__ void __launch_bounds__(128)
-attn_join_kernel(const FwdOut f, int splits, long long rows, int Hq, int Tq, int D) {
-    const int per = D / 8;
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= rows * per) return;
-    const long long row = i / per;  // token * Hq + head
-    const int c = (int)(i % per) * 8;
-    const long long token = row / Hq;
-    const int head = (int)(row % Hq);
-    const float *pl = f.part_lse + (size_t)head * Tq + token;
-    const float *px = f.part + row * D + c;
-    float top = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, __ldg(pl + (size_t)s * rows));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float w = expf(__ldg(pl + (size_t)s * rows) - ref);
-        total += w;
-        float x[8];
-        load_vec<float, 8, true>(px + (size_t)s * rows * D, x);
+attn_join_kernel(const AttnArgs A, const FwdOut f, int slots, int least, int blocks) {
+    __shared__ SharedOut so;
+    count_tiles(A, so, slots);
+    const unsigned size = share_size(A, so, slots, least, blocks);
+    const int slot = quotient(blockIdx.x, A.heads), hx = blockIdx.x - slot * A.heads.d;
+    const int parts = (so.tiles[slot] + size - 1) / size;
+    int before = 0;
+#pragma unroll 1
+    for (int x = threadIdx.x & 31; x < slot; x += 32) before += (so.tiles[x] + size - 1) / size;
+    before = __reduce_add_sync(0xffffffffu, before);
+    // (One block at least waits, so that this launch does not end before the one whose parts it joins.)
+    if (parts <= 1 && (blockIdx.x | blockIdx.y) > 0) return;
+    wait_for_primary();
+    if (parts <= 1) return;
+    const Slot q = shared_slot(A, so, slot);
+    const int per = 128 / A.pack, qhead = hx / A.subs * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+    const int chunks = A.D / 8;
+    const int rows = min(q.len - q.first, per) * A.pack;
+    const size_t step = (size_t)A.heads.d * f.part_rows;
+    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < rows * chunks; i += gridDim.y * blockDim.x) {
+        const int row = i / chunks, c = (i - row * chunks) * 8;
+        const size_t first = ((size_t)before * A.heads.d + hx) * f.part_rows + row;
+        const float *pl = f.part_lse + first, *px = f.part + first * A.D + c;
+        float top = -INFINITY, total = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+        for (int s = 0; s < parts; s += 4) {
+            float l[4];
+            float4 x[4][2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(w, x[e], o[e]);
+            for (int e = 0; e < 4; ++e) {
+                const bool have = s + e < parts;
+                const size_t at = (size_t)(s + e) * step;
+                l[e] = have ? __ldcg(pl + at) : -INFINITY;
+                x[e][0] = have ? __ldcg(reinterpret_cast<const float4 *>(px + at * A.D)) : make_float4(0, 0, 0, 0);
+                x[e][1] = have ? __ldcg(reinterpret_cast<const float4 *>(px + at * A.D) + 1) : make_float4(0, 0, 0, 0);
+            }
+            const float was = top;
+            top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), was);
+            const float ref = top == -INFINITY ? 0.0f : top, keep = expf(was - ref);
+            total *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] *= keep;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = expf(l[e] - ref);
+                total += w;
+                o[0] = fmaf(w, x[e][0].x, o[0]);
+                o[1] = fmaf(w, x[e][0].y, o[1]);
+                o[2] = fmaf(w, x[e][0].z, o[2]);
+                o[3] = fmaf(w, x[e][0].w, o[3]);
+                o[4] = fmaf(w, x[e][1].x, o[4]);
+                o[5] = fmaf(w, x[e][1].y, o[5]);
+                o[6] = fmaf(w, x[e][1].z, o[6]);
+                o[7] = fmaf(w, x[e][1].w, o[7]);
+            }
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] *= inv;
+        const size_t token = (size_t)q.base + q.first + row_token(A, row);
+        const int head = qhead + row_head(A, row);
+        store_result(f, (token * A.Hq + head) * A.D + c, o);
+        if (f.lse && c == 0) f.lse[(size_t)head * A.Tq + token] = total == 0.0f ? -INFINITY : top + logf(total);
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= inv;
-    store_result(f, row * D + c, o);
-    if (f.lse && c == 0) f.lse[(size_t)head * Tq + token] = total == 0.0f ? -INFINITY : top + logf(total);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1184,10 +1443,11 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
 
 // Whole warp.
 template <int DP, bool DKV>
-__device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, int steps, uint32_t tmem) {
+__device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, int steps, uint32_t tmem, int dim) {
     using S = BwdShape<DP>;
     using TL = Tile<DP>;
-    constexpr uint32_t kIdS = mma_idesc(128, kWalk, false), kIdAcc = mma_idesc(128, DP, true);
+    constexpr uint32_t kIdS = mma_idesc(128, kWalk, false);
+    const uint32_t id_acc = mma_idesc(128, (dim + 15) & ~15, true);
     constexpr uint32_t kSbo = 8 * TL::kRowBytes;
     constexpr uint32_t kXPanel = 128 * TL::kRowBytes, kYPanel = kWalk * TL::kRowBytes;
     volatile int *abort = &sh.abort;
@@ -1202,7 +1462,8 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
 #pragma unroll
         for (int which = 0; which < 2; ++which)
             mma_channels<DP, kXPanel, kYPanel>(tmem + (i % S::kPairs) * 2 * kWalk + which * kWalk,
-                                               x_desc + which * (S::kXBytes / 16), y + which * (S::kYBytes / 16), kIdS);
+                                               x_desc + which * (S::kXBytes / 16), y + which * (S::kYBytes / 16), kIdS,
+                                               dim);
         tc_commit_one(&sh.s_full[i % S::kPairs]);
         return true;
     };
@@ -1221,9 +1482,9 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         for (int h = 0; h < 2; ++h) {
             const uint64_t yh = y + h * 2 * TL::kRowBytes;
             if (DKV)
-                mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc + DP, p + h * 32, yh + S::kYBytes / 16, kIdAcc,
+                mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc + DP, p + h * 32, yh + S::kYBytes / 16, id_acc,
                                              i > 0 || h > 0);
-            mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc, p + kWalk + h * 32, yh, kIdAcc, i > 0 || h > 0);
+            mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc, p + kWalk + h * 32, yh, id_acc, i > 0 || h > 0);
         }
         tc_commit_one(&sh.y_empty[st]);
         if (i + S::kPairs < steps && !scores(i + S::kPairs)) return false;
@@ -1507,7 +1768,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
                               : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
     if (warp >= S::kCompute) {
         regs_less<S::Regs::kLess>();
-        if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem);
+        if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem, A.D);
         if (warp == S::kCompute + 1)
             issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
     } else {
@@ -1634,53 +1895,69 @@ int check_tensor(const Strided &t, int64_t T, int64_t H) {
     return RFDETR_OK;
 }
 
-// Which forward kernel, and over how many blocks each row tile's keys are split.
+// Which forward kernel, and whether the row tiles' keys are shared out over blocks.
 struct ForwardPlan {
     bool is_short;
-    int splits;     // blocks to a row tile's keys
-    bool alternate; // the two halves of such a block take key tiles in turn
-    int parts() const { return alternate ? 2 * splits : splits; }
+    bool alternate;  // one row tile a block, its key tiles taken by the block's halves in turn
+    int blocks;      // that the keys are shared out over (alternate only); 0: one block to a slot and head
+    int slot_rows;
+    long long slots;
 };
 
 ForwardPlan plan_forward(const AttnArgs &A) {
-    ForwardPlan p{false, 1, false};
-    const int per = 128 / A.pack;
+    const int per = 128 / A.pack, sms = num_sms();
     const long long heads = (long long)A.Hkv * A.subs;
     const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
-    const long long rows = A.Tq / n_seq, keys = A.Tk / n_seq;  // of the mean sequence
-    // One row tile to a sequence, its keys taken by halves; or blocks of two row tiles, if every sequence were
-    // the mean one.
+    const long long rows = A.Tq / n_seq, keys = A.Tk / n_seq, tiles = (keys + 127) / 128;  // of the mean sequence
+    // Row tiles, and pairs of them, if every sequence were the mean one.
+    const long long row_tiles = heads * n_seq * ((rows + per - 1) / per);
+    const long long pairs = heads * n_seq * ((rows + 2 * per - 1) / (2 * per));
     const bool single = rows <= per;
-    const long long blocks = heads * n_seq * (single ? 1 : (rows + 2 * per - 1) / (2 * per));
-    const long long tiles = (keys + 127) / 128;
+    ForwardPlan p{};
+    // (us, the alternating halves against pairs of row tiles; tokens x heads of channels.)  One to an SM at most:
+    // 300 tokens, 8 of 32: 9.3, 11.0; 4 x 577, 6 of 64: 12.5, 16.6; 1024 causal, 16 / 4 of 128: 16.6, 22.7; 4 x
+    // 300 over 2000 keys, 8 of 64: 20.7, 32.9; but 8 x 577, 6 of 64, 240 row tiles: 22.7, 18.6.  Up to two with a
+    // causal mask, if long (the longest begin first): 2048, 16 / 4 of 128: 28.8, 35.0; 4 x 1000, 8 of 64: 22.7,
+    // 22.2; 8 x 577: 20.7, 15.9; 3000, 16 / 4, 376 of them: 52.1, 49.1.  Up to one and a half where the keys
+    // are other tokens, which is how sequences of very different lengths come: 8 x 300 over 0 to 4000, 8 of 80:
+    // 37.1, 44.8; over 600 to 2400: 37.7, 41.2; but over 2000 each: 43.8, 36.5.  And where a pair's second
+    // would be empty: 128 x 1 over 2000, 16 / 4 of 128: 108.7, 117.6; 32 x 1 over 700, 8 of 64: 25.0, 28.2.
+    p.alternate = tiles >= 2 && (row_tiles <= sms ||
+                                 (tiles >= 8 && (single || (A.causal && row_tiles <= 2 * sms) ||
+                                                 (A.Tq != A.Tk && 2 * row_tiles <= 3 * sms))));
+    // Shared out over the SMs, a block to each: one token over 30,000 keys, 32 / 8 of 128: 38.4, whole 220; 4 x 64
+    // over 8000, 16 / 4: 39.3, 68.1; 4 x 1 over 2500, 8 of 64: 18.6, 22.7; but 16 x 1 over 4000, 16 / 4: 36.7,
+    // 41.7; 1601, 6 of 64, 13 key tiles: 29.3, 18.6.
+    bool share = p.alternate && tiles >= 16 && 2 * row_tiles <= sms;
+    long long times = 0;
+    // The short kernel against pairs of row tiles: 104 x 300, 8 of 32: 57, 103; 32 x 145, 6 of 64: 12.0, 16.2; 16
+    // x 64, 4 of 64: 6.3, 8.4; 16 x 300 over 1000, 8 of 32: 35.0, 39.6; but 8 x 300, 8 of 32, 128 pairs: 14.5,
+    // 12.5; 16 of 1 to 1601, 6 of 64: 54.7, 53.2.  (Single tokens, against halves: 32 x 1 over 700, 8 of 64: 22.7,
+    // 25.0; over 1500: 41.2, 37.1.)
+    p.is_short = !p.alternate && rows <= 4 * per &&
+                 (keys <= 128 || (pairs > sms && keys <= 512) || (single && tiles < 8));
     const KnobValue forced = knob(kKnobAttnFwd);
     if (forced.count > 0 && forced.v[0] > 0) {
         p.is_short = forced.v[0] == 2;
-        p.splits = p.is_short || forced.v[1] < 1 ? 1 : forced.v[1] > 64 ? 64 : forced.v[1];
         p.alternate = forced.v[0] == 3;
-        return p;
+        times = !p.alternate || forced.v[1] < 2 ? 0 : forced.v[1] > 64 ? 64 : forced.v[1];
+        share = times > 0;
     }
-    // Few blocks with many keys: split into one block to an SM, or, where the keys are other tokens and their
-    // lengths may differ from block to block, in two even if that leaves some SMs with two; four key tiles at
-    // least to a block (eight in turn).  One token over 30,000 keys, 32 / 8
-    // heads of 128: 334 us whole, 42.3 in 16, 58.3 in 37; 4 x 64 tokens over 8000 keys, 16 / 4: 107.7 whole, 34.8 in 9,
-    // 47.5 in 18; 8 x 300 over 0 to 4000 keys, 8 of 80: 58 whole, 42 in two, but 2048 causal
-    // tokens, 16 / 4 of 128: 35.0 whole, 42.9 in two.  Halves in turn: one token each over
-    // 1 to 16384 keys, 16 / 4 heads of 128: 47.1 us in 4, 54.2 without in 9.
-    long long s = num_sms() / (blocks > 0 ? blocks : 1);
-    if (s < 2 && A.Tq != A.Tk) s = (3ll * num_sms() / 2 + blocks / 2) / (blocks > 0 ? blocks : 1);
-    if (s > tiles / (single ? 8 : 4)) s = tiles / (single ? 8 : 4);
-    p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-    p.alternate = single && tiles >= 4;
-    if (p.parts() > 1) return p;
-    // 104 x 300 tokens, 8 heads of 32: 62 us in the short kernel, 103 in the long one; 32 x 145, 6 of 64: 12.7
-    // and 16.2; 16 of 1 to 1601, 6 of 64: 52.6 and 52.8; 8 x 300 over 0 to 4000 keys, 8 of 80: 100 and 58.
-    p.is_short = rows <= 4 * per && keys <= 512;
+    p.slot_rows = p.is_short || p.alternate ? per : per * 2;
+    p.slots = slots_for(A.Tq, p.slot_rows, A.n_seq);
+    if (share && p.slots <= kSharedSlots) {
+        const long long most = p.slots * heads;
+        p.blocks = (int)(times > 0 ? most * times : most > sms ? most : sms);
+    }
     return p;
 }
 
-size_t split_bytes(const AttnArgs &A, int parts) {
-    return parts <= 1 ? 0 : (size_t)parts * A.Tq * A.Hq * (A.D + 1) * sizeof(float);
+int part_rows(const AttnArgs &A) {
+    const int per = 128 / A.pack;
+    return (A.Tq < per ? A.Tq : per) * A.pack;
+}
+size_t split_bytes(const AttnArgs &A, const ForwardPlan &p) {
+    return (size_t)p.blocks * part_rows(A) * (A.D + 1) * sizeof(float);
 }
 
 template <int DP>
@@ -1691,35 +1968,46 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
     if (!make_map(&mq, q, A.Tq, A.Hq, A.D, A.pack, per, q.p) || !make_map(&mk, k, A.Tk, A.Hkv, A.D, 1, keys, q.p) ||
         !make_map(&mv, v, A.Tk, A.Hkv, A.D, 1, keys, q.p))
         return RFDETR_ERR_CUDA;
-    const int slot_rows = plan.is_short || plan.alternate ? per : per * 2;
-    const long long slots = slots_for(A.Tq, slot_rows, A.n_seq);
-    const long long blocks = slots * A.Hkv * A.subs;
+    const long long blocks = plan.slots * A.Hkv * A.subs;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    A.slot_rows = divisor(slot_rows);
+    const int slots = (int)plan.slots;
+    A.slot_rows = divisor(plan.slot_rows);
     A.heads = divisor(A.Hkv * A.subs);
-    const dim3 grid((unsigned)blocks, 1, (unsigned)plan.splits);
     if (plan.is_short) {
         using S = ShortShape<DP>;
         const long long stay = (long long)S::kBlocks * num_sms();
         if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
         attn_forward_short_kernel<DP>
-            <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, f, (int)slots);
+            <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, f, slots);
         return launch_status();
     }
     using S = LongShape<DP, false>;  // (its block and shared memory are those of the alternating kernel too)
     auto launch = [&](auto kernel) {
         if (int st = allow_smem(kernel, S::kSmem)) return st;
-        kernel<<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, f, (int)slots);
+        kernel<<<(unsigned)(plan.blocks ? plan.blocks : blocks), S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, f, slots);
         return launch_status();
     };
-    if (plan.parts() == 1) return launch(attn_forward_long_kernel<DP, false, false>);
-    if (int st = plan.alternate ? launch(attn_forward_long_kernel<DP, true, true>)
-                                : launch(attn_forward_long_kernel<DP, true, false>))
-        return st;
-    const long long rows = (long long)A.Tq * A.Hq, n = rows * (A.D / 8);
-    if ((n + 127) / 128 > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    attn_join_kernel<<<(unsigned)((n + 127) / 128), 128, 0, stream>>>(f, plan.parts(), rows, A.Hq, A.Tq, A.D);
-    return launch_status();
+    if (plan.blocks == 0)
+        return plan.alternate ? launch(attn_forward_long_kernel<DP, true, false>)
+                              : launch(attn_forward_long_kernel<DP, false, false>);
+    if (int st = launch(attn_forward_long_kernel<DP, true, true>)) return st;
+    const int most = A.Tq < plan.slot_rows ? A.Tq : plan.slot_rows;  // tokens of a slot
+    cudaLaunchConfig_t config{};
+    const int items = most * A.pack * (A.D / 8), threads = items <= 512 ? 32 : 128;
+    const int chunks = (items + threads - 1) / threads;
+    config.gridDim = dim3((unsigned)blocks, (unsigned)(chunks < 16 ? chunks : 16));
+    config.blockDim = dim3((unsigned)threads);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    if (cudaLaunchKernelEx(&config, attn_join_kernel, A, f, slots, S::kLeast, plan.blocks) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return RFDETR_ERR_CUDA;
+    }
+    return RFDETR_OK;
 }
 
 // Blocks that share a held tile's steps, in the kernel that holds keys and in the one that holds
@@ -1840,7 +2128,7 @@ extern "C" size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, i
     if (check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim) != RFDETR_OK) return 0;
     const AttnArgs A = make_args(nullptr, nullptr, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, 0,
                                  1.0f, 128);
-    return split_bytes(A, plan_forward(A).parts());
+    return split_bytes(A, plan_forward(A));
 }
 
 extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride,
@@ -1866,12 +2154,13 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
                                  causal, scale, 128);
     const ForwardPlan p = plan_forward(A);
-    const size_t need = split_bytes(A, p.parts());
+    const size_t need = split_bytes(A, p);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return RFDETR_ERR_WORKSPACE;
-    FwdOut f{static_cast<bf16 *>(output), static_cast<bf16 *>(output_low), lse, nullptr, nullptr};
+    FwdOut f{static_cast<bf16 *>(output), static_cast<bf16 *>(output_low), lse};
     if (need) {
         f.part = static_cast<float *>(workspace);
-        f.part_lse = f.part + (size_t)p.parts() * A.Tq * A.Hq * A.D;
+        f.part_rows = part_rows(A);
+        f.part_lse = f.part + (size_t)p.blocks * f.part_rows * A.D;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (padded_dim(head_dim)) {

@@ -115,7 +115,7 @@ enum Knob {
     kKnobLsapStepCap,   // "RFDETR_LSAP_STEP_CAP": scan steps an augmenting path may take (default: the column count)
     kKnobTopkSort,      // "RFDETR_TOPK_SORT": any value selects the one-CTA sort kernels
     kKnobTopkUnstaged,  // "RFDETR_TOPK_UNSTAGED": any value keeps the radix select's keys out of shared memory
-    kKnobAttnFwd,       // "RFDETR_ATTN_FWD": packed attention forward (1 long, 2 short, 3 alternating kernel; key splits of 1 and 3)
+    kKnobAttnFwd,       // "RFDETR_ATTN_FWD": packed attention forward (1 long, 2 short, 3 alternating kernel; blocks that 3 shares keys over)
     kKnobAttnBwd,       // "RFDETR_ATTN_BWD": packed attention backward (blocks sharing a tile of keys, of queries: 1, 2, 4)
     kKnobCount
 };

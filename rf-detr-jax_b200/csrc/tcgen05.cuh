@@ -52,6 +52,11 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // Makes this thread's shared-memory writes visible to the tensor core and TMA (async proxy).
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Lets the stream's next kernel, launched to overlap this one, have the SMs that it leaves; that kernel waits
+// for all of this one's results before it reads them.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void mbar_arrive_one(uint64_t *bar) {
     asm volatile(
         "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"

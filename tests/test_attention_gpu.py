@@ -354,6 +354,66 @@ def test_one_token_over_long_keys(pkg):
     _check(pkg, (2, 0, 1), (3000, 3000, 3000), heads=7, kv=1, dim=80, causal=True)
 
 
+@pytest.mark.parametrize("dim", [32, 64, 80, 128])
+@pytest.mark.parametrize("heads,kv", [(16, 4), (6, 6), (12, 1)])
+def test_keys_shared_out(pkg, heads, kv, dim):
+    """Few rows over keys of very different lengths, none and one among them: how many blocks a slot gets
+    depends on all of them."""
+    keys = (5000, 0, 129, 3001, 1, 9000, 128, 40)
+    size = pkg._native.lib().rfdetr_packed_attention_workspace_bytes
+    assert size(8, 8, sum(keys), heads, kv, dim) > 0
+    _check(pkg, (1,) * 8, keys, heads, kv, dim, causal=True, grad=False)
+    _check(pkg, (3, 2, 0, 1, 5, 7, 1, 2), keys, heads, kv, dim, causal=True)
+    _check(pkg, (1, 5, 0), (20000, 7, 300), heads, kv, dim)
+
+
+def test_keys_shared_out_over_many_slots(pkg, tuning):
+    """More slots than a warp has lanes, and more than the blocks look through (then none are shared out)."""
+    rng = np.random.default_rng(3)
+    for n, knob in ((40, "3,2"), (150, "3,3"), (400, "3,3")):
+        tuning("RFDETR_ATTN_FWD", knob)
+        lengths = [int(x) for x in rng.integers(0, 3, n)]
+        keys = [int(x) if rng.random() > 0.3 else 0 for x in rng.integers(0, 2500 if n < 100 else 600, n)]
+        _check(pkg, lengths, keys, heads=4, kv=2, dim=64, causal=True)
+
+
+def test_offsets_that_do_not_ascend(pkg, tuning):
+    """Unchecked: the results are then of no use, but every kernel stays within the tensors."""
+    rng = np.random.default_rng(4)
+    q, k, v = _bf16(rng, 300, 4, 64), _bf16(rng, 2000, 2, 64), _bf16(rng, 2000, 2, 64)
+    off = torch.tensor([-5, 200, 100, 250, 7000, 20, 300], dtype=torch.int32, device=DEV)
+    koff = torch.tensor([1500, 300, 2500, -1, 900, 100, 2000], dtype=torch.int32, device=DEV)
+    for knob in ("1", "2", "3", "3,4"):
+        tuning("RFDETR_ATTN_FWD", knob)
+        pkg.packed_attention(q, k, v, off, koff, causal=True, return_lse=True)
+        _fault_free(pkg)
+
+
+def test_captured_in_a_graph(pkg):
+    """Forward alone, with keys shared out and joined, replayed on other inputs and other lengths."""
+    rng = np.random.default_rng(5)
+    q, k, v = _bf16(rng, 8, 16, 128), _bf16(rng, 20000, 4, 128), _bf16(rng, 20000, 4, 128)
+    off, koff = _offsets((1,) * 8), _offsets((9000, 1, 3000, 0, 500, 64, 7000, 435))
+    call = lambda: pkg.packed_attention(q, k, v, off, koff, causal=True, return_lse=True)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for seed in (6, 7):
+        rng = np.random.default_rng(seed)
+        for x in (q, k, v):
+            x.copy_(_bf16(rng, *x.shape))
+        cuts = np.sort(rng.integers(0, 20001, 7))
+        koff.copy_(torch.tensor([0, *cuts.tolist(), 20000], dtype=torch.int32))
+        graph.replay()
+        for a, b in zip(got, call()):
+            assert torch.equal(a, b)
+
+
 def test_rows_beyond_32_bit_offsets(pkg):
     """Keys, values and cotangents whose rows lie further apart than 2^31 elements (a wide cache)."""
     rng = np.random.default_rng(31)
