@@ -18,20 +18,22 @@ from . import _native as N
 def _packed(name: str, t: torch.Tensor) -> torch.Tensor:
     """Checks ``[tokens, heads, dim]`` bf16 and returns it with strides the kernels take (a view of
     a fused projection passes as it is; anything else is made contiguous)."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
     if t.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
-    token, head, channel = t.stride()
+    strides = t.stride()
+    if len(strides) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
+    token, head, channel = strides
     if channel != 1 or token <= 0 or head <= 0 or (token | head) & 7 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _offsets(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] < 1 or t.dtype not in (torch.int32, torch.int64):
+    dtype = t.dtype
+    if t.dim() != 1 or t.numel() < 1 or (dtype != torch.int32 and dtype != torch.int64):
         raise ValueError(f"{name} must be int32 [sequences + 1]")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
@@ -47,18 +49,19 @@ def attention_forward(query, key, value, offsets, key_offsets, causal, scale, wa
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
     sequences = offsets.numel() - 1
-    out = query.new_empty((tokens, heads, dim))
-    lse = query.new_empty((heads, tokens), dtype=torch.float32) if want_lse else None
-    low = query.new_empty((tokens, heads, dim)) if want_low else None
+    out = query.new_empty(tokens, heads, dim)
+    lse = query.new_empty(heads, tokens, dtype=torch.float32) if want_lse else None
+    low = query.new_empty(tokens, heads, dim) if want_low else None
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
     workspace = query.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     status = lib.rfdetr_packed_attention(
         N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
-        out.data_ptr(), N.ptr(low), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads, kv_heads, dim,
-        int(causal), scale)
-    N.check(status, "rfdetr_packed_attention")
+        out.data_ptr(), N.ptr(low), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads,
+        kv_heads, dim, causal, scale)
+    if status:
+        N.check(status, "rfdetr_packed_attention")
     return out, lse, low
 
 
@@ -69,7 +72,7 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
     grad_output = _packed("grad_output", grad_output.to(query.dtype))
     if grad_lse is not None:
         grad_lse = grad_lse.to(torch.float32).contiguous()
-    grads = tuple(t.new_empty(t.shape) for t in (query, key, value))
+    grads = query.new_empty(tokens, heads, dim), key.new_empty(key.shape), value.new_empty(key.shape)
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_backward_workspace_bytes(tokens, heads)
     workspace = query.new_empty(max(1, ws_bytes), dtype=torch.uint8)
@@ -79,7 +82,8 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
         out.data_ptr(), N.ptr(low), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
         N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
         offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale)
-    N.check(status, "rfdetr_packed_attention_backward")
+    if status:
+        N.check(status, "rfdetr_packed_attention_backward")
     return grads
 
 
@@ -132,7 +136,7 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         (and through the log-sum-exp).  A query without any key, and rows outside all sequences,
         give 0 (log-sum-exp ``-inf``) and gradient 0.
     """
-    N.require_cuda(query, key, value, offsets, key_offsets)
+    N.same_device(query, key, value, offsets, key_offsets)
     query, key, value = _packed("query", query), _packed("key", key), _packed("value", value)
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, key_dim = key.shape

@@ -1302,38 +1302,40 @@ attn_join_kernel(const AttnArgs A, const FwdOut f, int slots, int least, int blo
 // blocks: one holds a tile of 128 keys (K, V) and walks the queries, accumulating dK and dV in
 // TMEM; the other holds 128 query rows (Q, g) and walks the keys, accumulating dQ.  Both form S and
 // dP again (three products where one kernel with atomics would share two of them).
-//   X0, X1: the held tiles (K, V or Q, g); Y0, Y1: the walked ones, 64 rows a step (Q, g or K, V)
-//   A = X0 Y0^T, B = X1 Y1^T  (128 x 64 each, TMEM)  ->  P = exp2(scale log2(e) A - log2(e) lse),
+//   X0, X1: the held tiles (K, V or Q, g); Y0, Y1: the walked ones, 64 or 32 rows a step (Q, g or K, V)
+//   A = X0 Y0^T, B = X1 Y1^T  (128 x 64 or 32 each, TMEM)  ->  P = exp2(scale log2(e) A - log2(e) lse),
 //   dS = P (B - delta)        (bf16, written over A and B)
 //   acc0 += dS Y0             (dK or dQ, times scale at the end), acc1 += P Y1 (dV)
 // With few held tiles (or, under a causal mask, one that walks far longer than the mean) a cluster of
 // blocks shares a tile's steps; their accumulators are added through distributed shared memory, in
 // rank order, each block writing its share of the columns.
-// Two warpgroups turn a pair (A, B) into P and dS, each 32 of its 64 columns.  64 rows a step is what TMEM
-// leaves.  Up to 64 channels, one pair and two accumulators take half of it, and two blocks of an SM cover each
-// other, their starts and ends too; with 128, two pairs alternate in one block: while one is in work, the
-// tensor core forms the other and adds the one before.  (Two pairs in one block with 64 channels: 440 against
-// 403 us for 4 x 2048 tokens of 12 heads, 392 against 277 for 104 x 300 of 8 heads of 32, forward included.)
+// A warpgroup turns 32 columns of a pair (A, B) into P and dS.  64 rows a step, two warpgroups to a pair, is what
+// TMEM leaves.  Up to 64 channels, one pair and two accumulators take half of it, and two blocks of an SM cover
+// each other, their starts and ends too; up to 32, with 32 rows a step, a quarter, and four blocks do (104 x 300
+// tokens of 8 heads of 32: 94 us for dK and dV, 62 for dQ, with 64 rows and two blocks 107 and 79).  With 128, two
+// pairs alternate in one block: while one is in work, the tensor core forms the other and adds the one
+// before.  (Two pairs in one block with 64 channels: 440 against 403 us for 4 x 2048 tokens of 12 heads, 392
+// against 277 for 104 x 300 of 8 heads of 32, forward included.)
 // What bounds it is the chain of a step, as forward: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, take
-// 310 us for dK and dV (two blocks to a tile; four products a step) and 195 us for dQ (three), 1.0 and 1.2
-// PFLOP/s of what they compute; 104 x 300 tokens, 8 heads of 32, 106 and 79 us.
+// 311 us for dK and dV (two blocks to a tile; four products a step) and 197 us for dQ (three), 1.0 and 1.2
+// PFLOP/s of what they compute.
 // P and dS are rounded to bf16 for the tensor core; every sum is float32.
 // A row that sees exactly one key has P = 1 whatever its score, so its dS is set to what is left of
 // it, the cotangent of its lse, rather than to the difference of two roundings of the same number.
 // ---------------------------------------------------------------------------------------------
-constexpr int kWalk = 64;  // rows of Y a step
-
 template <int DP> struct BwdShape {
+    static constexpr int kWalk = DP == 32 ? 32 : 64;  // rows of Y a step
     static constexpr int kPairs = DP <= 64 ? 1 : 2;
     static constexpr int kXBytes = 128 * DP * 2;
     static constexpr int kYBytes = kWalk * DP * 2;
     static constexpr int kStages = 4;
-    static constexpr int kCompute = kPairs * 8;  // warps
-    static constexpr int kThreads = kPairs * 256 + 128;
-    static constexpr int kBlocks = kPairs == 2 ? 1 : 2;
-    // 65536 / 640 -> 96; 65536 / 768 -> 80.
+    static constexpr int kHalves = kWalk / 32;  // warpgroups to a pair
+    static constexpr int kCompute = kPairs * kHalves * 4;  // warps
+    static constexpr int kThreads = kCompute * 32 + (DP == 32 ? 64 : 128);
+    static constexpr int kBlocks = DP == 32 ? 4 : DP == 64 ? 2 : 1;
+    // 65536 / 640 -> 96; 65536 / 768 -> 80.  (With 32 channels, 65536 / (4 x 192) -> 80 for all.)
     using Regs = std::conditional_t<kPairs == 2, Registers<4, 96, 104, 64>, Registers<2, 80, 96, 48>>;
-    static constexpr int kTmem = kPairs == 2 ? 512 : 256;
+    static constexpr int kTmem = 512 / kBlocks;
     static constexpr int kAcc = kPairs * 2 * kWalk;  // first accumulator column
     static_assert(kAcc + 2 * DP <= kTmem, "TMEM");
     static constexpr size_t kSmem = 1024 + 2 * kXBytes + (size_t)kStages * 2 * kYBytes;
@@ -1344,9 +1346,9 @@ struct BwdShared {
     uint32_t tmem;
     int abort;
     // Per walked row, for the dK/dV kernel: -log2(e) lse, -delta and the lse's cotangent.
-    alignas(16) float neg_lse2[4][kWalk];
-    alignas(16) float neg_delta[4][kWalk];
-    alignas(16) float one_ds[4][kWalk];
+    alignas(16) float neg_lse2[4][64];
+    alignas(16) float neg_delta[4][64];
+    alignas(16) float one_ds[4][64];
 };
 
 // What a block walks.  DKV: `steps_per_sub` tiles of `tok` tokens from token `first` on, for each of
@@ -1368,6 +1370,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                         const CUtensorMap *my1, BwdShared &sh, uint32_t smem_x, uint32_t smem_y, const BwdRange &r,
                         const float *lse, const float *delta, const float *g_lse) {
     using S = BwdShape<DP>;
+    constexpr int kWalk = S::kWalk;
     using TL = Tile<DP>;
     const int lane = threadIdx.x & 31;
     volatile int *abort = &sh.abort;
@@ -1445,6 +1448,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
 template <int DP, bool DKV>
 __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, int steps, uint32_t tmem, int dim) {
     using S = BwdShape<DP>;
+    constexpr int kWalk = S::kWalk;
     using TL = Tile<DP>;
     constexpr uint32_t kIdS = mma_idesc(128, kWalk, false);
     const uint32_t id_acc = mma_idesc(128, (dim + 15) & ~15, true);
@@ -1476,10 +1480,9 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         const uint64_t y = yt_desc + st * (2 * S::kYBytes / 16);
         if (!wait_warp(&sh.ds_ready[i % S::kPairs], (i / S::kPairs) & 1, abort)) return false;
         tc_fence_after();
-        static_assert(kWalk == 64, "four steps");
         const uint32_t p = tmem + (i % S::kPairs) * 2 * kWalk;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < S::kHalves; ++h) {
             const uint64_t yh = y + h * 2 * TL::kRowBytes;
             if (DKV)
                 mma_ts_one<2, TL::kRowBytes>(tmem + S::kAcc + DP, p + h * 32, yh + S::kYBytes / 16, id_acc,
@@ -1493,13 +1496,14 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
     return true;
 }
 
-// Warpgroups 2 w and 2 w + 1: the steps i with i % kPairs == w, the first 32 columns and the others.
+// The kHalves warpgroups w: the steps i with i % kPairs == w, 32 columns each.
 template <int DP, bool DKV>
 __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const float *lse,
                           const float *delta, const float *g_lse) {
     using S = BwdShape<DP>;
+    constexpr int kWalk = S::kWalk;
     volatile int *abort = &sh.abort;
-    const int w = threadIdx.x >> 8, c0 = ((threadIdx.x >> 7) & 1) * 32, row = threadIdx.x & 127;
+    const int group = threadIdx.x >> 7, w = group / S::kHalves, c0 = group % S::kHalves * 32, row = threadIdx.x & 127;
     const uint32_t ts = tmem + ((uint32_t)((threadIdx.x >> 5) & 3) << 21) + w * 2 * kWalk + c0;
     const float2 sc2 = make_float2(A.scale_log2, A.scale_log2);
     const int shift = r.klen - r.qlen;  // under a causal mask token t sees keys <= t + shift
@@ -1690,6 +1694,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
                      const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ g_lse,
                      bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots, int ranks) {
     using S = BwdShape<DP>;
+    constexpr int kWalk = S::kWalk;
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(16) BwdShared sh;
     const int warp = warp_index();
@@ -1739,7 +1744,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
             mbar_init(&sh.y_raw, 1);
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&sh.s_full[b], 1);
-                mbar_init(&sh.ds_ready[b], 8);
+                mbar_init(&sh.ds_ready[b], S::kHalves * 4);
             }
             mbar_init(&sh.acc_done, 1);
             mbar_init(&sh.drain, 1);
@@ -1749,7 +1754,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         __syncwarp();
         tmem_alloc(&sh.tmem, S::kTmem);
     }
-    // Rows of a step that no box ever fills (heads that do not divide 64) must hold numbers.
+    // Rows of a step that no box ever fills (heads that do not divide a step) must hold numbers.
     if (DKV && r.tok * A.pack < kWalk) {
         for (int i = threadIdx.x; i < S::kStages * 2 * S::kYBytes / 16; i += S::kThreads)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_y + i * 16), "r"(0) : "memory");
@@ -1767,20 +1772,20 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const size_t row_at = DKV ? ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D
                               : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
     if (warp >= S::kCompute) {
-        regs_less<S::Regs::kLess>();
+        if constexpr (DP > 32) regs_less<S::Regs::kLess>();
         if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem, A.D);
         if (warp == S::kCompute + 1)
             issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
     } else {
-        regs_more<S::Regs::kMore>();
+        if constexpr (DP > 32) regs_more<S::Regs::kMore>();
         bwd_grads<DP, DKV>(A, sh, r, tmem, lse, delta, g_lse);
         __syncwarp();
-        if (ranks == 1) store_acc<DP, DKV, 2 * S::kPairs>(A, acc, steps > 0, row_at, live, g0, g1);
+        if (ranks == 1) store_acc<DP, DKV, S::kCompute / 4>(A, acc, steps > 0, row_at, live, g0, g1);
     }
     if (ranks > 1) {
         // Every product of this block is done, so its shared memory is free.
         __syncthreads();
-        share_acc<DP, DKV, 2 * S::kPairs>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
+        share_acc<DP, DKV, S::kCompute / 4>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
     }
     __syncwarp();
     tc_fence_before();
@@ -2016,7 +2021,8 @@ struct BackwardPlan {
     int kv_ranks, q_ranks;
 };
 
-BackwardPlan plan_backward(const AttnArgs &A) {
+template <int DP> BackwardPlan plan_backward(const AttnArgs &A) {
+    using S = BwdShape<DP>;
     const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
     const long long rows = (A.Tq + n_seq - 1) / n_seq, keys = (A.Tk + n_seq - 1) / n_seq;  // of the mean sequence
     const int per = 128 / A.pack;
@@ -2026,8 +2032,8 @@ BackwardPlan plan_backward(const AttnArgs &A) {
         return r;
     };
     BackwardPlan p;
-    p.kv_ranks = ranks(n_seq * A.Hkv * ((keys + 127) / 128), rows * A.pack * A.subs / kWalk);
-    p.q_ranks = ranks(n_seq * A.Hkv * A.subs * ((rows + per - 1) / per), keys / kWalk);
+    p.kv_ranks = ranks(n_seq * A.Hkv * ((keys + 127) / 128), rows * A.pack * A.subs / S::kWalk);
+    p.q_ranks = ranks(n_seq * A.Hkv * A.subs * ((rows + per - 1) / per), keys / S::kWalk);
     const KnobValue forced = knob(kKnobAttnBwd);
     auto valid = [](int r) { return r == 1 || r == 2 || r == 4; };
     if (forced.count > 0 && valid(forced.v[0])) p.kv_ranks = forced.v[0];
@@ -2061,7 +2067,8 @@ template <int DP>
 int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
                     const float *lse, const float *delta, const float *g_lse, bf16 *dq, bf16 *dk, bf16 *dv,
                     cudaStream_t stream) {
-    const BackwardPlan plan = plan_backward(A);
+    constexpr int kWalk = BwdShape<DP>::kWalk;
+    const BackwardPlan plan = plan_backward<DP>(A);
     CUtensorMap kx, vx, qy, gy, qx, gx, ky, vy;
     const int ytok = kWalk / A.pack, xtok = 128 / A.pack;
     if (!make_map(&kx, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) || !make_map(&vx, v, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
@@ -2203,7 +2210,7 @@ extern "C" int rfdetr_packed_attention_backward(
     const size_t need = rfdetr_packed_attention_backward_workspace_bytes(tokens, n_heads);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 4))) return RFDETR_ERR_WORKSPACE;
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
-                                 causal, scale, kWalk);
+                                 causal, scale, head_dim <= 32 ? BwdShape<32>::kWalk : BwdShape<64>::kWalk);
     float *delta = static_cast<float *>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tokens > 0) {

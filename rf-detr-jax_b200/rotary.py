@@ -13,9 +13,10 @@ from . import _native as N
 
 
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.dim() != 3:
+    strides = t.stride()
+    if len(strides) != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
-    return t if t.stride(2) == 1 else t.contiguous()
+    return t if strides[2] == 1 else t.contiguous()
 
 
 def _pairs(t: torch.Tensor) -> torch.Tensor:
@@ -31,17 +32,18 @@ def rotary_launch(query, key, positions, inv_freq, sections, interleaved, invers
     tokens, heads, dim = query.shape
     if interleaved:
         query, key = _pairs(query), None if key is None else _pairs(key)
-    out = query.new_empty((tokens, heads, dim))
+    out = query.new_empty(tokens, heads, dim)
     key_out, kv_heads, key_strides = None, 0, (0, 0)
     if key is not None:
         kv_heads, key_strides = key.shape[1], key.stride()[:2]
-        key_out = key.new_empty((tokens, kv_heads, dim))
+        key_out = key.new_empty(tokens, kv_heads, dim)
     status = N.lib().rfdetr_axial_rotary(
         N.stream_of(query), query.data_ptr(), *query.stride()[:2], N.ptr(key), *key_strides,
         N.dtype_code(query.dtype), positions.data_ptr(), N.F32 if positions.dtype == torch.float32 else N.I32,
-        inv_freq.data_ptr(), N.int64_array(sections), len(sections), out.data_ptr(), N.ptr(key_out), tokens, heads,
-        kv_heads, dim, int(interleaved), int(inverse))
-    N.check(status, "rfdetr_axial_rotary")
+        inv_freq.data_ptr(), N.const_int64_array(sections), len(sections), out.data_ptr(), N.ptr(key_out), tokens, heads,
+        kv_heads, dim, interleaved, inverse)
+    if status:
+        N.check(status, "rfdetr_axial_rotary")
     return out, key_out
 
 
@@ -78,16 +80,16 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         ``(query, key)`` turned, contiguous, in their own type; differentiable with respect to
         both (not to the positions or frequencies).
     """
-    N.require_cuda(query, key, positions, inv_freq)
+    N.same_device(query, key, positions, inv_freq)
     query = _rows("query", query)
     tokens, _, dim = query.shape
-    if query.dtype not in (torch.float32, torch.bfloat16):
+    if query.dtype != torch.float32 and query.dtype != torch.bfloat16:
         raise ValueError(f"query must be float32 or bfloat16, got {query.dtype}")
     if key is not None:
         key = _rows("key", key)
         if key.shape[0] != tokens or key.shape[2] != dim or key.dtype != query.dtype:
             raise ValueError("key must have the query's tokens, head_dim and type")
-    sections = tuple(int(n) for n in sections)
+    sections = tuple(map(int, sections))
     half = sum(sections)
     if not 1 <= len(sections) <= 8 or min(sections) < 0 or half < 1 or 2 * half > dim:
         raise ValueError(f"sections {sections} do not fit head_dim {dim}")
@@ -95,7 +97,7 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"positions must be [{tokens}, {len(sections)}], got {list(positions.shape)}")
     if positions.dtype == torch.int64:
         positions = positions.to(torch.int32)
-    if positions.dtype not in (torch.float32, torch.int32):
+    if positions.dtype != torch.float32 and positions.dtype != torch.int32:
         raise ValueError(f"positions must be float32 or int32, got {positions.dtype}")
     if inv_freq.shape != (half,) or inv_freq.dtype != torch.float32:
         raise ValueError(f"inv_freq must be float32 [{half}]")
