@@ -54,8 +54,18 @@ bool encode_tensor_map(CUtensorMap *map, CUtensorMapDataType dtype, int rank, co
         es[i] = 1;
         if (i + 1 < rank) st[i] = strides_bytes[i];
     }
-    return encode(map, dtype, (cuuint32_t)rank, const_cast<void *>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    auto call = [&] {
+        return encode(map, dtype, (cuuint32_t)rank, const_cast<void *>(base), d, st, bx, es,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // A thread that has made no runtime call yet has no context: any binds the device's.
+        if (cudaFree(nullptr) != cudaSuccess) return false;
+        r = call();
+    }
+    return r == CUDA_SUCCESS;
 }
 
 }  // namespace rfdetr

@@ -3,6 +3,8 @@ the oracle derives from the operator's roundings (bf16 weights and results, floa
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -249,6 +251,32 @@ def test_same_bits_each_time_and_on_another_stream(pkg):
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_a_thread_that_has_made_no_other_call(pkg):
+    """A new thread has no current context of the device until some call gives it one."""
+    rng = np.random.default_rng(8)
+    q, k, v, g = (_bf16(rng, 40, 2, 64) for _ in range(4))
+    off = _offsets((40,))
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    want = pkg.packed_attention(q, k, v, off)
+    loss = (pkg.packed_attention(*leaves, off).float() * g.float()).sum()
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    out, status = torch.empty_like(q), []
+    lib = pkg._native.lib()
+    args = [stream]
+    for x in (q, k, v):
+        args += [x.data_ptr(), *x.stride()[:2]]
+    args += [off.data_ptr(), None, out.data_ptr(), None, None, None, 0, 1, 40, 40, 2, 2, 64, 0, 0.125]
+    thread = threading.Thread(target=lambda: status.append(lib.rfdetr_packed_attention(*args)))
+    thread.start()
+    thread.join()
+    assert status == [pkg._native.OK]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    loss.backward()
+    assert all(torch.isfinite(x.grad).all() for x in leaves)
 
 
 def test_empty_tensors(pkg):
