@@ -1349,6 +1349,19 @@ struct BwdShared {
     alignas(16) float neg_lse2[4][64];
     alignas(16) float neg_delta[4][64];
     alignas(16) float one_ds[4][64];
+    float row_dot[128];  // dQ: o.g of the held rows
+};
+
+// What both kernels know of the query rows.  The dQ kernel runs first and leaves delta = o.g - (the lse's
+// cotangent) for the other; o is the output with what its rounding lost (with the rounded output alone dQ and
+// dK were off by 1.5 to 1.6 times what plain bf16 calls are, with both by 1.4).  (With a kernel of its own for
+// delta, and without the overlap of the two, 16 of 1 to 1601 tokens, 6 heads of 64, took 200 us both passes, now
+// 189; 104 x 300, 8 of 32: 232 and 231.)
+struct BwdRows {
+    const bf16 *out, *low, *g;
+    long long g_token, g_head;
+    const float *lse, *g_lse;  // g_lse: or null
+    float *delta;
 };
 
 // What a block walks.  DKV: `steps_per_sub` tiles of `tok` tokens from token `first` on, for each of
@@ -1368,7 +1381,7 @@ struct BwdRange {
 template <int DP, bool DKV>
 __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtensorMap *mx1, const CUtensorMap *my0,
                         const CUtensorMap *my1, BwdShared &sh, uint32_t smem_x, uint32_t smem_y, const BwdRange &r,
-                        const float *lse, const float *delta, const float *g_lse) {
+                        const BwdRows &f) {
     using S = BwdShape<DP>;
     constexpr int kWalk = S::kWalk;
     using TL = Tile<DP>;
@@ -1386,6 +1399,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
             tma_load_3d_one(smem_x + S::kXBytes + o, mx1, &sh.x_full, p * TL::kCols, head, at);
         }
     }
+    if (DKV) wait_for_primary();
     const int yrows = DKV ? r.tok * A.pack : kWalk;
     unsigned raw_phase = 0;
     int i = 0;
@@ -1417,9 +1431,9 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 float nl = 0.0f, nd = 0.0f, od = 0.0f;
                 if (c < good) {
                     const size_t x = (size_t)(head + row_head(A, c)) * A.Tq + base + at + row_token(A, c);
-                    nl = -lse[x] * kLog2e;
-                    nd = -delta[x];
-                    if (g_lse) od = g_lse[x];
+                    nl = -f.lse[x] * kLog2e;
+                    nd = -__ldcg(f.delta + x);
+                    if (f.g_lse) od = f.g_lse[x];
                 }
                 sh.neg_lse2[st][c] = nl;
                 sh.neg_delta[st][c] = nd;
@@ -1498,8 +1512,8 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
 
 // The kHalves warpgroups w: the steps i with i % kPairs == w, 32 columns each.
 template <int DP, bool DKV>
-__device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const float *lse,
-                          const float *delta, const float *g_lse) {
+__device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const BwdRows &f,
+                          bool write_delta) {
     using S = BwdShape<DP>;
     constexpr int kWalk = S::kWalk;
     volatile int *abort = &sh.abort;
@@ -1512,12 +1526,42 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     const int tok = r.q0 + row_token(A, row);
     int limit = 0;
     float row_nl = 0.0f, row_nd = 0.0f, row_od = 0.0f;
-    if (!DKV && row_token(A, row) < r.qtok) {
-        limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
-        const size_t x = (size_t)(r.qhead + row_head(A, row)) * A.Tq + r.qbase + tok;
-        row_nl = -lse[x] * kLog2e;
-        row_nd = -delta[x];
-        if (g_lse) row_od = g_lse[x];
+    if (!DKV) {
+        // o.g of the held rows: DP / 8 lanes to a row, so that a warp's loads lie together (a thread to 32
+        // channels of a row took 6 us a block with 128 channels).
+        constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
+        static_assert(S::kCompute * 4 * kRows == 128, "four turns");
+        const int lane = threadIdx.x & 31, c = lane % kLanes * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = ((threadIdx.x >> 5) * 4 + k) * kRows + lane / kLanes;
+            float sum = 0.0f;
+            if (row_token(A, at) < r.qtok && c < A.D) {
+                const size_t token = (size_t)r.qbase + r.q0 + row_token(A, at);
+                const int head = r.qhead + row_head(A, at);
+                const size_t o = (token * A.Hq + head) * A.D + c;
+                float a[8], b[8], l[8];
+                load_vec<bf16, 8, true>(f.out + o, a);
+                load_vec<bf16, 8, true>(f.low + o, l);
+                load_vec<bf16, 8, true>(f.g + token * f.g_token + head * f.g_head + c, b);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(l[e], b[e], sum);
+            }
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane % kLanes == 0) sh.row_dot[at] = sum;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(S::kCompute * 32) : "memory");
+        if (row_token(A, row) < r.qtok) {
+            limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
+            const size_t x = (size_t)(r.qhead + row_head(A, row)) * A.Tq + r.qbase + tok;
+            row_nl = -f.lse[x] * kLog2e;
+            if (f.g_lse) row_od = f.g_lse[x];
+            row_nd = row_od - sh.row_dot[row];
+            if (write_delta && group == 0) f.delta[x] = -row_nd;
+        }
     }
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
@@ -1691,8 +1735,7 @@ template <int DP, bool DKV>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, const __grid_constant__ CUtensorMap mx1,
                      const __grid_constant__ CUtensorMap my0, const __grid_constant__ CUtensorMap my1,
-                     const float *__restrict__ lse, const float *__restrict__ delta, const float *__restrict__ g_lse,
-                     bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots, int ranks) {
+                     const BwdRows f, bf16 *__restrict__ g0, bf16 *__restrict__ g1, int slots, int ranks) {
     using S = BwdShape<DP>;
     constexpr int kWalk = S::kWalk;
     extern __shared__ unsigned char dyn[];
@@ -1706,6 +1749,10 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const int per = DKV ? 128 : 128 / A.pack;
     const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, A.slot_rows, slot)
                        : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
+    // The dK/dV launch overlaps the dQ one's end: its loads wait for delta, and its first block at least, so that it
+    // does not end before the other.
+    if (!DKV) launch_dependents();
+    else if (blockIdx.x == 0) wait_for_primary();
     if (x.first >= x.len) return;
     const int G = A.Hq / A.Hkv;
     BwdRange r;
@@ -1775,10 +1822,10 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         if constexpr (DP > 32) regs_less<S::Regs::kLess>();
         if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem, A.D);
         if (warp == S::kCompute + 1)
-            issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, lse, delta, g_lse);
+            issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, f);
     } else {
         if constexpr (DP > 32) regs_more<S::Regs::kMore>();
-        bwd_grads<DP, DKV>(A, sh, r, tmem, lse, delta, g_lse);
+        bwd_grads<DP, DKV>(A, sh, r, tmem, f, rank == 0);
         __syncwarp();
         if (ranks == 1) store_acc<DP, DKV, S::kCompute / 4>(A, acc, steps > 0, row_at, live, g0, g1);
     }
@@ -1803,39 +1850,6 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, S::kTmem);
-    }
-}
-
-// delta[h][t] = o.g - c per row, LANES lanes of eight channels to a row; o is the output with what its rounding
-// lost (with the rounded output alone dQ and dK were off by 1.5 to 1.6 times what plain bf16 calls are, with both
-// by 1.4).  Reads three rows and writes one number: 31,200 tokens of 256 channels 8.2 us (5.8 TB/s).
-template <int LANES>
-__global__ void __launch_bounds__(256)
-attn_delta_kernel(const bf16 *__restrict__ out, const bf16 *__restrict__ low, const bf16 *__restrict__ g,
-                  long long g_token, long long g_head,
-                  const float *__restrict__ g_lse, int Tq, int Hq, int D, float *__restrict__ delta) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = i / LANES;  // token * Hq + head
-    const int c = (int)(i % LANES) * 8;
-    const bool live = row < (long long)Tq * Hq && c < D;
-    const long long token = row / Hq;
-    const int head = (int)(row % Hq);
-    float sum = 0.0f;
-    if (live) {
-        float a[8], b[8];
-        load_vec<bf16, 8, true>(out + row * D + c, a);
-        load_vec<bf16, 8, true>(g + token * g_token + head * g_head + c, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
-        load_vec<bf16, 8, true>(low + row * D + c, a);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (live && c == 0) {
-        const size_t x = (size_t)head * Tq + token;
-        delta[x] = sum - (g_lse ? g_lse[x] : 0.0f);
     }
 }
 
@@ -2042,7 +2056,7 @@ template <int DP> BackwardPlan plan_backward(const AttnArgs &A) {
 }
 
 template <int DP, bool DKV, typename... Args>
-int launch_backward_kernel(long long tiles, int ranks, cudaStream_t stream, Args... args) {
+int launch_backward_kernel(long long tiles, int ranks, bool overlap, cudaStream_t stream, Args... args) {
     using S = BwdShape<DP>;
     if (tiles * ranks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
     if (int st = allow_smem(attn_backward_kernel<DP, DKV>, S::kSmem)) return st;
@@ -2051,11 +2065,16 @@ int launch_backward_kernel(long long tiles, int ranks, cudaStream_t stream, Args
     config.blockDim = dim3(S::kThreads);
     config.dynamicSmemBytes = S::kSmem;
     config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
-    config.attrs = &attr;
-    config.numAttrs = ranks > 1 ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    config.attrs = attr;
+    if (ranks > 1) {
+        attr[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[config.numAttrs++].val.clusterDim = {(unsigned)ranks, 1, 1};
+    }
+    if (overlap) {
+        attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     if (cudaLaunchKernelEx(&config, attn_backward_kernel<DP, DKV>, args..., ranks) != cudaSuccess) {
         (void)cudaGetLastError();
         return RFDETR_ERR_CUDA;
@@ -2065,7 +2084,7 @@ int launch_backward_kernel(long long tiles, int ranks, cudaStream_t stream, Args
 
 template <int DP>
 int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
-                    const float *lse, const float *delta, const float *g_lse, bf16 *dq, bf16 *dk, bf16 *dv,
+                    const BwdRows &f, bf16 *dq, bf16 *dk, bf16 *dv,
                     cudaStream_t stream) {
     constexpr int kWalk = BwdShape<DP>::kWalk;
     const BackwardPlan plan = plan_backward<DP>(A);
@@ -2076,20 +2095,18 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
         !make_map(&qy, q, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) || !make_map(&gy, g, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) ||
         !make_map(&qx, q, A.Tq, A.Hq, A.D, A.pack, xtok, k.p) || !make_map(&gx, g, A.Tq, A.Hq, A.D, A.pack, xtok, k.p))
         return RFDETR_ERR_CUDA;
-    if (A.Tk > 0) {
-        const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
-        A.slot_rows = divisor(128);
-        A.heads = divisor(A.Hkv);
-        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, stream, A, kx, vx, qy, gy, lse, delta,
-                                                      g_lse, dk, dv, (int)slots))
-            return st;
-    }
     if (A.Tq > 0) {
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
         A.slot_rows = divisor(xtok);
         A.heads = divisor(A.Hkv * A.subs);
-        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, stream, A, qx, gx, ky, vy, lse, delta,
-                                                       g_lse, dq, nullptr, (int)slots))
+        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq, nullptr, (int)slots))
+            return st;
+    }
+    if (A.Tk > 0) {
+        const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
+        A.slot_rows = divisor(128);
+        A.heads = divisor(A.Hkv);
+        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk, dv, (int)slots))
             return st;
     }
     return RFDETR_OK;
@@ -2211,28 +2228,15 @@ extern "C" int rfdetr_packed_attention_backward(
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 4))) return RFDETR_ERR_WORKSPACE;
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
                                  causal, scale, head_dim <= 32 ? BwdShape<32>::kWalk : BwdShape<64>::kWalk);
-    float *delta = static_cast<float *>(workspace);
+    const BwdRows f{static_cast<const bf16 *>(output), static_cast<const bf16 *>(output_low),
+                    static_cast<const bf16 *>(grad_output), grad_token_stride, grad_head_stride, lse, grad_lse,
+                    static_cast<float *>(workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tokens > 0) {
-        const int dp = padded_dim(head_dim);
-        const long long rows = (long long)tokens * n_heads, blocks = (rows * (dp / 8) + 255) / 256;
-        if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-        const bf16 *low = static_cast<const bf16 *>(output_low);
-        const bf16 *o = static_cast<const bf16 *>(output), *go = static_cast<const bf16 *>(grad_output);
-        auto launch = [&](auto kernel) {
-            kernel<<<(unsigned)blocks, 256, 0, s>>>(o, low, go, grad_token_stride, grad_head_stride, grad_lse, (int)tokens,
-                                                    (int)n_heads, (int)head_dim, delta);
-        };
-        if (dp == 32) launch(attn_delta_kernel<4>);
-        else if (dp == 64) launch(attn_delta_kernel<8>);
-        else launch(attn_delta_kernel<16>);
-        if (int st = launch_status()) return st;
-    }
     bf16 *dq = static_cast<bf16 *>(grad_query), *dk = static_cast<bf16 *>(grad_key),
          *dv = static_cast<bf16 *>(grad_value);
     switch (padded_dim(head_dim)) {
-        case 32: return launch_backward<32>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
-        case 64: return launch_backward<64>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
-        default: return launch_backward<128>(A, q, k, v, g, lse, delta, grad_lse, dq, dk, dv, s);
+        case 32: return launch_backward<32>(A, q, k, v, g, f, dq, dk, dv, s);
+        case 64: return launch_backward<64>(A, q, k, v, g, f, dq, dk, dv, s);
+        default: return launch_backward<128>(A, q, k, v, g, f, dq, dk, dv, s);
     }
 }
