@@ -96,6 +96,21 @@ inline int launch_status() {
     return err == cudaSuccess ? RFDETR_OK : RFDETR_ERR_CUDA;
 }
 
+// A divisor known to the host, and division by it for x up to 2^31 (Granlund and Montgomery's: the high half
+// of x times 2^32 (2^shift - d) / d, rounded up, plus x, shifted).
+struct Divisor {
+    unsigned magic, shift;
+    int d;
+};
+inline Divisor divisor(int d) {
+    unsigned l = 0;
+    while ((1ll << l) < d) ++l;
+    return {(unsigned)(((1ull << 32) * ((1ull << l) - (unsigned)d)) / (unsigned)d + 1), l, d};
+}
+__device__ __forceinline__ int quotient(int x, const Divisor &d) {
+    return (int)((__umulhi(d.magic, (unsigned)x) + (unsigned)x) >> d.shift);
+}
+
 int num_sms();  // SM count of the current device (cached per device)
 
 // Process-wide tuning knobs, for experiments and tests.  A knob holds up to five integers, set

@@ -32,6 +32,7 @@ struct RotaryArgs {
     long long T;
     int D, half;
     int per_block;           // tokens
+    Divisor per_token, per_head, half_of;  // pieces of a token and of a head; half
     float sign;              // -1: the inverse turn
 };
 
@@ -46,22 +47,28 @@ __device__ __forceinline__ float second_of(float x1, float x2, float2 r) {
 
 // Pieces of VEC channels.  A head's pieces: the turned ones first (one piece of x1 and one of x2,
 // or one piece of VEC / 2 pairs), then the copied ones.  A thread asks for its first piece before the
-// sines are formed, so that their time covers the load's.  More pieces in flight per thread cost more in
-// resident threads than they gave: 32,768 tokens of 20 x 128 channels, bf16, 65 us (5.2 TB/s, 81% of the
-// measured copy rate) with one, 70 with two, 88 with four; 20,011 of 8 x 80, partly turned, 30.7, 28.7 and
-// 36.2 us there and back.
+// sines are formed, so that their time covers the load's.  32,768 tokens of 20 x 128 channels, bf16, take 54 us
+// (6.2 TB/s, 96% of the measured copy rate), 20,011 of 8 x 80, partly turned, 25.8 there and back; with a
+// second piece in flight per thread 3 us more and 0.7 less.  Places are found with known divisors (57.6 and 31.0
+// us by division).
+
+// Where frequency i's cosine and sine are: one place is left out after every piece's, so that the pieces of a warp's
+// lanes read from different banks (without: 7 us more for the first of the tokens above).
+template <int VEC, bool INTERLEAVED> __host__ __device__ constexpr int turn_at(int i) {
+    constexpr int kGroup = INTERLEAVED ? VEC / 2 : VEC;
+    return kGroup > 1 ? i + i / kGroup : i;
+}
 
 template <typename T, typename P, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotaryThreads) axial_rotary_kernel(const RotaryArgs A) {
     using V = typename Raw<VEC * (int)sizeof(T)>::T;
-    extern __shared__ float2 turn[];  // [token][half]
+    extern __shared__ float2 turn[];  // [token][turn_at(half)]
+    const int pitch = turn_at<VEC, INTERLEAVED>(A.half);
     const long long t0 = (long long)blockIdx.x * A.per_block;
     const int tokens = (int)min((long long)A.per_block, A.T - t0);
     const int R = 2 * A.half;
-    const int turned = INTERLEAVED ? R / VEC : A.half / VEC;
-    const int per_head = turned + (A.D - R) / VEC;
-    const int per_token = per_head * (A.heads[0] + A.heads[1]);
-    const int pieces = tokens * per_token;
+    const int turned = (INTERLEAVED ? R : A.half) / VEC;
+    const int pieces = tokens * A.per_token.d;
 
     struct Piece {
         T *out;
@@ -70,9 +77,9 @@ __global__ void __launch_bounds__(kRotaryThreads) axial_rotary_kernel(const Rota
         V x1, x2;
     } p;
     auto ask = [&](int x) {
-        const int t = x / per_token, y = x - t * per_token;
-        int h = y / per_head;
-        const int piece = y - h * per_head;
+        const int t = quotient(x, A.per_token), y = x - t * A.per_token.d;
+        int h = quotient(y, A.per_head);
+        const int piece = y - h * A.per_head.d;
         const int which = h >= A.heads[0];
         h -= which ? A.heads[0] : 0;
         const T *in = static_cast<const T *>(A.in[which]) + (t0 + t) * A.token[which] + h * A.head[which];
@@ -87,19 +94,19 @@ __global__ void __launch_bounds__(kRotaryThreads) axial_rotary_kernel(const Rota
 
     const P *pos = static_cast<const P *>(A.positions) + t0 * A.n_axes;
     for (int x = threadIdx.x; x < tokens * A.half; x += kRotaryThreads) {
-        const int t = x / A.half, i = x - t * A.half;
+        const int t = quotient(x, A.half_of), i = x - t * A.half;
         int axis = 0;
         while (i >= A.ends[axis]) ++axis;
         const double turns = (double)pos[t * A.n_axes + axis] * (double)__ldg(A.inv_freq + i) * kInvTwoPi;
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        turn[x] = make_float2(c, s * A.sign);
+        turn[t * pitch + turn_at<VEC, INTERLEAVED>(i)] = make_float2(c, s * A.sign);
     }
     __syncthreads();
 
     for (int x = threadIdx.x; x < pieces;) {
         if (p.turns) {
-            const float2 *cs = turn + p.token * A.half + (INTERLEAVED ? p.c / 2 : p.c);
+            const float2 *cs = turn + p.token * pitch + turn_at<VEC, INTERLEAVED>(INTERLEAVED ? p.c / 2 : p.c);
             const T *a = reinterpret_cast<const T *>(&p.x1), *b = reinterpret_cast<const T *>(&p.x2);
             float u[VEC], w[VEC];
             if constexpr (INTERLEAVED) {
@@ -134,14 +141,16 @@ template <typename T, typename P, int VEC>
 int launch_rotary(const RotaryArgs &A, bool interleaved, cudaStream_t stream) {
     const long long blocks = (A.T + A.per_block - 1) / A.per_block;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    const size_t smem = (size_t)A.per_block * A.half * sizeof(float2);
+    auto smem = [&](int pitch) { return (size_t)A.per_block * pitch * sizeof(float2); };
     if (interleaved) {
         if constexpr (VEC >= 2)
-            axial_rotary_kernel<T, P, VEC, true><<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(A);
+            axial_rotary_kernel<T, P, VEC, true>
+                <<<(unsigned)blocks, kRotaryThreads, smem(turn_at<VEC, true>(A.half)), stream>>>(A);
         else
             return RFDETR_ERR_SHAPE;
     } else {
-        axial_rotary_kernel<T, P, VEC, false><<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(A);
+        axial_rotary_kernel<T, P, VEC, false>
+            <<<(unsigned)blocks, kRotaryThreads, smem(turn_at<VEC, false>(A.half)), stream>>>(A);
     }
     return launch_status();
 }
@@ -203,11 +212,12 @@ extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t quer
     };
     if (!fits(vec)) vec = fits(2) ? 2 : 1;
     if (interleaved && vec < 2) return RFDETR_ERR_ALIGN;
-    // Tokens to a block: two pieces to a thread (one: 84 us for the first of the tokens above; eight: 66 us, and
-    // 35.1 for the second),
-    // fewer where that would leave SMs without four blocks, and no more than 16 KB of sines.
+    // Tokens to a block: two pieces to a thread (one: 69.7 us for the first of the tokens above and 29.0 for the
+    // second; four: 53.5 and 26.6; eight: 56.9 and 28.5), fewer where that would leave SMs without four blocks, and no more than 16 KB of sines.
     const long long turned = interleaved ? 2 * half / vec : half / vec;
-    const long long per_token = (turned + (head_dim - 2 * half) / vec) * (n_heads + n_kv_heads);
+    const long long per_head = turned + (head_dim - 2 * half) / vec;
+    const long long per_token = per_head * (n_heads + n_kv_heads);
+    A.per_head = divisor((int)per_head), A.per_token = divisor((int)per_token), A.half_of = divisor((int)half);
     long long per = 2ll * kRotaryThreads / per_token;
     const long long spread = tokens / (4ll * num_sms()), most = 16384 / (half * (long long)sizeof(float2));
     per = per > spread ? spread : per;
