@@ -429,7 +429,7 @@ __device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return mi
 // (setmaxnreg): a row of S is 128 values.
 // What bounds it is the chain of a row tile from S through the maximum, the exponentials and P to P V, of
 // which two tiles in flight hide about half: 10,052 causal tokens of six prompts, 16 / 4 heads of 128, take
-// 129 us, 970 TFLOP/s of the products that the mask leaves (59% of the measured peak), with the tensor pipe
+// 127 us, 990 TFLOP/s of the products that the mask leaves (60% of the measured peak), with the tensor pipe
 // 50%, the special-function unit 45% and the issue slots 37% busy.  Four warpgroups, two to a row tile, took
 // 150 us: what each waits for is the other roles, not its own work.
 // Where the launch has no more row tiles than SMs, two to a block would leave SMs without one: a block has one, and
@@ -849,8 +849,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
         if (warp == 8) {
             if (r.end > r.j0) long_mma_loop<DP, ALT>(sh, smem_q, smem_kv, r, tmem, A.D);
         } else if (warp == 9) {
-            issued = long_load<DP, ALT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per, kbase,
-                                   klen);
+            issued = long_load<DP, ALT>(A, &mq, &mk, &mv, sh, smem_q, smem_kv, r, kvh, qhead, q.base + q.first, per,
+                                        kbase, klen);
         }
     } else {
         regs_more<S::Regs::kMore>();
@@ -978,8 +978,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
 // it works (104 x 300 tokens of 8 heads of 32: blocks that come and go cost 13.7 us by themselves, and
 // finding their rows 14 more, of 62).  128 threads: each owns a row, warp 0 also issues the copies and
 // the products.  64 keys a tile, so that S and O of four blocks fit TMEM and a row of S is 64 registers.
-// Those 104 x 300 tokens take 57 us (62 with `low`), 32 x 145 of 6 heads of 64 12.0 us: latencies still (a third of the special
-// functions' rate, 42% of the issue slots); 256 threads, half a row each, took 66 and 15.3 us.
+// Those 104 x 300 tokens take 57 us (62 with `low`), 32 x 145 of 6 heads of 64 12.0 us: latencies still (40% of the
+// special functions' rate, 41% of the issue slots); 256 threads, half a row each, took 66 and 15.3 us.
 template <int DP> struct ShortShape {
     static constexpr int kKeys = 64;
     static constexpr int kQBytes = 128 * DP * 2;
@@ -1561,8 +1561,8 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             continue;
         }
         tc_fence_after();
-        // Of this thread's columns c0 ..: [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or the
-        // whole row is (DQ) a query with a single key.
+        // Of this thread's columns c0 ..: [lo, hi) of this row are seen; those in [one_lo, one_hi) belong to (DKV) or
+        // the whole row is (DQ) a query with a single key.
         int lo = 0, hi = kWalk, one_lo = 0, one_hi = 0;
         bool mask;
         if (DKV) {
@@ -1802,7 +1802,8 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21) + S::kAcc;
     const bool live = DKV ? r.k0 + row < r.klen : row_token(A, row) < r.qtok;
     const size_t row_at = DKV ? ((size_t)(r.kbase + r.k0 + row) * A.Hkv + r.kvh) * A.D
-                              : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) * A.D;
+                              : ((size_t)(r.qbase + r.q0 + row_token(A, row)) * A.Hq + r.qhead + row_head(A, row)) *
+                                    A.D;
     if (warp >= S::kCompute) {
         if constexpr (DP > 32) regs_less<S::Regs::kLess>();
         if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem, A.D);
@@ -1988,7 +1989,8 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
     using S = LongShape<DP, false>;  // (its block and shared memory are those of the alternating kernel too)
     auto launch = [&](auto kernel) {
         if (int st = allow_smem(kernel, S::kSmem)) return st;
-        kernel<<<(unsigned)(plan.blocks ? plan.blocks : blocks), S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, f, slots);
+        const unsigned grid = (unsigned)(plan.blocks ? plan.blocks : blocks);
+        kernel<<<grid, S::kThreads, S::kSmem, stream>>>(A, mq, mk, mv, f, slots);
         return launch_status();
     };
     if (plan.blocks == 0)
@@ -2069,29 +2071,32 @@ int launch_backward_kernel(long long tiles, int ranks, bool overlap, cudaStream_
 
 template <int DP>
 int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
-                    const BwdRows &f, bf16 *dq, bf16 *dk, bf16 *dv,
-                    cudaStream_t stream) {
+                    const BwdRows &f, bf16 *dq, bf16 *dk, bf16 *dv, cudaStream_t stream) {
     constexpr int kWalk = BwdShape<DP>::kWalk;
     const BackwardPlan plan = plan_backward<DP>(A);
     CUtensorMap kx, vx, qy, gy, qx, gx, ky, vy;
     const int ytok = kWalk / A.pack, xtok = 128 / A.pack;
     if (!make_map(&kx, k, A.Tk, A.Hkv, A.D, 1, 128, q.p) || !make_map(&vx, v, A.Tk, A.Hkv, A.D, 1, 128, q.p) ||
         !make_map(&ky, k, A.Tk, A.Hkv, A.D, 1, kWalk, q.p) || !make_map(&vy, v, A.Tk, A.Hkv, A.D, 1, kWalk, q.p) ||
-        !make_map(&qy, q, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) || !make_map(&gy, g, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) ||
-        !make_map(&qx, q, A.Tq, A.Hq, A.D, A.pack, xtok, k.p) || !make_map(&gx, g, A.Tq, A.Hq, A.D, A.pack, xtok, k.p))
+        !make_map(&qy, q, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) ||
+        !make_map(&gy, g, A.Tq, A.Hq, A.D, A.pack, ytok, k.p) ||
+        !make_map(&qx, q, A.Tq, A.Hq, A.D, A.pack, xtok, k.p) ||
+        !make_map(&gx, g, A.Tq, A.Hq, A.D, A.pack, xtok, k.p))
         return RFDETR_ERR_CUDA;
     if (A.Tq > 0) {
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
         A.slot_rows = divisor(xtok);
         A.heads = divisor(A.Hkv * A.subs);
-        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq, nullptr, (int)slots))
+        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq,
+                                                       nullptr, (int)slots))
             return st;
     }
     if (A.Tk > 0) {
         const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
         A.slot_rows = divisor(128);
         A.heads = divisor(A.Hkv);
-        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk, dv, (int)slots))
+        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk,
+                                                      dv, (int)slots))
             return st;
     }
     return RFDETR_OK;
@@ -2157,8 +2162,8 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     if (int st = check_tensor(q, tokens, n_heads)) return st;
     if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
     if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
-    if (!output || !aligned(output, 16) || !aligned(output_low, 16) || !aligned(lse, 4) || !offsets || !aligned(offsets, 4) ||
-        !aligned(key_offsets, 4))
+    if (!output || !aligned(output, 16) || !aligned(output_low, 16) || !aligned(lse, 4) || !offsets ||
+        !aligned(offsets, 4) || !aligned(key_offsets, 4))
         return RFDETR_ERR_ALIGN;
     const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
                                  causal, scale, 128);
@@ -2204,8 +2209,8 @@ extern "C" int rfdetr_packed_attention_backward(
     if (int st = check_tensor(k, key_tokens, n_kv_heads)) return st;
     if (int st = check_tensor(v, key_tokens, n_kv_heads)) return st;
     if (!offsets || !aligned(offsets, 4) || !aligned(key_offsets, 4)) return RFDETR_ERR_ALIGN;
-    if (tokens > 0 && (!output || !aligned(output, 16) || !output_low || !aligned(output_low, 16) || !grad_query || !aligned(grad_query, 16) || !lse ||
-                       !aligned(lse, 4) || !aligned(grad_lse, 4)))
+    if (tokens > 0 && (!output || !aligned(output, 16) || !output_low || !aligned(output_low, 16) || !grad_query ||
+                       !aligned(grad_query, 16) || !lse || !aligned(lse, 4) || !aligned(grad_lse, 4)))
         return RFDETR_ERR_ALIGN;
     if (key_tokens > 0 && (!grad_key || !grad_value || !aligned(grad_key, 16) || !aligned(grad_value, 16)))
         return RFDETR_ERR_ALIGN;

@@ -248,12 +248,13 @@ set_losses.defvjp(_set_losses_fwd, _set_losses_bwd)
 def packed_attention(query, key, value, offsets, key_offsets, causal=False, scale=None):
     """Attention within the sequences of packed rows (the padded batches of ``layers.py:54-98``
     without their padding): ``(output [T, H, D], lse [H, T])``."""
-    out, _, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    out, _, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale, False)
     return out, lse
 
 
-def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale):
-    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype), jax.ShapeDtypeStruct(query.shape, query.dtype),
+def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale, keep_low):
+    low = query.shape if keep_low else (0, *query.shape[1:])  # what the output's rounding lost, for the gradient
+    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype), jax.ShapeDtypeStruct(low, query.dtype),
             jax.ShapeDtypeStruct((query.shape[1], query.shape[0]), jnp.float32))
     return jax.ffi.ffi_call("RfdetrPackedAttention", outs)(
         query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32),
@@ -261,7 +262,7 @@ def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scal
 
 
 def _packed_attention_fwd(query, key, value, offsets, key_offsets, causal, scale):
-    out, low, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale)
+    out, low, lse = _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale, True)
     return (out, lse), (query, key, value, offsets, key_offsets, out, low, lse)
 
 
@@ -269,8 +270,8 @@ def _packed_attention_bwd(causal, scale, residuals, g):
     query, key, value, offsets, key_offsets, out, low, lse = residuals
     shapes = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key, value))
     grads = jax.ffi.ffi_call("RfdetrPackedAttentionBwd", shapes)(
-        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, low, lse, g[0].astype(out.dtype),
-        g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
+        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, low, lse,
+        g[0].astype(out.dtype), g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
         scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
     return *grads, None, None
 

@@ -377,7 +377,7 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrSetLosses, SetLosses,
                                   .Ret<ffi::Buffer<ffi::F32>>());
 
 // Packed attention: (query [T, H, D], key, value [Tk, Hkv, D] bf16, offsets, key_offsets int32 [S + 1])
-// -> (output, output_low, lse [H, T]).
+// -> (output, output_low [T or 0 where no gradient is wanted, H, D], lse [H, T]).
 static ffi::Error PackedAttention(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query,
                                   ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
                                   ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets, int32_t causal,
@@ -397,8 +397,9 @@ static ffi::Error PackedAttention(cudaStream_t stream, ffi::ScratchAllocator scr
     return status_error(
         rfdetr_packed_attention(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
                                 value.untyped_data(), Hkv * D, D, offsets.typed_data(), key_offsets.typed_data(),
-                                output->untyped_data(), output_low->untyped_data(), lse->typed_data(), ws, bytes, S, T, Tk, H, Hkv, D, causal,
-                                scale),
+                                output->untyped_data(),
+                                output_low->element_count() ? output_low->untyped_data() : nullptr,
+                                lse->typed_data(), ws, bytes, S, T, Tk, H, Hkv, D, causal, scale),
         "RfdetrPackedAttention");
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrPackedAttention, PackedAttention,
@@ -422,8 +423,7 @@ static ffi::Error PackedAttentionBwd(cudaStream_t stream, ffi::ScratchAllocator 
                                      ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
                                      ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets,
                                      ffi::Buffer<ffi::BF16> output, ffi::Buffer<ffi::BF16> output_low,
-                                     ffi::Buffer<ffi::F32> lse,
-                                     ffi::Buffer<ffi::BF16> grad_output, ffi::Buffer<ffi::F32> grad_lse,
+                                     ffi::Buffer<ffi::F32> lse, ffi::Buffer<ffi::BF16> grad_output, ffi::Buffer<ffi::F32> grad_lse,
                                      int32_t causal, float scale, ffi::Result<ffi::Buffer<ffi::BF16>> grad_query,
                                      ffi::Result<ffi::Buffer<ffi::BF16>> grad_key,
                                      ffi::Result<ffi::Buffer<ffi::BF16>> grad_value) {
@@ -439,7 +439,8 @@ static ffi::Error PackedAttentionBwd(cudaStream_t stream, ffi::ScratchAllocator 
     return status_error(
         rfdetr_packed_attention_backward(
             stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D, value.untyped_data(), Hkv * D, D,
-            offsets.typed_data(), key_offsets.typed_data(), output.untyped_data(), output_low.untyped_data(), lse.typed_data(),
+            offsets.typed_data(), key_offsets.typed_data(), output.untyped_data(), output_low.untyped_data(),
+            lse.typed_data(),
             grad_output.untyped_data(), H * D, D, grad_lse.typed_data(), grad_query->untyped_data(),
             grad_key->untyped_data(), grad_value->untyped_data(), ws, bytes, dim(offsets, 0) - 1, T, Tk, H, Hkv, D,
             causal, scale),
