@@ -2027,9 +2027,14 @@ template <int DP> BackwardPlan plan_backward(const AttnArgs &A) {
     const long long n_seq = A.n_seq > 0 ? A.n_seq : 1;
     const long long rows = (A.Tq + n_seq - 1) / n_seq, keys = (A.Tk + n_seq - 1) / n_seq;  // of the mean sequence
     const int per = 128 / A.pack;
+    // While each has an SM of its own, down to four steps a block; with many steps, up to four an SM.  (us, tokens x
+    // heads of channels, alone and shared by so many for keys, queries: 300, 8 of 32: 26.8, 22.7 by 2, 2; 577, 6 of
+    // 64: 34.9, 28.8 by 2, 2; 1000 causal, 8 of 128: 41.2, 35.0 by 2, 2 and 55.5 by 4, 4; 2048, 8 of 32: 112.8, 70.2 by
+    // 4, 4; but 300, 8 of 128, four steps: 24.8, 26.7 by 2, 2; 4 x 577, 120 tiles: 37.0, 43.0 by 1, 2.)
     auto ranks = [&](long long blocks, long long steps) {
+        const long long sms = num_sms();
         int r = 1;
-        while (r < 4 && blocks * r < 2ll * num_sms() && steps >= 16 * r) r *= 2;
+        while (r < 4 && ((blocks * 2 * r <= sms && steps >= 8 * r) || (blocks * r < 2 * sms && steps >= 16 * r))) r *= 2;
         return r;
     };
     BackwardPlan p;
