@@ -372,8 +372,8 @@ int rfdetr_allreduce_sum_f32(void *stream, float *const *buffers, unsigned *cons
  *   output_low  as output, or NULL: what each result lost in its rounding to bf16, itself as bf16.  The backward
  *           call needs it (its output . grad_output is taken from both).
  * Query i of sequence s sees its keys j, with `causal` those with j <= i + Lk - Lq.  Head h reads
- * key head h / (n_heads / n_kv_heads).  A query that sees no key, and every row outside all
- * sequences, gets output 0 and lse -inf; such rows of query, key and value have gradient 0.
+ * key head h / (n_heads / n_kv_heads).  A query that sees no key (or whose float32 scores are all -inf),
+ * and every row outside all sequences, gets output 0 and lse -inf; such rows of query, key and value have gradient 0.
  * Scores, softmax statistics and sums are float32; the softmax weights (and, backward, dS) are
  * rounded to bf16 for the tensor cores.  A non-finite value reaches the outputs of its own sequence
  * only.  Bitwise reproducible.

@@ -133,8 +133,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     Returns:
         ``[tokens, heads, head_dim]`` bfloat16, differentiable with respect to query, key and value
-        (and through the log-sum-exp).  A query without any key, and rows outside all sequences,
-        give 0 (log-sum-exp ``-inf``) and gradient 0.
+        (and through the log-sum-exp).  A query without any key (or with all scores ``-inf``), and rows
+        outside all sequences, give 0 (log-sum-exp ``-inf``) and gradient 0.
     """
     N.same_device(query, key, value, offsets, key_offsets)
     query, key, value = _packed("query", query), _packed("key", key), _packed("value", value)

@@ -13,6 +13,7 @@
 // slot), which never overlap and always suffice, so no plan has to be made and no length has to be
 // known on the host.  The rows before the first and after the last sequence count as sequences
 // without keys: their outputs and gradients are zero.  Offsets are clamped to the tensors.
+// Scores are float32: a row whose scores are all -inf has no weights and is treated as one that sees no key.
 //
 // Queries of the heads that share a key head are rows of one tile (token-major, heads inner), so
 // K and V are read once for all of them and a few tokens still fill a tile.
@@ -1349,6 +1350,10 @@ struct BwdRows {
     float *delta;
 };
 
+// -log2(e) lse, for P = exp2(S' - lse').  A row whose scores are all -inf has lse -inf and, as forward, no weights:
+// -inf too, where its negation would make them NaN.
+__device__ __forceinline__ float neg_lse2(float lse) { return lse == -INFINITY ? -INFINITY : -lse * kLog2e; }
+
 // What a block walks.  DKV: `steps_per_sub` tiles of `tok` tokens from token `first` on, for each of
 // `subs` head groups.  DQ: tiles of 64 keys.
 struct BwdRange {
@@ -1416,7 +1421,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 float nl = 0.0f, nd = 0.0f, od = 0.0f;
                 if (c < good) {
                     const size_t x = (size_t)(head + row_head(A, c)) * A.Tq + base + at + row_token(A, c);
-                    nl = -f.lse[x] * kLog2e;
+                    nl = neg_lse2(f.lse[x]);
                     nd = -__ldcg(f.delta + x);
                     if (f.g_lse) od = f.g_lse[x];
                 }
@@ -1542,7 +1547,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         if (row_token(A, row) < r.qtok) {
             limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
             const size_t x = (size_t)(r.qhead + row_head(A, row)) * A.Tq + r.qbase + tok;
-            row_nl = -f.lse[x] * kLog2e;
+            row_nl = neg_lse2(f.lse[x]);
             if (f.g_lse) row_od = f.g_lse[x];
             row_nd = row_od - sh.row_dot[row];
             if (write_delta && group == 0) f.delta[x] = -row_nd;

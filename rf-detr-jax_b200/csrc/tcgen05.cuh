@@ -267,11 +267,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // (which takes 8 cycles of an SM quarter for a warp's exponentials, the other pipes idle).  x is
 // split into its nearest integer n and a rest f in [-1/2, 1/2]; 2^f is a polynomial of degree 5 fitted
 // by Lawson's reweighted least squares to the least relative error (2.4e-7 in float32 with the
-// rounding of its steps, as ex2.approx), and n is added to its exponent field.  Below 2^-126 the
-// result stays 2^-126; a NaN does not come out finite and small.
+// rounding of its steps, as ex2.approx).  2^n is made from n + 127 as its exponent field and multiplied:
+// x is held at -127 and more, where that field is 0 and 2^n with it, so that -inf gives 0, and NaN, which
+// the polynomial carries, stays NaN (adding n to the polynomial's own exponent field would turn it into a number).
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
     const float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
     const float2 t = add2(x, make_float2(kMagic, kMagic));
     const float2 n = add2(t, make_float2(-kMagic, -kMagic));
@@ -282,9 +283,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     p = fma2(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
     p = fma2(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
     p = fma2(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
-    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-    return p;
+    return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                               __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 // Two bf16 (round to nearest even) in one register, `lo` in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
