@@ -222,7 +222,7 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
     }
 }
 
-// Whole warp: moves the reference to the new maximum where some row's grew far enough, and O and the
+// Whole warp: moves the reference to the new maximum where some live row's grew far enough, and O and the
 // sum with it.
 template <int DP> __device__ __forceinline__ void move_reference(RowState &r, uint32_t to, float mx, bool first,
                                                                  float sc) {
@@ -247,14 +247,16 @@ template <int DP> __device__ __forceinline__ void move_reference(RowState &r, ui
 }
 
 // Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
-// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
+// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.  A row that is
+// not `live` holds whatever lies behind the tile's queries (another sequence's, or what shared memory held
+// before): its maximum counts as -inf, so that it moves no other row's reference, and with it no bits.
 // loaded() is called once S has been read, settle() before P is written or O touched (it returns
 // false to give up), written(half) after each half of P.
 // Tiles that are seen whole, the many, are read once into registers and run straight through; the
 // others go over S twice in a small loop.
 template <int DP, typename Loaded, typename Settle, typename Written>
 __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
-                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
+                                             int seen, bool live, bool first, float sc, Loaded loaded, Settle settle,
                                              Written written) {
     constexpr int KEYS = 128;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -265,7 +267,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
         tmem_wait_ld();
         pin<KEYS>(s);
         loaded();
-        const float mx = max_of<KEYS>(s);
+        const float mx = live ? max_of<KEYS>(s) : -INFINITY;
         if (!settle()) return false;
         move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
@@ -288,6 +290,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
+        mx = live ? mx : -INFINITY;
         if (!settle()) return false;
         move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
@@ -316,7 +319,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 // sequences they are many.
 template <int DP>
 __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_t to, int cols, bool all, int seen,
-                                               bool first, float sc) {
+                                               bool live, bool first, float sc) {
     float s[64];
     tmem_ld32(ts, s);
     if (cols > 32) tmem_ld32(ts + 32, s + 32);
@@ -330,7 +333,7 @@ __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    move_reference<DP>(r, to, live ? max_of<64>(s) : -INFINITY, first, sc);
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
@@ -896,8 +899,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 };
                 if (warp_live) {
                     ok = softmax_tile<DP>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
-                                                    k0 + S::kKeys <= all_see, limit - k0, i == 0, A.scale_log2, loaded,
-                                                    settle, written);
+                                          k0 + S::kKeys <= all_see, limit - k0, live, i == 0, A.scale_log2, loaded,
+                                          settle, written);
                 } else {
                     loaded();
                     ok = settle();
@@ -1144,8 +1147,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             }
             const int k0 = i * KEYS;
             if (warp_live)
-                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
-                                   A.scale_log2);
+                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, live,
+                                   i == 0, A.scale_log2);
             // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
             if (k0 + KEYS > it.klen) {
                 ok = wait_warp(&sh.v_full[t & 1], (t >> 1) & 1, abort) && ok;
