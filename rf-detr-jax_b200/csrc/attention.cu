@@ -101,7 +101,9 @@ __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *oth
 
 inline long long slots_for(long long T, long long R, long long n_seq) { return T / R + n_seq + 2; }
 
-// Polls of a wait before the block gives up.  Every wait here is for work of the same block.
+// Polls of a wait before the block gives up.  Every wait here is for work of the same block: where a kernel overlaps
+// the one before it, each warp passes wait_for_primary(), which is not counted, before it first polls for anything
+// that comes from there.
 constexpr int kAttnWaitLimit = 1 << 21;
 
 // A whole warp's wait: all of its lanes go on, or none (tensor memory is moved by warps).  Written to
@@ -1479,6 +1481,7 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
         return true;
     };
     if (!wait_warp(&sh.x_full, 0, abort)) return false;
+    if (DKV) wait_for_primary();  // y_full comes after it
     if (!scores(0)) return false;
     if (S::kPairs == 2 && steps > 1 && !scores(1)) return false;
 #pragma unroll 1
@@ -1558,6 +1561,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
     }
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
     const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
+    if (DKV) wait_for_primary();  // s_full comes after it
     // A warp without a live row leaves its rows of P and dS as they are: they reach no other row.
     const bool warp_live = DKV ? r.k0 + (row & ~31) < r.klen : (row & ~31) < r.qtok * A.pack;
 #pragma unroll 1
@@ -1742,7 +1746,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     const int per = DKV ? 128 : 128 / A.pack;
     const Slot x = DKV ? find_slot(A.k_off, A.q_off, A.n_seq, A.Tk, A.Tq, A.slot_rows, slot)
                        : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
-    // The dK/dV launch overlaps the dQ one's end: its loads wait for delta, and its first block at least, so that it
+    // The dK/dV launch overlaps the dQ one's end: its warps wait for delta, and its first block at least, so that it
     // does not end before the other.
     if (!DKV) launch_dependents();
     else if (blockIdx.x == 0) wait_for_primary();
