@@ -1748,8 +1748,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
                        : find_slot(A.q_off, A.k_off, A.n_seq, A.Tq, A.Tk, A.slot_rows, slot);
     // The dK/dV launch overlaps the dQ one's end: its warps wait for delta, and its first block at least, so that it
     // does not end before the other.
-    if (!DKV) launch_dependents();
-    else if (blockIdx.x == 0) wait_for_primary();
+    if (DKV && blockIdx.x == 0) wait_for_primary();
     if (x.first >= x.len) return;
     const int G = A.Hq / A.Hkv;
     BwdRange r;
@@ -1808,6 +1807,9 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    // Only now that this block has its TMEM: a dK/dV block holds its own until all of this launch has ended, so one
+    // let in before could keep a block of this launch waiting for the columns that it holds.
+    if (!DKV) launch_dependents();
 
     int issued = 0;
     const int row = threadIdx.x & 127;

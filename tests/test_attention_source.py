@@ -39,3 +39,11 @@ def test_bounded_waits_cover_this_block_only(name):
     # A lambda's polls count from its first call.
     calls = [m.start() for m in re.finditer(r"!scores\(", body)] or polls
     assert passed < min(calls)
+
+
+def test_no_dependent_before_tensor_memory():
+    """A dQ block lets dK/dV blocks in once it has its tensor memory: they hold theirs until its whole launch ends."""
+    body = _body("attn_backward_kernel")
+    alloc, lets_in = body.find("tmem_alloc("), body.find("launch_dependents()")
+    assert 0 <= alloc < body.find("__syncthreads()", alloc) < lets_in
+    assert body.count("launch_dependents()") == 1
