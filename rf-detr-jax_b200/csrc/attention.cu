@@ -1682,28 +1682,33 @@ __device__ __forceinline__ void store_acc(const AttnArgs &A, uint32_t acc, bool 
     }
 }
 
-// Whole block: this block's accumulator columns into its shared memory (column-major: a warp's rows
-// are consecutive), then the cluster's sums of this block's share of the columns to memory.
+// Compute warps: this block's accumulator columns into its shared memory (column-major: a warp's rows are
+// consecutive).
 template <int DP, bool DKV, int GROUPS>
-__device__ void share_acc(const AttnArgs &A, uint32_t acc, bool any, uint32_t smem, int ranks, int rank, size_t row_at,
-                          bool live, bf16 *g0, bf16 *g1) {
+__device__ __forceinline__ void stage_acc(uint32_t acc, bool any, uint32_t smem) {
     constexpr int kAll = DKV ? 2 * DP : DP;
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
-    if (w < GROUPS) {
 #pragma unroll 1
-        for (int c = w * 16; c < kAll; c += GROUPS * 16) {
-            float o[16];
-            if (any) {
-                tmem_ld16(acc + c, o);
-                tmem_wait_ld();
-                pin<16>(o);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + ((c + e) * 128 + row) * 4), "f"(any ? o[e] : 0.0f)
-                             : "memory");
+    for (int c = w * 16; c < kAll; c += GROUPS * 16) {
+        float o[16];
+        if (any) {
+            tmem_ld16(acc + c, o);
+            tmem_wait_ld();
+            pin<16>(o);
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + ((c + e) * 128 + row) * 4), "f"(any ? o[e] : 0.0f)
+                         : "memory");
     }
+}
+
+// Whole block: the cluster's sums of this block's share of the columns to memory.
+template <int DP, bool DKV, int GROUPS>
+__device__ __forceinline__ void share_acc(const AttnArgs &A, uint32_t smem, int ranks, int rank, size_t row_at,
+                                          bool live, bf16 *g0, bf16 *g1) {
+    constexpr int kAll = DKV ? 2 * DP : DP;
+    const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
     cluster_sync();
     const int cols = kAll / ranks;
     if (w < GROUPS) {
@@ -1832,7 +1837,7 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     if (ranks > 1) {
         // Every product of this block is done, so its shared memory is free.
         __syncthreads();
-        share_acc<DP, DKV, S::kCompute / 4>(A, acc, steps > 0, smem_x, ranks, rank, row_at, live, g0, g1);
+        if (warp < S::kCompute) stage_acc<DP, DKV, S::kCompute / 4>(acc, steps > 0, smem_x);
     }
     __syncwarp();
     tc_fence_before();
@@ -1850,6 +1855,12 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, S::kTmem);
+    }
+    // The block gives its TMEM back before it waits for the cluster's others: one of them may still be waiting for
+    // TMEM on its own SM, held there by a block that waits for one more.
+    if (ranks > 1) {
+        __syncwarp();
+        share_acc<DP, DKV, S::kCompute / 4>(A, smem_x, ranks, rank, row_at, live, g0, g1);
     }
 }
 
