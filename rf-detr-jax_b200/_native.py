@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "librfdetr_b200.so")
@@ -179,6 +180,15 @@ def same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
             device = -1
     if device < 0:
         require_cuda(first, *others)
+
+
+def has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether a tensor carries a forward-mode derivative, of which ``requires_grad`` says nothing.  A call that goes past
+    its autograd function would drop it in silence; the function refuses it."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t)[1] is not None:
+            return True
+    return False
 
 
 @functools.lru_cache(maxsize=256)

@@ -132,8 +132,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
             ascend within the tensors; otherwise the kernels clamp them.
 
     Returns:
-        ``[tokens, heads, head_dim]`` bfloat16, differentiable with respect to query, key and value
-        (and through the log-sum-exp).  A query without any key (or with all scores ``-inf``), and rows
+        ``[tokens, heads, head_dim]`` bfloat16, differentiable (in reverse mode) with respect to query, key and
+        value (and through the log-sum-exp).  A query without any key (or with all scores ``-inf``), and rows
         outside all sequences, give 0 (log-sum-exp ``-inf``) and gradient 0.
     """
     N.same_device(query, key, value, offsets, key_offsets)
@@ -163,7 +163,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         _check_offsets("offsets", offsets, tokens)
         if key_offsets is not None:
             _check_offsets("key_offsets", key_offsets, key_tokens)
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+    if ((torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
+            or N.has_tangent(query, key, value)):
         out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)
     else:
         out, lse, _ = attention_forward(query, key, value, offsets, key_offsets, bool(causal), scale, return_lse,

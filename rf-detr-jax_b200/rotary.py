@@ -77,8 +77,8 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         interleaved: pairs of channels ``(2i, 2i + 1)`` instead of ``(i, i + sum(sections))``.
 
     Returns:
-        ``(query, key)`` turned, contiguous, in their own type; differentiable with respect to
-        both (not to the positions or frequencies).
+        ``(query, key)`` turned, contiguous, in their own type; differentiable (in reverse mode) with
+        respect to both (not to the positions or frequencies).
     """
     N.same_device(query, key, positions, inv_freq)
     query = _rows("query", query)
@@ -108,6 +108,7 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     if interleaved and dim % 2:
         raise ValueError("interleaved pairs need an even head_dim")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+    if ((torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)))
+            or N.has_tangent(query, key, positions, inv_freq)):
         return AxialRotaryFunction.apply(query, key, positions, inv_freq, sections, bool(interleaved))
     return rotary_launch(query, key, positions, inv_freq, sections, bool(interleaved), False)
