@@ -22,8 +22,8 @@
 extern "C" {
 #endif
 
-/* Element types (int32 for rotary positions only). */
-enum rfdetr_dtype { RFDETR_F32 = 0, RFDETR_BF16 = 1, RFDETR_I32 = 2 };
+/* Element types (integers for rotary positions only). */
+enum rfdetr_dtype { RFDETR_F32 = 0, RFDETR_BF16 = 1, RFDETR_I32 = 2, RFDETR_I64 = 3 };
 
 /* Status codes. */
 enum rfdetr_status {
@@ -411,7 +411,7 @@ int rfdetr_packed_attention_backward(void *stream, const void *query, int64_t qu
  * -theta, which is the gradient.  Angles are reduced in float64.
  *   query [tokens, n_heads, head_dim], key [tokens, n_kv_heads, head_dim] (n_kv_heads may be 0): f32 or
  *   bf16, strides in elements, channels contiguous; outputs contiguous, not overlapping the inputs;
- *   positions [tokens, n_axes] f32 or int32 contiguous; inv_freq device f32; sections host int64.
+ *   positions [tokens, n_axes] f32, int32 or int64 contiguous; inv_freq device f32; sections host int64.
  * Limits: head_dim <= 1024, n_axes <= 8; interleaved pairs must be aligned to a pair.
  * No reference counterpart: the reference's backbone adds learned positions.
  * ------------------------------------------------------------------------------------- */

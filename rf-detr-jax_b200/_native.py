@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(HERE, "librfdetr_b200.so")
 
 F32 = 0
 BF16 = 1
-I32 = 2  # rotary positions
+I32 = 2  # I32, I64: rotary positions
+I64 = 3
 
 OK = 0
 ERR_SHAPE = 1

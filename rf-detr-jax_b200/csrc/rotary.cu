@@ -172,7 +172,8 @@ extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t quer
                                    void *key_out, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
                                    int64_t head_dim, int interleaved, int inverse) {
     using namespace rfdetr;
-    if (dtype_size(dtype) == 0 || (position_dtype != RFDETR_F32 && position_dtype != RFDETR_I32))
+    if (dtype_size(dtype) == 0 ||
+        (position_dtype != RFDETR_F32 && position_dtype != RFDETR_I32 && position_dtype != RFDETR_I64))
         return RFDETR_ERR_DTYPE;
     if (tokens < 0 || tokens > (1ll << 40) || n_heads < 0 || n_heads > 65536 || n_kv_heads < 0 || n_kv_heads > 65536 ||
         head_dim < 2 || head_dim > 1024 || n_axes < 1 || n_axes > kMaxAxes || !sections)
@@ -192,7 +193,7 @@ extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t quer
     const int size = dtype_size(dtype);
     if ((n_heads && (!query || !query_out || !aligned(query, size) || !aligned(query_out, size))) ||
         (n_kv_heads && (!key || !key_out || !aligned(key, size) || !aligned(key_out, size))) || !positions ||
-        !aligned(positions, 4) || !inv_freq || !aligned(inv_freq, 4))
+        !aligned(positions, position_dtype == RFDETR_I64 ? 8 : 4) || !inv_freq || !aligned(inv_freq, 4))
         return RFDETR_ERR_ALIGN;
     A.in[0] = query, A.in[1] = key, A.out[0] = query_out, A.out[1] = key_out;
     A.token[0] = query_token_stride, A.token[1] = key_token_stride;
@@ -224,8 +225,12 @@ extern "C" int rfdetr_axial_rotary(void *stream, const void *query, int64_t quer
     per = per > most ? most : per;
     A.per_block = (int)(per < 1 ? 1 : per);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool il = interleaved != 0, real = position_dtype == RFDETR_F32;
-    if (dtype == RFDETR_BF16)
-        return real ? dispatch_rotary<bf16, float>(A, il, vec, s) : dispatch_rotary<bf16, int32_t>(A, il, vec, s);
-    return real ? dispatch_rotary<float, float>(A, il, vec, s) : dispatch_rotary<float, int32_t>(A, il, vec, s);
+    const bool il = interleaved != 0;
+    auto with = [&](auto element) {
+        using T = decltype(element);
+        if (position_dtype == RFDETR_F32) return dispatch_rotary<T, float>(A, il, vec, s);
+        if (position_dtype == RFDETR_I32) return dispatch_rotary<T, int32_t>(A, il, vec, s);
+        return dispatch_rotary<T, int64_t>(A, il, vec, s);
+    };
+    return dtype == RFDETR_BF16 ? with(bf16{}) : with(float{});
 }

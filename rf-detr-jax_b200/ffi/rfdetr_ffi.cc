@@ -466,14 +466,16 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrPackedAttentionBwd, PackedAttentionBwd,
                                   .Ret<ffi::Buffer<ffi::BF16>>()
                                   .Ret<ffi::Buffer<ffi::BF16>>());
 
-// Rotary positions: (query [T, H, D], key [T, Hkv, D], positions [T, A] f32 or int32, inv_freq) ->
+// Rotary positions: (query [T, H, D], key [T, Hkv, D], positions [T, A] f32, int32 or int64, inv_freq) ->
 // (query, key) turned; `inverse` for the gradient.
 static ffi::Error AxialRotary(cudaStream_t stream, ffi::AnyBuffer query, ffi::AnyBuffer key, ffi::AnyBuffer positions,
                               ffi::Buffer<ffi::F32> inv_freq, ffi::Span<const int64_t> sections, int32_t interleaved,
                               int32_t inverse, ffi::Result<ffi::AnyBuffer> query_out,
                               ffi::Result<ffi::AnyBuffer> key_out) {
     const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Hkv = dim(key, 1);
-    const int pd = positions.element_type() == ffi::DataType::S32 ? RFDETR_I32 : dtype_code(positions.element_type());
+    const int pd = positions.element_type() == ffi::DataType::S32   ? RFDETR_I32
+                   : positions.element_type() == ffi::DataType::S64 ? RFDETR_I64
+                                                                    : dtype_code(positions.element_type());
     return status_error(
         rfdetr_axial_rotary(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
                             dtype_code(query.element_type()), positions.untyped_data(), pd, inv_freq.typed_data(),

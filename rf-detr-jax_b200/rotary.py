@@ -12,6 +12,9 @@ from torch.autograd.function import once_differentiable
 from . import _native as N
 
 
+_POSITION_CODES = {torch.float32: N.F32, torch.int32: N.I32, torch.int64: N.I64}
+
+
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
     strides = t.stride()
     if len(strides) != 3:
@@ -39,7 +42,7 @@ def rotary_launch(query, key, positions, inv_freq, sections, interleaved, invers
         key_out = key.new_empty(tokens, kv_heads, dim)
     status = N.lib().rfdetr_axial_rotary(
         N.stream_of(query), query.data_ptr(), *query.stride()[:2], N.ptr(key), *key_strides,
-        N.dtype_code(query.dtype), positions.data_ptr(), N.F32 if positions.dtype == torch.float32 else N.I32,
+        N.dtype_code(query.dtype), positions.data_ptr(), _POSITION_CODES[positions.dtype],
         inv_freq.data_ptr(), N.const_int64_array(sections), len(sections), out.data_ptr(), N.ptr(key_out), tokens, heads,
         kv_heads, dim, interleaved, inverse)
     if status:
@@ -70,7 +73,7 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
     Args:
         query, key: ``[tokens, heads, head_dim]`` and ``[tokens, kv_heads, head_dim]`` float32 or
             bfloat16 (views of a fused projection are read in place); ``key`` may be None.
-        positions: ``[tokens, axes]`` float32 or int32 (int64 is narrowed).
+        positions: ``[tokens, axes]`` float32, int32 or int64.
         inv_freq: ``[sum(sections)]`` float32, radians per unit of position.
         sections: frequencies per axis, in order; ``2 * sum(sections) <= head_dim`` and the channels
             beyond are copied.
@@ -95,10 +98,8 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"sections {sections} do not fit head_dim {dim}")
     if positions.shape != (tokens, len(sections)):
         raise ValueError(f"positions must be [{tokens}, {len(sections)}], got {list(positions.shape)}")
-    if positions.dtype == torch.int64:
-        positions = positions.to(torch.int32)
-    if positions.dtype != torch.float32 and positions.dtype != torch.int32:
-        raise ValueError(f"positions must be float32 or int32, got {positions.dtype}")
+    if positions.dtype not in _POSITION_CODES:
+        raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
     if inv_freq.shape != (half,) or inv_freq.dtype != torch.float32:
         raise ValueError(f"inv_freq must be float32 [{half}]")
     if positions.requires_grad or inv_freq.requires_grad:
