@@ -33,7 +33,9 @@ def _offsets(name: str, t: torch.Tensor) -> torch.Tensor:
     dtype = t.dtype
     if t.dim() != 1 or t.numel() < 1 or (dtype != torch.int32 and dtype != torch.int64):
         raise ValueError(f"{name} must be int32 [sequences + 1]")
-    return t if dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if dtype == torch.int64:  # clamped like any others, to the tensors by the kernels
+        return t.clamp(0, 0x7fffffff).to(torch.int32).contiguous()
+    return t.contiguous()
 
 
 def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
@@ -122,7 +124,7 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
             of a fused projection are read in place (channels contiguous, strides multiples of 8).
         key, value: ``[key_tokens, kv_heads, head_dim]``; head ``h`` reads key head
             ``h // (heads // kv_heads)``.
-        offsets: int32 ``[sequences + 1]`` on the device: sequence ``s`` is rows ``offsets[s]`` to
+        offsets: int32 (or int64) ``[sequences + 1]`` on the device: sequence ``s`` is rows ``offsets[s]`` to
             ``offsets[s + 1] - 1`` of ``query``.
         key_offsets: the same for ``key`` and ``value``; None where they are the queries' own tokens.
         causal: query ``i`` of ``Lq`` sees keys ``j <= i + Lk - Lq`` (the last query sees all).
@@ -152,6 +154,7 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 3.4028234663852886e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    given, given_keys = offsets, key_offsets
     offsets = _offsets("offsets", offsets)
     if key_offsets is not None:
         key_offsets = _offsets("key_offsets", key_offsets)
@@ -160,9 +163,9 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     elif key_tokens != tokens:
         raise ValueError("key_offsets is needed where keys and queries are not the same tokens")
     if check:
-        _check_offsets("offsets", offsets, tokens)
+        _check_offsets("offsets", given, tokens)
         if key_offsets is not None:
-            _check_offsets("key_offsets", key_offsets, key_tokens)
+            _check_offsets("key_offsets", given_keys, key_tokens)
     if ((torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
             or N.has_tangent(query, key, value)):
         out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)

@@ -252,12 +252,17 @@ def packed_attention(query, key, value, offsets, key_offsets, causal=False, scal
     return out, lse
 
 
+def _offsets(t):
+    """As int32, values past it clamped (the kernels clamp to the tensors)."""
+    return jnp.clip(t, 0, 0x7fffffff).astype(jnp.int32)
+
+
 def _packed_attention_call(query, key, value, offsets, key_offsets, causal, scale, keep_low):
     low = query.shape if keep_low else (0, *query.shape[1:])  # what the output's rounding lost, for the gradient
     outs = (jax.ShapeDtypeStruct(query.shape, query.dtype), jax.ShapeDtypeStruct(low, query.dtype),
             jax.ShapeDtypeStruct((query.shape[1], query.shape[0]), jnp.float32))
     return jax.ffi.ffi_call("RfdetrPackedAttention", outs)(
-        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32),
+        query, key, value, _offsets(offsets), _offsets(key_offsets),
         causal=np.int32(1 if causal else 0), scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
 
 
@@ -270,7 +275,7 @@ def _packed_attention_bwd(causal, scale, residuals, g):
     query, key, value, offsets, key_offsets, out, low, lse = residuals
     shapes = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key, value))
     grads = jax.ffi.ffi_call("RfdetrPackedAttentionBwd", shapes)(
-        query, key, value, offsets.astype(jnp.int32), key_offsets.astype(jnp.int32), out, low, lse,
+        query, key, value, _offsets(offsets), _offsets(key_offsets), out, low, lse,
         g[0].astype(out.dtype), g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
         scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale))
     return *grads, None, None

@@ -53,3 +53,20 @@ def test_addresses_of_wide_positions(pkg):
     call = lambda at: N.lib().rfdetr_axial_rotary(None, 16, 8, 4, None, 0, 0, N.F32, at, N.I64, 16, sections, 1, 16,  # noqa: E731
                                                   None, 1, 1, 0, 4, 0, 0)
     assert call(20) == N.ERR_ALIGN and call(18) == N.ERR_ALIGN
+
+
+def test_offsets_past_32_bits(pkg):
+    """They are clamped to the tensors like any others, and `check` sees them as they are."""
+    q, k, v = (torch.randn((100, 2, 32), device=DEV).to(torch.bfloat16) for _ in range(3))
+    near = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    far = lambda *x: torch.tensor(x, dtype=torch.int64, device=DEV)  # noqa: E731
+    want = pkg.packed_attention(q, k, v, near(0, 60, 100))
+    assert torch.equal(pkg.packed_attention(q, k, v, far(0, 60, 2 ** 32 + 70)), want)
+    assert torch.equal(pkg.packed_attention(q, k, v, far(-2 ** 32 + 7, 60, 2 ** 62)), want)
+    assert torch.equal(pkg.packed_attention(q, k, v, far(0, 60, 100), far(0, 60, 2 ** 33), check=False), want)
+    assert torch.equal(pkg.packed_attention(q, k, v, far(0, 60, 100), check=True), want)
+    for offsets in (far(0, 60, 2 ** 32 + 100), far(2 ** 32, 60, 100), far(-2 ** 32, 60, 100)):
+        with pytest.raises(ValueError, match="ascend"):
+            pkg.packed_attention(q, k, v, offsets, check=True)
+        with pytest.raises(ValueError, match="ascend"):
+            pkg.packed_attention(q, k, v, near(0, 60, 100), offsets, check=True)
