@@ -1,8 +1,10 @@
 // XLA FFI handlers binding librfdetr_b200.so into JAX: one handler per C entry point of
 // include/rfdetr_b200.h, so the kernels run inside jit and shard_map on XLA's own stream.
 //
-// NOT COMPILED IN THIS REPOSITORY: JAX/jaxlib (which ship the XLA FFI headers) are absent from
-// this image and from the GPU hosts.  Where jaxlib is installed, build with
+// NOT COMPILED AGAINST XLA IN THIS REPOSITORY: JAX/jaxlib (which ship the XLA FFI headers) are absent
+// from this image and from the GPU hosts.  The tests compile it against a stand-in for the header
+// (tests/ffi), hold each binding to its function's parameters and call the handlers of the packed
+// attention and of the rotary positions with buffers that do not fit.  Where jaxlib is installed, build with
 //
 //   g++ -O2 -std=c++17 -shared -fPIC -o librfdetr_ffi.so rfdetr_ffi.cc \
 //       -I"$(python -c 'import jax.ffi; print(jax.ffi.include_dir())')" -I../../include \
@@ -22,7 +24,9 @@
 //   the host inside the step.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "rfdetr_b200.h"
@@ -53,6 +57,14 @@ int64_t dim(const ffi::AnyBuffer &b, int i) { return b.dimensions()[i]; }
 template <ffi::DataType T>
 int64_t dim(const ffi::Buffer<T> &b, int i) {
     return b.dimensions()[i];
+}
+
+// Whether a buffer has these dimensions: an entry point reads and writes by the sizes that it is given, which come
+// from one buffer each.
+template <typename B>
+bool has_dims(const B &b, std::initializer_list<int64_t> want) {
+    const auto d = b.dimensions();
+    return d.size() == want.size() && std::equal(want.begin(), want.end(), d.begin());
 }
 
 }  // namespace
@@ -378,14 +390,27 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrSetLosses, SetLosses,
 
 // Packed attention: (query [T, H, D], key, value [Tk, Hkv, D] bf16, offsets, key_offsets int32 [S + 1])
 // -> (output, output_low [T or 0 where no gradient is wanted, H, D], lse [H, T]).
+static bool attention_inputs_fit(const ffi::Buffer<ffi::BF16> &query, const ffi::Buffer<ffi::BF16> &key,
+                                 const ffi::Buffer<ffi::BF16> &value, const ffi::Buffer<ffi::S32> &offsets,
+                                 const ffi::Buffer<ffi::S32> &key_offsets) {
+    return query.dimensions().size() == 3 && key.dimensions().size() == 3 && offsets.dimensions().size() == 1 &&
+           dim(offsets, 0) >= 1 && has_dims(key_offsets, {dim(offsets, 0)}) && dim(key, 2) == dim(query, 2) &&
+           has_dims(value, {dim(key, 0), dim(key, 1), dim(key, 2)});
+}
+
 static ffi::Error PackedAttention(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query,
                                   ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
                                   ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets, int32_t causal,
                                   float scale, ffi::Result<ffi::Buffer<ffi::BF16>> output,
                                   ffi::Result<ffi::Buffer<ffi::BF16>> output_low,
                                   ffi::Result<ffi::Buffer<ffi::F32>> lse) {
+    if (!attention_inputs_fit(query, key, value, offsets, key_offsets))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrPackedAttention");
     const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
     const int64_t S = dim(offsets, 0) - 1;
+    if (!has_dims(*output, {T, H, D}) || !(has_dims(*output_low, {T, H, D}) || has_dims(*output_low, {0, H, D})) ||
+        !has_dims(*lse, {H, T}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrPackedAttention");
     const size_t bytes = rfdetr_packed_attention_workspace_bytes(S, T, Tk, H, Hkv, D);
     void *ws = nullptr;
     if (bytes) {
@@ -427,7 +452,13 @@ static ffi::Error PackedAttentionBwd(cudaStream_t stream, ffi::ScratchAllocator 
                                      int32_t causal, float scale, ffi::Result<ffi::Buffer<ffi::BF16>> grad_query,
                                      ffi::Result<ffi::Buffer<ffi::BF16>> grad_key,
                                      ffi::Result<ffi::Buffer<ffi::BF16>> grad_value) {
+    if (!attention_inputs_fit(query, key, value, offsets, key_offsets))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrPackedAttentionBwd");
     const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
+    if (!has_dims(output, {T, H, D}) || !has_dims(output_low, {T, H, D}) || !has_dims(lse, {H, T}) ||
+        !has_dims(grad_output, {T, H, D}) || !has_dims(grad_lse, {H, T}) || !has_dims(*grad_query, {T, H, D}) ||
+        !has_dims(*grad_key, {Tk, Hkv, D}) || !has_dims(*grad_value, {Tk, Hkv, D}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrPackedAttentionBwd");
     const size_t bytes = rfdetr_packed_attention_backward_workspace_bytes(T, H);
     void *ws = nullptr;
     if (bytes) {
@@ -472,10 +503,22 @@ static ffi::Error AxialRotary(cudaStream_t stream, ffi::AnyBuffer query, ffi::An
                               ffi::Buffer<ffi::F32> inv_freq, ffi::Span<const int64_t> sections, int32_t interleaved,
                               int32_t inverse, ffi::Result<ffi::AnyBuffer> query_out,
                               ffi::Result<ffi::AnyBuffer> key_out) {
+    if (query.dimensions().size() != 3 || key.dimensions().size() != 3)
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrAxialRotary");
     const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Hkv = dim(key, 1);
+    int64_t half = 0;
+    for (const int64_t section : sections) half += section;
+    if (!has_dims(key, {T, Hkv, D}) || !has_dims(positions, {T, static_cast<int64_t>(sections.size())}) ||
+        !has_dims(inv_freq, {half}) || !has_dims(*query_out, {T, H, D}) || !has_dims(*key_out, {T, Hkv, D}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrAxialRotary");
+    if (key.element_type() != query.element_type() || query_out->element_type() != query.element_type() ||
+        key_out->element_type() != query.element_type())
+        return status_error(RFDETR_ERR_DTYPE, "RfdetrAxialRotary");
     const int pd = positions.element_type() == ffi::DataType::S32   ? RFDETR_I32
                    : positions.element_type() == ffi::DataType::S64 ? RFDETR_I64
-                                                                    : dtype_code(positions.element_type());
+                   : positions.element_type() == ffi::DataType::F32 ? RFDETR_F32
+                                                                    : -1;
+    if (pd < 0) return status_error(RFDETR_ERR_DTYPE, "RfdetrAxialRotary");
     return status_error(
         rfdetr_axial_rotary(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
                             dtype_code(query.element_type()), positions.untyped_data(), pd, inv_freq.typed_data(),
