@@ -1946,15 +1946,21 @@ ForwardPlan plan_forward(const AttnArgs &A) {
     ForwardPlan p{};
     // (us, the alternating halves against pairs of row tiles; tokens x heads of channels.)  One to an SM at most:
     // 300 tokens, 8 of 32: 9.3, 11.0; 4 x 577, 6 of 64: 12.5, 16.6; 1024 causal, 16 / 4 of 128: 16.6, 22.7; 4 x
-    // 300 over 2000 keys, 8 of 64: 20.7, 32.9; but 8 x 577, 6 of 64, 240 row tiles: 22.7, 18.6.  Up to two with a
-    // causal mask, if long (the longest begin first): 2048, 16 / 4 of 128: 28.8, 35.0; 4 x 1000, 8 of 64: 22.7,
-    // 22.2; 8 x 577: 20.7, 15.9; 3000, 16 / 4, 376 of them: 52.1, 49.1.  Up to one and a half where the keys
-    // are other tokens, which is how sequences of very different lengths come: 8 x 300 over 0 to 4000, 8 of 80:
-    // 37.1, 44.8; over 600 to 2400: 37.7, 41.2; but over 2000 each: 43.8, 36.5.  And where a pair's second
-    // would be empty: 128 x 1 over 2000, 16 / 4 of 128: 108.7, 117.6; 32 x 1 over 700, 8 of 64: 25.0, 28.2.
+    // 300 over 2000 keys, 8 of 64: 20.7, 32.9; but 8 x 577, 6 of 64, 240 row tiles: 22.7, 18.6.  With more, for
+    // long keys:
+    // * under a causal mask up to two an SM (the longest begin first): 2048, 16 / 4 of 128: 28.8, 35.0; 4 x 1000, 8 of
+    //   64: 22.7, 22.2; 8 x 577: 20.7, 15.9; 3000, 16 / 4, 376 of them: 52.1, 49.1;
+    // * up to one and a half where the keys are other tokens and there are several sequences.  Whether the keys' counts
+    //   differ the host does not know; where they do, halves take 0.8 of the time in the mean of 135 sizes (0.47 to
+    //   1.2; 8 x 300 over 0 to 4000, 8 of 80: 32.6, 57.1; over 700 to 3200: 28.9, 48.1), where they are equal 1.04
+    //   with up to 64 channels and 1.17 with more (45 sizes; 8 x 300 over 2000 each, 8 of 64: 35.7, 34.2; of 80:
+    //   38.9, 33.8).  A single sequence has one count, and pairs: 3000 over 2000, 8 of 80: 39.0, 33.7;
+    // * where a pair's second would be empty: 24 x 100 over 1000, 8 of 32: 23.1, 28.2; 128 x 1 over 2000, 16 / 4 of
+    //   128: 108.7, 117.6; 32 x 1 over 700, 8 of 64: 25.0, 28.2.
+    const bool unequal = A.Tq != A.Tk && n_seq > 1;  // as far as can be told
     p.alternate = tiles >= 2 && (row_tiles <= sms ||
                                  (tiles >= 8 && (single || (A.causal && row_tiles <= 2 * sms) ||
-                                                 (A.Tq != A.Tk && 2 * row_tiles <= 3 * sms))));
+                                                 (unequal && 2 * row_tiles <= 3 * sms))));
     // Shared out over the SMs, a block to each: one token over 30,000 keys, 32 / 8 of 128: 38.4, whole 220; 4 x 64
     // over 8000, 16 / 4: 39.3, 68.1; 4 x 1 over 2500, 8 of 64: 18.6, 22.7; but 16 x 1 over 4000, 16 / 4: 36.7,
     // 41.7; 1601, 6 of 64, 13 key tiles: 29.3, 18.6.
