@@ -1948,8 +1948,10 @@ ForwardPlan plan_forward(const AttnArgs &A) {
     // 300 tokens, 8 of 32: 9.3, 11.0; 4 x 577, 6 of 64: 12.5, 16.6; 1024 causal, 16 / 4 of 128: 16.6, 22.7; 4 x
     // 300 over 2000 keys, 8 of 64: 20.7, 32.9; but 8 x 577, 6 of 64, 240 row tiles: 22.7, 18.6.  With more, for
     // long keys:
-    // * under a causal mask up to two an SM (the longest begin first): 2048, 16 / 4 of 128: 28.8, 35.0; 4 x 1000, 8 of
-    //   64: 22.7, 22.2; 8 x 577: 20.7, 15.9; 3000, 16 / 4, 376 of them: 52.1, 49.1;
+    // * under a causal mask up to one and a half an SM (the longest begin first): 2 x 1601, 8 of 64: 19.7, 26.4; 1601,
+    //   16 / 4 of 128: 21.4, 28.0; 4 x 1024, 6 of 64: 18.9, 19.7; and with ten key tiles up to two: 2048, 16 / 4 of
+    //   128: 27.4, 34.1; 2 x 3000, 6 of 64: 32, 46.5; 2 x 1300, 12 of 64: 21.7, 23.6; but 4 x 1024, 8 of 64, 256 row
+    //   tiles of eight: 21.4, 19.6; 6 x 900, 6 of 64: 22.6, 19.6;
     // * up to one and a half where the keys are other tokens and there are several sequences.  Whether the keys' counts
     //   differ the host does not know; where they do, halves take 0.8 of the time in the mean of 135 sizes (0.47 to
     //   1.2; 8 x 300 over 0 to 4000, 8 of 80: 32.6, 57.1; over 700 to 3200: 28.9, 48.1), where they are equal 1.04
@@ -1959,8 +1961,8 @@ ForwardPlan plan_forward(const AttnArgs &A) {
     //   128: 108.7, 117.6; 32 x 1 over 700, 8 of 64: 25.0, 28.2.
     const bool unequal = A.Tq != A.Tk && n_seq > 1;  // as far as can be told
     p.alternate = tiles >= 2 && (row_tiles <= sms ||
-                                 (tiles >= 8 && (single || (A.causal && row_tiles <= 2 * sms) ||
-                                                 (unequal && 2 * row_tiles <= 3 * sms))));
+                                 (tiles >= 8 && (single || ((A.causal || unequal) && 2 * row_tiles <= 3 * sms))) ||
+                                 (tiles >= 10 && A.causal && row_tiles <= 2 * sms));
     // Shared out over the SMs, a block to each: one token over 30,000 keys, 32 / 8 of 128: 38.4, whole 220; 4 x 64
     // over 8000, 16 / 4: 39.3, 68.1; 4 x 1 over 2500, 8 of 64: 18.6, 22.7; but 16 x 1 over 4000, 16 / 4: 36.7,
     // 41.7; 1601, 6 of 64, 13 key tiles: 29.3, 18.6.

@@ -44,3 +44,11 @@ def test_other_tokens(pkg, tuning, lengths, keys, want):
     """192 row tiles.  The keys of a single sequence are of one count, whatever their number is next to the queries':
     no row tile's work is longer than another's."""
     assert _chosen(pkg, tuning, lengths, keys, 8, 80, False) == want
+
+
+@pytest.mark.parametrize("lengths,heads,want", [((1024,) * 4, 8, "pairs"), ((900,) * 6, 6, "pairs"),
+                                                ((1024,) * 4, 6, "halves"), ((1300,) * 2, 12, "halves"),
+                                                ((2048,) * 2, 8, "halves")])
+def test_causal(pkg, tuning, lengths, heads, want):
+    """More row tiles than SMs: halves pay up to one and a half an SM, and with ten key tiles up to two."""
+    assert _chosen(pkg, tuning, lengths, None, heads, 64, True) == want
