@@ -43,7 +43,15 @@ class DecoderLayer(nn.Module):
         self.norms = nn.ModuleList(nn.LayerNorm(hidden) for _ in range(3))
         # 8 frequencies to each of x and y: turns of up to 64 radians across the image.
         freq = 64.0 * 100.0 ** (-torch.arange(8) / 8)
-        self.register_buffer("inv_freq", torch.cat((freq, freq)).float())
+        self.register_buffer("inv_freq", torch.cat((freq, freq)), persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        """Conversions of the layer: the frequencies follow its device, not its type (in bf16 their turns
+        would be off by up to 0.011 radians across the image)."""
+        freq = self.inv_freq
+        super()._apply(fn, recurse)
+        self.inv_freq = freq.to(self.inv_freq.device)
+        return self
 
     def self_attention(self, queries, centers, group_offsets):
         """``queries [B, G * Q, C]`` with ``centers [B, G * Q, 2]`` in [0, 1]; every group a sequence."""
@@ -51,7 +59,7 @@ class DecoderLayer(nn.Module):
         qkv = self.qkv(queries).view(batch * count, 3 * self.heads, hidden // self.heads)
         q, k, v = qkv.split(self.heads, 1)
         # Frequencies 0 to 7 turn by x, 8 to 15 by y.
-        q, k = rf.axial_rotary(q, k, centers.reshape(batch * count, 2), self.inv_freq.float(), (8, 8))
+        q, k = rf.axial_rotary(q, k, centers.reshape(batch * count, 2), self.inv_freq, (8, 8))
         return self.out(rf.packed_attention(q, k, v, group_offsets).view(batch, count, hidden))
 
     def cross_attention(self, queries, boxes, memory, shape):
