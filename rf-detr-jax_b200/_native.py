@@ -153,10 +153,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle by device index, where torch has this function (it makes no promise of it).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t: torch.Tensor) -> int:
-    """The current torch stream of ``t``'s device, as a raw ``cudaStream_t`` (without the stream object that
-    ``torch.cuda.current_stream`` makes, 2.3 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    """The current torch stream of ``t``'s device, as a raw ``cudaStream_t`` (where possible without the stream object
+    that ``torch.cuda.current_stream`` makes, 2.3 us a call)."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
