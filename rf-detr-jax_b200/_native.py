@@ -192,6 +192,8 @@ def same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
 def has_tangent(*tensors: torch.Tensor | None) -> bool:
     """Whether a tensor carries a forward-mode derivative, of which ``requires_grad`` says nothing.  A call that goes past
     its autograd function would drop it in silence; the function refuses it."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open; without torch's own note of it each is asked
+        return False
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t)[1] is not None:
             return True
