@@ -17,7 +17,7 @@ Components (each a thin host wrapper over ``librfdetr_b200.so``, see ``include/r
 """
 
 from . import _native
-from ._native import check_device_status, set_tuning
+from ._native import check_device_faults, check_device_status, set_tuning
 from .attention import PackedAttentionFunction, packed_attention
 from .collective import PeerAllReduce
 from .matcher import CriterionConfig, build_cost_matrix, hungarian_match, match_stacked
@@ -37,6 +37,7 @@ __all__ = [
     "PackedAttentionFunction",
     "PeerAllReduce",
     "build_cost_matrix",
+    "check_device_faults",
     "check_device_status",
     "hungarian_match",
     "match_stacked",

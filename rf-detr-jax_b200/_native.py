@@ -127,6 +127,19 @@ def check_device_status(status: torch.Tensor, what: str = "device status") -> No
     check(int(status.reshape(-1)[0].item()), what)
 
 
+def check_device_faults(device: torch.device | str | int | None = None) -> None:
+    """Raises ``RuntimeError`` if a bounded device wait gave up since the last call, on any stream of ``device`` (the
+    current one by default), in a kernel that has ended: the outputs of that call are undefined.  Synchronises the
+    current stream.  Calls that launch such kernels (the sampler's backward, packed attention) do not read the word
+    themselves; a training loop may every so many steps."""
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream().cuda_stream
+        status = lib().rfdetr_take_device_fault(stream)
+    if status == ERR_LIMIT:
+        raise RuntimeError("a bounded device wait gave up: outputs since the last check may be undefined")
+    check(status, "rfdetr_take_device_fault")
+
+
 def status_text(status: int) -> str:
     return lib().rfdetr_status_string(status).decode()
 
