@@ -102,7 +102,7 @@ def axial_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch
         raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
     if inv_freq.shape != (half,) or inv_freq.dtype != torch.float32:
         raise ValueError(f"inv_freq must be float32 [{half}]")
-    if positions.requires_grad or inv_freq.requires_grad:
+    if torch.is_grad_enabled() and (positions.requires_grad or inv_freq.requires_grad):
         raise ValueError("positions and inv_freq have no gradient")
     if dim > 1024:
         raise ValueError(f"head_dim must be at most 1024, got {dim}")
