@@ -61,8 +61,10 @@ bool encode_tensor_map(CUtensorMap *map, CUtensorMapDataType dtype, int rank, co
     };
     CUresult r = call();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {
-        // A thread that has made no runtime call yet has no context: any binds the device's.
-        if (cudaFree(nullptr) != cudaSuccess) return false;
+        // A thread that has made no runtime call yet has no context.  Choosing its device binds the device's, and is
+        // allowed while any thread captures a graph (a call that allocates or frees would end the capture).
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return false;
         r = call();
     }
     return r == CUDA_SUCCESS;
