@@ -199,9 +199,12 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-// A row's softmax so far: P and sum are relative to exp2(m scale log2(e)).
+// A row's softmax so far: P and sum are relative to exp2(m scale log2(e)).  A tile's row that is no query of its
+// sequence holds whatever lies behind those (another sequence's, or what shared memory held before): it starts from
+// m = inf, where no score moves the reference, and so does not change how the other rows' weights round.
 struct RowState {
     float m, sum;
+    __device__ explicit RowState(bool live) : m(live ? -INFINITY : INFINITY), sum(0.0f) {}
 };
 
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
@@ -229,7 +232,7 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
 template <int DP> __device__ __forceinline__ void move_reference(RowState &r, uint32_t to, float mx, bool first,
                                                                  float sc) {
     if (first) {
-        r.m = mx;
+        r.m = fmaxf(r.m, mx);
     } else if (__any_sync(0xffffffffu, mx * sc > r.m * sc + kLazy)) {
         const float to_m = fmaxf(r.m, mx);
         const float f = to_m == -INFINITY ? 1.0f : exp2_fast((r.m - to_m) * sc);
@@ -249,16 +252,14 @@ template <int DP> __device__ __forceinline__ void move_reference(RowState &r, ui
 }
 
 // Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
-// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.  A row that is
-// not `live` holds whatever lies behind the tile's queries (another sequence's, or what shared memory held
-// before): its maximum counts as -inf, so that it moves no other row's reference, and with it no bits.
+// columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
 // loaded() is called once S has been read, settle() before P is written or O touched (it returns
 // false to give up), written(half) after each half of P.
 // Tiles that are seen whole, the many, are read once into registers and run straight through; the
 // others go over S twice in a small loop.
 template <int DP, typename Loaded, typename Settle, typename Written>
 __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
-                                             int seen, bool live, bool first, float sc, Loaded loaded, Settle settle,
+                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
                                              Written written) {
     constexpr int KEYS = 128;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -269,7 +270,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
         tmem_wait_ld();
         pin<KEYS>(s);
         loaded();
-        const float mx = live ? max_of<KEYS>(s) : -INFINITY;
+        const float mx = max_of<KEYS>(s);
         if (!settle()) return false;
         move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
@@ -292,7 +293,6 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
-        mx = live ? mx : -INFINITY;
         if (!settle()) return false;
         move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
@@ -321,7 +321,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 // sequences they are many.
 template <int DP>
 __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_t to, int cols, bool all, int seen,
-                                               bool live, bool first, float sc) {
+                                               bool first, float sc) {
     float s[64];
     tmem_ld32(ts, s);
     if (cols > 32) tmem_ld32(ts + 32, s + 32);
@@ -335,7 +335,7 @@ __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    move_reference<DP>(r, to, live ? max_of<64>(s) : -INFINITY, first, sc);
+    move_reference<DP>(r, to, max_of<64>(s), first, sc);
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
@@ -873,7 +873,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
             // Keys that every row of the tile sees (rows past the last token do not count).
             const int all_see = A.causal ? min(klen, tok_first + 1 + klen - q.len) : klen;
-            RowState rs{-INFINITY, 0.0f};
+            RowState rs(live);
             const int n = r.cnt[t];
             bool ok = true;
 #pragma unroll 1
@@ -901,8 +901,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 };
                 if (warp_live) {
                     ok = softmax_tile<DP>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
-                                          k0 + S::kKeys <= all_see, limit - k0, live, i == 0, A.scale_log2, loaded,
-                                          settle, written);
+                                          k0 + S::kKeys <= all_see, limit - k0, i == 0, A.scale_log2, loaded, settle,
+                                          written);
                 } else {
                     loaded();
                     ok = settle();
@@ -1130,7 +1130,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         const bool warp_live = it.any && (row & ~31) < it.ntok * A.pack;
         const int limit = A.causal ? min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)) : it.klen;
         const int all_see = A.causal ? min(it.klen, it.tok0 + 1 + it.klen - it.qlen) : it.klen;
-        RowState rs{-INFINITY, 0.0f};
+        RowState rs(live);
 #pragma unroll 1
         for (int i = 0; i < it.n; ++i) {
             const int t = g + i;
@@ -1149,8 +1149,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             }
             const int k0 = i * KEYS;
             if (warp_live)
-                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, live,
-                                   i == 0, A.scale_log2);
+                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
+                                   A.scale_log2);
             // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
             if (k0 + KEYS > it.klen) {
                 ok = wait_warp(&sh.v_full[t & 1], (t >> 1) & 1, abort) && ok;
