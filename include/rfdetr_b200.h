@@ -376,8 +376,10 @@ int rfdetr_allreduce_sum_f32(void *stream, float *const *buffers, unsigned *cons
  * and every row outside all sequences, gets output 0 and lse -inf; such rows of query, key and value have gradient 0.
  * Scores, softmax statistics and sums are float32; the softmax weights (and, backward, dS) are
  * rounded to bf16 for the tensor cores.  A non-finite value reaches the outputs of its own sequence
- * only.  Bitwise reproducible.
- * Limits: head_dim a multiple of 8 up to 128, n_heads a multiple of n_kv_heads, scale > 0.
+ * only.  Bitwise reproducible: equal calls give equal bits.  (How sums are split is chosen by the shapes of the whole
+ * call, unused rows included; the same sequence in a larger buffer may differ in its last bits.)
+ * Limits: head_dim a multiple of 8 up to 128, n_heads a multiple of n_kv_heads, scale > 0.  Offsets that do not ascend
+ * leave results undefined (within the tensors).
  * rfdetr_packed_attention needs a 16-byte aligned workspace of the size its query returns (0 unless
  * the keys are split over blocks); the backward call one of tokens * n_heads floats.  grad_lse may be NULL.
  * ------------------------------------------------------------------------------------- */

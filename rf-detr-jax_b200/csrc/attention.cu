@@ -435,7 +435,7 @@ __device__ __forceinline__ int tile_cols(int sees, int k0, int keys) { return mi
 // (setmaxnreg): a row of S is 128 values.
 // What bounds it is the chain of a row tile from S through the maximum, the exponentials and P to P V, of
 // which two tiles in flight hide about half: 10,052 causal tokens of six prompts, 16 / 4 heads of 128, take
-// 127 us, 990 TFLOP/s of the products that the mask leaves (60% of the measured peak), with the tensor pipe
+// 122 us, 1020 TFLOP/s of the products that the mask leaves (62% of the measured peak), with the tensor pipe
 // 50%, the special-function unit 45% and the issue slots 37% busy.  Four warpgroups, two to a row tile, took
 // 150 us: what each waits for is the other roles, not its own work.
 // Where the launch has no more row tiles than SMs, two to a block would leave SMs without one: a block has one, and
@@ -474,7 +474,7 @@ struct LongRange {
 
 // Shared-out keys.  The host does not know the lengths, so each block looks at all of them: a slot with w key
 // tiles gets ceil(w / c) blocks a head, with the smallest c that the launch's blocks allow.  Eight single tokens
-// over 1 to 16384 keys, 16 / 4 heads of 128, take 40.5 us, of them 3.5 until a block has its share, 26 for
+// over 1 to 16384 keys, 16 / 4 heads of 128, take 39.3 us, of them 3.5 until a block has its share, 26 for
 // its keys (5.9 TB/s all together), 7 for the join; with four blocks to each slot, whatever its length, 48.
 constexpr int kSharedSlots = 384;  // at most, so that a thread sees to each
 
