@@ -58,16 +58,17 @@ def listed():
         {"name": "normed_part_fwd", "op": "rotary", "train": False, "tokens": 20011, "heads": 7, "kv_heads": 1,
          "dim": 80, "rotary": 48, "axes": 3, "extent": 100, "interleaved": True, "type": "bf16"},
         # The gradients of a backbone of 12 layers of 384 channels and its decoder, each a tensor by
-        # itself, clipped in float32 into the optimizer's buffer.
+        # itself, clipped in float32 into the optimizer's buffer; the tensors stay from step to step.
         {"name": "clip_model", "op": "clip", "counts": "48x147456,24x589824,12x1536,133x384,226944,221184,"
-         "36x65536,6x524288,6x2048,90x256,3x23296,91", "type": "f32", "out": "f32", "flat": False, "limit": 0.1},
+         "36x65536,6x524288,6x2048,90x256,3x23296,91", "type": "f32", "out": "f32", "flat": False, "kept": True,
+         "limit": 0.1},
         # The same gradients in one flat buffer, as a data-parallel step reduces them, in bf16, clipped into
         # the float32 buffer that the optimizer reads.
         {"name": "clip_flat", "op": "clip", "counts": "27361627", "type": "bf16", "out": "f32", "flat": True,
-         "limit": 0.1},
+         "kept": False, "limit": 0.1},
         # One decoder layer's gradients, views of a flat buffer at odd places; the norm is below the limit.
         {"name": "clip_layer", "op": "clip", "counts": "196608,768,65536,256,16384,64,8192,32,65536,256,65536,256,"
-         "262144,1024,262144,256,6x256,91", "type": "bf16", "out": "bf16", "flat": True, "limit": 2.0},
+         "262144,1024,262144,256,6x256,91", "type": "bf16", "out": "bf16", "flat": True, "kept": False, "limit": 2.0},
     ]
 
 
@@ -126,7 +127,7 @@ def _draw_clip(rng):
     rng.shuffle(counts)
     kind, out = rng.choice([("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16")])
     return {"op": "clip", "counts": ",".join(map(str, counts)), "type": kind, "out": out, "flat": rng.random() < 0.5,
-            "limit": rng.choice([0.01, 0.1, 0.5, 2.0])}
+            "kept": rng.random() < 0.5, "limit": rng.choice([0.01, 0.1, 0.5, 2.0])}
 
 
 def _numbers(text):
@@ -218,6 +219,8 @@ def _prepare_clip(state, case, gen, normal):
     # The limit as a part of what the norm will be, about: sizes' mean square is (10^-4 - 10^-10) / (6 ln 10).
     expected = math.sqrt(sum(counts) * (1e-4 - 1e-10) / (6 * math.log(10.0)))
     state["max_norm"] = case["limit"] * expected
+    if own and case["kept"]:
+        state["clipper"] = _package().GradientClipper(state["gradients"], out=state["outs"])
 
 
 # ---- one pass --------------------------------------------------------------------------------
@@ -262,7 +265,10 @@ def _own_rotary(state):
 
 
 def _own_clip(state):
-    norm = _package().clip_gradients(state["gradients"], state["max_norm"], out=state["outs"])
+    if state["case"]["kept"]:
+        norm = state["clipper"].clip(state["max_norm"])
+    else:
+        norm = _package().clip_gradients(state["gradients"], state["max_norm"], out=state["outs"])
     return {"norm": norm, "out": state["out"]}
 
 
