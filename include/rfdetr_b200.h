@@ -423,6 +423,57 @@ int rfdetr_axial_rotary(void *stream, const void *query, int64_t query_token_str
                         int64_t n_axes, void *query_out, void *key_out, int64_t tokens, int64_t n_heads,
                         int64_t n_kv_heads, int64_t head_dim, int interleaved, int inverse);
 
+/* ---------------------------------------------------------------------------------------
+ * Norms of queries and keys for each head, with rotary positions on the result, in one pass.
+ *
+ * y = turn(x_c / sqrt(mean_c x_c^2 + eps) * weight_c), the turn, positions and limits those of rfdetr_axial_rotary
+ * (forward turn), the mean over all head_dim channels.  The weights [head_dim] are f32 or bf16 device arrays, shared
+ * by the heads of query and of key, or NULL for ones.  Sums are float32; results are rounded to `dtype` once.
+ * Where head_dim, strides and addresses are multiples of 16 bytes values are read in pieces of so many, else one by
+ * one.  n_kv_heads may be 0 (key is then not read).
+ * The backward call takes the forward's inputs and the outputs' cotangents (grad_*_out, strided as the inputs) and
+ * writes contiguous gradients of query and key and, where they are not NULL, of the weights, in the weights' types; for
+ * those it needs a workspace of the size its query returns, 4-byte aligned.  Bitwise reproducible.
+ * Limits: head_dim <= 256, eps >= 0.  No reference counterpart.
+ * ------------------------------------------------------------------------------------- */
+int rfdetr_normed_rotary(void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride,
+                         const void *key, int64_t key_token_stride, int64_t key_head_stride, int dtype,
+                         const void *query_weight, int query_weight_dtype, const void *key_weight,
+                         int key_weight_dtype, float eps, const void *positions, int position_dtype,
+                         const float *inv_freq, const int64_t *sections, int64_t n_axes, void *query_out,
+                         void *key_out, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                         int interleaved);
+size_t rfdetr_normed_rotary_backward_workspace_bytes(int64_t head_dim);
+int rfdetr_normed_rotary_backward(void *stream, const void *query, int64_t query_token_stride,
+                                  int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                  int64_t key_head_stride, const void *grad_query_out,
+                                  int64_t grad_query_token_stride, int64_t grad_query_head_stride,
+                                  const void *grad_key_out, int64_t grad_key_token_stride,
+                                  int64_t grad_key_head_stride, int dtype, const void *query_weight,
+                                  int query_weight_dtype, const void *key_weight, int key_weight_dtype, float eps,
+                                  const void *positions, int position_dtype, const float *inv_freq,
+                                  const int64_t *sections, int64_t n_axes, void *grad_query, void *grad_key,
+                                  void *grad_query_weight, void *grad_key_weight, void *workspace,
+                                  size_t workspace_bytes, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                  int64_t head_dim, int interleaved);
+
+/* ---------------------------------------------------------------------------------------
+ * The norm of all gradients together, and the gradients clipped to a limit of it.
+ *
+ * norm = sqrt(sum of g^2 over all values of all tensors); every output value is g, or where norm > max_norm
+ * g * (max_norm / norm) (a NaN norm makes every result NaN, an infinite one makes finite values 0).
+ *   gradients, outputs   host arrays of n_tensors device pointers; an output may be its gradient (same type), no
+ *                        tensors may share memory otherwise;  types: f32 or bf16 each;  counts: values of each (may be
+ *                        0), aligned to their type;  norm: device f32 scalar.
+ * The host arrays are read during the call alone.  Squares and sums are float64; bitwise reproducible.  Two
+ * launches for up to 1000 tensors.  The 8-byte aligned workspace is of the size its query returns.
+ * No reference counterpart among the calls above: it stands between the all-reduce and the optimizer of a train step.
+ * ------------------------------------------------------------------------------------- */
+size_t rfdetr_clip_gradients_workspace_bytes(int64_t n_tensors);
+int rfdetr_clip_gradients(void *stream, const void *const *gradients, const int32_t *gradient_types,
+                          void *const *outputs, const int32_t *output_types, const int64_t *counts,
+                          int64_t n_tensors, double max_norm, float *norm, void *workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,17 +13,21 @@ Components (each a thin host wrapper over ``librfdetr_b200.so``, see ``include/r
 * :mod:`.losses` -- IA-BCE or focal and matched-pair box losses of stacked layers, with gradients;
 * :mod:`.attention` -- softmax attention over packed sequences, forward + backward;
 * :mod:`.rotary` -- rotary positions with several axes on queries and keys;
+* :mod:`.normed_rotary` -- the same after a norm of every head, in one pass;
+* :mod:`.clip` -- the norm of all gradients together, and their clipping;
 * :mod:`.collective` -- the data-parallel gradient all-reduce over NVLink peer memory.
 """
 
 from . import _native
 from ._native import check_device_faults, check_device_status, set_tuning
 from .attention import PackedAttentionFunction, packed_attention
+from .clip import GradientClipper, clip_gradients
 from .collective import PeerAllReduce
 from .matcher import CriterionConfig, build_cost_matrix, hungarian_match, match_stacked
 from .ops import (MSDeformAttnFunction, MSDeformAttnPrologueFunction, ms_deform_attn, ms_deform_attn_core,
                   ms_deform_attn_core_rows, msda_prologue)
 from .losses import SetLossFunction, set_losses
+from .normed_rotary import NormedRotaryFunction, normed_axial_rotary
 from .postprocess import post_process
 from .rotary import AxialRotaryFunction, axial_rotary
 from .topk import select_rows, top_k, two_stage_topk
@@ -38,6 +42,10 @@ __all__ = [
     "PeerAllReduce",
     "build_cost_matrix",
     "check_device_faults",
+    "clip_gradients",
+    "GradientClipper",
+    "normed_axial_rotary",
+    "NormedRotaryFunction",
     "check_device_status",
     "hungarian_match",
     "match_stacked",

@@ -83,6 +83,14 @@ SIGNATURES = {
                                          [_vp] * 5 + [ctypes.c_size_t] + [_i64] * 6 + [_int, _f32]),
     "rfdetr_axial_rotary": (_int, [_vp] + [_vp, _i64, _i64] * 2 + [_int, _vp, _int, _vp, _c_int64_p, _i64, _vp, _vp] +
                             [_i64] * 4 + [_int, _int]),
+    "rfdetr_normed_rotary": (_int, [_vp] + [_vp, _i64, _i64] * 2 + [_int] + [_vp, _int] * 2 + [_f32, _vp, _int, _vp,
+                                    _c_int64_p, _i64, _vp, _vp] + [_i64] * 4 + [_int]),
+    "rfdetr_normed_rotary_backward_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "rfdetr_normed_rotary_backward": (_int, [_vp] + [_vp, _i64, _i64] * 4 + [_int] + [_vp, _int] * 2 +
+                                      [_f32, _vp, _int, _vp, _c_int64_p, _i64] + [_vp] * 5 + [ctypes.c_size_t] +
+                                      [_i64] * 4 + [_int]),
+    "rfdetr_clip_gradients_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "rfdetr_clip_gradients": (_int, [_vp] * 6 + [_i64, ctypes.c_double, _vp, _vp, ctypes.c_size_t]),
     "rfdetr_set_losses": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                                  _f32, ctypes.c_int32, _vp, _vp, _vp, _vp]),
 }
@@ -176,6 +184,18 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream(t.device).cuda_stream
     return _raw_stream(t.device.index)
+
+
+# The current device's index, where torch has this function.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def on_device(t: torch.Tensor, entry, *args):
+    """Calls an entry point with ``t``'s device current: a launch on a stream of another device fails."""
+    if _current_device() == t.get_device():
+        return entry(*args)
+    with torch.cuda.device(t.device):
+        return entry(*args)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

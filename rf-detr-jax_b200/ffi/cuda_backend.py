@@ -37,7 +37,8 @@ _lib = ctypes.cdll.LoadLibrary(os.environ.get("RFDETR_FFI_LIB", os.path.join(_HE
 
 HANDLERS = ("RfdetrMsdaFwd", "RfdetrMsdaBwd", "RfdetrMsdaBwdNoAlloc", "RfdetrMsdaPrologue", "RfdetrMsdaPrologueBwd",
             "RfdetrTopkSelect", "RfdetrSelectRows", "RfdetrMatchCost", "RfdetrLsapBatched", "RfdetrMatchStacked",
-            "RfdetrSetLosses", "RfdetrPackedAttention", "RfdetrPackedAttentionBwd", "RfdetrAxialRotary")
+            "RfdetrSetLosses", "RfdetrPackedAttention", "RfdetrPackedAttentionBwd", "RfdetrAxialRotary",
+            "RfdetrNormedRotary", "RfdetrNormedRotaryBwd", "RfdetrClipGradients")
 for _name in HANDLERS:
     jax.ffi.register_ffi_target(_name, jax.ffi.pycapsule(getattr(_lib, _name)), platform="CUDA")
 
@@ -306,3 +307,38 @@ def _axial_rotary_bwd(sections, interleaved, residuals, g):
 
 
 axial_rotary.defvjp(_axial_rotary_fwd, _axial_rotary_bwd)
+
+
+@functools.partial(jax.custom_vjp, nondiff_argnums=(6, 7, 8))
+def normed_axial_rotary(query, key, query_weight, key_weight, positions, inv_freq, sections, interleaved=False,
+                        eps=1e-6):
+    """Every head of queries and keys normed (root mean square, times a weight ``[head_dim]``) and turned by its
+    token's positions."""
+    outs = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key))
+    return jax.ffi.ffi_call("RfdetrNormedRotary", outs)(
+        query, key, query_weight, key_weight, positions, inv_freq.astype(jnp.float32),
+        sections=np.asarray(sections, np.int64), interleaved=np.int32(1 if interleaved else 0), eps=np.float32(eps))
+
+
+def _normed_axial_rotary_fwd(query, key, query_weight, key_weight, positions, inv_freq, sections, interleaved, eps):
+    out = normed_axial_rotary(query, key, query_weight, key_weight, positions, inv_freq, sections, interleaved, eps)
+    return out, (query, key, query_weight, key_weight, positions, inv_freq)
+
+
+def _normed_axial_rotary_bwd(sections, interleaved, eps, residuals, g):
+    outs = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in residuals[:4])
+    grads = jax.ffi.ffi_call("RfdetrNormedRotaryBwd", outs)(
+        *residuals[:5], residuals[5].astype(jnp.float32), *(x.astype(residuals[0].dtype) for x in g),
+        sections=np.asarray(sections, np.int64), interleaved=np.int32(1 if interleaved else 0), eps=np.float32(eps))
+    return *grads, None, None
+
+
+normed_axial_rotary.defvjp(_normed_axial_rotary_fwd, _normed_axial_rotary_bwd)
+
+
+# ---- clipping ----------------------------------------------------------------------------------
+def clip_gradients(flat, max_norm):
+    """The gradients of a step in one buffer ``[n]``, scaled to a norm of ``max_norm`` at most: ``(clipped, norm)``."""
+    outs = (jax.ShapeDtypeStruct(flat.shape, flat.dtype), jax.ShapeDtypeStruct((1,), jnp.float32))
+    clipped, norm = jax.ffi.ffi_call("RfdetrClipGradients", outs)(flat, max_norm=np.float32(max_norm))
+    return clipped, norm[0]

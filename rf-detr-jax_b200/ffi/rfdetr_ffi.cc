@@ -538,3 +538,153 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrAxialRotary, AxialRotary,
                                   .Attr<int32_t>("inverse")
                                   .Ret<ffi::AnyBuffer>()
                                   .Ret<ffi::AnyBuffer>());
+
+// Normed queries and keys with rotary positions: (query [T, H, D], key [T, Hkv, D], query_weight, key_weight [D] or [0]
+// for ones, positions [T, A] f32, int32 or int64, inv_freq) -> (query, key).
+static int position_code(ffi::DataType t) {
+    return t == ffi::DataType::S32 ? RFDETR_I32 : t == ffi::DataType::S64 ? RFDETR_I64 : t == ffi::DataType::F32 ? RFDETR_F32 : -1;
+}
+
+static int normed_rotary_fits(const ffi::AnyBuffer &query, const ffi::AnyBuffer &key, const ffi::AnyBuffer &query_weight,
+                              const ffi::AnyBuffer &key_weight, const ffi::AnyBuffer &positions,
+                              const ffi::Buffer<ffi::F32> &inv_freq, ffi::Span<const int64_t> sections) {
+    if (query.dimensions().size() != 3 || key.dimensions().size() != 3) return RFDETR_ERR_SHAPE;
+    const int64_t T = dim(query, 0), D = dim(query, 2);
+    int64_t half = 0;
+    for (const int64_t section : sections) half += section;
+    if (!has_dims(key, {T, dim(key, 1), D}) || !has_dims(positions, {T, static_cast<int64_t>(sections.size())}) ||
+        !has_dims(inv_freq, {half}) || !(has_dims(query_weight, {D}) || has_dims(query_weight, {0})) ||
+        !(has_dims(key_weight, {D}) || has_dims(key_weight, {0})))
+        return RFDETR_ERR_SHAPE;
+    if (key.element_type() != query.element_type() || position_code(positions.element_type()) < 0)
+        return RFDETR_ERR_DTYPE;
+    return RFDETR_OK;
+}
+
+static const void *weight_data(const ffi::AnyBuffer &w) { return dim(w, 0) ? w.untyped_data() : nullptr; }
+
+static ffi::Error NormedRotary(cudaStream_t stream, ffi::AnyBuffer query, ffi::AnyBuffer key,
+                               ffi::AnyBuffer query_weight, ffi::AnyBuffer key_weight, ffi::AnyBuffer positions,
+                               ffi::Buffer<ffi::F32> inv_freq, ffi::Span<const int64_t> sections, int32_t interleaved,
+                               float eps, ffi::Result<ffi::AnyBuffer> query_out, ffi::Result<ffi::AnyBuffer> key_out) {
+    if (int st = normed_rotary_fits(query, key, query_weight, key_weight, positions, inv_freq, sections))
+        return status_error(st, "RfdetrNormedRotary");
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Hkv = dim(key, 1);
+    if (!has_dims(*query_out, {T, H, D}) || !has_dims(*key_out, {T, Hkv, D}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrNormedRotary");
+    if (query_out->element_type() != query.element_type() || key_out->element_type() != query.element_type())
+        return status_error(RFDETR_ERR_DTYPE, "RfdetrNormedRotary");
+    return status_error(
+        rfdetr_normed_rotary(stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D,
+                             dtype_code(query.element_type()), weight_data(query_weight),
+                             dtype_code(query_weight.element_type()), weight_data(key_weight),
+                             dtype_code(key_weight.element_type()), eps, positions.untyped_data(),
+                             position_code(positions.element_type()), inv_freq.typed_data(), sections.begin(),
+                             static_cast<int64_t>(sections.size()), query_out->untyped_data(), key_out->untyped_data(),
+                             T, H, Hkv, D, interleaved),
+        "RfdetrNormedRotary");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrNormedRotary, NormedRotary,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<ffi::Span<const int64_t>>("sections")
+                                  .Attr<int32_t>("interleaved")
+                                  .Attr<float>("eps")
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// Its gradients: (query, key, query_weight, key_weight, positions, inv_freq, grad_query_out, grad_key_out) ->
+// (grad_query, grad_key, grad_query_weight, grad_key_weight).
+static ffi::Error NormedRotaryBwd(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::AnyBuffer query,
+                                  ffi::AnyBuffer key, ffi::AnyBuffer query_weight, ffi::AnyBuffer key_weight,
+                                  ffi::AnyBuffer positions, ffi::Buffer<ffi::F32> inv_freq,
+                                  ffi::AnyBuffer grad_query_out, ffi::AnyBuffer grad_key_out,
+                                  ffi::Span<const int64_t> sections, int32_t interleaved, float eps,
+                                  ffi::Result<ffi::AnyBuffer> grad_query, ffi::Result<ffi::AnyBuffer> grad_key,
+                                  ffi::Result<ffi::AnyBuffer> grad_query_weight,
+                                  ffi::Result<ffi::AnyBuffer> grad_key_weight) {
+    if (int st = normed_rotary_fits(query, key, query_weight, key_weight, positions, inv_freq, sections))
+        return status_error(st, "RfdetrNormedRotaryBwd");
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Hkv = dim(key, 1);
+    if (!has_dims(grad_query_out, {T, H, D}) || !has_dims(grad_key_out, {T, Hkv, D}) ||
+        !has_dims(*grad_query, {T, H, D}) || !has_dims(*grad_key, {T, Hkv, D}) ||
+        !has_dims(*grad_query_weight, {dim(query_weight, 0)}) || !has_dims(*grad_key_weight, {dim(key_weight, 0)}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrNormedRotaryBwd");
+    for (const ffi::DataType t : {grad_query_out.element_type(), grad_key_out.element_type(),
+                                  grad_query->element_type(), grad_key->element_type()})
+        if (t != query.element_type()) return status_error(RFDETR_ERR_DTYPE, "RfdetrNormedRotaryBwd");
+    if (grad_query_weight->element_type() != query_weight.element_type() ||
+        grad_key_weight->element_type() != key_weight.element_type())
+        return status_error(RFDETR_ERR_DTYPE, "RfdetrNormedRotaryBwd");
+    const size_t bytes = rfdetr_normed_rotary_backward_workspace_bytes(D);
+    void *ws = nullptr;
+    if (bytes) {
+        auto block = scratch.Allocate(bytes, 256);
+        if (!block.has_value())
+            return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrNormedRotaryBwd: workspace");
+        ws = *block;
+    }
+    return status_error(
+        rfdetr_normed_rotary_backward(
+            stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D, grad_query_out.untyped_data(),
+            H * D, D, grad_key_out.untyped_data(), Hkv * D, D, dtype_code(query.element_type()),
+            weight_data(query_weight), dtype_code(query_weight.element_type()), weight_data(key_weight),
+            dtype_code(key_weight.element_type()), eps, positions.untyped_data(),
+            position_code(positions.element_type()), inv_freq.typed_data(), sections.begin(),
+            static_cast<int64_t>(sections.size()), grad_query->untyped_data(), grad_key->untyped_data(),
+            dim(query_weight, 0) ? grad_query_weight->untyped_data() : nullptr,
+            dim(key_weight, 0) ? grad_key_weight->untyped_data() : nullptr, ws, bytes, T, H, Hkv, D, interleaved),
+        "RfdetrNormedRotaryBwd");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrNormedRotaryBwd, NormedRotaryBwd,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Attr<ffi::Span<const int64_t>>("sections")
+                                  .Attr<int32_t>("interleaved")
+                                  .Attr<float>("eps")
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// Gradients in one flat buffer, as the all-reduce leaves them, clipped: gradients [n] -> (clipped [n], norm [1]).
+static ffi::Error ClipGradients(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::AnyBuffer gradients,
+                                float max_norm, ffi::Result<ffi::AnyBuffer> clipped,
+                                ffi::Result<ffi::Buffer<ffi::F32>> norm) {
+    if (gradients.dimensions().size() != 1 || !has_dims(*clipped, {dim(gradients, 0)}) || !has_dims(*norm, {1}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrClipGradients");
+    const size_t bytes = rfdetr_clip_gradients_workspace_bytes(1);
+    auto block = scratch.Allocate(bytes, 256);
+    if (!block.has_value())
+        return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrClipGradients: workspace");
+    const void *in = gradients.untyped_data();
+    void *out = clipped->untyped_data();
+    const int32_t in_type = dtype_code(gradients.element_type()), out_type = dtype_code(clipped->element_type());
+    const int64_t count = dim(gradients, 0);
+    return status_error(rfdetr_clip_gradients(stream, &in, &in_type, &out, &out_type, &count, 1, max_norm,
+                                              norm->typed_data(), *block, bytes),
+                        "RfdetrClipGradients");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrClipGradients, ClipGradients,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Attr<float>("max_norm")
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
