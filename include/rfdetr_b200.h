@@ -404,6 +404,35 @@ int rfdetr_packed_attention_backward(void *stream, const void *query, int64_t qu
                                      int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int causal, float scale);
 
 /* ---------------------------------------------------------------------------------------
+ * The same attention with changed scores.
+ *
+ * score_cap > 0 (0: none): s -> score_cap tanh(s / score_cap), of the scaled product.  distance_slopes, device f32
+ * [n_heads] or NULL: then s -> s - distance_slopes[h] |i + Lk - Lq - j| (the last query is level with the last key).
+ * prefix, device int32 [n_sequences] or NULL, with `causal` alone: every query of sequence s sees the keys j <
+ * prefix[s] as well (values are clamped to the sequence).  lse is of the changed scores.  The slopes have no gradient.
+ * With neither the calls are those above, bit for bit.  Workspaces, limits and everything else are theirs too;
+ * score_cap lies in 2^-64 .. 2^64, and scale / score_cap is a normal float.  A capped score of an infinite product is
+ * +-score_cap.  Capped scores are off by 6.5e-7 of their value at most.
+ * ------------------------------------------------------------------------------------- */
+int rfdetr_packed_attention_scored(void *stream, const void *query, int64_t query_token_stride,
+                                   int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                   int64_t key_head_stride, const void *value, int64_t value_token_stride,
+                                   int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
+                                   void *output, void *output_low, float *lse, void *workspace, size_t workspace_bytes,
+                                   int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
+                                   int64_t n_kv_heads, int64_t head_dim, int causal, float scale, float score_cap,
+                                   const float *distance_slopes, const int32_t *prefix);
+int rfdetr_packed_attention_scored_backward(
+    void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride, const void *key,
+    int64_t key_token_stride, int64_t key_head_stride, const void *value, int64_t value_token_stride,
+    int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets, const void *output,
+    const void *output_low, const float *lse, const void *grad_output, int64_t grad_token_stride,
+    int64_t grad_head_stride, const float *grad_lse, void *grad_query, void *grad_key, void *grad_value,
+    void *workspace, size_t workspace_bytes, int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
+    int64_t n_kv_heads, int64_t head_dim, int causal, float scale, float score_cap, const float *distance_slopes,
+    const int32_t *prefix);
+
+/* ---------------------------------------------------------------------------------------
  * Rotary positions with several axes (time, height, width) on queries and keys, one launch.
  *
  * Frequency i of sum(sections) belongs to axis a(i), the sections being consecutive, and turns a

@@ -20,7 +20,7 @@ Components (each a thin host wrapper over ``librfdetr_b200.so``, see ``include/r
 
 from . import _native
 from ._native import check_device_faults, check_device_status, set_tuning
-from .attention import PackedAttentionFunction, packed_attention
+from .attention import PackedAttentionFunction, ScoredAttentionFunction, packed_attention
 from .clip import GradientClipper, clip_gradients
 from .collective import PeerAllReduce
 from .matcher import CriterionConfig, build_cost_matrix, hungarian_match, match_stacked
@@ -39,6 +39,7 @@ __all__ = [
     "MSDeformAttnFunction",
     "packed_attention",
     "PackedAttentionFunction",
+    "ScoredAttentionFunction",
     "PeerAllReduce",
     "build_cost_matrix",
     "check_device_faults",

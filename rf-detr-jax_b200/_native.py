@@ -81,6 +81,11 @@ SIGNATURES = {
     "rfdetr_packed_attention_backward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "rfdetr_packed_attention_backward": (_int, [_vp] + [_vp, _i64, _i64] * 3 + [_vp] * 5 + [_vp, _i64, _i64] +
                                          [_vp] * 5 + [ctypes.c_size_t] + [_i64] * 6 + [_int, _f32]),
+    "rfdetr_packed_attention_scored": (_int, [_vp] + [_vp, _i64, _i64] * 3 + [_vp] * 6 + [ctypes.c_size_t] +
+                                       [_i64] * 6 + [_int, _f32, _f32, _vp, _vp]),
+    "rfdetr_packed_attention_scored_backward": (_int, [_vp] + [_vp, _i64, _i64] * 3 + [_vp] * 5 + [_vp, _i64, _i64] +
+                                                [_vp] * 5 + [ctypes.c_size_t] + [_i64] * 6 +
+                                                [_int, _f32, _f32, _vp, _vp]),
     "rfdetr_axial_rotary": (_int, [_vp] + [_vp, _i64, _i64] * 2 + [_int, _vp, _int, _vp, _c_int64_p, _i64, _vp, _vp] +
                             [_i64] * 4 + [_int, _int]),
     "rfdetr_normed_rotary": (_int, [_vp] + [_vp, _i64, _i64] * 2 + [_int] + [_vp, _int] * 2 + [_f32, _vp, _int, _vp,

@@ -45,7 +45,8 @@ def _check_offsets(name: str, t: torch.Tensor, total: int) -> None:
         raise ValueError(f"{name} must ascend within [0, {total}]")
 
 
-def attention_forward(query, key, value, offsets, key_offsets, causal, scale, want_lse, want_low):
+def attention_forward(query, key, value, offsets, key_offsets, causal, scale, want_lse, want_low, cap=0.0, slopes=None,
+                      prefix=None):
     """One forward call; inputs already checked.  Returns ``(output, lse or None, low or None)``, low being
     what the output lost in its rounding to bf16 (the backward pass reads it)."""
     tokens, heads, dim = query.shape
@@ -57,17 +58,18 @@ def attention_forward(query, key, value, offsets, key_offsets, causal, scale, wa
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
     workspace = query.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-    status = lib.rfdetr_packed_attention(
-        N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+    status = N.on_device(
+        query, lib.rfdetr_packed_attention_scored, N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
         out.data_ptr(), N.ptr(low), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads,
-        kv_heads, dim, causal, scale)
+        kv_heads, dim, causal, scale, cap, N.ptr(slopes), N.ptr(prefix))
     if status:
         N.check(status, "rfdetr_packed_attention")
     return out, lse, low
 
 
-def attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, low, lse, grad_output, grad_lse):
+def attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, low, lse, grad_output, grad_lse,
+                       cap=0.0, slopes=None, prefix=None):
     """One backward call; returns ``(grad_query, grad_key, grad_value)``, contiguous."""
     tokens, heads, dim = query.shape
     key_tokens, kv_heads, _ = key.shape
@@ -78,12 +80,13 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
     lib = N.lib()
     ws_bytes = lib.rfdetr_packed_attention_backward_workspace_bytes(tokens, heads)
     workspace = query.new_empty(max(1, ws_bytes), dtype=torch.uint8)
-    status = lib.rfdetr_packed_attention_backward(
-        N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+    status = N.on_device(
+        query, lib.rfdetr_packed_attention_scored_backward, N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
         out.data_ptr(), N.ptr(low), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
         N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
-        offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale)
+        offsets.numel() - 1, tokens, key_tokens, heads, kv_heads, dim, int(causal), scale, cap, N.ptr(slopes),
+        N.ptr(prefix))
     if status:
         N.check(status, "rfdetr_packed_attention_backward")
     return grads
@@ -114,9 +117,57 @@ class PackedAttentionFunction(torch.autograd.Function):
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
 
+class ScoredAttentionFunction(torch.autograd.Function):
+    """The same with changed scores."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, offsets, key_offsets, causal, scale, cap, slopes, prefix):
+        out, lse, low = attention_forward(query, key, value, offsets, key_offsets, causal, scale, True, True, cap,
+                                          slopes, prefix)
+        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, low, lse, slopes, prefix)
+        ctx.how = (causal, scale, cap)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output, grad_lse):
+        query, key, value, offsets, key_offsets, out, low, lse, slopes, prefix = ctx.saved_tensors
+        if grad_output is None and grad_lse is None:
+            return (None,) * 10
+        if grad_output is None:
+            grad_output = torch.zeros_like(out)
+        causal, scale, cap = ctx.how
+        grads = attention_backward(query, key, value, offsets, key_offsets, causal, scale, out, low, lse, grad_output,
+                                   grad_lse, cap, slopes, prefix)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *(None,) * 7)
+
+
+def _score_change(score_cap, distance_slopes, prefix, heads, sequences, causal, scale):
+    """Checked ``(cap, slopes, prefix)``; cap 0 for none."""
+    cap = 0.0 if score_cap is None else float(score_cap)
+    if score_cap is not None and not (2.0 ** -64 <= cap <= 2.0 ** 64 and 2.0 ** -126 <= scale / cap < 2.0 ** 128):
+        raise ValueError(f"score_cap must be positive (2^-64 to 2^64, scale / score_cap a float32), got {score_cap}")
+    if distance_slopes is not None:
+        if distance_slopes.shape != (heads,) or distance_slopes.dtype != torch.float32:
+            raise ValueError(f"distance_slopes must be float32 [{heads}], got {distance_slopes.dtype} "
+                             f"{list(distance_slopes.shape)}")
+        if torch.is_grad_enabled() and distance_slopes.requires_grad:
+            raise ValueError("distance_slopes have no gradient")
+        distance_slopes = distance_slopes.contiguous()
+    if prefix is not None:
+        if not causal:
+            raise ValueError("prefix needs causal: without it every query sees all keys")
+        if prefix.shape != (sequences,) or prefix.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"prefix must be int32 [{sequences}], got {prefix.dtype} {list(prefix.shape)}")
+        prefix = _offsets("prefix", prefix) if sequences else None
+    return cap, distance_slopes, prefix
+
+
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: torch.Tensor,
                      key_offsets: torch.Tensor | None = None, *, causal: bool = False, scale: float | None = None,
-                     return_lse: bool = False, check: bool = False):
+                     return_lse: bool = False, check: bool = False, score_cap: float | None = None,
+                     distance_slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None):
     """``softmax(scale * q k^T) v`` within each sequence of packed tensors.
 
     Args:
@@ -132,6 +183,11 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         return_lse: also return the scores' log-sum-exp ``[heads, tokens]`` float32.
         check: read the offsets on the host (synchronises) and raise ``ValueError`` unless they
             ascend within the tensors; otherwise the kernels clamp them.
+        score_cap: scores ``s`` become ``score_cap * tanh(s / score_cap)``.
+        distance_slopes: ``[heads]`` float32 on the device: from the (capped) score of query ``i`` and key ``j``
+            ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.
+        prefix: int32 (or int64) ``[sequences]`` on the device, with ``causal``: every query of sequence ``s`` also sees
+            its first ``prefix[s]`` keys (clamped to the sequence).
 
     Returns:
         ``[tokens, heads, head_dim]`` bfloat16, differentiable (in reverse mode) with respect to query, key and
@@ -166,7 +222,17 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         _check_offsets("offsets", given, tokens)
         if key_offsets is not None:
             _check_offsets("key_offsets", given_keys, key_tokens)
-    if ((torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
+    if score_cap is not None or distance_slopes is not None or prefix is not None:
+        N.same_device(query, distance_slopes, prefix)
+        change = _score_change(score_cap, distance_slopes, prefix, heads, offsets.numel() - 1, causal, scale)
+        if ((torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
+                or N.has_tangent(query, key, value, distance_slopes)):
+            out, lse = ScoredAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale,
+                                                     *change)
+        else:
+            out, lse, _ = attention_forward(query, key, value, offsets, key_offsets, bool(causal), scale, return_lse,
+                                            False, *change)
+    elif ((torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
             or N.has_tangent(query, key, value)):
         out, lse = PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, bool(causal), scale)
     else:

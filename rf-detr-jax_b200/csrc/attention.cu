@@ -15,6 +15,10 @@
 // without keys: their outputs and gradients are zero.  Offsets are clamped to the tensors.
 // Scores are float32: a row whose scores are all -inf has no weights and is treated as one that sees no key.
 //
+// Scores may be changed on the way: capped, S' = cap tanh(S / cap); lowered by distance, S'' = S' - slope_h |i + Lk -
+// Lq - j|; and under a causal mask a sequence may have a prefix of keys, j < prefix_s, that all of its queries see.  The
+// backward pass then has dS_ij = P_ij (dP_ij - delta_i) (1 - (S'_ij / cap)^2).
+//
 // Queries of the heads that share a key head are rows of one tile (token-major, heads inner), so
 // K and V are read once for all of them and a few tokens still fill a tile.
 #include <cfloat>
@@ -39,7 +43,24 @@ struct AttnArgs {
     float scale, scale_log2;
     Divisor slot_rows;  // rows (of the tensor that the launch tiles) in a slot
     Divisor heads;      // key heads x head groups: blocks or row tiles to a slot
+    // Of changed scores (kBiased, kCapped) alone.
+    float unit;             // scale log2(e)
+    float cap_in, cap_out;  // scale / cap, cap log2(e)
+    float cap_inv;          // 1 / cap_out
+    float cap_poly[4];      // cap_out times the polynomial's coefficients
+    const float *slopes;    // [Hq] or null
+    const int32_t *prefix;  // [n_seq] or null
 };
+
+// What a launch does to its scores, a template argument of the kernels: only scales them; lowers them by distance or
+// sees a prefix; caps them as well.
+constexpr int kPlain = 0, kBiased = 1, kCapped = 2;
+
+// Keys that every query of sequence `seq` (of klen keys) sees; seq is negative outside all sequences.
+template <int MOD> __device__ __forceinline__ int prefix_of(const AttnArgs &A, int seq, int klen) {
+    if constexpr (MOD == kPlain) return 0;
+    return A.causal && A.prefix && seq >= 0 ? min(max(__ldg(A.prefix + seq), 0), klen) : 0;
+}
 
 // A tile row's token within the tile and its head among the packed ones.
 __device__ __forceinline__ int row_token(const AttnArgs &A, int row) { return (row * A.pack_inv) >> 16; }
@@ -63,6 +84,7 @@ struct Slot {
     int first;  // first row of the slot within the sequence
     int base, len;  // the sequence's first row in the packed tensor, and its rows
     int other_base, other_len;  // the same of the tensor on the other side (none outside all sequences)
+    int seq;  // the sequence; -1 outside all
 };
 
 // Whole warp.  Extended sequence x: rows off_at(x) .. off_at(x + 1), x = 0 and n_seq + 1 being the
@@ -92,6 +114,7 @@ __device__ __forceinline__ Slot find_slot(const int32_t *off, const int32_t *oth
             const bool real = lo >= 1 && lo <= n_seq;
             r.other_base = real ? a : 0;
             r.other_len = real ? max(0, b - a) : 0;
+            r.seq = real ? lo - 1 : -1;
             return r;
         }
         lo += p * step;
@@ -199,6 +222,99 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+// ---- changed scores ----
+// tanh on the FMA pipe: x (1 + u Q(u)), u = x^2, for |x| up to kCapReach, Q fitted to the least largest relative error
+// (6.5e-7: with scores around 20, 1.3e-5 of them, a hundredth of what rounding P to bf16 loses).  Scores beyond that,
+// which a cap keeps rare, take 1 - 2 / (1 + e^2x) in a loop over the tile in TMEM, small and away from the straight
+// code; which of the two a score takes depends on that score alone.
+constexpr float kCapReach = 0.75f;
+constexpr float kCapPoly[4] = {-0.33329668641090393f, 0.13268236815929413f, -0.0502779483795166f, 0.013105831108987331f};
+
+template <int N> __device__ __forceinline__ bool beyond_reach(const AttnArgs &A, const float *s) {
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < N; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = fmaxf(fmaxf(a[e], fabsf(s[c + e])), fabsf(s[c + e + 4]));
+    }
+    const float most = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
+    return __any_sync(0xffffffffu, __fmul_rn(most, A.cap_in) > kCapReach);
+}
+
+// N products to capped scores in units of log2, all within reach.
+template <int N> __device__ __forceinline__ void cap_near(const AttnArgs &A, float *s) {
+    const float2 in = make_float2(A.cap_in, A.cap_in), one = make_float2(A.cap_out, A.cap_out);
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+        const float2 x = mul2(make_float2(s[c], s[c + 1]), in), u = mul2(x, x);
+        float2 w = fma2(make_float2(A.cap_poly[3], A.cap_poly[3]), u, make_float2(A.cap_poly[2], A.cap_poly[2]));
+        w = fma2(w, u, make_float2(A.cap_poly[1], A.cap_poly[1]));
+        w = fma2(w, u, make_float2(A.cap_poly[0], A.cap_poly[0]));
+        const float2 y = mul2(x, fma2(w, u, one));
+        s[c] = y.x;
+        s[c + 1] = y.y;
+    }
+}
+
+// Whole warp: n columns of products at TMEM `ts` to capped scores, whatever their size.
+__device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n) {
+#pragma unroll 1
+    for (int c = 0; c < n; c += 16) {
+        float s[16];
+        tmem_ld16(ts + c, s);
+        tmem_wait_ld();
+        pin<16>(s);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float x = __fmul_rn(s[e], A.cap_in), u = __fmul_rn(x, x);
+            float w = fmaf(A.cap_poly[3], u, A.cap_poly[2]);
+            w = fmaf(w, u, A.cap_poly[1]);
+            w = fmaf(w, u, A.cap_poly[0]);
+            const float near = __fmul_rn(x, fmaf(w, u, A.cap_out));
+            float r;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * (2.0f * kLog2e))));
+            s[e] = fabsf(x) <= kCapReach ? near : fmaf(-2.0f * A.cap_out, r, A.cap_out);
+        }
+        tmem_st16(ts + c, reinterpret_cast<uint32_t *>(s));
+    }
+    tmem_wait_st();
+}
+
+// A row's scores: N products of keys k0 .. at TMEM `ts`, read into s already, become scores in units of log2.
+template <int MOD> struct RowScores {
+    float slope = 0.0f;  // in units of log2
+    int level = 0;       // the key at distance 0
+    __device__ RowScores() {}
+    __device__ RowScores(const AttnArgs &A, int head, int at, bool live) {
+        if constexpr (MOD != kPlain) {
+            level = at;
+            if (A.slopes && live) slope = __ldg(A.slopes + head) * kLog2e;
+        }
+    }
+    template <int N> __device__ __forceinline__ void change(const AttnArgs &A, float *s, uint32_t ts, int k0) const {
+        if constexpr (MOD == kPlain) return;
+        if constexpr (MOD == kCapped) {
+            if (beyond_reach<N>(A, s)) {
+                cap_tmem(A, ts, N);
+#pragma unroll
+                for (int c = 0; c < N; c += 32) tmem_ld32(ts + c, s + c);
+                tmem_wait_ld();
+                pin<N>(s);
+            } else {
+                cap_near<N>(A, s);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c) s[c] *= A.unit;
+        }
+        if (A.slopes) {
+            const float d = (float)(k0 - level);
+#pragma unroll
+            for (int c = 0; c < N; ++c) s[c] = fmaf(-slope, fabsf(d + (float)c), s[c]);
+        }
+    }
+};
+
 // A row's softmax so far: P and sum are relative to exp2(m scale log2(e)).  A tile's row that is no query of its
 // sequence holds whatever lies behind those (another sequence's, or what shared memory held before): it starts from
 // m = inf, where no score moves the reference, and so does not change how the other rows' weights round.
@@ -210,12 +326,13 @@ struct RowState {
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
 // the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
 // with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
-template <int N, bool POLY>
+template <int N, bool POLY, int MOD>
 __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
     const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
 #pragma unroll
     for (int c = 0; c < N / 2; ++c) {
-        float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), sc2, ref2);
+        float2 x = MOD == kPlain ? fma2(make_float2(s[2 * c], s[2 * c + 1]), sc2, ref2)
+                                 : add2(make_float2(s[2 * c], s[2 * c + 1]), ref2);
         if (POLY && (c % 8 == 4)) {
             x = exp2_poly(x);
         } else {
@@ -257,11 +374,12 @@ template <int DP> __device__ __forceinline__ void move_reference(RowState &r, ui
 // false to give up), written(half) after each half of P.
 // Tiles that are seen whole, the many, are read once into registers and run straight through; the
 // others go over S twice in a small loop.
-template <int DP, typename Loaded, typename Settle, typename Written>
-__device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all,
-                                             int seen, bool first, float sc, Loaded loaded, Settle settle,
-                                             Written written) {
+template <int DP, int MOD, typename Loaded, typename Settle, typename Written>
+__device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<MOD> &scores, int k0, RowState &r,
+                                             uint32_t ts, uint32_t tp, uint32_t to, int cols, bool all, int seen,
+                                             bool first, Loaded loaded, Settle settle, Written written) {
     constexpr int KEYS = 128;
+    const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     if (all) {
         float s[KEYS];
@@ -269,6 +387,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
         for (int c = 0; c < KEYS; c += 32) tmem_ld32(ts + c, s + c);
         tmem_wait_ld();
         pin<KEYS>(s);
+        scores.template change<KEYS>(A, s, ts, k0);
         loaded();
         const float mx = max_of<KEYS>(s);
         if (!settle()) return false;
@@ -277,7 +396,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t p[KEYS / 4];
-            exp_pack<KEYS / 2, true>(s + h * (KEYS / 2), sc, ref, p, acc);
+            exp_pack<KEYS / 2, true, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
             tmem_st32(tp + h * 32, p);
             tmem_wait_st();
             written(h);
@@ -290,9 +409,14 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
             tmem_ld32(ts + c, s);
             tmem_wait_ld();
             pin<32>(s);
+            if constexpr (MOD != kPlain) {
+                scores.template change<32>(A, s, ts + c, k0 + c);
+                tmem_st32(ts + c, reinterpret_cast<uint32_t *>(s));
+            }
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
+        if constexpr (MOD != kPlain) tmem_wait_st();
         if (!settle()) return false;
         move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
@@ -305,7 +429,7 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[e] = c + e < seen ? s[e] : -INFINITY;
             uint32_t p[16];
-            exp_pack<32, false>(s, sc, ref, p, acc);
+            exp_pack<32, false, MOD>(s, sc, ref, p, acc);
             tmem_st16(tp + c / 2, p);
         }
         tmem_wait_st();
@@ -319,14 +443,16 @@ __device__ __forceinline__ bool softmax_tile(RowState &r, uint32_t ts, uint32_t 
 
 // The same for one warpgroup's tile of 64 keys, P over S.  Masked tiles run straight through too: in short
 // sequences they are many.
-template <int DP>
-__device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_t to, int cols, bool all, int seen,
-                                               bool first, float sc) {
+template <int DP, int MOD>
+__device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScores<MOD> &scores, int k0, RowState &r,
+                                               uint32_t ts, uint32_t to, int cols, bool all, int seen, bool first) {
+    const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
     float s[64];
     tmem_ld32(ts, s);
     if (cols > 32) tmem_ld32(ts + 32, s + 32);
     tmem_wait_ld();
     pin<64>(s);
+    scores.template change<64>(A, s, ts, k0);  // (columns past `cols` hold anything, and are masked)
     if (!all) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -340,13 +466,13 @@ __device__ __forceinline__ void softmax_tile64(RowState &r, uint32_t ts, uint32_
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
     if (all) {
-        exp_pack<64, false>(s, sc, ref, p, acc);
+        exp_pack<64, false, MOD>(s, sc, ref, p, acc);
         tmem_st32(ts, p);
     } else {
-        exp_pack<32, false>(s, sc, ref, p, acc);
+        exp_pack<32, false, MOD>(s, sc, ref, p, acc);
         tmem_st16(ts, p);
         if (cols > 32) {
-            exp_pack<32, false>(s + 32, sc, ref, p + 16, acc);
+            exp_pack<32, false, MOD>(s + 32, sc, ref, p + 16, acc);
             tmem_st16(ts + 16, p + 16);
         }
     }
@@ -501,11 +627,12 @@ __device__ __forceinline__ Slot shared_slot(const AttnArgs &A, const SharedOut &
     const bool real = lo >= 1 && lo <= A.n_seq;
     r.other_base = real ? so.other[lo] : 0;
     r.other_len = real ? max(0, so.other[lo + 1] - r.other_base) : 0;
+    r.seq = real ? lo - 1 : -1;
     return r;
 }
 
 // All threads of a block (two barriers).
-__device__ __forceinline__ void count_tiles(const AttnArgs &A, SharedOut &so, int slots) {
+template <int MOD> __device__ __forceinline__ void count_tiles(const AttnArgs &A, SharedOut &so, int slots) {
 #pragma unroll 1
     for (int x = threadIdx.x; x < A.n_seq + 3; x += blockDim.x) {
         so.off[x] = off_at(A.q_off, A.n_seq, A.Tq, x);
@@ -516,7 +643,9 @@ __device__ __forceinline__ void count_tiles(const AttnArgs &A, SharedOut &so, in
     for (int x = threadIdx.x; x < slots; x += blockDim.x) {
         const Slot q = shared_slot(A, so, x);
         const int end = min(q.len, q.first + A.slot_rows.d);
-        const int sees = A.causal ? min(q.other_len, max(0, end + q.other_len - q.len)) : q.other_len;
+        const int sees = A.causal ? max(min(q.other_len, max(0, end + q.other_len - q.len)),
+                                        prefix_of<MOD>(A, q.seq, q.other_len))
+                                  : q.other_len;
         so.tiles[x] = q.first >= q.len ? 0 : max(1, (sees + 127) / 128);
     }
     __syncthreads();
@@ -753,7 +882,7 @@ __device__ bool long_mma_loop(LongShared &sh, uint32_t smem_q, uint32_t smem_kv,
 // The two halves of an ALT block's warpgroups.
 __device__ __forceinline__ void half_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int DP, bool ALT, bool SPLIT>
+template <int DP, bool ALT, bool SPLIT, int MOD>
 __global__ void __launch_bounds__(LongShape<DP, ALT>::kThreads, 1)
 attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -795,7 +924,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
         launch_dependents();
         start();
         tc_fence_before();
-        count_tiles(A, so, slots);
+        count_tiles<MOD>(A, so, slots);
         tc_fence_after();
         share = find_share(A, so, slots, share_size(A, so, slots, S::kLeast, gridDim.x), blockIdx.x);
         if (share.slot < 0) {
@@ -816,6 +945,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
     const int kbase = q.other_base, klen = q.other_len;
     const int kvh = hx / A.subs;
     const int qhead = kvh * (A.Hq / A.Hkv) + (hx % A.subs) * A.pack;
+    const int prefix = prefix_of<MOD>(A, q.seq, klen);
 
     LongRange r;
     int n[2];  // key tiles of each row tile
@@ -824,7 +954,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
         const int first = q.first + (ALT ? 0 : t * per);
         r.tok[t] = min(per, max(0, q.len - first));
         const int last = first + r.tok[t] - 1;
-        r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? min(klen, max(0, last + 1 + klen - q.len)) : klen;
+        r.sees[t] = r.tok[t] == 0 ? 0 : A.causal ? max(min(klen, max(0, last + 1 + klen - q.len)), prefix) : klen;
         n[t] = (r.sees[t] + S::kKeys - 1) / S::kKeys;
     }
     r.j0 = 0;
@@ -870,9 +1000,10 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const int tok_first = q.first + (ALT ? 0 : t * per), tok = tok_first + row_token(A, row);
             const bool live = row_token(A, row) < r.tok[t];
             const bool warp_live = (row & ~31) < r.tok[t] * A.pack;
-            const int limit = A.causal ? min(klen, max(0, tok + 1 + klen - q.len)) : klen;
+            const int limit = A.causal ? max(min(klen, max(0, tok + 1 + klen - q.len)), prefix) : klen;
             // Keys that every row of the tile sees (rows past the last token do not count).
-            const int all_see = A.causal ? min(klen, tok_first + 1 + klen - q.len) : klen;
+            const int all_see = A.causal ? max(min(klen, tok_first + 1 + klen - q.len), prefix) : klen;
+            const RowScores<MOD> scores(A, qhead + row_head(A, row), tok + klen - q.len, live);
             RowState rs(live);
             const int n = r.cnt[t];
             bool ok = true;
@@ -900,9 +1031,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                     mbar_arrive_one(&sh.p_half[t][h]);
                 };
                 if (warp_live) {
-                    ok = softmax_tile<DP>(rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
-                                          k0 + S::kKeys <= all_see, limit - k0, i == 0, A.scale_log2, loaded, settle,
-                                          written);
+                    ok = softmax_tile<DP, MOD>(A, scores, k0, rs, ts, tp, to, tile_cols(r.sees[t], k0, S::kKeys),
+                                               k0 + S::kKeys <= all_see, limit - k0, i == 0, loaded, settle, written);
                 } else {
                     loaded();
                     ok = settle();
@@ -1007,10 +1137,11 @@ struct ShortItem {
     int ntok, qlen;
     int kvh, krow, klen;
     int sees, n;             // keys that the tile works on, key tiles
+    int prefix;              // keys that every query sees, whatever the mask
     bool any;                // a row tile at all
 };
 
-__device__ __forceinline__ ShortItem short_item(const AttnArgs &A, int slots, int idx, int per) {
+template <int MOD> __device__ __forceinline__ ShortItem short_item(const AttnArgs &A, int slots, int idx, int per) {
     ShortItem t;
     const int s = quotient(idx, A.heads), hx = idx - s * A.heads.d;
     // Later slots first: under a causal mask they see more keys.
@@ -1024,12 +1155,13 @@ __device__ __forceinline__ ShortItem short_item(const AttnArgs &A, int slots, in
     t.qlen = q.len;
     t.krow = q.other_base;
     t.klen = q.other_len;
-    t.sees = A.causal ? min(t.klen, max(0, q.first + t.ntok + t.klen - q.len)) : t.klen;
+    t.prefix = prefix_of<MOD>(A, q.seq, t.klen);
+    t.sees = A.causal ? max(min(t.klen, max(0, q.first + t.ntok + t.klen - q.len)), t.prefix) : t.klen;
     t.n = t.any ? (t.sees + ShortShape<32>::kKeys - 1) / ShortShape<32>::kKeys : 0;
     return t;
 }
 
-template <int DP>
+template <int DP, int MOD>
 __global__ void __launch_bounds__(128, ShortShape<DP>::kBlocks)
 attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mq,
                           const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -1062,7 +1194,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         tmem_alloc(&sh.tmem, S::kTmem);
     }
     int idx = blockIdx.x;
-    ShortItem it = short_item(A, slots, idx, per);
+    ShortItem it = short_item<MOD>(A, slots, idx, per);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1125,11 +1257,13 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         ShortItem next;
         next.any = false;
         next.n = 0;
-        if (idx < items) next = short_item(A, slots, idx, per);
+        if (idx < items) next = short_item<MOD>(A, slots, idx, per);
         const bool live = it.any && row_tok < it.ntok;
         const bool warp_live = it.any && (row & ~31) < it.ntok * A.pack;
-        const int limit = A.causal ? min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)) : it.klen;
-        const int all_see = A.causal ? min(it.klen, it.tok0 + 1 + it.klen - it.qlen) : it.klen;
+        const int limit =
+            A.causal ? max(min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)), it.prefix) : it.klen;
+        const int all_see = A.causal ? max(min(it.klen, it.tok0 + 1 + it.klen - it.qlen), it.prefix) : it.klen;
+        const RowScores<MOD> row_scores(A, it.qhead + row_head(A, row), it.tok0 + row_tok + it.klen - it.qlen, live);
         RowState rs(live);
 #pragma unroll 1
         for (int i = 0; i < it.n; ++i) {
@@ -1149,8 +1283,8 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             }
             const int k0 = i * KEYS;
             if (warp_live)
-                softmax_tile64<DP>(rs, ts, to, tile_cols(it.sees, k0, KEYS), k0 + KEYS <= all_see, limit - k0, i == 0,
-                                   A.scale_log2);
+                softmax_tile64<DP, MOD>(A, row_scores, k0, rs, ts, to, tile_cols(it.sees, k0, KEYS),
+                                        k0 + KEYS <= all_see, limit - k0, i == 0);
             // Rows of V that are not this sequence's (P is 0 there, but 0 x inf is not).
             if (k0 + KEYS > it.klen) {
                 ok = wait_warp(&sh.v_full[t & 1], (t >> 1) & 1, abort) && ok;
@@ -1219,10 +1353,11 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
 // were shared out; eight channels per thread.  A part that saw no keys has lse -inf, weight 0 and wrote zeros.
 // Blocks look up their parts while the last of them are still in work, and read four parts at a time (weights
 // relative to the largest lse so far).
+template <int MOD>
 __global__ void __launch_bounds__(128)
 attn_join_kernel(const AttnArgs A, const FwdOut f, int slots, int least, int blocks) {
     __shared__ SharedOut so;
-    count_tiles(A, so, slots);
+    count_tiles<MOD>(A, so, slots);
     const unsigned size = share_size(A, so, slots, least, blocks);
     const int slot = quotient(blockIdx.x, A.heads), hx = blockIdx.x - slot * A.heads.d;
     const int parts = (so.tiles[slot] + size - 1) / size;
@@ -1340,6 +1475,9 @@ struct BwdShared {
     alignas(16) float neg_lse2[4][64];
     alignas(16) float neg_delta[4][64];
     alignas(16) float one_ds[4][64];
+    // Of changed scores: the row's slope in units of log2, and the key it is level with, from the held tile's first on.
+    alignas(16) float slope2[4][64];
+    alignas(16) float level[4][64];
     float row_dot[128];  // dQ: o.g of the held rows
 };
 
@@ -1370,10 +1508,11 @@ struct BwdRange {
     int k0;         // DKV: first key of the held tile
     int q0, qtok;   // DQ: first token and tokens of the held tile
     int kvh, qhead; // key head; DQ: first query head of the tile (DKV: of the key head)
+    int prefix;     // keys that every query sees, whatever the mask
 };
 
 // Whole warp; returns how many steps were asked for.
-template <int DP, bool DKV>
+template <int DP, bool DKV, int MOD>
 __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtensorMap *mx1, const CUtensorMap *my0,
                         const CUtensorMap *my1, BwdShared &sh, uint32_t smem_x, uint32_t smem_y, const BwdRange &r,
                         const BwdRows &f) {
@@ -1433,6 +1572,12 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 sh.neg_lse2[st][c] = nl;
                 sh.neg_delta[st][c] = nd;
                 sh.one_ds[st][c] = od;
+                if constexpr (MOD != kPlain) {
+                    if (A.slopes) {
+                        sh.slope2[st][c] = c < good ? __ldg(A.slopes + head + row_head(A, c)) * kLog2e : 0.0f;
+                        sh.level[st][c] = (float)(at + row_token(A, c) + r.klen - r.qlen - r.k0);
+                    }
+                }
             }
             __syncwarp();
         }
@@ -1507,7 +1652,7 @@ __device__ bool bwd_mma_loop(BwdShared &sh, uint32_t smem_x, uint32_t smem_y, in
 }
 
 // The kHalves warpgroups w: the steps i with i % kPairs == w, 32 columns each.
-template <int DP, bool DKV>
+template <int DP, bool DKV, int MOD>
 __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, uint32_t tmem, const BwdRows &f,
                           bool write_delta) {
     using S = BwdShape<DP>;
@@ -1551,7 +1696,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         }
         asm volatile("bar.sync 1, %0;" ::"n"(S::kCompute * 32) : "memory");
         if (row_token(A, row) < r.qtok) {
-            limit = A.causal ? min(r.klen, max(0, tok + 1 + shift)) : r.klen;
+            limit = A.causal ? max(min(r.klen, max(0, tok + 1 + shift)), r.prefix) : r.klen;
             const size_t x = (size_t)(r.qhead + row_head(A, row)) * A.Tq + r.qbase + tok;
             row_nl = neg_lse2(f.lse[x]);
             if (f.g_lse) row_od = f.g_lse[x];
@@ -1559,8 +1704,10 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             if (write_delta && group == 0) f.delta[x] = -row_nd;
         }
     }
+    const RowScores<MOD> scores(A, DKV ? 0 : r.qhead + row_head(A, row), DKV ? 0 : tok + shift,
+                                !DKV && row_token(A, row) < r.qtok);
     // DQ: keys that every row of the tile sees, and whether some row sees a single one.
-    const int all_see = A.causal ? min(r.klen, r.q0 + 1 + shift) : r.klen;
+    const int all_see = A.causal ? max(min(r.klen, r.q0 + 1 + shift), r.prefix) : r.klen;
     if (DKV) wait_for_primary();  // s_full comes after it
     // A warp without a live row leaves its rows of P and dS as they are: they reach no other row.
     const bool warp_live = DKV ? r.k0 + (row & ~31) < r.klen : (row & ~31) < r.qtok * A.pack;
@@ -1580,13 +1727,16 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         if (DKV) {
             const int at = r.first + ((r.start + i) % r.steps_per_sub) * r.tok;
             const int good = min(r.tok, r.qlen - at) * A.pack;
-            mask = good < kWalk || r.k0 + 128 > r.klen || (A.causal && at + shift < r.k0 + 127);
+            mask = good < kWalk || r.k0 + 128 > r.klen ||
+                   (A.causal && at + shift < r.k0 + 127 && r.prefix < r.k0 + 128);
             if (mask) {
                 hi = key < r.klen ? good : 0;
                 if (A.causal) {
-                    lo = min(max(key - shift - at, 0), kWalk) * A.pack;
+                    lo = key < r.prefix ? 0 : min(max(key - shift - at, 0), kWalk) * A.pack;
                     one_lo = min(max(-shift - at, -kWalk), kWalk) * A.pack;  // the token that sees key 0 only
                     one_hi = one_lo + A.pack;
+                    if (MOD != kPlain && r.prefix == 1) one_lo = 0;  // with a prefix of one all before it do too,
+                    if (MOD != kPlain && r.prefix > 1) one_hi = one_lo;  // with a longer one none does
                 }
                 if (r.klen == 1) {
                     one_lo = 0;
@@ -1607,6 +1757,18 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         tmem_wait_ld();
         pin<32>(s);
         pin<32>(d);
+        if constexpr (MOD == kCapped) {
+            if (beyond_reach<32>(A, s)) {
+                cap_tmem(A, ts, 32);
+                tmem_ld32(ts, s);
+                tmem_wait_ld();
+                pin<32>(s);
+            } else {
+                cap_near<32>(A, s);
+            }
+        }
+        // DQ: from the key that the row is level with to the first of this thread's columns.
+        const float ahead = DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level);
         uint32_t ps[16], pd[16];
         // Straight code in either case: the exponentials' latencies overlap.
         auto weights = [&](auto masked) {
@@ -1620,8 +1782,26 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
                 nd = make_float4(row_nd, row_nd, row_nd, row_nd);
             }
-            const float2 a = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(nl.x, nl.y));
-            const float2 b = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(nl.z, nl.w));
+            if constexpr (MOD != kPlain) {
+                if (A.slopes) {
+                    if (DKV) {
+                        const float4 m = *reinterpret_cast<const float4 *>(&sh.slope2[st][c0 + c]);
+                        const float4 at = *reinterpret_cast<const float4 *>(&sh.level[st][c0 + c]);
+                        nl.x = fmaf(-m.x, fabsf(at.x - (float)row), nl.x);
+                        nl.y = fmaf(-m.y, fabsf(at.y - (float)row), nl.y);
+                        nl.z = fmaf(-m.z, fabsf(at.z - (float)row), nl.z);
+                        nl.w = fmaf(-m.w, fabsf(at.w - (float)row), nl.w);
+                    } else {
+                        nl.x = fmaf(-scores.slope, fabsf(ahead + (float)c), nl.x);
+                        nl.y = fmaf(-scores.slope, fabsf(ahead + (float)(c + 1)), nl.y);
+                        nl.z = fmaf(-scores.slope, fabsf(ahead + (float)(c + 2)), nl.z);
+                        nl.w = fmaf(-scores.slope, fabsf(ahead + (float)(c + 3)), nl.w);
+                    }
+                }
+            }
+            const float2 s01 = make_float2(s[c], s[c + 1]), s23 = make_float2(s[c + 2], s[c + 3]);
+            const float2 a = MOD == kCapped ? add2(s01, make_float2(nl.x, nl.y)) : fma2(s01, sc2, make_float2(nl.x, nl.y));
+            const float2 b = MOD == kCapped ? add2(s23, make_float2(nl.z, nl.w)) : fma2(s23, sc2, make_float2(nl.z, nl.w));
             float p[4] = {exp2_fast(a.x), exp2_fast(a.y), exp2_fast(b.x), exp2_fast(b.y)};
             const float2 e = mul2(make_float2(p[0], p[1]), add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
             const float2 f =
@@ -1634,6 +1814,16 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                     p[k] = seen & bit ? p[k] : 0.0f;
                     ds[k] = seen & bit ? ds[k] : 0.0f;
                     if (masked == 2 && (one & bit)) ds[k] = DKV ? sh.one_ds[st][c0 + c + k] : row_od;
+                }
+            }
+            if constexpr (MOD == kCapped) {  // times 1 - (S' / cap)^2
+                const float2 inv = make_float2(A.cap_inv, A.cap_inv), minus = make_float2(-1.0f, -1.0f);
+                const float2 t01 = mul2(s01, inv), t23 = mul2(s23, inv), one2 = make_float2(1.0f, 1.0f);
+                const float2 f01 = fma2(mul2(t01, minus), t01, one2), f23 = fma2(mul2(t23, minus), t23, one2);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float f = k == 0 ? f01.x : k == 1 ? f01.y : k == 2 ? f23.x : f23.y;
+                    ds[k] = !masked || (seen & (1u << (c + k))) ? ds[k] * f : 0.0f;
                 }
             }
             ps[c / 2] = pack_bf16(p[0], p[1]);
@@ -1733,7 +1923,7 @@ __device__ __forceinline__ void share_acc(const AttnArgs &A, uint32_t smem, int 
     cluster_sync();  // no block leaves while another reads its shared memory
 }
 
-template <int DP, bool DKV>
+template <int DP, bool DKV, int MOD>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, const __grid_constant__ CUtensorMap mx1,
                      const __grid_constant__ CUtensorMap my0, const __grid_constant__ CUtensorMap my1,
@@ -1762,17 +1952,18 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
     r.tok = kWalk / A.pack;
     r.first = r.k0 = r.q0 = r.qtok = 0;
     r.steps_per_sub = 1;
+    r.prefix = prefix_of<MOD>(A, x.seq, DKV ? x.len : x.other_len);
     if (DKV) {
         r.kbase = x.base, r.klen = x.len, r.k0 = x.first;
         r.qbase = x.other_base, r.qlen = x.other_len;
-        r.first = A.causal ? min(r.qlen, max(0, r.k0 + r.qlen - r.klen)) : 0;
+        r.first = A.causal && r.k0 >= r.prefix ? min(r.qlen, max(0, r.k0 + r.qlen - r.klen)) : 0;
         r.steps_per_sub = (r.qlen - r.first + r.tok - 1) / r.tok;
         r.steps = r.steps_per_sub * A.subs;
     } else {
         r.qbase = x.base, r.qlen = x.len, r.q0 = x.first;
         r.kbase = x.other_base, r.klen = x.other_len;
         r.qtok = min(per, r.qlen - r.q0);
-        const int sees = A.causal ? min(r.klen, max(0, r.q0 + r.qtok + r.klen - r.qlen)) : r.klen;
+        const int sees = A.causal ? max(min(r.klen, max(0, r.q0 + r.qtok + r.klen - r.qlen)), r.prefix) : r.klen;
         r.steps = (sees + kWalk - 1) / kWalk;
     }
     const int each = (r.steps + ranks - 1) / ranks;
@@ -1827,10 +2018,10 @@ attn_backward_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap mx0, 
         if constexpr (DP > 32) regs_less<S::Regs::kLess>();
         if (warp == S::kCompute && steps > 0) bwd_mma_loop<DP, DKV>(sh, smem_x, smem_y, steps, tmem, A.D);
         if (warp == S::kCompute + 1)
-            issued = bwd_load<DP, DKV>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, f);
+            issued = bwd_load<DP, DKV, MOD>(A, &mx0, &mx1, &my0, &my1, sh, smem_x, smem_y, r, f);
     } else {
         if constexpr (DP > 32) regs_more<S::Regs::kMore>();
-        bwd_grads<DP, DKV>(A, sh, r, tmem, f, rank == 0);
+        bwd_grads<DP, DKV, MOD>(A, sh, r, tmem, f, rank == 0);
         __syncwarp();
         if (ranks == 1) store_acc<DP, DKV, S::kCompute / 4>(A, acc, steps > 0, row_at, live, g0, g1);
     }
@@ -1998,7 +2189,7 @@ size_t split_bytes(const AttnArgs &A, const ForwardPlan &p) {
     return (size_t)p.blocks * part_rows(A) * (A.D + 1) * sizeof(float);
 }
 
-template <int DP>
+template <int DP, int MOD>
 int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const Strided &k, const Strided &v,
                    const FwdOut &f, cudaStream_t stream) {
     const int per = 128 / A.pack, keys = plan.is_short ? ShortShape<DP>::kKeys : LongShape<DP, false>::kKeys;
@@ -2009,13 +2200,14 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
     const long long blocks = plan.slots * A.Hkv * A.subs;
     if (blocks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
     const int slots = (int)plan.slots;
+    if (MOD != kPlain) A.scale = 1.0f / kLog2e, A.scale_log2 = 1.0f;  // scores come in units of log2
     A.slot_rows = divisor(plan.slot_rows);
     A.heads = divisor(A.Hkv * A.subs);
     if (plan.is_short) {
         using S = ShortShape<DP>;
         const long long stay = (long long)S::kBlocks * num_sms();
-        if (int st = allow_smem(attn_forward_short_kernel<DP>, S::kSmem)) return st;
-        attn_forward_short_kernel<DP>
+        if (int st = allow_smem(attn_forward_short_kernel<DP, MOD>, S::kSmem)) return st;
+        attn_forward_short_kernel<DP, MOD>
             <<<(unsigned)(blocks < stay ? blocks : stay), 128, S::kSmem, stream>>>(A, mq, mk, mv, f, slots);
         return launch_status();
     }
@@ -2027,9 +2219,9 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
         return launch_status();
     };
     if (plan.blocks == 0)
-        return plan.alternate ? launch(attn_forward_long_kernel<DP, true, false>)
-                              : launch(attn_forward_long_kernel<DP, false, false>);
-    if (int st = launch(attn_forward_long_kernel<DP, true, true>)) return st;
+        return plan.alternate ? launch(attn_forward_long_kernel<DP, true, false, MOD>)
+                              : launch(attn_forward_long_kernel<DP, false, false, MOD>);
+    if (int st = launch(attn_forward_long_kernel<DP, true, true, MOD>)) return st;
     const int most = A.Tq < plan.slot_rows ? A.Tq : plan.slot_rows;  // tokens of a slot
     cudaLaunchConfig_t config{};
     const int items = most * A.pack * (A.D / 8), threads = items <= 512 ? 32 : 128;
@@ -2042,7 +2234,7 @@ int launch_forward(AttnArgs A, const ForwardPlan &plan, const Strided &q, const 
     attr.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    if (cudaLaunchKernelEx(&config, attn_join_kernel, A, f, slots, S::kLeast, plan.blocks) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&config, attn_join_kernel<MOD>, A, f, slots, S::kLeast, plan.blocks) != cudaSuccess) {
         (void)cudaGetLastError();
         return RFDETR_ERR_CUDA;
     }
@@ -2080,11 +2272,11 @@ template <int DP> BackwardPlan plan_backward(const AttnArgs &A) {
     return p;
 }
 
-template <int DP, bool DKV, typename... Args>
+template <int DP, bool DKV, int MOD, typename... Args>
 int launch_backward_kernel(long long tiles, int ranks, bool overlap, cudaStream_t stream, Args... args) {
     using S = BwdShape<DP>;
     if (tiles * ranks > 0x7fffffffll) return RFDETR_ERR_SHAPE;
-    if (int st = allow_smem(attn_backward_kernel<DP, DKV>, S::kSmem)) return st;
+    if (int st = allow_smem(attn_backward_kernel<DP, DKV, MOD>, S::kSmem)) return st;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3((unsigned)(tiles * ranks));
     config.blockDim = dim3(S::kThreads);
@@ -2100,14 +2292,14 @@ int launch_backward_kernel(long long tiles, int ranks, bool overlap, cudaStream_
         attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
-    if (cudaLaunchKernelEx(&config, attn_backward_kernel<DP, DKV>, args..., ranks) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&config, attn_backward_kernel<DP, DKV, MOD>, args..., ranks) != cudaSuccess) {
         (void)cudaGetLastError();
         return RFDETR_ERR_CUDA;
     }
     return RFDETR_OK;
 }
 
-template <int DP>
+template <int DP, int MOD>
 int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Strided &v, const Strided &g,
                     const BwdRows &f, bf16 *dq, bf16 *dk, bf16 *dv, cudaStream_t stream) {
     constexpr int kWalk = BwdShape<DP>::kWalk;
@@ -2125,7 +2317,7 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
         A.slot_rows = divisor(xtok);
         A.heads = divisor(A.Hkv * A.subs);
-        if (int st = launch_backward_kernel<DP, false>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq,
+        if (int st = launch_backward_kernel<DP, false, MOD>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq,
                                                        nullptr, (int)slots))
             return st;
     }
@@ -2133,7 +2325,7 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
         const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
         A.slot_rows = divisor(128);
         A.heads = divisor(A.Hkv);
-        if (int st = launch_backward_kernel<DP, true>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk,
+        if (int st = launch_backward_kernel<DP, true, MOD>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk,
                                                       dv, (int)slots))
             return st;
     }
@@ -2142,7 +2334,7 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
 
 AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, int64_t Tq, int64_t Tk, int64_t Hq,
                    int64_t Hkv, int64_t D, int causal, float scale, int most_packed) {
-    AttnArgs A;
+    AttnArgs A{};
     A.q_off = q_off;
     A.k_off = k_off ? k_off : q_off;
     A.n_seq = (int)n_seq;
@@ -2158,6 +2350,49 @@ AttnArgs make_args(const int32_t *q_off, const int32_t *k_off, int64_t n_seq, in
     A.scale = scale;
     A.scale_log2 = scale * kLog2e;
     return A;
+}
+
+// What a call does to its scores; cap 0: no cap.
+struct ScoreChange {
+    float cap;
+    const float *slopes;
+    const int32_t *prefix;
+    bool any() const { return cap != 0.0f || slopes || prefix; }
+};
+
+int check_change(const ScoreChange &m, float scale) {
+    if (m.cap != 0.0f) {
+        // (In units of the cap scores are products times scale / cap, which has to be a number.)
+        if (!(m.cap >= 0x1p-64f && m.cap <= 0x1p64f)) return RFDETR_ERR_SHAPE;
+        const float in = scale / m.cap;
+        if (!(in >= FLT_MIN && in <= FLT_MAX)) return RFDETR_ERR_SHAPE;
+    }
+    return aligned(m.slopes, 4) && aligned(m.prefix, 4) ? RFDETR_OK : RFDETR_ERR_ALIGN;
+}
+
+void set_change(AttnArgs &A, const ScoreChange &m) {
+    A.unit = A.scale_log2;
+    A.slopes = m.slopes;
+    A.prefix = m.prefix;
+    if (m.cap == 0.0f) return;
+    A.cap_in = A.scale / m.cap;
+    A.cap_out = m.cap * kLog2e;
+    A.cap_inv = 1.0f / A.cap_out;
+    for (int k = 0; k < 4; ++k) A.cap_poly[k] = A.cap_out * kCapPoly[k];
+}
+
+// Calls f with the head's padded size and what is done to scores, as types.
+template <typename F> int with_kernels(int64_t head_dim, const ScoreChange &m, F f) {
+    auto with = [&](auto dp) {
+        if (m.cap != 0.0f) return f(dp, std::integral_constant<int, kCapped>{});
+        if (m.any()) return f(dp, std::integral_constant<int, kBiased>{});
+        return f(dp, std::integral_constant<int, kPlain>{});
+    };
+    switch (padded_dim(head_dim)) {
+        case 32: return with(std::integral_constant<int, 32>{});
+        case 64: return with(std::integral_constant<int, 64>{});
+        default: return with(std::integral_constant<int, 128>{});
+    }
 }
 
 }  // namespace
@@ -2183,17 +2418,20 @@ extern "C" size_t rfdetr_packed_attention_workspace_bytes(int64_t n_sequences, i
     return split_bytes(A, plan_forward(A));
 }
 
-extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride,
+extern "C" int rfdetr_packed_attention_scored(void *stream, const void *query, int64_t query_token_stride,
                                        int64_t query_head_stride, const void *key, int64_t key_token_stride,
                                        int64_t key_head_stride, const void *value, int64_t value_token_stride,
                                        int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
                                        void *output, void *output_low, float *lse, void *workspace,
                                        size_t workspace_bytes,
                                        int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
-                                       int64_t n_kv_heads, int64_t head_dim, int causal, float scale) {
+                                       int64_t n_kv_heads, int64_t head_dim, int causal, float scale,
+                                       float score_cap, const float *distance_slopes, const int32_t *prefix) {
     using namespace rfdetr;
+    const ScoreChange change{score_cap, distance_slopes, prefix};
     if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
     if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
+    if (int st = check_change(change, scale)) return st;
     if (tokens == 0) return RFDETR_OK;
     const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
         v{value, value_token_stride, value_head_stride};
@@ -2203,8 +2441,9 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
     if (!output || !aligned(output, 16) || !aligned(output_low, 16) || !aligned(lse, 4) || !offsets ||
         !aligned(offsets, 4) || !aligned(key_offsets, 4))
         return RFDETR_ERR_ALIGN;
-    const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
-                                 causal, scale, 128);
+    AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, causal,
+                           scale, 128);
+    set_change(A, change);
     const ForwardPlan p = plan_forward(A);
     const size_t need = split_bytes(A, p);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return RFDETR_ERR_WORKSPACE;
@@ -2215,11 +2454,24 @@ extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t 
         f.part_lse = f.part + (size_t)p.blocks * f.part_rows * A.D;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch (padded_dim(head_dim)) {
-        case 32: return launch_forward<32>(A, p, q, k, v, f, s);
-        case 64: return launch_forward<64>(A, p, q, k, v, f, s);
-        default: return launch_forward<128>(A, p, q, k, v, f, s);
-    }
+    return with_kernels(head_dim, change, [&](auto dp, auto mod) {
+        return launch_forward<decltype(dp)::value, decltype(mod)::value>(A, p, q, k, v, f, s);
+    });
+}
+
+extern "C" int rfdetr_packed_attention(void *stream, const void *query, int64_t query_token_stride,
+                                       int64_t query_head_stride, const void *key, int64_t key_token_stride,
+                                       int64_t key_head_stride, const void *value, int64_t value_token_stride,
+                                       int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets,
+                                       void *output, void *output_low, float *lse, void *workspace,
+                                       size_t workspace_bytes, int64_t n_sequences, int64_t tokens,
+                                       int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                       int causal, float scale) {
+    return rfdetr_packed_attention_scored(
+        stream, query, query_token_stride, query_head_stride, key, key_token_stride, key_head_stride, value,
+        value_token_stride, value_head_stride, offsets, key_offsets, output, output_low, lse, workspace,
+        workspace_bytes, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, causal, scale, 0.0f, nullptr,
+        nullptr);
 }
 
 extern "C" size_t rfdetr_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t n_heads) {
@@ -2227,7 +2479,7 @@ extern "C" size_t rfdetr_packed_attention_backward_workspace_bytes(int64_t token
     return (size_t)tokens * n_heads * sizeof(float);
 }
 
-extern "C" int rfdetr_packed_attention_backward(
+extern "C" int rfdetr_packed_attention_scored_backward(
     void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride, const void *key,
     int64_t key_token_stride, int64_t key_head_stride, const void *value, int64_t value_token_stride,
     int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets, const void *output,
@@ -2235,10 +2487,12 @@ extern "C" int rfdetr_packed_attention_backward(
     int64_t grad_head_stride,
     const float *grad_lse, void *grad_query, void *grad_key, void *grad_value, void *workspace, size_t workspace_bytes,
     int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
-    int causal, float scale) {
+    int causal, float scale, float score_cap, const float *distance_slopes, const int32_t *prefix) {
     using namespace rfdetr;
+    const ScoreChange change{score_cap, distance_slopes, prefix};
     if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
     if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
+    if (int st = check_change(change, scale)) return st;
     if (tokens == 0 && key_tokens == 0) return RFDETR_OK;
     const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
         v{value, value_token_stride, value_head_stride}, g{grad_output, grad_token_stride, grad_head_stride};
@@ -2254,17 +2508,31 @@ extern "C" int rfdetr_packed_attention_backward(
         return RFDETR_ERR_ALIGN;
     const size_t need = rfdetr_packed_attention_backward_workspace_bytes(tokens, n_heads);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 4))) return RFDETR_ERR_WORKSPACE;
-    const AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim,
-                                 causal, scale, head_dim <= 32 ? BwdShape<32>::kWalk : BwdShape<64>::kWalk);
+    AttnArgs A = make_args(offsets, key_offsets, n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, causal,
+                           scale, head_dim <= 32 ? BwdShape<32>::kWalk : BwdShape<64>::kWalk);
+    set_change(A, change);
     const BwdRows f{static_cast<const bf16 *>(output), static_cast<const bf16 *>(output_low),
                     static_cast<const bf16 *>(grad_output), grad_token_stride, grad_head_stride, lse, grad_lse,
                     static_cast<float *>(workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bf16 *dq = static_cast<bf16 *>(grad_query), *dk = static_cast<bf16 *>(grad_key),
          *dv = static_cast<bf16 *>(grad_value);
-    switch (padded_dim(head_dim)) {
-        case 32: return launch_backward<32>(A, q, k, v, g, f, dq, dk, dv, s);
-        case 64: return launch_backward<64>(A, q, k, v, g, f, dq, dk, dv, s);
-        default: return launch_backward<128>(A, q, k, v, g, f, dq, dk, dv, s);
-    }
+    return with_kernels(head_dim, change, [&](auto dp, auto mod) {
+        return launch_backward<decltype(dp)::value, decltype(mod)::value>(A, q, k, v, g, f, dq, dk, dv, s);
+    });
+}
+
+extern "C" int rfdetr_packed_attention_backward(
+    void *stream, const void *query, int64_t query_token_stride, int64_t query_head_stride, const void *key,
+    int64_t key_token_stride, int64_t key_head_stride, const void *value, int64_t value_token_stride,
+    int64_t value_head_stride, const int32_t *offsets, const int32_t *key_offsets, const void *output,
+    const void *output_low, const float *lse, const void *grad_output, int64_t grad_token_stride,
+    int64_t grad_head_stride, const float *grad_lse, void *grad_query, void *grad_key, void *grad_value,
+    void *workspace, size_t workspace_bytes, int64_t n_sequences, int64_t tokens, int64_t key_tokens, int64_t n_heads,
+    int64_t n_kv_heads, int64_t head_dim, int causal, float scale) {
+    return rfdetr_packed_attention_scored_backward(
+        stream, query, query_token_stride, query_head_stride, key, key_token_stride, key_head_stride, value,
+        value_token_stride, value_head_stride, offsets, key_offsets, output, output_low, lse, grad_output,
+        grad_token_stride, grad_head_stride, grad_lse, grad_query, grad_key, grad_value, workspace, workspace_bytes,
+        n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim, causal, scale, 0.0f, nullptr, nullptr);
 }
