@@ -30,7 +30,8 @@ constexpr int kNormThreads = 256, kNormWarps = kNormThreads / 32;
 constexpr int kMostDim = 256;
 constexpr double kTurnsPerRadian = 0.15915494309189533576888;
 
-// How a lane finds the partners of its channels: it holds both (paired, interleaved), or through shared memory.
+// How a lane finds the partners of its channels: it holds both, from two pieces half apart (kPaired) or from one
+// (kInterleaved), or they meet through shared memory (kExchange).
 enum { kPaired, kInterleaved, kExchange };
 
 struct NormArgs {
@@ -52,16 +53,41 @@ struct NormArgs {
     int D, half;
     bool interleaved;
     int per_chunk;                // tokens that share a forming of sines
+    int sines_at_once;            // of them, by the threads of a block
     int pieces, lanes;            // of a row; lanes that hold it
     Divisor lanes_of, half_of;
     float eps, inv_dim;
     float *partial;               // backward: [blocks][2][D], or null
 };
 
-__device__ __forceinline__ double position_at(const NormArgs &A, long long i) {
-    if (A.position_type == RFDETR_I32) return (double)static_cast<const int32_t *>(A.positions)[i];
-    if (A.position_type == RFDETR_I64) return (double)static_cast<const int64_t *>(A.positions)[i];
-    return (double)static_cast<const float *>(A.positions)[i];
+// A position times a frequency (radians per unit), in turns, reduced to half a turn at most.  Where the position is a
+// float and the turns are below 2^22 the frequency in turns and the product are each carried as two floats, good
+// to 2^-46 of the product; otherwise, and to the same end, float64.
+__device__ __forceinline__ float turns_of(const NormArgs &A, long long at, float inv_freq) {
+    constexpr float kHigh = (float)kTurnsPerRadian, kLow = (float)(kTurnsPerRadian - (double)kHigh);
+    float p;
+    double far;
+    bool exact = true;
+    if (A.position_type == RFDETR_F32) {
+        p = __ldg(static_cast<const float *>(A.positions) + at);
+        far = (double)p;
+    } else if (A.position_type == RFDETR_I32) {
+        const int32_t v = __ldg(static_cast<const int32_t *>(A.positions) + at);
+        p = (float)v;
+        far = (double)v;
+        exact = v > -(1 << 24) && v < 1 << 24;
+    } else {
+        const long long v = __ldg(static_cast<const long long *>(A.positions) + at);
+        p = (float)v;
+        far = (double)v;
+        exact = v > -(1 << 24) && v < 1 << 24;
+    }
+    const float f = __fmul_rn(inv_freq, kHigh), low = fmaf(inv_freq, kLow, fmaf(inv_freq, kHigh, -f));
+    const float turns = __fmul_rn(p, f);
+    if (exact && fabsf(turns) < 4194304.0f)
+        return __fsub_rn(turns, rintf(turns)) + fmaf(p, low, fmaf(p, f, -turns));
+    const double all = far * (double)inv_freq * kTurnsPerRadian;
+    return (float)(all - rint(all));
 }
 
 // Places in shared memory: one is left out after every VEC, so that lanes' pieces lie in different banks.
@@ -69,6 +95,12 @@ template <int VEC> __host__ __device__ constexpr int spread(int i) { return VEC 
 
 // The sum over the lanes of a row, in each of them; `at` is the lane's place in the row.
 __device__ __forceinline__ float row_sum(float x, int at, int lanes) {
+    if ((lanes & (lanes - 1)) == 0) {
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2)
+            if (o < lanes) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
         if (o >= lanes) break;
@@ -78,272 +110,552 @@ __device__ __forceinline__ float row_sum(float x, int at, int lanes) {
     return __shfl_sync(0xffffffffu, x, (threadIdx.x & 31) - at);
 }
 
-// N pieces to a lane (the row's pieces at, at + lanes, ...), each of K vectors of VEC channels.
-template <typename T, int VEC, int MODE, int N, bool BACK> struct Rows {
+// 1 / sqrt(x), the hardware's approximation and a step of Newton's: within an ulp or so.
+__device__ __forceinline__ float inverse_root(float x) {
+    const float r = rsqrtf(x);
+    const float e = fmaf(-x * r, r, 1.0f);
+    return x > 0.0f && x <= FLT_MAX ? fmaf(0.5f * r, e, r) : r;  // (0 and inf: their roots' inverses as they are)
+}
+
+// A lane's row, a head of a token of one of the two tensors, and its way to the next of its rows in a chunk.
+template <typename T> struct Row {
+    const T *x, *g;
+    T *y;
+    int h, token;  // tokens from the chunk's first on
+    bool live;
+};
+struct Stride {
+    int t, h, y;  // tokens and heads on (heads past the last are the next token's), and elements of the output
+    long long x, g, wrap_x, wrap_g;
+};
+
+template <bool BACK> __device__ __forceinline__ Stride stride_of(const NormArgs &A, int which, int step) {
+    Stride s;
+    const int heads = A.heads[which];
+    s.t = quotient(step, A.heads_of[which]);
+    s.h = step - s.t * heads;
+    s.y = step * A.D;
+    s.x = s.t * A.token[which] + s.h * A.head[which];
+    s.wrap_x = A.token[which] - heads * A.head[which];
+    s.g = BACK ? s.t * A.grad_token[which] + s.h * A.grad_head[which] : 0;
+    s.wrap_g = BACK ? A.grad_token[which] - heads * A.grad_head[which] : 0;
+    return s;
+}
+template <typename T, bool BACK>
+__device__ __forceinline__ Row<T> row_of(const NormArgs &A, int which, long long t0, int row, bool live) {
+    Row<T> r;
+    r.token = quotient(row, A.heads_of[which]);
+    r.h = row - r.token * A.heads[which];
+    r.live = live;
+    const long long t = t0 + r.token;
+    r.x = static_cast<const T *>(A.in[which]) + t * A.token[which] + r.h * A.head[which];
+    r.g = BACK ? static_cast<const T *>(A.grad[which]) + t * A.grad_token[which] + r.h * A.grad_head[which] : nullptr;
+    r.y = static_cast<T *>(A.out[which]) + (t0 * A.heads[which] + row) * A.D;
+    return r;
+}
+template <typename T, bool BACK> __device__ __forceinline__ void go_on(Row<T> &r, const Stride &s, int heads) {
+    r.token += s.t;
+    r.h += s.h;
+    r.x += s.x;
+    if (BACK) r.g += s.g;
+    r.y += s.y;
+    if (r.h >= heads) {
+        r.h -= heads;
+        ++r.token;
+        r.x += s.wrap_x;
+        if (BACK) r.g += s.wrap_g;
+    }
+}
+
+// VEC values to 16-byte-aligned memory; bf16 rounded two at a time.
+template <typename T, int VEC> __device__ __forceinline__ void put_values(T *p, const float *x) {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) w[e / 2] = pack_bf16(x[e], x[e + 1]);
+        using V = typename Raw<VEC * 2>::T;
+        *reinterpret_cast<V *>(p) = *reinterpret_cast<V *>(w);
+    } else {
+        store_vec<T, VEC>(p, x);
+    }
+}
+
+// N of float32 pairs from and to 16-byte-aligned shared memory, as wide as they go.
+template <int N> __device__ __forceinline__ void load_pairs(const float *p, int stride4, float2 *v) {
+    if constexpr (N == 1) {
+        v[0] = *reinterpret_cast<const float2 *>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float4 x = *reinterpret_cast<const float4 *>(p + (i / 2) * stride4);
+            v[i] = make_float2(x.x, x.y);
+            v[i + 1] = make_float2(x.z, x.w);
+        }
+    }
+}
+
+// Rows whose lanes hold both partners of their pairs.  A lane has N pieces of P pairs of channels, as float32 pairs
+// (of neighbouring channel pairs) of first partners and of second: packed arithmetic takes half the issue slots, which is what
+// bounds the plain form of this (32,768 tokens of 16 + 4 heads of 128, bf16: 95 us forward and 167 backward with
+// scalar arithmetic and places found by division for every row).
+// In shared memory cosines and sines, and weights, lie by pieces: four pairs' of all pieces, then the next four.
+template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
+    static constexpr int P = MODE == kPaired ? VEC : VEC / 2, Q = P / 2;  // pairs, float2 of them
     static constexpr int K = MODE == kPaired ? 2 : 1;
     using V = typename Raw<VEC * (int)sizeof(T)>::T;
-    using Values = float[N][K][VEC];
-
+    struct Values {
+        float2 a[N][Q], b[N][Q];
+    };
     struct Raws {
         V x[N][K], g[BACK ? N : 1][K];
     };
+    // What is the same for every row.
+    struct Lane {
+        int c[N];        // first channel, elements; paired: of the first vector
+        bool has[N], turns[N];
+    };
 
-    // First channel of vector k of a piece, and whether there is such a vector.
-    static __device__ __forceinline__ int channel(const NormArgs &A, int piece, int k) {
-        if (MODE != kPaired) return piece * VEC;
-        const int turned = A.half / VEC;
-        return piece < turned ? piece * VEC + k * A.half : 2 * A.half + (piece - turned) * VEC;
-    }
-    static __device__ __forceinline__ bool has(const NormArgs &A, int piece, int k) {
-        return piece < A.pieces && (MODE != kPaired || k == 0 || piece < A.half / VEC);
-    }
-
-    static __device__ __forceinline__ void load(const NormArgs &A, int which, long long t, int h, int at, bool live,
-                                                Raws &r) {
-        const T *x = static_cast<const T *>(A.in[which]) + t * A.token[which] + h * A.head[which];
-        const T *g = BACK ? static_cast<const T *>(A.grad[which]) + t * A.grad_token[which] + h * A.grad_head[which]
-                          : nullptr;
+    static __device__ __forceinline__ Lane lane_of(const NormArgs &A, int at) {
+        Lane l;
+        const int turned = MODE == kPaired ? A.half / VEC : (2 * A.half + VEC - 1) / VEC;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int piece = at + n * A.lanes;
+            l.has[n] = piece < A.pieces;
+            l.turns[n] = piece < turned;
+            l.c[n] = MODE != kPaired || l.turns[n] ? piece * VEC : 2 * A.half + (piece - turned) * VEC;
+        }
+        return l;
+    }
+    // Shared memory: floats of a token's cosines and sines, of a weight, and where a channel's or pair's value goes.
+    static __host__ __device__ int turn_floats(const NormArgs &A) { return 2 * ((A.half + P - 1) / P * P); }
+    static __host__ __device__ int row_floats(const NormArgs &A) { return (2 * A.pieces * P + 3) / 4 * 4; }
+    static __device__ __forceinline__ int by_pieces(int i, int pieces) {  // of value i, P to a piece
+        if (P < 4) return i;
+        return ((i % P / 4) * pieces + i / P) * 4 + i % 4;
+    }
+    static __device__ __forceinline__ int turn_place(const NormArgs &A, int i) {
+        return by_pieces(i, (A.half + P - 1) / P);
+    }
+    // Of channel c in a weight's row: first partners, then second ones.
+    static __device__ __forceinline__ int weight_place(const NormArgs &A, int c) {
+        const int all = A.pieces * P;
+        if (MODE == kInterleaved) return (c & 1) * all + by_pieces(c >> 1, A.pieces);
+        const int R = 2 * A.half, turned = A.half / VEC;
+        if (c >= R) return by_pieces(turned * P + c - R, A.pieces);
+        return c >= A.half ? all + by_pieces(c - A.half, A.pieces) : by_pieces(c, A.pieces);
+    }
+    static __device__ __forceinline__ void weights(const NormArgs &A, const float *w, int piece, float2 *a, float2 *b) {
+        constexpr int kPlace = P < 4 ? P : 4;
+        load_pairs<Q>(w + piece * kPlace, A.pieces * 4, a);
+        load_pairs<Q>(w + A.pieces * P + piece * kPlace, A.pieces * 4, b);
+    }
+
+    static __device__ __forceinline__ void load(const NormArgs &A, const Lane &l, const Row<T> &w, Raws &r) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const bool ok = live && has(A, piece, k);
-                const int c = channel(A, piece, k);
-                r.x[n][k] = ok ? __ldg(reinterpret_cast<const V *>(x + c)) : V{};
-                if (BACK) r.g[n][k] = ok ? __ldg(reinterpret_cast<const V *>(g + c)) : V{};
+                const bool ok = w.live && l.has[n] && (k == 0 || l.turns[n]);
+                const int c = l.c[n] + k * A.half;
+                r.x[n][k] = ok ? __ldg(reinterpret_cast<const V *>(w.x + c)) : V{};
+                if (BACK) r.g[n][k] = ok ? __ldg(reinterpret_cast<const V *>(w.g + c)) : V{};
             }
+    }
+    static __device__ __forceinline__ float wide(const V &v, int e) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(&v)[e / 2];
+            return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+        } else {
+            return to_f32(reinterpret_cast<const T *>(&v)[e]);
         }
     }
     static __device__ __forceinline__ void widen(const V (&raw)[N][K], Values &v) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[n][k][e] = to_f32(reinterpret_cast<const T *>(&raw[n][k])[e]);
-    }
-
-    // Turns a row's values; `turn` holds the token's cosines and sines, `room` a row for the exchange.  Whole warp.
-    template <int SIGN>
-    static __device__ __forceinline__ void turned(const NormArgs &A, Values &v, int at, bool live, const float2 *turn,
-                                                  float *room) {
-        const int R = 2 * A.half;
-        if (MODE == kExchange) {
-            __syncwarp();  // the row before has been read
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int c = channel(A, at + n * A.lanes, 0) + e;
-                    if (live && c < R) room[spread<VEC>(c)] = v[n][0][e];
+            for (int i = 0; i < Q; ++i) {
+                if (MODE == kPaired) {
+                    v.a[n][i] = make_float2(wide(raw[n][0], 2 * i), wide(raw[n][0], 2 * i + 1));
+                    v.b[n][i] = make_float2(wide(raw[n][K - 1], 2 * i), wide(raw[n][K - 1], 2 * i + 1));
+                } else {
+                    v.a[n][i] = make_float2(wide(raw[n][0], 4 * i), wide(raw[n][0], 4 * i + 2));
+                    v.b[n][i] = make_float2(wide(raw[n][0], 4 * i + 1), wide(raw[n][0], 4 * i + 3));
                 }
-            __syncwarp();
-        }
-        if (!live) return;
+            }
+    }
+    template <bool INVERSE>
+    static __device__ __forceinline__ void turned(const NormArgs &A, const Lane &l, int at, Values &v, const float *turn) {
+        const float2 minus = make_float2(-1.0f, -1.0f);
+        const int pieces = (A.half + P - 1) / P;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int piece = at + n * A.lanes, c = channel(A, piece, 0);
-            if (MODE == kPaired) {
-                if (!has(A, piece, K - 1)) continue;
+            if (!l.turns[n]) continue;
+            float2 c[Q], s[Q];
+            constexpr int kPlace = P < 4 ? P : 4;
+            load_pairs<Q>(turn + (at + n * A.lanes) * kPlace, pieces * 4, c);
+            load_pairs<Q>(turn + pieces * P + (at + n * A.lanes) * kPlace, pieces * 4, s);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float2 r = turn[spread<VEC>(c) + e];
-                    const float x1 = v[n][0][e], x2 = v[n][K - 1][e], s = SIGN * r.y;
-                    v[n][0][e] = fmaf(x1, r.x, -(x2 * s));
-                    v[n][K - 1][e] = fmaf(x2, r.x, x1 * s);
+            for (int i = 0; i < Q; ++i) {
+                const float2 x = v.a[n][i], y = v.b[n][i], xs = mul2(x, s[i]), ys = mul2(y, s[i]);
+                float2 u = INVERSE ? fma2(x, c[i], ys) : fma2(x, c[i], mul2(ys, minus));
+                float2 w = INVERSE ? fma2(y, c[i], mul2(xs, minus)) : fma2(y, c[i], xs);
+                if (MODE == kInterleaved) {  // of the last piece some may not turn
+                    const int pair = l.c[n] / 2 + 2 * i;
+                    if (pair >= A.half) u.x = x.x, w.x = y.x;
+                    if (pair + 1 >= A.half) u.y = x.y, w.y = y.y;
                 }
-            } else if (MODE == kInterleaved) {
-#pragma unroll
-                for (int e = 0; e + 1 < VEC; e += 2) {
-                    if (c + e >= R) continue;
-                    const float2 r = turn[spread<VEC / 2>((c + e) / 2)];
-                    const float x1 = v[n][0][e], x2 = v[n][0][e + 1], s = SIGN * r.y;
-                    v[n][0][e] = fmaf(x1, r.x, -(x2 * s));
-                    v[n][0][e + 1] = fmaf(x2, r.x, x1 * s);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int d = c + e;
-                    if (d >= R) continue;
-                    const bool first = A.interleaved ? !(d & 1) : d < A.half;
-                    const int other = A.interleaved ? d ^ 1 : first ? d + A.half : d - A.half;
-                    const float2 r = turn[spread<VEC>(A.interleaved ? d >> 1 : first ? d : other)];
-                    const float s = first ? -SIGN * r.y : SIGN * r.y;
-                    v[n][0][e] = fmaf(v[n][0][e], r.x, room[spread<VEC>(other)] * s);
-                }
+                v.a[n][i] = u;
+                v.b[n][i] = w;
             }
         }
     }
-
-    static __device__ __forceinline__ void store(const NormArgs &A, const Values &v, int which, long long t, int h,
-                                                 int at, bool live) {
-        T *y = static_cast<T *>(A.out[which]) + (t * A.heads[which] + h) * A.D;
+    static __device__ __forceinline__ void store(const NormArgs &A, const Lane &l, T *y, const Values &v, float r,
+                                                 bool live) {
+        const float2 r2 = make_float2(r, r);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (!live || !l.has[n]) continue;
+            float x[K][VEC];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const float2 u = mul2(v.a[n][i], r2), w = mul2(v.b[n][i], r2);
+                if (MODE == kPaired) {
+                    x[0][2 * i] = u.x, x[0][2 * i + 1] = u.y;
+                    x[K - 1][2 * i] = w.x, x[K - 1][2 * i + 1] = w.y;
+                } else {
+                    x[0][4 * i] = u.x, x[0][4 * i + 2] = u.y;
+                    x[0][4 * i + 1] = w.x, x[0][4 * i + 3] = w.y;
+                }
+            }
+            put_values<T, VEC>(y + l.c[n], x[0]);
+            if (MODE == kPaired && l.turns[n]) put_values<T, VEC>(y + l.c[n] + A.half, x[K - 1]);
+        }
+    }
+    static __device__ __forceinline__ float square(const Values &v) {
+        float2 sum = make_float2(0.0f, 0.0f), more = sum;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (live && has(A, at + n * A.lanes, k))
-                    store_vec<T, VEC>(y + channel(A, at + n * A.lanes, k), v[n][k]);
+            for (int i = 0; i < Q; ++i) {
+                sum = fma2(v.a[n][i], v.a[n][i], sum);
+                more = fma2(v.b[n][i], v.b[n][i], more);
+            }
+        return (sum.x + sum.y) + (more.x + more.y);
     }
 
     // A row from its raw values to its result; backward adds to the weights' gradient.  Whole warp.
-    static __device__ __forceinline__ void row(const NormArgs &A, const Raws &raw, int which, long long t, int h,
-                                               int at, bool live, const float *weight, const float2 *turn, float *room,
-                                               Values &dw) {
+    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &l, const Raws &raw, T *y, bool live, int at,
+                                               const float *weight, const float *turn, float *, Values &dw) {
+        Values x;
+        widen(raw.x, x);
+        const float sum = square(x);
+        if (!BACK) {
+            const float r = inverse_root(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if (!l.has[n]) continue;
+                float2 wa[Q], wb[Q];
+                weights(A, weight, at + n * A.lanes, wa, wb);
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    x.a[n][i] = mul2(x.a[n][i], wa[i]);
+                    x.b[n][i] = mul2(x.b[n][i], wb[i]);
+                }
+            }
+            turned<false>(A, l, at, x, turn);
+            store(A, l, y, x, r, live);
+            return;
+        }
+        Values g;
+        if constexpr (BACK) widen(raw.g, g);
+        turned<true>(A, l, at, g, turn);
+        Values wh;
+        float2 dot = make_float2(0.0f, 0.0f), more = dot;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float2 wa[Q], wb[Q];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) wa[i] = wb[i] = make_float2(0.0f, 0.0f);
+            if (l.has[n]) weights(A, weight, at + n * A.lanes, wa, wb);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                wh.a[n][i] = mul2(g.a[n][i], wa[i]);
+                wh.b[n][i] = mul2(g.b[n][i], wb[i]);
+                dot = fma2(wh.a[n][i], x.a[n][i], dot);
+                more = fma2(wh.b[n][i], x.b[n][i], more);
+            }
+        }
+        const float r = inverse_root(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
+        const float back = -(row_sum((dot.x + dot.y) + (more.x + more.y), at, A.lanes) * A.inv_dim * r * r);
+        const float2 back2 = make_float2(back, back), r2 = make_float2(r, r);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                wh.a[n][i] = fma2(x.a[n][i], back2, wh.a[n][i]);
+                wh.b[n][i] = fma2(x.b[n][i], back2, wh.b[n][i]);
+                x.a[n][i] = mul2(x.a[n][i], r2);
+                x.b[n][i] = mul2(x.b[n][i], r2);
+            }
+        if (live) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    dw.a[n][i] = fma2(g.a[n][i], x.a[n][i], dw.a[n][i]);
+                    dw.b[n][i] = fma2(g.b[n][i], x.b[n][i], dw.b[n][i]);
+                }
+        }
+        store(A, l, y, wh, r, live);
+    }
+    // A lane's sums of dw to its row of shared memory, where the weights' values have their places.
+    static __device__ __forceinline__ void put(const NormArgs &A, const Lane &l, int at, const Values &v, float *to) {
+        constexpr int kPlace = P < 4 ? P : 4;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (!l.has[n]) continue;
+            const int piece = at + n * A.lanes;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int place = (i / 4) * A.pieces * 4 + piece * kPlace + i % 4;
+                to[place] = i & 1 ? v.a[n][i / 2].y : v.a[n][i / 2].x;
+                to[A.pieces * P + place] = i & 1 ? v.b[n][i / 2].y : v.b[n][i / 2].x;
+            }
+        }
+    }
+};
+
+// Rows whose partners meet through shared memory; a lane has N pieces of VEC channels.
+template <typename T, int VEC, int N, bool BACK> struct ExchangeRows {
+    using V = typename Raw<VEC * (int)sizeof(T)>::T;
+    using Values = float[N][VEC];
+    struct Raws {
+        V x[N], g[BACK ? N : 1];
+    };
+    struct Lane {
+        int at;
+    };
+
+    static __device__ __forceinline__ Lane lane_of(const NormArgs &, int at) { return {at}; }
+    static __host__ __device__ int turn_floats(const NormArgs &A) { return 2 * (spread<VEC>(A.half) + 1); }
+    static __host__ __device__ int row_floats(const NormArgs &A) { return spread<VEC>(A.D) + 1; }
+    static __device__ __forceinline__ int turn_place(const NormArgs &, int i) { return spread<VEC>(i); }
+    static __device__ __forceinline__ int weight_place(const NormArgs &, int c) { return spread<VEC>(c); }
+
+    static __device__ __forceinline__ void load(const NormArgs &A, const Lane &l, const Row<T> &w, Raws &r) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int piece = l.at + n * A.lanes;
+            const bool ok = w.live && piece < A.pieces;
+            r.x[n] = ok ? __ldg(reinterpret_cast<const V *>(w.x + piece * VEC)) : V{};
+            if (BACK) r.g[n] = ok ? __ldg(reinterpret_cast<const V *>(w.g + piece * VEC)) : V{};
+        }
+    }
+    static __device__ __forceinline__ void widen(const V (&raw)[N], Values &v) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[n][e] = to_f32(reinterpret_cast<const T *>(&raw[n])[e]);
+    }
+    // Whole warp.
+    template <bool INVERSE>
+    static __device__ __forceinline__ void turned(const NormArgs &A, Values &v, int at, bool live, const float *turn,
+                                                  float *room) {
+        const int R = 2 * A.half;
+        __syncwarp();  // the row before has been read
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int c = (at + n * A.lanes) * VEC + e;
+                if (live && c < R) room[spread<VEC>(c)] = v[n][e];
+            }
+        __syncwarp();
+        if (!live) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int d = (at + n * A.lanes) * VEC + e;
+                if (d >= R) continue;
+                const bool first = A.interleaved ? !(d & 1) : d < A.half;
+                const int other = A.interleaved ? d ^ 1 : first ? d + A.half : d - A.half;
+                const float *cs = turn + spread<VEC>(A.interleaved ? d >> 1 : first ? d : other);
+                const float s = cs[spread<VEC>(A.half) + 1];
+                v[n][e] = fmaf(v[n][e], cs[0], room[spread<VEC>(other)] * (first != INVERSE ? -s : s));
+            }
+    }
+    static __device__ __forceinline__ void store(const NormArgs &A, T *y, int at, Values &v, bool live) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (live && at + n * A.lanes < A.pieces) put_values<T, VEC>(y + (at + n * A.lanes) * VEC, v[n]);
+    }
+    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &, const Raws &raw, T *y, bool live, int at,
+                                               const float *weight, const float *turn, float *room, Values &dw) {
         Values x;
         widen(raw.x, x);
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) sum = fmaf(x[n][k][e], x[n][k][e], sum);
+            for (int e = 0; e < VEC; ++e) sum = fmaf(x[n][e], x[n][e], sum);
         if (!BACK) {
-            const float r = __frsqrt_rn(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
+            const float r = inverse_root(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int n = 0; n < N; ++n) {
+                const float *w = weight + spread<VEC>((at + n * A.lanes) * VEC);
+                const bool ok = at + n * A.lanes < A.pieces;
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const float *w = weight + spread<VEC>(channel(A, at + n * A.lanes, k));
-                    const bool ok = has(A, at + n * A.lanes, k);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) x[n][k][e] *= r * (ok ? w[e] : 0.0f);
-                }
-            turned<1>(A, x, at, live, turn, room);
-            store(A, x, which, t, h, at, live);
+                for (int e = 0; e < VEC; ++e) x[n][e] *= r * (ok ? w[e] : 0.0f);
+            }
+            turned<false>(A, x, at, live, turn, room);
+            store(A, y, at, x, live);
             return;
         }
-        Values g;
+        Values g, wh;
         if constexpr (BACK) widen(raw.g, g);
-        turned<-1>(A, g, at, live, turn, room);
+        turned<true>(A, g, at, live, turn, room);
         float dot = 0.0f;
-        Values wh;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
+            const float *w = weight + spread<VEC>((at + n * A.lanes) * VEC);
+            const bool ok = at + n * A.lanes < A.pieces;
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const float *w = weight + spread<VEC>(channel(A, at + n * A.lanes, k));
-                const bool ok = has(A, at + n * A.lanes, k);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    wh[n][k][e] = g[n][k][e] * (ok ? w[e] : 0.0f);
-                    dot = fmaf(wh[n][k][e], x[n][k][e], dot);
-                }
+            for (int e = 0; e < VEC; ++e) {
+                wh[n][e] = g[n][e] * (ok ? w[e] : 0.0f);
+                dot = fmaf(wh[n][e], x[n][e], dot);
             }
-        const float r = __frsqrt_rn(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
+        }
+        const float r = inverse_root(fmaf(row_sum(sum, at, A.lanes), A.inv_dim, A.eps));
         const float back = row_sum(dot, at, A.lanes) * A.inv_dim * r * r;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (live) dw[n][k][e] = fmaf(g[n][k][e], x[n][k][e] * r, dw[n][k][e]);
-                    wh[n][k][e] = r * fmaf(-x[n][k][e], back, wh[n][k][e]);
-                }
-        store(A, wh, which, t, h, at, live);
+            for (int e = 0; e < VEC; ++e) {
+                wh[n][e] = r * fmaf(-x[n][e], back, wh[n][e]);
+                if (live) dw[n][e] = fmaf(g[n][e], x[n][e] * r, dw[n][e]);
+            }
+        store(A, y, at, wh, live);
     }
-};
-
-// Floats of shared memory: sines, both weights, and the larger of the exchange's rows and the sums of dw.
-template <int VEC, int MODE> struct NormRoom {
-    static constexpr int kGroup = MODE == kInterleaved ? VEC / 2 : VEC;
-    int pitch, weights, row, sines, all;
-    __host__ __device__ NormRoom(const NormArgs &A, bool back) {
-        pitch = spread<kGroup>(A.half) + 1;
-        sines = 2 * A.per_chunk * pitch;
-        row = spread<VEC>(A.D) + 1;
-        weights = 2 * row;
-        const int rows = kNormWarps * (32 / A.lanes);
-        all = sines + weights + (back || MODE == kExchange ? rows * row : 0);
+    static __device__ __forceinline__ void put(const NormArgs &A, const Lane &, int at, const Values &v, float *to) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (at + n * A.lanes < A.pieces)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) to[spread<VEC>((at + n * A.lanes) * VEC) + e] = v[n][e];
     }
 };
 
 template <typename T, int VEC, int MODE, int N, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, BACK || N == 2 ? 2 : 4) normed_rotary_kernel(const NormArgs A) {
-    using S = Rows<T, VEC, MODE, N, BACK>;
-    using Room = NormRoom<VEC, MODE>;
-    extern __shared__ float2 turn[];
-    const Room room(A, BACK);
-    float *weights = reinterpret_cast<float *>(turn) + room.sines;
+using RowsOf = std::conditional_t<MODE == kExchange, ExchangeRows<T, VEC, N, BACK>,
+                                  PairRows<T, VEC, MODE == kExchange ? kPaired : MODE, N, BACK>>;
+
+// Floats of shared memory: sines, both weights, and the exchange's rows or the sums of dw.
+template <typename S, bool EXCHANGE> struct NormRoom {
+    int pitch, row, sines, all;
+    __host__ __device__ NormRoom(const NormArgs &A, bool back) {
+        pitch = S::turn_floats(A);
+        sines = (A.per_chunk * pitch + 3) / 4 * 4;
+        row = S::row_floats(A);
+        const int rows = kNormWarps * (32 / A.lanes);
+        all = sines + 2 * row + (back || EXCHANGE ? rows * row : 0);
+    }
+};
+
+template <bool BACK> constexpr int kNormBlocks = BACK ? 2 : 3;  // to an SM
+
+template <typename T, int VEC, int MODE, int N, bool BACK>
+__global__ void __launch_bounds__(kNormThreads, kNormBlocks<BACK>) normed_rotary_kernel(const NormArgs A) {
+    using S = RowsOf<T, VEC, MODE, N, BACK>;
+    extern __shared__ __align__(16) float turn[];
+    const NormRoom<S, MODE == kExchange> room(A, BACK);
+    float *weights = turn + room.sines;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows_a_warp = 32 / A.lanes;
     const int sub = quotient(lane, A.lanes_of), at = lane - sub * A.lanes;
     const bool used = sub < rows_a_warp;
-    float *mine = weights + room.weights + (warp * rows_a_warp + min(sub, rows_a_warp - 1)) * room.row;
-    constexpr int kStep = kNormWarps;  // rows, times rows_a_warp, from one of a lane's to the next
+    float *mine = weights + 2 * room.row + (warp * rows_a_warp + min(sub, rows_a_warp - 1)) * room.row;
+    const int step = kNormWarps * rows_a_warp;  // rows from one of a lane's to the next
+    const typename S::Lane place = S::lane_of(A, at);
 
     typename S::Values dw[BACK ? 2 : 1] = {};
 #pragma unroll 1
     for (long long chunk = blockIdx.x; chunk < A.chunks; chunk += gridDim.x) {
         const long long t0 = chunk * A.per_chunk;
         const int tokens = (int)min((long long)A.per_chunk, A.T - t0);
-        // The first row is asked for before the sines are formed, so that their time covers the load's.
-        typename S::Raws raw;
-        auto ask = [&](int which, int x) {
-            const int at_row = x + sub, t = quotient(at_row, A.heads_of[which]);
-            S::load(A, which, t0 + t, at_row - t * A.heads[which], at, used && at_row < tokens * A.heads[which], raw);
-        };
+        // The first row is asked for before the sines are formed, so that their time covers the load's, and
+        // each further one before the one before is worked on.
         const int start = warp * rows_a_warp;
-        if (start < tokens * A.heads[0]) ask(0, start);
+        typename S::Raws ahead;
+        Row<T> next;
+        auto ask = [&](int which) {
+            next = row_of<T, BACK>(A, which, t0, start + sub, used && start + sub < tokens * A.heads[which]);
+            S::load(A, place, next, ahead);
+        };
+        if (start < tokens * A.heads[0]) ask(0);
         __syncthreads();
         if (chunk == blockIdx.x) {
+            for (int i = threadIdx.x; i < 2 * room.row; i += kNormThreads) weights[i] = 0.0f;  // (places of no channel)
+            __syncthreads();
             for (int i = threadIdx.x; i < 2 * A.D; i += kNormThreads) {
                 const int which = i >= A.D, c = i - which * A.D;
                 const void *w = A.weight[which];
-                weights[which * room.row + spread<VEC>(c)] =
+                weights[which * room.row + S::weight_place(A, c)] =
                     !w ? 1.0f
                        : A.weight_type[which] == RFDETR_BF16 ? to_f32(static_cast<const bf16 *>(w)[c])
                                                              : static_cast<const float *>(w)[c];
             }
         }
-        for (int x = threadIdx.x; x < tokens * A.half; x += kNormThreads) {
-            const int t = quotient(x, A.half_of), i = x - t * A.half;
+        // A thread keeps to one frequency.
+        const int first = quotient(threadIdx.x, A.half_of), i = threadIdx.x - first * A.half;
+        if (first < A.sines_at_once) {
             int axis = 0;
             while (i >= A.ends[axis]) ++axis;
-            const double turns = position_at(A, (t0 + t) * A.n_axes + axis) * (double)__ldg(A.inv_freq + i) *
-                                 kTurnsPerRadian;
-            float s, c;
-            sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-            turn[t * room.pitch + spread<Room::kGroup>(i)] = make_float2(c, s);
+            const float inv_freq = __ldg(A.inv_freq + i);
+            float *cs = turn + first * room.pitch + S::turn_place(A, i);
+#pragma unroll 1
+            for (int t = first; t < tokens; t += A.sines_at_once) {
+                float s, c;
+                sincospif(2.0f * turns_of(A, (t0 + t) * A.n_axes + axis, inv_freq), &s, &c);
+                cs[0] = c;
+                cs[room.pitch / 2] = s;
+                cs += A.sines_at_once * room.pitch;
+            }
         }
         __syncthreads();
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const int rows = tokens * A.heads[which];
+            if (which == 1 && start < rows) ask(1);
+            const Stride stride = stride_of<BACK>(A, which, step);
 #pragma unroll 1
-            for (int x = start; x < rows; x += kStep * rows_a_warp) {
-                if (which == 1 || x != start) ask(which, x);
-                const int at_row = x + sub, t = quotient(at_row, A.heads_of[which]);
-                const bool live = used && at_row < rows;
-                S::row(A, raw, which, t0 + t, at_row - t * A.heads[which], at, live, weights + which * room.row,
-                       turn + (live ? t : 0) * room.pitch, mine, dw[BACK ? which : 0]);
+            for (int x = start; x < rows; x += step) {
+                const typename S::Raws raw = ahead;
+                T *const to = next.y;
+                const bool live = next.live;
+                const float *cs = turn + (live ? next.token : 0) * room.pitch;
+                if (x + step < rows) {
+                    go_on<T, BACK>(next, stride, A.heads[which]);
+                    next.live = used && x + step + sub < rows;
+                    S::load(A, place, next, ahead);
+                }
+                S::row(A, place, raw, to, live, at, weights + which * room.row, cs, mine, dw[BACK ? which : 0]);
             }
         }
     }
     if constexpr (BACK) {
         launch_dependents();
         if (!A.partial) return;
-        float *sums = weights + room.weights;
+        float *sums = weights + 2 * room.row;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             __syncthreads();
-            if (used)
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int k = 0; k < S::K; ++k)
-                        if (S::has(A, at + n * A.lanes, k))
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e)
-                                mine[spread<VEC>(S::channel(A, at + n * A.lanes, k)) + e] = dw[which][n][k][e];
+            if (used) S::put(A, place, at, dw[which], mine);
             __syncthreads();
             for (int c = threadIdx.x; c < A.D; c += kNormThreads) {
                 float sum = 0.0f;
-                for (int r = 0; r < kNormWarps * rows_a_warp; ++r) sum += sums[r * room.row + spread<VEC>(c)];
+                for (int r = 0; r < kNormWarps * rows_a_warp; ++r) sum += sums[r * room.row + S::weight_place(A, c)];
                 A.partial[((size_t)blockIdx.x * 2 + which) * A.D + c] = sum;
             }
         }
@@ -384,20 +696,25 @@ constexpr int kBackBlocks = 2;  // to an SM
 
 template <typename T, int VEC, int MODE, int N, bool BACK>
 int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
-    A.lanes = A.pieces < 32 ? A.pieces : 32;
+    A.lanes = (A.pieces + N - 1) / N;
     A.lanes_of = divisor(A.lanes);
-    // Tokens that share a forming of sines: four rows to a lane, fewer where that would leave SMs without
-    // work, and no more than 16 KB of sines.
-    const int rows = A.heads[0] + A.heads[1], at_once = kNormWarps * (32 / A.lanes);
-    long long per = 4ll * at_once / rows;
-    const long long spread_out = A.T / ((BACK ? kBackBlocks : 4) * (long long)num_sms());
-    const long long most = 16384 / (A.half * (long long)sizeof(float2));
+    // Tokens that share a forming of sines: eight rows to a lane, fewer where that would leave SMs without blocks (but a row
+    // to a lane), and no more than 16 KB of sines.
+    const int at_once = kNormWarps * (32 / A.lanes);
+    constexpr int kBlocks = kNormBlocks<BACK>;
+    static_assert(!BACK || kBlocks <= kBackBlocks, "the workspace");
+    const long long one = at_once / (A.heads[0] + A.heads[1]), spread_out = A.T / (kBlocks * (long long)num_sms());
+    long long per = 8 * one;
     per = per > spread_out ? spread_out : per;
+    per = per < one ? one : per;
+    const long long most = 16384 / (A.half * (long long)sizeof(float2));
     per = per > most ? most : per;
     A.per_chunk = (int)(per < 1 ? 1 : per);
+    A.sines_at_once = kNormThreads / A.half;  // half is 128 at most
     A.chunks = (A.T + A.per_chunk - 1) / A.per_chunk;
-    const size_t bytes = NormRoom<VEC, MODE>(A, BACK).all * sizeof(float);
-    const long long stay = (BACK ? kBackBlocks : 4) * (long long)num_sms();
+    const size_t bytes =
+        NormRoom<RowsOf<T, VEC, MODE, N, BACK>, MODE == kExchange>(A, BACK).all * sizeof(float);
+    const long long stay = kBlocks * (long long)num_sms();
     const int blocks = (int)(A.chunks < stay ? A.chunks : stay);
     auto kernel = normed_rotary_kernel<T, VEC, MODE, N, BACK>;
     if (bytes > 48 * 1024 &&
@@ -431,12 +748,10 @@ template <typename T, bool BACK> int dispatch_normed(NormArgs &A, bool whole, co
     }
     const bool paired = !A.interleaved && A.half % V == 0;
     A.pieces = paired ? A.half / V + (A.D - 2 * A.half) / V : A.D / V;
+    // Sixteen bf16 values (eight float32) to a lane, so that what a row costs besides them is shared.
     auto with = [&](auto mode) {
         constexpr int M = decltype(mode)::value;
-        if constexpr (kMostDim / V > 32) {
-            if (A.pieces > 32) return launch_normed<T, V, M, 2, BACK>(A, dw, stream);
-        }
-        return launch_normed<T, V, M, 1, BACK>(A, dw, stream);
+        return launch_normed<T, V, M, M == kPaired ? 1 : 2, BACK>(A, dw, stream);
     };
     if (paired) return with(std::integral_constant<int, kPaired>{});
     if (A.interleaved) return with(std::integral_constant<int, kInterleaved>{});
