@@ -47,14 +47,16 @@ struct AttnArgs {
     float unit;             // scale log2(e)
     float cap_in, cap_out;  // scale / cap, cap log2(e)
     float cap_inv;          // 1 / cap_out
-    float cap_poly[4];      // cap_out times the polynomial's coefficients
+    float near, mid;        // products up to which the polynomials reach
+    float cap_near[4];      // of a product's square
+    float cap_mid[8];       // of the square of a product times cap_in
     const float *slopes;    // [Hq] or null
     const int32_t *prefix;  // [n_seq] or null
 };
 
 // What a launch does to its scores, a template argument of the kernels: only scales them; lowers them by distance or
-// sees a prefix; caps them as well.
-constexpr int kPlain = 0, kBiased = 1, kCapped = 2;
+// sees a prefix; caps them as well; forward, caps them so low that no running maximum is needed (kMostBounded).
+constexpr int kPlain = 0, kBiased = 1, kCapped = 2, kBounded = 3;
 
 // Keys that every query of sequence `seq` (of klen keys) sees; seq is negative outside all sequences.
 template <int MOD> __device__ __forceinline__ int prefix_of(const AttnArgs &A, int seq, int klen) {
@@ -223,57 +225,103 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
 }
 
 // ---- changed scores ----
-// tanh on the FMA pipe: x (1 + u Q(u)), u = x^2, for |x| up to kCapReach, Q fitted to the least largest relative error
-// (6.5e-7: with scores around 20, 1.3e-5 of them, a hundredth of what rounding P to bf16 loses).  Scores beyond that,
-// which a cap keeps rare, take 1 - 2 / (1 + e^2x) in a loop over the tile in TMEM, small and away from the straight
-// code; which of the two a score takes depends on that score alone.
-constexpr float kCapReach = 0.75f;
-constexpr float kCapPoly[4] = {-0.33329668641090393f, 0.13268236815929413f, -0.0502779483795166f, 0.013105831108987331f};
+// A capped score in units of log2 is cap log2(e) tanh(x), x = scale / cap times the product.  The special-function unit
+// already has an exponential for every score, so tanh goes to the FMA pipe: x (1 + u Q(u)), u = x^2, the Q fitted to the
+// least largest relative error.  Up to |x| = 1/2, where a cap leaves nearly all scores, Q has three terms (6.4e-7: of
+// scores around 15 that is 1e-5, a hundredth of what rounding P to bf16 loses) and its coefficients hold the scale, five
+// packed operations for two scores; up to 3/2 seven terms (7.5e-7).  Beyond, 1 - 2 / (1 + e^2x), in a loop over the tile in TMEM,
+// small and away from the straight code.  A warp takes the same form for all scores of a tile, the one that its largest
+// needs (of those that its queries see: no other sequence's values change a bit).
+constexpr float kNear = 0.5f, kMid = 1.5f;
+constexpr float kNearPoly[3] = {-0.33328160643577576f, 0.13205359876155853f, -0.0447506345808506f};
+constexpr float kMidPoly[7] = {-0.3333057165145874f, 0.13300476968288422f, -0.05260444059967995f, 0.01905897632241249f,
+                               -0.005512249656021595f, 0.0010445077205076814f, -9.210196003550664e-05f};
 
-template <int N> __device__ __forceinline__ bool beyond_reach(const AttnArgs &A, const float *s) {
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
+// The largest magnitude of N products, of those whose bits are set (`bits_of(c)`: of products c .. c + 31).
+template <int N, typename Bits> __device__ __forceinline__ float largest(const float *s, Bits bits_of) {
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < N; c += 8) {
+    for (int c = 0; c < N; c += 32) {
+        const uint32_t m = bits_of(c);
+        if (m == 0xffffffffu) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = fmaxf(fmaxf(a[e], fabsf(s[c + e])), fabsf(s[c + e + 4]));
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = fmaxf(fmaxf(a[i], fabsf(s[c + e + i])), fabsf(s[c + e + i + 4]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) a[e & 3] = m & (1u << e) ? fmaxf(a[e & 3], fabsf(s[c + e])) : a[e & 3];
+        }
     }
-    const float most = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-    return __any_sync(0xffffffffu, __fmul_rn(most, A.cap_in) > kCapReach);
+    return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-// N products to capped scores in units of log2, all within reach.
-template <int N> __device__ __forceinline__ void cap_near(const AttnArgs &A, float *s) {
-    const float2 in = make_float2(A.cap_in, A.cap_in), one = make_float2(A.cap_out, A.cap_out);
+// A number for each of 32 keys in a row, linear in the key, as pairs: eight at a time, each from the eight before (so
+// that there are four pairs of constants, not sixteen to load).
+struct Line {
+    float2 v[4], step;
+    __device__ __forceinline__ Line(float2 along, float2 first) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fma2(along, make_float2(2 * j, 2 * j + 1), first);
+        step = mul2(along, twice(8.0f));
+    }
+    // Of keys c, c + 1, for even c that rise by two from 0.
+    __device__ __forceinline__ float2 at(int c) {
+        float2 &x = v[c / 2 % 4];
+        if (c >= 8) x = add2(x, step);
+        return x;
+    }
+};
+
+// s[c] w + bias(c), or without BIAS s[c] w, for N products within near reach.
+template <int N, bool BIAS> __device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float2 slope, float2 b) {
+    const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
+                 p3 = twice(A.cap_near[3]);
+#pragma unroll
+    for (int c0 = 0; c0 < N; c0 += 32) {
+        Line bias(slope, fma2(slope, twice(c0), b));
+#pragma unroll
+        for (int c = 0; c < (N < 32 ? N : 32); c += 2) {
+            const float2 x = make_float2(s[c0 + c], s[c0 + c + 1]), u = mul2(x, x);
+            const float2 w = fma2(fma2(fma2(p3, u, p2), u, p1), u, p0);
+            const float2 y = BIAS ? fma2(x, w, bias.at(c)) : mul2(x, w);
+            s[c0 + c] = y.x;
+            s[c0 + c + 1] = y.y;
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void cap_mid(const AttnArgs &A, float *s) {
+    const float2 in = twice(A.cap_in);
 #pragma unroll
     for (int c = 0; c < N; c += 2) {
         const float2 x = mul2(make_float2(s[c], s[c + 1]), in), u = mul2(x, x);
-        float2 w = fma2(make_float2(A.cap_poly[3], A.cap_poly[3]), u, make_float2(A.cap_poly[2], A.cap_poly[2]));
-        w = fma2(w, u, make_float2(A.cap_poly[1], A.cap_poly[1]));
-        w = fma2(w, u, make_float2(A.cap_poly[0], A.cap_poly[0]));
-        const float2 y = mul2(x, fma2(w, u, one));
+        float2 w = fma2(twice(A.cap_mid[7]), u, twice(A.cap_mid[6]));
+#pragma unroll
+        for (int k = 5; k >= 0; --k) w = fma2(w, u, twice(A.cap_mid[k]));
+        const float2 y = mul2(x, w);
         s[c] = y.x;
         s[c + 1] = y.y;
     }
 }
-
-// Whole warp: n columns of products at TMEM `ts` to capped scores, whatever their size.
+// Whole warp: n columns of products at TMEM `ts` to capped scores, whatever their size.  (Near 0 the far form would lose
+// what it subtracts from: there the polynomial.)
 __device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n) {
 #pragma unroll 1
     for (int c = 0; c < n; c += 16) {
-        float s[16];
+        float s[16], y[16];
         tmem_ld16(ts + c, s);
         tmem_wait_ld();
         pin<16>(s);
 #pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = s[e];
+        cap_near<16, false>(A, y, twice(0.0f), twice(0.0f));
+#pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float x = __fmul_rn(s[e], A.cap_in), u = __fmul_rn(x, x);
-            float w = fmaf(A.cap_poly[3], u, A.cap_poly[2]);
-            w = fmaf(w, u, A.cap_poly[1]);
-            w = fmaf(w, u, A.cap_poly[0]);
-            const float near = __fmul_rn(x, fmaf(w, u, A.cap_out));
             float r;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * (2.0f * kLog2e))));
-            s[e] = fabsf(x) <= kCapReach ? near : fmaf(-2.0f * A.cap_out, r, A.cap_out);
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(s[e] * A.cap_in * (2.0f * kLog2e))));
+            s[e] = fabsf(s[e]) <= A.near ? y[e] : fmaf(-2.0f * A.cap_out, r, A.cap_out);
         }
         tmem_st16(ts + c, reinterpret_cast<uint32_t *>(s));
     }
@@ -284,34 +332,98 @@ __device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n) 
 template <int MOD> struct RowScores {
     float slope = 0.0f;  // in units of log2
     int level = 0;       // the key at distance 0
+    bool live = false;
     __device__ RowScores() {}
-    __device__ RowScores(const AttnArgs &A, int head, int at, bool live) {
+    __device__ RowScores(const AttnArgs &A, int head, int at, bool is_live) {
         if constexpr (MOD != kPlain) {
             level = at;
+            live = is_live;
             if (A.slopes && live) slope = __ldg(A.slopes + head) * kLog2e;
         }
     }
-    template <int N> __device__ __forceinline__ void change(const AttnArgs &A, float *s, uint32_t ts, int k0) const {
-        if constexpr (MOD == kPlain) return;
-        if constexpr (MOD == kCapped) {
-            if (beyond_reach<N>(A, s)) {
-                cap_tmem(A, ts, N);
+    // Which side of the row's level N keys from k0 on are, for all of the warp's rows: 1 before it, -1 behind, 0 both.
+    template <int N> __device__ __forceinline__ int side_of(const AttnArgs &A, int k0) const {
+        if (!A.slopes) return 0;
+        if (__all_sync(0xffffffffu, k0 + N - 1 <= level)) return 1;
+        return __all_sync(0xffffffffu, k0 >= level) ? -1 : 0;
+    }
+    // Whole warp: products out of near reach to capped scores, or false, with nothing done.  `seen`: of the N, how many from
+    // the first on this row sees.
+    template <int N> __device__ __forceinline__ bool cap_far(const AttnArgs &A, float *s, uint32_t ts, int seen) const {
+        const int n = live ? seen : 0;
+        const float most = largest<N>(s, [&](int c) { return n >= c + 32 ? 0xffffffffu : bits(0, n - c); });
+        if (!__any_sync(0xffffffffu, most > A.near)) return false;
+        if (__any_sync(0xffffffffu, most > A.mid)) {
+            cap_tmem(A, ts, N);
 #pragma unroll
-                for (int c = 0; c < N; c += 32) tmem_ld32(ts + c, s + c);
-                tmem_wait_ld();
-                pin<N>(s);
-            } else {
-                cap_near<N>(A, s);
-            }
+            for (int c = 0; c < N; c += 32) tmem_ld32(ts + c, s + c);
+            tmem_wait_ld();
+            pin<N>(s);
         } else {
-#pragma unroll
-            for (int c = 0; c < N; ++c) s[c] *= A.unit;
+            cap_mid<N>(A, s);
         }
-        if (A.slopes) {
-            const float d = (float)(k0 - level);
+        return true;
+    }
+    // Products to scores that lack nothing, `capped` of them already are.
+    template <int N> __device__ __forceinline__ void finish(const AttnArgs &A, float *s, int k0, bool capped) const {
+        const int side = side_of<N>(A, k0);
+        // On one side the bias is linear in the key and takes part in the last operation.
+        const float2 along = twice(side < 0 ? -slope : slope), b = mul2(along, twice((float)(k0 - level)));
+        if (MOD >= kCapped && !capped) {
+            if (side != 0) cap_near<N, true>(A, s, along, b);
+            else cap_near<N, false>(A, s, along, b);
+            if (side != 0 || !A.slopes) return;
+        } else if (MOD == kBiased) {
+            const float2 unit = twice(A.unit);
+            if (side == 0) {
 #pragma unroll
-            for (int c = 0; c < N; ++c) s[c] = fmaf(-slope, fabsf(d + (float)c), s[c]);
+                for (int c = 0; c < N; c += 2) {
+                    const float2 y = mul2(make_float2(s[c], s[c + 1]), unit);
+                    s[c] = y.x;
+                    s[c + 1] = y.y;
+                }
+                if (!A.slopes) return;
+            } else {
+#pragma unroll
+                for (int c0 = 0; c0 < N; c0 += 32) {
+                    Line bias(along, fma2(along, twice(c0), b));
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 y = fma2(make_float2(s[c0 + c], s[c0 + c + 1]), unit, bias.at(c));
+                        s[c0 + c] = y.x;
+                        s[c0 + c + 1] = y.y;
+                    }
+                }
+                return;
+            }
+        } else if (!A.slopes) {
+            return;
         }
+#pragma unroll
+        for (int c0 = 0; c0 < N; c0 += 32) {
+            Line ahead(twice(1.0f), twice((float)(k0 + c0 - level)));
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                const float2 d = ahead.at(c);
+                s[c0 + c] = fmaf(-slope, fabsf(d.x), s[c0 + c]);
+                s[c0 + c + 1] = fmaf(-slope, fabsf(d.y), s[c0 + c + 1]);
+            }
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void change(const AttnArgs &A, float *s, uint32_t ts, int k0, int seen) const {
+        if constexpr (MOD == kPlain) return;
+        bool capped = false;
+        if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, seen);
+        finish<N>(A, s, k0, capped);
+    }
+    // Where scores lie within cap log2(e) of 0, their weights are numbers relative to that and a quarter of the cap more
+    // (2^-90 to 2^54 at the largest cap, as far from float32's and bf16's ends as sums and values can want), lowered by the
+    // least distance of a key that the row sees: no maximum has to be known before the first exponential.
+    __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
+        if (limit <= 0) return 0.25f * A.cap_out;
+        const int nearest = abs(min(max(level, 0), limit - 1) - level), farthest = max(abs(level), abs(limit - 1 - level));
+        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
     }
 };
 
@@ -320,8 +432,13 @@ template <int MOD> struct RowScores {
 // m = inf, where no score moves the reference, and so does not change how the other rows' weights round.
 struct RowState {
     float m, sum;
-    __device__ explicit RowState(bool live) : m(live ? -INFINITY : INFINITY), sum(0.0f) {}
+    __device__ explicit RowState(bool live, float from = -INFINITY) : m(live ? from : INFINITY), sum(0.0f) {}
 };
+template <int MOD>
+__device__ __forceinline__ RowState first_state(const AttnArgs &A, const RowScores<MOD> &scores, bool live, int limit) {
+    if constexpr (MOD == kBounded) return RowState(live, scores.reference(A, limit));
+    return RowState(live);
+}
 
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
 // the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
@@ -387,14 +504,22 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         for (int c = 0; c < KEYS; c += 32) tmem_ld32(ts + c, s + c);
         tmem_wait_ld();
         pin<KEYS>(s);
-        scores.template change<KEYS>(A, s, ts, k0);
+        bool capped = false;
+        if constexpr (MOD == kBounded) capped = scores.template cap_far<KEYS>(A, s, ts, KEYS);
+        else scores.template change<KEYS>(A, s, ts, k0, KEYS);
         loaded();
-        const float mx = max_of<KEYS>(s);
-        if (!settle()) return false;
-        move_reference<DP>(r, to, mx, first, sc);
+        if constexpr (MOD == kBounded) {
+            if (!settle()) return false;
+        } else {
+            const float mx = max_of<KEYS>(s);
+            if (!settle()) return false;
+            move_reference<DP>(r, to, mx, first, sc);
+        }
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if constexpr (MOD == kBounded)
+                scores.template finish<KEYS / 2>(A, s + h * (KEYS / 2), k0 + h * (KEYS / 2), capped);
             uint32_t p[KEYS / 4];
             exp_pack<KEYS / 2, true, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
             tmem_st32(tp + h * 32, p);
@@ -404,21 +529,24 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
     } else {
         float mx = -INFINITY;
         float s[32];
+        if (MOD == kBounded && !settle()) return false;
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
+        for (int c = 0; c < cols && MOD != kBounded; c += 32) {
             tmem_ld32(ts + c, s);
             tmem_wait_ld();
             pin<32>(s);
             if constexpr (MOD != kPlain) {
-                scores.template change<32>(A, s, ts + c, k0 + c);
+                scores.template change<32>(A, s, ts + c, k0 + c, seen - c);
                 tmem_st32(ts + c, reinterpret_cast<uint32_t *>(s));
             }
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
         if constexpr (MOD != kPlain) tmem_wait_st();
-        if (!settle()) return false;
-        move_reference<DP>(r, to, mx, first, sc);
+        if constexpr (MOD != kBounded) {
+            if (!settle()) return false;
+            move_reference<DP>(r, to, mx, first, sc);
+        }
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
         // P of 32 keys takes 16 columns: over S it stays behind what has been read.
 #pragma unroll 1
@@ -426,6 +554,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
             tmem_ld32(ts + c, s);
             tmem_wait_ld();
             pin<32>(s);
+            if constexpr (MOD == kBounded) scores.template change<32>(A, s, ts + c, k0 + c, seen - c);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[e] = c + e < seen ? s[e] : -INFINITY;
             uint32_t p[16];
@@ -452,7 +581,7 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     if (cols > 32) tmem_ld32(ts + 32, s + 32);
     tmem_wait_ld();
     pin<64>(s);
-    scores.template change<64>(A, s, ts, k0);  // (columns past `cols` hold anything, and are masked)
+    scores.template change<64>(A, s, ts, k0, seen);  // (columns past `cols` hold anything, and are masked)
     if (!all) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -461,7 +590,7 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    if constexpr (MOD != kBounded) move_reference<DP>(r, to, max_of<64>(s), first, sc);
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
@@ -1004,7 +1133,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             // Keys that every row of the tile sees (rows past the last token do not count).
             const int all_see = A.causal ? max(min(klen, tok_first + 1 + klen - q.len), prefix) : klen;
             const RowScores<MOD> scores(A, qhead + row_head(A, row), tok + klen - q.len, live);
-            RowState rs(live);
+            RowState rs = first_state<MOD>(A, scores, live, limit);
             const int n = r.cnt[t];
             bool ok = true;
 #pragma unroll 1
@@ -1264,7 +1393,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             A.causal ? max(min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)), it.prefix) : it.klen;
         const int all_see = A.causal ? max(min(it.klen, it.tok0 + 1 + it.klen - it.qlen), it.prefix) : it.klen;
         const RowScores<MOD> row_scores(A, it.qhead + row_head(A, row), it.tok0 + row_tok + it.klen - it.qlen, live);
-        RowState rs(live);
+        RowState rs = first_state<MOD>(A, row_scores, live, limit);
 #pragma unroll 1
         for (int i = 0; i < it.n; ++i) {
             const int t = g + i;
@@ -1758,20 +1887,25 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         pin<32>(s);
         pin<32>(d);
         if constexpr (MOD == kCapped) {
-            if (beyond_reach<32>(A, s)) {
-                cap_tmem(A, ts, 32);
-                tmem_ld32(ts, s);
-                tmem_wait_ld();
-                pin<32>(s);
+            const float most = largest<32>(s, [&](int) { return mask ? seen : 0xffffffffu; });
+            if (__any_sync(0xffffffffu, most > A.near)) {
+                if (__any_sync(0xffffffffu, most > A.mid)) {
+                    cap_tmem(A, ts, 32);
+                    tmem_ld32(ts, s);
+                    tmem_wait_ld();
+                    pin<32>(s);
+                } else {
+                    cap_mid<32>(A, s);
+                }
             } else {
-                cap_near<32>(A, s);
+                cap_near<32, false>(A, s, twice(0.0f), twice(0.0f));
             }
         }
         // DQ: from the key that the row is level with to the first of this thread's columns.
-        const float ahead = DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level);
+        Line ahead(twice(1.0f), twice(DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level)));
         uint32_t ps[16], pd[16];
         // Straight code in either case: the exponentials' latencies overlap.
-        auto weights = [&](auto masked) {
+        auto weights = [&, ahead](auto masked) mutable {
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
             float4 nl, nd;
@@ -1787,15 +1921,18 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                     if (DKV) {
                         const float4 m = *reinterpret_cast<const float4 *>(&sh.slope2[st][c0 + c]);
                         const float4 at = *reinterpret_cast<const float4 *>(&sh.level[st][c0 + c]);
-                        nl.x = fmaf(-m.x, fabsf(at.x - (float)row), nl.x);
-                        nl.y = fmaf(-m.y, fabsf(at.y - (float)row), nl.y);
-                        nl.z = fmaf(-m.z, fabsf(at.z - (float)row), nl.z);
-                        nl.w = fmaf(-m.w, fabsf(at.w - (float)row), nl.w);
+                        const float2 d01 = add2(make_float2(at.x, at.y), twice(-(float)row));
+                        const float2 d23 = add2(make_float2(at.z, at.w), twice(-(float)row));
+                        nl.x = fmaf(-m.x, fabsf(d01.x), nl.x);
+                        nl.y = fmaf(-m.y, fabsf(d01.y), nl.y);
+                        nl.z = fmaf(-m.z, fabsf(d23.x), nl.z);
+                        nl.w = fmaf(-m.w, fabsf(d23.y), nl.w);
                     } else {
-                        nl.x = fmaf(-scores.slope, fabsf(ahead + (float)c), nl.x);
-                        nl.y = fmaf(-scores.slope, fabsf(ahead + (float)(c + 1)), nl.y);
-                        nl.z = fmaf(-scores.slope, fabsf(ahead + (float)(c + 2)), nl.z);
-                        nl.w = fmaf(-scores.slope, fabsf(ahead + (float)(c + 3)), nl.w);
+                        const float2 d01 = ahead.at(c), d23 = ahead.at(c + 2);
+                        nl.x = fmaf(-scores.slope, fabsf(d01.x), nl.x);
+                        nl.y = fmaf(-scores.slope, fabsf(d01.y), nl.y);
+                        nl.z = fmaf(-scores.slope, fabsf(d23.x), nl.z);
+                        nl.w = fmaf(-scores.slope, fabsf(d23.y), nl.w);
                     }
                 }
             }
@@ -2362,10 +2499,10 @@ struct ScoreChange {
 
 int check_change(const ScoreChange &m, float scale) {
     if (m.cap != 0.0f) {
-        // (In units of the cap scores are products times scale / cap, which has to be a number.)
-        if (!(m.cap >= 0x1p-64f && m.cap <= 0x1p64f)) return RFDETR_ERR_SHAPE;
+        // (The polynomials' coefficients hold up to the sixth power of scale / cap.)
         const float in = scale / m.cap;
-        if (!(in >= FLT_MIN && in <= FLT_MAX)) return RFDETR_ERR_SHAPE;
+        if (!(m.cap > 0.0f && in >= 0x1p-20f && in <= 0x1p20f)) return RFDETR_ERR_SHAPE;
+        if (!(m.cap >= 0x1p-64f && m.cap <= 0x1p64f)) return RFDETR_ERR_SHAPE;
     }
     return aligned(m.slopes, 4) && aligned(m.prefix, 4) ? RFDETR_OK : RFDETR_ERR_ALIGN;
 }
@@ -2378,12 +2515,24 @@ void set_change(AttnArgs &A, const ScoreChange &m) {
     A.cap_in = A.scale / m.cap;
     A.cap_out = m.cap * kLog2e;
     A.cap_inv = 1.0f / A.cap_out;
-    for (int k = 0; k < 4; ++k) A.cap_poly[k] = A.cap_out * kCapPoly[k];
+    A.near = kNear / A.cap_in;
+    A.mid = kMid / A.cap_in;
+    const double in2 = (double)A.cap_in * A.cap_in;
+    A.cap_near[0] = A.unit;
+    A.cap_mid[0] = A.cap_out;
+    double power = A.unit;
+    for (int k = 0; k < 3; ++k) A.cap_near[k + 1] = (float)((power *= in2) * kNearPoly[k]);
+    for (int k = 0; k < 7; ++k) A.cap_mid[k + 1] = A.cap_out * kMidPoly[k];
 }
 
+// Caps (in units of log2) up to which the forward kernels need no running maximum.
+constexpr float kMostBounded = 72.5f;
+
 // Calls f with the head's padded size and what is done to scores, as types.
-template <typename F> int with_kernels(int64_t head_dim, const ScoreChange &m, F f) {
+template <bool FORWARD, typename F> int with_kernels(int64_t head_dim, const ScoreChange &m, F f) {
     auto with = [&](auto dp) {
+        if constexpr (FORWARD)
+            if (m.cap != 0.0f && m.cap * kLog2e <= kMostBounded) return f(dp, std::integral_constant<int, kBounded>{});
         if (m.cap != 0.0f) return f(dp, std::integral_constant<int, kCapped>{});
         if (m.any()) return f(dp, std::integral_constant<int, kBiased>{});
         return f(dp, std::integral_constant<int, kPlain>{});
@@ -2454,7 +2603,7 @@ extern "C" int rfdetr_packed_attention_scored(void *stream, const void *query, i
         f.part_lse = f.part + (size_t)p.blocks * f.part_rows * A.D;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return with_kernels(head_dim, change, [&](auto dp, auto mod) {
+    return with_kernels<true>(head_dim, change, [&](auto dp, auto mod) {
         return launch_forward<decltype(dp)::value, decltype(mod)::value>(A, p, q, k, v, f, s);
     });
 }
@@ -2517,7 +2666,7 @@ extern "C" int rfdetr_packed_attention_scored_backward(
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     bf16 *dq = static_cast<bf16 *>(grad_query), *dk = static_cast<bf16 *>(grad_key),
          *dv = static_cast<bf16 *>(grad_value);
-    return with_kernels(head_dim, change, [&](auto dp, auto mod) {
+    return with_kernels<false>(head_dim, change, [&](auto dp, auto mod) {
         return launch_backward<decltype(dp)::value, decltype(mod)::value>(A, q, k, v, g, f, dq, dk, dv, s);
     });
 }
