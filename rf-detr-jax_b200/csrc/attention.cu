@@ -224,6 +224,27 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+// 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
+// the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
+// with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
+template <int N, bool POLY, int MOD>
+__device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
+    const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
+#pragma unroll
+    for (int c = 0; c < N / 2; ++c) {
+        float2 x = MOD == kPlain ? fma2(make_float2(s[2 * c], s[2 * c + 1]), sc2, ref2)
+                                 : add2(make_float2(s[2 * c], s[2 * c + 1]), ref2);
+        if (POLY && (c % 8 == 4)) {
+            x = exp2_poly(x);
+        } else {
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
+        }
+        acc[c & 1] = add2(acc[c & 1], x);
+        p[c] = pack_bf16(x.x, x.y);
+    }
+}
+
 // ---- changed scores ----
 // A capped score in units of log2 is cap log2(e) tanh(x), x = scale / cap times the product.  The special-function unit
 // already has an exponential for every score, so tanh goes to the FMA pipe: x (1 + u Q(u)), u = x^2, the Q fitted to the
@@ -249,7 +270,8 @@ template <int N, typename Bits> __device__ __forceinline__ float largest(const f
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = fmaxf(fmaxf(a[i], fabsf(s[c + e + i])), fabsf(s[c + e + i + 4]));
+                for (int i = 0; i < 4; ++i)
+                    asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(a[i]) : "f"(s[c + e + i]), "f"(s[c + e + i + 4]));
         } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) a[e & 3] = m & (1u << e) ? fmaxf(a[e & 3], fabsf(s[c + e])) : a[e & 3];
@@ -292,6 +314,28 @@ template <int N, bool BIAS> __device__ __forceinline__ void cap_near(const AttnA
         }
     }
 }
+// 2^(s[c] w + bias(c)) of N products within near reach, packed to bf16; adds them to acc[2].  The reference comes with the
+// bias: one run through the values, in which the special-function unit's exponentials and the polynomials overlap.
+template <int N, bool LINE>
+__device__ __forceinline__ void cap_near_exp(const AttnArgs &A, const float *s, float2 slope, float2 b, uint32_t *p,
+                                             float2 *acc) {
+    const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
+                 p3 = twice(A.cap_near[3]);
+#pragma unroll
+    for (int c0 = 0; c0 < N; c0 += 32) {
+        Line bias(slope, fma2(slope, twice(c0), b));
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            const float2 x = make_float2(s[c0 + c], s[c0 + c + 1]), u = mul2(x, x);
+            const float2 w = fma2(fma2(fma2(p3, u, p2), u, p1), u, p0);
+            float2 y = fma2(x, w, LINE ? bias.at(c) : b);
+            y.x = exp2_fast(y.x);
+            y.y = exp2_fast(y.y);
+            acc[c / 2 & 1] = add2(acc[c / 2 & 1], y);
+            p[(c0 + c) / 2] = pack_bf16(y.x, y.y);
+        }
+    }
+}
 template <int N> __device__ __forceinline__ void cap_mid(const AttnArgs &A, float *s) {
     const float2 in = twice(A.cap_in);
 #pragma unroll
@@ -305,25 +349,35 @@ template <int N> __device__ __forceinline__ void cap_mid(const AttnArgs &A, floa
         s[c + 1] = y.y;
     }
 }
-// Whole warp: n columns of products at TMEM `ts` to capped scores, whatever their size.  (Near 0 the far form would lose
-// what it subtracts from: there the polynomial.)
-__device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n) {
+// Whole warp: n columns of products at TMEM `ts` to capped scores; `far`: some are out of the middle reach.  (Near 0 the far
+// form would lose what it subtracts from: there the polynomial.)
+template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n, bool far) {
 #pragma unroll 1
-    for (int c = 0; c < n; c += 16) {
-        float s[16], y[16];
-        tmem_ld16(ts + c, s);
+    for (int c = 0; c < n; c += STEP) {
+        float s[STEP];
+        if constexpr (STEP == 32) tmem_ld32(ts + c, s);
+        else tmem_ld16(ts + c, s);
         tmem_wait_ld();
-        pin<16>(s);
+        pin<STEP>(s);
+        if (!far) {
+            cap_mid<STEP>(A, s);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = s[e];
-        cap_near<16, false>(A, y, twice(0.0f), twice(0.0f));
+            for (int e0 = 0; e0 < STEP; e0 += 8) {
+                float y[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float r;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(s[e] * A.cap_in * (2.0f * kLog2e))));
-            s[e] = fabsf(s[e]) <= A.near ? y[e] : fmaf(-2.0f * A.cap_out, r, A.cap_out);
+                for (int e = 0; e < 8; ++e) y[e] = s[e0 + e];
+                cap_near<8, false>(A, y, twice(0.0f), twice(0.0f));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float &x = s[e0 + e], r;
+                    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * A.cap_in * (2.0f * kLog2e))));
+                    x = fabsf(x) <= A.near ? y[e] : fmaf(-2.0f * A.cap_out, r, A.cap_out);
+                }
+            }
         }
-        tmem_st16(ts + c, reinterpret_cast<uint32_t *>(s));
+        if constexpr (STEP == 32) tmem_st32(ts + c, reinterpret_cast<uint32_t *>(s));
+        else tmem_st16(ts + c, reinterpret_cast<uint32_t *>(s));
     }
     tmem_wait_st();
 }
@@ -352,16 +406,12 @@ template <int MOD> struct RowScores {
     template <int N> __device__ __forceinline__ bool cap_far(const AttnArgs &A, float *s, uint32_t ts, int seen) const {
         const int n = live ? seen : 0;
         const float most = largest<N>(s, [&](int c) { return n >= c + 32 ? 0xffffffffu : bits(0, n - c); });
-        if (!__any_sync(0xffffffffu, most > A.near)) return false;
-        if (__any_sync(0xffffffffu, most > A.mid)) {
-            cap_tmem(A, ts, N);
+        if (__builtin_expect(!__any_sync(0xffffffffu, most > A.near), 1)) return false;
+        cap_tmem<32>(A, ts, N, __any_sync(0xffffffffu, most > A.mid));
 #pragma unroll
-            for (int c = 0; c < N; c += 32) tmem_ld32(ts + c, s + c);
-            tmem_wait_ld();
-            pin<N>(s);
-        } else {
-            cap_mid<N>(A, s);
-        }
+        for (int c = 0; c < N; c += 32) tmem_ld32(ts + c, s + c);
+        tmem_wait_ld();
+        pin<N>(s);
         return true;
     }
     // Products to scores that lack nothing, `capped` of them already are.
@@ -410,6 +460,23 @@ template <int MOD> struct RowScores {
             }
         }
     }
+    // kBounded: weights relative to 2^-ref of N scores that are all seen, from products or, `capped`, capped scores.
+    template <int N>
+    __device__ __forceinline__ void weights(const AttnArgs &A, float *s, int k0, bool capped, float ref, uint32_t *p,
+                                            float2 *acc) const {
+        const int side = side_of<N>(A, k0);
+        if (!capped && (side != 0 || !A.slopes)) {
+            if (side != 0) {
+                const float along = side < 0 ? -slope : slope;
+                cap_near_exp<N, true>(A, s, twice(along), twice(fmaf(along, (float)(k0 - level), ref)), p, acc);
+            } else {
+                cap_near_exp<N, false>(A, s, twice(0.0f), twice(ref), p, acc);
+            }
+            return;
+        }
+        finish<N>(A, s, k0, capped);
+        exp_pack<N, false, MOD>(s, 1.0f, ref, p, acc);
+    }
     template <int N>
     __device__ __forceinline__ void change(const AttnArgs &A, float *s, uint32_t ts, int k0, int seen) const {
         if constexpr (MOD == kPlain) return;
@@ -438,27 +505,6 @@ template <int MOD>
 __device__ __forceinline__ RowState first_state(const AttnArgs &A, const RowScores<MOD> &scores, bool live, int limit) {
     if constexpr (MOD == kBounded) return RowState(live, scores.reference(A, limit));
     return RowState(live);
-}
-
-// 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
-// the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
-// with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
-template <int N, bool POLY, int MOD>
-__device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
-    const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
-#pragma unroll
-    for (int c = 0; c < N / 2; ++c) {
-        float2 x = MOD == kPlain ? fma2(make_float2(s[2 * c], s[2 * c + 1]), sc2, ref2)
-                                 : add2(make_float2(s[2 * c], s[2 * c + 1]), ref2);
-        if (POLY && (c % 8 == 4)) {
-            x = exp2_poly(x);
-        } else {
-            x.x = exp2_fast(x.x);
-            x.y = exp2_fast(x.y);
-        }
-        acc[c & 1] = add2(acc[c & 1], x);
-        p[c] = pack_bf16(x.x, x.y);
-    }
 }
 
 // Whole warp: moves the reference to the new maximum where some live row's grew far enough, and O and the
@@ -518,10 +564,12 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if constexpr (MOD == kBounded)
-                scores.template finish<KEYS / 2>(A, s + h * (KEYS / 2), k0 + h * (KEYS / 2), capped);
             uint32_t p[KEYS / 4];
-            exp_pack<KEYS / 2, true, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
+            if constexpr (MOD == kBounded) {
+                scores.template weights<KEYS / 2>(A, s + h * (KEYS / 2), k0 + h * (KEYS / 2), capped, ref, p, acc);
+            } else {
+                exp_pack<KEYS / 2, true, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
+            }
             tmem_st32(tp + h * 32, p);
             tmem_wait_st();
             written(h);
@@ -581,7 +629,13 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     if (cols > 32) tmem_ld32(ts + 32, s + 32);
     tmem_wait_ld();
     pin<64>(s);
-    scores.template change<64>(A, s, ts, k0, seen);  // (columns past `cols` hold anything, and are masked)
+    bool capped = false;
+    if constexpr (MOD == kBounded) capped = scores.template cap_far<64>(A, s, ts, seen);  // (past `cols` there is anything)
+    if constexpr (MOD == kBounded) {
+        if (!all) scores.template finish<64>(A, s, k0, capped);
+    } else {
+        scores.template change<64>(A, s, ts, k0, seen);
+    }
     if (!all) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -595,7 +649,8 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
     if (all) {
-        exp_pack<64, false, MOD>(s, sc, ref, p, acc);
+        if constexpr (MOD == kBounded) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
+        else exp_pack<64, false, MOD>(s, sc, ref, p, acc);
         tmem_st32(ts, p);
     } else {
         exp_pack<32, false, MOD>(s, sc, ref, p, acc);
@@ -1886,18 +1941,16 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         tmem_wait_ld();
         pin<32>(s);
         pin<32>(d);
+        bool near = false;
         if constexpr (MOD == kCapped) {
             const float most = largest<32>(s, [&](int) { return mask ? seen : 0xffffffffu; });
-            if (__any_sync(0xffffffffu, most > A.near)) {
-                if (__any_sync(0xffffffffu, most > A.mid)) {
-                    cap_tmem(A, ts, 32);
-                    tmem_ld32(ts, s);
-                    tmem_wait_ld();
-                    pin<32>(s);
-                } else {
-                    cap_mid<32>(A, s);
-                }
-            } else {
+            near = __builtin_expect(!__any_sync(0xffffffffu, most > A.near), 1);
+            if (!near) {
+                cap_tmem<16>(A, ts, 32, __any_sync(0xffffffffu, most > A.mid));
+                tmem_ld32(ts, s);
+                tmem_wait_ld();
+                pin<32>(s);
+            } else if (mask) {
                 cap_near<32, false>(A, s, twice(0.0f), twice(0.0f));
             }
         }
@@ -1905,7 +1958,7 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         Line ahead(twice(1.0f), twice(DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level)));
         uint32_t ps[16], pd[16];
         // Straight code in either case: the exponentials' latencies overlap.
-        auto weights = [&, ahead](auto masked) mutable {
+        auto weights = [&, ahead](auto masked, auto products) mutable {
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
             float4 nl, nd;
@@ -1936,7 +1989,14 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                     }
                 }
             }
-            const float2 s01 = make_float2(s[c], s[c + 1]), s23 = make_float2(s[c + 2], s[c + 3]);
+            float2 s01 = make_float2(s[c], s[c + 1]), s23 = make_float2(s[c + 2], s[c + 3]);
+            if constexpr (MOD == kCapped && products) {  // within near reach, to scores
+                const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
+                             p3 = twice(A.cap_near[3]);
+                const float2 u01 = mul2(s01, s01), u23 = mul2(s23, s23);
+                s01 = mul2(s01, fma2(fma2(fma2(p3, u01, p2), u01, p1), u01, p0));
+                s23 = mul2(s23, fma2(fma2(fma2(p3, u23, p2), u23, p1), u23, p0));
+            }
             const float2 a = MOD == kCapped ? add2(s01, make_float2(nl.x, nl.y)) : fma2(s01, sc2, make_float2(nl.x, nl.y));
             const float2 b = MOD == kCapped ? add2(s23, make_float2(nl.z, nl.w)) : fma2(s23, sc2, make_float2(nl.z, nl.w));
             float p[4] = {exp2_fast(a.x), exp2_fast(a.y), exp2_fast(b.x), exp2_fast(b.y)};
@@ -1969,9 +2029,11 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             pd[c / 2 + 1] = pack_bf16(ds[2], ds[3]);
         }
         };
-        if (!mask) weights(std::integral_constant<int, 0>{});
-        else if (!__any_sync(0xffffffffu, one)) weights(std::integral_constant<int, 1>{});
-        else weights(std::integral_constant<int, 2>{});
+        using std::integral_constant;
+        if (MOD == kCapped && near && !mask) weights(integral_constant<int, 0>{}, integral_constant<int, 1>{});
+        else if (!mask) weights(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+        else if (!__any_sync(0xffffffffu, one)) weights(integral_constant<int, 1>{}, integral_constant<int, 0>{});
+        else weights(integral_constant<int, 2>{}, integral_constant<int, 0>{});
         // Over this half of A and B: the other half may not have been read yet.
         if (DKV) tmem_st16(ts, ps);
         tmem_st16(ts + kWalk, pd);
