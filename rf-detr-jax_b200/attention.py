@@ -146,8 +146,8 @@ class ScoredAttentionFunction(torch.autograd.Function):
 def _score_change(score_cap, distance_slopes, prefix, heads, sequences, causal, scale):
     """Checked ``(cap, slopes, prefix)``; cap 0 for none."""
     cap = 0.0 if score_cap is None else float(score_cap)
-    if score_cap is not None and not (2.0 ** -64 <= cap <= 2.0 ** 64 and 2.0 ** -19 <= scale / cap <= 2.0 ** 19):
-        raise ValueError(f"score_cap must be positive and within 2^19 of scale either way, got {score_cap} with {scale}")
+    if score_cap is not None and not (2.0 ** -39 <= cap <= 2.0 ** 39 and 2.0 ** -19 <= scale / cap <= 2.0 ** 19):
+        raise ValueError(f"score_cap must be positive, 2^-39 to 2^39 and within 2^19 of scale either way, got {score_cap} with {scale}")
     if distance_slopes is not None:
         if distance_slopes.shape != (heads,) or distance_slopes.dtype != torch.float32:
             raise ValueError(f"distance_slopes must be float32 [{heads}], got {distance_slopes.dtype} "

@@ -46,7 +46,7 @@ struct AttnArgs {
     // Of changed scores (kBiased, kCapped) alone.
     float unit;             // scale log2(e)
     float cap_in, cap_out;  // scale / cap, cap log2(e)
-    float cap_inv;          // 1 / cap_out
+    float cap_back;         // -1 / cap_out^2
     float near, mid;        // products up to which the polynomials reach
     float cap_near[4];      // of a product's square
     float cap_mid[8];       // of the square of a product times cap_in
@@ -2000,9 +2000,17 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
             const float2 a = MOD == kCapped ? add2(s01, make_float2(nl.x, nl.y)) : fma2(s01, sc2, make_float2(nl.x, nl.y));
             const float2 b = MOD == kCapped ? add2(s23, make_float2(nl.z, nl.w)) : fma2(s23, sc2, make_float2(nl.z, nl.w));
             float p[4] = {exp2_fast(a.x), exp2_fast(a.y), exp2_fast(b.x), exp2_fast(b.y)};
-            const float2 e = mul2(make_float2(p[0], p[1]), add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
-            const float2 f =
-                mul2(make_float2(p[2], p[3]), add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
+            float2 e = mul2(make_float2(p[0], p[1]), add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
+            float2 f = mul2(make_float2(p[2], p[3]), add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
+            float2 turn01 = twice(1.0f), turn23 = turn01;  // 1 - (S' / cap)^2
+            if constexpr (MOD == kCapped) {
+                turn01 = fma2(mul2(s01, s01), twice(A.cap_back), turn01);
+                turn23 = fma2(mul2(s23, s23), twice(A.cap_back), turn23);
+                if constexpr (masked == 0) {
+                    e = mul2(e, turn01);
+                    f = mul2(f, turn23);
+                }
+            }
             float ds[4] = {e.x, e.y, f.x, f.y};
             if (masked) {
 #pragma unroll
@@ -2013,14 +2021,11 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                     if (masked == 2 && (one & bit)) ds[k] = DKV ? sh.one_ds[st][c0 + c + k] : row_od;
                 }
             }
-            if constexpr (MOD == kCapped) {  // times 1 - (S' / cap)^2
-                const float2 inv = make_float2(A.cap_inv, A.cap_inv), minus = make_float2(-1.0f, -1.0f);
-                const float2 t01 = mul2(s01, inv), t23 = mul2(s23, inv), one2 = make_float2(1.0f, 1.0f);
-                const float2 f01 = fma2(mul2(t01, minus), t01, one2), f23 = fma2(mul2(t23, minus), t23, one2);
+            if constexpr (MOD == kCapped && masked != 0) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float f = k == 0 ? f01.x : k == 1 ? f01.y : k == 2 ? f23.x : f23.y;
-                    ds[k] = !masked || (seen & (1u << (c + k))) ? ds[k] * f : 0.0f;
+                    const float t = k == 0 ? turn01.x : k == 1 ? turn01.y : k == 2 ? turn23.x : turn23.y;
+                    ds[k] = seen & (1u << (c + k)) ? ds[k] * t : 0.0f;
                 }
             }
             ps[c / 2] = pack_bf16(p[0], p[1]);
@@ -2564,7 +2569,7 @@ int check_change(const ScoreChange &m, float scale) {
         // (The polynomials' coefficients hold up to the sixth power of scale / cap.)
         const float in = scale / m.cap;
         if (!(m.cap > 0.0f && in >= 0x1p-20f && in <= 0x1p20f)) return RFDETR_ERR_SHAPE;
-        if (!(m.cap >= 0x1p-64f && m.cap <= 0x1p64f)) return RFDETR_ERR_SHAPE;
+        if (!(m.cap >= 0x1p-40f && m.cap <= 0x1p40f)) return RFDETR_ERR_SHAPE;
     }
     return aligned(m.slopes, 4) && aligned(m.prefix, 4) ? RFDETR_OK : RFDETR_ERR_ALIGN;
 }
@@ -2576,7 +2581,7 @@ void set_change(AttnArgs &A, const ScoreChange &m) {
     if (m.cap == 0.0f) return;
     A.cap_in = A.scale / m.cap;
     A.cap_out = m.cap * kLog2e;
-    A.cap_inv = 1.0f / A.cap_out;
+    A.cap_back = (float)(-1.0 / ((double)A.cap_out * A.cap_out));
     A.near = kNear / A.cap_in;
     A.mid = kMid / A.cap_in;
     const double in2 = (double)A.cap_in * A.cap_in;
