@@ -38,7 +38,8 @@ _lib = ctypes.cdll.LoadLibrary(os.environ.get("RFDETR_FFI_LIB", os.path.join(_HE
 HANDLERS = ("RfdetrMsdaFwd", "RfdetrMsdaBwd", "RfdetrMsdaBwdNoAlloc", "RfdetrMsdaPrologue", "RfdetrMsdaPrologueBwd",
             "RfdetrTopkSelect", "RfdetrSelectRows", "RfdetrMatchCost", "RfdetrLsapBatched", "RfdetrMatchStacked",
             "RfdetrSetLosses", "RfdetrPackedAttention", "RfdetrPackedAttentionBwd", "RfdetrAxialRotary",
-            "RfdetrNormedRotary", "RfdetrNormedRotaryBwd", "RfdetrClipGradients")
+            "RfdetrNormedRotary", "RfdetrNormedRotaryBwd", "RfdetrClipGradients", "RfdetrScoredAttention",
+            "RfdetrScoredAttentionBwd")
 for _name in HANDLERS:
     jax.ffi.register_ffi_target(_name, jax.ffi.pycapsule(getattr(_lib, _name)), platform="CUDA")
 
@@ -283,6 +284,52 @@ def _packed_attention_bwd(causal, scale, residuals, g):
 
 
 packed_attention.defvjp(_packed_attention_fwd, _packed_attention_bwd)
+
+
+def _change(distance_slopes, prefix):
+    """Absent ones as empty buffers."""
+    return (jnp.zeros((0,), jnp.float32) if distance_slopes is None else distance_slopes.astype(jnp.float32),
+            jnp.zeros((0,), jnp.int32) if prefix is None else _offsets(prefix))
+
+
+@functools.partial(jax.custom_vjp, nondiff_argnums=(7, 8, 9))
+def scored_attention(query, key, value, offsets, key_offsets, distance_slopes=None, prefix=None, causal=False, scale=None,
+                     score_cap=None):
+    """:func:`packed_attention` whose scores are capped, lowered by ``slope * distance`` or see a prefix."""
+    out, _, lse = _scored_attention_call(query, key, value, offsets, key_offsets, distance_slopes, prefix, causal,
+                                         scale, score_cap, False)
+    return out, lse
+
+
+def _scored_attention_call(query, key, value, offsets, key_offsets, distance_slopes, prefix, causal, scale, score_cap,
+                           keep_low):
+    low = query.shape if keep_low else (0, *query.shape[1:])
+    outs = (jax.ShapeDtypeStruct(query.shape, query.dtype), jax.ShapeDtypeStruct(low, query.dtype),
+            jax.ShapeDtypeStruct((query.shape[1], query.shape[0]), jnp.float32))
+    return jax.ffi.ffi_call("RfdetrScoredAttention", outs)(
+        query, key, value, _offsets(offsets), _offsets(key_offsets), *_change(distance_slopes, prefix),
+        causal=np.int32(1 if causal else 0), scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale),
+        score_cap=np.float32(0.0 if score_cap is None else score_cap))
+
+
+def _scored_attention_fwd(query, key, value, offsets, key_offsets, distance_slopes, prefix, causal, scale, score_cap):
+    out, low, lse = _scored_attention_call(query, key, value, offsets, key_offsets, distance_slopes, prefix, causal,
+                                           scale, score_cap, True)
+    return (out, lse), (query, key, value, offsets, key_offsets, distance_slopes, prefix, out, low, lse)
+
+
+def _scored_attention_bwd(causal, scale, score_cap, residuals, g):
+    query, key, value, offsets, key_offsets, distance_slopes, prefix, out, low, lse = residuals
+    shapes = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key, value))
+    grads = jax.ffi.ffi_call("RfdetrScoredAttentionBwd", shapes)(
+        query, key, value, _offsets(offsets), _offsets(key_offsets), *_change(distance_slopes, prefix), out, low, lse,
+        g[0].astype(out.dtype), g[1].astype(jnp.float32), causal=np.int32(1 if causal else 0),
+        scale=np.float32(query.shape[-1] ** -0.5 if scale is None else scale),
+        score_cap=np.float32(0.0 if score_cap is None else score_cap))
+    return *grads, None, None, None, None
+
+
+scored_attention.defvjp(_scored_attention_fwd, _scored_attention_bwd)
 
 
 @functools.partial(jax.custom_vjp, nondiff_argnums=(4, 5))

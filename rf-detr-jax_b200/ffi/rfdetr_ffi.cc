@@ -4,7 +4,7 @@
 // NOT COMPILED AGAINST XLA IN THIS REPOSITORY: JAX/jaxlib (which ship the XLA FFI headers) are absent
 // from this image and from the GPU hosts.  The tests compile it against a stand-in for the header
 // (tests/ffi), hold each binding to its function's parameters and call the handlers of the packed
-// attention and of the rotary positions with buffers that do not fit.  Where jaxlib is installed, build with
+// attention, of the rotary positions and of the clipping with buffers that do not fit.  Where jaxlib is installed, build with
 //
 //   g++ -O2 -std=c++17 -shared -fPIC -o librfdetr_ffi.so rfdetr_ffi.cc \
 //       -I"$(python -c 'import jax.ffi; print(jax.ffi.include_dir())')" -I../../include \
@@ -542,7 +542,12 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrAxialRotary, AxialRotary,
 // Normed queries and keys with rotary positions: (query [T, H, D], key [T, Hkv, D], query_weight, key_weight [D] or [0]
 // for ones, positions [T, A] f32, int32 or int64, inv_freq) -> (query, key).
 static int position_code(ffi::DataType t) {
-    return t == ffi::DataType::S32 ? RFDETR_I32 : t == ffi::DataType::S64 ? RFDETR_I64 : t == ffi::DataType::F32 ? RFDETR_F32 : -1;
+    switch (t) {
+        case ffi::DataType::S32: return RFDETR_I32;
+        case ffi::DataType::S64: return RFDETR_I64;
+        case ffi::DataType::F32: return RFDETR_F32;
+        default: return -1;
+    }
 }
 
 static int normed_rotary_fits(const ffi::AnyBuffer &query, const ffi::AnyBuffer &key, const ffi::AnyBuffer &query_weight,
@@ -688,3 +693,117 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrClipGradients, ClipGradients,
                                   .Attr<float>("max_norm")
                                   .Ret<ffi::AnyBuffer>()
                                   .Ret<ffi::Buffer<ffi::F32>>());
+
+// Packed attention with changed scores: the plain handler's arguments, distance_slopes f32 [H] or [0] for none, prefix
+// int32 [S] or [0] for none, score_cap 0 for none.
+static bool change_fits(const ffi::Buffer<ffi::F32> &slopes, const ffi::Buffer<ffi::S32> &prefix, int64_t H, int64_t S) {
+    return (has_dims(slopes, {H}) || has_dims(slopes, {0})) && (has_dims(prefix, {S}) || has_dims(prefix, {0}));
+}
+
+static ffi::Error ScoredAttention(cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query,
+                                  ffi::Buffer<ffi::BF16> key, ffi::Buffer<ffi::BF16> value,
+                                  ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets,
+                                  ffi::Buffer<ffi::F32> slopes, ffi::Buffer<ffi::S32> prefix, int32_t causal,
+                                  float scale, float score_cap, ffi::Result<ffi::Buffer<ffi::BF16>> output,
+                                  ffi::Result<ffi::Buffer<ffi::BF16>> output_low,
+                                  ffi::Result<ffi::Buffer<ffi::F32>> lse) {
+    if (!attention_inputs_fit(query, key, value, offsets, key_offsets))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrScoredAttention");
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
+    const int64_t S = dim(offsets, 0) - 1;
+    if (!change_fits(slopes, prefix, H, S) || !has_dims(*output, {T, H, D}) ||
+        !(has_dims(*output_low, {T, H, D}) || has_dims(*output_low, {0, H, D})) || !has_dims(*lse, {H, T}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrScoredAttention");
+    const size_t bytes = rfdetr_packed_attention_workspace_bytes(S, T, Tk, H, Hkv, D);
+    void *ws = nullptr;
+    if (bytes) {
+        auto block = scratch.Allocate(bytes, 256);
+        if (!block.has_value())
+            return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrScoredAttention: workspace");
+        ws = *block;
+    }
+    return status_error(
+        rfdetr_packed_attention_scored(
+            stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D, value.untyped_data(), Hkv * D, D,
+            offsets.typed_data(), key_offsets.typed_data(), output->untyped_data(),
+            output_low->element_count() ? output_low->untyped_data() : nullptr, lse->typed_data(), ws, bytes, S, T, Tk,
+            H, Hkv, D, causal, scale, score_cap, dim(slopes, 0) ? slopes.typed_data() : nullptr,
+            dim(prefix, 0) ? prefix.typed_data() : nullptr),
+        "RfdetrScoredAttention");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrScoredAttention, ScoredAttention,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Attr<int32_t>("causal")
+                                  .Attr<float>("scale")
+                                  .Attr<float>("score_cap")
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// Its gradients: (query, key, value, offsets, key_offsets, distance_slopes, prefix, output, output_low, lse, grad_output,
+// grad_lse) -> (grad_query, grad_key, grad_value).
+static ffi::Error ScoredAttentionBwd(
+    cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query, ffi::Buffer<ffi::BF16> key,
+    ffi::Buffer<ffi::BF16> value, ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets,
+    ffi::Buffer<ffi::F32> slopes, ffi::Buffer<ffi::S32> prefix, ffi::Buffer<ffi::BF16> output,
+    ffi::Buffer<ffi::BF16> output_low, ffi::Buffer<ffi::F32> lse, ffi::Buffer<ffi::BF16> grad_output,
+    ffi::Buffer<ffi::F32> grad_lse, int32_t causal, float scale, float score_cap,
+    ffi::Result<ffi::Buffer<ffi::BF16>> grad_query, ffi::Result<ffi::Buffer<ffi::BF16>> grad_key,
+    ffi::Result<ffi::Buffer<ffi::BF16>> grad_value) {
+    if (!attention_inputs_fit(query, key, value, offsets, key_offsets))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrScoredAttentionBwd");
+    const int64_t T = dim(query, 0), H = dim(query, 1), D = dim(query, 2), Tk = dim(key, 0), Hkv = dim(key, 1);
+    const int64_t S = dim(offsets, 0) - 1;
+    if (!change_fits(slopes, prefix, H, S) || !has_dims(output, {T, H, D}) || !has_dims(output_low, {T, H, D}) ||
+        !has_dims(lse, {H, T}) || !has_dims(grad_output, {T, H, D}) || !has_dims(grad_lse, {H, T}) ||
+        !has_dims(*grad_query, {T, H, D}) || !has_dims(*grad_key, {Tk, Hkv, D}) || !has_dims(*grad_value, {Tk, Hkv, D}))
+        return status_error(RFDETR_ERR_SHAPE, "RfdetrScoredAttentionBwd");
+    const size_t bytes = rfdetr_packed_attention_backward_workspace_bytes(T, H);
+    void *ws = nullptr;
+    if (bytes) {
+        auto block = scratch.Allocate(bytes, 256);
+        if (!block.has_value())
+            return ffi::Error(ffi::ErrorCode::kResourceExhausted, "RfdetrScoredAttentionBwd: workspace");
+        ws = *block;
+    }
+    return status_error(
+        rfdetr_packed_attention_scored_backward(
+            stream, query.untyped_data(), H * D, D, key.untyped_data(), Hkv * D, D, value.untyped_data(), Hkv * D, D,
+            offsets.typed_data(), key_offsets.typed_data(), output.untyped_data(), output_low.untyped_data(),
+            lse.typed_data(), grad_output.untyped_data(), H * D, D, grad_lse.typed_data(), grad_query->untyped_data(),
+            grad_key->untyped_data(), grad_value->untyped_data(), ws, bytes, S, T, Tk, H, Hkv, D, causal, scale,
+            score_cap, dim(slopes, 0) ? slopes.typed_data() : nullptr,
+            dim(prefix, 0) ? prefix.typed_data() : nullptr),
+        "RfdetrScoredAttentionBwd");
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrScoredAttentionBwd, ScoredAttentionBwd,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int32_t>("causal")
+                                  .Attr<float>("scale")
+                                  .Attr<float>("score_cap")
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
