@@ -460,6 +460,17 @@ template <int MOD> struct RowScores {
             }
         }
     }
+    // N products to scores for a reference: within near reach exactly, those beyond it at its end (a little lower than they
+    // are).
+    template <int N> __device__ __forceinline__ void near_scores(const AttnArgs &A, float *s, int k0) const {
+#pragma unroll
+        for (int c = 0; c < N; ++c) s[c] = fminf(fmaxf(s[c], -A.near), A.near);
+        cap_near<N, false>(A, s, twice(0.0f), twice(0.0f));
+        if (!A.slopes) return;
+        const float d = (float)(k0 - level);
+#pragma unroll
+        for (int c = 0; c < N; ++c) s[c] = fmaf(-slope, fabsf(d + (float)c), s[c]);
+    }
     // kBounded: weights relative to 2^-ref of N scores that are all seen, from products or, `capped`, capped scores.
     template <int N>
     __device__ __forceinline__ void weights(const AttnArgs &A, float *s, int k0, bool capped, float ref, uint32_t *p,
@@ -484,13 +495,16 @@ template <int MOD> struct RowScores {
         if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, seen);
         finish<N>(A, s, k0, capped);
     }
-    // Where scores lie within cap log2(e) of 0, their weights are numbers relative to that and a quarter of the cap more
-    // (2^-90 to 2^54 at the largest cap, as far from float32's and bf16's ends as sums and values can want), lowered by the
-    // least distance of a key that the row sees: no maximum has to be known before the first exponential.
+    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to a reference that is near them once
+    // stay numbers: the largest score of the row's first tile, or a quarter of the cap below 0, lowered by the least distance
+    // of a key that the row sees, where that is more (weights up to 2^90 at the largest cap, those of a row whose scores are all at
+    // -cap 2^-54; float32 and bf16 end at 2^+-126).  From the second tile on no maximum has to be known before the first
+    // exponential.  (With a reference that no score sets, the weight of a row's main key is rounded like any other's, and
+    // not the 1 that it is: of two keys, 30 times the error.)
     __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
-        if (limit <= 0) return 0.25f * A.cap_out;
+        if (limit <= 0) return -0.25f * A.cap_out;
         const int nearest = abs(min(max(level, 0), limit - 1) - level), farthest = max(abs(level), abs(limit - 1 - level));
-        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
+        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), -0.25f * A.cap_out);
     }
 };
 
@@ -544,6 +558,20 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
     constexpr int KEYS = 128;
     const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    if (MOD == kBounded && first) {  // the reference; the tile is gone over again below
+        float mx = -INFINITY, s[32];
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+            tmem_ld32(ts + c, s);
+            tmem_wait_ld();
+            pin<32>(s);
+            // (Capped in TMEM they would be capped twice.)
+            scores.template near_scores<32>(A, s, k0 + c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
+        }
+        r.m = fmaxf(r.m, mx);
+    }
     if (all) {
         float s[KEYS];
 #pragma unroll
@@ -632,7 +660,7 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     bool capped = false;
     if constexpr (MOD == kBounded) capped = scores.template cap_far<64>(A, s, ts, seen);  // (past `cols` there is anything)
     if constexpr (MOD == kBounded) {
-        if (!all) scores.template finish<64>(A, s, k0, capped);
+        if (!all || first) scores.template finish<64>(A, s, k0, capped);
     } else {
         scores.template change<64>(A, s, ts, k0, seen);
     }
@@ -644,12 +672,12 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    if constexpr (MOD != kBounded) move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    if (MOD != kBounded || first) move_reference<DP>(r, to, max_of<64>(s), first, sc);
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     uint32_t p[32];
     if (all) {
-        if constexpr (MOD == kBounded) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
+        if (MOD == kBounded && !first) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
         else exp_pack<64, false, MOD>(s, sc, ref, p, acc);
         tmem_st32(ts, p);
     } else {
