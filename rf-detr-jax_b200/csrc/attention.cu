@@ -558,7 +558,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
     constexpr int KEYS = 128;
     const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
     float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    if (MOD == kBounded && first) {  // the reference; the tile is gone over again below
+    if (MOD == kBounded && first && !all) {  // the reference; the tile is gone over again below
         float mx = -INFINITY, s[32];
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
@@ -579,7 +579,19 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         tmem_wait_ld();
         pin<KEYS>(s);
         bool capped = false;
-        if constexpr (MOD == kBounded) capped = scores.template cap_far<KEYS>(A, s, ts, KEYS);
+        if constexpr (MOD == kBounded) {
+            // Capped scores rise with the products: the largest product's.  (Lowered by distance they do not; then the
+            // reference that no score sets, for a tile of 128 keys and more.)
+            if (first && !A.slopes) {
+                float top[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top[e] = 0.0f;
+                top[0] = max_of<KEYS>(s);
+                scores.template near_scores<8>(A, top, k0);
+                r.m = fmaxf(r.m, top[0]);
+            }
+            capped = scores.template cap_far<KEYS>(A, s, ts, KEYS);
+        }
         else scores.template change<KEYS>(A, s, ts, k0, KEYS);
         loaded();
         if constexpr (MOD == kBounded) {
