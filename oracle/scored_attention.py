@@ -21,6 +21,10 @@ def scored_attention(q, k, v, offsets, key_offsets=None, causal=False, scale=Non
     subtracts from the cap), and E of the distance's part and of the result, which is also how far lse is off.  P is then
     off by P (e + sum P e) beside its rounding U P; dS by that of its P, delta by what o is off, and the
     cap's derivative, 1 - t^2, by 2 t times t's error.
+
+    out may be divided by the sum of the rounded weights rather than of the exact ones: with P_j (1 + d_j), |d_j| <= U,
+    sum P d v / (1 + sum P d) - o sum P d / (1 + sum P d) is U (sum P |v| + |o|) at most, and the result's own rounding U
+    |o| more: U (sum P |v| + 2 |o|) in all.
     """
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     T, H, D = q.shape
@@ -74,7 +78,7 @@ def scored_attention(q, k, v, offsets, key_offsets=None, causal=False, scale=Non
             a = p @ np.abs(vh)
             r["out"][rows, h] = o
             o_off = p_off @ np.abs(vh)
-            r["out_bound"][rows, h] = U * (a + np.abs(o)) + o_off
+            r["out_bound"][rows, h] = U * (a + 2.0 * np.abs(o)) + o_off
             with np.errstate(divide="ignore"):
                 r["lse"][h, rows] = np.where(some, top + np.log(z), -np.inf)
             r["lse_bound"][h, rows] = np.where(some, F + E * np.abs(top) + pe.sum(1), 0.0)

@@ -227,6 +227,13 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
 // the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
 // with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
+// The weights as they were rounded, of a pair, added up.
+__device__ __forceinline__ void add_rounded(float2 &acc, uint32_t p) {
+    acc = add2(acc, make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
+}
+
 template <int N, bool POLY, int MOD>
 __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
     const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
@@ -242,6 +249,7 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
         }
         acc[c & 1] = add2(acc[c & 1], x);
         p[c] = pack_bf16(x.x, x.y);
+        if constexpr (MOD == kBounded) add_rounded(acc[2 + (c & 1)], p[c]);
     }
 }
 
@@ -257,8 +265,6 @@ constexpr float kNear = 0.5f, kMid = 1.5f;
 constexpr float kNearPoly[3] = {-0.33328160643577576f, 0.13205359876155853f, -0.0447506345808506f};
 constexpr float kMidPoly[7] = {-0.3333057165145874f, 0.13300476968288422f, -0.05260444059967995f, 0.01905897632241249f,
                                -0.005512249656021595f, 0.0010445077205076814f, -9.210196003550664e-05f};
-
-__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
 // The largest magnitude of N products, of those whose bits are set (`bits_of(c)`: of products c .. c + 31).
 template <int N, typename Bits> __device__ __forceinline__ float largest(const float *s, Bits bits_of) {
@@ -333,6 +339,7 @@ __device__ __forceinline__ void cap_near_exp(const AttnArgs &A, const float *s, 
             y.y = exp2_fast(y.y);
             acc[c / 2 & 1] = add2(acc[c / 2 & 1], y);
             p[(c0 + c) / 2] = pack_bf16(y.x, y.y);
+            if constexpr (LINE) add_rounded(acc[2 + (c / 2 & 1)], p[(c0 + c) / 2]);
         }
     }
 }
@@ -460,16 +467,13 @@ template <int MOD> struct RowScores {
             }
         }
     }
-    // N products to scores for a reference: within near reach exactly, those beyond it at its end (a little lower than they
-    // are).
-    template <int N> __device__ __forceinline__ void near_scores(const AttnArgs &A, float *s, int k0) const {
+    // The capped score of the largest of a row's products (that of the end of near reach, where it lies beyond).
+    __device__ __forceinline__ float score_of(const AttnArgs &A, float most) const {
+        float s[8];
 #pragma unroll
-        for (int c = 0; c < N; ++c) s[c] = fminf(fmaxf(s[c], -A.near), A.near);
-        cap_near<N, false>(A, s, twice(0.0f), twice(0.0f));
-        if (!A.slopes) return;
-        const float d = (float)(k0 - level);
-#pragma unroll
-        for (int c = 0; c < N; ++c) s[c] = fmaf(-slope, fabsf(d + (float)c), s[c]);
+        for (int e = 0; e < 8; ++e) s[e] = fminf(fmaxf(most, -A.near), A.near);
+        cap_near<8, false>(A, s, twice(0.0f), twice(0.0f));
+        return s[0];
     }
     // kBounded: weights relative to 2^-ref of N scores that are all seen, from products or, `capped`, capped scores.
     template <int N>
@@ -495,16 +499,19 @@ template <int MOD> struct RowScores {
         if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, seen);
         finish<N>(A, s, k0, capped);
     }
-    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to a reference that is near them once
-    // stay numbers: the largest score of the row's first tile, or a quarter of the cap below 0, lowered by the least distance
-    // of a key that the row sees, where that is more (weights up to 2^90 at the largest cap, those of a row whose scores are all at
-    // -cap 2^-54; float32 and bf16 end at 2^+-126).  From the second tile on no maximum has to be known before the first
-    // exponential.  (With a reference that no score sets, the weight of a row's main key is rounded like any other's, and
-    // not the 1 that it is: of two keys, 30 times the error.)
+    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to one reference for the row stay
+    // numbers, and no maximum has to be known before the exponentials.  Without a bias it is the largest score of the row's
+    // first tile, which the largest product gives (capped scores rise with the products), or a quarter of the cap
+    // below 0, where that is more.  With one it is a quarter of the cap above 0, lowered by the least distance of a key that
+    // the row sees.  Weights then reach from 2^-90 (of a row's main key) to 2^90 at the largest cap; float32 and bf16 end at
+    // 2^+-126.  But no weight need be 1, as the main key's is where its score sets the reference, and its rounding to
+    // bf16 would show (of two keys, 30 times the error).  So with a bias results are divided by the sum of the rounded
+    // weights: what they share cancels.  The log-sum-exp keeps the exact ones' sum.
     __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
-        if (limit <= 0) return -0.25f * A.cap_out;
+        if (!A.slopes) return -0.25f * A.cap_out;
+        if (limit <= 0) return 0.25f * A.cap_out;
         const int nearest = abs(min(max(level, 0), limit - 1) - level), farthest = max(abs(level), abs(limit - 1 - level));
-        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), -0.25f * A.cap_out);
+        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
     }
 };
 
@@ -513,7 +520,12 @@ template <int MOD> struct RowScores {
 // m = inf, where no score moves the reference, and so does not change how the other rows' weights round.
 struct RowState {
     float m, sum;
+    float dealt = 0.0f;  // kBounded with a bias: the sum of the weights as they were rounded
     __device__ explicit RowState(bool live, float from = -INFINITY) : m(live ? from : INFINITY), sum(0.0f) {}
+    template <int MOD> __device__ __forceinline__ float inverse(const AttnArgs &A) const {
+        const float of = MOD == kBounded && A.slopes ? dealt : sum;
+        return of == 0.0f ? 0.0f : 1.0f / of;
+    }
 };
 template <int MOD>
 __device__ __forceinline__ RowState first_state(const AttnArgs &A, const RowScores<MOD> &scores, bool live, int limit) {
@@ -557,21 +569,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
                                              bool first, Loaded loaded, Settle settle, Written written) {
     constexpr int KEYS = 128;
     const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
-    float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    if (MOD == kBounded && first && !all) {  // the reference; the tile is gone over again below
-        float mx = -INFINITY, s[32];
-#pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
-            tmem_ld32(ts + c, s);
-            tmem_wait_ld();
-            pin<32>(s);
-            // (Capped in TMEM they would be capped twice.)
-            scores.template near_scores<32>(A, s, k0 + c);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
-        }
-        r.m = fmaxf(r.m, mx);
-    }
+    float2 acc[4] = {twice(0.0f), twice(0.0f), twice(0.0f), twice(0.0f)};
     if (all) {
         float s[KEYS];
 #pragma unroll
@@ -580,16 +578,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         pin<KEYS>(s);
         bool capped = false;
         if constexpr (MOD == kBounded) {
-            // Capped scores rise with the products: the largest product's.  (Lowered by distance they do not; then the
-            // reference that no score sets, for a tile of 128 keys and more.)
-            if (first && !A.slopes) {
-                float top[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top[e] = 0.0f;
-                top[0] = max_of<KEYS>(s);
-                scores.template near_scores<8>(A, top, k0);
-                r.m = fmaxf(r.m, top[0]);
-            }
+            if (first && !A.slopes) r.m = fmaxf(r.m, scores.score_of(A, max_of<KEYS>(s)));
             capped = scores.template cap_far<KEYS>(A, s, ts, KEYS);
         }
         else scores.template change<KEYS>(A, s, ts, k0, KEYS);
@@ -618,20 +607,23 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         float mx = -INFINITY;
         float s[32];
         if (MOD == kBounded && !settle()) return false;
+        const bool look = MOD != kBounded || (first && !A.slopes);  // for the largest
 #pragma unroll 1
-        for (int c = 0; c < cols && MOD != kBounded; c += 32) {
+        for (int c = 0; c < cols && look; c += 32) {
             tmem_ld32(ts + c, s);
             tmem_wait_ld();
             pin<32>(s);
-            if constexpr (MOD != kPlain) {
+            if constexpr (MOD == kBiased || MOD == kCapped) {
                 scores.template change<32>(A, s, ts + c, k0 + c, seen - c);
                 tmem_st32(ts + c, reinterpret_cast<uint32_t *>(s));
             }
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
-        if constexpr (MOD != kPlain) tmem_wait_st();
-        if constexpr (MOD != kBounded) {
+        if constexpr (MOD == kBounded) {
+            if (look) r.m = fmaxf(r.m, scores.score_of(A, mx));
+        } else {
+            if constexpr (MOD != kPlain) tmem_wait_st();
             if (!settle()) return false;
             move_reference<DP>(r, to, mx, first, sc);
         }
@@ -655,6 +647,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         written(1);
     }
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+    if constexpr (MOD == kBounded) r.dealt += (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
     return true;
 }
 
@@ -670,9 +663,21 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     tmem_wait_ld();
     pin<64>(s);
     bool capped = false;
-    if constexpr (MOD == kBounded) capped = scores.template cap_far<64>(A, s, ts, seen);  // (past `cols` there is anything)
     if constexpr (MOD == kBounded) {
-        if (!all || first) scores.template finish<64>(A, s, k0, capped);
+        if (first && !A.slopes) {
+            float most = -INFINITY;
+            if (all) {
+                most = max_of<64>(s);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 64; ++c) most = c < seen ? fmaxf(most, s[c]) : most;
+            }
+            r.m = fmaxf(r.m, scores.score_of(A, most));
+        }
+        capped = scores.template cap_far<64>(A, s, ts, seen);  // (past `cols` there is anything)
+    }
+    if constexpr (MOD == kBounded) {
+        if (!all) scores.template finish<64>(A, s, k0, capped);
     } else {
         scores.template change<64>(A, s, ts, k0, seen);
     }
@@ -684,12 +689,12 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    if (MOD != kBounded || first) move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    if constexpr (MOD != kBounded) move_reference<DP>(r, to, max_of<64>(s), first, sc);
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
-    float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    float2 acc[4] = {twice(0.0f), twice(0.0f), twice(0.0f), twice(0.0f)};
     uint32_t p[32];
     if (all) {
-        if (MOD == kBounded && !first) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
+        if constexpr (MOD == kBounded) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
         else exp_pack<64, false, MOD>(s, sc, ref, p, acc);
         tmem_st32(ts, p);
     } else {
@@ -702,6 +707,7 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     }
     tmem_wait_st();
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+    if constexpr (MOD == kBounded) r.dealt += (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
 }
 
 // Where results go.  `low` is what a result lost in its rounding to bf16, itself in bf16, for the backward
@@ -727,12 +733,12 @@ __device__ __forceinline__ void store_result(const FwdOut &f, size_t at, const f
 // Whole warp: a row's result from O (or zeros) and its log-sum-exp.  With PAIR columns `from` .. `end` of a row's sum
 // of two, O times `times` and `other` (the first column's place) times `more`; where `part_row` is not negative,
 // to that row of the parts.
-template <int DP, bool PAIR>
+template <int DP, bool PAIR, int MOD>
 __device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, long long part_row, const RowState &r,
                                           uint32_t to, bool any, bool live, size_t token, int head, int from = 0,
                                           int end = DP, float times = 1.0f, const float *other = nullptr,
                                           float more = 0.0f) {
-    const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
+    const float inv = r.inverse<MOD>(A);
     const bool is_part = PAIR && part_row >= 0;
     if (live && from == 0) {
         const float l = r.sum == 0.0f ? -INFINITY : r.m * A.scale + logf(r.sum);
@@ -1270,7 +1276,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const int head = qhead + row_head(A, row);
             const long long part_row = SPLIT && sh.part_row >= 0 ? sh.part_row + row : -1;
             if (!ALT) {
-                if (ok) write_row<DP, false>(A, f, -1, rs, to, n > 0, live, token, head);
+                if (ok) write_row<DP, false, MOD>(A, f, -1, rs, to, n > 0, live, token, head);
             } else {
                 // Each half gives the other its sums of half of the channels, through the room of K and V once
                 // both are through with it.
@@ -1279,7 +1285,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 float *give = side + (1 - t) * 128 * kSide, *take = side + t * 128 * kSide;
                 half_barrier();
                 if (ok && warp_live) {
-                    if (live) *reinterpret_cast<float2 *>(give + DP / 2) = make_float2(rs.m, rs.sum);
+                    if (live) *reinterpret_cast<float4 *>(give + DP / 2) = make_float4(rs.m, rs.sum, rs.dealt, 0.0f);
 #pragma unroll 1
                     for (int c = 0; c < DP / 2; c += 16) {
                         float o[16];
@@ -1301,7 +1307,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 if (__all_sync(0xffffffffu, ok && !*abort) && warp_live) {
                     float a = 0.0f, b = 0.0f;
                     if (live) {
-                        const float2 y = *reinterpret_cast<const float2 *>(take + DP / 2);
+                        const float4 y = *reinterpret_cast<const float4 *>(take + DP / 2);
                         const float m = fmaxf(rs.m, y.x);
                         a = rs.m == -INFINITY ? 0.0f : exp2f((rs.m - m) * A.scale_log2);
                         b = y.x == -INFINITY ? 0.0f : exp2f((y.x - m) * A.scale_log2);
@@ -1309,8 +1315,9 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                         const float s0 = t == 0 ? rs.sum * a : y.y * b, s1 = t == 0 ? y.y * b : rs.sum * a;
                         rs.m = m;
                         rs.sum = s0 + s1;
+                        if constexpr (MOD == kBounded) rs.dealt = t == 0 ? rs.dealt * a + y.z * b : y.z * b + rs.dealt * a;
                     }
-                    write_row<DP, true>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
+                    write_row<DP, true, MOD>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
                                                (t + 1) * (DP / 2), a, take, b);
                 }
             }
@@ -1548,7 +1555,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         tc_fence_after();
         // (O is written over only after the next row tile's first barrier.)
         if (ok && it.any)
-            write_row<DP, false>(A, f, -1, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
+            write_row<DP, false, MOD>(A, f, -1, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
                                  it.qhead + row_head(A, row));
         tc_fence_before();
         g += it.n;
