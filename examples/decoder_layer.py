@@ -4,8 +4,10 @@ detection groups' queries, then deformable cross-attention over a feature map.
 The groups attend only within themselves, so they are packed sequences (:func:`packed_attention`
 with offsets instead of a mask or a padded batch); the queries' reference points enter the attention
 as rotary positions on two axes (:func:`axial_rotary`); the sampler's prologue and the sampler
-follow.  Run it on a GPU: ``python examples/decoder_layer.py [--images N] [--groups G] [--steps K]``;
-it fits random targets and prints the loss.
+follow.  With ``normed`` the queries and keys are normed head by head in the pass that turns them
+(:func:`normed_axial_rotary`) and the scores are capped; each step's gradients are clipped
+(:func:`clip_gradients`).  Run it on a GPU: ``python examples/decoder_layer.py [--images N] [--groups G] [--steps K]
+[--normed] [--clip NORM]``; it fits random targets and prints the loss.
 """
 
 from __future__ import annotations
@@ -30,9 +32,11 @@ class DecoderLayer(nn.Module):
     """Self-attention (8 heads of 32) within groups, cross-attention (16 heads of 16, 2 points) and a
     feed-forward network, each with its residual and LayerNorm, hidden size 256."""
 
-    def __init__(self, hidden=256, heads=8, sampler_heads=16, points=2):
+    def __init__(self, hidden=256, heads=8, sampler_heads=16, points=2, normed=False, score_cap=None):
         super().__init__()
         self.heads, self.sampler_heads, self.points = heads, sampler_heads, points
+        self.score_cap = score_cap
+        self.head_norms = nn.ParameterList(nn.Parameter(torch.ones(hidden // heads)) for _ in range(2 if normed else 0))
         self.qkv = nn.Linear(hidden, 3 * hidden)
         self.out = nn.Linear(hidden, hidden)
         self.offsets = nn.Linear(hidden, sampler_heads * points * 2)
@@ -59,8 +63,13 @@ class DecoderLayer(nn.Module):
         qkv = self.qkv(queries).view(batch * count, 3 * self.heads, hidden // self.heads)
         q, k, v = qkv.split(self.heads, 1)
         # Frequencies 0 to 7 turn by x, 8 to 15 by y.
-        q, k = rf.axial_rotary(q, k, centers.reshape(batch * count, 2), self.inv_freq, (8, 8))
-        return self.out(rf.packed_attention(q, k, v, group_offsets).view(batch, count, hidden))
+        centers = centers.reshape(batch * count, 2)
+        if len(self.head_norms):
+            q, k = rf.normed_axial_rotary(q, k, centers, self.inv_freq, (8, 8), *self.head_norms)
+        else:
+            q, k = rf.axial_rotary(q, k, centers, self.inv_freq, (8, 8))
+        attended = rf.packed_attention(q, k, v, group_offsets, score_cap=self.score_cap)
+        return self.out(attended.view(batch, count, hidden))
 
     def cross_attention(self, queries, boxes, memory, shape):
         batch, _, hidden = queries.shape
@@ -89,10 +98,11 @@ def inputs(images, groups, per_group, shape, hidden, device, seed=0):
     return normal(images, groups * per_group, hidden), boxes, normal(images, shape[0] * shape[1], hidden)
 
 
-def fit(images=2, groups=13, per_group=300, steps=20, shape=(24, 24), device="cuda:0"):
-    """Trains one layer towards random targets; returns the losses."""
+def fit(images=2, groups=13, per_group=300, steps=20, shape=(24, 24), device="cuda:0", normed=False, score_cap=None,
+        clip=None):
+    """Trains one layer towards random targets, its gradients' norm clipped to ``clip``; returns the losses."""
     torch.manual_seed(0)
-    layer = DecoderLayer().to(device=device, dtype=torch.bfloat16)
+    layer = DecoderLayer(normed=normed, score_cap=score_cap).to(device=device, dtype=torch.bfloat16)
     queries, boxes, memory = inputs(images, groups, per_group, shape, 256, device)
     target = torch.randn_like(queries)
     offsets = group_offsets(images, groups, per_group, device)
@@ -102,6 +112,8 @@ def fit(images=2, groups=13, per_group=300, steps=20, shape=(24, 24), device="cu
         optimizer.zero_grad(set_to_none=True)
         loss = (layer(queries, boxes, memory, shape, offsets) - target).float().square().mean()
         loss.backward()
+        if clip is not None:
+            rf.clip_gradients([p.grad for p in layer.parameters()], clip)
         optimizer.step()
         losses.append(loss.detach())
     return [float(x) for x in losses]
@@ -112,6 +124,9 @@ if __name__ == "__main__":
     parser.add_argument("--images", type=int, default=2)
     parser.add_argument("--groups", type=int, default=13)
     parser.add_argument("--steps", type=int, default=20)
+    parser.add_argument("--normed", action="store_true")
+    parser.add_argument("--clip", type=float)
     args = parser.parse_args()
-    for i, value in enumerate(fit(args.images, args.groups, steps=args.steps)):
+    for i, value in enumerate(fit(args.images, args.groups, steps=args.steps, normed=args.normed,
+                                  score_cap=30.0 if args.normed else None, clip=args.clip)):
         print(f"step {i}: loss {value:.4f}")
