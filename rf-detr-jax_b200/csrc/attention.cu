@@ -356,6 +356,11 @@ template <int N> __device__ __forceinline__ void cap_mid(const AttnArgs &A, floa
         s[c + 1] = y.y;
     }
 }
+__device__ __forceinline__ float far_score(const AttnArgs &A, float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * A.cap_in * (2.0f * kLog2e))));
+    return fmaf(-2.0f * A.cap_out, r, A.cap_out);
+}
 // Whole warp: n columns of products at TMEM `ts` to capped scores; `far`: some are out of the middle reach.  (Near 0 the far
 // form would lose what it subtracts from: there the polynomial.)
 template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n, bool far) {
@@ -377,9 +382,8 @@ template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, 
                 cap_near<8, false>(A, y, twice(0.0f), twice(0.0f));
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    float &x = s[e0 + e], r;
-                    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * A.cap_in * (2.0f * kLog2e))));
-                    x = fabsf(x) <= A.near ? y[e] : fmaf(-2.0f * A.cap_out, r, A.cap_out);
+                    float &x = s[e0 + e];
+                    x = fabsf(x) <= A.near ? y[e] : far_score(A, x);
                 }
             }
         }
@@ -467,13 +471,12 @@ template <int MOD> struct RowScores {
             }
         }
     }
-    // The capped score of the largest of a row's products (that of the end of near reach, where it lies beyond).
+    // The capped score of the largest of a row's products.
     __device__ __forceinline__ float score_of(const AttnArgs &A, float most) const {
-        float s[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = fminf(fmaxf(most, -A.near), A.near);
-        cap_near<8, false>(A, s, twice(0.0f), twice(0.0f));
-        return s[0];
+        const float u = most * most;
+        const float near =
+            most * fmaf(fmaf(fmaf(A.cap_near[3], u, A.cap_near[2]), u, A.cap_near[1]), u, A.cap_near[0]);
+        return fabsf(most) <= A.near ? near : far_score(A, most);
     }
     // kBounded: weights relative to 2^-ref of N scores that are all seen, from products or, `capped`, capped scores.
     template <int N>
@@ -501,14 +504,14 @@ template <int MOD> struct RowScores {
     }
     // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to one reference for the row stay
     // numbers, and no maximum has to be known before the exponentials.  Without a bias it is the largest score of the row's
-    // first tile, which the largest product gives (capped scores rise with the products), or a quarter of the cap
-    // below 0, where that is more.  With one it is a quarter of the cap above 0, lowered by the least distance of a key that
-    // the row sees.  Weights then reach from 2^-90 (of a row's main key) to 2^90 at the largest cap; float32 and bf16 end at
-    // 2^+-126.  But no weight need be 1, as the main key's is where its score sets the reference, and its rounding to
-    // bf16 would show (of two keys, 30 times the error).  So with a bias results are divided by the sum of the rounded
-    // weights: what they share cancels.  The log-sum-exp keeps the exact ones' sum.
+    // first tile, which the largest product gives (capped scores rise with the products), or what is 100 below the cap,
+    // where that is more (caps of 35 and less never meet it).  With one it is a quarter of the cap above 0, lowered by
+    // the least distance of a key that the row sees.  The weight of a row's main key then lies between 2^-90 and 2^100 at the
+    // largest cap; float32 and bf16 end at 2^+-126.  But no weight need be 1, as the main key's is where its score sets the
+    // reference, and its rounding to bf16 would show (of two keys, 30 times the error).  So with a bias results are divided
+    // by the sum of the rounded weights: what they share cancels.  The log-sum-exp keeps the exact ones' sum.
     __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
-        if (!A.slopes) return -0.25f * A.cap_out;
+        if (!A.slopes) return A.cap_out - 100.0f;
         if (limit <= 0) return 0.25f * A.cap_out;
         const int nearest = abs(min(max(level, 0), limit - 1) - level), farthest = max(abs(level), abs(limit - 1 - level));
         return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
@@ -1990,7 +1993,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
         pin<32>(d);
         bool near = false;
         if constexpr (MOD == kCapped) {
-            const float most = largest<32>(s, [&](int) { return mask ? seen : 0xffffffffu; });
+            // (DQ: a row that is no query holds another sequence's; DKV: without a mask all rows are keys.)
+            const uint32_t own = mask ? seen : DKV || scores.live ? 0xffffffffu : 0u;
+            const float most = largest<32>(s, [&](int) { return own; });
             near = __builtin_expect(!__any_sync(0xffffffffu, most > A.near), 1);
             if (!near) {
                 cap_tmem<16>(A, ts, 32, __any_sync(0xffffffffu, most > A.mid));
@@ -2613,10 +2618,10 @@ struct ScoreChange {
 
 int check_change(const ScoreChange &m, float scale) {
     if (m.cap != 0.0f) {
-        // (The polynomials' coefficients hold up to the sixth power of scale / cap.)
-        const float in = scale / m.cap;
-        if (!(m.cap > 0.0f && in >= 0x1p-20f && in <= 0x1p20f)) return RFDETR_ERR_SHAPE;
-        if (!(m.cap >= 0x1p-40f && m.cap <= 0x1p40f)) return RFDETR_ERR_SHAPE;
+        // The near polynomial's coefficients, scale (scale / cap)^2k, have to be numbers.
+        const double in = (double)scale / m.cap, last = kNearPoly[2] * (double)scale * kLog2e * in * in * in * in * in * in;
+        if (!(m.cap >= 0x1p-40f && m.cap <= 0x1p40f && in >= 0x1p-20 && in <= 0x1p20)) return RFDETR_ERR_SHAPE;
+        if (!(-last >= FLT_MIN && -last <= FLT_MAX)) return RFDETR_ERR_SHAPE;
     }
     return aligned(m.slopes, 4) && aligned(m.prefix, 4) ? RFDETR_OK : RFDETR_ERR_ALIGN;
 }

@@ -186,6 +186,40 @@ def test_one_key_has_no_score_gradient(pkg):
     assert not dq[:31].any() and dq[31:].any()
 
 
+@pytest.mark.parametrize("knob", ["1", "2", "3", "3,2"])
+def test_one_key_gives_its_value(pkg, tuning, knob):
+    """A row that sees one key is that key's value, whatever its score, distance and cap: bit for bit."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    rng = np.random.default_rng(7)
+    for dim in (32, 64, 128):
+        for how in (dict(score_cap=40.0), dict(score_cap=2.0), dict(score_cap=1e3),
+                    dict(distance_slopes=torch.tensor([0.7, 0.01], device=DEV)),
+                    dict(score_cap=40.0, distance_slopes=torch.tensor([0.7, 0.01], device=DEV))):
+            q, k, v = (_bf16(rng, 150, 2, dim, size=3.0) for _ in range(3))
+            out = pkg.packed_attention(q, k[:3], v[:3], _offsets((100, 0, 50)), _offsets((1, 1, 1)), **how)
+            assert torch.equal(out[:100], v[:1].expand(100, 2, dim)) and torch.equal(out[100:], v[2:3].expand(50, 2, dim))
+            out = pkg.packed_attention(q, k, v, _offsets((150,)), causal=True, **how)
+            assert torch.equal(out[0], v[0])
+
+
+def test_rows_without_a_query_choose_nothing(pkg):
+    """A tile's rows behind its sequence's last query hold the next sequence's: their products, out of every polynomial's
+    reach, change no bit of its gradients, in tiles whose last warp has one live row."""
+    rng = np.random.default_rng(8)
+    for dim in (32, 64, 128):
+        q, k, v, g = (_bf16(rng, 500, 2, dim) for _ in range(4))
+        off = _offsets((257, 243))
+        loud = q.clone()
+        loud[257:] *= 100.0
+        got = []
+        for x in (q, loud):
+            leaves = [y.clone().requires_grad_(True) for y in (x, k, v)]
+            out = pkg.packed_attention(*leaves, off, score_cap=12.0)
+            got.append([out, *torch.autograd.grad(out, leaves, g)])
+        for a, b in zip(*got):
+            assert torch.equal(a[:257], b[:257])
+
+
 def test_foreign_rows_change_nothing(pkg):
     """NaN, infinities and large values in rows outside the sequences, and in other sequences, change no bit."""
     rng = np.random.default_rng(3)
