@@ -383,7 +383,8 @@ template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float &x = s[e0 + e];
-                    x = fabsf(x) <= A.near ? y[e] : far_score(A, x);
+                    const float z = far_score(A, x);  // (of all: no branch)
+                    x = fabsf(x) <= A.near ? y[e] : z;
                 }
             }
         }
