@@ -14,7 +14,8 @@ for the three pieces of the training hot path:
 * ``oracle/lsap.c``  -- a C restatement of SciPy's ``linear_sum_assignment`` (Crouse's shortest
   augmenting path), which the reference calls at ``matcher.py:173``.
 * ``oracle.attention``, ``oracle.rotary`` -- packed attention and rotary positions with their
-  gradients in float64, and the largest error that the kernels' roundings leave in each element.
+  gradients in float64, and the largest error that the kernels' roundings leave in each element;
+  ``oracle.scored_attention``, ``oracle.normed_rotary`` -- the same with changed scores and after norms.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and ``bench.py``'s CPU-baseline / reference legs may
 import anything from here, and only as the checker or the timed CPU baseline.  The product

@@ -260,7 +260,9 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
 // scores around 15 that is 1e-5, a hundredth of what rounding P to bf16 loses) and its coefficients hold the scale, five
 // packed operations for two scores; up to 3/2 seven terms (7.5e-7).  Beyond, 1 - 2 / (1 + e^2x), in a loop over the tile in TMEM,
 // small and away from the straight code.  A warp takes the same form for all scores of a tile, the one that its largest
-// needs (of those that its queries see: no other sequence's values change a bit).
+// needs (of those that its queries see: no other sequence's values change a bit).  Five prompts of 6257 causal tokens, 16 /
+// 4 heads of 128, take 78 us as they are, 91 under a cap of 50 and 173 under one of 8, which most tiles pass (scores' spread
+// 3); 7000 + 2501 + 66 tokens, 8 / 2 of 128, backward 390 and, under a cap of 30, 499.
 constexpr float kNear = 0.5f, kMid = 1.5f;
 constexpr float kNearPoly[3] = {-0.33328160643577576f, 0.13205359876155853f, -0.0447506345808506f};
 constexpr float kMidPoly[7] = {-0.3333057165145874f, 0.13300476968288422f, -0.05260444059967995f, 0.01905897632241249f,
