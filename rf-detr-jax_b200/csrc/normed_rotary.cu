@@ -55,6 +55,7 @@ struct NormArgs {
     long long T, chunks;
     int D, half;
     bool interleaved;
+    bool full;                    // no lane of a row lacks a piece, or a piece its second vector
     int per_chunk;                // tokens that share a forming of sines
     int sines_at_once;            // of them, by the threads of a block
     int pieces, lanes;            // of a row; lanes that hold it
@@ -147,6 +148,7 @@ template <bool BACK> __device__ __forceinline__ Stride stride_of(const NormArgs 
 template <typename T, bool BACK>
 __device__ __forceinline__ Row<T> row_of(const NormArgs &A, int which, long long t0, int row, bool live) {
     Row<T> r;
+    row = live ? row : 0;
     r.token = quotient(row, A.heads_of[which]);
     r.h = row - r.token * A.heads[which];
     r.live = live;
@@ -255,6 +257,16 @@ template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
     }
 
     static __device__ __forceinline__ void load(const NormArgs &A, const Lane &l, const Row<T> &w, Raws &r) {
+        if (A.full) {  // every lane of a row has all of its vectors (a row that is none reads another one's, for nothing)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    r.x[n][k] = __ldg(reinterpret_cast<const V *>(w.x + l.c[n] + k * A.half));
+                    if (BACK) r.g[n][k] = __ldg(reinterpret_cast<const V *>(w.g + l.c[n] + k * A.half));
+                }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -639,8 +651,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks<BACK>) normed_rotary
                 const bool live = next.live;
                 const float *cs = turn + (live ? next.token : 0) * room.pitch;
                 if (x + step < rows) {
-                    go_on<T, BACK>(next, stride, A.heads[which]);
                     next.live = used && x + step + sub < rows;
+                    if (next.live) go_on<T, BACK>(next, stride, A.heads[which]);  // else it stays at a row that is
                     S::load(A, place, next, ahead);
                 }
                 S::row(A, place, raw, to, live, at, weights + which * room.row, cs, mine, dw[BACK ? which : 0]);
@@ -701,6 +713,7 @@ template <typename T, int VEC, int MODE, int N, bool BACK>
 int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
     A.lanes = (A.pieces + N - 1) / N;
     A.lanes_of = divisor(A.lanes);
+    A.full = MODE != kExchange && A.pieces == A.lanes * N && (MODE != kPaired || 2 * A.half == A.D);
     // Tokens that share a forming of sines: eight rows to a lane, no more than 16 KB of sines, and of those as many as give
     // every block that stays the same number of chunks (20,011 tokens of 8 x 80: 445 chunks for 444 blocks took 19.8 us).
     constexpr int kBlocks = kNormBlocks<BACK>;
