@@ -18,13 +18,13 @@ def scored_attention(q, k, v, offsets, key_offsets=None, causal=False, scale=Non
 
     Returns a dict of ``out``, ``lse`` and, with ``grad``, ``dq``, ``dk``, ``dv``, and of the bounds under the same
     names + ``_bound``.  A score is off by e: the product's F sum |scale q k|, the cap's CAP |s'| + E cap (its far form
-    subtracts from the cap), and E of the distance's part and of the result, which is also how far lse is off.  P is then
-    off by P (e + sum P e) beside its rounding U P; dS by that of its P, delta by what o is off, and the
+    subtracts from the cap), and E of the distance's part and of the result, which is also how far lse is off.  P is
+    then off by P (e + sum P e) beside its rounding U P; dS by that of its P, delta by what o is off, and the
     cap's derivative, 1 - t^2, by 2 t times t's error.
 
     out may be divided by the sum of the rounded weights rather than of the exact ones: with P_j (1 + d_j), |d_j| <= U,
-    sum P d v / (1 + sum P d) - o sum P d / (1 + sum P d) is U (sum P |v| + |o|) at most, and the result's own rounding U
-    |o| more: U (sum P |v| + 2 |o|) in all.
+    sum P d v / (1 + sum P d) - o sum P d / (1 + sum P d) is U (sum P |v| + |o|) at most, and the result's own rounding
+    U |o| more: U (sum P |v| + 2 |o|) in all.
     """
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     T, H, D = q.shape

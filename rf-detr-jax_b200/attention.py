@@ -59,7 +59,8 @@ def attention_forward(query, key, value, offsets, key_offsets, causal, scale, wa
     ws_bytes = lib.rfdetr_packed_attention_workspace_bytes(sequences, tokens, key_tokens, heads, kv_heads, dim)
     workspace = query.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     status = N.on_device(
-        query, lib.rfdetr_packed_attention_scored, N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+        query, lib.rfdetr_packed_attention_scored, N.stream_of(query), query.data_ptr(), *query.stride()[:2],
+        key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
         out.data_ptr(), N.ptr(low), N.ptr(lse), N.ptr(workspace), ws_bytes, sequences, tokens, key_tokens, heads,
         kv_heads, dim, causal, scale, cap, N.ptr(slopes), N.ptr(prefix))
@@ -81,7 +82,8 @@ def attention_backward(query, key, value, offsets, key_offsets, causal, scale, o
     ws_bytes = lib.rfdetr_packed_attention_backward_workspace_bytes(tokens, heads)
     workspace = query.new_empty(max(1, ws_bytes), dtype=torch.uint8)
     status = N.on_device(
-        query, lib.rfdetr_packed_attention_scored_backward, N.stream_of(query), query.data_ptr(), *query.stride()[:2], key.data_ptr(), *key.stride()[:2],
+        query, lib.rfdetr_packed_attention_scored_backward, N.stream_of(query), query.data_ptr(), *query.stride()[:2],
+        key.data_ptr(), *key.stride()[:2],
         value.data_ptr(), *value.stride()[:2], offsets.data_ptr(), N.ptr(key_offsets),
         out.data_ptr(), N.ptr(low), lse.data_ptr(), grad_output.data_ptr(), *grad_output.stride()[:2],
         N.ptr(grad_lse), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), workspace.data_ptr(), ws_bytes,
@@ -186,8 +188,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         check: read the offsets on the host (synchronises) and raise ``ValueError`` unless they
             ascend within the tensors; otherwise the kernels clamp them.
         score_cap: scores ``s`` become ``score_cap * tanh(s / score_cap)``.
-        distance_slopes: ``[heads]`` float32 (finite) on the device: from the (capped) score of query ``i`` and key ``j``
-            ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.
+        distance_slopes: ``[heads]`` float32 (finite) on the device: from the (capped) score of query ``i`` and key
+            ``j`` ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.
         prefix: int32 (or int64) ``[sequences]`` on the device, with ``causal``: every query of sequence ``s`` also sees
             its first ``prefix[s]`` keys (clamped to the sequence).
 

@@ -43,7 +43,8 @@ class GradientClipper:
     the results go to) once, so that a step's call does not look at every tensor again.
 
     The clipper keeps the tensors; each must keep its memory (be written in place, as the views of a flat buffer are,
-    or a captured graph's gradients).  ``out`` as for :func:`clip_gradients`; the gradients have to be contiguous with it.
+    or a captured graph's gradients).  ``out`` as for :func:`clip_gradients`; the gradients have to be contiguous with
+    it.
     """
 
     def __init__(self, gradients, out=None):

@@ -16,8 +16,8 @@
 // Scores are float32: a row whose scores are all -inf has no weights and is treated as one that sees no key.
 //
 // Scores may be changed on the way: capped, S' = cap tanh(S / cap); lowered by distance, S'' = S' - slope_h |i + Lk -
-// Lq - j|; and under a causal mask a sequence may have a prefix of keys, j < prefix_s, that all of its queries see.  The
-// backward pass then has dS_ij = P_ij (dP_ij - delta_i) (1 - (S'_ij / cap)^2).
+// Lq - j|; and under a causal mask a sequence may have a prefix of keys, j < prefix_s, that all of its queries see.
+// The backward pass then has dS_ij = P_ij (dP_ij - delta_i) (1 - (S'_ij / cap)^2).
 //
 // Queries of the heads that share a key head are rows of one tile (token-major, heads inner), so
 // K and V are read once for all of them and a few tokens still fill a tile.
@@ -254,15 +254,16 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
 }
 
 // ---- changed scores ----
-// A capped score in units of log2 is cap log2(e) tanh(x), x = scale / cap times the product.  The special-function unit
-// already has an exponential for every score, so tanh goes to the FMA pipe: x (1 + u Q(u)), u = x^2, the Q fitted to the
-// least largest relative error.  Up to |x| = 1/2, where a cap leaves nearly all scores, Q has three terms (6.4e-7: of
-// scores around 15 that is 1e-5, a hundredth of what rounding P to bf16 loses) and its coefficients hold the scale, five
-// packed operations for two scores; up to 3/2 seven terms (7.5e-7).  Beyond, 1 - 2 / (1 + e^2x), in a loop over the tile in TMEM,
-// small and away from the straight code.  A warp takes the same form for all scores of a tile, the one that its largest
-// needs (of those that its queries see: no other sequence's values change a bit).  Five prompts of 6257 causal tokens, 16 /
-// 4 heads of 128, take 78 us as they are, 91 under a cap of 50 and 173 under one of 8, which most tiles pass (scores' spread
-// 3); 7000 + 2501 + 66 tokens, 8 / 2 of 128, backward 390 and, under a cap of 30, 499.
+// A capped score in units of log2 is cap log2(e) tanh(x), x = scale / cap times the product.  The special-function
+// unit already has an exponential for every score, so tanh goes to the FMA pipe: x (1 + u Q(u)), u = x^2, the Q fitted
+// to the least largest relative error.  Up to |x| = 1/2, where a cap leaves nearly all scores, Q has three terms
+// (6.4e-7: of scores around 15 that is 1e-5, a hundredth of what rounding P to bf16 loses) and its coefficients hold
+// the scale, five packed operations for two scores; up to 3/2 seven terms (7.5e-7).  Beyond, 1 - 2 / (1 + e^2x), in a
+// loop over the tile in TMEM, small and away from the straight code.  A warp takes the same form for all scores of a
+// tile, the one that its largest needs (of those that its queries see: no other sequence's values change a bit).  Five
+// prompts of 6257 causal tokens, 16 / 4 heads of 128, take 78 us as they are, 91 under a cap of 50 and 173 under one
+// of 8, which most tiles pass (scores' spread 3); 7000 + 2501 + 66 tokens, 8 / 2 of 128, backward 390 and, under a cap
+// of 30, 499.
 constexpr float kNear = 0.5f, kMid = 1.5f;
 constexpr float kNearPoly[3] = {-0.33328160643577576f, 0.13205359876155853f, -0.0447506345808506f};
 constexpr float kMidPoly[7] = {-0.3333057165145874f, 0.13300476968288422f, -0.05260444059967995f, 0.01905897632241249f,
@@ -306,7 +307,8 @@ struct Line {
 };
 
 // s[c] w + bias(c), or without BIAS s[c] w, for N products within near reach.
-template <int N, bool BIAS> __device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float2 slope, float2 b) {
+template <int N, bool BIAS>
+__device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float2 slope, float2 b) {
     const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
                  p3 = twice(A.cap_near[3]);
 #pragma unroll
@@ -322,8 +324,8 @@ template <int N, bool BIAS> __device__ __forceinline__ void cap_near(const AttnA
         }
     }
 }
-// 2^(s[c] w + bias(c)) of N products within near reach, packed to bf16; adds them to acc[2].  The reference comes with the
-// bias: one run through the values, in which the special-function unit's exponentials and the polynomials overlap.
+// 2^(s[c] w + bias(c)) of N products within near reach, packed to bf16; adds them to acc[2].  The reference comes with
+// the bias: one run through the values, in which the special-function unit's exponentials and the polynomials overlap.
 template <int N, bool LINE>
 __device__ __forceinline__ void cap_near_exp(const AttnArgs &A, const float *s, float2 slope, float2 b, uint32_t *p,
                                              float2 *acc) {
@@ -363,8 +365,8 @@ __device__ __forceinline__ float far_score(const AttnArgs &A, float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * A.cap_in * (2.0f * kLog2e))));
     return fmaf(-2.0f * A.cap_out, r, A.cap_out);
 }
-// Whole warp: n columns of products at TMEM `ts` to capped scores; `far`: some are out of the middle reach.  (Near 0 the far
-// form would lose what it subtracts from: there the polynomial.)
+// Whole warp: n columns of products at TMEM `ts` to capped scores; `far`: some are out of the middle reach.  (Near 0
+// the far form would lose what it subtracts from: there the polynomial.)
 template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, uint32_t ts, int n, bool far) {
 #pragma unroll 1
     for (int c = 0; c < n; c += STEP) {
@@ -415,8 +417,8 @@ template <int MOD> struct RowScores {
         if (__all_sync(0xffffffffu, k0 + N - 1 <= level)) return 1;
         return __all_sync(0xffffffffu, k0 >= level) ? -1 : 0;
     }
-    // Whole warp: products out of near reach to capped scores, or false, with nothing done.  `seen`: of the N, how many from
-    // the first on this row sees.
+    // Whole warp: products out of near reach to capped scores, or false, with nothing done.  `seen`: of the N, how
+    // many from the first on this row sees.
     template <int N> __device__ __forceinline__ bool cap_far(const AttnArgs &A, float *s, uint32_t ts, int seen) const {
         const int n = live ? seen : 0;
         const float most = largest<N>(s, [&](int c) { return n >= c + 32 ? 0xffffffffu : bits(0, n - c); });
@@ -505,18 +507,20 @@ template <int MOD> struct RowScores {
         if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, seen);
         finish<N>(A, s, k0, capped);
     }
-    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to one reference for the row stay
-    // numbers, and no maximum has to be known before the exponentials.  Without a bias it is the largest score of the row's
-    // first tile, which the largest product gives (capped scores rise with the products), or what is 100 below the cap,
-    // where that is more (caps of 35 and less never meet it).  With one it is a quarter of the cap above 0, lowered by
-    // the least distance of a key that the row sees.  The weight of a row's main key then lies between 2^-90 and 2^100 at the
-    // largest cap; float32 and bf16 end at 2^+-126.  But no weight need be 1, as the main key's is where its score sets the
-    // reference, and its rounding to bf16 would show (of two keys, 30 times the error).  So with a bias results are divided
-    // by the sum of the rounded weights: what they share cancels.  The log-sum-exp keeps the exact ones' sum.
+    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to one reference for the row
+    // stay numbers, and no maximum has to be known before the exponentials.  Without a bias it is the largest score of
+    // the row's first tile, which the largest product gives (capped scores rise with the products), or what is 100
+    // below the cap, where that is more (caps of 35 and less never meet it).  With one it is a quarter of the cap
+    // above 0, lowered by the least distance of a key that the row sees.  The weight of a row's main key then lies
+    // between 2^-90 and 2^100 at the largest cap; float32 and bf16 end at 2^+-126.  But no weight need be 1, as the
+    // main key's is where its score sets the reference, and its rounding to bf16 would show (of two keys, 30 times the
+    // error).  So with a bias results are divided by the sum of the rounded weights: what they share cancels.  The
+    // log-sum-exp keeps the exact ones' sum.
     __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
         if (!A.slopes) return A.cap_out - 100.0f;
         if (limit <= 0) return 0.25f * A.cap_out;
-        const int nearest = abs(min(max(level, 0), limit - 1) - level), farthest = max(abs(level), abs(limit - 1 - level));
+        const int nearest = abs(min(max(level, 0), limit - 1) - level);
+        const int farthest = max(abs(level), abs(limit - 1 - level));
         return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
     }
 };
@@ -1321,7 +1325,8 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                         const float s0 = t == 0 ? rs.sum * a : y.y * b, s1 = t == 0 ? y.y * b : rs.sum * a;
                         rs.m = m;
                         rs.sum = s0 + s1;
-                        if constexpr (MOD == kBounded) rs.dealt = t == 0 ? rs.dealt * a + y.z * b : y.z * b + rs.dealt * a;
+                        if constexpr (MOD == kBounded)
+                            rs.dealt = t == 0 ? rs.dealt * a + y.z * b : y.z * b + rs.dealt * a;
                     }
                     write_row<DP, true, MOD>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
                                                (t + 1) * (DP / 2), a, take, b);
@@ -2052,8 +2057,9 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 s01 = mul2(s01, fma2(fma2(fma2(p3, u01, p2), u01, p1), u01, p0));
                 s23 = mul2(s23, fma2(fma2(fma2(p3, u23, p2), u23, p1), u23, p0));
             }
-            const float2 a = MOD == kCapped ? add2(s01, make_float2(nl.x, nl.y)) : fma2(s01, sc2, make_float2(nl.x, nl.y));
-            const float2 b = MOD == kCapped ? add2(s23, make_float2(nl.z, nl.w)) : fma2(s23, sc2, make_float2(nl.z, nl.w));
+            const float2 nl01 = make_float2(nl.x, nl.y), nl23 = make_float2(nl.z, nl.w);
+            const float2 a = MOD == kCapped ? add2(s01, nl01) : fma2(s01, sc2, nl01);
+            const float2 b = MOD == kCapped ? add2(s23, nl23) : fma2(s23, sc2, nl23);
             float p[4] = {exp2_fast(a.x), exp2_fast(a.y), exp2_fast(b.x), exp2_fast(b.y)};
             float2 e = mul2(make_float2(p[0], p[1]), add2(make_float2(d[c], d[c + 1]), make_float2(nd.x, nd.y)));
             float2 f = mul2(make_float2(p[2], p[3]), add2(make_float2(d[c + 2], d[c + 3]), make_float2(nd.z, nd.w)));
@@ -2576,16 +2582,16 @@ int launch_backward(AttnArgs A, const Strided &q, const Strided &k, const Stride
         const long long slots = slots_for(A.Tq, xtok, A.n_seq), blocks = slots * A.Hkv * A.subs;
         A.slot_rows = divisor(xtok);
         A.heads = divisor(A.Hkv * A.subs);
-        if (int st = launch_backward_kernel<DP, false, MOD>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f, dq,
-                                                       nullptr, (int)slots))
+        if (int st = launch_backward_kernel<DP, false, MOD>(blocks, plan.q_ranks, false, stream, A, qx, gx, ky, vy, f,
+                                                            dq, nullptr, (int)slots))
             return st;
     }
     if (A.Tk > 0) {
         const long long slots = slots_for(A.Tk, 128, A.n_seq), blocks = slots * A.Hkv;
         A.slot_rows = divisor(128);
         A.heads = divisor(A.Hkv);
-        if (int st = launch_backward_kernel<DP, true, MOD>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f, dk,
-                                                      dv, (int)slots))
+        if (int st = launch_backward_kernel<DP, true, MOD>(blocks, plan.kv_ranks, A.Tq > 0, stream, A, kx, vx, qy, gy, f,
+                                                           dk, dv, (int)slots))
             return st;
     }
     return RFDETR_OK;
@@ -2622,7 +2628,8 @@ struct ScoreChange {
 int check_change(const ScoreChange &m, float scale) {
     if (m.cap != 0.0f) {
         // The near polynomial's coefficients, scale (scale / cap)^2k, have to be numbers.
-        const double in = (double)scale / m.cap, last = kNearPoly[2] * (double)scale * kLog2e * in * in * in * in * in * in;
+        const double in = (double)scale / m.cap, in2 = in * in;
+        const double last = kNearPoly[2] * (double)scale * kLog2e * in2 * in2 * in2;
         if (!(m.cap >= 0x1p-40f && m.cap <= 0x1p40f && in >= 0x1p-20 && in <= 0x1p20)) return RFDETR_ERR_SHAPE;
         if (!(-last >= FLT_MIN && -last <= FLT_MAX)) return RFDETR_ERR_SHAPE;
     }

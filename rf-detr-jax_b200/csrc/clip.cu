@@ -33,7 +33,8 @@ constexpr int kMostTensors = 1000;  // of one launch, whose arguments have 32,76
 struct ClipTensor {
     const void *in;
     void *out;
-    long long start;  // the tensor's place in the range, times four; plus 1 where the input is bf16, 2 where the output is
+    long long start;  // the tensor's place in the range, times four; plus 1 where the input is bf16, plus 2 where the
+                      // output is
     long long count;
 };
 template <int N> struct ClipTable {
@@ -136,9 +137,9 @@ gradient_norm_kernel(const __grid_constant__ ClipTable<N> table, const ClipArgs 
     }
 }
 
-// A warp's n values from p, times f, to q; the last pieces first.  A piece is 16 bytes of the wider of the two types, so
-// that a warp's loads and its stores lie together (bf16 to float32 in pieces of 16 bytes of bf16, two stores each: 41 us
-// for 27 million values, cold; so: 28).
+// A warp's n values from p, times f, to q; the last pieces first.  A piece is 16 bytes of the wider of the two types,
+// so that a warp's loads and its stores lie together (bf16 to float32 in pieces of 16 bytes of bf16, two stores each:
+// 41 us for 27 million values, cold; so: 28).
 template <typename T, typename Q> __device__ __forceinline__ void scaled(const T *p, Q *q, long long n, float f) {
     constexpr int V = 16 / (sizeof(T) > sizeof(Q) ? sizeof(T) : sizeof(Q)), U = sizeof(T) * V < 16 ? 8 : 4;
     using In = typename Raw<V * (int)sizeof(T)>::T;

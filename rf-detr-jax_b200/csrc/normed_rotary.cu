@@ -8,17 +8,16 @@
 //   dx_c = r (w_c h_c - x_c r^2 mean_c' (w_c' h_c' x_c'))
 // r is formed again from x, which the gradient reads anyway.
 //
-// The floor is memory: forward x in and y out, backward x and g in and dx out; nothing is kept between them.  What bounds
-// it now is the issue of instructions, 64% of the slots forward and 54% backward: 32,768 tokens of 16 + 4 heads of 128,
-// bf16, take 72 and 130 us, 4.7 and 3.9 TB/s; 20,011 of 7 + 1 of 80, 48 channels interleaved, 15.2 forward.  A row
-// (one head of one token) is read once, in 16-byte pieces, by as many neighbouring lanes as it has pieces (ten for 80
-// channels of bf16, three rows to a warp), summed by shuffles, and turned in registers.  Where half is a
-// multiple of a piece a lane holds both partners of its pairs; otherwise they meet through shared memory, so that any
-// half is read in whole pieces.  Blocks stay for the launch: a lane's channels are the same in every row,
-// so the weights' gradients are summed in its registers, then over the block, and a second launch adds the blocks' sums
-// in order (no atomics: equal calls give equal bits).
-// Sums, norms and angles are float32 (angles reduced from a product carried twice as far); values are rounded to the
-// output's type once.
+// The floor is memory: forward x in and y out, backward x and g in and dx out; nothing is kept between them.  What
+// bounds it now is the issue of instructions, 64% of the slots forward and 54% backward: 32,768 tokens of 16 + 4 heads
+// of 128, bf16, take 72 and 130 us, 4.7 and 3.9 TB/s; 20,011 of 7 + 1 of 80, 48 channels interleaved, 15.2 forward.  A
+// row (one head of one token) is read once, in 16-byte pieces, by as many neighbouring lanes as it has pieces (ten for
+// 80 channels of bf16, three rows to a warp), summed by shuffles, and turned in registers.  Where half is a multiple
+// of a piece a lane holds both partners of its pairs; otherwise they meet through shared memory, so that any half is
+// read in whole pieces.  Blocks stay for the launch: a lane's channels are the same in every row, so the weights'
+// gradients are summed in its registers, then over the block, and a second launch adds the blocks' sums in order (no
+// atomics: equal calls give equal bits).  Sums, norms and angles are float32 (angles reduced from a product carried
+// twice as far); values are rounded to the output's type once.
 #include <cfloat>
 #include <type_traits>
 
@@ -201,9 +200,9 @@ template <int N> __device__ __forceinline__ void load_pairs(const float *p, int 
 
 // Rows whose lanes hold both partners of their pairs.  A lane has N pieces of P pairs of channels, as float32 pairs
 // (of neighbouring channel pairs) of first partners and of second: packed arithmetic takes half the issue slots (with
-// scalar arithmetic, and places found by division for every row, the first of the sizes above took 95 us forward and 167
-// backward).
-// In shared memory cosines and sines, and weights, lie by pieces: four pairs' of all pieces, then the next four.
+// scalar arithmetic, and places found by division for every row, the first of the sizes above took 95 us forward and
+// 167 backward).  In shared memory cosines and sines, and weights, lie by pieces: four pairs' of all pieces, then the
+// next four.
 template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
     static constexpr int P = MODE == kPaired ? VEC : VEC / 2, Q = P / 2;  // pairs, float2 of them
     static constexpr int K = MODE == kPaired ? 2 : 1;
@@ -257,7 +256,8 @@ template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
     }
 
     static __device__ __forceinline__ void load(const NormArgs &A, const Lane &l, const Row<T> &w, Raws &r) {
-        if (A.full) {  // every lane of a row has all of its vectors (a row that is none reads another one's, for nothing)
+        // Every lane of a row has all of its vectors (a row that is none reads another one's, for nothing).
+        if (A.full) {
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -300,7 +300,8 @@ template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
             }
     }
     template <bool INVERSE>
-    static __device__ __forceinline__ void turned(const NormArgs &A, const Lane &l, int at, Values &v, const float *turn) {
+    static __device__ __forceinline__ void turned(const NormArgs &A, const Lane &l, int at, Values &v,
+                                                  const float *turn) {
         const float2 minus = make_float2(-1.0f, -1.0f);
         const int pieces = (A.half + P - 1) / P;
 #pragma unroll
@@ -360,8 +361,8 @@ template <typename T, int VEC, int MODE, int N, bool BACK> struct PairRows {
     }
 
     // A row from its raw values to its result; backward adds to the weights' gradient.  Whole warp.
-    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &l, const Raws &raw, T *y, bool live, int at,
-                                               const float *weight, const float *turn, float *, Values &dw) {
+    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &l, const Raws &raw, T *y, bool live,
+                                               int at, const float *weight, const float *turn, float *, Values &dw) {
         Values x;
         widen(raw.x, x);
         const float sum = square(x);
@@ -506,8 +507,8 @@ template <typename T, int VEC, int N, bool BACK> struct ExchangeRows {
         for (int n = 0; n < N; ++n)
             if (live && at + n * A.lanes < A.pieces) put_values<T, VEC>(y + (at + n * A.lanes) * VEC, v[n]);
     }
-    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &, const Raws &raw, T *y, bool live, int at,
-                                               const float *weight, const float *turn, float *room, Values &dw) {
+    static __device__ __forceinline__ void row(const NormArgs &A, const Lane &, const Raws &raw, T *y, bool live,
+                                               int at, const float *weight, const float *turn, float *room, Values &dw) {
         Values x;
         widen(raw.x, x);
         float sum = 0.0f;
@@ -714,8 +715,9 @@ int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
     A.lanes = (A.pieces + N - 1) / N;
     A.lanes_of = divisor(A.lanes);
     A.full = MODE != kExchange && A.pieces == A.lanes * N && (MODE != kPaired || 2 * A.half == A.D);
-    // Tokens that share a forming of sines: eight rows to a lane, no more than 16 KB of sines, and of those as many as give
-    // every block that stays the same number of chunks (20,011 tokens of 8 x 80: 445 chunks for 444 blocks took 19.8 us).
+    // Tokens that share a forming of sines: eight rows to a lane, no more than 16 KB of sines, and of those as many as
+    // give every block that stays the same number of chunks (20,011 tokens of 8 x 80: 445 chunks for 444 blocks took
+    // 19.8 us).
     constexpr int kBlocks = kNormBlocks<BACK>;
     static_assert(!BACK || kBlocks <= kBackBlocks, "the workspace");
     const long long stay = kBlocks * (long long)num_sms();
@@ -757,7 +759,8 @@ int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
     return RFDETR_OK;
 }
 
-template <typename T, bool BACK> int dispatch_normed(NormArgs &A, bool whole, const WeightGrads &dw, cudaStream_t stream) {
+template <typename T, bool BACK>
+int dispatch_normed(NormArgs &A, bool whole, const WeightGrads &dw, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     if (!whole) {  // a value at a time
         A.pieces = A.D;

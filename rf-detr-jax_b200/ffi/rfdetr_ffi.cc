@@ -4,7 +4,8 @@
 // NOT COMPILED AGAINST XLA IN THIS REPOSITORY: JAX/jaxlib (which ship the XLA FFI headers) are absent
 // from this image and from the GPU hosts.  The tests compile it against a stand-in for the header
 // (tests/ffi), hold each binding to its function's parameters and call the handlers of the packed
-// attention, of the rotary positions and of the clipping with buffers that do not fit.  Where jaxlib is installed, build with
+// attention, of the rotary positions and of the clipping with buffers that do not fit.  Where jaxlib is installed,
+// build with
 //
 //   g++ -O2 -std=c++17 -shared -fPIC -o librfdetr_ffi.so rfdetr_ffi.cc \
 //       -I"$(python -c 'import jax.ffi; print(jax.ffi.include_dir())')" -I../../include \
@@ -550,8 +551,8 @@ static int position_code(ffi::DataType t) {
     }
 }
 
-static int normed_rotary_fits(const ffi::AnyBuffer &query, const ffi::AnyBuffer &key, const ffi::AnyBuffer &query_weight,
-                              const ffi::AnyBuffer &key_weight, const ffi::AnyBuffer &positions,
+static int normed_rotary_fits(const ffi::AnyBuffer &query, const ffi::AnyBuffer &key,
+                              const ffi::AnyBuffer &query_weight, const ffi::AnyBuffer &key_weight, const ffi::AnyBuffer &positions,
                               const ffi::Buffer<ffi::F32> &inv_freq, ffi::Span<const int64_t> sections) {
     if (query.dimensions().size() != 3 || key.dimensions().size() != 3) return RFDETR_ERR_SHAPE;
     const int64_t T = dim(query, 0), D = dim(query, 2);
@@ -696,7 +697,8 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrClipGradients, ClipGradients,
 
 // Packed attention with changed scores: the plain handler's arguments, distance_slopes f32 [H] or [0] for none, prefix
 // int32 [S] or [0] for none, score_cap 0 for none.
-static bool change_fits(const ffi::Buffer<ffi::F32> &slopes, const ffi::Buffer<ffi::S32> &prefix, int64_t H, int64_t S) {
+static bool change_fits(const ffi::Buffer<ffi::F32> &slopes, const ffi::Buffer<ffi::S32> &prefix, int64_t H,
+                        int64_t S) {
     return (has_dims(slopes, {H}) || has_dims(slopes, {0})) && (has_dims(prefix, {S}) || has_dims(prefix, {0}));
 }
 
@@ -749,8 +751,8 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(RfdetrScoredAttention, ScoredAttention,
                                   .Ret<ffi::Buffer<ffi::BF16>>()
                                   .Ret<ffi::Buffer<ffi::F32>>());
 
-// Its gradients: (query, key, value, offsets, key_offsets, distance_slopes, prefix, output, output_low, lse, grad_output,
-// grad_lse) -> (grad_query, grad_key, grad_value).
+// Its gradients: (query, key, value, offsets, key_offsets, distance_slopes, prefix, output, output_low, lse,
+// grad_output, grad_lse) -> (grad_query, grad_key, grad_value).
 static ffi::Error ScoredAttentionBwd(
     cudaStream_t stream, ffi::ScratchAllocator scratch, ffi::Buffer<ffi::BF16> query, ffi::Buffer<ffi::BF16> key,
     ffi::Buffer<ffi::BF16> value, ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S32> key_offsets,
