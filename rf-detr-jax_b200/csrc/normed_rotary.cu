@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks<BACK>) normed_rotary
 }
 
 // The blocks' sums of dw, 32 columns to a block, added in order.
-constexpr int kSumRows = 16;
+constexpr int kSumRows = 32;
 __global__ void __launch_bounds__(32 * kSumRows)
 weight_grad_kernel(const float *partial, int blocks, int D, void *dwq, int q_type, void *dwk, int k_type) {
     __shared__ float part[kSumRows][33];
@@ -687,7 +687,7 @@ weight_grad_kernel(const float *partial, int blocks, int D, void *dwq, int q_typ
     wait_for_primary();
     float sum = 0.0f;
     if (column < 2 * D) {
-#pragma unroll 4
+#pragma unroll 8
         for (int b = threadIdx.y; b < blocks; b += kSumRows) sum += __ldcg(partial + (size_t)b * 2 * D + column);
     }
     part[threadIdx.y][threadIdx.x] = sum;
