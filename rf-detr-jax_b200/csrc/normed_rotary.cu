@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "normed_plan.cuh"
 #include "tcgen05.cuh"
 
 namespace rfdetr {
@@ -31,10 +32,6 @@ constexpr int kAxes = 8;
 constexpr int kNormThreads = 256, kNormWarps = kNormThreads / 32;
 constexpr int kMostDim = 256;
 constexpr double kTurnsPerRadian = 0.15915494309189533576888;
-
-// How a lane finds the partners of its channels: it holds both, from two pieces half apart (kPaired) or from one
-// (kInterleaved), or they meet through shared memory (kExchange).
-enum { kPaired, kInterleaved, kExchange };
 
 struct NormArgs {
     const void *in[2];            // q, k
@@ -711,8 +708,12 @@ struct WeightGrads {
 constexpr int kBackBlocks = 2;  // to an SM
 
 template <typename T, int VEC, int MODE, int N, bool BACK>
-int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
-    A.lanes = (A.pieces + N - 1) / N;
+int launch_normed(NormArgs &A, const NormPlan &plan, const WeightGrads &dw, cudaStream_t stream) {
+    // A row lies within a warp: with more lanes the kernel's step from row to row would be 0.
+    if (plan.lanes < 1 || plan.lanes > 32 || plan.each != N || plan.mode != MODE || plan.vec != VEC)
+        return RFDETR_ERR_SHAPE;
+    A.pieces = plan.pieces;
+    A.lanes = plan.lanes;
     A.lanes_of = divisor(A.lanes);
     A.full = MODE != kExchange && A.pieces == A.lanes * N && (MODE != kPaired || 2 * A.half == A.D);
     // Tokens that share a forming of sines: eight rows to a lane, no more than 16 KB of sines, and of those as many as
@@ -762,20 +763,16 @@ int launch_normed(NormArgs &A, const WeightGrads &dw, cudaStream_t stream) {
 template <typename T, bool BACK>
 int dispatch_normed(NormArgs &A, bool whole, const WeightGrads &dw, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    if (!whole) {  // a value at a time
-        A.pieces = A.D;
-        return launch_normed<T, 1, kExchange, kMostDim / 32, BACK>(A, dw, stream);
+    const NormPlan p = plan_normed(sizeof(T), A.D, A.half, A.interleaved, whole);
+    if (!whole) return launch_normed<T, 1, kExchange, 8, BACK>(A, p, dw, stream);
+    switch (p.mode) {
+        case kInterleaved: return launch_normed<T, V, kInterleaved, 2, BACK>(A, p, dw, stream);
+        case kExchange: return launch_normed<T, V, kExchange, 2, BACK>(A, p, dw, stream);
+        default: break;
     }
-    const bool paired = !A.interleaved && A.half % V == 0;
-    A.pieces = paired ? A.half / V + (A.D - 2 * A.half) / V : A.D / V;
-    // Sixteen bf16 values (eight float32) to a lane, so that what a row costs besides them is shared.
-    auto with = [&](auto mode) {
-        constexpr int M = decltype(mode)::value;
-        return launch_normed<T, V, M, M == kPaired ? 1 : 2, BACK>(A, dw, stream);
-    };
-    if (paired) return with(std::integral_constant<int, kPaired>{});
-    if (A.interleaved) return with(std::integral_constant<int, kInterleaved>{});
-    return with(std::integral_constant<int, kExchange>{});
+    if constexpr (V == 4)
+        if (p.each == 2) return launch_normed<T, V, kPaired, 2, BACK>(A, p, dw, stream);
+    return launch_normed<T, V, kPaired, 1, BACK>(A, p, dw, stream);
 }
 
 struct NormCall {

@@ -227,3 +227,13 @@ def test_refusals(pkg):
             bad()
     with torch.no_grad():
         f(q, q, pos, freq, (8,))
+
+
+# Float32 rows with two pieces to a lane, where one piece each would be more than a warp's lanes, and the widest with one.
+@pytest.mark.parametrize("dim", [136, 160, 192, 256])
+@pytest.mark.parametrize("turned", [8, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wide_heads_turned_in_part(pkg, dim, turned, dtype):
+    sections = (turned // 2 - turned // 4, turned // 4)
+    for tokens, heads, kv in ((1, 1, 1), (41, 3, 2), (1500, 2, 1)):
+        _check(pkg, tokens, heads, kv, dim, sections, False, dtype, seed=dim + turned + tokens)
