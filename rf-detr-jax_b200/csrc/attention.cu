@@ -44,7 +44,7 @@ struct AttnArgs {
     Divisor slot_rows;  // rows (of the tensor that the launch tiles) in a slot
     Divisor heads;      // key heads x head groups: blocks or row tiles to a slot
     // Of changed scores (kBiased, kCapped) alone.
-    float unit;             // scale log2(e)
+    float unit, per_unit;   // scale log2(e), and 1 over it
     float cap_in, cap_out;  // scale / cap, cap log2(e)
     float cap_back;         // -1 / cap_out^2
     float near, mid;        // products up to which the polynomials reach
@@ -55,7 +55,7 @@ struct AttnArgs {
 };
 
 // What a launch does to its scores, a template argument of the kernels: only scales them; lowers them by distance or
-// sees a prefix; caps them as well; forward, caps them so low that no running maximum is needed (kMostBounded).
+// sees a prefix; caps them as well; forward, caps them without a bias, so that products tell how large scores can be.
 constexpr int kPlain = 0, kBiased = 1, kCapped = 2, kBounded = 3;
 
 // Keys that every query of sequence `seq` (of klen keys) sees; seq is negative outside all sequences.
@@ -224,16 +224,11 @@ template <int N> __device__ __forceinline__ float max_of(const float *s) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
 // 2^(sc s + ref) of N values in pairs, packed to bf16; adds them to acc[2].  With POLY one pair of eight takes
 // the FMA pipe: 8192 + 3001 + 130 causal tokens, 8 / 2 heads of 128, forward, 156 us without, 152 with one, 151
 // with two of eight (three: slower again).  The short kernel, whose four blocks hide more, gains nothing by it.
-__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
-
-// The weights as they were rounded, of a pair, added up.
-__device__ __forceinline__ void add_rounded(float2 &acc, uint32_t p) {
-    acc = add2(acc, make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
-}
-
 template <int N, bool POLY, int MOD>
 __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, uint32_t *p, float2 *acc) {
     const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(ref, ref);
@@ -249,7 +244,6 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
         }
         acc[c & 1] = add2(acc[c & 1], x);
         p[c] = pack_bf16(x.x, x.y);
-        if constexpr (MOD == kBounded) add_rounded(acc[2 + (c & 1)], p[c]);
     }
 }
 
@@ -261,9 +255,9 @@ __device__ __forceinline__ void exp_pack(const float *s, float sc, float ref, ui
 // the scale, five packed operations for two scores; up to 3/2 seven terms (7.5e-7).  Beyond, 1 - 2 / (1 + e^2x), in a
 // loop over the tile in TMEM, small and away from the straight code.  A warp takes the same form for all scores of a
 // tile, the one that its largest needs (of those that its queries see: no other sequence's values change a bit).  Five
-// prompts of 6257 causal tokens, 16 / 4 heads of 128, take 78 us as they are, 91 under a cap of 50 and 173 under one
-// of 8, which most tiles pass (scores' spread 3); 7000 + 2501 + 66 tokens, 8 / 2 of 128, backward 390 and, under a cap
-// of 30, 499.
+// prompts of 6257 causal tokens, 16 / 4 heads of 128, take 78 us as they are, 88 under a cap of 50 and 161 under one
+// of 8, which most tiles pass (scores' spread 3); 7000 + 2501 + 66 tokens, 8 / 2 of 128, backward 391 and, under a cap
+// of 30, 498.
 constexpr float kNear = 0.5f, kMid = 1.5f;
 constexpr float kNearPoly[3] = {-0.33328160643577576f, 0.13205359876155853f, -0.0447506345808506f};
 constexpr float kMidPoly[7] = {-0.3333057165145874f, 0.13300476968288422f, -0.05260444059967995f, 0.01905897632241249f,
@@ -324,27 +318,21 @@ __device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float2 slo
         }
     }
 }
-// 2^(s[c] w + bias(c)) of N products within near reach, packed to bf16; adds them to acc[2].  The reference comes with
-// the bias: one run through the values, in which the special-function unit's exponentials and the polynomials overlap.
-template <int N, bool LINE>
-__device__ __forceinline__ void cap_near_exp(const AttnArgs &A, const float *s, float2 slope, float2 b, uint32_t *p,
-                                             float2 *acc) {
+// 2^(s[c] w + ref) of N products within near reach, packed to bf16; adds them to acc[2].  One run through the values, in
+// which the special-function unit's exponentials and the polynomials overlap.
+template <int N>
+__device__ __forceinline__ void cap_near_exp(const AttnArgs &A, const float *s, float ref, uint32_t *p, float2 *acc) {
     const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
-                 p3 = twice(A.cap_near[3]);
+                 p3 = twice(A.cap_near[3]), ref2 = twice(ref);
 #pragma unroll
-    for (int c0 = 0; c0 < N; c0 += 32) {
-        Line bias(slope, fma2(slope, twice(c0), b));
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-            const float2 x = make_float2(s[c0 + c], s[c0 + c + 1]), u = mul2(x, x);
-            const float2 w = fma2(fma2(fma2(p3, u, p2), u, p1), u, p0);
-            float2 y = fma2(x, w, LINE ? bias.at(c) : b);
-            y.x = exp2_fast(y.x);
-            y.y = exp2_fast(y.y);
-            acc[c / 2 & 1] = add2(acc[c / 2 & 1], y);
-            p[(c0 + c) / 2] = pack_bf16(y.x, y.y);
-            if constexpr (LINE) add_rounded(acc[2 + (c / 2 & 1)], p[(c0 + c) / 2]);
-        }
+    for (int c = 0; c < N; c += 2) {
+        const float2 x = make_float2(s[c], s[c + 1]), u = mul2(x, x);
+        const float2 w = fma2(fma2(fma2(p3, u, p2), u, p1), u, p0);
+        float2 y = fma2(x, w, ref2);
+        y.x = exp2_fast(y.x);
+        y.y = exp2_fast(y.y);
+        acc[c / 2 & 1] = add2(acc[c / 2 & 1], y);
+        p[c / 2] = pack_bf16(y.x, y.y);
     }
 }
 template <int N> __device__ __forceinline__ void cap_mid(const AttnArgs &A, float *s) {
@@ -417,11 +405,13 @@ template <int MOD> struct RowScores {
         if (__all_sync(0xffffffffu, k0 + N - 1 <= level)) return 1;
         return __all_sync(0xffffffffu, k0 >= level) ? -1 : 0;
     }
-    // Whole warp: products out of near reach to capped scores, or false, with nothing done.  `seen`: of the N, how
-    // many from the first on this row sees.
-    template <int N> __device__ __forceinline__ bool cap_far(const AttnArgs &A, float *s, uint32_t ts, int seen) const {
+    // The largest magnitude of N products, of which this row sees the first `seen`.
+    template <int N> __device__ __forceinline__ float most_of(const float *s, int seen) const {
         const int n = live ? seen : 0;
-        const float most = largest<N>(s, [&](int c) { return n >= c + 32 ? 0xffffffffu : bits(0, n - c); });
+        return largest<N>(s, [&](int c) { return n >= c + 32 ? 0xffffffffu : bits(0, n - c); });
+    }
+    // Whole warp: products out of near reach to capped scores, or false, with nothing done.
+    template <int N> __device__ __forceinline__ bool cap_far(const AttnArgs &A, float *s, uint32_t ts, float most) const {
         if (__builtin_expect(!__any_sync(0xffffffffu, most > A.near), 1)) return false;
         cap_tmem<32>(A, ts, N, __any_sync(0xffffffffu, most > A.mid));
 #pragma unroll
@@ -476,52 +466,18 @@ template <int MOD> struct RowScores {
             }
         }
     }
-    // The capped score of the largest of a row's products.
-    __device__ __forceinline__ float score_of(const AttnArgs &A, float most) const {
-        const float u = most * most;
-        const float near =
-            most * fmaf(fmaf(fmaf(A.cap_near[3], u, A.cap_near[2]), u, A.cap_near[1]), u, A.cap_near[0]);
-        return fabsf(most) <= A.near ? near : far_score(A, most);
-    }
-    // kBounded: weights relative to 2^-ref of N scores that are all seen, from products or, `capped`, capped scores.
-    template <int N>
-    __device__ __forceinline__ void weights(const AttnArgs &A, float *s, int k0, bool capped, float ref, uint32_t *p,
-                                            float2 *acc) const {
-        const int side = side_of<N>(A, k0);
-        if (!capped && (side != 0 || !A.slopes)) {
-            if (side != 0) {
-                const float along = side < 0 ? -slope : slope;
-                cap_near_exp<N, true>(A, s, twice(along), twice(fmaf(along, (float)(k0 - level), ref)), p, acc);
-            } else {
-                cap_near_exp<N, false>(A, s, twice(0.0f), twice(ref), p, acc);
-            }
-            return;
-        }
-        finish<N>(A, s, k0, capped);
-        exp_pack<N, false, MOD>(s, 1.0f, ref, p, acc);
+    // The capped score of a product.
+    __device__ __forceinline__ float score_of(const AttnArgs &A, float x) const {
+        const float u = x * x;
+        const float near = x * fmaf(fmaf(fmaf(A.cap_near[3], u, A.cap_near[2]), u, A.cap_near[1]), u, A.cap_near[0]);
+        return fabsf(x) <= A.near ? near : far_score(A, x);
     }
     template <int N>
     __device__ __forceinline__ void change(const AttnArgs &A, float *s, uint32_t ts, int k0, int seen) const {
         if constexpr (MOD == kPlain) return;
         bool capped = false;
-        if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, seen);
+        if constexpr (MOD >= kCapped) capped = cap_far<N>(A, s, ts, most_of<N>(s, seen));
         finish<N>(A, s, k0, capped);
-    }
-    // Where scores lie within cap log2(e) of 0 (lowered by distance), weights relative to one reference for the row
-    // stay numbers, and no maximum has to be known before the exponentials.  Without a bias it is the largest score of
-    // the row's first tile, which the largest product gives (capped scores rise with the products), or what is 100
-    // below the cap, where that is more (caps of 35 and less never meet it).  With one it is a quarter of the cap
-    // above 0, lowered by the least distance of a key that the row sees.  The weight of a row's main key then lies
-    // between 2^-90 and 2^100 at the largest cap; float32 and bf16 end at 2^+-126.  But no weight need be 1, as the
-    // main key's is where its score sets the reference, and its rounding to bf16 would show (of two keys, 30 times the
-    // error).  So with a bias results are divided by the sum of the rounded weights: what they share cancels.  The
-    // log-sum-exp keeps the exact ones' sum.
-    __device__ __forceinline__ float reference(const AttnArgs &A, int limit) const {
-        if (!A.slopes) return A.cap_out - 100.0f;
-        if (limit <= 0) return 0.25f * A.cap_out;
-        const int nearest = abs(min(max(level, 0), limit - 1) - level);
-        const int farthest = max(abs(level), abs(limit - 1 - level));
-        return fmaf(-slope, (float)(slope >= 0.0f ? nearest : farthest), 0.25f * A.cap_out);
     }
 };
 
@@ -530,18 +486,8 @@ template <int MOD> struct RowScores {
 // m = inf, where no score moves the reference, and so does not change how the other rows' weights round.
 struct RowState {
     float m, sum;
-    float dealt = 0.0f;  // kBounded with a bias: the sum of the weights as they were rounded
-    __device__ explicit RowState(bool live, float from = -INFINITY) : m(live ? from : INFINITY), sum(0.0f) {}
-    template <int MOD> __device__ __forceinline__ float inverse(const AttnArgs &A) const {
-        const float of = MOD == kBounded && A.slopes ? dealt : sum;
-        return of == 0.0f ? 0.0f : 1.0f / of;
-    }
+    __device__ explicit RowState(bool live) : m(live ? -INFINITY : INFINITY), sum(0.0f) {}
 };
-template <int MOD>
-__device__ __forceinline__ RowState first_state(const AttnArgs &A, const RowScores<MOD> &scores, bool live, int limit) {
-    if constexpr (MOD == kBounded) return RowState(live, scores.reference(A, limit));
-    return RowState(live);
-}
 
 // Whole warp: moves the reference to the new maximum where some live row's grew far enough, and O and the
 // sum with it.
@@ -567,6 +513,25 @@ template <int DP> __device__ __forceinline__ void move_reference(RowState &r, ui
     }
 }
 
+// kBounded: the magnitude of a tile's products up to which they are within near reach and no score passes the reference
+// by kQuiet (a capped score is at most scale log2(e) times its product, and the cap).  Such a tile needs no maximum of
+// its own; in any other the reference moves as in the other kernels, so that weights and sums stay below 2^kQuiet times
+// their true scale whatever the cap and the order of the keys, and a row's largest weight is not below 1.  With 8 powers,
+// as kLazy, 95 us for 5 prompts of 6257 causal tokens, 16 / 4 heads of 128, cap 50 (scores' spread 3); with 20, which
+// hardly any tile passes after a row's first, 88; with a maximum in every tile 106.
+constexpr float kQuiet = 20.0f;
+__device__ __forceinline__ float quiet_up_to(const AttnArgs &A, const RowState &r) {
+    return fminf(A.near, (r.m + kQuiet) * A.per_unit);
+}
+// kBounded, whole warp: moves the reference after N scores that are all seen, `capped` already or products.
+template <int DP, int N>
+__device__ __forceinline__ void move_if_reached(const AttnArgs &A, const RowScores<kBounded> &scores, RowState &r,
+                                                uint32_t to, const float *s, bool capped, float most, bool first) {
+    if (!first && !__any_sync(0xffffffffu, fminf(A.unit * most, A.cap_out) > r.m + kQuiet)) return;
+    const float mx = max_of<N>(s);
+    move_reference<DP>(r, to, capped ? mx : scores.score_of(A, mx), first, 1.0f);
+}
+
 // Whole warp: one key tile of S at TMEM `ts` (this warp's lanes) becomes P at `tp`; `to` is O.  `cols`
 // columns are in use, of which this row sees `seen`; `all` says that every row sees all KEYS.
 // loaded() is called once S has been read, settle() before P is written or O touched (it returns
@@ -579,7 +544,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
                                              bool first, Loaded loaded, Settle settle, Written written) {
     constexpr int KEYS = 128;
     const float sc = MOD == kPlain ? A.scale_log2 : 1.0f;
-    float2 acc[4] = {twice(0.0f), twice(0.0f), twice(0.0f), twice(0.0f)};
+    float2 acc[2] = {twice(0.0f), twice(0.0f)};
     if (all) {
         float s[KEYS];
 #pragma unroll
@@ -587,14 +552,19 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         tmem_wait_ld();
         pin<KEYS>(s);
         bool capped = false;
+        float most = 0.0f;
+        bool loud = false;
         if constexpr (MOD == kBounded) {
-            if (first && !A.slopes) r.m = fmaxf(r.m, scores.score_of(A, max_of<KEYS>(s)));
-            capped = scores.template cap_far<KEYS>(A, s, ts, KEYS);
+            most = scores.template most_of<KEYS>(s, KEYS);
+            loud = __builtin_expect(__any_sync(0xffffffffu, most > quiet_up_to(A, r)), 0);
+            if (loud) capped = scores.template cap_far<KEYS>(A, s, ts, most);
+        } else {
+            scores.template change<KEYS>(A, s, ts, k0, KEYS);
         }
-        else scores.template change<KEYS>(A, s, ts, k0, KEYS);
         loaded();
         if constexpr (MOD == kBounded) {
             if (!settle()) return false;
+            if (loud) move_if_reached<DP, KEYS>(A, scores, r, to, s, capped, most, first);
         } else {
             const float mx = max_of<KEYS>(s);
             if (!settle()) return false;
@@ -604,11 +574,8 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t p[KEYS / 4];
-            if constexpr (MOD == kBounded) {
-                scores.template weights<KEYS / 2>(A, s + h * (KEYS / 2), k0 + h * (KEYS / 2), capped, ref, p, acc);
-            } else {
-                exp_pack<KEYS / 2, true, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
-            }
+            if (MOD == kBounded && !capped) cap_near_exp<KEYS / 2>(A, s + h * (KEYS / 2), ref, p, acc);
+            else exp_pack<KEYS / 2, MOD != kBounded, MOD>(s + h * (KEYS / 2), sc, ref, p, acc);
             tmem_st32(tp + h * 32, p);
             tmem_wait_st();
             written(h);
@@ -616,10 +583,8 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
     } else {
         float mx = -INFINITY;
         float s[32];
-        if (MOD == kBounded && !settle()) return false;
-        const bool look = MOD != kBounded || (first && !A.slopes);  // for the largest
 #pragma unroll 1
-        for (int c = 0; c < cols && look; c += 32) {
+        for (int c = 0; c < cols; c += 32) {
             tmem_ld32(ts + c, s);
             tmem_wait_ld();
             pin<32>(s);
@@ -631,12 +596,11 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
         if constexpr (MOD == kBounded) {
-            if (look) r.m = fmaxf(r.m, scores.score_of(A, mx));
-        } else {
-            if constexpr (MOD != kPlain) tmem_wait_st();
-            if (!settle()) return false;
-            move_reference<DP>(r, to, mx, first, sc);
+            if (mx != -INFINITY) mx = scores.score_of(A, mx);
         }
+        if constexpr (MOD == kBiased || MOD == kCapped) tmem_wait_st();
+        if (!settle()) return false;
+        move_reference<DP>(r, to, mx, first, sc);
         const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
         // P of 32 keys takes 16 columns: over S it stays behind what has been read.
 #pragma unroll 1
@@ -657,7 +621,6 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
         written(1);
     }
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-    if constexpr (MOD == kBounded) r.dealt += (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
     return true;
 }
 
@@ -673,20 +636,10 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     tmem_wait_ld();
     pin<64>(s);
     bool capped = false;
+    float most = 0.0f;
     if constexpr (MOD == kBounded) {
-        if (first && !A.slopes) {
-            float most = -INFINITY;
-            if (all) {
-                most = max_of<64>(s);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 64; ++c) most = c < seen ? fmaxf(most, s[c]) : most;
-            }
-            r.m = fmaxf(r.m, scores.score_of(A, most));
-        }
-        capped = scores.template cap_far<64>(A, s, ts, seen);  // (past `cols` there is anything)
-    }
-    if constexpr (MOD == kBounded) {
+        most = scores.template most_of<64>(s, seen);  // (past `cols` there is anything)
+        capped = scores.template cap_far<64>(A, s, ts, most);
         if (!all) scores.template finish<64>(A, s, k0, capped);
     } else {
         scores.template change<64>(A, s, ts, k0, seen);
@@ -699,12 +652,17 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
             for (int c = 0; c < 32; ++c) s[h * 32 + c] = m & (1u << c) ? s[h * 32 + c] : -INFINITY;
         }
     }
-    if constexpr (MOD != kBounded) move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    if constexpr (MOD == kBounded) {
+        if (all) move_if_reached<DP, 64>(A, scores, r, to, s, capped, most, first);
+        else move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    } else {
+        move_reference<DP>(r, to, max_of<64>(s), first, sc);
+    }
     const float ref = r.m == -INFINITY ? 0.0f : -r.m * sc;
-    float2 acc[4] = {twice(0.0f), twice(0.0f), twice(0.0f), twice(0.0f)};
+    float2 acc[2] = {twice(0.0f), twice(0.0f)};
     uint32_t p[32];
     if (all) {
-        if constexpr (MOD == kBounded) scores.template weights<64>(A, s, k0, capped, ref, p, acc);
+        if (MOD == kBounded && !capped) cap_near_exp<64>(A, s, ref, p, acc);
         else exp_pack<64, false, MOD>(s, sc, ref, p, acc);
         tmem_st32(ts, p);
     } else {
@@ -717,7 +675,6 @@ __device__ __forceinline__ void softmax_tile64(const AttnArgs &A, const RowScore
     }
     tmem_wait_st();
     r.sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-    if constexpr (MOD == kBounded) r.dealt += (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
 }
 
 // Where results go.  `low` is what a result lost in its rounding to bf16, itself in bf16, for the backward
@@ -743,12 +700,12 @@ __device__ __forceinline__ void store_result(const FwdOut &f, size_t at, const f
 // Whole warp: a row's result from O (or zeros) and its log-sum-exp.  With PAIR columns `from` .. `end` of a row's sum
 // of two, O times `times` and `other` (the first column's place) times `more`; where `part_row` is not negative,
 // to that row of the parts.
-template <int DP, bool PAIR, int MOD>
+template <int DP, bool PAIR>
 __device__ __forceinline__ void write_row(const AttnArgs &A, const FwdOut &f, long long part_row, const RowState &r,
                                           uint32_t to, bool any, bool live, size_t token, int head, int from = 0,
                                           int end = DP, float times = 1.0f, const float *other = nullptr,
                                           float more = 0.0f) {
-    const float inv = r.inverse<MOD>(A);
+    const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
     const bool is_part = PAIR && part_row >= 0;
     if (live && from == 0) {
         const float l = r.sum == 0.0f ? -INFINITY : r.m * A.scale + logf(r.sum);
@@ -1244,7 +1201,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             // Keys that every row of the tile sees (rows past the last token do not count).
             const int all_see = A.causal ? max(min(klen, tok_first + 1 + klen - q.len), prefix) : klen;
             const RowScores<MOD> scores(A, qhead + row_head(A, row), tok + klen - q.len, live);
-            RowState rs = first_state<MOD>(A, scores, live, limit);
+            RowState rs(live);
             const int n = r.cnt[t];
             bool ok = true;
 #pragma unroll 1
@@ -1286,7 +1243,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
             const int head = qhead + row_head(A, row);
             const long long part_row = SPLIT && sh.part_row >= 0 ? sh.part_row + row : -1;
             if (!ALT) {
-                if (ok) write_row<DP, false, MOD>(A, f, -1, rs, to, n > 0, live, token, head);
+                if (ok) write_row<DP, false>(A, f, -1, rs, to, n > 0, live, token, head);
             } else {
                 // Each half gives the other its sums of half of the channels, through the room of K and V once
                 // both are through with it.
@@ -1295,7 +1252,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 float *give = side + (1 - t) * 128 * kSide, *take = side + t * 128 * kSide;
                 half_barrier();
                 if (ok && warp_live) {
-                    if (live) *reinterpret_cast<float4 *>(give + DP / 2) = make_float4(rs.m, rs.sum, rs.dealt, 0.0f);
+                    if (live) *reinterpret_cast<float2 *>(give + DP / 2) = make_float2(rs.m, rs.sum);
 #pragma unroll 1
                     for (int c = 0; c < DP / 2; c += 16) {
                         float o[16];
@@ -1317,7 +1274,7 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                 if (__all_sync(0xffffffffu, ok && !*abort) && warp_live) {
                     float a = 0.0f, b = 0.0f;
                     if (live) {
-                        const float4 y = *reinterpret_cast<const float4 *>(take + DP / 2);
+                        const float2 y = *reinterpret_cast<const float2 *>(take + DP / 2);
                         const float m = fmaxf(rs.m, y.x);
                         a = rs.m == -INFINITY ? 0.0f : exp2f((rs.m - m) * A.scale_log2);
                         b = y.x == -INFINITY ? 0.0f : exp2f((y.x - m) * A.scale_log2);
@@ -1325,11 +1282,9 @@ attn_forward_long_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap m
                         const float s0 = t == 0 ? rs.sum * a : y.y * b, s1 = t == 0 ? y.y * b : rs.sum * a;
                         rs.m = m;
                         rs.sum = s0 + s1;
-                        if constexpr (MOD == kBounded)
-                            rs.dealt = t == 0 ? rs.dealt * a + y.z * b : y.z * b + rs.dealt * a;
                     }
-                    write_row<DP, true, MOD>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
-                                               (t + 1) * (DP / 2), a, take, b);
+                    write_row<DP, true>(A, f, part_row, rs, to, n > 0, live, token, head, t * (DP / 2),
+                                        (t + 1) * (DP / 2), a, take, b);
                 }
             }
         }
@@ -1506,7 +1461,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
             A.causal ? max(min(it.klen, max(0, it.tok0 + row_tok + 1 + it.klen - it.qlen)), it.prefix) : it.klen;
         const int all_see = A.causal ? max(min(it.klen, it.tok0 + 1 + it.klen - it.qlen), it.prefix) : it.klen;
         const RowScores<MOD> row_scores(A, it.qhead + row_head(A, row), it.tok0 + row_tok + it.klen - it.qlen, live);
-        RowState rs = first_state<MOD>(A, row_scores, live, limit);
+        RowState rs(live);
 #pragma unroll 1
         for (int i = 0; i < it.n; ++i) {
             const int t = g + i;
@@ -1566,7 +1521,7 @@ attn_forward_short_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap 
         tc_fence_after();
         // (O is written over only after the next row tile's first barrier.)
         if (ok && it.any)
-            write_row<DP, false, MOD>(A, f, -1, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
+            write_row<DP, false>(A, f, -1, rs, to, it.n > 0, live, (size_t)it.qrow + row_tok,
                                  it.qhead + row_head(A, row));
         tc_fence_before();
         g += it.n;
@@ -2643,6 +2598,7 @@ void set_change(AttnArgs &A, const ScoreChange &m) {
     if (m.cap == 0.0f) return;
     A.cap_in = A.scale / m.cap;
     A.cap_out = m.cap * kLog2e;
+    A.per_unit = 1.0f / A.unit;
     A.cap_back = (float)(-1.0 / ((double)A.cap_out * A.cap_out));
     A.near = kNear / A.cap_in;
     A.mid = kMid / A.cap_in;
@@ -2654,14 +2610,11 @@ void set_change(AttnArgs &A, const ScoreChange &m) {
     for (int k = 0; k < 7; ++k) A.cap_mid[k + 1] = A.cap_out * kMidPoly[k];
 }
 
-// Caps (in units of log2) up to which the forward kernels need no running maximum.
-constexpr float kMostBounded = 72.5f;
-
 // Calls f with the head's padded size and what is done to scores, as types.
 template <bool FORWARD, typename F> int with_kernels(int64_t head_dim, const ScoreChange &m, F f) {
     auto with = [&](auto dp) {
         if constexpr (FORWARD)
-            if (m.cap != 0.0f && m.cap * kLog2e <= kMostBounded) return f(dp, std::integral_constant<int, kBounded>{});
+            if (m.cap != 0.0f && !m.slopes) return f(dp, std::integral_constant<int, kBounded>{});
         if (m.cap != 0.0f) return f(dp, std::integral_constant<int, kCapped>{});
         if (m.any()) return f(dp, std::integral_constant<int, kBiased>{});
         return f(dp, std::integral_constant<int, kPlain>{});

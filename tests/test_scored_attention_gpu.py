@@ -334,3 +334,39 @@ def test_refusals(pkg):
         with pytest.raises(ValueError):
             f(**bad)
     f(score_cap=1.0, distance_slopes=m, prefix=pre, causal=True)
+
+
+def _tiers(rng, heads, kv, dim, queries, values, cap=50.0):
+    """Queries, keys and values whose scores lie in runs of 64 keys around these parts of the cap, low ones first, so that
+    a row's largest score comes late and far above its first ones; `values`: the values' size."""
+    at = np.repeat([-1.5, -1.2, -1.4, -0.6, 0.1, -1.0, 0.4, 1.2, -0.5, 2.5, 1.4, -2.5, 0.0, 3.0, 1.6], 64)
+    one = dim ** -0.25 * np.ones(dim)
+    q = 20.0 * one + 0.5 * rng.standard_normal((queries, heads, dim))
+    k = cap / 20.0 * at[:, None, None] * one + 0.05 * rng.standard_normal((len(at), kv, dim))
+    v = values * rng.standard_normal((len(at), kv, dim))
+    return [torch.tensor(x.astype(np.float32), device=DEV).to(torch.bfloat16) for x in (q, k, v)]
+
+
+@pytest.mark.parametrize("knob", ["1", "2", "3", "3,4"])
+@pytest.mark.parametrize("values", [2.0 ** -60, 1.0, 2.0 ** 80])
+def test_values_of_any_size(pkg, tuning, knob, values):
+    """Weights stay near 1 whatever the first keys' scores: results are as far from float64 as their values' sizes say,
+    be those tiny or large."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    rng = np.random.default_rng(9)
+    for dim, cap, slopes, causal, prefix in ((32, 50.0, None, False, None), (64, 50.0, None, True, (960,)),
+                                             (128, 50.0, None, True, None), (64, 35.0, (0.01, -0.02), True, (300,)),
+                                             (128, 50.0, (0.05, 0.004), False, None), (32, 60.0, (0.01, 0.0), True, None),
+                                             (128, 60.0, None, True, None)):
+        for queries in (1, 150, 960):
+            q, k, v = _tiers(rng, 2, 1, dim, queries, values)
+            m = None if slopes is None else torch.tensor(slopes, dtype=torch.float32, device=DEV)
+            pre = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device=DEV)
+            out, lse = pkg.packed_attention(q, k, v, _offsets((queries,)), _offsets((960,)), causal=causal, score_cap=cap,
+                                            distance_slopes=m, prefix=pre, return_lse=True)
+            r = scored_attention(_f64(q), _f64(k), _f64(v), [0, queries], [0, 960], causal, None, cap,
+                                 None if m is None else _f64(m), prefix)
+            assert out.isfinite().all()
+            _close("lse", lse, r["lse"], r["lse_bound"])
+            _close("out", out.double() / values, r["out"] / values, r["out_bound"] / values)
+    _fault_free(pkg)
