@@ -188,8 +188,10 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         check: read the offsets on the host (synchronises) and raise ``ValueError`` unless they
             ascend within the tensors; otherwise the kernels clamp them.
         score_cap: scores ``s`` become ``score_cap * tanh(s / score_cap)``.
-        distance_slopes: ``[heads]`` float32 (finite) on the device: from the (capped) score of query ``i`` and key
-            ``j`` ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.
+        distance_slopes: ``[heads]`` float32 on the device: from the (capped) score of query ``i`` and key ``j``
+            ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.  Slopes
+            are finite, negative ones times the longest distance too; scores are float32, so that a product past its
+            range leaves a key out.
         prefix: int32 (or int64) ``[sequences]`` on the device, with ``causal``: every query of sequence ``s`` also sees
             its first ``prefix[s]`` keys (clamped to the sequence).
 

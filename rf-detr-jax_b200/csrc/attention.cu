@@ -283,36 +283,39 @@ template <int N, typename Bits> __device__ __forceinline__ float largest(const f
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-// A number for each of 32 keys in a row, linear in the key, as pairs: eight at a time, each from the eight before (so
-// that there are four pairs of constants, not sixteen to load).
-struct Line {
-    float2 v[4], step;
-    __device__ __forceinline__ Line(float2 along, float2 first) {
+// How far each of 32 keys in a row lies ahead of a row's level, from the first's distance on, as pairs: eight at a time,
+// each from the eight before (so that there are four pairs to start with, not sixteen to load).  Whole numbers, exact up
+// to 2^24: a bias is slope times distance rounded once, and 0 at distance 0 however steep the slope.  (Stepping the bias
+// itself takes one packed operation less, forward 153 us instead of 159 for 7000 + 2501 + 66 causal tokens, 8 / 2 heads
+// of 128, uncapped; but it is off by roundings of the tile's largest, so that a slope of 8 moves the score of a key that
+// a row is level with by 3e-5.)
+struct Ahead {
+    float2 v[4];
+    __device__ __forceinline__ explicit Ahead(float first) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = fma2(along, make_float2(2 * j, 2 * j + 1), first);
-        step = mul2(along, twice(8.0f));
+        for (int j = 0; j < 4; ++j) v[j] = add2(twice(first), make_float2(2 * j, 2 * j + 1));
     }
     // Of keys c, c + 1, for even c that rise by two from 0.
     __device__ __forceinline__ float2 at(int c) {
         float2 &x = v[c / 2 % 4];
-        if (c >= 8) x = add2(x, step);
+        if (c >= 8) x = add2(x, twice(8.0f));
         return x;
     }
 };
 
-// s[c] w + bias(c), or without BIAS s[c] w, for N products within near reach.
+// Of N products within near reach s[c] w or, with BIAS, s[c] w + along (first + c).
 template <int N, bool BIAS>
-__device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float2 slope, float2 b) {
+__device__ __forceinline__ void cap_near(const AttnArgs &A, float *s, float along, float first) {
     const float2 p0 = twice(A.cap_near[0]), p1 = twice(A.cap_near[1]), p2 = twice(A.cap_near[2]),
                  p3 = twice(A.cap_near[3]);
 #pragma unroll
     for (int c0 = 0; c0 < N; c0 += 32) {
-        Line bias(slope, fma2(slope, twice(c0), b));
+        Ahead ahead(first + (float)c0);
 #pragma unroll
         for (int c = 0; c < (N < 32 ? N : 32); c += 2) {
             const float2 x = make_float2(s[c0 + c], s[c0 + c + 1]), u = mul2(x, x);
             const float2 w = fma2(fma2(fma2(p3, u, p2), u, p1), u, p0);
-            const float2 y = BIAS ? fma2(x, w, bias.at(c)) : mul2(x, w);
+            const float2 y = BIAS ? fma2(x, w, mul2(twice(along), ahead.at(c))) : mul2(x, w);
             s[c0 + c] = y.x;
             s[c0 + c + 1] = y.y;
         }
@@ -371,7 +374,7 @@ template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, 
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] = s[e0 + e];
-                cap_near<8, false>(A, y, twice(0.0f), twice(0.0f));
+                cap_near<8, false>(A, y, 0.0f, 0.0f);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float &x = s[e0 + e];
@@ -386,6 +389,11 @@ template <int STEP> __device__ __forceinline__ void cap_tmem(const AttnArgs &A, 
     tmem_wait_st();
 }
 
+// A head's slope in units of log2, a number whatever the finite slope.
+__device__ __forceinline__ float slope_of(const AttnArgs &A, int head) {
+    return fminf(fmaxf(__ldg(A.slopes + head) * kLog2e, -FLT_MAX), FLT_MAX);
+}
+
 // A row's scores: N products of keys k0 .. at TMEM `ts`, read into s already, become scores in units of log2.
 template <int MOD> struct RowScores {
     float slope = 0.0f;  // in units of log2
@@ -396,7 +404,7 @@ template <int MOD> struct RowScores {
         if constexpr (MOD != kPlain) {
             level = at;
             live = is_live;
-            if (A.slopes && live) slope = __ldg(A.slopes + head) * kLog2e;
+            if (A.slopes && live) slope = slope_of(A, head);
         }
     }
     // Which side of the row's level N keys from k0 on are, for all of the warp's rows: 1 before it, -1 behind, 0 both.
@@ -423,11 +431,11 @@ template <int MOD> struct RowScores {
     // Products to scores that lack nothing, `capped` of them already are.
     template <int N> __device__ __forceinline__ void finish(const AttnArgs &A, float *s, int k0, bool capped) const {
         const int side = side_of<N>(A, k0);
-        // On one side the bias is linear in the key and takes part in the last operation.
-        const float2 along = twice(side < 0 ? -slope : slope), b = mul2(along, twice((float)(k0 - level)));
+        // On one side the bias is linear in the key: packed, and added in the last operation.
+        const float along = side < 0 ? -slope : slope, first = (float)(k0 - level);
         if (MOD >= kCapped && !capped) {
-            if (side != 0) cap_near<N, true>(A, s, along, b);
-            else cap_near<N, false>(A, s, along, b);
+            if (side != 0) cap_near<N, true>(A, s, along, first);
+            else cap_near<N, false>(A, s, along, first);
             if (side != 0 || !A.slopes) return;
         } else if (MOD == kBiased) {
             const float2 unit = twice(A.unit);
@@ -442,10 +450,11 @@ template <int MOD> struct RowScores {
             } else {
 #pragma unroll
                 for (int c0 = 0; c0 < N; c0 += 32) {
-                    Line bias(along, fma2(along, twice(c0), b));
+                    Ahead ahead(first + (float)c0);
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        const float2 y = fma2(make_float2(s[c0 + c], s[c0 + c + 1]), unit, bias.at(c));
+                        const float2 y = fma2(make_float2(s[c0 + c], s[c0 + c + 1]), unit,
+                                              mul2(twice(along), ahead.at(c)));
                         s[c0 + c] = y.x;
                         s[c0 + c + 1] = y.y;
                     }
@@ -457,7 +466,7 @@ template <int MOD> struct RowScores {
         }
 #pragma unroll
         for (int c0 = 0; c0 < N; c0 += 32) {
-            Line ahead(twice(1.0f), twice((float)(k0 + c0 - level)));
+            Ahead ahead(first + (float)c0);
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
                 const float2 d = ahead.at(c);
@@ -1771,7 +1780,7 @@ __device__ int bwd_load(const AttnArgs &A, const CUtensorMap *mx0, const CUtenso
                 sh.one_ds[st][c] = od;
                 if constexpr (MOD != kPlain) {
                     if (A.slopes) {
-                        sh.slope2[st][c] = c < good ? __ldg(A.slopes + head + row_head(A, c)) * kLog2e : 0.0f;
+                        sh.slope2[st][c] = c < good ? slope_of(A, head + row_head(A, c)) : 0.0f;
                         sh.level[st][c] = (float)(at + row_token(A, c) + r.klen - r.qlen - r.k0);
                     }
                 }
@@ -1966,11 +1975,11 @@ __device__ void bwd_grads(const AttnArgs &A, BwdShared &sh, const BwdRange &r, u
                 tmem_wait_ld();
                 pin<32>(s);
             } else if (mask) {
-                cap_near<32, false>(A, s, twice(0.0f), twice(0.0f));
+                cap_near<32, false>(A, s, 0.0f, 0.0f);
             }
         }
         // DQ: from the key that the row is level with to the first of this thread's columns.
-        Line ahead(twice(1.0f), twice(DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level)));
+        Ahead ahead(DKV ? 0.0f : (float)((r.start + i) * kWalk + c0 - scores.level));
         uint32_t ps[16], pd[16];
         // Straight code in either case: the exponentials' latencies overlap.
         auto weights = [&, ahead](auto masked, auto products) mutable {

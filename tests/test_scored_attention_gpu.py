@@ -370,3 +370,15 @@ def test_values_of_any_size(pkg, tuning, knob, values):
             _close("lse", lse, r["lse"], r["lse_bound"])
             _close("out", out.double() / values, r["out"] / values, r["out_bound"] / values)
     _fault_free(pkg)
+
+
+@pytest.mark.parametrize("slope", [0.5, 8.0, 1e3, 1e6, 3e38])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_steep_slopes(pkg, dim, slope):
+    """A bias is slope times distance rounded once: exactly 0 for the key that a row is level with, wherever in its tile
+    that lies (at the end of one, for a single query over whole tiles of keys), and steep slopes leave that key alone."""
+    for cap in (None, 20.0, 60.0):
+        _check(pkg, (1, 1, 1, 1), (128, 64, 640, 131), heads=2, kv=1, dim=dim, causal=True, cap=cap, slopes=(slope, 0.25),
+               seed=dim)
+        _check(pkg, (40, 3), (168, 130), heads=2, kv=1, dim=dim, causal=False, cap=cap, slopes=(slope, 0.25), seed=dim)
+        _check(pkg, (300, 64), heads=2, kv=1, dim=dim, causal=True, cap=cap, slopes=(0.25, slope), prefix=(150, 3), seed=dim)
