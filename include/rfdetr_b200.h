@@ -492,9 +492,10 @@ int rfdetr_normed_rotary_backward(void *stream, const void *query, int64_t query
  *
  * norm = sqrt(sum of g^2 over all values of all tensors); every output value is g, or where norm > max_norm
  * g * (max_norm / norm) (a NaN norm makes every result NaN, an infinite one makes finite values 0).
- *   gradients, outputs   host arrays of n_tensors device pointers; an output may be its gradient (same type), no
- *                        tensors may share memory otherwise;  types: f32 or bf16 each;  counts: values of each (may be
- *                        0), aligned to their type;  norm: device f32 scalar.
+ *   gradients, outputs   host arrays of n_tensors device pointers; an output may be its gradient (same type); one that
+ *                        shares memory with another, or with a gradient otherwise, is refused (RFDETR_ERR_SHAPE);
+ *                        types: f32 or bf16 each;  counts: values of each (may be 0), aligned to their type;  norm:
+ *                        device f32 scalar.
  * The host arrays are read during the call alone.  Squares and sums are float64; bitwise reproducible.  Two
  * launches for up to 1000 tensors.  The 8-byte aligned workspace is of the size its query returns.
  * No reference counterpart among the calls above: it stands between the all-reduce and the optimizer of a train step.

@@ -114,7 +114,7 @@ def clip_gradients(gradients, max_norm: float, *, out=None) -> torch.Tensor:
         max_norm: the limit, not negative; ``inf`` for the norm alone.
         out: where the results go: None for the gradients themselves, or tensors with as many values each, contiguous,
             float32 or bfloat16 (bfloat16 gradients clipped into float32 ones, for instance).  They may be the
-            gradients, but no two tensors may share memory otherwise.
+            gradients themselves; results that share memory with one another, or with a gradient otherwise, are refused.
 
     Returns:
         The norm before clipping, a float32 scalar on the device.  Where it is ``max_norm`` at most the values stay

@@ -16,7 +16,10 @@
 // Equal calls give equal bits.
 // 361 float32 tensors of 27.4 million values into others: 55 us, 21 for the norm (5.2 TB/s), 34 for the rest; one
 // bf16 buffer of as many values into a float32 one 38, 13 and 25.
+#include <algorithm>
 #include <cfloat>
+#include <memory>
+#include <new>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -243,6 +246,47 @@ struct ClipCall {
     const int32_t *in_types, *out_types;
 };
 
+// Addresses of a tensor's bytes.
+struct ClipSpan {
+    uintptr_t from, to;
+};
+ClipSpan span_of(const void *p, int type, int64_t count) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return {at, at + (uintptr_t)count * dtype_size(type)};
+}
+
+// Refuses results that share memory with one another, or with a gradient that is not their own: the second launch would
+// read what it has written.  Lists in the order of their addresses (a flat buffer's views) take one look at each
+// tensor, others a sort; 361 shuffled tensors' call takes 8 to 10 us up to here, in order 6.
+int check_memory(const ClipCall &c, int64_t n) {
+    const std::unique_ptr<ClipSpan[]> room(new (std::nothrow) ClipSpan[n + 1]);
+    if (!room) return RFDETR_ERR_CAPACITY;
+    ClipSpan *const spans = room.get();
+    int64_t k = 0;
+    bool in_order = true;
+    for (int64_t i = 0; i < n; ++i) {
+        if (c.counts[i] == 0) continue;
+        spans[k] = span_of(c.out[i], c.out_types[i], c.counts[i]);
+        in_order = in_order && (k == 0 || spans[k - 1].to <= spans[k].from);
+        ++k;
+    }
+    if (!in_order) {
+        std::sort(spans, spans + k, [](const ClipSpan &a, const ClipSpan &b) { return a.from < b.from; });
+        for (int64_t i = 1; i < k; ++i)
+            if (spans[i - 1].to > spans[i].from) return RFDETR_ERR_SHAPE;
+    }
+    for (int64_t i = 0; i < n; ++i) {
+        if (c.counts[i] == 0 || (c.in[i] == c.out[i] && c.in_types[i] == c.out_types[i])) continue;
+        const ClipSpan in = span_of(c.in[i], c.in_types[i], c.counts[i]);
+        if (in.to <= spans[0].from || in.from >= spans[k - 1].to) continue;
+        // The last result that begins before the gradient's end must not reach past its start.
+        const ClipSpan *next = std::lower_bound(spans, spans + k, in.to,
+                                                [](const ClipSpan &s, uintptr_t end) { return s.from < end; });
+        if (next > spans && next[-1].to > in.from) return RFDETR_ERR_SHAPE;
+    }
+    return RFDETR_OK;
+}
+
 // The tensors that have values, from `from` on, up to N of them; returns where the next table begins.
 template <int N> int64_t fill_table(ClipTable<N> &table, ClipArgs &A, const ClipCall &c, int64_t from, int64_t n) {
     A = {};
@@ -330,9 +374,10 @@ extern "C" int rfdetr_clip_gradients(void *stream, const void *const *gradients,
         if (counts[i] && gradients[i] == outputs[i] && in != out) return RFDETR_ERR_DTYPE;
     }
     if (!norm || !aligned(norm, 4)) return RFDETR_ERR_ALIGN;
+    const ClipCall c{gradients, outputs, counts, gradient_types, output_types};
+    if (int st = check_memory(c, n_tensors)) return st;
     if (!workspace || workspace_bytes < rfdetr_clip_gradients_workspace_bytes(n_tensors) || !aligned(workspace, 8))
         return RFDETR_ERR_WORKSPACE;
-    const ClipCall c{gradients, outputs, counts, gradient_types, output_types};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double *sums = static_cast<double *>(workspace);
     // The arguments are copied at every launch: a short list takes a short table.

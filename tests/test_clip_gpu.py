@@ -177,3 +177,18 @@ def test_refusals(pkg):
     y = torch.empty(10, device=DEV)
     f(torch.ones(20, device=DEV)[::2], math.inf, out=y)  # strided gradients are read where there is somewhere to put them
     assert (y == 1).all()
+
+
+def test_results_that_share_memory_are_refused(pkg):
+    x = torch.ones(100, device=DEV)
+    a, b = x[:40], x[40:80]
+    f = pkg.clip_gradients
+    for bad in (lambda: f([x[:10], x[5:20]], 1.0), lambda: f([x, b], 1.0), lambda: f([a, b], 1.0, out=[b, a]),
+                lambda: f([a, b], 1.0, out=[x[1:41], x[50:90]]), lambda: f(a, 1.0, out=x[:80].view(torch.bfloat16)[2:42]),
+                lambda: pkg.GradientClipper([b, x[20:60]]).clip(1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    y = torch.empty(100, device=DEV)
+    f([a, a], 1e9, out=[y[:40], y[40:80]])  # gradients alike, results apart
+    f([a, b], 1e9, out=[a, y[:40]])
+    assert torch.equal(y[:80], x[:80])
