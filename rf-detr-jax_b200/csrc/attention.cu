@@ -2589,7 +2589,8 @@ struct ScoreChange {
     bool any() const { return cap != 0.0f || slopes || prefix; }
 };
 
-int check_change(const ScoreChange &m, float scale) {
+int check_change(const ScoreChange &m, float scale, int causal) {
+    if (m.prefix && !causal) return RFDETR_ERR_SHAPE;
     if (m.cap != 0.0f) {
         // The near polynomial's coefficients, scale (scale / cap)^2k, have to be numbers.
         const double in = (double)scale / m.cap, in2 = in * in;
@@ -2671,7 +2672,7 @@ extern "C" int rfdetr_packed_attention_scored(void *stream, const void *query, i
     const ScoreChange change{score_cap, distance_slopes, prefix};
     if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
     if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
-    if (int st = check_change(change, scale)) return st;
+    if (int st = check_change(change, scale, causal)) return st;
     if (tokens == 0) return RFDETR_OK;
     const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
         v{value, value_token_stride, value_head_stride};
@@ -2732,7 +2733,7 @@ extern "C" int rfdetr_packed_attention_scored_backward(
     const ScoreChange change{score_cap, distance_slopes, prefix};
     if (int st = check_sizes(n_sequences, tokens, key_tokens, n_heads, n_kv_heads, head_dim)) return st;
     if (!(scale > 0.0f) || scale > FLT_MAX) return RFDETR_ERR_SHAPE;
-    if (int st = check_change(change, scale)) return st;
+    if (int st = check_change(change, scale, causal)) return st;
     if (tokens == 0 && key_tokens == 0) return RFDETR_OK;
     const Strided q{query, query_token_stride, query_head_stride}, k{key, key_token_stride, key_head_stride},
         v{value, value_token_stride, value_head_stride}, g{grad_output, grad_token_stride, grad_head_stride};

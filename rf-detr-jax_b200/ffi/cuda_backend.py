@@ -295,7 +295,8 @@ def _change(distance_slopes, prefix):
 @functools.partial(jax.custom_vjp, nondiff_argnums=(7, 8, 9))
 def scored_attention(query, key, value, offsets, key_offsets, distance_slopes=None, prefix=None, causal=False,
                      scale=None, score_cap=None):
-    """:func:`packed_attention` whose scores are capped, lowered by ``slope * distance`` or see a prefix."""
+    """:func:`packed_attention` whose scores are capped, lowered by ``slope * distance`` or, under a causal mask, see a
+    prefix (refused without one)."""
     out, _, lse = _scored_attention_call(query, key, value, offsets, key_offsets, distance_slopes, prefix, causal,
                                          scale, score_cap, False)
     return out, lse

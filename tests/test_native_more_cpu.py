@@ -110,3 +110,13 @@ def test_another_device_is_made_current(pkg, monkeypatch):
     monkeypatch.setattr(N, "_current_device", lambda: 1)
     N.on_device(Fake(), order.append, "call")
     assert order == ["call"]
+
+
+def test_a_prefix_needs_a_causal_mask(pkg):
+    """As the Python function says: without a mask every query sees all keys, and a prefix would be ignored."""
+    N = pkg._native
+    assert _scored(N, T=0, causal=0) == N.ERR_SHAPE and _scored(N, T=0, causal=0, prefix=None) == N.OK
+    back = lambda causal, prefix: N.lib().rfdetr_packed_attention_scored_backward(  # noqa: E731
+        None, 16, 128, 64, 16, 128, 64, 16, 128, 64, 16, None, 16, 16, 16, 16, 128, 64, None, 16, 16, 16, None, 0,
+        1, 4, 4, 2, 2, 64, causal, 0.1, 30.0, None, prefix)
+    assert back(0, 16) == N.ERR_SHAPE and back(1, 16) == back(0, None) == N.ERR_WORKSPACE
