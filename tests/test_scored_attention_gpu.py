@@ -382,3 +382,61 @@ def test_steep_slopes(pkg, dim, slope):
                seed=dim)
         _check(pkg, (40, 3), (168, 130), heads=2, kv=1, dim=dim, causal=False, cap=cap, slopes=(slope, 0.25), seed=dim)
         _check(pkg, (300, 64), heads=2, kv=1, dim=dim, causal=True, cap=cap, slopes=(0.25, slope), prefix=(150, 3), seed=dim)
+
+
+@pytest.mark.parametrize("knob", ["1", "2", "3", "3,4"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap", [8.0, 35.0, 50.0, 51.0, 60.0, 100.0])
+def test_scores_past_the_cap_in_every_forward_kernel(pkg, tuning, knob, dim, cap):
+    """Products of up to about one and up to about three caps, so that all forms of the cap are met in every kernel, with
+    and without slopes and prefixes, in whole tiles and masked ones."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    for part in (0.35, 1.0):
+        for slopes, causal, prefix in ((None, False, None), (None, True, (300, 0)), ((0.5, 0.004, -0.01, 0.1), True, None),
+                                       ((0.03, 0.0, 0.2, 0.01), False, None), ((0.1, 0.02, 0.3, 0.0), True, (129, 400))):
+            _check(pkg, (310, 100), (1000, 400), dim=dim, causal=causal, cap=cap, slopes=slopes, prefix=prefix,
+                   size=part * cap, grad=False, seed=int(cap) + dim)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("cap", [8.0, 50.0, 60.0])
+def test_gradients_of_scores_past_the_cap(pkg, dim, cap):
+    for part in (0.35, 1.0):
+        for slopes, causal, prefix in ((None, False, None), ((0.5, 0.004, -0.01, 0.1), True, None),
+                                       ((0.03, 0.0, 0.2, 0.01), True, (150, 3))):
+            _check(pkg, (310, 64, 1), dim=dim, causal=causal, cap=cap, slopes=slopes,
+                   prefix=None if prefix is None else (*prefix, 0), size=part * cap, seed=dim, with_lse_grad=True)
+
+
+@pytest.mark.parametrize("knob", ["1", "2", "3", "3,4"])
+def test_the_entries_without_a_change_are_the_plain_ones(pkg, tuning, knob):
+    """``rfdetr_packed_attention`` and its gradients, and the entries with changed scores given none: equal bits."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    N = pkg._native
+    lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
+    rng = np.random.default_rng(11)
+    for dim in (32, 64, 128):
+        T, Tk, H, Hkv, lengths, keys = 410, 1400, 4, 2, (310, 100), (1000, 400)
+        q, k, v, g = (_bf16(rng, n, h, dim) for n, h in ((T, H), (Tk, Hkv), (Tk, Hkv), (T, H)))
+        off, koff = _offsets(lengths), _offsets(keys)
+        sizes = (2, T, Tk, H, Hkv, dim, 1, dim ** -0.5)
+        rows = lambda x: (x.data_ptr(), x.stride(0), x.stride(1))  # noqa: E731
+        results = []
+        for forward, backward, more in (
+                (lib.rfdetr_packed_attention, lib.rfdetr_packed_attention_backward, ()),
+                (lib.rfdetr_packed_attention_scored, lib.rfdetr_packed_attention_scored_backward, (0.0, None, None))):
+            out, low, dq = (torch.zeros_like(q) for _ in range(3))
+            dk, dv = torch.zeros_like(k), torch.zeros_like(v)
+            lse = torch.zeros(H, T, device=DEV)
+            room = torch.zeros(max(lib.rfdetr_packed_attention_workspace_bytes(*sizes[:6]),
+                                   lib.rfdetr_packed_attention_backward_workspace_bytes(T, H)), dtype=torch.uint8,
+                               device=DEV)
+            assert forward(stream, *rows(q), *rows(k), *rows(v), off.data_ptr(), koff.data_ptr(), out.data_ptr(),
+                           low.data_ptr(), lse.data_ptr(), room.data_ptr(), room.numel(), *sizes, *more) == N.OK
+            assert backward(stream, *rows(q), *rows(k), *rows(v), off.data_ptr(), koff.data_ptr(), out.data_ptr(),
+                            low.data_ptr(), lse.data_ptr(), *rows(g), None, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                            room.data_ptr(), room.numel(), *sizes, *more) == N.OK
+            results.append((out, low, lse, dq, dk, dv))
+        for a, b in zip(*results):
+            assert a.any() and torch.equal(a, b)
+    _fault_free(pkg)
