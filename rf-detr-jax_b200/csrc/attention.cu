@@ -605,7 +605,7 @@ __device__ __forceinline__ bool softmax_tile(const AttnArgs &A, const RowScores<
             for (int e = 0; e < 32; ++e) mx = c + e < seen ? fmaxf(mx, s[e]) : mx;
         }
         if constexpr (MOD == kBounded) {
-            if (mx != -INFINITY) mx = scores.score_of(A, mx);
+            if (seen > 0) mx = scores.score_of(A, mx);  // (all of them -inf: minus the cap)
         }
         if constexpr (MOD == kBiased || MOD == kCapped) tmem_wait_st();
         if (!settle()) return false;

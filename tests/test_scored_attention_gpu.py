@@ -440,3 +440,18 @@ def test_the_entries_without_a_change_are_the_plain_ones(pkg, tuning, knob):
         for a, b in zip(*results):
             assert a.any() and torch.equal(a, b)
     _fault_free(pkg)
+
+
+@pytest.mark.parametrize("knob", ["1", "2", "3", "3,2"])
+@pytest.mark.parametrize("keys", [5, 128, 300])
+def test_products_that_are_all_minus_infinity(pkg, tuning, knob, keys):
+    """They are capped like any others: equal scores of minus the cap, whatever the tile's size."""
+    tuning("RFDETR_ATTN_FWD", knob)
+    rng = np.random.default_rng(keys)
+    for cap in (3.0, 40.0, 70.0):
+        q, k, v = _bf16(rng, 3, 1, 64), _bf16(rng, keys, 1, 64), _bf16(rng, keys, 1, 64)
+        q[:, 0, 0], k[:, 0, 0] = 1.0, -float("inf")
+        out, lse = pkg.packed_attention(q, k, v, _offsets((3,)), _offsets((keys,)), score_cap=cap, return_lse=True)
+        assert (lse - (np.log(keys) - cap)).abs().max() <= 2.0 ** -20 * (cap + 10)
+        want, size = _f64(v).mean(0), np.abs(_f64(v)).mean(0)
+        assert (np.abs(_f64(out) - want) <= 2.0 ** -8 * (np.abs(want) + size)).all()
