@@ -412,7 +412,8 @@ int rfdetr_packed_attention_backward(void *stream, const void *query, int64_t qu
  * prefix, device int32 [n_sequences] or NULL, with `causal` alone (RFDETR_ERR_SHAPE without): every query of sequence s
  * sees the keys j < prefix[s] as well (values are clamped to the sequence).  lse is of the changed scores.  The slopes have no gradient.
  * With neither the calls are those above, bit for bit.  Workspaces, limits and everything else are theirs too;
- * score_cap lies in 2^-40 .. 2^40 and scale / score_cap in 2^-20 .. 2^20.  A capped score of an infinite product is
+ * score_cap lies in 2^-40 .. 2^40, scale / score_cap in 2^-20 .. 2^20 and scale (scale / score_cap)^6 in float32's range.
+ * A capped score of an infinite product is
  * +-score_cap.  Capped scores are right to 8e-7 of their value and 2^-21 of the cap.
  * ------------------------------------------------------------------------------------- */
 int rfdetr_packed_attention_scored(void *stream, const void *query, int64_t query_token_stride,

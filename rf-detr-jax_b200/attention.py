@@ -150,8 +150,8 @@ def _score_change(score_cap, distance_slopes, prefix, heads, sequences, causal, 
     cap = 0.0 if score_cap is None else float(score_cap)
     if score_cap is not None and not (2.0 ** -39 <= cap <= 2.0 ** 39 and 2.0 ** -19 <= scale / cap <= 2.0 ** 19
                                       and 2.0 ** -120 <= scale * (scale / cap) ** 6 <= 2.0 ** 127):
-        raise ValueError(f"score_cap must be positive, 2^-39 to 2^39 and within 2^19 of scale either way, got "
-                         f"{score_cap} with {scale}")
+        raise ValueError(f"score_cap must be positive, 2^-39 to 2^39 and within 2^19 of scale either way, and "
+                         f"scale (scale / score_cap)^6 within float32's range, got {score_cap} with {scale}")
     if distance_slopes is not None:
         if distance_slopes.shape != (heads,) or distance_slopes.dtype != torch.float32:
             raise ValueError(f"distance_slopes must be float32 [{heads}], got {distance_slopes.dtype} "
@@ -187,7 +187,7 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         return_lse: also return the scores' log-sum-exp ``[heads, tokens]`` float32.
         check: read the offsets on the host (synchronises) and raise ``ValueError`` unless they
             ascend within the tensors; otherwise the kernels clamp them.
-        score_cap: scores ``s`` become ``score_cap * tanh(s / score_cap)``.
+        score_cap: scores ``s`` become ``score_cap * tanh(s / score_cap)``; positive, at a scale of 1/8 up to 92,000.
         distance_slopes: ``[heads]`` float32 on the device: from the (capped) score of query ``i`` and key ``j``
             ``slope * |i + Lk - Lq - j|`` is taken, the last query being level with the last key.  No gradient.  Slopes
             are finite, negative ones times the longest distance too; scores are float32, so that a product past its

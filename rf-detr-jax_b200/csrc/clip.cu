@@ -2,9 +2,10 @@
 //   n = sqrt(sum of g^2 over all values of all tensors),  y = g * (n <= limit ? 1 : limit / n)
 //
 // The bound is memory: every value is read for the norm and, before any result can be written, the norm has to be
-// whole, so every value is read once more; what fits in L2 (126 MB) comes from there the second time.  Two launches:
-// the first leaves one sum for each block, the second adds them up again in each block, in the same order, and
-// writes the results.  It walks backwards, from what was read last.
+// whole, so every value is read once more.  Two launches: the first leaves one sum for each block, the second adds them
+// up again in each block, in the same order, and writes the results.  It walks backwards, from what was read last, and
+// finds some of that in L2 (126 MB, which the results take too): of 109 MB float32 it reads 52 from memory, of 55 MB
+// bf16 18.
 //
 // The tensors' table travels as a kernel argument, so a call copies nothing to the device, may be captured and needs
 // no table that lives on.  Tensors differ in length from one value to millions; laid end to end, each rounded
@@ -15,7 +16,7 @@
 // loses nothing that float32 could show.  The conversions take 36% of their unit's rate from float32, 63% from bf16.
 // Equal calls give equal bits.
 // 361 float32 tensors of 27.4 million values into others: 55 us, 21 for the norm (5.2 TB/s), 34 for the rest; one
-// bf16 buffer of as many values into a float32 one 38, 13 and 25.
+// bf16 buffer of as many values into a float32 one 38, 13 and 25.  In place, past the limit: 45 float32, 27 bf16.
 #include <algorithm>
 #include <cfloat>
 #include <memory>

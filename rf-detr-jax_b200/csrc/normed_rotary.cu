@@ -10,9 +10,10 @@
 //
 // The floor is memory: forward x in and y out, backward x and g in and dx out; nothing is kept between them.  What
 // bounds it now is the issue of instructions, 64% of the slots forward and 54% backward: 32,768 tokens of 16 + 4 heads
-// of 128, bf16, take 72 and 130 us, 4.7 and 3.9 TB/s; 20,011 of 7 + 1 of 80, 48 channels interleaved, 15.2 forward.  A
-// row (one head of one token) is read once, in 16-byte pieces, by as many neighbouring lanes as it has pieces (ten for
-// 80 channels of bf16, three rows to a warp), summed by shuffles, and turned in registers.  Where half is a multiple
+// of 128, bf16, take 73 and 129 us, 4.6 and 3.9 TB/s; 20,011 of 7 + 1 of 80, 48 channels interleaved, 14.4 and 28.2;
+// float32, 8192 of 16 + 4 of 256, 64 turned, 93 and 181, 3.6 and 2.8 TB/s.  A row (one head of one token) is read once,
+// in 16-byte pieces, by as many neighbouring lanes as it has pieces, or half as many (normed_plan.cuh; ten for 80
+// channels of bf16, three rows to a warp), summed by shuffles, and turned in registers.  Where half is a multiple
 // of a piece a lane holds both partners of its pairs; otherwise they meet through shared memory, so that any half is
 // read in whole pieces.  Blocks stay for the launch: a lane's channels are the same in every row, so the weights'
 // gradients are summed in its registers, then over the block, and a second launch adds the blocks' sums in order (no

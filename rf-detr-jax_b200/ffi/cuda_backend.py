@@ -360,8 +360,8 @@ axial_rotary.defvjp(_axial_rotary_fwd, _axial_rotary_bwd)
 @functools.partial(jax.custom_vjp, nondiff_argnums=(6, 7, 8))
 def normed_axial_rotary(query, key, query_weight, key_weight, positions, inv_freq, sections, interleaved=False,
                         eps=1e-6):
-    """Every head of queries and keys normed (root mean square, times a weight ``[head_dim]``) and turned by its
-    token's positions."""
+    """Every head of queries and keys normed (root mean square, times a weight ``[head_dim]``, or ``[0]`` for ones) and
+    turned by its token's positions.  Queries alone: a key of no heads, ``[tokens, 0, head_dim]``."""
     outs = tuple(jax.ShapeDtypeStruct(x.shape, x.dtype) for x in (query, key))
     return jax.ffi.ffi_call("RfdetrNormedRotary", outs)(
         query, key, query_weight, key_weight, positions, inv_freq.astype(jnp.float32),
